@@ -275,6 +275,104 @@ int mxk_host_read_points_f32(const char* path, int64_t n, int d, int padded_d, f
  * line, the same bytes as the reference (formatted on all host threads). */
 int mxk_host_write_labels(const char* path, const int* labels, int64_t n);
 
+/* ---- paged MX cache of keys and values (no counterpart in the reference) ---- */
+
+/* Element type of rows handed to and taken from the cache. */
+typedef enum { MXK_F32 = 0, MXK_F16 = 1, MXK_BF16 = 2 } mxk_dtype;
+
+/* Keys and values of many sequences, held as the MX rows of mxk_quantize_rows in
+ * pages of page_size tokens.  All four buffers are device memory of the caller,
+ * 16-byte aligned and contiguous:
+ *   k_values, v_values  [pages][kv_heads][page_size][head_dim * bits / 8]
+ *   k_scales, v_scales  [pages][kv_heads][page_size][head_dim / 32]
+ * A token's place is its slot, page * page_size + place in the page.  bits in
+ * {4, 6, 8}; head_dim % 32 == 0, at most 512; page_size % 16 == 0; kv_heads,
+ * pages >= 1. */
+typedef struct {
+    int bits;
+    int kv_heads;
+    int head_dim;
+    int page_size;
+    int64_t pages;
+    void* k_values;
+    uint8_t* k_scales;
+    void* v_values;
+    uint8_t* v_scales;
+} mxk_cache;
+
+/* Rows of `tokens` tokens x kv_heads heads x head_dim features, the features
+ * contiguous, strides in elements (of any sign and size). */
+typedef struct {
+    void* data;
+    int64_t token_stride;
+    int64_t head_stride;
+} mxk_rows;
+
+/* Quantises the keys and values of `tokens` new tokens into the cache: token i's
+ * rows go to slots[i] (int64, device) with the bytes mxk_quantize_rows(bits, ...)
+ * gives for them.  A slot outside [0, pages * page_size) marks a token that is
+ * not kept.  Two tokens with the same slot: which one stays is not defined.
+ * Asynchronous on `stream`; no workspace. */
+int mxk_cache_write(const mxk_cache* cache, int dtype, int64_t tokens, const mxk_rows* k, const mxk_rows* v,
+                    const int64_t* slots, void* stream);
+
+/* Reads slots back: row (i, h) of k and v receives the value that the cache holds
+ * at slots[i], element * 2^(scale - 127), rounded once to dtype (to nearest even;
+ * exact in float32 unless it overflows).  A slot outside [0, pages * page_size)
+ * reads as zeros.  Asynchronous on `stream`; no workspace. */
+int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int64_t* slots, const mxk_rows* k,
+                   const mxk_rows* v, void* stream);
+
+/* Attention of the newest tokens of `seqs` sequences over their cached tokens.
+ *
+ * Sequence i has L = kv_lens[i] cached tokens (token t in slot
+ * page_table[i * page_table_stride + t / page_size] * page_size + t % page_size)
+ * and n = cu_q[i + 1] - cu_q[i] query tokens, rows cu_q[i] .. of q and out; its
+ * query token j sits at position p = L - n + j.  Query head h reads key and value
+ * head h / (heads / kv_heads).  Token t takes part when t < L, when t <= p if
+ * causal is set, and when t > p - window if window > 0 (causal only).  With s the
+ * products scale * q . k over the tokens that take part,
+ *     out = sum_t exp(s_t) v_t / sum_t exp(s_t),    lse = log(sum_t exp(s_t));
+ * a row with no such token gets zeros and -inf.  Tokens outside [0, L) are never
+ * read; a NaN among the keys or values reaches the rows that see its token only.
+ *
+ * cu_q (seqs + 1), page_table, kv_lens: int32 on the device.  max_q and max_kv
+ * are bounds on n and L known to the host: they choose the launch, and a longer
+ * sequence's output is not defined (no memory outside the given buffers is
+ * touched).  The page table holds max_kv / page_size pages (rounded up) per
+ * sequence.  q and out: dtype MXK_F16 or MXK_BF16, `tokens` rows of `heads` heads
+ * (out may not overlap q).  lse (optional): float32 [tokens][heads].
+ * head_dim must be 64 or 128 (others: MXK_ERR_UNSUPPORTED).
+ *
+ * Products are taken in f16 with float32 sums: every MX element times its scale
+ * is exact in f16 relative to a power of two that moves with the data (values
+ * below 2^-24 of the largest magnitude met in the same head may lose bits), q's
+ * rows are scaled into f16 by a power of two, and exp(s - max) is rounded to f16
+ * for the product with v.  Statistics are float32.  The result does not depend on
+ * timing: partial sums join in a fixed order.
+ *
+ * Asynchronous on `stream`; partial sums live in the library's stream-ordered
+ * pool on the current device (mxk_release_workspace). */
+typedef struct {
+    int dtype;
+    int heads;
+    int64_t tokens;
+    int seqs;
+    int max_q;
+    int64_t max_kv;
+    mxk_rows q;
+    const int* cu_q;
+    const int* page_table;
+    int64_t page_table_stride;
+    const int* kv_lens;
+    float scale;
+    int causal;
+    int64_t window;
+    mxk_rows out;
+    float* lse;
+} mxk_attention;
+int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* args, void* stream);
+
 /* ---- kernel timing (CUDA events around each launch on its stream) ---------- */
 int mxk_profile_enable(int on);
 /* Copies up to max entries of {name, launches, total_ms} for the current device. */

@@ -1,0 +1,760 @@
+// Attention of new tokens over the paged MX cache: the kernel for few query rows
+// and the entry point (no counterpart in the reference).
+//
+//     out_r = sum_t exp(s_rt) v_t / sum_t exp(s_rt),   s_rt = scale * q_r . k_t
+//
+// With few rows per key head (decoding: one token times the heads of a group) the
+// cached rows are read once and used for a handful of products each, so their
+// bytes over HBM bandwidth bound it: 2 * (D * bits / 8 + D / 32) per token and key
+// head.  attention_rows_kernel keeps that stream busy:
+//
+//  * A CTA of four warps; every warp streams its own 16-token granules through its
+//    own ring of shared-memory stages (16-byte asynchronous copies, no barrier
+//    between warps) and keeps its own running maximum, sum and output rows in
+//    registers.  The warps join once per unit.
+//  * Products are m16n8k16 f16 with the 16 query rows as M.  Tensor throughput is
+//    no concern here (tcgen05 needs 64 or more rows to pay), fragments straight
+//    from the raw bytes are: the order of features inside a product is free as
+//    long as q and k agree, so a lane reads a contiguous quarter of a key row, and
+//    a contiguous eighth of four value rows, and converts in registers.  The row
+//    pitches in shared memory keep those reads free of bank conflicts.
+//  * The MX scale of a key block becomes an f16 factor relative to the row's
+//    largest scale (exact unless two blocks of one row differ by more than 2^30),
+//    the row's own factor goes onto the finished score.  Value blocks are scaled
+//    relative to the power of two of the largest value scale met so far, which
+//    only moves up, like the running maximum.
+#include <limits>
+
+#include "attention.cuh"
+
+namespace mxk {
+namespace {
+
+using dev::ex2;
+using dev::kExpShift;
+using dev::kMaxSlack;
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kRows = 16;     // query rows of a unit
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kGranule = 16;  // tokens of one step of a warp
+constexpr int kKeys = kGranule * kWarps;
+
+// Shared-memory row pitches (bytes) of the key and value granules; each makes the
+// lanes of one load instruction touch all banks once.  Keys are read row by row,
+// a quarter per lane; values four rows per lane, an eighth each.
+template <int D, int BITS>
+struct Pitch;
+template <> struct Pitch<128, 8> { static constexpr int k = 144, v = 144; };
+template <> struct Pitch<128, 6> { static constexpr int k = 96, v = 112; };
+template <> struct Pitch<128, 4> { static constexpr int k = 64, v = 80; };
+template <> struct Pitch<64, 8> { static constexpr int k = 64, v = 80; };
+template <> struct Pitch<64, 6> { static constexpr int k = 48, v = 48; };
+template <> struct Pitch<64, 4> { static constexpr int k = 32, v = 48; };
+
+template <int D, int BITS>
+struct Stage {
+    static constexpr int row = D * BITS / 8;
+    static constexpr int chunks = row / 16;       // 16-byte copies of a row
+    static constexpr int scale_bytes = D / 32;    // of a row
+    static constexpr int v_at = kGranule * Pitch<D, BITS>::k;
+    static constexpr int ks_at = v_at + kGranule * Pitch<D, BITS>::v;
+    static constexpr int vs_at = ks_at + kGranule * scale_bytes;
+    static constexpr int bytes = vs_at + kGranule * scale_bytes;
+    static constexpr int stages = 3;
+    static constexpr int ring = kWarps * stages * bytes;
+    static constexpr int join = kWarps * kRows * D * 4;  // the warps' outputs, after the ring is done
+    static constexpr int smem = ring > join ? ring : join;
+    static_assert(bytes % 16 == 0, "stages start on 16-byte boundaries");
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// N bytes of shared memory into words (the last one zero-extended).
+template <int N>
+__device__ __forceinline__ void lds_bytes(uint32_t at, uint32_t* w) {
+    if constexpr (N % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 16; ++i)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
+                         : "r"(at + 16 * i));
+    } else if constexpr (N % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 8; ++i)
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[2 * i]), "=r"(w[2 * i + 1]) : "r"(at + 8 * i));
+    } else if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(at + 4 * i));
+    } else {
+        static_assert(N == 6, "rows end on even bytes");
+        uint16_t a, b, c;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(a) : "r"(at));
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(at + 2));
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(c) : "r"(at + 4));
+        w[0] = a | ((uint32_t)b << 16);
+        w[1] = c;
+    }
+}
+
+__device__ __forceinline__ uint32_t lds_u8(uint32_t at) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .u16 t;\n\tld.shared.u8 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(v) : "r"(at));
+    return v;
+}
+
+// The j-th group of four 6-bit codes of a packed row, one per byte.
+__device__ __forceinline__ uint32_t four6(const uint32_t* w, int j) {
+    const int bit = 24 * j, i = bit / 32, s = bit % 32;
+    const uint32_t v = s <= 8 ? w[i] >> s : __funnelshift_r(w[i], w[i + 1], s);
+    return dev::spread6(v);
+}
+
+// f16 pair of 2^(e0), 2^(e1), zero where that is below f16's range (e <= 15).
+__device__ __forceinline__ uint32_t pow2_f16x2(int e0, int e1) {
+    const float a = __uint_as_float((uint32_t)max(e0 + 127, 0) << 23);
+    const float b = __uint_as_float((uint32_t)max(e1 + 127, 0) << 23);
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// c += a (16 x 16, row) * b (16 x 8, column), f16 operands, f32 sums.
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Largest of the scale bytes of a key row (at least 1, so that 2^(max - 127) is a
+// normal float; blocks are scaled relative to it whatever it is).
+template <int D>
+__device__ __forceinline__ int row_scale(uint32_t w) {
+    int m = max((int)(w & 255u), (int)((w >> 8) & 255u));
+    if constexpr (D == 128) m = max(m, max((int)((w >> 16) & 255u), (int)(w >> 24)));
+    return max(m, 1);
+}
+
+// Element headroom: codes are at most 448 < 2^9, f16 reaches 2^16, so block
+// factors go up to 2^6; keys use it fully, values start at 2^4 and may grow to 2^6
+// before their reference moves.
+constexpr int kKeyLift = 6;
+constexpr int kValueLift = 4, kValueMax = 6;
+constexpr int kQueryExp = 12;  // query rows are scaled to a largest magnitude in [2^12, 2^13)
+
+template <int D, int BITS>
+__global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const AttentionParams p) {
+    using S = Stage<D, BITS>;
+    using P = Pitch<D, BITS>;
+    constexpr int kSteps = D / 16;       // k-steps of q . k
+    constexpr int kTiles = D / 8;        // 8-feature tiles of the output
+    constexpr int kShare = S::row / 4;   // bytes of a key row a lane reads
+    constexpr int vShare = S::row / 8;   // bytes of a value row a lane reads
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int64_t scratch[kWarps + 2];
+    __shared__ float stat_max[kWarps][kRows], stat_sum[kWarps][kRows];
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, c = lane & 3;
+    const uint32_t ring = dev::smem_addr(smem) + warp * (S::stages * S::bytes);
+
+    const dev::Share share = dev::take_share<kRows, kKeys, kThreads>(p, scratch);
+    if (share.tiles == 0) {
+        if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0), p.part_ends[blockIdx.x] = 0;
+        return;
+    }
+    dev::Walk w = dev::walk_to<kRows, kKeys>(p, share.seq, share.offset);
+    int64_t left = share.tiles;
+    bool open = false, went_on = false, ended = false;
+
+    while (left > 0) {
+        const int tile0 = w.tile;
+        const int tiles = (int)(left < w.tiles - tile0 ? left : w.tiles - tile0);
+        const int rows = w.view.n * p.group - w.rt * kRows < kRows ? w.view.n * p.group - w.rt * kRows : kRows;
+        const int64_t len = w.view.len;
+
+        // This lane's rows (g and g + 8): tokens [lo, hi) take part.  Rows past the
+        // unit's see everything; they are zero queries and never written.
+        int64_t lo[2], hi[2];
+        int64_t row_at[2];
+        bool real[2];
+        int64_t all_lo = 0, all_hi = len, any_lo, any_hi;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = w.rt * kRows + g + 8 * i;
+            real[i] = g + 8 * i < rows;
+            const int j = r / p.group;
+            lo[i] = 0, hi[i] = len;
+            if (real[i]) dev::seen_range(p, w.view, j, j, lo[i], hi[i]);
+            row_at[i] = (int64_t)(w.view.row0 + j) * p.q_token +
+                        (int64_t)(w.head * p.group + (r - j * p.group)) * p.q_head;
+        }
+        {
+            const int r0 = w.rt * kRows, r1 = r0 + rows - 1;
+            dev::seen_range(p, w.view, r0 / p.group, r1 / p.group, any_lo, any_hi);  // seen by some row
+            int64_t a, b;
+            dev::seen_range(p, w.view, r0 / p.group, r0 / p.group, a, all_hi);  // the first row ends first,
+            dev::seen_range(p, w.view, r1 / p.group, r1 / p.group, all_lo, b);  // the last begins last
+        }
+
+        // q as the A operand: features c * D/4 + 4 i .. + 3 of rows g, g + 8 at step i.
+        uint32_t qa[kSteps][4];
+        float row_factor[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float x[D / 4];
+            const uint16_t* q = static_cast<const uint16_t*>(p.q) + (row_at[i] + c * (D / 4));
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                uint32_t a = 0, b = 0;
+                if (real[i]) {
+                    if (p.q_vec) {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(q) + k);
+                        a = v.x, b = v.y;
+                    } else {
+                        a = q[4 * k] | ((uint32_t)q[4 * k + 1] << 16);
+                        b = q[4 * k + 2] | ((uint32_t)q[4 * k + 3] << 16);
+                    }
+                }
+                if (p.dtype == MXK_F16) {
+                    const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&a));
+                    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&b));
+                    x[4 * k] = u.x, x[4 * k + 1] = u.y, x[4 * k + 2] = v.x, x[4 * k + 3] = v.y;
+                } else {
+                    x[4 * k] = __uint_as_float(a << 16), x[4 * k + 1] = __uint_as_float(a & 0xffff0000u);
+                    x[4 * k + 2] = __uint_as_float(b << 16), x[4 * k + 3] = __uint_as_float(b & 0xffff0000u);
+                }
+            }
+            float amax = 0.0f;
+#pragma unroll
+            for (int k = 0; k < D / 4; ++k) amax = fmaxf(amax, fabsf(x[k]));
+            amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
+            // 2^(12 - exponent) in two factors, each a normal float
+            int e = amax > 0.0f ? (int)(__float_as_uint(amax) >> 23) - 127 : 0;
+            e = max(e, -126);
+            const int down = (kQueryExp - e) / 2, rest = kQueryExp - e - down;
+            const float f0 = __uint_as_float((uint32_t)(down + 127) << 23);
+            const float f1 = __uint_as_float((uint32_t)(rest + 127) << 23);
+            row_factor[i] = p.scale_log2 * __uint_as_float((uint32_t)(127 - down - kKeyLift / 2) << 23) *
+                            __uint_as_float((uint32_t)(127 - rest - kKeyLift / 2) << 23);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const __half2 u = __floats2half2_rn(x[4 * k] * f0 * f1, x[4 * k + 1] * f0 * f1);
+                const __half2 v = __floats2half2_rn(x[4 * k + 2] * f0 * f1, x[4 * k + 3] * f0 * f1);
+                qa[k][i] = *reinterpret_cast<const uint32_t*>(&u);
+                qa[k][2 + i] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+        }
+
+        float o[kTiles][4];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        const float neg_inf = __int_as_float(0xff800000);
+        float run_max[2] = {neg_inf, neg_inf};  // of rows g, g + 8, log2 units
+        float base[2] = {-kExpShift, -kExpShift};  // what is subtracted from a score: run_max - kExpShift
+        float sum[2] = {0.0f, 0.0f};               // this lane's share of the rows' sums
+        int vref = 0;                              // values are held relative to 2^(vref - 127); 0: none yet
+
+        // The warp's granules: numbers first, first + 4, ... of the sequence below `end`.
+        const int64_t gran0 = (w.first + tile0) * kWarps + warp;
+        int64_t end = (w.first + tile0 + tiles) * kWarps;
+        const int64_t seen_end = any_hi <= any_lo ? 0 : (any_hi + kGranule - 1) / kGranule;
+        end = end < seen_end ? end : seen_end;
+        const int steps = end > gran0 ? (int)((end - gran0 + kWarps - 1) / kWarps) : 0;
+        const int* table = p.page_table + (int64_t)w.seq * p.table_stride;
+        const unsigned per_page = (unsigned)p.page_size / kGranule;
+
+        auto page_of = [&](int step) -> int {
+            if (step >= steps) return 0;
+            const unsigned gr = (unsigned)(gran0 + (int64_t)step * kWarps);
+            const int page = __ldg(table + gr / per_page);
+            return page < 0 ? 0 : (page >= p.pages ? p.pages - 1 : page);
+        };
+        auto issue = [&](int step, int page) {
+            if (step < steps) {
+                const int64_t gr = gran0 + (int64_t)step * kWarps;
+                const int in_page = (int)((unsigned)gr % per_page) * kGranule;
+                const int64_t row = ((int64_t)page * p.kv_heads + w.head) * p.page_size + in_page;
+                const int valid = (int)(len - gr * kGranule < kGranule ? len - gr * kGranule : kGranule);
+                const uint32_t at = ring + (step % S::stages) * S::bytes;
+#pragma unroll
+                for (int i = 0; i < S::chunks; ++i) {
+                    const int idx = lane + 32 * i;
+                    const bool is_v = idx >= kGranule * S::chunks;
+                    const int in = is_v ? idx - kGranule * S::chunks : idx;
+                    const int r = in / S::chunks, ch = in - r * S::chunks;
+                    const uint8_t* src = (is_v ? p.v_values : p.k_values) + (row + r) * S::row + ch * 16;
+                    copy16(at + (is_v ? S::v_at + r * P::v : r * P::k) + ch * 16, src, r < valid ? 16 : 0);
+                }
+                constexpr int sc = kGranule * S::scale_bytes / 16;
+                if (lane < 2 * sc) {
+                    const int side = lane / sc, ch = lane - side * sc;
+                    copy16(at + (side ? S::vs_at : S::ks_at) + ch * 16,
+                           (side ? p.v_scales : p.k_scales) + row * S::scale_bytes + ch * 16, 16);
+                }
+            }
+            copy_commit();
+        };
+
+#pragma unroll
+        for (int s = 0; s < S::stages - 1; ++s) issue(s, page_of(s));
+        int next_page = page_of(S::stages - 1);
+
+        for (int step = 0; step < steps; ++step) {
+            copy_wait<S::stages - 2>();
+            __syncwarp();
+            issue(step + S::stages - 1, next_page);
+            next_page = page_of(step + S::stages);
+            const uint32_t at = ring + (step % S::stages) * S::bytes;
+            const int64_t t0 = (gran0 + (int64_t)step * kWarps) * kGranule;
+
+            // scores: 16 rows x 2 tiles of 8 tokens
+            float s[2][4];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+                const int t = g + 8 * nt;
+                uint32_t kw[(kShare + 3) / 4];
+                lds_bytes<kShare>(at + t * P::k + c * kShare, kw);
+                uint32_t sw;
+                if constexpr (D == 128) {
+                    lds_bytes<4>(at + S::ks_at + t * 4, &sw);
+                } else {
+                    uint16_t h;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at + S::ks_at + t * 2));
+                    sw = h;
+                }
+                const int top = row_scale<D>(sw);
+                const int own = (int)((sw >> (8 * (D == 128 ? c : c >> 1))) & 255u);
+                const uint32_t f = pow2_f16x2(own - top + kKeyLift, own - top + kKeyLift);
+                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+                if constexpr (BITS == 4) {
+#pragma unroll
+                    for (int k = 0; k < kSteps; k += 2) {
+                        uint32_t h[4];
+                        dev::e2m1x8_to_f16(kw[k / 2], h);
+                        mma16816(s[nt], qa[k], hmul2(h[0], f), hmul2(h[1], f));
+                        mma16816(s[nt], qa[k + 1], hmul2(h[2], f), hmul2(h[3], f));
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) {
+                        const uint32_t four = BITS == 8 ? kw[k] : four6(kw, k);
+                        constexpr int kCode = BITS == 4 ? 8 : BITS;
+                        mma16816(s[nt], qa[k], hmul2(dev::codes_to_f16x2<kCode>(four), f),
+                                 hmul2(dev::codes_to_f16x2<kCode>(four >> 16), f));
+                    }
+                }
+                // the rows' and the tokens' own factors
+                const float tok = __uint_as_float((uint32_t)top << 23);
+                const float ta = __shfl_sync(kFull, tok, 8 * c), tb = __shfl_sync(kFull, tok, 8 * c + 4);
+                s[nt][0] = s[nt][0] * row_factor[0] * ta, s[nt][1] = s[nt][1] * row_factor[0] * tb;
+                s[nt][2] = s[nt][2] * row_factor[1] * ta, s[nt][3] = s[nt][3] * row_factor[1] * tb;
+            }
+            const bool partly = t0 < all_lo || t0 + kGranule > all_hi;
+            if (partly) {
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int64_t t = t0 + 8 * nt + 2 * c + (e & 1);
+                        if (t < lo[e >> 1] || t >= hi[e >> 1]) s[nt][e] = neg_inf;
+                    }
+            }
+
+            // Raise the maximum of the rows where some score exceeds it by more than the
+            // slack (row by row: a row's result does not depend on its neighbours).
+            const float m0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+            const float m1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+            if (__any_sync(kFull, m0 > run_max[0] + kMaxSlack || m1 > run_max[1] + kMaxSlack)) {
+                float m[2] = {m0, m1};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    m[i] = fmaxf(m[i], __shfl_xor_sync(kFull, m[i], 1));
+                    m[i] = fmaxf(m[i], __shfl_xor_sync(kFull, m[i], 2));
+                    if (!(m[i] > run_max[i] + kMaxSlack)) m[i] = run_max[i];
+                    const float f = m[i] == run_max[i] ? 1.0f : ex2(run_max[i] - m[i]);
+                    run_max[i] = m[i];
+                    base[i] = (m[i] == neg_inf ? 0.0f : m[i]) - kExpShift;
+                    sum[i] *= f;
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) o[n][2 * i] *= f, o[n][2 * i + 1] *= f;
+                }
+            }
+            uint32_t pa[4];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+                const float p0 = ex2(s[nt][0] - base[0]), p1 = ex2(s[nt][1] - base[0]);
+                const float p2 = ex2(s[nt][2] - base[1]), p3 = ex2(s[nt][3] - base[1]);
+                sum[0] += p0 + p1, sum[1] += p2 + p3;
+                const __half2 a = __floats2half2_rn(p0, p1), b = __floats2half2_rn(p2, p3);
+                pa[2 * nt] = *reinterpret_cast<const uint32_t*>(&a);
+                pa[2 * nt + 1] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+
+            // values: this lane's tokens 2c, 2c + 1, 2c + 8, 2c + 9
+            uint32_t vw[4][(vShare + 3) / 4];
+            int vs[4];
+            constexpr int blocks = D / 32;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = 2 * c + (i & 1) + 8 * (i >> 1);
+                lds_bytes<vShare>(at + S::v_at + t * P::v + g * vShare, vw[i]);
+                vs[i] = (int)lds_u8(at + S::vs_at + t * blocks + (D == 128 ? g >> 1 : g >> 2));
+                if (t0 + kGranule > len && t0 + t >= len) vs[i] = 0;  // the values there are zero
+            }
+            const int top = (int)__reduce_max_sync(kFull, (unsigned)max(max(vs[0], vs[1]), max(vs[2], vs[3])));
+            if (vref == 0 || top > vref + kValueMax) {
+                const int ref = max(top - kValueLift, 1);
+                if (vref != 0) {
+                    const float f = __uint_as_float((uint32_t)max(vref - ref + 127, 0) << 23);
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[n][e] *= f;
+                }
+                vref = ref;
+            }
+            const uint32_t f0 = pow2_f16x2(vs[0] - vref, vs[1] - vref), f1 = pow2_f16x2(vs[2] - vref, vs[3] - vref);
+            bool nans = false;
+            if constexpr (BITS == 8) {
+                // A stored NaN belongs to the rows that see its token: where some row
+                // does not, it is taken out here and put into the others' sums below.
+                if (partly) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < vShare / 4; ++j) {
+                            const uint32_t bad = __vcmpeq4(vw[i][j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                            nans |= bad != 0;
+                            vw[i][j] &= ~bad;
+                        }
+                    nans = __any_sync(kFull, nans);
+                }
+            }
+            if constexpr (BITS == 4) {
+#pragma unroll
+                for (int j = 0; j < vShare / 4; ++j) {
+                    // bytes of (token, token + 1) nibbles: even features, then odd ones
+                    uint32_t even[2][4], odd[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t a = vw[2 * h][j], b = vw[2 * h + 1][j];
+                        dev::e2m1x8_to_f16((a & 0x0f0f0f0fu) | ((b << 4) & 0xf0f0f0f0u), even[h]);
+                        dev::e2m1x8_to_f16(((a >> 4) & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u), odd[h]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        mma16816(o[8 * j + 2 * i], pa, hmul2(even[0][i], f0), hmul2(even[1][i], f1));
+                        mma16816(o[8 * j + 2 * i + 1], pa, hmul2(odd[0][i], f0), hmul2(odd[1][i], f1));
+                    }
+                }
+            } else {
+                constexpr int kCode = BITS == 4 ? 8 : BITS;
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) {
+                    uint32_t four[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) four[i] = BITS == 8 ? vw[i][j] : four6(vw[i], j);
+                    // (token, token + 1) bytes of features 0, 1 and of 2, 3
+                    const uint32_t a01 = __byte_perm(four[0], four[1], 0x5140), a23 = __byte_perm(four[0], four[1], 0x7362);
+                    const uint32_t b01 = __byte_perm(four[2], four[3], 0x5140), b23 = __byte_perm(four[2], four[3], 0x7362);
+                    mma16816(o[4 * j], pa, hmul2(dev::codes_to_f16x2<kCode>(a01), f0),
+                             hmul2(dev::codes_to_f16x2<kCode>(b01), f1));
+                    mma16816(o[4 * j + 1], pa, hmul2(dev::codes_to_f16x2<kCode>(a01 >> 16), f0),
+                             hmul2(dev::codes_to_f16x2<kCode>(b01 >> 16), f1));
+                    mma16816(o[4 * j + 2], pa, hmul2(dev::codes_to_f16x2<kCode>(a23), f0),
+                             hmul2(dev::codes_to_f16x2<kCode>(b23), f1));
+                    mma16816(o[4 * j + 3], pa, hmul2(dev::codes_to_f16x2<kCode>(a23 >> 16), f0),
+                             hmul2(dev::codes_to_f16x2<kCode>(b23 >> 16), f1));
+                }
+            }
+            if (nans) {
+                for (int t = 0; t < kGranule; ++t)
+                    for (int i = 0; i < 2; ++i) {
+                        if (t0 + t < lo[i] || t0 + t >= hi[i]) continue;
+#pragma unroll
+                        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if ((lds_u8(at + S::v_at + t * P::v + (2 * c + e) * vShare + n) & 0x7fu) == 0x7fu)
+                                    o[n][2 * i + e] = __int_as_float(0x7fc00000);
+                    }
+            }
+        }
+
+        // Join the warps: common maxima, outputs in true units, sums.
+        copy_wait<0>();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            sum[i] += __shfl_xor_sync(kFull, sum[i], 1);
+            sum[i] += __shfl_xor_sync(kFull, sum[i], 2);
+            if (c == 0) stat_max[warp][g + 8 * i] = run_max[i], stat_sum[warp][g + 8 * i] = sum[i];
+        }
+        __syncthreads();  // the rings are done with as well
+        float* joined = reinterpret_cast<float*>(smem);
+        const float vfactor = vref ? __uint_as_float((uint32_t)vref << 23) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = g + 8 * i;
+            float top = stat_max[0][r];
+#pragma unroll
+            for (int k = 1; k < kWarps; ++k) top = fmaxf(top, stat_max[k][r]);
+            const float f = run_max[i] == top ? 1.0f : ex2(run_max[i] - top);
+            // features (2c + e) * D/8 + n, four at a time; the 16-byte chunks of a row are
+            // permuted so that eight lanes write to eight different bank groups
+            float4* dst = reinterpret_cast<float4*>(joined + (warp * kRows + r) * D);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int n = 0; n < kTiles; n += 4) {
+                    const int chunk = (2 * c + e) * (D / 32) + n / 4;
+                    const float4 v = make_float4(o[n][2 * i + e] * f * vfactor, o[n + 1][2 * i + e] * f * vfactor,
+                                                 o[n + 2][2 * i + e] * f * vfactor, o[n + 3][2 * i + e] * f * vfactor);
+                    dst[chunk ^ (c | ((g & 1) << 2))] = v;
+                }
+        }
+        __syncthreads();
+        const bool whole = tile0 == 0 && tiles == w.tiles;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (tile0 == 0 ? 1 : 0);
+        for (int idx = tid; idx < rows * (D / 4); idx += kThreads) {
+            const int r = idx / (D / 4), chunk = idx - r * (D / 4);
+            const int at = chunk ^ ((chunk / (D / 16)) | ((r & 1) << 2));
+            float top = neg_inf, total = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) top = fmaxf(top, stat_max[k][r]);
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                const float4 x = reinterpret_cast<const float4*>(joined + (k * kRows + r) * D)[at];
+                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                total += stat_sum[k][r] * (stat_max[k][r] == top ? 1.0f : ex2(stat_max[k][r] - top));
+            }
+            if (whole) {
+                const int row = w.rt * kRows + r, j = row / p.group;
+                const int head = w.head * p.group + (row - j * p.group);
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                dev::store4(p, w.view.row0 + j, head, chunk * 4,
+                            make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                if (p.lse && chunk == 0)
+                    p.lse[(int64_t)(w.view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
+            } else {
+                reinterpret_cast<float4*>(p.part + (slot * kRows + r) * D)[chunk] = v;
+                if (chunk == 0) p.part_stat[slot * kRows + r] = make_float2(top, total);
+            }
+        }
+        if (!whole) {
+            if (tile0 == 0) {
+                open = true;
+                if (tid == 0) p.part_open[blockIdx.x] = make_int4(w.seq, w.rt, w.head, 1);
+            } else {
+                went_on = true;
+                ended = tile0 + tiles == w.tiles;
+            }
+        }
+        __syncthreads();  // before the rings are filled again
+        left -= tiles;
+        w.tile += tiles;
+        if (left > 0) dev::walk_on<kRows, kKeys>(p, w);
+    }
+    if (tid == 0) {
+        if (!open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
+        p.part_ends[blockIdx.x] = went_on && ended ? 1 : 0;
+    }
+}
+
+// Block (x, y): the unit that CTA x began and did not finish, rows y, y + gridDim.y, ...;
+// a thread owns four features.  The parts are the beginning (slot 2x + 1) and what
+// the following CTAs did first (slots 2j), up to the one that finished the unit.
+template <int ROWS, int D>
+__global__ void __launch_bounds__(128) attention_join_kernel(const AttentionParams p) {
+    constexpr int kLanes = D / 4;              // threads of a row
+    constexpr int kSub = 128 / kLanes;         // rows at a time
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 unit = p.part_open[blockIdx.x];
+    if (!unit.w) return;
+    int last = blockIdx.x + 1;
+    while (last < (int)gridDim.x - 1 && !p.part_ends[last]) ++last;
+    const dev::SeqView view = dev::seq_view(p, unit.x);
+    const int rows = view.n * p.group - unit.y * ROWS < ROWS ? view.n * p.group - unit.y * ROWS : ROWS;
+    const int chunk = threadIdx.x % kLanes;
+    for (int r = blockIdx.y * kSub + threadIdx.x / kLanes; r < rows; r += gridDim.y * kSub) {
+        int64_t slot = 2 * (int64_t)blockIdx.x + 1;
+        float top = p.part_stat[slot * ROWS + r].x;
+        for (int j = blockIdx.x + 1; j <= last; ++j) top = fmaxf(top, p.part_stat[2 * (int64_t)j * ROWS + r].x);
+        float total = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int j = blockIdx.x; j <= last; ++j) {
+            if (j > (int)blockIdx.x) slot = 2 * (int64_t)j;
+            const float2 st = p.part_stat[slot * ROWS + r];
+            const float f = st.x == top ? 1.0f : dev::ex2(st.x - top);
+            const float4 x = reinterpret_cast<const float4*>(p.part + (slot * ROWS + r) * D)[chunk];
+            total += st.y * f;
+            v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+        }
+        const int row = unit.y * ROWS + r, j = row / p.group;
+        const int head = unit.z * p.group + (row - j * p.group);
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        dev::store4(p, view.row0 + j, head, chunk * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
+    }
+}
+
+// Memory of a launch's partial sums.
+struct Workspace {
+    void* ptr = nullptr;
+    cudaStream_t stream;
+    explicit Workspace(cudaStream_t s) : stream(s) {}
+    ~Workspace() {
+        if (ptr) cudaFreeAsync(ptr, stream);
+    }
+    Workspace(const Workspace&) = delete;
+    Workspace& operator=(const Workspace&) = delete;
+    int take(AttentionParams& p, int64_t ctas, int rows, int d) {
+        const size_t part = (size_t)(2 * ctas * rows) * d * 4, stat = (size_t)(2 * ctas * rows) * 8;
+        cudaMemPool_t pool = workspace_pool();
+        if (!pool) return fail(MXK_ERR_CUDA, "cache_attention: cannot create the workspace pool");
+        MXK_CUDA(cudaMallocFromPoolAsync(&ptr, part + stat + (size_t)ctas * 20, pool, stream));
+        p.part = static_cast<float*>(ptr);
+        p.part_stat = reinterpret_cast<float2*>(static_cast<char*>(ptr) + part);
+        p.part_open = reinterpret_cast<int4*>(static_cast<char*>(ptr) + part + stat);
+        p.part_ends = reinterpret_cast<int*>(p.part_open + ctas);
+        return MXK_OK;
+    }
+};
+
+template <int ROWS, int D>
+int join_parts(const AttentionParams& p, int ctas, int grid_y, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas, (unsigned)grid_y);
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    LaunchScope scope("attention_join", stream);
+    MXK_CUDA(cudaLaunchKernelEx(&cfg, attention_join_kernel<ROWS, D>, p));
+    return MXK_OK;
+}
+
+template <int D, int BITS>
+int launch_rows(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
+    using S = Stage<D, BITS>;
+    static thread_local int ready_device = -1;
+    int dev = 0;
+    MXK_CUDA(cudaGetDevice(&dev));
+    if (ready_device != dev) {
+        MXK_CUDA(cudaFuncSetAttribute(attention_rows_kernel<D, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      S::smem));
+        ready_device = dev;
+    }
+    static const int sms = sm_count();
+    const int64_t ctas = most_tiles < 3 * sms ? most_tiles : 3 * sms;
+    Workspace ws(stream);
+    MXK_CHECK(ws.take(p, ctas, kRows, D));
+    {
+        LaunchScope scope("attention_rows", stream);
+        attention_rows_kernel<D, BITS><<<(unsigned)ctas, kThreads, S::smem, stream>>>(p);
+        MXK_CUDA(cudaGetLastError());
+    }
+    return join_parts<kRows, D>(p, (int)ctas, 4, stream);
+}
+
+template <int D>
+int launch_rows_bits(int bits, const AttentionParams& p, int64_t most_tiles, cudaStream_t stream) {
+    if (bits == 8) return launch_rows<D, 8>(p, most_tiles, stream);
+    if (bits == 6) return launch_rows<D, 6>(p, most_tiles, stream);
+    return launch_rows<D, 4>(p, most_tiles, stream);
+}
+
+}  // namespace
+}  // namespace mxk
+
+extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* a, void* stream) {
+    using namespace mxk;
+    MXK_CHECK(check_cache(cache, "cache_attention"));
+    MXK_REQUIRE(a, "cache_attention: args is null");
+    MXK_REQUIRE(a->dtype == MXK_F16 || a->dtype == MXK_BF16, "cache_attention: dtype must be MXK_F16 or MXK_BF16");
+    MXK_REQUIRE(a->heads >= 1 && a->heads <= 65535 && a->heads % cache->kv_heads == 0,
+                "cache_attention: heads must be a positive multiple of the cache's kv_heads");
+    MXK_REQUIRE(a->tokens >= 0 && a->tokens <= std::numeric_limits<int>::max() && a->seqs >= 0,
+                "cache_attention: tokens and seqs must be in [0, 2^31)");
+    MXK_REQUIRE(a->max_q >= 0 && a->max_kv >= 0, "cache_attention: max_q and max_kv must not be negative");
+    MXK_REQUIRE((int64_t)a->max_q * a->heads <= std::numeric_limits<int>::max() / 2 &&
+                    a->max_kv <= std::numeric_limits<int>::max() / 2,
+                "cache_attention: max_q * heads and max_kv must be below 2^30");
+    MXK_REQUIRE(a->window >= 0 && (a->window == 0 || a->causal), "cache_attention: a window needs causal");
+    MXK_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, "cache_attention: scale must be finite");
+    if (cache->head_dim != 64 && cache->head_dim != 128)
+        return fail(MXK_ERR_UNSUPPORTED, "cache_attention: head_dim must be 64 or 128");
+    if (a->tokens == 0 || a->seqs == 0 || a->max_q == 0) return MXK_OK;
+    MXK_REQUIRE(a->q.data && a->out.data && a->cu_q && a->page_table && a->kv_lens,
+                "cache_attention: q, out, cu_q, page_table and kv_lens must be non-null");
+    MXK_REQUIRE((reinterpret_cast<uintptr_t>(a->q.data) | reinterpret_cast<uintptr_t>(a->out.data)) % 2 == 0 &&
+                    (reinterpret_cast<uintptr_t>(a->cu_q) | reinterpret_cast<uintptr_t>(a->page_table) |
+                     reinterpret_cast<uintptr_t>(a->kv_lens) | reinterpret_cast<uintptr_t>(a->lse)) % 4 == 0,
+                "cache_attention: pointers must be aligned to their elements");
+    const int64_t need = (a->max_kv + cache->page_size - 1) / cache->page_size;
+    MXK_REQUIRE(a->seqs == 1 || a->page_table_stride >= need,
+                "cache_attention: page_table_stride is below the pages of max_kv tokens");
+
+    AttentionParams p{};
+    p.k_values = static_cast<const uint8_t*>(cache->k_values);
+    p.v_values = static_cast<const uint8_t*>(cache->v_values);
+    p.k_scales = cache->k_scales;
+    p.v_scales = cache->v_scales;
+    p.kv_heads = cache->kv_heads;
+    p.page_size = cache->page_size;
+    p.pages = (int)cache->pages;
+    p.q = a->q.data;
+    p.out = a->out.data;
+    p.lse = a->lse;
+    p.q_token = a->q.token_stride, p.q_head = a->q.head_stride;
+    p.out_token = a->out.token_stride, p.out_head = a->out.head_stride;
+    p.tokens = a->tokens;
+    p.dtype = a->dtype;
+    p.heads = a->heads;
+    p.group = a->heads / cache->kv_heads;
+    p.seqs = a->seqs;
+    p.q_vec = rows_aligned(a->q, 2, 8);
+    p.out_vec = rows_aligned(a->out, 2, 8);
+    p.cu_q = a->cu_q;
+    p.page_table = a->page_table;
+    p.table_stride = a->page_table_stride;
+    p.max_kv = a->max_kv;
+    p.kv_lens = a->kv_lens;
+    p.scale_log2 = a->scale * 1.44269504088896f;
+    p.causal = a->causal != 0;
+    p.window = a->window;
+    p.min_rows = 1;
+    p.max_rows = std::numeric_limits<int>::max();
+
+    // Key tiles there can be at most: of one row tile of every sequence, a window
+    // touching at most one tile more than it and the row tile's tokens fill.
+    const int64_t row_tiles = ((int64_t)a->max_q * p.group + kRows - 1) / kRows;
+    int64_t span = a->max_kv;
+    if (p.window > 0 && p.window + kRows < span) span = p.window + kRows;
+    const int64_t per_unit = span / kKeys + 2;
+    const int64_t most_tiles = (int64_t)a->seqs * p.kv_heads * row_tiles * per_unit;
+    return cache->head_dim == 128
+               ? launch_rows_bits<128>(cache->bits, p, most_tiles, as_stream(stream))
+               : launch_rows_bits<64>(cache->bits, p, most_tiles, as_stream(stream));
+}

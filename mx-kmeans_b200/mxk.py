@@ -46,6 +46,33 @@ class KernelStat(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 48), ("launches", ctypes.c_uint64), ("total_ms", ctypes.c_double)]
 
 
+F32, F16, BF16 = range(3)  # mxk_dtype
+
+
+class Cache(ctypes.Structure):
+    """mxk_cache: sizes and device pointers of a paged MX cache."""
+
+    _fields_ = [("bits", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("pages", ctypes.c_int64), ("k_values", ctypes.c_void_p),
+                ("k_scales", ctypes.c_void_p), ("v_values", ctypes.c_void_p), ("v_scales", ctypes.c_void_p)]
+
+
+class Rows(ctypes.Structure):
+    """mxk_rows: rows of tokens x heads x features with strides in elements."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class Attention(ctypes.Structure):
+    """mxk_attention: the arguments of mxk_cache_attention."""
+
+    _fields_ = [("dtype", ctypes.c_int), ("heads", ctypes.c_int), ("tokens", ctypes.c_int64),
+                ("seqs", ctypes.c_int), ("max_q", ctypes.c_int), ("max_kv", ctypes.c_int64), ("q", Rows),
+                ("cu_q", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("page_table_stride", ctypes.c_int64),
+                ("kv_lens", ctypes.c_void_p), ("scale", ctypes.c_float), ("causal", ctypes.c_int),
+                ("window", ctypes.c_int64), ("out", Rows), ("lse", ctypes.c_void_p)]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
@@ -90,6 +117,9 @@ SIGNATURES = {
     "mxk_host_read_points_ex": ([ctypes.c_char_p, _I64, _I, _I, _I, _I64, _P], _I),
     "mxk_host_read_points_f32": ([ctypes.c_char_p, _I64, _I, _I, _P], _I),
     "mxk_host_write_labels": ([ctypes.c_char_p, _P, _I64], _I),
+    "mxk_cache_write": ([ctypes.POINTER(Cache), _I, _I64, ctypes.POINTER(Rows), ctypes.POINTER(Rows), _P, _P], _I),
+    "mxk_cache_read": ([ctypes.POINTER(Cache), _I, _I64, _P, ctypes.POINTER(Rows), ctypes.POINTER(Rows), _P], _I),
+    "mxk_cache_attention": ([ctypes.POINTER(Cache), ctypes.POINTER(Attention), _P], _I),
     "mxk_profile_enable": ([_I], _I),
     "mxk_profile_read": ([ctypes.POINTER(KernelStat), _I, ctypes.POINTER(_I)], _I),
 }
@@ -327,6 +357,129 @@ def kmeans_mixed_sharded(comm, points, centroids, labels, options=None, stream=N
                                           _ptr(points), _ptr(centroids), _ptr(labels), ctypes.byref(opts),
                                           ctypes.byref(iters), _stream(stream)))
     return iters.value
+
+
+# ----------------------------------------------------------------------------- paged MX cache
+
+def _tensor(t, name, dtype, *shape):
+    """t as named: a CUDA tensor of `dtype` with `shape` (None: any size)."""
+    if not t.is_cuda or t.dtype != dtype or t.dim() != len(shape) or any(
+            n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise MxkInvalidArgument(ERR_INVALID, f"{name}: a CUDA {dtype} tensor of shape {shape} is needed, got "
+                                              f"{t.device} {t.dtype} {tuple(t.shape)}")
+
+
+class PagedCache:
+    """Paged MX keys and values over the caller's tensors (mxk_cache): values
+    [pages, kv_heads, page_size, head_dim * bits / 8] and scales
+    [pages, kv_heads, page_size, head_dim / 32], uint8 and contiguous."""
+
+    def __init__(self, k_values, k_scales, v_values, v_scales, bits):
+        import torch
+        if bits not in (4, 6, 8):
+            raise MxkInvalidArgument(ERR_INVALID, "bits must be 4, 6 or 8")
+        if k_values.dim() != 4 or k_scales.dim() != 4:
+            raise MxkInvalidArgument(ERR_INVALID, "cache tensors have 4 dimensions")
+        pages, heads, page, blocks = k_scales.shape
+        for t, name, last in ((k_values, "k_values", blocks * 4 * bits), (k_scales, "k_scales", blocks),
+                              (v_values, "v_values", blocks * 4 * bits), (v_scales, "v_scales", blocks)):
+            _tensor(t, name, torch.uint8, pages, heads, page, last)
+            if not t.is_contiguous() or t.device != k_scales.device:
+                raise MxkInvalidArgument(ERR_INVALID, f"{name} must be contiguous, all four on one device")
+        self.k_values, self.k_scales, self.v_values, self.v_scales = k_values, k_scales, v_values, v_scales
+        self.bits, self.pages, self.kv_heads, self.page_size = bits, pages, heads, page
+        self.head_dim, self.device = blocks * 32, k_scales.device
+        self.struct = Cache(bits, heads, blocks * 32, page, pages, k_values.data_ptr(), k_scales.data_ptr(),
+                            v_values.data_ptr(), v_scales.data_ptr())
+
+    @classmethod
+    def empty(cls, pages, page_size, kv_heads, head_dim, bits=8, device="cuda"):
+        """A cache of zeros."""
+        import torch
+
+        def make(last):
+            return torch.zeros(pages, kv_heads, page_size, last, dtype=torch.uint8, device=device)
+        return cls(make(head_dim * bits // 8), make(head_dim // 32), make(head_dim * bits // 8),
+                   make(head_dim // 32), bits)
+
+
+_DTYPES = {}
+
+
+def _dtype(t, name):
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    if t.dtype not in _DTYPES:
+        raise MxkInvalidArgument(ERR_INVALID, f"{name}: float32, float16 or bfloat16 is needed, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _rows(t, name, heads, dim):
+    """mxk_rows of t [tokens, heads, dim], whose features must be contiguous."""
+    if not t.is_cuda or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
+        raise MxkInvalidArgument(ERR_INVALID, f"{name}: a CUDA tensor of shape [tokens, {heads}, {dim}] is needed, "
+                                              f"got {t.device} {tuple(t.shape)}")
+    strides = t.stride()
+    if strides[2] != 1:
+        raise MxkInvalidArgument(ERR_INVALID, f"{name}: the features of a row must be contiguous")
+    return Rows(t.data_ptr(), strides[0], strides[1])
+
+
+def _cache_pair(cache, k, v, slots):
+    import torch
+    kr, vr = (_rows(t, n, cache.kv_heads, cache.head_dim) for t, n in ((k, "k"), (v, "v")))
+    if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
+        raise MxkInvalidArgument(ERR_INVALID, "k and v must have the same type and number of tokens")
+    _tensor(slots, "slots", torch.int64, k.shape[0])
+    if not slots.is_contiguous():
+        raise MxkInvalidArgument(ERR_INVALID, "slots must be contiguous")
+    return _dtype(k, "k"), kr, vr
+
+
+def cache_write(cache, k, v, slots, stream=None):
+    """Quantise the rows of k and v [tokens, kv_heads, head_dim] into the cache's
+    slots (int64; page * page_size + place; one outside the cache: not kept)."""
+    dtype, kr, vr = _cache_pair(cache, k, v, slots)
+    check(load().mxk_cache_write(cache.struct, dtype, k.shape[0], kr, vr, slots.data_ptr(), _stream(stream)))
+
+
+def cache_read(cache, slots, k, v, stream=None):
+    """The values that the cache holds at `slots` into k and v [tokens, kv_heads,
+    head_dim] (zeros for a slot outside the cache)."""
+    dtype, kr, vr = _cache_pair(cache, k, v, slots)
+    check(load().mxk_cache_read(cache.struct, dtype, k.shape[0], slots.data_ptr(), kr, vr, _stream(stream)))
+
+
+def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale=None, causal=True, window=0,
+                    lse=None, stream=None):
+    """Attention of each sequence's newest tokens over its cached ones (mxk.h,
+    mxk_cache_attention): q, out [tokens, heads, head_dim] float16 or bfloat16;
+    cu_q [seqs + 1], page_table [seqs, pages], kv_lens [seqs] int32; max_q, max_kv:
+    bounds on a sequence's new and cached tokens; scale: 1 / sqrt(head_dim) unless
+    given; lse: float32 [tokens, heads] or None."""
+    import torch
+    tokens, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+    qr, outr = _rows(q, "q", heads, cache.head_dim), _rows(out, "out", heads, cache.head_dim)
+    seqs = kv_lens.shape[0] if kv_lens.dim() else 0
+    i32 = torch.int32
+    _tensor(cu_q, "cu_q", i32, seqs + 1)
+    _tensor(kv_lens, "kv_lens", i32, seqs)
+    _tensor(page_table, "page_table", i32, seqs, None)
+    if not (cu_q.is_contiguous() and kv_lens.is_contiguous()) or page_table.stride(1) != 1 < page_table.shape[1]:
+        raise MxkInvalidArgument(ERR_INVALID, "cu_q, kv_lens and the rows of page_table must be contiguous")
+    if page_table.shape[1] * cache.page_size < max_kv:
+        raise MxkInvalidArgument(ERR_INVALID, "page_table has fewer pages than max_kv tokens need")
+    if out.dtype != q.dtype or out.shape[0] != tokens:
+        raise MxkInvalidArgument(ERR_INVALID, "out must have q's type and number of tokens")
+    if lse is not None:
+        _tensor(lse, "lse", torch.float32, tokens, heads)
+        if not lse.is_contiguous():
+            raise MxkInvalidArgument(ERR_INVALID, "lse must be contiguous")
+    args = Attention(_dtype(q, "q"), heads, tokens, seqs, max_q, max_kv, qr, cu_q.data_ptr(), page_table.data_ptr(),
+                     page_table.stride(0), kv_lens.data_ptr(), cache.head_dim ** -0.5 if scale is None else scale,
+                     bool(causal), window, outr, None if lse is None else lse.data_ptr())
+    check(load().mxk_cache_attention(cache.struct, args, _stream(stream)))
 
 
 def profile_enable(on=True):
