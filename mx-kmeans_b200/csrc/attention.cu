@@ -31,6 +31,13 @@ namespace mxk {
 namespace {
 
 using dev::ex2;
+using dev::four6;
+using dev::hmul2;
+using dev::kKeyLift;
+using dev::kQueryExp;
+using dev::kValueLift;
+using dev::kValueMax;
+using dev::pow2_f16x2;
 using dev::kExpShift;
 using dev::kMaxSlack;
 
@@ -40,6 +47,9 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kGranule = 16;  // tokens of one step of a warp
 constexpr int kKeys = kGranule * kWarps;
+// Rows per key head up to which this kernel is taken, one pass over the keys for
+// every 16 of them.
+constexpr int kMostFewRows = 32;
 
 // Shared-memory row pitches (bytes) of the key and value granules; each makes the
 // lanes of one load instruction touch all banks once.  Keys are read row by row,
@@ -111,26 +121,6 @@ __device__ __forceinline__ uint32_t lds_u8(uint32_t at) {
     return v;
 }
 
-// The j-th group of four 6-bit codes of a packed row, one per byte.
-__device__ __forceinline__ uint32_t four6(const uint32_t* w, int j) {
-    const int bit = 24 * j, i = bit / 32, s = bit % 32;
-    const uint32_t v = s <= 8 ? w[i] >> s : __funnelshift_r(w[i], w[i + 1], s);
-    return dev::spread6(v);
-}
-
-// f16 pair of 2^(e0), 2^(e1), zero where that is below f16's range (e <= 15).
-__device__ __forceinline__ uint32_t pow2_f16x2(int e0, int e1) {
-    const float a = __uint_as_float((uint32_t)max(e0 + 127, 0) << 23);
-    const float b = __uint_as_float((uint32_t)max(e1 + 127, 0) << 23);
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 // c += a (16 x 16, row) * b (16 x 8, column), f16 operands, f32 sums.
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -148,13 +138,6 @@ __device__ __forceinline__ int row_scale(uint32_t w) {
     if constexpr (D == 128) m = max(m, max((int)((w >> 16) & 255u), (int)(w >> 24)));
     return max(m, 1);
 }
-
-// Element headroom: codes are at most 448 < 2^9, f16 reaches 2^16, so block
-// factors go up to 2^6; keys use it fully, values start at 2^4 and may grow to 2^6
-// before their reference moves.
-constexpr int kKeyLift = 6;
-constexpr int kValueLift = 4, kValueMax = 6;
-constexpr int kQueryExp = 12;  // query rows are scaled to a largest magnitude in [2^12, 2^13)
 
 template <int D, int BITS>
 __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const AttentionParams p) {
@@ -578,83 +561,6 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
     }
 }
 
-// Block (x, y): the unit that CTA x began and did not finish, rows y, y + gridDim.y, ...;
-// a thread owns four features.  The parts are the beginning (slot 2x + 1) and what
-// the following CTAs did first (slots 2j), up to the one that finished the unit.
-template <int ROWS, int D>
-__global__ void __launch_bounds__(128) attention_join_kernel(const AttentionParams p) {
-    constexpr int kLanes = D / 4;              // threads of a row
-    constexpr int kSub = 128 / kLanes;         // rows at a time
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 unit = p.part_open[blockIdx.x];
-    if (!unit.w) return;
-    int last = blockIdx.x + 1;
-    while (last < (int)gridDim.x - 1 && !p.part_ends[last]) ++last;
-    const dev::SeqView view = dev::seq_view(p, unit.x);
-    const int rows = view.n * p.group - unit.y * ROWS < ROWS ? view.n * p.group - unit.y * ROWS : ROWS;
-    const int chunk = threadIdx.x % kLanes;
-    for (int r = blockIdx.y * kSub + threadIdx.x / kLanes; r < rows; r += gridDim.y * kSub) {
-        int64_t slot = 2 * (int64_t)blockIdx.x + 1;
-        float top = p.part_stat[slot * ROWS + r].x;
-        for (int j = blockIdx.x + 1; j <= last; ++j) top = fmaxf(top, p.part_stat[2 * (int64_t)j * ROWS + r].x);
-        float total = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int j = blockIdx.x; j <= last; ++j) {
-            if (j > (int)blockIdx.x) slot = 2 * (int64_t)j;
-            const float2 st = p.part_stat[slot * ROWS + r];
-            const float f = st.x == top ? 1.0f : dev::ex2(st.x - top);
-            const float4 x = reinterpret_cast<const float4*>(p.part + (slot * ROWS + r) * D)[chunk];
-            total += st.y * f;
-            v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
-        }
-        const int row = unit.y * ROWS + r, j = row / p.group;
-        const int head = unit.z * p.group + (row - j * p.group);
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        dev::store4(p, view.row0 + j, head, chunk * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-        if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
-    }
-}
-
-// Memory of a launch's partial sums.
-struct Workspace {
-    void* ptr = nullptr;
-    cudaStream_t stream;
-    explicit Workspace(cudaStream_t s) : stream(s) {}
-    ~Workspace() {
-        if (ptr) cudaFreeAsync(ptr, stream);
-    }
-    Workspace(const Workspace&) = delete;
-    Workspace& operator=(const Workspace&) = delete;
-    int take(AttentionParams& p, int64_t ctas, int rows, int d) {
-        const size_t part = (size_t)(2 * ctas * rows) * d * 4, stat = (size_t)(2 * ctas * rows) * 8;
-        cudaMemPool_t pool = workspace_pool();
-        if (!pool) return fail(MXK_ERR_CUDA, "cache_attention: cannot create the workspace pool");
-        MXK_CUDA(cudaMallocFromPoolAsync(&ptr, part + stat + (size_t)ctas * 20, pool, stream));
-        p.part = static_cast<float*>(ptr);
-        p.part_stat = reinterpret_cast<float2*>(static_cast<char*>(ptr) + part);
-        p.part_open = reinterpret_cast<int4*>(static_cast<char*>(ptr) + part + stat);
-        p.part_ends = reinterpret_cast<int*>(p.part_open + ctas);
-        return MXK_OK;
-    }
-};
-
-template <int ROWS, int D>
-int join_parts(const AttentionParams& p, int ctas, int grid_y, cudaStream_t stream) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas, (unsigned)grid_y);
-    cfg.blockDim = dim3(128);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    LaunchScope scope("attention_join", stream);
-    MXK_CUDA(cudaLaunchKernelEx(&cfg, attention_join_kernel<ROWS, D>, p));
-    return MXK_OK;
-}
-
 template <int D, int BITS>
 int launch_rows(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
     using S = Stage<D, BITS>;
@@ -747,14 +653,20 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     p.min_rows = 1;
     p.max_rows = std::numeric_limits<int>::max();
 
-    // Key tiles there can be at most: of one row tile of every sequence, a window
-    // touching at most one tile more than it and the row tile's tokens fill.
-    const int64_t row_tiles = ((int64_t)a->max_q * p.group + kRows - 1) / kRows;
-    int64_t span = a->max_kv;
-    if (p.window > 0 && p.window + kRows < span) span = p.window + kRows;
-    const int64_t per_unit = span / kKeys + 2;
-    const int64_t most_tiles = (int64_t)a->seqs * p.kv_heads * row_tiles * per_unit;
-    return cache->head_dim == 128
-               ? launch_rows_bits<128>(cache->bits, p, most_tiles, as_stream(stream))
-               : launch_rows_bits<64>(cache->bits, p, most_tiles, as_stream(stream));
+    // Sequences with few rows per key head go to the rows kernel, the others to the
+    // tiles kernel; a single sequence has one kernel chosen by its bound, several are
+    // sorted by the kernels themselves.
+    const cudaStream_t st = as_stream(stream);
+    const int64_t rows = (int64_t)a->max_q * p.group;
+    if (rows > kMostFewRows) {
+        AttentionParams many = p;
+        if (a->seqs > 1) many.min_rows = kMostFewRows + 1;
+        MXK_CHECK(launch_attention_tiles(cache->bits, cache->head_dim, many, a->max_q, st));
+        if (a->seqs == 1) return MXK_OK;
+        p.max_rows = kMostFewRows;
+    }
+    const int few_q = rows > kMostFewRows ? (kMostFewRows + p.group - 1) / p.group : a->max_q;
+    const int64_t most = attention_tile_bound(p, few_q, kRows, kKeys);
+    return cache->head_dim == 128 ? launch_rows_bits<128>(cache->bits, p, most, st)
+                                  : launch_rows_bits<64>(cache->bits, p, most, st);
 }

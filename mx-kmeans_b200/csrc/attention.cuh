@@ -48,6 +48,19 @@ struct AttentionParams {
     int* part_ends;     // [CTAs]: 1 if the unit that the CTA went on with ends in it
 };
 
+// Key tiles there can be at most when no sequence has more than max_q query and
+// p.max_kv cached tokens: a window touches at most one tile more than it and the
+// row tile's tokens fill.
+inline int64_t attention_tile_bound(const AttentionParams& p, int max_q, int rows, int keys) {
+    const int64_t row_tiles = ((int64_t)max_q * p.group + rows - 1) / rows;
+    int64_t span = p.max_kv;
+    if (p.window > 0 && p.window + rows < span) span = p.window + rows;
+    return (int64_t)p.seqs * p.kv_heads * row_tiles * (span / keys + 2);
+}
+
+// attention_tiles.cu: many query rows per key head.
+int launch_attention_tiles(int bits, int head_dim, const AttentionParams& p, int max_q, cudaStream_t stream);
+
 namespace dev {
 
 // exp(s - max) is held as 2^(s2 - m2 + kExpShift) with s2, m2 in log2 units: up
@@ -62,6 +75,33 @@ __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+
+// Element headroom: codes are at most 448 < 2^9, f16 reaches 2^16, so block
+// factors go up to 2^6; keys use it fully, values start at 2^4 and may grow to 2^6
+// before their reference moves.
+constexpr int kKeyLift = 6;
+constexpr int kValueLift = 4, kValueMax = 6;
+constexpr int kQueryExp = 12;  // query rows are scaled to a largest magnitude in [2^12, 2^13)
+
+// The j-th group of four 6-bit codes of a packed row, one per byte.
+__device__ __forceinline__ uint32_t four6(const uint32_t* w, int j) {
+    const int bit = 24 * j, i = bit / 32, s = bit % 32;
+    const uint32_t v = s <= 8 ? w[i] >> s : __funnelshift_r(w[i], w[i + 1], s);
+    return dev::spread6(v);
+}
+
+// f16 pair of 2^(e0), 2^(e1), zero where that is below f16's range (e <= 15).
+__device__ __forceinline__ uint32_t pow2_f16x2(int e0, int e1) {
+    const float a = __uint_as_float((uint32_t)max(e0 + 127, 0) << 23);
+    const float b = __uint_as_float((uint32_t)max(e1 + 127, 0) << 23);
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // One sequence as the host's bounds let it be seen.
@@ -250,5 +290,81 @@ __device__ __forceinline__ float row_lse(float m2, float sum) {
 
 }  // namespace dev
 
+// Block (x, y): the unit that CTA x began and did not finish, rows y, y + gridDim.y, ...;
+// a thread owns four features.  The parts are the beginning (slot 2x + 1) and what
+// the following CTAs did first (slots 2j), up to the one that finished the unit.
+template <int ROWS, int D>
+__global__ void __launch_bounds__(128) attention_join_kernel(const AttentionParams p) {
+    constexpr int kLanes = D / 4;              // threads of a row
+    constexpr int kSub = 128 / kLanes;         // rows at a time
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 unit = p.part_open[blockIdx.x];
+    if (!unit.w) return;
+    int last = blockIdx.x + 1;
+    while (last < (int)gridDim.x - 1 && !p.part_ends[last]) ++last;
+    const dev::SeqView view = dev::seq_view(p, unit.x);
+    const int rows = view.n * p.group - unit.y * ROWS < ROWS ? view.n * p.group - unit.y * ROWS : ROWS;
+    const int chunk = threadIdx.x % kLanes;
+    for (int r = blockIdx.y * kSub + threadIdx.x / kLanes; r < rows; r += gridDim.y * kSub) {
+        int64_t slot = 2 * (int64_t)blockIdx.x + 1;
+        float top = p.part_stat[slot * ROWS + r].x;
+        for (int j = blockIdx.x + 1; j <= last; ++j) top = fmaxf(top, p.part_stat[2 * (int64_t)j * ROWS + r].x);
+        float total = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int j = blockIdx.x; j <= last; ++j) {
+            if (j > (int)blockIdx.x) slot = 2 * (int64_t)j;
+            const float2 st = p.part_stat[slot * ROWS + r];
+            const float f = st.x == top ? 1.0f : dev::ex2(st.x - top);
+            const float4 x = reinterpret_cast<const float4*>(p.part + (slot * ROWS + r) * D)[chunk];
+            total += st.y * f;
+            v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+        }
+        const int row = unit.y * ROWS + r, j = row / p.group;
+        const int head = unit.z * p.group + (row - j * p.group);
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        dev::store4(p, view.row0 + j, head, chunk * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
+    }
+}
+
+// Memory of a launch's partial sums.
+struct Workspace {
+    void* ptr = nullptr;
+    cudaStream_t stream;
+    explicit Workspace(cudaStream_t s) : stream(s) {}
+    ~Workspace() {
+        if (ptr) cudaFreeAsync(ptr, stream);
+    }
+    Workspace(const Workspace&) = delete;
+    Workspace& operator=(const Workspace&) = delete;
+    int take(AttentionParams& p, int64_t ctas, int rows, int d) {
+        const size_t part = (size_t)(2 * ctas * rows) * d * 4, stat = (size_t)(2 * ctas * rows) * 8;
+        cudaMemPool_t pool = workspace_pool();
+        if (!pool) return fail(MXK_ERR_CUDA, "cache_attention: cannot create the workspace pool");
+        MXK_CUDA(cudaMallocFromPoolAsync(&ptr, part + stat + (size_t)ctas * 20, pool, stream));
+        p.part = static_cast<float*>(ptr);
+        p.part_stat = reinterpret_cast<float2*>(static_cast<char*>(ptr) + part);
+        p.part_open = reinterpret_cast<int4*>(static_cast<char*>(ptr) + part + stat);
+        p.part_ends = reinterpret_cast<int*>(p.part_open + ctas);
+        return MXK_OK;
+    }
+};
+
+template <int ROWS, int D>
+inline int join_parts(const AttentionParams& p, int ctas, int grid_y, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas, (unsigned)grid_y);
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    LaunchScope scope("attention_join", stream);
+    MXK_CUDA(cudaLaunchKernelEx(&cfg, attention_join_kernel<ROWS, D>, p));
+    return MXK_OK;
+}
 
 }  // namespace mxk
