@@ -46,6 +46,11 @@ struct AttentionParams {
     float2* part_stat;  // [2 * CTAs][tile rows]: running maximum (log2 units), sum
     int4* part_open;    // [CTAs]: {sequence, row tile, key head, 1} of the unit begun and left unfinished, or {.., 0}
     int* part_ends;     // [CTAs]: 1 if the unit that the CTA went on with ends in it
+    // keys and values converted beforehand (tiles kernel), [seqs][kv_heads][max_tiles]
+    uint8_t* ready_k;
+    uint8_t* ready_v;
+    int2* ready_meta;   // reference scales of the keys and values; bit 16 of y: NaNs taken out
+    int max_tiles;
 };
 
 // Key tiles there can be at most when no sequence has more than max_q query and
@@ -59,7 +64,7 @@ inline int64_t attention_tile_bound(const AttentionParams& p, int max_q, int row
 }
 
 // attention_tiles.cu: many query rows per key head.
-int launch_attention_tiles(int bits, int head_dim, const AttentionParams& p, int max_q, cudaStream_t stream);
+int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, cudaStream_t stream);
 
 namespace dev {
 
@@ -331,6 +336,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionPara
 // Memory of a launch's partial sums.
 struct Workspace {
     void* ptr = nullptr;
+    void* extra = nullptr;
     cudaStream_t stream;
     explicit Workspace(cudaStream_t s) : stream(s) {}
     ~Workspace() {
@@ -338,11 +344,14 @@ struct Workspace {
     }
     Workspace(const Workspace&) = delete;
     Workspace& operator=(const Workspace&) = delete;
-    int take(AttentionParams& p, int64_t ctas, int rows, int d) {
+    // extra: bytes at `extra`, 256-byte aligned.
+    int take(AttentionParams& p, int64_t ctas, int rows, int d, int64_t extra_bytes = 0) {
         const size_t part = (size_t)(2 * ctas * rows) * d * 4, stat = (size_t)(2 * ctas * rows) * 8;
+        const size_t own = (part + stat + (size_t)ctas * 20 + 255) / 256 * 256;
         cudaMemPool_t pool = workspace_pool();
         if (!pool) return fail(MXK_ERR_CUDA, "cache_attention: cannot create the workspace pool");
-        MXK_CUDA(cudaMallocFromPoolAsync(&ptr, part + stat + (size_t)ctas * 20, pool, stream));
+        MXK_CUDA(cudaMallocFromPoolAsync(&ptr, own + (size_t)extra_bytes, pool, stream));
+        extra = static_cast<char*>(ptr) + own;
         p.part = static_cast<float*>(ptr);
         p.part_stat = reinterpret_cast<float2*>(static_cast<char*>(ptr) + part);
         p.part_open = reinterpret_cast<int4*>(static_cast<char*>(ptr) + part + stat);

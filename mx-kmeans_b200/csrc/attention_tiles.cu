@@ -1,4 +1,4 @@
-// Attention of new tokens over the paged MX cache: the kernel for many query rows
+// Attention of new tokens over the paged MX cache: the kernels for many query rows
 // per key head (no counterpart in the reference).
 //
 // With many rows the two products bound it (4 * rows * keys * D operations), with
@@ -7,22 +7,27 @@
 // 128, each with its scores and its output in TMEM, so the tensor core multiplies
 // for one tile while the other one is in its softmax.
 //
-//   warps 0-3, 4-7   softmax of row tile 0, 1: a thread owns one row -- its query,
-//                    running maximum and sum, its weights and its output row
-//   warps 8-11       converters: packed keys and values from the cache's pages to
-//                    f16 tiles in shared memory (SWIZZLE_128B), two stages each
-//   warp 12          the only thread that issues products (warps 13-15 idle):
-//                    S = Q K^T from shared memory, O += P V with P from TMEM
+//   softmax     two warpgroups, one per row tile; a thread owns one row: its query,
+//               running maximum and sum, its weights and its output row
+//   products    one warp, whose elected lane issues S = Q K^T from shared memory and
+//               O += P V with P from TMEM
+//   keys and    two stages each of f16 tiles in shared memory (SWIZZLE_128B), filled
+//   values      either by four converter warps from the packed pages, or, when many
+//               row tiles share a key head, by bulk copies of tiles that
+//               attention_unpack_kernel has converted once for all of them
 //
 // P (f16) overwrites the S it came from, so TMEM holds S0 S1 O0 O1, 512 columns at
 // D = 128.  Values are the right operand as they lie in the cache (one row per
 // token), read by the tensor core as an N-major operand, so nothing is transposed.
 //
-// Scales: the keys of a 128-token tile are converted relative to the tile's
-// largest scale, which goes into the factor of the scores (per tile and row);
-// values relative to a reference that moves up with the data (attention_rows_kernel
-// does the same), on which the output rows are rescaled together with the running
-// maximum, both rarely.
+// Scales: the keys of a 128-token tile are held relative to the tile's largest
+// scale, which goes into the factor of the scores (per tile and row).  Values are
+// held relative to a reference of their tile, a multiple of kRefStep octaves at or
+// above its largest scale; the output rows are kept relative to the largest
+// reference so far, and a tile with a smaller one has its weights scaled down by the
+// difference, so a row is rescaled only when the reference goes up or its maximum does.
+#include <type_traits>
+
 #include "attention.cuh"
 
 namespace mxk {
@@ -33,22 +38,37 @@ using dev::kExpShift;
 using dev::kKeyLift;
 using dev::kMaxSlack;
 using dev::kQueryExp;
-using dev::kValueLift;
-using dev::kValueMax;
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kTileRows = 128;           // M of one product
 constexpr int kRows = 2 * kTileRows;     // rows of a unit
 constexpr int kKeys = 128;               // tokens of a key tile
+constexpr int kStages = 2;               // of keys and of values
+constexpr int kMeta = 4;                 // key tiles whose references are kept (converter warps)
+constexpr int kRefStep = 4;              // value references are multiples of this many octaves
 constexpr int kSoftmaxWarps = 8;
-constexpr int kConvertWarps = 4;
-constexpr int kThreads = 512;            // whole warpgroups, for the register split
-// Registers a thread: the kernel is launched with 128, warps 12-15 give theirs up.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 160, kConvertRegs = 144, kProductRegs = 48;
-static_assert(256 * kSoftmaxRegs + 128 * (kConvertRegs + kProductRegs) <= kThreads * kLaunchRegs,
-              "the split draws on what the block was launched with");
-constexpr int kStages = 2;
-constexpr int kMeta = 4;                 // key tiles whose references are kept
+
+// Rows per key head above which its keys are converted beforehand, and the most
+// memory that may take.
+constexpr int kReadyRows = kRows;
+constexpr int64_t kReadyBytes = 4ll << 30;
+
+// The two kernels' warps and registers.  Warpgroups give up or take registers of
+// those the block was launched with: the softmax of ready-made tiles holds a row's 128
+// scores in registers, next to converter warps it reads them from TMEM twice.
+struct Packed {
+    static constexpr int convert_warps = 8;
+    static constexpr int product_warp = kSoftmaxWarps + convert_warps;
+    static constexpr int threads = 640;
+    static constexpr int launch_regs = 96, softmax_regs = 120, convert_regs = 80, product_regs = 72;
+    static_assert(256 * softmax_regs + 256 * convert_regs + 128 * product_regs <= threads * launch_regs, "");
+};
+struct Ready {
+    static constexpr int product_warp = kSoftmaxWarps, load_warp = kSoftmaxWarps + 1;
+    static constexpr int threads = 384;
+    static constexpr int launch_regs = 168, softmax_regs = 208, product_regs = 88;
+    static_assert(256 * softmax_regs + 128 * product_regs <= threads * launch_regs, "");
+};
 
 template <int D>
 struct Smem {
@@ -60,13 +80,33 @@ struct Smem {
     static constexpr int total = v + kStages * tile + 1024;  // 1024: alignment
 };
 
-struct Bars {
+struct Shared {
     uint64_t q_ready[2];       // the tile's queries are in shared memory
     uint64_t k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
     uint64_t s_full[2];        // scores are in TMEM
     uint64_t p_ready[2];       // weights are in TMEM, the output may be added to
     uint64_t o_done[2];        // the tile's product with the values has finished
     uint64_t drain;
+    int2 meta[kMeta];          // converter warps: the key tile's references
+    int nan_unit[4];           // converter warps: unit in which a NaN was taken out of a partly seen tile
+    int abort_word;
+    uint32_t tmem;
+};
+
+// What the roles of a CTA share.
+struct Block {
+    uint8_t* smem;
+    Shared* sh;
+    uint32_t tmem;
+    unsigned* err;
+    __device__ __forceinline__ volatile int* abort_flag() const { return &sh->abort_word; }
+    // Bounded wait of a whole warp; false: it gave up, leave for the end of the kernel.
+    __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
+        return __all_sync(kFull, dev::mbar_wait(bar, parity, abort_flag(), err));
+    }
+    __device__ __forceinline__ bool wait_lean(uint64_t* bar, uint32_t parity) const {
+        return __all_sync(kFull, dev::mbar_wait_lean(bar, parity, abort_flag(), err));
+    }
 };
 
 // A pass over the CTA's share: every role makes the same one.
@@ -92,27 +132,27 @@ struct Cursor {
         const int r = w.view.n * p.group - w.rt * kRows;
         return r < kRows ? r : kRows;
     }
+    __device__ __forceinline__ bool whole() const { return tile0 == 0 && tiles == w.tiles; }
 };
 
-// Tokens seen by some and by all rows of a unit.
-struct UnitRange {
-    int64_t any_lo, any_hi, all_lo, all_hi;
+// Key tiles [from, to) of the cursor's share of its unit are seen whole by all its rows.
+struct Whole {
+    int from, to;
 };
-__device__ __forceinline__ UnitRange unit_range(const AttentionParams& p, const Cursor& c) {
-    UnitRange u;
+__device__ __forceinline__ Whole whole_tiles(const AttentionParams& p, const Cursor& c) {
     const int r0 = c.w.rt * kRows, j0 = r0 / p.group, j1 = (r0 + c.rows(p) - 1) / p.group;
-    int64_t x;
-    dev::seen_range(p, c.w.view, j0, j1, u.any_lo, u.any_hi);
-    dev::seen_range(p, c.w.view, j0, j0, x, u.all_hi);
-    dev::seen_range(p, c.w.view, j1, j1, u.all_lo, x);
-    return u;
+    int64_t lo, hi, x;
+    dev::seen_range(p, c.w.view, j0, j0, x, hi);   // the first row ends first,
+    dev::seen_range(p, c.w.view, j1, j1, lo, x);   // the last begins last
+    const int64_t first = c.w.first + c.tile0;
+    const int64_t a = (lo + kKeys - 1) / kKeys - first, b = (hi < 0 ? 0 : hi) / kKeys - first;
+    Whole wt;
+    wt.from = a < 0 ? 0 : (a < c.tiles ? (int)a : c.tiles);
+    wt.to = b < 0 ? 0 : (b < c.tiles ? (int)b : c.tiles);
+    return wt;
 }
 
-__device__ __forceinline__ int2 lds_int2(uint32_t at) {
-    int2 v;
-    asm volatile("ld.shared.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
-    return v;
-}
+// ---------------------------------------------------------------- key and value tiles
 
 template <int N>
 __device__ __forceinline__ void ldg_bytes(const uint8_t* src, uint32_t* w) {
@@ -149,556 +189,791 @@ __device__ __forceinline__ void convert16(const uint32_t* w, uint32_t f, uint32_
     }
 }
 
+// Eight warps turning a tile of 128 packed rows into f16: a thread converts 16-element
+// piece `u` of every kStep-th row.  Eight neighbouring lanes cover the 16-byte chunks of
+// two rows, so the swizzled stores meet no shared-memory bank twice.
 template <int D, int BITS>
-__global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const AttentionParams p, unsigned* err) {
+struct Converter {
+    static constexpr int row_bytes = D * BITS / 8;
+    static constexpr int pieces = D / 16;                   // of a row
+    static constexpr int piece_words = BITS / 2;
+    static constexpr int warp_rows = 32 / pieces;
+    static constexpr int step = 8 * warp_rows;              // rows of one pass of the eight warps
+    static constexpr int passes = kKeys / step;
+    using Words = uint32_t[passes][piece_words];
+
+    int lane, u, r0;
+    bool high;  // r0 is in the second 32 rows of a pass
+
+    __device__ __forceinline__ explicit Converter(int warp) {
+        lane = threadIdx.x & 31;
+        u = D == 128 ? (lane & 3) | ((lane >> 4) << 2) : lane & 3;
+        r0 = warp_rows * warp + (D == 128 ? (lane >> 2) & 3 : lane >> 2);
+        high = warp_rows * warp >= 32;
+    }
+
+    // Lane i < 8 has the cached row of the tile's token 16 i; `valid` tokens exist.
+    __device__ __forceinline__ uint32_t place(const AttentionParams& p, int seq, int head, int64_t t0, int valid) const {
+        uint32_t row = 0;
+        if (lane < 8 && 16 * lane < valid) {
+            const unsigned per_page = (unsigned)p.page_size / 16u;
+            const unsigned gr = (unsigned)(t0 / 16) + lane;
+            const unsigned at = gr / per_page;
+            int page = __ldg(p.page_table + (int64_t)seq * p.table_stride + at);
+            page = page < 0 ? 0 : (page >= p.pages ? p.pages - 1 : page);
+            row = ((uint32_t)page * p.kv_heads + head) * p.page_size + (gr - at * per_page) * 16u;
+        }
+        return row;
+    }
+    __device__ __forceinline__ void load(uint32_t place, int valid, const uint8_t* values, Words& x) const {
+#pragma unroll
+        for (int i = 0; i < passes; ++i) {
+            const int r = r0 + step * i;
+            const uint32_t row = __shfl_sync(kFull, place, r >> 4) + (r & 15);
+#pragma unroll
+            for (int k = 0; k < piece_words; ++k) x[i][k] = 0;
+            if (r < valid)
+                ldg_bytes<4 * piece_words>(values + (uint64_t)row * row_bytes + u * (4 * piece_words), x[i]);
+        }
+    }
+    // Scale bytes of rows lane + 32 i.
+    __device__ __forceinline__ void load_scales(uint32_t place, int valid, const uint8_t* scales, uint32_t (&s)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = lane + 32 * i;
+            const uint32_t row = __shfl_sync(kFull, place, r >> 4) + (r & 15);
+            s[i] = 0;
+            if (r < valid) {
+                if constexpr (D == 128)
+                    s[i] = __ldg(reinterpret_cast<const uint32_t*>(scales) + row);
+                else
+                    s[i] = __ldg(reinterpret_cast<const uint16_t*>(scales) + row);
+            }
+        }
+    }
+    static __device__ __forceinline__ int top_scale(const uint32_t (&s)[4]) {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) m = max(m, (s[i] >> (8 * b)) & 255u);
+        return (int)__reduce_max_sync(kFull, m);
+    }
+    // The tile's references: keys are lifted to 2^kKeyLift below theirs.
+    static __device__ __forceinline__ int key_ref(const uint32_t (&s)[4]) { return max(top_scale(s), 1); }
+    static __device__ __forceinline__ int value_ref(const uint32_t (&s)[4]) {
+        // top - ref in (kKeyLift - kRefStep, kKeyLift]
+        return max(((top_scale(s) - kKeyLift + kRefStep - 1) >> 2) << 2, 1);
+    }
+    // f16 relative to the scale byte `ref` into a SWIZZLE_128B tile image.
+    __device__ __forceinline__ void store(const Words& x, const uint32_t (&s)[4], int ref, uint8_t* tile) const {
+#pragma unroll
+        for (int i = 0; i < passes; ++i) {
+            const int r = r0 + step * i;
+            uint32_t sw;
+            if constexpr (step == 32)
+                sw = __shfl_sync(kFull, s[i], r & 31);
+            else
+                sw = __shfl_sync(kFull, high ? s[2 * i + 1] : s[2 * i], r & 31);
+            const int e = (int)((sw >> (8 * (u >> 1))) & 255u) - ref;
+            uint32_t h[8];
+            convert16<BITS>(x[i], dev::pow2_f16x2(e, e), h);
+            uint8_t* row = tile + (u >> 2) * Smem<D>::half + r * 128;
+            const int chunk = (u & 3) * 2;
+            *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+    }
+    // Zeroes E4M3 NaNs; true if there were any among this thread's.
+    static __device__ __forceinline__ bool take_out_nans(Words& x) {
+        bool any = false;
+        if constexpr (BITS == 8) {
+#pragma unroll
+            for (int i = 0; i < passes; ++i)
+#pragma unroll
+                for (int k = 0; k < piece_words; ++k) {
+                    const uint32_t bad = __vcmpeq4(x[i][k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                    any |= bad != 0;
+                    x[i][k] &= ~bad;
+                }
+        }
+        return any;
+    }
+};
+static_assert(kRefStep == 4, "value_ref rounds to multiples of four");
+
+// Converts the key tiles that some row sees once for all row tiles of a key head.
+// Block x: key tile x % max_tiles of (sequence, head) x / max_tiles; the f16 tiles lie
+// in the workspace as shared memory will hold them.  HBM bounds it: D * bits / 8 + D / 32
+// bytes of a row read, 2 D written.
+template <int D, int BITS>
+__global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionParams p) {
+    using C = Converter<D, BITS>;
+    const int tile = blockIdx.x % p.max_tiles, sh = blockIdx.x / p.max_tiles;
+    const int seq = sh / p.kv_heads, head = sh - seq * p.kv_heads;
+    const dev::SeqView view = dev::seq_view(p, seq);
+    const int64_t rows = (int64_t)view.n * p.group;
+    if (rows == 0 || rows < p.min_rows || rows > p.max_rows) return;
+    int64_t lo, hi;
+    dev::seen_range(p, view, 0, view.n - 1, lo, hi);
+    const int64_t t0 = (int64_t)tile * kKeys;
+    // rows that see nothing still have key tile 0, of zeros where no token exists
+    if (tile != 0 && (t0 >= hi || t0 + kKeys <= lo)) return;
+    const int64_t rest = view.len - t0;
+    const int valid = rest < 0 ? 0 : (rest < kKeys ? (int)rest : kKeys);
+    const C cv(threadIdx.x >> 5);
+    const uint32_t place = cv.place(p, seq, head, t0, valid);
+    uint32_t ks[4], vs[4];
+    typename C::Words kx, vx;
+    cv.load_scales(place, valid, p.k_scales, ks);
+    cv.load_scales(place, valid, p.v_scales, vs);
+    cv.load(place, valid, p.k_values, kx);
+    cv.load(place, valid, p.v_values, vx);
+    const int kref = C::key_ref(ks), vref = C::value_ref(vs);
+    const int nans = __syncthreads_or(C::take_out_nans(vx));
+    cv.store(kx, ks, kref - kKeyLift, p.ready_k + (int64_t)blockIdx.x * Smem<D>::tile);
+    cv.store(vx, vs, vref, p.ready_v + (int64_t)blockIdx.x * Smem<D>::tile);
+    if (threadIdx.x == 0) p.ready_meta[blockIdx.x] = make_int2(kref, vref | (nans ? 1 << 16 : 0));
+}
+
+// Converter warps: every key tile of the CTA's share, rows loaded one tile ahead of
+// their conversion and page numbers two.
+template <int D, int BITS>
+__device__ __forceinline__ bool convert_role(const AttentionParams& p, const Block& b, Cursor c, int warp) {
+    using C = Converter<D, BITS>;
+    const C cv(warp);
+    typename C::Words kx, vx;
+    uint32_t ks[4], vs[4];
+    Cursor ahead = c;
+    int at = 0;  // key tile of `ahead`'s unit
+    bool more = true;
+    struct Place {
+        uint32_t row;
+        int valid;  // tokens that exist; -1: no such tile
+    };
+    auto here = [&]() -> Place {
+        const int64_t t0 = (ahead.w.first + ahead.tile0 + at) * kKeys, rest = ahead.w.view.len - t0;
+        const int valid = rest < 0 ? 0 : (rest < kKeys ? (int)rest : kKeys);
+        return Place{cv.place(p, ahead.w.seq, ahead.w.head, t0, valid), valid};
+    };
+    auto advance = [&]() -> Place {
+        if (more && ++at == ahead.tiles) at = 0, more = ahead.next(p);
+        return more ? here() : Place{0, -1};
+    };
+    Place pl = here();
+    cv.load_scales(pl.row, pl.valid, p.k_scales, ks);
+    cv.load_scales(pl.row, pl.valid, p.v_scales, vs);
+    cv.load(pl.row, pl.valid, p.k_values, kx);
+    cv.load(pl.row, pl.valid, p.v_values, vx);
+    Place then = advance();
+    int stage = 0, meta_at = 0;
+    uint32_t phase = 1;  // the first pass over the stages finds them empty
+    do {
+        const Whole whole = whole_tiles(p, c);
+        for (int t = 0; t < c.tiles; ++t) {
+            const int kref = C::key_ref(ks), vref = C::value_ref(vs);
+            uint32_t vs_now[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vs_now[i] = vs[i];
+
+            if (!b.wait(&b.sh->k_empty[stage], phase)) return false;
+            cv.store(kx, ks, kref - kKeyLift, b.smem + Smem<D>::k + stage * Smem<D>::tile);
+            if (warp == 0 && cv.lane == 0) b.sh->meta[meta_at % kMeta] = make_int2(kref, vref);
+            dev::fence_proxy_async();
+            dev::mbar_arrive(&b.sh->k_full[stage]);
+
+            // the next key tile is on its way while this one's values are converted
+            pl = then;
+            if (pl.valid >= 0) {
+                cv.load_scales(pl.row, pl.valid, p.k_scales, ks);
+                cv.load_scales(pl.row, pl.valid, p.v_scales, vs);
+                cv.load(pl.row, pl.valid, p.k_values, kx);
+                then = advance();
+            }
+            // a NaN belongs to the rows that see it: they get it at the end
+            if (t < whole.from || t >= whole.to)
+                if (C::take_out_nans(vx)) *reinterpret_cast<volatile int*>(&b.sh->nan_unit[c.unit & 3]) = c.unit;
+            if (!b.wait(&b.sh->v_empty[stage], phase)) return false;
+            cv.store(vx, vs_now, vref, b.smem + Smem<D>::v + stage * Smem<D>::tile);
+            dev::fence_proxy_async();
+            dev::mbar_arrive(&b.sh->v_full[stage]);
+            if (pl.valid >= 0) cv.load(pl.row, pl.valid, p.v_values, vx);
+
+            ++meta_at;
+            if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+    } while (c.next(p));
+    return true;
+}
+
+// Index of a key tile among the converted ones.
+__device__ __forceinline__ int64_t ready_at(const AttentionParams& p, const Cursor& c) {
+    return ((int64_t)c.w.seq * p.kv_heads + c.w.head) * p.max_tiles + c.w.first + c.tile0;
+}
+
+// One warp copying ready-made tiles (its elected lane).
+template <int D>
+__device__ __forceinline__ void load_role(const AttentionParams& p, const Block& b, Cursor c) {
+    constexpr int bytes = Smem<D>::tile;
+    int stage = 0, issued = 0;
+    uint32_t phase = 1;
+    bool ok = true, values = true;  // values: the last tile's were issued as well
+    do {
+        const int64_t at = ready_at(p, c);
+        for (int t = 0; t < c.tiles && ok; ++t) {
+            ok = b.wait_lean(&b.sh->k_empty[stage], phase);
+            if (!ok) break;
+            if (dev::elect_one()) {
+                dev::mbar_arrive_expect_tx(&b.sh->k_full[stage], bytes);
+                dev::bulk_load(b.smem + Smem<D>::k + stage * bytes, p.ready_k + (at + t) * bytes, bytes, &b.sh->k_full[stage]);
+            }
+            __syncwarp();
+            values = ok = b.wait_lean(&b.sh->v_empty[stage], phase);
+            if (ok && dev::elect_one()) {
+                dev::mbar_arrive_expect_tx(&b.sh->v_full[stage], bytes);
+                dev::bulk_load(b.smem + Smem<D>::v + stage * bytes, p.ready_v + (at + t) * bytes, bytes, &b.sh->v_full[stage]);
+            }
+            __syncwarp();
+            ++issued;
+            if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+    } while (ok && c.next(p));
+    // Copies in flight must land before the CTA's memory goes: the last tile of each stage.
+    for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
+        const uint32_t parity = (uint32_t)(i / kStages) & 1u;
+        const long long start = clock64();
+        while (!(dev::mbar_try_wait(&b.sh->k_full[i % kStages], parity) &&
+                 ((i == issued - 1 && !values) || dev::mbar_try_wait(&b.sh->v_full[i % kStages], parity))))
+            if (clock64() - start > dev::kWaitLimitCycles) break;
+    }
+}
+
+// --------------------------------------------------------------------------- products
+
+template <int D>
+__device__ __forceinline__ void product_role(const AttentionParams& p, const Block& b, Cursor c) {
     using L = Smem<D>;
-    constexpr int kRowBytes = D * BITS / 8;
-    constexpr int kUnits = D / 16;      // 16-element pieces of a row; a converter thread has as many of a tile
-    constexpr int kUnitBytes = 2 * BITS;
-    constexpr int kScales = D / 32;     // scale bytes of a row
-    constexpr uint32_t kO = 2 * kKeys;  // first TMEM column of the outputs
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ __align__(8) Bars bars;
-    __shared__ int64_t scratch[kThreads / 32 + 2];
-    __shared__ uint32_t tmem_slot;
-    __shared__ int abort_word;
-    __shared__ int2 meta[kMeta];        // per key tile: the keys' and the values' reference scales
-    __shared__ int nan_unit[4];         // unit whose values had a NaN taken out of a partly seen tile
-    volatile int* abort_flag = &abort_word;
+    constexpr uint32_t idesc_s = dev::f16_idesc(kTileRows, kKeys, false);
+    constexpr uint32_t idesc_o = dev::f16_idesc(kTileRows, D, true);
+    // The whole warp walks, one elected lane issues: descriptors and addresses stay
+    // warp-uniform and are advanced by constants.
+    const uint32_t base = dev::smem_addr(b.smem);
+    const uint64_t q_desc = dev::smem_desc(base + L::q, 16, 1024, dev::kLayoutSwizzle128);
+    const uint64_t k_desc = dev::smem_desc(base + L::k, 16, 1024, dev::kLayoutSwizzle128);
+    const uint64_t v_desc = dev::smem_desc(base + L::v, L::half, 1024, dev::kLayoutSwizzle128);
+    Shared* sh = b.sh;
+    bool ok = true;
+    uint32_t k_stage = 0, v_stage = 0, k_phase = 0, v_phase = 0, p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
+    do {
+        const int nw = __shfl_sync(kFull, c.rows(p) > kTileRows ? 2 : 1, 0);
+        const int tiles = __shfl_sync(kFull, c.tiles, 0);
+        for (int t = 0; t <= tiles && ok; ++t) {
+            // weighted values of key tile t - 1, scores of key tile t
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                if (w >= nw || !ok) continue;
+                if (t > 0) {
+                    if (w == 0) ok = b.wait_lean(&sh->v_full[v_stage], v_phase);
+                    if (ok) ok = b.wait_lean(&sh->p_ready[w], p_phase[w]);
+                    p_phase[w] ^= 1;
+                    dev::tc_fence_after();
+                    const uint64_t vd = v_desc + (uint64_t)(v_stage * (L::tile >> 4));
+                    if (ok && dev::elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < kKeys / 16; ++i)
+                            dev::tc_mma_f16_ta(b.tmem + 2 * kKeys + w * D, b.tmem + w * kKeys + 8 * i,
+                                               vd + i * (2048 >> 4), idesc_o, i > 0 || t > 1);
+                        dev::tc_commit(&sh->o_done[w]);
+                        if (w == nw - 1) dev::tc_commit(&sh->v_empty[v_stage]);
+                    }
+                    __syncwarp();
+                }
+                if (t < tiles && ok) {
+                    if (w == 0) ok = b.wait_lean(&sh->k_full[k_stage], k_phase);
+                    if (ok && t == 0) ok = b.wait_lean(&sh->q_ready[w], q_phase[w]), q_phase[w] ^= 1;
+                    dev::tc_fence_after();
+                    const uint64_t kd = k_desc + (uint64_t)(k_stage * (L::tile >> 4));
+                    const uint64_t qd = q_desc + (uint64_t)(w * (L::tile >> 4));
+                    if (ok && dev::elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            const uint32_t at = ((i / 4) * L::half + (i % 4) * 32) >> 4;
+                            dev::tc_mma_f16(b.tmem + w * kKeys, qd + at, kd + at, idesc_s, i > 0);
+                        }
+                        dev::tc_commit(&sh->s_full[w]);
+                        if (w == nw - 1) dev::tc_commit(&sh->k_empty[k_stage]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (t > 0 && ++v_stage == kStages) v_stage = 0, v_phase ^= 1;
+            if (t < tiles && ++k_stage == kStages) k_stage = 0, k_phase ^= 1;
+        }
+    } while (ok && c.next(p));
+    // Products in flight must not outlive the CTA's memory.
+    if (dev::elect_one()) {
+        dev::tc_commit(&sh->drain);
+        const long long start = clock64();
+        while (!dev::mbar_try_wait(&sh->drain, 0))
+            if (clock64() - start > dev::kWaitLimitCycles) break;
+    }
+    __syncwarp();
+}
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// ---------------------------------------------------------------------------- softmax
 
-    const dev::Share share = dev::take_share<kRows, kKeys, kThreads>(p, scratch);
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Columns of a key tile that a row sees, [from, to).
+struct Columns {
+    int from, to;
+};
+
+// Folds 32 scores (columns `at` ..) into the running maxima m; MASKED: those seen only.
+template <bool MASKED>
+__device__ __forceinline__ void fold_top(const uint32_t (&s)[32], int at, Columns c, float (&m)[4]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        float a = __uint_as_float(s[i]), b = __uint_as_float(s[i + 1]);
+        if constexpr (MASKED) {
+            const float neg_inf = __int_as_float(0xff800000);
+            a = at + i < c.from || at + i >= c.to ? neg_inf : a;
+            b = at + i + 1 < c.from || at + i + 1 >= c.to ? neg_inf : b;
+        }
+        m[(i / 2) & 3] = max3f(m[(i / 2) & 3], a, b);
+    }
+}
+
+// Weights 2^(score * f - base) of 32 scores, added to sum, to f16 pairs.  GENERAL: those
+// seen only, and the f16 ones scaled by `down`.
+template <bool GENERAL>
+__device__ __forceinline__ void fold_weights(const uint32_t (&s)[32], int at, Columns c, float f, float base, float down,
+                                             float2 (&sum)[2], uint32_t (&pw)[16]) {
+    const float2 f2 = make_float2(f, f), b2 = make_float2(-base, -base);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        float2 t = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, b2);
+        t.x = ex2(t.x), t.y = ex2(t.y);
+        if constexpr (GENERAL) {
+            if (at + i < c.from || at + i >= c.to) t.x = 0.0f;
+            if (at + i + 1 < c.from || at + i + 1 >= c.to) t.y = 0.0f;
+        }
+        sum[(i / 2) & 1] = __fadd2_rn(sum[(i / 2) & 1], t);
+        if constexpr (GENERAL) t.x *= down, t.y *= down;
+        const __half2 u = __float22half2_rn(t);
+        pw[i / 2] = *reinterpret_cast<const uint32_t*>(&u);
+    }
+}
+
+// Features of a value row that are NaN (8-bit elements) among the tokens [k0, k1) that
+// a row sees, as bits.
+template <int D>
+__device__ __noinline__ uint4 nan_features(const uint8_t* values, const int* table, int page_size, int pages,
+                                           int kv_heads, int head, int64_t k0, int64_t k1) {
+    uint32_t bad[4] = {0, 0, 0, 0};
+    for (int64_t k = k0; k < k1; ++k) {
+        int page = __ldg(table + k / page_size);
+        page = page < 0 ? 0 : (page >= pages ? pages - 1 : page);
+        const uint32_t* v = reinterpret_cast<const uint32_t*>(
+            values + (((int64_t)page * kv_heads + head) * page_size + k % page_size) * D);
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) {
+            const uint32_t b = __vcmpeq4(__ldg(v + i) & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            const uint32_t bits = (b & 1u) | ((b >> 7) & 2u) | ((b >> 14) & 4u) | ((b >> 21) & 8u);
+            bad[i / 8] |= bits << (4 * (i % 8));
+        }
+    }
+    return make_uint4(bad[0], bad[1], bad[2], bad[3]);
+}
+
+// This row's query into shared memory, scaled by a power of two to a largest magnitude in
+// [2^12, 2^13); a negative scale of the scores goes into its sign.  Returns the factor
+// that makes scores of its products with lifted keys, less the keys' reference.
+template <int D>
+__device__ __forceinline__ float put_query(const AttentionParams& p, int64_t at, bool real, uint8_t* dst, int r) {
+    const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
+    uint32_t x[D / 2];
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) {
+        x[2 * i] = x[2 * i + 1] = 0;
+        if (real) {
+            if (p.q_vec) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(q) + i);
+                x[2 * i] = v.x, x[2 * i + 1] = v.y;
+            } else {
+                x[2 * i] = q[4 * i] | ((uint32_t)q[4 * i + 1] << 16);
+                x[2 * i + 1] = q[4 * i + 2] | ((uint32_t)q[4 * i + 3] << 16);
+            }
+        }
+    }
+    const bool f16 = p.dtype == MXK_F16;
+    auto pair = [&](uint32_t v) -> float2 {
+        if (f16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    };
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 2; ++i) {
+        const float2 v = pair(x[i]);
+        amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+    }
+    int e = amax > 0.0f ? (int)(__float_as_uint(amax) >> 23) - 127 : 0;
+    e = max(e, -126);
+    const int down = (kQueryExp - e) / 2, rest = kQueryExp - e - down;
+    const float f0 = __uint_as_float((uint32_t)(down + 127) << 23);
+    const float f1 = copysignf(__uint_as_float((uint32_t)(rest + 127) << 23), p.scale_log2);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 v = pair(x[4 * i + k]);
+            const __half2 u = __floats2half2_rn(v.x * f0 * f1, v.y * f0 * f1);
+            h[k] = *reinterpret_cast<const uint32_t*>(&u);
+        }
+        *reinterpret_cast<uint4*>(dst + (i / 8) * Smem<D>::half + (((i % 8) ^ (r & 7)) << 4)) =
+            make_uint4(h[0], h[1], h[2], h[3]);
+    }
+    return fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 - down - kKeyLift / 2) << 23) *
+           __uint_as_float((uint32_t)(127 - rest - kKeyLift / 2) << 23);
+}
+
+// HOLD: a row's scores stay in registers (ready-made tiles), else they are read twice.
+template <int D, bool HOLD>
+__device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Block& b, Cursor c, int warp) {
+    using L = Smem<D>;
+    Shared* sh = b.sh;
+    const int w = warp >> 2;                                    // row tile
+    const int r = threadIdx.x & (kTileRows - 1);                // row in the tile
+    const uint32_t lane_base = b.tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    const uint32_t s_col = lane_base + w * kKeys, o_col = lane_base + 2 * kKeys + w * D;
+    const float neg_inf = __int_as_float(0xff800000);
+    uint32_t s_phase = 0, o_phase = 0;
+    int meta_at = 0;
+    bool open = false, went_on = false, ended = false;
+    do {
+        const int rows = c.rows(p);
+        if (w * kTileRows < rows) {
+            const bool real = w * kTileRows + r < rows;
+            const bool warp_real = w * kTileRows + (r & ~31) < rows;
+            const int row = c.w.rt * kRows + w * kTileRows + r;
+            const int j = row / p.group, head = c.w.head * p.group + (row - j * p.group);
+            const Whole whole = whole_tiles(p, c);
+            int64_t lo = 0, hi = c.w.view.len;
+            if (real) dev::seen_range(p, c.w.view, j, j, lo, hi);
+            const int64_t first_key = (c.w.first + c.tile0) * kKeys;
+            const float row_factor =
+                put_query<D>(p, (int64_t)(c.w.view.row0 + j) * p.q_token + (int64_t)head * p.q_head, real,
+                             b.smem + L::q + w * L::tile + r * 128, r);
+            dev::fence_proxy_async();
+            dev::mbar_arrive(&sh->q_ready[w]);
+
+            float run_max = neg_inf, base = -kExpShift, sum = 0.0f;
+            int vrun = 0;  // the output is held relative to 2^(vrun - 127)
+            bool nans = false;
+            const int2* meta = HOLD ? p.ready_meta + ready_at(p, c) : nullptr;
+            int2 ref = HOLD ? __ldg(meta) : make_int2(0, 0);
+            for (int t = 0; t < c.tiles; ++t) {
+                if (!b.wait(&sh->s_full[w], s_phase)) return false;
+                s_phase ^= 1;
+                dev::tc_fence_after();
+                if constexpr (!HOLD) ref = *const_cast<const int2*>(&sh->meta[(meta_at + t) % kMeta]);
+                if (warp_real) {
+                    const float f = row_factor * __uint_as_float((uint32_t)ref.x << 23);
+                    const int vref = ref.y & 0xffff;
+                    if constexpr (HOLD) {
+                        nans |= ref.y >> 16;
+                        if (t + 1 < c.tiles) ref = __ldg(meta + t + 1);
+                    }
+                    const bool partly = t < whole.from || t >= whole.to;
+                    Columns cols{0, kKeys};
+                    if (partly) {
+                        const int64_t t0 = first_key + (int64_t)t * kKeys;
+                        cols.from = lo > t0 ? (lo - t0 < kKeys ? (int)(lo - t0) : kKeys) : 0;
+                        cols.to = hi < t0 ? 0 : (hi - t0 < kKeys ? (int)(hi - t0) : kKeys);
+                    }
+                    // the largest score
+                    uint32_t s[HOLD ? 4 : 2][32];
+                    float m4[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
+                    if constexpr (HOLD) {
+#pragma unroll
+                        for (int h = 0; h < kKeys / 32; ++h) dev::tmem_ld_32x32b_x32(s_col + 32 * h, s[h]);
+                        dev::tmem_wait_ld();
+                        if (partly) {
+#pragma unroll
+                            for (int h = 0; h < kKeys / 32; ++h) fold_top<true>(s[h], 32 * h, cols, m4);
+                        } else {
+#pragma unroll
+                            for (int h = 0; h < kKeys / 32; ++h) fold_top<false>(s[h], 32 * h, cols, m4);
+                        }
+                    } else {
+                        auto tops = [&](auto masked) {
+                            dev::tmem_ld_32x32b_x32(s_col, s[0]);
+#pragma unroll
+                            for (int h = 0; h < kKeys / 32; ++h) {
+                                dev::tmem_wait_ld();
+                                if (h + 1 < kKeys / 32) dev::tmem_ld_32x32b_x32(s_col + 32 * (h + 1), s[(h + 1) & 1]);
+                                fold_top<decltype(masked)::value>(s[h & 1], 32 * h, cols, m4);
+                            }
+                        };
+                        if (partly)
+                            tops(std::true_type{});
+                        else
+                            tops(std::false_type{});
+                    }
+                    float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    if (top != neg_inf) top *= f;
+
+                    // Raise the row's maximum, or the reference of the output, if need be.
+                    const bool raise = top > run_max + kMaxSlack;
+                    const bool shift = vref > vrun;
+                    if (__any_sync(kFull, raise) || shift) {
+                        const float m = raise ? top : run_max;
+                        float g = m == run_max ? 1.0f : ex2(run_max - m);
+                        run_max = m;
+                        base = (m == neg_inf ? 0.0f : m) - kExpShift;
+                        sum *= g;
+                        if (t > 0) {  // the output so far, once the products before have finished
+                            if (shift) g *= __uint_as_float((uint32_t)max(vrun - vref + 127, 0) << 23);
+                            if (!b.wait(&sh->o_done[w], o_phase ^ 1)) return false;
+                            dev::tc_fence_after();
+#pragma unroll
+                            for (int h = 0; h < D / 32; ++h) {
+                                uint32_t o[32];
+                                dev::tmem_ld_32x32b_x32(o_col + 32 * h, o);
+                                dev::tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
+                                dev::tmem_st_32x32b_x32(o_col + 32 * h, o);
+                            }
+                        }
+                        if (shift) vrun = vref;
+                    }
+                    // the weights, over the scores they come from
+                    const float down = __uint_as_float((uint32_t)max(vref - vrun + 127, 0) << 23);
+                    float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                    auto weights = [&](auto general) {
+                        constexpr bool kGeneral = decltype(general)::value;
+                        if constexpr (!HOLD) dev::tmem_ld_32x32b_x32(s_col, s[0]);
+#pragma unroll
+                        for (int h = 0; h < kKeys / 32; ++h) {
+                            uint32_t pw[16];
+                            if constexpr (!HOLD) {
+                                dev::tmem_wait_ld();
+                                if (h + 1 < kKeys / 32) dev::tmem_ld_32x32b_x32(s_col + 32 * (h + 1), s[(h + 1) & 1]);
+                            }
+                            fold_weights<kGeneral>(s[HOLD ? h : h & 1], 32 * h, cols, f, base, down, part, pw);
+                            dev::tmem_st_32x32b_x16(s_col + 16 * h, pw);
+                        }
+                    };
+                    if (partly || vref != vrun)
+                        weights(std::true_type{});
+                    else
+                        weights(std::false_type{});
+                    dev::tmem_wait_st();
+                    sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+                }
+                dev::tc_fence_before();
+                dev::mbar_arrive(&sh->p_ready[w]);
+                o_phase ^= 1;
+            }
+
+            // The output row.
+            if (!b.wait(&sh->o_done[w], o_phase ^ 1)) return false;
+            dev::tc_fence_after();
+            if (warp_real) {
+                const bool all = c.whole();
+                // NaNs that were taken out of the values, for the rows that see them
+                uint32_t bad[4] = {0, 0, 0, 0};
+                if constexpr (!HOLD) nans = *reinterpret_cast<volatile int*>(&sh->nan_unit[c.unit & 3]) == c.unit;
+                if (nans && real) {
+                    const int64_t end = first_key + (int64_t)c.tiles * kKeys;
+                    const uint4 f = nan_features<D>(p.v_values, p.page_table + (int64_t)c.w.seq * p.table_stride,
+                                                    p.page_size, p.pages, p.kv_heads, c.w.head,
+                                                    lo > first_key ? lo : first_key, hi < end ? hi : end);
+                    bad[0] = f.x, bad[1] = f.y, bad[2] = f.z, bad[3] = f.w;
+                }
+                const float vfactor = __uint_as_float((uint32_t)vrun << 23);
+                const float inv = all ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+                const int64_t slot = 2 * (int64_t)blockIdx.x + (c.tile0 == 0 ? 1 : 0);
+                const int tile_row = w * kTileRows + r;
+#pragma unroll
+                for (int h = 0; h < D / 32; ++h) {
+                    uint32_t o[32];
+                    dev::tmem_ld_32x32b_x32(o_col + 32 * h, o);
+                    dev::tmem_wait_ld();
+                    if (real) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            float v = __uint_as_float(o[i]) * inv * vfactor;
+                            if (sum == 0.0f) v = 0.0f;
+                            if (bad[h] >> i & 1u) v = __int_as_float(0x7fc00000);
+                            o[i] = __float_as_uint(v);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 v = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
+                                                         __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                            if (all)
+                                dev::store4(p, c.w.view.row0 + j, head, 32 * h + i, v);
+                            else
+                                *reinterpret_cast<float4*>(p.part + (slot * kRows + tile_row) * D + 32 * h + i) = v;
+                        }
+                    }
+                }
+                if (real) {
+                    if (!all)
+                        p.part_stat[slot * kRows + tile_row] = make_float2(run_max, sum);
+                    else if (p.lse)
+                        p.lse[(int64_t)(c.w.view.row0 + j) * p.heads + head] = dev::row_lse(run_max, sum);
+                }
+            }
+            dev::tc_fence_before();
+        }
+        meta_at += c.tiles;
+        if (!c.whole()) {
+            if (c.tile0 == 0) {
+                open = true;
+                if (threadIdx.x == 0) p.part_open[blockIdx.x] = make_int4(c.w.seq, c.w.rt, c.w.head, 1);
+            } else {
+                went_on = true;
+                ended = c.tile0 + c.tiles == c.w.tiles;
+            }
+        }
+    } while (c.next(p));
+    if (threadIdx.x == 0) {
+        if (!open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
+        p.part_ends[blockIdx.x] = went_on && ended ? 1 : 0;
+    }
+    return true;
+}
+
+// ---------------------------------------------------------------------------- kernels
+
+// Barriers, TMEM and the cursor; false: the CTA has no share.
+template <int D, class Cfg, int FULL_COUNT>
+__device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_raw, Shared* sh, int64_t* scratch,
+                                      unsigned* err, Block& b, Cursor& c) {
+    const int tid = threadIdx.x;
+    const dev::Share share = dev::take_share<kRows, kKeys, Cfg::threads>(p, scratch);
     if (share.tiles == 0) {
         if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0), p.part_ends[blockIdx.x] = 0;
-        return;
+        return false;
     }
     if (tid == 0) {
-        abort_word = 0;
+        sh->abort_word = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            dev::mbar_init(&bars.q_ready[i], kTileRows);
-            dev::mbar_init(&bars.s_full[i], 1);
-            dev::mbar_init(&bars.p_ready[i], kTileRows);
-            dev::mbar_init(&bars.o_done[i], 1);
+            dev::mbar_init(&sh->q_ready[i], kTileRows);
+            dev::mbar_init(&sh->s_full[i], 1);
+            dev::mbar_init(&sh->p_ready[i], kTileRows);
+            dev::mbar_init(&sh->o_done[i], 1);
         }
 #pragma unroll
         for (int i = 0; i < kStages; ++i) {
-            dev::mbar_init(&bars.k_full[i], 32 * kConvertWarps);
-            dev::mbar_init(&bars.v_full[i], 32 * kConvertWarps);
-            dev::mbar_init(&bars.k_empty[i], 1);
-            dev::mbar_init(&bars.v_empty[i], 1);
+            dev::mbar_init(&sh->k_full[i], FULL_COUNT);
+            dev::mbar_init(&sh->v_full[i], FULL_COUNT);
+            dev::mbar_init(&sh->k_empty[i], 1);
+            dev::mbar_init(&sh->v_empty[i], 1);
         }
-        dev::mbar_init(&bars.drain, 1);
+        dev::mbar_init(&sh->drain, 1);
         dev::fence_barrier_init();
     }
-    if (tid < 4) nan_unit[tid] = -1;
-    if (warp == 0) dev::tmem_alloc(&tmem_slot, 512);
+    if (tid < 4) sh->nan_unit[tid] = -1;
+    if (tid < 32) dev::tmem_alloc(&sh->tmem, 512);
     dev::tc_fence_before();
     __syncthreads();
     dev::tc_fence_after();
-    const uint32_t tmem = tmem_slot;
-
-    Cursor c;
+    b.smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    b.sh = sh;
+    b.tmem = __shfl_sync(kFull, sh->tmem, 0);
+    b.err = err;
     c.w = dev::walk_to<kRows, kKeys>(p, share.seq, share.offset);
     c.left = share.tiles;
     c.unit = 0;
     c.take();
+    return true;
+}
 
-    // Every wait is bounded; a wait that gives up raises the CTA's abort flag and the
-    // roles leave for the end, warp by warp.
-#define MXK_WAIT(bar, parity)                                                                  \
-    do {                                                                                       \
-        const bool ok_ = dev::mbar_wait((bar), (parity), abort_flag, err);                     \
-        if (!__all_sync(kFull, ok_)) goto done;                                                \
-    } while (0)
-
-    if (warp < kSoftmaxWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        // ------------------------------------------------------------ softmax
-        const int w = warp >> 2;                        // row tile
-        const int r = tid & (kTileRows - 1);            // row in the tile
-        const uint32_t lane_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const uint32_t s_col = lane_base + w * kKeys, o_col = lane_base + kO + w * D;
-        const float neg_inf = __int_as_float(0xff800000);
-        uint32_t s_phase = 0, o_phase = 0;
-        int meta_at = 0;
-        bool open = false, went_on = false, ended = false;
-        do {
-            const int rows = c.rows(p);
-            if (w * kTileRows < rows) {
-                const bool real = w * kTileRows + r < rows;
-                const bool warp_real = w * kTileRows + (r & ~31) < rows;
-                const int row = c.w.rt * kRows + w * kTileRows + r;
-                const int j = row / p.group, head = c.w.head * p.group + (row - j * p.group);
-                const UnitRange range = unit_range(p, c);
-                int64_t lo = 0, hi = c.w.view.len;
-                if (real) dev::seen_range(p, c.w.view, j, j, lo, hi);
-
-                // This row's query into shared memory, scaled by a power of two to a largest
-                // magnitude in [2^12, 2^13); a negative scale of the scores goes into its sign.
-                float row_factor;
-                {
-                    const int64_t at = (int64_t)(c.w.view.row0 + j) * p.q_token + (int64_t)head * p.q_head;
-                    const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
-                    uint32_t x[D / 2];
-#pragma unroll
-                    for (int i = 0; i < D / 4; ++i) {
-                        x[2 * i] = x[2 * i + 1] = 0;
-                        if (real) {
-                            if (p.q_vec) {
-                                const uint2 v = __ldg(reinterpret_cast<const uint2*>(q) + i);
-                                x[2 * i] = v.x, x[2 * i + 1] = v.y;
-                            } else {
-                                x[2 * i] = q[4 * i] | ((uint32_t)q[4 * i + 1] << 16);
-                                x[2 * i + 1] = q[4 * i + 2] | ((uint32_t)q[4 * i + 3] << 16);
-                            }
-                        }
-                    }
-                    const bool f16 = p.dtype == MXK_F16;
-                    auto pair = [&](uint32_t v) -> float2 {
-                        if (f16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-                        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-                    };
-                    float amax = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < D / 2; ++i) {
-                        const float2 v = pair(x[i]);
-                        amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
-                    }
-                    int e = amax > 0.0f ? (int)(__float_as_uint(amax) >> 23) - 127 : 0;
-                    e = max(e, -126);
-                    const int down = (kQueryExp - e) / 2, rest = kQueryExp - e - down;
-                    const float f0 = __uint_as_float((uint32_t)(down + 127) << 23);
-                    const float f1 = copysignf(__uint_as_float((uint32_t)(rest + 127) << 23), p.scale_log2);
-                    row_factor = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 - down - kKeyLift / 2) << 23) *
-                                 __uint_as_float((uint32_t)(127 - rest - kKeyLift / 2) << 23);
-                    uint8_t* dst = smem + L::q + w * L::tile + r * 128;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        uint32_t h[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float2 v = pair(x[4 * i + k]);
-                            const __half2 u = __floats2half2_rn(v.x * f0 * f1, v.y * f0 * f1);
-                            h[k] = *reinterpret_cast<const uint32_t*>(&u);
-                        }
-                        *reinterpret_cast<uint4*>(dst + (i / 8) * L::half + (((i % 8) ^ (r & 7)) << 4)) =
-                            make_uint4(h[0], h[1], h[2], h[3]);
-                    }
-                }
-                dev::fence_proxy_async();
-                dev::mbar_arrive(&bars.q_ready[w]);
-
-                float run_max = neg_inf, base = -kExpShift, sum = 0.0f;
-                int vref = 0;
-                for (int t = 0; t < c.tiles; ++t) {
-                    MXK_WAIT(&bars.s_full[w], s_phase);
-                    s_phase ^= 1;
-                    dev::tc_fence_after();
-                    const int2 ref = lds_int2(dev::smem_addr(&meta[(meta_at + t) % kMeta]));
-                    if (warp_real) {
-                        const float f = row_factor * __uint_as_float((uint32_t)ref.x << 23);
-                        const int64_t t0 = (c.w.first + c.tile0 + t) * kKeys;
-                        const bool partly = t0 < range.all_lo || t0 + kKeys > range.all_hi;
-                        int from = 0, to = kKeys;  // columns that take part
-                        if (partly) {
-                            from = lo > t0 ? (lo - t0 < kKeys ? (int)(lo - t0) : kKeys) : 0;
-                            to = hi < t0 ? 0 : (hi - t0 < kKeys ? (int)(hi - t0) : kKeys);
-                        }
-                        // the largest score
-                        float top = neg_inf;
-#pragma unroll
-                        for (int h = 0; h < kKeys / 32; ++h) {
-                            uint32_t s[32];
-                            dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
-                            dev::tmem_wait_ld();
-                            if (partly) {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    if (32 * h + i < from || 32 * h + i >= to) s[i] = 0xff800000u;
-                            }
-                            float m[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) m[i & 3] = fmaxf(m[i & 3], __uint_as_float(s[i]));
-                            top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
-                        }
-                        if (top != neg_inf) top *= f;
-                        const bool raise = top > run_max + kMaxSlack;
-                        const bool shift = ref.y != vref;
-                        if (__any_sync(kFull, raise) || shift) {
-                            const float m = raise ? top : run_max;
-                            float g = m == run_max ? 1.0f : ex2(run_max - m);
-                            run_max = m;
-                            base = (m == neg_inf ? 0.0f : m) - kExpShift;
-                            sum *= g;
-                            if (t > 0) {  // the output so far, once the products before have finished
-                                if (shift) g *= __uint_as_float((uint32_t)max(vref - ref.y + 127, 0) << 23);
-                                MXK_WAIT(&bars.o_done[w], o_phase ^ 1);
-                                dev::tc_fence_after();
-#pragma unroll
-                                for (int h = 0; h < D / 32; ++h) {
-                                    uint32_t o[32];
-                                    dev::tmem_ld_32x32b_x32(o_col + 32 * h, o);
-                                    dev::tmem_wait_ld();
-#pragma unroll
-                                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
-                                    dev::tmem_st_32x32b_x32(o_col + 32 * h, o);
-                                }
-                                dev::tmem_wait_st();
-                            }
-                            vref = ref.y;
-                        }
-                        // the weights, over the scores they come from
-                        float part[2] = {0.0f, 0.0f};
-#pragma unroll
-                        for (int h = 0; h < kKeys / 32; ++h) {
-                            uint32_t s[32];
-                            dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
-                            dev::tmem_wait_ld();
-                            uint32_t pw[16];
-#pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                float a = ex2(fmaf(__uint_as_float(s[i]), f, -base));
-                                float b = ex2(fmaf(__uint_as_float(s[i + 1]), f, -base));
-                                if (partly) {
-                                    if (32 * h + i < from || 32 * h + i >= to) a = 0.0f;
-                                    if (32 * h + i + 1 < from || 32 * h + i + 1 >= to) b = 0.0f;
-                                }
-                                part[0] += a, part[1] += b;
-                                const __half2 u = __floats2half2_rn(a, b);
-                                pw[i / 2] = *reinterpret_cast<const uint32_t*>(&u);
-                            }
-                            dev::tmem_st_32x32b_x16(s_col + 16 * h, pw);
-                        }
-                        dev::tmem_wait_st();
-                        sum += part[0] + part[1];
-                    }
-                    dev::tc_fence_before();
-                    dev::mbar_arrive(&bars.p_ready[w]);
-                    o_phase ^= 1;
-                }
-                meta_at += c.tiles;
-
-                // The output row.
-                MXK_WAIT(&bars.o_done[w], o_phase ^ 1);
-                dev::tc_fence_after();
-                if (warp_real) {
-                    const bool whole = c.tile0 == 0 && c.tiles == c.w.tiles;
-                    // NaNs that were taken out of the values, for the rows that see them
-                    uint32_t bad[D / 32] = {};
-                    if constexpr (BITS == 8) {
-                        if (*reinterpret_cast<volatile int*>(&nan_unit[c.unit & 3]) == c.unit && real) {
-                            for (int t = 0; t < c.tiles; ++t) {
-                                const int64_t t0 = (c.w.first + c.tile0 + t) * kKeys;
-                                if (!(t0 < range.all_lo || t0 + kKeys > range.all_hi)) continue;
-                                for (int64_t k = t0 > lo ? t0 : lo; k < hi && k < t0 + kKeys; ++k) {
-                                    int page = __ldg(p.page_table + (int64_t)c.w.seq * p.table_stride + k / p.page_size);
-                                    page = page < 0 ? 0 : (page >= p.pages ? p.pages - 1 : page);
-                                    const uint8_t* v = p.v_values + (((int64_t)page * p.kv_heads + c.w.head) * p.page_size +
-                                                                     k % p.page_size) * kRowBytes;
-#pragma unroll 1
-                                    for (int i = 0; i < D; ++i)
-                                        if ((v[i] & 0x7fu) == 0x7fu) {
-#pragma unroll
-                                            for (int b = 0; b < D / 32; ++b)
-                                                if (b == i / 32) bad[b] |= 1u << (i & 31);
-                                        }
-                                }
-                            }
-                        }
-                    }
-                    const float vfactor = __uint_as_float((uint32_t)vref << 23);
-                    const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
-                    const int64_t slot = 2 * (int64_t)blockIdx.x + (c.tile0 == 0 ? 1 : 0);
-                    const int tile_row = w * kTileRows + r;
-#pragma unroll
-                    for (int h = 0; h < D / 32; ++h) {
-                        uint32_t o[32];
-                        dev::tmem_ld_32x32b_x32(o_col + 32 * h, o);
-                        dev::tmem_wait_ld();
-                        if (real) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                float v = __uint_as_float(o[i]) * inv * vfactor;
-                                if (sum == 0.0f) v = 0.0f;
-                                if (BITS == 8 && (bad[h] >> i & 1u)) v = __int_as_float(0x7fc00000);
-                                o[i] = __float_as_uint(v);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 32; i += 4) {
-                                const float4 v = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
-                                                             __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-                                if (whole)
-                                    dev::store4(p, c.w.view.row0 + j, head, 32 * h + i, v);
-                                else
-                                    *reinterpret_cast<float4*>(p.part + (slot * kRows + tile_row) * D + 32 * h + i) = v;
-                            }
-                        }
-                    }
-                    if (real) {
-                        if (!whole)
-                            p.part_stat[slot * kRows + tile_row] = make_float2(run_max, sum);
-                        else if (p.lse)
-                            p.lse[(int64_t)(c.w.view.row0 + j) * p.heads + head] = dev::row_lse(run_max, sum);
-                    }
-                }
-                dev::tc_fence_before();
-            } else {
-                meta_at += c.tiles;
-            }
-            if (!(c.tile0 == 0 && c.tiles == c.w.tiles)) {
-                if (c.tile0 == 0) {
-                    open = true;
-                    if (tid == 0) p.part_open[blockIdx.x] = make_int4(c.w.seq, c.w.rt, c.w.head, 1);
-                } else {
-                    went_on = true;
-                    ended = c.tile0 + c.tiles == c.w.tiles;
-                }
-            }
-        } while (c.next(p));
-        if (tid == 0) {
-            if (!open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
-            p.part_ends[blockIdx.x] = went_on && ended ? 1 : 0;
-        }
-    } else if (warp < kSoftmaxWarps + kConvertWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
-        // --------------------------------------------------------- converters
-        // A thread converts piece u of kUnits rows: eight neighbouring lanes cover the
-        // 16-byte chunks of two rows, so the swizzled stores meet no bank twice.
-        const int cw = warp - kSoftmaxWarps;
-        const int u = D == 128 ? (lane & 3) | ((lane >> 4) << 2) : lane & 3;
-        const int r0 = D == 128 ? 4 * cw + ((lane >> 2) & 3) : 8 * cw + (lane >> 2);  // and every kStep-th row
-        constexpr int kStep = kKeys / kUnits;
-        const unsigned per_page = (unsigned)p.page_size / 16u;
-
-        uint32_t kx[kUnits][kUnitBytes / 4], vx[kUnits][kUnitBytes / 4];
-        uint32_t ks[4], vs[4];  // scale bytes of rows lane + 32 i
-
-        // Where the key tile `t` of the cursor's unit lies: lane i < 8 has granule i's first row.
-        struct Place {
-            uint32_t row;
-            int valid;
-        };
-        auto place = [&](const Cursor& at, int t) -> Place {
-            Place pl{0, 0};
-            const int64_t t0 = (at.w.first + at.tile0 + t) * kKeys;
-            const int64_t rest = at.w.view.len - t0;
-            pl.valid = rest < 0 ? 0 : (rest < kKeys ? (int)rest : kKeys);
-            if (lane < 8 && 16 * lane < pl.valid) {
-                const unsigned gr = (unsigned)(t0 / 16) + lane;
-                int page = __ldg(p.page_table + (int64_t)at.w.seq * p.table_stride + gr / per_page);
-                page = page < 0 ? 0 : (page >= p.pages ? p.pages - 1 : page);
-                pl.row = ((uint32_t)page * p.kv_heads + at.w.head) * p.page_size + (gr % per_page) * 16u;
-            }
-            return pl;
-        };
-        auto load = [&](const Place& pl, const uint8_t* values, uint32_t (&x)[kUnits][kUnitBytes / 4]) {
-#pragma unroll
-            for (int i = 0; i < kUnits; ++i) {
-                const int r = r0 + kStep * i;
-                const uint32_t row = __shfl_sync(kFull, pl.row, r >> 4) + (r & 15);
-#pragma unroll
-                for (int k = 0; k < kUnitBytes / 4; ++k) x[i][k] = 0;
-                if (r < pl.valid) ldg_bytes<kUnitBytes>(values + (uint64_t)row * kRowBytes + u * kUnitBytes, x[i]);
-            }
-        };
-        auto load_scales = [&](const Place& pl, const uint8_t* scales, uint32_t (&s)[4]) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = lane + 32 * i;
-                const uint32_t row = __shfl_sync(kFull, pl.row, r >> 4) + (r & 15);
-                s[i] = 0;
-                if (r < pl.valid) {
-                    if constexpr (D == 128)
-                        s[i] = __ldg(reinterpret_cast<const uint32_t*>(scales) + row);
-                    else
-                        s[i] = __ldg(reinterpret_cast<const uint16_t*>(scales) + row);
-                }
-            }
-        };
-        auto top_scale = [&](const uint32_t (&s)[4]) -> int {
-            unsigned m = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int b = 0; b < kScales; ++b) m = max(m, (s[i] >> (8 * b)) & 255u);
-            return (int)__reduce_max_sync(kFull, m);
-        };
-        // f16 of x relative to the scale byte `ref`, into a shared-memory tile
-        auto store = [&](const uint32_t (&x)[kUnits][kUnitBytes / 4], const uint32_t (&s)[4], int ref, uint8_t* tile) {
-#pragma unroll
-            for (int i = 0; i < kUnits; ++i) {
-                const int r = r0 + kStep * i;
-                const uint32_t sw = __shfl_sync(kFull, s[kStep * i / 32], r & 31);
-                const int e = (int)((sw >> (8 * (u >> 1))) & 255u) - ref;
-                uint32_t h[8];
-                convert16<BITS>(x[i], dev::pow2_f16x2(e, e), h);
-                uint8_t* row = tile + (u >> 2) * L::half + r * 128;
-                const int chunk = (u & 3) * 2;
-                *reinterpret_cast<uint4*>(row + ((chunk ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
-            }
-        };
-
-        Cursor ahead = c;  // one key tile ahead of c
-        int at = 0;        // key tile of `ahead`'s unit
-        bool more = true;
-        Place pl = place(ahead, 0);
-        load_scales(pl, p.k_scales, ks);
-        load_scales(pl, p.v_scales, vs);
-        load(pl, p.k_values, kx);
-        load(pl, p.v_values, vx);
-        int vref = 0, stage = 0, meta_at = 0;
-        uint32_t phase = 1;  // the first pass over the stages finds them empty
-        do {
-            const UnitRange range = unit_range(p, c);
-            vref = 0;
-            for (int t = 0; t < c.tiles; ++t) {
-                const int64_t t0 = (c.w.first + c.tile0 + t) * kKeys;
-                const bool partly = t0 < range.all_lo || t0 + kKeys > range.all_hi;
-                const int kref = max(top_scale(ks), 1), vtop = top_scale(vs);
-                if (vref == 0 || vtop > vref + kValueMax) vref = max(vtop - kValueLift, 1);
-                uint32_t vs_now[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vs_now[i] = vs[i];
-
-                MXK_WAIT(&bars.k_empty[stage], phase);
-                store(kx, ks, kref - kKeyLift, smem + L::k + stage * L::tile);
-                if (cw == 0 && lane == 0) meta[meta_at % kMeta] = make_int2(kref, vref);
-                dev::fence_proxy_async();
-                dev::mbar_arrive(&bars.k_full[stage]);
-
-                // the next key tile is on its way while this one's values are converted
-                if (more) {
-                    if (++at == ahead.tiles) at = 0, more = ahead.next(p);
-                }
-                if (more) {
-                    pl = place(ahead, at);
-                    load_scales(pl, p.k_scales, ks);
-                    load_scales(pl, p.v_scales, vs);
-                    load(pl, p.k_values, kx);
-                }
-                if constexpr (BITS == 8) {
-                    if (partly) {  // a NaN belongs to the rows that see it: they get it at the end
-                        bool nans = false;
-#pragma unroll
-                        for (int i = 0; i < kUnits; ++i)
-#pragma unroll
-                            for (int k = 0; k < kUnitBytes / 4; ++k) {
-                                const uint32_t b = __vcmpeq4(vx[i][k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                                nans |= b != 0;
-                                vx[i][k] &= ~b;
-                            }
-                        if (nans) *reinterpret_cast<volatile int*>(&nan_unit[c.unit & 3]) = c.unit;
-                    }
-                }
-                MXK_WAIT(&bars.v_empty[stage], phase);
-                store(vx, vs_now, vref, smem + L::v + stage * L::tile);
-                dev::fence_proxy_async();
-                dev::mbar_arrive(&bars.v_full[stage]);
-                if (more) load(pl, p.v_values, vx);
-
-                ++meta_at;
-                if (++stage == kStages) stage = 0, phase ^= 1;
-            }
-        } while (c.next(p));
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProductRegs));
-        // ----------------------------------------------------------- products
-        constexpr uint32_t idesc_s = dev::f16_idesc(kTileRows, kKeys, false);
-        constexpr uint32_t idesc_o = dev::f16_idesc(kTileRows, D, true);
-        const uint32_t base = dev::smem_addr(smem);
-        if (warp == kSoftmaxWarps + kConvertWarps && lane == 0) {
-            bool ok = true;
-            int k_stage = 0, v_stage = 0;
-            uint32_t k_phase = 0, v_phase = 0, p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
-            auto scores = [&](int w) {  // S_w = Q_w K^T
-                dev::tc_fence_after();
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t at = (i / 4) * L::half + (i % 4) * 32;
-                    dev::tc_mma_f16(tmem + w * kKeys,
-                                    dev::smem_desc(base + L::q + w * L::tile + at, 16, 1024, dev::kLayoutSwizzle128),
-                                    dev::smem_desc(base + L::k + k_stage * L::tile + at, 16, 1024, dev::kLayoutSwizzle128),
-                                    idesc_s, i > 0);
-                }
-                dev::tc_commit(&bars.s_full[w]);
-            };
-            do {
-                const int nw = c.rows(p) > kTileRows ? 2 : 1;
-                for (int t = 0; t <= c.tiles && ok; ++t) {
-                    // scores of key tile t, weighted values of key tile t - 1
-                    for (int w = 0; w < nw && ok; ++w) {
-                        if (t > 0) {
-                            ok = dev::mbar_wait_lean(&bars.p_ready[w], p_phase[w], abort_flag, err);
-                            if (ok && w == 0) ok = dev::mbar_wait_lean(&bars.v_full[v_stage], v_phase, abort_flag, err);
-                            if (!ok) break;
-                            p_phase[w] ^= 1;
-                            dev::tc_fence_after();
-#pragma unroll
-                            for (int i = 0; i < kKeys / 16; ++i)
-                                dev::tc_mma_f16_ta(
-                                    tmem + kO + w * D, tmem + w * kKeys + 8 * i,
-                                    dev::smem_desc(base + L::v + v_stage * L::tile + i * 2048, L::half, 1024,
-                                                   dev::kLayoutSwizzle128),
-                                    idesc_o, t > 1 || i > 0);
-                            dev::tc_commit(&bars.o_done[w]);
-                            if (w == nw - 1) dev::tc_commit(&bars.v_empty[v_stage]);
-                        }
-                        if (t < c.tiles) {
-                            if (w == 0) ok = dev::mbar_wait_lean(&bars.k_full[k_stage], k_phase, abort_flag, err);
-                            if (ok && t == 0) {
-                                ok = dev::mbar_wait_lean(&bars.q_ready[w], q_phase[w], abort_flag, err);
-                                q_phase[w] ^= 1;
-                            }
-                            if (!ok) break;
-                            scores(w);
-                        }
-                    }
-                    if (!ok) break;
-                    if (t > 0) {
-                        if (++v_stage == kStages) v_stage = 0, v_phase ^= 1;
-                    }
-                    if (t < c.tiles) {
-                        dev::tc_commit(&bars.k_empty[k_stage]);
-                        if (++k_stage == kStages) k_stage = 0, k_phase ^= 1;
-                    }
-                }
-            } while (ok && c.next(p));
-            // Products in flight must not outlive the CTA's memory.
-            dev::tc_commit(&bars.drain);
-            const long long start = clock64();
-            while (!dev::mbar_try_wait(&bars.drain, 0))
-                if (clock64() - start > dev::kWaitLimitCycles) break;
-        }
-        __syncwarp();
-    }
-#undef MXK_WAIT
-done:
+__device__ __forceinline__ void finish(const AttentionParams& p, const Block& b) {
     dev::tc_fence_before();
     __syncthreads();
     dev::tc_fence_after();
-    if (warp == 0) dev::tmem_dealloc(tmem, 512);
+    if (threadIdx.x < 32) dev::tmem_dealloc(b.tmem, 512);
     // After a wait gave up nothing of this CTA is joined.
-    if (tid == 0 && *abort_flag) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0), p.part_ends[blockIdx.x] = 1;
+    if (threadIdx.x == 0 && *b.abort_flag())
+        p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0), p.part_ends[blockIdx.x] = 1;
 }
 
 template <int D, int BITS>
-int launch(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
-    constexpr int smem = Smem<D>::total;
-    static thread_local int ready_device = -1;
+__global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(const AttentionParams p, unsigned* err) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) Shared shared;
+    __shared__ int64_t scratch[Packed::threads / 32 + 2];
+    Block b;
+    Cursor c;
+    if (!begin<D, Packed, 32 * Packed::convert_warps>(p, smem_raw, &shared, scratch, err, b, c)) return;
+    const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
+    if (warp < kSoftmaxWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Packed::softmax_regs));
+        softmax_role<D, false>(p, b, c, warp);
+    } else if (warp < Packed::product_warp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Packed::convert_regs));
+        convert_role<D, BITS>(p, b, c, warp - kSoftmaxWarps);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Packed::product_regs));
+        if (warp == Packed::product_warp) product_role<D>(p, b, c);
+    }
+    finish(p, b);
+}
+
+template <int D>
+__global__ void __launch_bounds__(Ready::threads, 1) attention_ready_kernel(const AttentionParams p, unsigned* err) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) Shared shared;
+    __shared__ int64_t scratch[Ready::threads / 32 + 2];
+    Block b;
+    Cursor c;
+    if (!begin<D, Ready, 1>(p, smem_raw, &shared, scratch, err, b, c)) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the converted tiles
+    const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
+    if (warp < kSoftmaxWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Ready::softmax_regs));
+        softmax_role<D, true>(p, b, c, warp);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Ready::product_regs));
+        if (warp == Ready::product_warp)
+            product_role<D>(p, b, c);
+        else if (warp == Ready::load_warp)
+            load_role<D>(p, b, c);
+    }
+    finish(p, b);
+}
+
+// Once per device: shared memory, and that the build has the registers the split assumes.
+template <class K>
+int prepare_kernel(K kernel, int smem, int regs, int& ready_device) {
     int dev = 0;
     MXK_CUDA(cudaGetDevice(&dev));
-    if (ready_device != dev) {
-        MXK_CUDA(cudaFuncSetAttribute(attention_tiles_kernel<D, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        cudaFuncAttributes attr{};
-        MXK_CUDA(cudaFuncGetAttributes(&attr, attention_tiles_kernel<D, BITS>));
-        if (attr.numRegs != kLaunchRegs)
-            return fail(MXK_ERR_CUDA, "cache_attention: the build does not have the registers its split assumes");
-        ready_device = dev;
-    }
+    if (ready_device == dev) return MXK_OK;
+    MXK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaFuncAttributes attr{};
+    MXK_CUDA(cudaFuncGetAttributes(&attr, kernel));
+    if (attr.numRegs != regs)
+        return fail(MXK_ERR_UNSUPPORTED, "cache_attention: kernel built with " + std::to_string(attr.numRegs) +
+                                             " registers, the register split needs " + std::to_string(regs));
+    ready_device = dev;
+    return MXK_OK;
+}
+
+template <int D, int BITS>
+int launch_packed(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
+    static thread_local int ready_device = -1;
+    MXK_CHECK(prepare_kernel(attention_tiles_kernel<D, BITS>, Smem<D>::total, Packed::launch_regs, ready_device));
     unsigned* err = device_error_word();
     if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
     static const int sms = sm_count();
@@ -707,24 +982,81 @@ int launch(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
     MXK_CHECK(ws.take(p, ctas, kRows, D));
     {
         LaunchScope scope("attention_tiles", stream);
-        attention_tiles_kernel<D, BITS><<<(unsigned)ctas, kThreads, smem, stream>>>(p, err);
+        attention_tiles_kernel<D, BITS><<<(unsigned)ctas, Packed::threads, Smem<D>::total, stream>>>(p, err);
         MXK_CUDA(cudaGetLastError());
     }
     return join_parts<kRows, D>(p, (int)ctas, 32, stream);
 }
 
+template <int D, int BITS>
+int launch_ready(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
+    static thread_local int ready_device = -1;
+    MXK_CHECK(prepare_kernel(attention_ready_kernel<D>, Smem<D>::total, Ready::launch_regs, ready_device));
+    unsigned* err = device_error_word();
+    if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
+    static const int sms = sm_count();
+    const int64_t ctas = most_tiles < sms ? most_tiles : sms;
+    const int64_t tiles = (int64_t)p.seqs * p.kv_heads * p.max_tiles;
+    Workspace ws(stream);
+    MXK_CHECK(ws.take(p, ctas, kRows, D, tiles * (2 * Smem<D>::tile + (int64_t)sizeof(int2))));
+    p.ready_k = static_cast<uint8_t*>(ws.extra);
+    p.ready_v = p.ready_k + tiles * Smem<D>::tile;
+    p.ready_meta = reinterpret_cast<int2*>(p.ready_v + tiles * Smem<D>::tile);
+    {
+        LaunchScope scope("attention_unpack", stream);
+        attention_unpack_kernel<D, BITS><<<(unsigned)tiles, 256, 0, stream>>>(p);
+        MXK_CUDA(cudaGetLastError());
+    }
+    {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)ctas);
+        cfg.blockDim = dim3(Ready::threads);
+        cfg.dynamicSmemBytes = Smem<D>::total;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        LaunchScope scope("attention_ready", stream);
+        MXK_CUDA(cudaLaunchKernelEx(&cfg, attention_ready_kernel<D>, p, err));
+    }
+    return join_parts<kRows, D>(p, (int)ctas, 32, stream);
+}
+
+template <int D, int BITS>
+int launch(const AttentionParams& p, bool ready, int max_q, cudaStream_t stream) {
+    const int64_t most = attention_tile_bound(p, max_q, kRows, kKeys);
+    return ready ? launch_ready<D, BITS>(p, most, stream) : launch_packed<D, BITS>(p, most, stream);
+}
+
 template <int D>
-int launch_bits(int bits, const AttentionParams& p, int64_t most_tiles, cudaStream_t stream) {
-    if (bits == 8) return launch<D, 8>(p, most_tiles, stream);
-    if (bits == 6) return launch<D, 6>(p, most_tiles, stream);
-    return launch<D, 4>(p, most_tiles, stream);
+int launch_bits(int bits, const AttentionParams& p, bool ready, int max_q, cudaStream_t stream) {
+    if (bits == 8) return launch<D, 8>(p, ready, max_q, stream);
+    if (bits == 6) return launch<D, 6>(p, ready, max_q, stream);
+    return launch<D, 4>(p, ready, max_q, stream);
 }
 
 }  // namespace
 
-int launch_attention_tiles(int bits, int head_dim, const AttentionParams& p, int max_q, cudaStream_t stream) {
-    const int64_t most = attention_tile_bound(p, max_q, kRows, kKeys);
-    return head_dim == 128 ? launch_bits<128>(bits, p, most, stream) : launch_bits<64>(bits, p, most, stream);
+int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, cudaStream_t stream) {
+    // Several row tiles of a key head share its keys: converting those once pays for
+    // writing and reading them as f16.
+    p.max_tiles = (int)((p.max_kv + kKeys - 1) / kKeys);
+    const int64_t bytes = (int64_t)p.seqs * p.kv_heads * p.max_tiles * 2 * kKeys * head_dim * 2;
+    const bool many = (int64_t)max_q * p.group > kReadyRows && p.max_tiles > 0 && bytes <= kReadyBytes;
+    const int few_q = (int)((kReadyRows + p.group - 1) / p.group);
+    if (many) {
+        AttentionParams q = p;
+        if (p.seqs > 1 && q.min_rows <= kReadyRows) q.min_rows = kReadyRows + 1;
+        MXK_CHECK(head_dim == 128 ? launch_bits<128>(bits, q, true, max_q, stream)
+                                  : launch_bits<64>(bits, q, true, max_q, stream));
+        if (p.seqs == 1) return MXK_OK;
+        p.max_rows = kReadyRows;
+        max_q = few_q;
+    }
+    return head_dim == 128 ? launch_bits<128>(bits, p, false, max_q, stream)
+                           : launch_bits<64>(bits, p, false, max_q, stream);
 }
 
 }  // namespace mxk
