@@ -46,6 +46,7 @@ constexpr int kKeys = 128;               // tokens of a key tile
 constexpr int kStages = 2;               // of keys and of values
 constexpr int kMeta = 4;                 // key tiles whose references are kept (converter warps)
 constexpr int kRefStep = 4;              // value references are multiples of this many octaves
+constexpr int kMostDown = 64;            // octaves that a float32 weight may be scaled down by
 constexpr int kSoftmaxWarps = 8;
 
 // Rows per key head above which its keys are converted beforehand, and the most
@@ -528,45 +529,80 @@ __device__ __forceinline__ float max3f(float a, float b, float c) {
     return r;
 }
 
-// Columns of a key tile that a row sees, [from, to).
-struct Columns {
-    int from, to;
-};
-
-// Folds 32 scores (columns `at` ..) into the running maxima m; MASKED: those seen only.
-template <bool MASKED>
-__device__ __forceinline__ void fold_top(const uint32_t (&s)[32], int at, Columns c, float (&m)[4]) {
+// Folds 32 scores into the running maxima m.
+__device__ __forceinline__ void fold_top(const uint32_t (&s)[32], float (&m)[4]) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-        float a = __uint_as_float(s[i]), b = __uint_as_float(s[i + 1]);
-        if constexpr (MASKED) {
-            const float neg_inf = __int_as_float(0xff800000);
-            a = at + i < c.from || at + i >= c.to ? neg_inf : a;
-            b = at + i + 1 < c.from || at + i + 1 >= c.to ? neg_inf : b;
-        }
-        m[(i / 2) & 3] = max3f(m[(i / 2) & 3], a, b);
-    }
+    for (int i = 0; i < 32; i += 2)
+        m[(i / 2) & 3] = max3f(m[(i / 2) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
 }
 
-// Weights 2^(score * f - base) of 32 scores, added to sum, to f16 pairs.  GENERAL: those
-// seen only, and the f16 ones scaled by `down`.
-template <bool GENERAL>
-__device__ __forceinline__ void fold_weights(const uint32_t (&s)[32], int at, Columns c, float f, float base, float down,
-                                             float2 (&sum)[2], uint32_t (&pw)[16]) {
+// Weights 2^(score * f - base) of 32 scores, added to sum, as f16 pairs.
+__device__ __forceinline__ void fold_weights(const uint32_t (&s)[32], float f, float base, float2 (&sum)[2],
+                                             uint32_t (&pw)[16]) {
     const float2 f2 = make_float2(f, f), b2 = make_float2(-base, -base);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
         float2 t = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, b2);
         t.x = ex2(t.x), t.y = ex2(t.y);
-        if constexpr (GENERAL) {
-            if (at + i < c.from || at + i >= c.to) t.x = 0.0f;
-            if (at + i + 1 < c.from || at + i + 1 >= c.to) t.y = 0.0f;
-        }
         sum[(i / 2) & 1] = __fadd2_rn(sum[(i / 2) & 1], t);
-        if constexpr (GENERAL) t.x *= down, t.y *= down;
         const __half2 u = __float22half2_rn(t);
         pw[i / 2] = *reinterpret_cast<const uint32_t*>(&u);
     }
+}
+
+// The rare steps, out of the way of the loop's registers.
+
+// An output row in TMEM times g.
+template <int D>
+__device__ __noinline__ void scale_output(uint32_t o_col, float g) {
+#pragma unroll 1
+    for (int h = 0; h < D / 32; ++h) {
+        uint32_t o[32];
+        dev::tmem_ld_32x32b_x32(o_col + 32 * h, o);
+        dev::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
+        dev::tmem_st_32x32b_x32(o_col + 32 * h, o);
+    }
+    dev::tmem_wait_st();
+}
+
+// The largest score of a key tile of which the row sees columns [from, to).
+__device__ __noinline__ float masked_top(uint32_t s_col, int from, int to) {
+    float m = __int_as_float(0xff800000);
+#pragma unroll 1
+    for (int h = 0; h < kKeys / 32; ++h) {
+        uint32_t s[32];
+        dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
+        dev::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (32 * h + i >= from && 32 * h + i < to) m = fmaxf(m, __uint_as_float(s[i]));
+    }
+    return m;
+}
+
+// Its weights, the f16 ones times `down`; returns their sum.
+__device__ __noinline__ float masked_weights(uint32_t s_col, int from, int to, float f, float base, float down) {
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int h = 0; h < kKeys / 32; ++h) {
+        uint32_t s[32], pw[16];
+        dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
+        dev::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            float a = ex2(fmaf(__uint_as_float(s[i]), f, -base)), b = ex2(fmaf(__uint_as_float(s[i + 1]), f, -base));
+            if (32 * h + i < from || 32 * h + i >= to) a = 0.0f;
+            if (32 * h + i + 1 < from || 32 * h + i + 1 >= to) b = 0.0f;
+            sum += a + b;
+            const __half2 u = __floats2half2_rn(a * down, b * down);
+            pw[i / 2] = *reinterpret_cast<const uint32_t*>(&u);
+        }
+        dev::tmem_st_32x32b_x16(s_col + 16 * h, pw);
+    }
+    dev::tmem_wait_st();
+    return sum;
 }
 
 // Features of a value row that are NaN (8-bit elements) among the tokens [k0, k1) that
@@ -689,75 +725,61 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                         nans |= ref.y >> 16;
                         if (t + 1 < c.tiles) ref = __ldg(meta + t + 1);
                     }
-                    const bool partly = t < whole.from || t >= whole.to;
-                    Columns cols{0, kKeys};
-                    if (partly) {
-                        const int64_t t0 = first_key + (int64_t)t * kKeys;
-                        cols.from = lo > t0 ? (lo - t0 < kKeys ? (int)(lo - t0) : kKeys) : 0;
-                        cols.to = hi < t0 ? 0 : (hi - t0 < kKeys ? (int)(hi - t0) : kKeys);
-                    }
-                    // the largest score
+                    if (t == 0) vrun = vref;
+                    const bool rare = t < whole.from || t >= whole.to || vrun - vref > kMostDown;
+                    int from = 0, to = kKeys;
                     uint32_t s[HOLD ? 4 : 2][32];
-                    float m4[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
-                    if constexpr (HOLD) {
-#pragma unroll
-                        for (int h = 0; h < kKeys / 32; ++h) dev::tmem_ld_32x32b_x32(s_col + 32 * h, s[h]);
-                        dev::tmem_wait_ld();
-                        if (partly) {
-#pragma unroll
-                            for (int h = 0; h < kKeys / 32; ++h) fold_top<true>(s[h], 32 * h, cols, m4);
-                        } else {
-#pragma unroll
-                            for (int h = 0; h < kKeys / 32; ++h) fold_top<false>(s[h], 32 * h, cols, m4);
-                        }
+                    float top;
+                    if (rare) {
+                        const int64_t t0 = first_key + (int64_t)t * kKeys;
+                        from = lo > t0 ? (lo - t0 < kKeys ? (int)(lo - t0) : kKeys) : 0;
+                        to = hi < t0 ? 0 : (hi - t0 < kKeys ? (int)(hi - t0) : kKeys);
+                        top = masked_top(s_col, from, to);
                     } else {
-                        auto tops = [&](auto masked) {
-                            dev::tmem_ld_32x32b_x32(s_col, s[0]);
+                        float m[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
+                        dev::tmem_ld_32x32b_x32(s_col, s[0]);
+                        if constexpr (HOLD) {
 #pragma unroll
-                            for (int h = 0; h < kKeys / 32; ++h) {
+                            for (int h = 1; h < kKeys / 32; ++h) dev::tmem_ld_32x32b_x32(s_col + 32 * h, s[h]);
+                            dev::tmem_wait_ld();
+                        }
+#pragma unroll
+                        for (int h = 0; h < kKeys / 32; ++h) {
+                            if constexpr (!HOLD) {
                                 dev::tmem_wait_ld();
                                 if (h + 1 < kKeys / 32) dev::tmem_ld_32x32b_x32(s_col + 32 * (h + 1), s[(h + 1) & 1]);
-                                fold_top<decltype(masked)::value>(s[h & 1], 32 * h, cols, m4);
                             }
-                        };
-                        if (partly)
-                            tops(std::true_type{});
-                        else
-                            tops(std::false_type{});
+                            fold_top(s[HOLD ? h : h & 1], m);
+                        }
+                        top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                     }
-                    float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                     if (top != neg_inf) top *= f;
 
                     // Raise the row's maximum, or the reference of the output, if need be.
                     const bool raise = top > run_max + kMaxSlack;
-                    const bool shift = vref > vrun;
-                    if (__any_sync(kFull, raise) || shift) {
+                    if (__any_sync(kFull, raise) || vref > vrun) {
                         const float m = raise ? top : run_max;
                         float g = m == run_max ? 1.0f : ex2(run_max - m);
                         run_max = m;
                         base = (m == neg_inf ? 0.0f : m) - kExpShift;
                         sum *= g;
+                        if (vref > vrun) g *= __uint_as_float((uint32_t)max(vrun - vref + 127, 0) << 23);
+                        vrun = max(vrun, vref);
                         if (t > 0) {  // the output so far, once the products before have finished
-                            if (shift) g *= __uint_as_float((uint32_t)max(vrun - vref + 127, 0) << 23);
                             if (!b.wait(&sh->o_done[w], o_phase ^ 1)) return false;
                             dev::tc_fence_after();
-#pragma unroll
-                            for (int h = 0; h < D / 32; ++h) {
-                                uint32_t o[32];
-                                dev::tmem_ld_32x32b_x32(o_col + 32 * h, o);
-                                dev::tmem_wait_ld();
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
-                                dev::tmem_st_32x32b_x32(o_col + 32 * h, o);
-                            }
+                            scale_output<D>(o_col, g);
                         }
-                        if (shift) vrun = vref;
                     }
-                    // the weights, over the scores they come from
-                    const float down = __uint_as_float((uint32_t)max(vref - vrun + 127, 0) << 23);
-                    float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                    auto weights = [&](auto general) {
-                        constexpr bool kGeneral = decltype(general)::value;
+                    // The weights, over the scores they come from, scaled by 2^(vref - vrun): up to
+                    // kMostDown octaves in their exponents, which float32 sums do not notice.
+                    const int down = min(vrun - vref, kMostDown);
+                    const float shifted = base + (float)down, up = __uint_as_float((uint32_t)(127 + down) << 23);
+                    if (rare) {
+                        sum += up * masked_weights(s_col, from, to, f, shifted,
+                                                   __uint_as_float((uint32_t)max(vref - vrun + down + 127, 0) << 23));
+                    } else {
+                        float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                         if constexpr (!HOLD) dev::tmem_ld_32x32b_x32(s_col, s[0]);
 #pragma unroll
                         for (int h = 0; h < kKeys / 32; ++h) {
@@ -766,16 +788,12 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                                 dev::tmem_wait_ld();
                                 if (h + 1 < kKeys / 32) dev::tmem_ld_32x32b_x32(s_col + 32 * (h + 1), s[(h + 1) & 1]);
                             }
-                            fold_weights<kGeneral>(s[HOLD ? h : h & 1], 32 * h, cols, f, base, down, part, pw);
+                            fold_weights(s[HOLD ? h : h & 1], f, shifted, part, pw);
                             dev::tmem_st_32x32b_x16(s_col + 16 * h, pw);
                         }
-                    };
-                    if (partly || vref != vrun)
-                        weights(std::true_type{});
-                    else
-                        weights(std::false_type{});
-                    dev::tmem_wait_st();
-                    sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+                        dev::tmem_wait_st();
+                        sum += up * ((part[0].x + part[0].y) + (part[1].x + part[1].y));
+                    }
                 }
                 dev::tc_fence_before();
                 dev::mbar_arrive(&sh->p_ready[w]);
