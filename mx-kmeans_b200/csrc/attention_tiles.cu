@@ -43,6 +43,7 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kTileRows = 128;           // M of one product
 constexpr int kRows = 2 * kTileRows;     // rows of a unit
 constexpr int kKeys = 128;               // tokens of a key tile
+constexpr int kHalf = kKeys / 2;         // tokens of one step of the softmax
 constexpr int kStages = 2;               // of keys and of values
 constexpr int kMeta = 4;                 // key tiles whose references are kept (converter warps)
 constexpr int kRefStep = 4;              // value references are multiples of this many octaves
@@ -55,8 +56,7 @@ constexpr int kReadyRows = kRows;
 constexpr int64_t kReadyBytes = 4ll << 30;
 
 // The two kernels' warps and registers.  Warpgroups give up or take registers of
-// those the block was launched with: the softmax of ready-made tiles holds a row's 128
-// scores in registers, next to converter warps it reads them from TMEM twice.
+// those the block was launched with.
 struct Packed {
     static constexpr int convert_warps = 8;
     static constexpr int product_warp = kSoftmaxWarps + convert_warps;
@@ -67,7 +67,7 @@ struct Packed {
 struct Ready {
     static constexpr int product_warp = kSoftmaxWarps, load_warp = kSoftmaxWarps + 1;
     static constexpr int threads = 384;
-    static constexpr int launch_regs = 168, softmax_regs = 208, product_regs = 88;
+    static constexpr int launch_regs = 168, softmax_regs = 200, product_regs = 104;
     static_assert(256 * softmax_regs + 128 * product_regs <= threads * launch_regs, "");
 };
 
@@ -84,9 +84,9 @@ struct Smem {
 struct Shared {
     uint64_t q_ready[2];       // the tile's queries are in shared memory
     uint64_t k_full[kStages], v_full[kStages], k_empty[kStages], v_empty[kStages];
-    uint64_t s_full[2];        // scores are in TMEM
-    uint64_t p_ready[2];       // weights are in TMEM, the output may be added to
-    uint64_t o_done[2];        // the tile's product with the values has finished
+    uint64_t s_full[2][2];     // [row tile][half of the key tile] scores are in TMEM
+    uint64_t p_ready[2][2];    // the half's weights are in TMEM, the output may be added to
+    uint64_t o_done[2][2];     // the half's product with the values has finished
     uint64_t drain;
     int2 meta[kMeta];          // converter warps: the key tile's references
     int nan_unit[4];           // converter warps: unit in which a NaN was taken out of a partly seen tile
@@ -454,7 +454,7 @@ __device__ __forceinline__ void load_role(const AttentionParams& p, const Block&
 template <int D>
 __device__ __forceinline__ void product_role(const AttentionParams& p, const Block& b, Cursor c) {
     using L = Smem<D>;
-    constexpr uint32_t idesc_s = dev::f16_idesc(kTileRows, kKeys, false);
+    constexpr uint32_t idesc_s = dev::f16_idesc(kTileRows, kHalf, false);
     constexpr uint32_t idesc_o = dev::f16_idesc(kTileRows, D, true);
     // The whole warp walks, one elected lane issues: descriptors and addresses stay
     // warp-uniform and are advanced by constants.
@@ -465,50 +465,68 @@ __device__ __forceinline__ void product_role(const AttentionParams& p, const Blo
     Shared* sh = b.sh;
     bool ok = true;
     uint32_t k_stage = 0, v_stage = 0, k_phase = 0, v_phase = 0, p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
+    // A key tile goes through in two halves of 64 tokens, each with its own columns: while
+    // a row tile's softmax works on one, the scores of the next are multiplied.
+    auto scores = [&](int w, int half) {
+        const uint64_t kd = k_desc + (uint64_t)(k_stage * (L::tile >> 4) + half * (kHalf * 128 >> 4));
+        const uint64_t qd = q_desc + (uint64_t)(w * (L::tile >> 4));
+        if (dev::elect_one()) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const uint32_t at = ((i / 4) * L::half + (i % 4) * 32) >> 4;
+                dev::tc_mma_f16(b.tmem + w * kKeys + half * kHalf, qd + at, kd + at, idesc_s, i > 0);
+            }
+            dev::tc_commit(&sh->s_full[w][half]);
+        }
+        __syncwarp();
+    };
+    auto release_keys = [&]() {
+        if (dev::elect_one()) dev::tc_commit(&sh->k_empty[k_stage]);
+        __syncwarp();
+        if (++k_stage == kStages) k_stage = 0, k_phase ^= 1;
+    };
     do {
         const int nw = __shfl_sync(kFull, c.rows(p) > kTileRows ? 2 : 1, 0);
         const int tiles = __shfl_sync(kFull, c.tiles, 0);
-        for (int t = 0; t <= tiles && ok; ++t) {
-            // weighted values of key tile t - 1, scores of key tile t
+        ok = b.wait_lean(&sh->k_full[k_stage], k_phase);
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                if (w >= nw || !ok) continue;
-                if (t > 0) {
-                    if (w == 0) ok = b.wait_lean(&sh->v_full[v_stage], v_phase);
-                    if (ok) ok = b.wait_lean(&sh->p_ready[w], p_phase[w]);
-                    p_phase[w] ^= 1;
+        for (int w = 0; w < 2; ++w)
+            if (w < nw && ok) ok = b.wait_lean(&sh->q_ready[w], q_phase[w]), q_phase[w] ^= 1;
+        if (!ok) break;
+        dev::tc_fence_after();
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+                if (w < nw) scores(w, half);
+        release_keys();
+        for (int t = 0; t < tiles && ok; ++t) {
+            // weighted values of key tile t, scores of key tile t + 1
+            ok = b.wait_lean(&sh->v_full[v_stage], v_phase);
+            if (ok && t + 1 < tiles) ok = b.wait_lean(&sh->k_full[k_stage], k_phase);
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    if (w >= nw || !ok) continue;
+                    ok = b.wait_lean(&sh->p_ready[w][half], p_phase[w]);
+                    if (!ok) continue;
+                    if (half == 1) p_phase[w] ^= 1;
                     dev::tc_fence_after();
-                    const uint64_t vd = v_desc + (uint64_t)(v_stage * (L::tile >> 4));
-                    if (ok && dev::elect_one()) {
+                    const uint64_t vd = v_desc + (uint64_t)(v_stage * (L::tile >> 4) + half * (kHalf * 128 >> 4));
+                    if (dev::elect_one()) {
 #pragma unroll
-                        for (int i = 0; i < kKeys / 16; ++i)
-                            dev::tc_mma_f16_ta(b.tmem + 2 * kKeys + w * D, b.tmem + w * kKeys + 8 * i,
-                                               vd + i * (2048 >> 4), idesc_o, i > 0 || t > 1);
-                        dev::tc_commit(&sh->o_done[w]);
-                        if (w == nw - 1) dev::tc_commit(&sh->v_empty[v_stage]);
+                        for (int i = 0; i < kHalf / 16; ++i)
+                            dev::tc_mma_f16_ta(b.tmem + 2 * kKeys + w * D, b.tmem + w * kKeys + half * kHalf + 8 * i,
+                                               vd + i * (2048 >> 4), idesc_o, i > 0 || half > 0 || t > 0);
+                        dev::tc_commit(&sh->o_done[w][half]);
+                        if (half == 1 && w == nw - 1) dev::tc_commit(&sh->v_empty[v_stage]);
                     }
                     __syncwarp();
+                    if (t + 1 < tiles) scores(w, half);
                 }
-                if (t < tiles && ok) {
-                    if (w == 0) ok = b.wait_lean(&sh->k_full[k_stage], k_phase);
-                    if (ok && t == 0) ok = b.wait_lean(&sh->q_ready[w], q_phase[w]), q_phase[w] ^= 1;
-                    dev::tc_fence_after();
-                    const uint64_t kd = k_desc + (uint64_t)(k_stage * (L::tile >> 4));
-                    const uint64_t qd = q_desc + (uint64_t)(w * (L::tile >> 4));
-                    if (ok && dev::elect_one()) {
-#pragma unroll
-                        for (int i = 0; i < D / 16; ++i) {
-                            const uint32_t at = ((i / 4) * L::half + (i % 4) * 32) >> 4;
-                            dev::tc_mma_f16(b.tmem + w * kKeys, qd + at, kd + at, idesc_s, i > 0);
-                        }
-                        dev::tc_commit(&sh->s_full[w]);
-                        if (w == nw - 1) dev::tc_commit(&sh->k_empty[k_stage]);
-                    }
-                    __syncwarp();
-                }
-            }
-            if (t > 0 && ++v_stage == kStages) v_stage = 0, v_phase ^= 1;
-            if (t < tiles && ++k_stage == kStages) k_stage = 0, k_phase ^= 1;
+            if (++v_stage == kStages) v_stage = 0, v_phase ^= 1;
+            if (ok && t + 1 < tiles) release_keys();
         }
     } while (ok && c.next(p));
     // Products in flight must not outlive the CTA's memory.
@@ -567,11 +585,11 @@ __device__ __noinline__ void scale_output(uint32_t o_col, float g) {
     dev::tmem_wait_st();
 }
 
-// The largest score of a key tile of which the row sees columns [from, to).
+// The largest score of a half key tile of which the row sees columns [from, to).
 __device__ __noinline__ float masked_top(uint32_t s_col, int from, int to) {
     float m = __int_as_float(0xff800000);
 #pragma unroll 1
-    for (int h = 0; h < kKeys / 32; ++h) {
+    for (int h = 0; h < kHalf / 32; ++h) {
         uint32_t s[32];
         dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
         dev::tmem_wait_ld();
@@ -586,7 +604,7 @@ __device__ __noinline__ float masked_top(uint32_t s_col, int from, int to) {
 __device__ __noinline__ float masked_weights(uint32_t s_col, int from, int to, float f, float base, float down) {
     float sum = 0.0f;
 #pragma unroll 1
-    for (int h = 0; h < kKeys / 32; ++h) {
+    for (int h = 0; h < kHalf / 32; ++h) {
         uint32_t s[32], pw[16];
         dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
         dev::tmem_wait_ld();
@@ -678,8 +696,8 @@ __device__ __forceinline__ float put_query(const AttentionParams& p, int64_t at,
            __uint_as_float((uint32_t)(127 - rest - kKeyLift / 2) << 23);
 }
 
-// HOLD: a row's scores stay in registers (ready-made tiles), else they are read twice.
-template <int D, bool HOLD>
+// READY: tiles were converted beforehand, their references lie in global memory.
+template <int D, bool READY>
 __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Block& b, Cursor c, int warp) {
     using L = Smem<D>;
     Shared* sh = b.sh;
@@ -688,7 +706,9 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
     const uint32_t lane_base = b.tmem + ((uint32_t)(32 * (warp & 3)) << 16);
     const uint32_t s_col = lane_base + w * kKeys, o_col = lane_base + 2 * kKeys + w * D;
     const float neg_inf = __int_as_float(0xff800000);
-    uint32_t s_phase = 0, o_phase = 0;
+    // Phases of s_full and o_done; a wait is never more than one completion behind, since
+    // the scores of a half follow the products of the half before the last.
+    uint32_t s_phase = 0, o_phase[2] = {0, 0};
     int meta_at = 0;
     bool open = false, went_on = false, ended = false;
     do {
@@ -711,46 +731,38 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             float run_max = neg_inf, base = -kExpShift, sum = 0.0f;
             int vrun = 0;  // the output is held relative to 2^(vrun - 127)
             bool nans = false;
-            const int2* meta = HOLD ? p.ready_meta + ready_at(p, c) : nullptr;
-            int2 ref = HOLD ? __ldg(meta) : make_int2(0, 0);
-            for (int t = 0; t < c.tiles; ++t) {
-                if (!b.wait(&sh->s_full[w], s_phase)) return false;
-                s_phase ^= 1;
+            const int2* meta = READY ? p.ready_meta + ready_at(p, c) : nullptr;
+            int2 ref = READY ? __ldg(meta) : make_int2(0, 0);
+            for (int t = 0; t < 2 * c.tiles; ++t) {  // halves of key tiles
+                if (!b.wait(&sh->s_full[w][t & 1], s_phase)) return false;
+                if (t & 1) s_phase ^= 1;
                 dev::tc_fence_after();
-                if constexpr (!HOLD) ref = *const_cast<const int2*>(&sh->meta[(meta_at + t) % kMeta]);
+                const uint32_t s_at = s_col + (t & 1) * kHalf;
+                if (!READY && !(t & 1)) ref = *const_cast<const int2*>(&sh->meta[(meta_at + t / 2) % kMeta]);
                 if (warp_real) {
                     const float f = row_factor * __uint_as_float((uint32_t)ref.x << 23);
                     const int vref = ref.y & 0xffff;
-                    if constexpr (HOLD) {
+                    if (READY && (t & 1)) {
                         nans |= ref.y >> 16;
-                        if (t + 1 < c.tiles) ref = __ldg(meta + t + 1);
+                        if (t + 1 < 2 * c.tiles) ref = __ldg(meta + t / 2 + 1);
                     }
                     if (t == 0) vrun = vref;
-                    const bool rare = t < whole.from || t >= whole.to || vrun - vref > kMostDown;
-                    int from = 0, to = kKeys;
-                    uint32_t s[HOLD ? 4 : 2][32];
+                    const bool rare = t < 2 * whole.from || t >= 2 * whole.to || vrun - vref > kMostDown;
+                    int from = 0, to = kHalf;
+                    uint32_t s[2][32];
                     float top;
                     if (rare) {
-                        const int64_t t0 = first_key + (int64_t)t * kKeys;
-                        from = lo > t0 ? (lo - t0 < kKeys ? (int)(lo - t0) : kKeys) : 0;
-                        to = hi < t0 ? 0 : (hi - t0 < kKeys ? (int)(hi - t0) : kKeys);
-                        top = masked_top(s_col, from, to);
+                        const int64_t t0 = first_key + (int64_t)t * kHalf;
+                        from = lo > t0 ? (lo - t0 < kHalf ? (int)(lo - t0) : kHalf) : 0;
+                        to = hi < t0 ? 0 : (hi - t0 < kHalf ? (int)(hi - t0) : kHalf);
+                        top = masked_top(s_at, from, to);
                     } else {
                         float m[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
-                        dev::tmem_ld_32x32b_x32(s_col, s[0]);
-                        if constexpr (HOLD) {
-#pragma unroll
-                            for (int h = 1; h < kKeys / 32; ++h) dev::tmem_ld_32x32b_x32(s_col + 32 * h, s[h]);
-                            dev::tmem_wait_ld();
-                        }
-#pragma unroll
-                        for (int h = 0; h < kKeys / 32; ++h) {
-                            if constexpr (!HOLD) {
-                                dev::tmem_wait_ld();
-                                if (h + 1 < kKeys / 32) dev::tmem_ld_32x32b_x32(s_col + 32 * (h + 1), s[(h + 1) & 1]);
-                            }
-                            fold_top(s[HOLD ? h : h & 1], m);
-                        }
+                        dev::tmem_ld_32x32b_x32(s_at, s[0]);
+                        dev::tmem_ld_32x32b_x32(s_at + 32, s[1]);
+                        dev::tmem_wait_ld();
+                        fold_top(s[0], m);
+                        fold_top(s[1], m);
                         top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                     }
                     if (top != neg_inf) top *= f;
@@ -766,7 +778,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                         if (vref > vrun) g *= __uint_as_float((uint32_t)max(vrun - vref + 127, 0) << 23);
                         vrun = max(vrun, vref);
                         if (t > 0) {  // the output so far, once the products before have finished
-                            if (!b.wait(&sh->o_done[w], o_phase ^ 1)) return false;
+                            if (!b.wait(&sh->o_done[w][(t - 1) & 1], (t & 1 ? o_phase[0] : o_phase[1]) ^ 1)) return false;
                             dev::tc_fence_after();
                             scale_output<D>(o_col, g);
                         }
@@ -776,38 +788,35 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                     const int down = min(vrun - vref, kMostDown);
                     const float shifted = base + (float)down, up = __uint_as_float((uint32_t)(127 + down) << 23);
                     if (rare) {
-                        sum += up * masked_weights(s_col, from, to, f, shifted,
+                        sum += up * masked_weights(s_at, from, to, f, shifted,
                                                    __uint_as_float((uint32_t)max(vref - vrun + down + 127, 0) << 23));
                     } else {
                         float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                        if constexpr (!HOLD) dev::tmem_ld_32x32b_x32(s_col, s[0]);
-#pragma unroll
-                        for (int h = 0; h < kKeys / 32; ++h) {
-                            uint32_t pw[16];
-                            if constexpr (!HOLD) {
-                                dev::tmem_wait_ld();
-                                if (h + 1 < kKeys / 32) dev::tmem_ld_32x32b_x32(s_col + 32 * (h + 1), s[(h + 1) & 1]);
-                            }
-                            fold_weights(s[HOLD ? h : h & 1], f, shifted, part, pw);
-                            dev::tmem_st_32x32b_x16(s_col + 16 * h, pw);
-                        }
+                        uint32_t pw[16];
+                        fold_weights(s[0], f, shifted, part, pw);
+                        dev::tmem_st_32x32b_x16(s_at, pw);
+                        fold_weights(s[1], f, shifted, part, pw);
+                        dev::tmem_st_32x32b_x16(s_at + 16, pw);
                         dev::tmem_wait_st();
                         sum += up * ((part[0].x + part[0].y) + (part[1].x + part[1].y));
                     }
                 }
                 dev::tc_fence_before();
-                dev::mbar_arrive(&sh->p_ready[w]);
-                o_phase ^= 1;
+                dev::mbar_arrive(&sh->p_ready[w][t & 1]);
+                if (t & 1)
+                    o_phase[1] ^= 1;
+                else
+                    o_phase[0] ^= 1;
             }
 
             // The output row.
-            if (!b.wait(&sh->o_done[w], o_phase ^ 1)) return false;
+            if (!b.wait(&sh->o_done[w][0], o_phase[0] ^ 1) || !b.wait(&sh->o_done[w][1], o_phase[1] ^ 1)) return false;
             dev::tc_fence_after();
             if (warp_real) {
                 const bool all = c.whole();
                 // NaNs that were taken out of the values, for the rows that see them
                 uint32_t bad[4] = {0, 0, 0, 0};
-                if constexpr (!HOLD) nans = *reinterpret_cast<volatile int*>(&sh->nan_unit[c.unit & 3]) == c.unit;
+                if constexpr (!READY) nans = *reinterpret_cast<volatile int*>(&sh->nan_unit[c.unit & 3]) == c.unit;
                 if (nans && real) {
                     const int64_t end = first_key + (int64_t)c.tiles * kKeys;
                     const uint4 f = nan_features<D>(p.v_values, p.page_table + (int64_t)c.w.seq * p.table_stride,
@@ -887,9 +896,12 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             dev::mbar_init(&sh->q_ready[i], kTileRows);
-            dev::mbar_init(&sh->s_full[i], 1);
-            dev::mbar_init(&sh->p_ready[i], kTileRows);
-            dev::mbar_init(&sh->o_done[i], 1);
+            dev::mbar_init(&sh->s_full[i][0], 1);
+            dev::mbar_init(&sh->s_full[i][1], 1);
+            dev::mbar_init(&sh->p_ready[i][0], kTileRows);
+            dev::mbar_init(&sh->p_ready[i][1], kTileRows);
+            dev::mbar_init(&sh->o_done[i][0], 1);
+            dev::mbar_init(&sh->o_done[i][1], 1);
         }
 #pragma unroll
         for (int i = 0; i < kStages; ++i) {
