@@ -733,24 +733,32 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             bool nans = false;
             const int2* meta = READY ? p.ready_meta + ready_at(p, c) : nullptr;
             int2 ref = READY ? __ldg(meta) : make_int2(0, 0);
-            for (int t = 0; t < 2 * c.tiles; ++t) {  // halves of key tiles
-                if (!b.wait(&sh->s_full[w][t & 1], s_phase)) return false;
-                if (t & 1) s_phase ^= 1;
-                dev::tc_fence_after();
-                const uint32_t s_at = s_col + (t & 1) * kHalf;
+            // Scores of the half at hand; the next half's are fetched as the registers get free.
+            uint32_t s[2][32];
+            if (!b.wait(&sh->s_full[w][0], s_phase)) return false;
+            dev::tc_fence_after();
+            if (warp_real) {
+                dev::tmem_ld_32x32b_x32(s_col, s[0]);
+                dev::tmem_ld_32x32b_x32(s_col + 32, s[1]);
+            }
+            const int halves = 2 * c.tiles;
+            for (int t = 0; t < halves; ++t) {
+                const uint32_t s_at = s_col + (t & 1) * kHalf, s_next = s_col + (~t & 1) * kHalf;
+                const uint32_t next_phase = s_phase ^ (t & 1);
+                bool fetched = false;
                 if (!READY && !(t & 1)) ref = *const_cast<const int2*>(&sh->meta[(meta_at + t / 2) % kMeta]);
                 if (warp_real) {
                     const float f = row_factor * __uint_as_float((uint32_t)ref.x << 23);
                     const int vref = ref.y & 0xffff;
                     if (READY && (t & 1)) {
                         nans |= ref.y >> 16;
-                        if (t + 1 < 2 * c.tiles) ref = __ldg(meta + t / 2 + 1);
+                        if (t + 1 < halves) ref = __ldg(meta + t / 2 + 1);
                     }
                     if (t == 0) vrun = vref;
                     const bool rare = t < 2 * whole.from || t >= 2 * whole.to || vrun - vref > kMostDown;
                     int from = 0, to = kHalf;
-                    uint32_t s[2][32];
                     float top;
+                    dev::tmem_wait_ld();
                     if (rare) {
                         const int64_t t0 = first_key + (int64_t)t * kHalf;
                         from = lo > t0 ? (lo - t0 < kHalf ? (int)(lo - t0) : kHalf) : 0;
@@ -758,9 +766,6 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                         top = masked_top(s_at, from, to);
                     } else {
                         float m[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
-                        dev::tmem_ld_32x32b_x32(s_at, s[0]);
-                        dev::tmem_ld_32x32b_x32(s_at + 32, s[1]);
-                        dev::tmem_wait_ld();
                         fold_top(s[0], m);
                         fold_top(s[1], m);
                         top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
@@ -795,8 +800,16 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                         uint32_t pw[16];
                         fold_weights(s[0], f, shifted, part, pw);
                         dev::tmem_st_32x32b_x16(s_at, pw);
+                        if (t + 1 < halves) {
+                            fetched = __all_sync(kFull, dev::mbar_test(&sh->s_full[w][~t & 1], next_phase));
+                            if (fetched) {
+                                dev::tc_fence_after();
+                                dev::tmem_ld_32x32b_x32(s_next, s[0]);
+                            }
+                        }
                         fold_weights(s[1], f, shifted, part, pw);
                         dev::tmem_st_32x32b_x16(s_at + 16, pw);
+                        if (fetched) dev::tmem_ld_32x32b_x32(s_next + 32, s[1]);
                         dev::tmem_wait_st();
                         sum += up * ((part[0].x + part[0].y) + (part[1].x + part[1].y));
                     }
@@ -807,6 +820,15 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                     o_phase[1] ^= 1;
                 else
                     o_phase[0] ^= 1;
+                if (t + 1 < halves && !fetched) {
+                    if (!b.wait(&sh->s_full[w][~t & 1], next_phase)) return false;
+                    dev::tc_fence_after();
+                    if (warp_real) {
+                        dev::tmem_ld_32x32b_x32(s_next, s[0]);
+                        dev::tmem_ld_32x32b_x32(s_next + 32, s[1]);
+                    }
+                }
+                if (t & 1) s_phase ^= 1;
             }
 
             // The output row.
