@@ -32,6 +32,8 @@ int check_cache(const mxk_cache* c, const char* who) {
 
 namespace {
 
+constexpr int kWritePasses = 1, kReadPasses = 2;
+
 struct Side {
     uint8_t* values;
     uint8_t* scales;
@@ -42,238 +44,316 @@ struct Side {
 struct CacheMove {
     Side side[2];  // keys, values
     const int64_t* slots;
-    int64_t n_slots;
-    unsigned items;      // (token, side, head, chunk) of this launch
-    unsigned per_token;  // 2 * kv_heads * chunks
-    unsigned chunks;     // head_dim / 16
+    int64_t tokens, n_slots;
+    int chunks;      // 16-feature pieces of a row
+    int block_rows;  // tokens of one pass of a block
     int kv_heads, page_size;
 };
 
-// Where an item's 16 features lie: `data` in the caller's rows (in elements),
-// `row` the cached row's index ((page * kv_heads + head) * page_size + place).
-struct Item {
-    int side, chunk;
-    int64_t data, row, slot;
+// A block moves `passes` times block_rows tokens of head blockIdx.y, keys (blockIdx.z = 0)
+// or values; a thread the same 16-feature piece of as many rows, all requested before the
+// first is converted.
+struct Mover {
+    Side side;
+    int head, row, chunk;
+    bool active;
+    __device__ __forceinline__ explicit Mover(const CacheMove& m) {
+        side = blockIdx.z ? m.side[1] : m.side[0];
+        head = blockIdx.y;
+        row = (int)threadIdx.x / m.chunks;
+        chunk = (int)threadIdx.x - row * m.chunks;
+        active = row < m.block_rows;
+    }
+    __device__ __forceinline__ int64_t token(const CacheMove& m, int pass, int passes) const {
+        return ((int64_t)blockIdx.x * passes + pass) * m.block_rows + row;
+    }
+    // Piece number of a slot's row in the cache, -1 if the slot lies outside.
+    __device__ __forceinline__ int64_t piece(const CacheMove& m, int64_t slot) const {
+        if (slot < 0 || slot >= m.n_slots) return -1;
+        int64_t page;
+        int place;
+        if ((slot >> 31) == 0) {
+            const unsigned p = (unsigned)slot / (unsigned)m.page_size;
+            page = p;
+            place = (int)((unsigned)slot - p * (unsigned)m.page_size);
+        } else {
+            page = slot / m.page_size;
+            place = (int)(slot - page * m.page_size);
+        }
+        return ((page * m.kv_heads + head) * m.page_size + place) * m.chunks + chunk;
+    }
+    template <class T>
+    __device__ __forceinline__ T* rows(int64_t token) const {
+        return reinterpret_cast<T*>(side.data) + token * side.token_stride + (int64_t)head * side.head_stride +
+               chunk * 16;
+    }
 };
 
-__device__ __forceinline__ Item locate(const CacheMove& m, unsigned g) {
-    Item it;
-    const unsigned token = g / m.per_token;
-    const unsigned in = g - token * m.per_token;
-    const unsigned row = in / m.chunks;
-    it.chunk = (int)(in - row * m.chunks);
-    it.side = row >= (unsigned)m.kv_heads;
-    const int head = (int)row - (it.side ? m.kv_heads : 0);
-    it.slot = __ldg(m.slots + token);
-    const Side s = it.side ? m.side[1] : m.side[0];
-    it.data = (int64_t)token * s.token_stride + (int64_t)head * s.head_stride + it.chunk * 16;
-    int64_t page;
-    int place;
-    if ((it.slot >> 31) == 0) {
-        const unsigned p = (unsigned)it.slot / (unsigned)m.page_size;
-        page = p;
-        place = (int)((unsigned)it.slot - p * (unsigned)m.page_size);
-    } else {
-        page = it.slot / m.page_size;
-        place = (int)(it.slot - page * m.page_size);
-    }
-    it.row = (page * m.kv_heads + head) * m.page_size + place;
-    return it;
+// 32 bytes in one access (sm_100): a thread's 16 two-byte elements then are whole
+// sectors.  As two 16-byte accesses every sector is moved in two halves (prompt of
+// 16,384 tokens in bf16: 26.6 us instead of 22.5 to read back).
+__device__ __forceinline__ void load32(const void* p, uint4& a, uint4& b) {
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                 : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, uint4 a, uint4 b) {
+    asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+                 "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w), "l"(p)
+                 : "memory");
 }
 
-template <class T, bool VEC>
-__device__ __forceinline__ void load16(const T* p, float (&x)[16]) {
-    if constexpr (VEC) {
-        constexpr int n = 16 / sizeof(T);  // elements of one 16-byte load
+// 16 elements as they lie in memory.  VEC: bytes of one access, 0: one element.
+template <class T, int VEC>
+struct Raw16 {
+    uint4 w[sizeof(T)];  // 16 * sizeof(T) bytes
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (VEC == 32) {
 #pragma unroll
-        for (int i = 0; i < 16 / n; ++i) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(p) + i);
-            T e[n];
-            memcpy(e, &w, 16);
+            for (int i = 0; i < (int)sizeof(T); i += 2) load32(reinterpret_cast<const uint4*>(p) + i, w[i], w[i + 1]);
+        } else if constexpr (VEC == 16) {
 #pragma unroll
-            for (int j = 0; j < n; ++j) x[i * n + j] = dev::to_float(e[j]);
+            for (int i = 0; i < (int)sizeof(T); ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        } else {
+            T e[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) e[i] = p[i];
+            memcpy(w, e, sizeof(w));
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = dev::to_float(p[i]);
     }
-}
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (VEC == 32) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T); i += 2) store32(reinterpret_cast<uint4*>(p) + i, w[i], w[i + 1]);
+        } else if constexpr (VEC == 16) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+        } else {
+            T e[16];
+            memcpy(e, w, sizeof(w));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = e[i];
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void to_float(float (&x)[16]) const {
+        T e[16];
+        memcpy(e, w, sizeof(w));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = dev::to_float(e[i]);
+    }
+    __device__ __forceinline__ void from_float(const float (&x)[16]) {
+        T e[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) e[i] = dev::from_float<T>(x[i]);
+        memcpy(w, e, sizeof(w));
+    }
+};
 
-template <class T, bool VEC>
-__device__ __forceinline__ void store16(T* p, const float (&x)[16]) {
-    if constexpr (VEC) {
-        constexpr int n = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < 16 / n; ++i) {
-            T e[n];
-#pragma unroll
-            for (int j = 0; j < n; ++j) e[j] = dev::from_float<T>(x[i * n + j]);
-            uint4 w;
-            memcpy(&w, e, 16);
-            reinterpret_cast<uint4*>(p)[i] = w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = dev::from_float<T>(x[i]);
-    }
+// The largest of three, NaN if one is NaN.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 // The hardware conversions round to nearest even and saturate as quantize_rows
 // does.  Below 8 bits a NaN becomes the largest magnitude with the NaN's sign
-// there, which the conversions do not promise, so it is replaced first.
-__device__ __forceinline__ float nan_to_most(float x, float most) { return x == x ? x : copysignf(most, x); }
+// there, which the conversions do not promise, so the caller replaces NaNs first.
 
 // Two E2M3 codes, one byte each, `lo` in the low byte.
 __device__ __forceinline__ uint32_t e2m3x2_pack(float lo, float hi) {
     uint16_t out;
-    asm("cvt.rn.satfinite.e2m3x2.f32 %0, %1, %2;"
-        : "=h"(out)
-        : "f"(nan_to_most(hi, 7.5f)), "f"(nan_to_most(lo, 7.5f)));
+    asm("cvt.rn.satfinite.e2m3x2.f32 %0, %1, %2;" : "=h"(out) : "f"(hi), "f"(lo));
     return out;
 }
 
 // Eight E2M1 codes, x[0] in the lowest nibble.
 __device__ __forceinline__ uint32_t e2m1x8_pack(const float* x) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = nan_to_most(x[i], 6.0f);
     uint32_t out;
     asm("{\n\t.reg .b8 a, b, c, d;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
         "mov.b32 %0, {a, b, c, d};\n\t}"
         : "=r"(out)
-        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+        : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
     return out;
 }
 
-template <int BITS, class T, bool VEC>
+template <int BITS, class T, int VEC>
 __global__ void __launch_bounds__(256) cache_write_kernel(const CacheMove m) {
-    const unsigned g = blockIdx.x * 256u + threadIdx.x;
-    const bool in_range = g < m.items;
-    const Item it = locate(m, in_range ? g : 0u);
-    // A pair of threads shares a token, so both leave the block's maximum alike.
-    const bool valid = in_range && it.slot >= 0 && it.slot < m.n_slots;
-    const Side s = it.side ? m.side[1] : m.side[0];
-    float x[16];
-    if (valid) {
-        load16<T, VEC>(reinterpret_cast<const T*>(s.data) + it.data, x);
-    } else {
+    constexpr int kPasses = kWritePasses;
+    const Mover mv(m);
+    int64_t at[kPasses];
+    Raw16<T, VEC> raw[kPasses];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+    for (int i = 0; i < kPasses; ++i) {
+        const int64_t token = mv.token(m, i, kPasses);
+        at[i] = mv.active && token < m.tokens ? mv.piece(m, __ldg(m.slots + token)) : -1;
+        if (at[i] >= 0)
+            raw[i].load(mv.template rows<const T>(token));
+        else
+            raw[i].zero();
     }
-    float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    if (!valid) return;
-    uint32_t e;
-    if constexpr (BITS == 8)
-        e = dev::ue8m0_mxfp8_scale(amax);
-    else
-        e = dev::ue8m0_encode(amax > 0.0f ? amax / (BITS == 6 ? 7.5f : 6.0f) : 1.0f);
-    const float rcp = dev::ue8m0_reciprocal(e);
+    for (int i = 0; i < kPasses; ++i) {
+        float x[16];
+        raw[i].to_float(x);
+        // The block's largest magnitude, NaN if it holds one: then once more without it.
+        // (The two pieces of a block share the token, so both are kept or neither.)
+        float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] *= rcp;  // the exact quotient by a power of two
-    const int64_t at = it.row * m.chunks + it.chunk;  // in units of 16 features
-    if constexpr (BITS == 8) {
-        uint32_t w[4];
+        for (int k = 0; k < 16; k += 2) amax = max3_nan(amax, fabsf(x[k]), fabsf(x[k + 1]));
+        amax = max3_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1), 0.0f);
+        const bool nans = amax != amax;
+        if (nans) {
+            amax = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = dev::e4m3x2_encode(x[4 * i], x[4 * i + 1]) | (dev::e4m3x2_encode(x[4 * i + 2], x[4 * i + 3]) << 16);
-        reinterpret_cast<uint4*>(s.values)[at] = make_uint4(w[0], w[1], w[2], w[3]);
-    } else if constexpr (BITS == 6) {
-        // four 6-bit codes in three bytes, lowest first
-        uint32_t v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t a = e2m3x2_pack(x[4 * i], x[4 * i + 1]), b = e2m3x2_pack(x[4 * i + 2], x[4 * i + 3]);
-            v[i] = (a & 0x3fu) | ((a >> 2) & 0xfc0u) | ((b & 0x3fu) << 12) | ((b & 0x3f00u) << 10);
+            for (int k = 0; k < 16; ++k) amax = fmaxf(amax, fabsf(x[k]));
+            amax = fmaxf(amax, __shfl_xor_sync(3u << (threadIdx.x & 30u), amax, 1));
         }
-        uint32_t* out = reinterpret_cast<uint32_t*>(s.values) + at * 3;
-        out[0] = v[0] | (v[1] << 24);
-        out[1] = (v[1] >> 8) | (v[2] << 16);
-        out[2] = (v[2] >> 16) | (v[3] << 8);
-    } else {
-        // low nibble = even feature
-        reinterpret_cast<uint2*>(s.values)[at] = make_uint2(e2m1x8_pack(x), e2m1x8_pack(x + 8));
+        if (at[i] < 0) continue;
+        uint32_t e;
+        if constexpr (BITS == 8)
+            e = dev::ue8m0_mxfp8_scale(amax);
+        else
+            e = dev::ue8m0_encode(amax > 0.0f ? amax / (BITS == 6 ? 7.5f : 6.0f) : 1.0f);
+        const float rcp = dev::ue8m0_reciprocal(e);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[k] *= rcp;  // the exact quotient by a power of two
+        if (BITS < 8 && nans) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[k] = x[k] == x[k] ? x[k] : copysignf(BITS == 6 ? 7.5f : 6.0f, x[k]);
+        }
+        if constexpr (BITS == 8) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                w[k] = dev::e4m3x2_encode(x[4 * k], x[4 * k + 1]) |
+                       (dev::e4m3x2_encode(x[4 * k + 2], x[4 * k + 3]) << 16);
+            reinterpret_cast<uint4*>(mv.side.values)[at[i]] = make_uint4(w[0], w[1], w[2], w[3]);
+        } else if constexpr (BITS == 6) {
+            // four 6-bit codes in three bytes, lowest first
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t a = e2m3x2_pack(x[4 * k], x[4 * k + 1]), b = e2m3x2_pack(x[4 * k + 2], x[4 * k + 3]);
+                v[k] = (a & 0x3fu) | ((a >> 2) & 0xfc0u) | ((b & 0x3fu) << 12) | ((b & 0x3f00u) << 10);
+            }
+            uint32_t* out = reinterpret_cast<uint32_t*>(mv.side.values) + at[i] * 3;
+            out[0] = v[0] | (v[1] << 24);
+            out[1] = (v[1] >> 8) | (v[2] << 16);
+            out[2] = (v[2] >> 16) | (v[3] << 8);
+        } else {
+            // low nibble = even feature
+            reinterpret_cast<uint2*>(mv.side.values)[at[i]] = make_uint2(e2m1x8_pack(x), e2m1x8_pack(x + 8));
+        }
+        if ((mv.chunk & 1) == 0) mv.side.scales[at[i] >> 1] = (uint8_t)e;
     }
-    if ((it.chunk & 1) == 0) s.scales[at >> 1] = (uint8_t)e;
 }
 
-template <int BITS, class T, bool VEC>
+template <int BITS, class T, int VEC>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheMove m) {
-    const unsigned g = blockIdx.x * 256u + threadIdx.x;
-    if (g >= m.items) return;
-    const Item it = locate(m, g);
-    const Side s = it.side ? m.side[1] : m.side[0];
-    float x[16];
-    if (it.slot >= 0 && it.slot < m.n_slots) {
-        const int64_t at = it.row * m.chunks + it.chunk;
-        uint32_t h2[8];  // the 16 elements
-        if constexpr (BITS == 8) {
-            const uint4 w = reinterpret_cast<const uint4*>(s.values)[at];
-            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    constexpr int kPasses = kReadPasses;
+    const Mover mv(m);
+    if (!mv.active) return;
+    int64_t at[kPasses];
+    uint32_t codes[kPasses][BITS / 2];
+    uint32_t scales[kPasses];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                h2[2 * i] = dev::codes_to_f16x2<8>(v[i]);
-                h2[2 * i + 1] = dev::codes_to_f16x2<8>(v[i] >> 16);
-            }
-        } else if constexpr (BITS == 6) {
-            const uint32_t* p = reinterpret_cast<const uint32_t*>(s.values) + at * 3;
-            const uint32_t a = p[0], b = p[1], c = p[2];
-            const uint32_t v[4] = {a, (a >> 24) | (b << 8), (b >> 16) | (c << 16), c >> 8};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t w = dev::spread6(v[i]);
-                h2[2 * i] = dev::codes_to_f16x2<6>(w);
-                h2[2 * i + 1] = dev::codes_to_f16x2<6>(w >> 16);
-            }
-        } else {
-            const uint2 w = reinterpret_cast<const uint2*>(s.values)[at];
-            uint32_t lo[4], hi[4];
-            dev::e2m1x8_to_f16(w.x, lo);
-            dev::e2m1x8_to_f16(w.y, hi);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) h2[i] = lo[i], h2[4 + i] = hi[i];
-        }
-        const float scale = dev::ue8m0_value(s.scales[at >> 1]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2[i]));
-            x[2 * i] = f.x * scale, x[2 * i + 1] = f.y * scale;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+    for (int i = 0; i < kPasses; ++i) {
+        const int64_t token = mv.token(m, i, kPasses);
+        at[i] = token < m.tokens ? mv.piece(m, __ldg(m.slots + token)) : -1;
     }
-    store16<T, VEC>(reinterpret_cast<T*>(s.data) + it.data, x);
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+#pragma unroll
+        for (int k = 0; k < BITS / 2; ++k) codes[i][k] = 0;
+        scales[i] = 127;
+        if (at[i] < 0) continue;
+        if constexpr (BITS == 8) {
+            const uint4 w = reinterpret_cast<const uint4*>(mv.side.values)[at[i]];
+            codes[i][0] = w.x, codes[i][1] = w.y, codes[i][2] = w.z, codes[i][3] = w.w;
+        } else if constexpr (BITS == 6) {
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(mv.side.values) + at[i] * 3;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) codes[i][k] = p[k];
+        } else {
+            const uint2 w = reinterpret_cast<const uint2*>(mv.side.values)[at[i]];
+            codes[i][0] = w.x, codes[i][1] = w.y;
+        }
+        scales[i] = mv.side.scales[at[i] >> 1];
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const int64_t token = mv.token(m, i, kPasses);
+        if (token >= m.tokens) break;
+        uint32_t h2[8];  // the 16 elements
+        if constexpr (BITS == 4) {
+            uint32_t lo[4], hi[4];
+            dev::e2m1x8_to_f16(codes[i][0], lo);
+            dev::e2m1x8_to_f16(codes[i][1], hi);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) h2[k] = lo[k], h2[4 + k] = hi[k];
+        } else {
+            constexpr int kCode = BITS == 4 ? 8 : BITS;
+            uint32_t v[4];
+            if constexpr (BITS == 8) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = codes[i][k];
+            } else {
+                const uint32_t a = codes[i][0], b = codes[i][1], c = codes[i][2];
+                v[0] = dev::spread6(a), v[1] = dev::spread6((a >> 24) | (b << 8));
+                v[2] = dev::spread6((b >> 16) | (c << 16)), v[3] = dev::spread6(c >> 8);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                h2[2 * k] = dev::codes_to_f16x2<kCode>(v[k]);
+                h2[2 * k + 1] = dev::codes_to_f16x2<kCode>(v[k] >> 16);
+            }
+        }
+        const float scale = dev::ue8m0_value(scales[i]);
+        float x[16];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2[k]));
+            x[2 * k] = f.x * scale, x[2 * k + 1] = f.y * scale;
+        }
+        Raw16<T, VEC> out;
+        out.from_float(x);
+        out.store(mv.template rows<T>(token));
+    }
+}
+
+template <bool WRITE, int BITS, class T, int VEC>
+int launch_vec(const CacheMove& m, cudaStream_t stream) {
+    const int64_t block_tokens = (int64_t)m.block_rows * (WRITE ? kWritePasses : kReadPasses);
+    const int64_t blocks = (m.tokens + block_tokens - 1) / block_tokens;
+    MXK_REQUIRE(blocks <= std::numeric_limits<int>::max(), "cache: too many tokens for one call");
+    const dim3 grid((unsigned)blocks, (unsigned)m.kv_heads, 2);
+    if constexpr (WRITE)
+        cache_write_kernel<BITS, T, VEC><<<grid, 256, 0, stream>>>(m);
+    else
+        cache_read_kernel<BITS, T, VEC><<<grid, 256, 0, stream>>>(m);
+    MXK_CUDA(cudaGetLastError());
+    return MXK_OK;
 }
 
 template <bool WRITE, int BITS, class T>
-void launch_typed(const CacheMove& m, bool vec, cudaStream_t stream) {
-    const unsigned blocks = (m.items + 255u) / 256u;
-    if constexpr (WRITE) {
-        if (vec)
-            cache_write_kernel<BITS, T, true><<<blocks, 256, 0, stream>>>(m);
-        else
-            cache_write_kernel<BITS, T, false><<<blocks, 256, 0, stream>>>(m);
-    } else {
-        if (vec)
-            cache_read_kernel<BITS, T, true><<<blocks, 256, 0, stream>>>(m);
-        else
-            cache_read_kernel<BITS, T, false><<<blocks, 256, 0, stream>>>(m);
-    }
+int launch_typed(const CacheMove& m, int vec, cudaStream_t stream) {
+    if (vec == 32) return launch_vec<WRITE, BITS, T, 32>(m, stream);
+    if (vec == 16) return launch_vec<WRITE, BITS, T, 16>(m, stream);
+    return launch_vec<WRITE, BITS, T, 0>(m, stream);
 }
 
 template <bool WRITE, int BITS>
-void launch_bits(const CacheMove& m, int dtype, bool vec, cudaStream_t stream) {
-    if (dtype == MXK_F32)
-        launch_typed<WRITE, BITS, float>(m, vec, stream);
-    else if (dtype == MXK_F16)
-        launch_typed<WRITE, BITS, __half>(m, vec, stream);
-    else
-        launch_typed<WRITE, BITS, __nv_bfloat16>(m, vec, stream);
+int launch_bits(const CacheMove& m, int dtype, int vec, cudaStream_t stream) {
+    if (dtype == MXK_F32) return launch_typed<WRITE, BITS, float>(m, vec, stream);
+    if (dtype == MXK_F16) return launch_typed<WRITE, BITS, __half>(m, vec, stream);
+    return launch_typed<WRITE, BITS, __nv_bfloat16>(m, vec, stream);
 }
 
 template <bool WRITE>
@@ -290,36 +370,24 @@ int cache_move(const char* who, const mxk_cache* c, int dtype, int64_t tokens, c
                     reinterpret_cast<uintptr_t>(slots) % 8 == 0,
                 w + ": k, v and slots must be aligned to their elements");
     CacheMove m{};
-    m.chunks = (unsigned)c->head_dim / 16u;
-    m.per_token = 2u * (unsigned)c->kv_heads * m.chunks;
+    const mxk_rows* rows[2] = {k, v};
+    for (int i = 0; i < 2; ++i)
+        m.side[i] = {static_cast<uint8_t*>(i ? c->v_values : c->k_values), i ? c->v_scales : c->k_scales,
+                     static_cast<char*>(rows[i]->data), rows[i]->token_stride, rows[i]->head_stride};
+    m.slots = slots;
+    m.tokens = tokens;
+    m.n_slots = cache_slots(*c);
+    m.chunks = c->head_dim / 16;
+    m.block_rows = 256 / m.chunks;
     m.kv_heads = c->kv_heads;
     m.page_size = c->page_size;
-    m.n_slots = cache_slots(*c);
-    const bool vec = rows_aligned(*k, size, 16) && rows_aligned(*v, size, 16);
-    // item numbers are 32 bits: more tokens go in several launches
-    const int64_t most = (int64_t)(0x7fffff00u / m.per_token);
-    for (int64_t first = 0; first < tokens; first += most) {
-        const int64_t n = tokens - first < most ? tokens - first : most;
-        const mxk_rows* rows[2] = {k, v};
-        for (int i = 0; i < 2; ++i) {
-            m.side[i].values = static_cast<uint8_t*>(i ? c->v_values : c->k_values);
-            m.side[i].scales = i ? c->v_scales : c->k_scales;
-            m.side[i].data = static_cast<char*>(rows[i]->data) + first * rows[i]->token_stride * size;
-            m.side[i].token_stride = rows[i]->token_stride;
-            m.side[i].head_stride = rows[i]->head_stride;
-        }
-        m.slots = slots + first;
-        m.items = (unsigned)n * m.per_token;
-        LaunchScope scope(WRITE ? "cache_write" : "cache_read", stream);
-        if (c->bits == 8)
-            launch_bits<WRITE, 8>(m, dtype, vec, stream);
-        else if (c->bits == 6)
-            launch_bits<WRITE, 6>(m, dtype, vec, stream);
-        else
-            launch_bits<WRITE, 4>(m, dtype, vec, stream);
-        MXK_CUDA(cudaGetLastError());
-    }
-    return MXK_OK;
+    const int vec = rows_aligned(*k, size, 32) && rows_aligned(*v, size, 32)   ? 32
+                    : rows_aligned(*k, size, 16) && rows_aligned(*v, size, 16) ? 16
+                                                                               : 0;
+    LaunchScope scope(WRITE ? "cache_write" : "cache_read", stream);
+    if (c->bits == 8) return launch_bits<WRITE, 8>(m, dtype, vec, stream);
+    if (c->bits == 6) return launch_bits<WRITE, 6>(m, dtype, vec, stream);
+    return launch_bits<WRITE, 4>(m, dtype, vec, stream);
 }
 
 }  // namespace
