@@ -157,12 +157,12 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
 
     const dev::Share share = dev::take_share<kRows, kKeys, kThreads>(p, scratch);
     if (share.tiles == 0) {
-        if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0), p.part_ends[blockIdx.x] = 0;
+        if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
         return;
     }
     dev::Walk w = dev::walk_to<kRows, kKeys>(p, share.seq, share.offset);
     int64_t left = share.tiles;
-    bool open = false, went_on = false, ended = false;
+    bool open = false;
 
     while (left > 0) {
         const int tile0 = w.tile;
@@ -541,28 +541,22 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
                 if (chunk == 0) p.part_stat[slot * kRows + r] = make_float2(top, total);
             }
         }
-        if (!whole) {
-            if (tile0 == 0) {
-                open = true;
-                if (tid == 0) p.part_open[blockIdx.x] = make_int4(w.seq, w.rt, w.head, 1);
-            } else {
-                went_on = true;
-                ended = tile0 + tiles == w.tiles;
-            }
+        if (!whole && tile0 == 0) {
+            open = true;
+            if (tid == 0)
+                p.part_open[blockIdx.x] =
+                    make_int4(w.seq, w.rt, w.head, share.followers(share.tiles - left, w.tiles));
         }
         __syncthreads();  // before the rings are filled again
         left -= tiles;
         w.tile += tiles;
         if (left > 0) dev::walk_on<kRows, kKeys>(p, w);
     }
-    if (tid == 0) {
-        if (!open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
-        p.part_ends[blockIdx.x] = went_on && ended ? 1 : 0;
-    }
+    if (tid == 0 && !open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
 }
 
 template <int D, int BITS>
-int launch_rows(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
+int launch_rows(AttentionParams p, int64_t most_tiles, int64_t most_rows, cudaStream_t stream) {
     using S = Stage<D, BITS>;
     static thread_local int ready_device = -1;
     int dev = 0;
@@ -581,14 +575,14 @@ int launch_rows(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
         attention_rows_kernel<D, BITS><<<(unsigned)ctas, kThreads, S::smem, stream>>>(p);
         MXK_CUDA(cudaGetLastError());
     }
-    return join_parts<kRows, D>(p, (int)ctas, 4, stream);
+    return join_parts<kRows, D>(p, (int)ctas, (int)(most_rows < kRows ? most_rows : kRows), stream);
 }
 
 template <int D>
-int launch_rows_bits(int bits, const AttentionParams& p, int64_t most_tiles, cudaStream_t stream) {
-    if (bits == 8) return launch_rows<D, 8>(p, most_tiles, stream);
-    if (bits == 6) return launch_rows<D, 6>(p, most_tiles, stream);
-    return launch_rows<D, 4>(p, most_tiles, stream);
+int launch_rows_bits(int bits, const AttentionParams& p, int64_t most_tiles, int64_t most_rows, cudaStream_t stream) {
+    if (bits == 8) return launch_rows<D, 8>(p, most_tiles, most_rows, stream);
+    if (bits == 6) return launch_rows<D, 6>(p, most_tiles, most_rows, stream);
+    return launch_rows<D, 4>(p, most_tiles, most_rows, stream);
 }
 
 }  // namespace
@@ -667,6 +661,6 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     }
     const int few_q = rows > kMostFewRows ? (kMostFewRows + p.group - 1) / p.group : a->max_q;
     const int64_t most = attention_tile_bound(p, few_q, kRows, kKeys);
-    return cache->head_dim == 128 ? launch_rows_bits<128>(cache->bits, p, most, st)
-                                  : launch_rows_bits<64>(cache->bits, p, most, st);
+    return cache->head_dim == 128 ? launch_rows_bits<128>(cache->bits, p, most, rows, st)
+                                  : launch_rows_bits<64>(cache->bits, p, most, rows, st);
 }

@@ -44,8 +44,8 @@ struct AttentionParams {
     // partial sums
     float* part;  // [2 * CTAs][tile rows][head_dim]
     float2* part_stat;  // [2 * CTAs][tile rows]: running maximum (log2 units), sum
-    int4* part_open;    // [CTAs]: {sequence, row tile, key head, 1} of the unit begun and left unfinished, or {.., 0}
-    int* part_ends;     // [CTAs]: 1 if the unit that the CTA went on with ends in it
+    int4* part_open;    // [CTAs]: {sequence, row tile, key head, n} of the unit that the CTA began and the n
+                        // following ones went on with; n = 0: it left none unfinished
     // keys and values converted beforehand (tiles kernel), [seqs][kv_heads][max_tiles]
     uint8_t* ready_k;
     uint8_t* ready_v;
@@ -167,6 +167,15 @@ struct Share {
     int64_t tiles;   // of this CTA
     int seq;         // first sequence of the share
     int64_t offset;  // of the share's first tile in that sequence
+    int64_t begin;   // the share's first tile among all,
+    int64_t total;   // of so many,
+    int64_t ctas;    // for so many CTAs
+
+    // CTAs after this one that work on a unit of n tiles whose first is `at` of the share.
+    __device__ __forceinline__ int followers(int64_t at, int64_t n) const {
+        const int64_t last = begin + at + n - 1;  // tile x belongs to CTA ceil((x + 1) ctas / total) - 1
+        return (int)(((last + 1) * ctas + total - 1) / total - 1 - blockIdx.x);
+    }
 };
 
 // All threads of the CTA; scratch: THREADS / 32 + 4 words of shared memory.
@@ -187,10 +196,11 @@ __device__ __forceinline__ Share take_share(const AttentionParams& p, int64_t* s
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) total += scratch[w];
     const int64_t ctas = total < gridDim.x ? total : gridDim.x;
-    Share s{0, 0, 0};
+    Share s{0, 0, 0, 0, total, ctas};
     if ((int64_t)blockIdx.x >= ctas) return s;
     const int64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
     s.tiles = end - begin;
+    s.begin = begin;
     int64_t before = 0;  // tiles of the sequences before this round's
     for (int base = 0; base < p.seqs; base += THREADS) {
         const int i = base + tid;
@@ -295,41 +305,64 @@ __device__ __forceinline__ float row_lse(float m2, float sum) {
 
 }  // namespace dev
 
-// Block (x, y): the unit that CTA x began and did not finish, rows y, y + gridDim.y, ...;
-// a thread owns four features.  The parts are the beginning (slot 2x + 1) and what
-// the following CTAs did first (slots 2j), up to the one that finished the unit.
+// Block (x, y): the unit that CTA x began and did not finish, rows y, y + gridDim.y, ...
+// Its parts are the beginning (slot 2x + 1) and what the following CTAs did first (slots
+// 2j).  The four warps take every fourth part (with D = 64 every half-warp every eighth),
+// so a unit in hundreds of parts has several rows of loads under way, and add up in a
+// fixed order.
 template <int ROWS, int D>
 __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionParams p) {
-    constexpr int kLanes = D / 4;              // threads of a row
-    constexpr int kSub = 128 / kLanes;         // rows at a time
+    constexpr int kLanes = D / 4;            // threads of a row
+    constexpr int kSub = 128 / kLanes;       // parts at a time
+    __shared__ float4 sums[kSub][kLanes];
+    __shared__ float stats[4], sub_totals[kSub];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 unit = p.part_open[blockIdx.x];
     if (!unit.w) return;
-    int last = blockIdx.x + 1;
-    while (last < (int)gridDim.x - 1 && !p.part_ends[last]) ++last;
     const dev::SeqView view = dev::seq_view(p, unit.x);
     const int rows = view.n * p.group - unit.y * ROWS < ROWS ? view.n * p.group - unit.y * ROWS : ROWS;
-    const int chunk = threadIdx.x % kLanes;
-    for (int r = blockIdx.y * kSub + threadIdx.x / kLanes; r < rows; r += gridDim.y * kSub) {
-        int64_t slot = 2 * (int64_t)blockIdx.x + 1;
-        float top = p.part_stat[slot * ROWS + r].x;
-        for (int j = blockIdx.x + 1; j <= last; ++j) top = fmaxf(top, p.part_stat[2 * (int64_t)j * ROWS + r].x);
+    const int tid = threadIdx.x, chunk = tid % kLanes, sub = tid / kLanes, parts = unit.w + 1;
+    auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(blockIdx.x + i) + (i == 0 ? 1 : 0); };
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        // the common maximum and the sum
+        float top = __int_as_float(0xff800000);
+        for (int i = tid; i < parts; i += 128) top = fmaxf(top, p.part_stat[slot(i) * ROWS + r].x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if ((tid & 31) == 0) stats[tid >> 5] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(stats[0], stats[1]), fmaxf(stats[2], stats[3]));
         float total = 0.0f;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int j = blockIdx.x; j <= last; ++j) {
-            if (j > (int)blockIdx.x) slot = 2 * (int64_t)j;
-            const float2 st = p.part_stat[slot * ROWS + r];
+#pragma unroll 4
+        for (int i = sub; i < parts; i += kSub) {
+            const float2 st = p.part_stat[slot(i) * ROWS + r];
+            const float4 x = reinterpret_cast<const float4*>(p.part + (slot(i) * ROWS + r) * D)[chunk];
             const float f = st.x == top ? 1.0f : dev::ex2(st.x - top);
-            const float4 x = reinterpret_cast<const float4*>(p.part + (slot * ROWS + r) * D)[chunk];
             total += st.y * f;
             v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
         }
-        const int row = unit.y * ROWS + r, j = row / p.group;
-        const int head = unit.z * p.group + (row - j * p.group);
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        dev::store4(p, view.row0 + j, head, chunk * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-        if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
+        sums[sub][chunk] = v;
+        // every thread of a sub has the same total
+        if (chunk == 0) sub_totals[sub] = total;
+        __syncthreads();
+        if (tid < kLanes) {
+            total = 0.0f;
+            v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < kSub; ++i) {
+                const float4 x = sums[i][chunk];
+                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                total += sub_totals[i];
+            }
+            const int row = unit.y * ROWS + r, j = row / p.group;
+            const int head = unit.z * p.group + (row - j * p.group);
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            dev::store4(p, view.row0 + j, head, chunk * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+            if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
+        }
+        __syncthreads();  // before the shared sums are written again
     }
 }
 
@@ -347,7 +380,7 @@ struct Workspace {
     // extra: bytes at `extra`, 256-byte aligned.
     int take(AttentionParams& p, int64_t ctas, int rows, int d, int64_t extra_bytes = 0) {
         const size_t part = (size_t)(2 * ctas * rows) * d * 4, stat = (size_t)(2 * ctas * rows) * 8;
-        const size_t own = (part + stat + (size_t)ctas * 20 + 255) / 256 * 256;
+        const size_t own = (part + stat + (size_t)ctas * 16 + 255) / 256 * 256;
         cudaMemPool_t pool = workspace_pool();
         if (!pool) return fail(MXK_ERR_CUDA, "cache_attention: cannot create the workspace pool");
         MXK_CUDA(cudaMallocFromPoolAsync(&ptr, own + (size_t)extra_bytes, pool, stream));
@@ -355,7 +388,6 @@ struct Workspace {
         p.part = static_cast<float*>(ptr);
         p.part_stat = reinterpret_cast<float2*>(static_cast<char*>(ptr) + part);
         p.part_open = reinterpret_cast<int4*>(static_cast<char*>(ptr) + part + stat);
-        p.part_ends = reinterpret_cast<int*>(p.part_open + ctas);
         return MXK_OK;
     }
 };

@@ -100,6 +100,7 @@ struct Block {
     Shared* sh;
     uint32_t tmem;
     unsigned* err;
+    dev::Share share;
     __device__ __forceinline__ volatile int* abort_flag() const { return &sh->abort_word; }
     // Bounded wait of a whole warp; false: it gave up, leave for the end of the kernel.
     __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
@@ -710,7 +711,8 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
     // the scores of a half follow the products of the half before the last.
     uint32_t s_phase = 0, o_phase[2] = {0, 0};
     int meta_at = 0;
-    bool open = false, went_on = false, ended = false;
+    bool open = false;
+    const int64_t share = c.left;
     do {
         const int rows = c.rows(p);
         if (w * kTileRows < rows) {
@@ -884,20 +886,14 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             dev::tc_fence_before();
         }
         meta_at += c.tiles;
-        if (!c.whole()) {
-            if (c.tile0 == 0) {
-                open = true;
-                if (threadIdx.x == 0) p.part_open[blockIdx.x] = make_int4(c.w.seq, c.w.rt, c.w.head, 1);
-            } else {
-                went_on = true;
-                ended = c.tile0 + c.tiles == c.w.tiles;
-            }
+        if (!c.whole() && c.tile0 == 0) {
+            open = true;
+            if (threadIdx.x == 0)
+                p.part_open[blockIdx.x] =
+                    make_int4(c.w.seq, c.w.rt, c.w.head, b.share.followers(share - c.left, c.w.tiles));
         }
     } while (c.next(p));
-    if (threadIdx.x == 0) {
-        if (!open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
-        p.part_ends[blockIdx.x] = went_on && ended ? 1 : 0;
-    }
+    if (threadIdx.x == 0 && !open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
     return true;
 }
 
@@ -910,7 +906,7 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
     const int tid = threadIdx.x;
     const dev::Share share = dev::take_share<kRows, kKeys, Cfg::threads>(p, scratch);
     if (share.tiles == 0) {
-        if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0), p.part_ends[blockIdx.x] = 0;
+        if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
         return false;
     }
     if (tid == 0) {
@@ -944,6 +940,7 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
     b.sh = sh;
     b.tmem = __shfl_sync(kFull, sh->tmem, 0);
     b.err = err;
+    b.share = share;
     c.w = dev::walk_to<kRows, kKeys>(p, share.seq, share.offset);
     c.left = share.tiles;
     c.unit = 0;
@@ -958,7 +955,7 @@ __device__ __forceinline__ void finish(const AttentionParams& p, const Block& b)
     if (threadIdx.x < 32) dev::tmem_dealloc(b.tmem, 512);
     // After a wait gave up nothing of this CTA is joined.
     if (threadIdx.x == 0 && *b.abort_flag())
-        p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0), p.part_ends[blockIdx.x] = 1;
+        p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
 }
 
 template <int D, int BITS>
@@ -1037,7 +1034,7 @@ int launch_packed(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
         attention_tiles_kernel<D, BITS><<<(unsigned)ctas, Packed::threads, Smem<D>::total, stream>>>(p, err);
         MXK_CUDA(cudaGetLastError());
     }
-    return join_parts<kRows, D>(p, (int)ctas, 32, stream);
+    return join_parts<kRows, D>(p, (int)ctas, 64, stream);
 }
 
 template <int D, int BITS>
@@ -1073,7 +1070,7 @@ int launch_ready(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
         LaunchScope scope("attention_ready", stream);
         MXK_CUDA(cudaLaunchKernelEx(&cfg, attention_ready_kernel<D>, p, err));
     }
-    return join_parts<kRows, D>(p, (int)ctas, 32, stream);
+    return join_parts<kRows, D>(p, (int)ctas, 64, stream);
 }
 
 template <int D, int BITS>

@@ -117,9 +117,9 @@ SIGNATURES = {
     "mxk_host_read_points_ex": ([ctypes.c_char_p, _I64, _I, _I, _I, _I64, _P], _I),
     "mxk_host_read_points_f32": ([ctypes.c_char_p, _I64, _I, _I, _P], _I),
     "mxk_host_write_labels": ([ctypes.c_char_p, _P, _I64], _I),
-    "mxk_cache_write": ([ctypes.POINTER(Cache), _I, _I64, ctypes.POINTER(Rows), ctypes.POINTER(Rows), _P, _P], _I),
-    "mxk_cache_read": ([ctypes.POINTER(Cache), _I, _I64, _P, ctypes.POINTER(Rows), ctypes.POINTER(Rows), _P], _I),
-    "mxk_cache_attention": ([ctypes.POINTER(Cache), ctypes.POINTER(Attention), _P], _I),
+    "mxk_cache_write": ([_P, _I, _I64, _P, _P, _P, _P], _I),
+    "mxk_cache_read": ([_P, _I, _I64, _P, _P, _P, _P], _I),
+    "mxk_cache_attention": ([_P, _P, _P], _I),
     "mxk_profile_enable": ([_I], _I),
     "mxk_profile_read": ([ctypes.POINTER(KernelStat), _I, ctypes.POINTER(_I)], _I),
 }
@@ -360,13 +360,48 @@ def kmeans_mixed_sharded(comm, points, centroids, labels, options=None, stream=N
 
 
 # ----------------------------------------------------------------------------- paged MX cache
+# These calls sit on a serving loop's critical path, where a few microseconds of
+# checks are a share of the step: each attribute of a tensor is looked at once.
 
-def _tensor(t, name, dtype, *shape):
-    """t as named: a CUDA tensor of `dtype` with `shape` (None: any size)."""
-    if not t.is_cuda or t.dtype != dtype or t.dim() != len(shape) or any(
-            n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise MxkInvalidArgument(ERR_INVALID, f"{name}: a CUDA {dtype} tensor of shape {shape} is needed, got "
-                                              f"{t.device} {t.dtype} {tuple(t.shape)}")
+def _bad(message):
+    return MxkInvalidArgument(ERR_INVALID, message)
+
+
+_torch = None
+_DTYPES = {}
+
+
+def _setup():
+    global _torch
+    import torch
+    _torch = torch
+    _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+
+
+def _launch_stream(cache, stream):
+    """Handle of the stream to launch on: the caller's or the current one of the cache's
+    device, which must be the current device."""
+    index = cache.index
+    if _torch._C._cuda_getDevice() != index:
+        raise _bad(f"the cache is on cuda:{index}, which is not the current device")
+    return stream.cuda_stream if stream is not None else _torch._C._cuda_getCurrentRawStream(index)
+
+
+def _vector(t, name, cache, dtype, *shape):
+    """Address of t, a contiguous tensor of `dtype` and `shape` on the cache's device."""
+    if t.dtype != dtype or tuple(t.shape) != shape or t.get_device() != cache.index or not t.is_contiguous():
+        raise _bad(f"{name}: a contiguous {dtype} tensor of shape {shape} on {cache.device} is needed, got {t.device} "
+                   f"{t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _rows(t, name, cache, tokens, heads):
+    """mxk_rows of t [tokens, heads, head_dim], whose features must be contiguous."""
+    strides = t.stride()
+    if tuple(t.shape) != (tokens, heads, cache.head_dim) or t.get_device() != cache.index or strides[2] != 1:
+        raise _bad(f"{name}: a tensor of shape [{tokens}, {heads}, {cache.head_dim}] on {cache.device} is needed, its "
+                   f"features contiguous, got {t.device} {tuple(t.shape)} with strides {strides}")
+    return Rows(t.data_ptr(), strides[0], strides[1])
 
 
 class PagedCache:
@@ -375,22 +410,23 @@ class PagedCache:
     [pages, kv_heads, page_size, head_dim / 32], uint8 and contiguous."""
 
     def __init__(self, k_values, k_scales, v_values, v_scales, bits):
-        import torch
+        if _torch is None:
+            _setup()
         if bits not in (4, 6, 8):
-            raise MxkInvalidArgument(ERR_INVALID, "bits must be 4, 6 or 8")
-        if k_values.dim() != 4 or k_scales.dim() != 4:
-            raise MxkInvalidArgument(ERR_INVALID, "cache tensors have 4 dimensions")
+            raise _bad("bits must be 4, 6 or 8")
+        if k_scales.dim() != 4 or not k_scales.is_cuda:
+            raise _bad("cache tensors have 4 dimensions and lie on a GPU")
         pages, heads, page, blocks = k_scales.shape
+        self.device, self.index = k_scales.device, k_scales.get_device()
         for t, name, last in ((k_values, "k_values", blocks * 4 * bits), (k_scales, "k_scales", blocks),
                               (v_values, "v_values", blocks * 4 * bits), (v_scales, "v_scales", blocks)):
-            _tensor(t, name, torch.uint8, pages, heads, page, last)
-            if not t.is_contiguous() or t.device != k_scales.device:
-                raise MxkInvalidArgument(ERR_INVALID, f"{name} must be contiguous, all four on one device")
+            _vector(t, name, self, _torch.uint8, pages, heads, page, last)
         self.k_values, self.k_scales, self.v_values, self.v_scales = k_values, k_scales, v_values, v_scales
         self.bits, self.pages, self.kv_heads, self.page_size = bits, pages, heads, page
-        self.head_dim, self.device = blocks * 32, k_scales.device
+        self.head_dim = blocks * 32
         self.struct = Cache(bits, heads, blocks * 32, page, pages, k_values.data_ptr(), k_scales.data_ptr(),
                             v_values.data_ptr(), v_scales.data_ptr())
+        self.handle = ctypes.addressof(self.struct)
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, bits=8, device="cuda"):
@@ -403,52 +439,29 @@ class PagedCache:
                    make(head_dim // 32), bits)
 
 
-_DTYPES = {}
-
-
-def _dtype(t, name):
-    if not _DTYPES:
-        import torch
-        _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-    if t.dtype not in _DTYPES:
-        raise MxkInvalidArgument(ERR_INVALID, f"{name}: float32, float16 or bfloat16 is needed, got {t.dtype}")
-    return _DTYPES[t.dtype]
-
-
-def _rows(t, name, heads, dim):
-    """mxk_rows of t [tokens, heads, dim], whose features must be contiguous."""
-    if not t.is_cuda or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-        raise MxkInvalidArgument(ERR_INVALID, f"{name}: a CUDA tensor of shape [tokens, {heads}, {dim}] is needed, "
-                                              f"got {t.device} {tuple(t.shape)}")
-    strides = t.stride()
-    if strides[2] != 1:
-        raise MxkInvalidArgument(ERR_INVALID, f"{name}: the features of a row must be contiguous")
-    return Rows(t.data_ptr(), strides[0], strides[1])
-
-
-def _cache_pair(cache, k, v, slots):
-    import torch
-    kr, vr = (_rows(t, n, cache.kv_heads, cache.head_dim) for t, n in ((k, "k"), (v, "v")))
-    if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
-        raise MxkInvalidArgument(ERR_INVALID, "k and v must have the same type and number of tokens")
-    _tensor(slots, "slots", torch.int64, k.shape[0])
-    if not slots.is_contiguous():
-        raise MxkInvalidArgument(ERR_INVALID, "slots must be contiguous")
-    return _dtype(k, "k"), kr, vr
+def _move(fn, cache, k, v, slots, stream):
+    dtype, tokens = k.dtype, k.shape[0]
+    code = _DTYPES.get(dtype)
+    if code is None or v.dtype != dtype:
+        raise _bad("k and v: the same one of float32, float16 and bfloat16 is needed")
+    kr = _rows(k, "k", cache, tokens, cache.kv_heads)
+    vr = _rows(v, "v", cache, tokens, cache.kv_heads)
+    at = _vector(slots, "slots", cache, _torch.int64, tokens)
+    return fn, code, tokens, kr, vr, at, _launch_stream(cache, stream)
 
 
 def cache_write(cache, k, v, slots, stream=None):
     """Quantise the rows of k and v [tokens, kv_heads, head_dim] into the cache's
     slots (int64; page * page_size + place; one outside the cache: not kept)."""
-    dtype, kr, vr = _cache_pair(cache, k, v, slots)
-    check(load().mxk_cache_write(cache.struct, dtype, k.shape[0], kr, vr, slots.data_ptr(), _stream(stream)))
+    fn, dtype, tokens, kr, vr, at, st = _move(load().mxk_cache_write, cache, k, v, slots, stream)
+    check(fn(cache.handle, dtype, tokens, ctypes.byref(kr), ctypes.byref(vr), at, st))
 
 
 def cache_read(cache, slots, k, v, stream=None):
     """The values that the cache holds at `slots` into k and v [tokens, kv_heads,
     head_dim] (zeros for a slot outside the cache)."""
-    dtype, kr, vr = _cache_pair(cache, k, v, slots)
-    check(load().mxk_cache_read(cache.struct, dtype, k.shape[0], slots.data_ptr(), kr, vr, _stream(stream)))
+    fn, dtype, tokens, kr, vr, at, st = _move(load().mxk_cache_read, cache, k, v, slots, stream)
+    check(fn(cache.handle, dtype, tokens, at, ctypes.byref(kr), ctypes.byref(vr), st))
 
 
 def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale=None, causal=True, window=0,
@@ -458,28 +471,26 @@ def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, sca
     cu_q [seqs + 1], page_table [seqs, pages], kv_lens [seqs] int32; max_q, max_kv:
     bounds on a sequence's new and cached tokens; scale: 1 / sqrt(head_dim) unless
     given; lse: float32 [tokens, heads] or None."""
-    import torch
-    tokens, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-    qr, outr = _rows(q, "q", heads, cache.head_dim), _rows(out, "out", heads, cache.head_dim)
-    seqs = kv_lens.shape[0] if kv_lens.dim() else 0
-    i32 = torch.int32
-    _tensor(cu_q, "cu_q", i32, seqs + 1)
-    _tensor(kv_lens, "kv_lens", i32, seqs)
-    _tensor(page_table, "page_table", i32, seqs, None)
-    if not (cu_q.is_contiguous() and kv_lens.is_contiguous()) or page_table.stride(1) != 1 < page_table.shape[1]:
-        raise MxkInvalidArgument(ERR_INVALID, "cu_q, kv_lens and the rows of page_table must be contiguous")
-    if page_table.shape[1] * cache.page_size < max_kv:
-        raise MxkInvalidArgument(ERR_INVALID, "page_table has fewer pages than max_kv tokens need")
-    if out.dtype != q.dtype or out.shape[0] != tokens:
-        raise MxkInvalidArgument(ERR_INVALID, "out must have q's type and number of tokens")
-    if lse is not None:
-        _tensor(lse, "lse", torch.float32, tokens, heads)
-        if not lse.is_contiguous():
-            raise MxkInvalidArgument(ERR_INVALID, "lse must be contiguous")
-    args = Attention(_dtype(q, "q"), heads, tokens, seqs, max_q, max_kv, qr, cu_q.data_ptr(), page_table.data_ptr(),
-                     page_table.stride(0), kv_lens.data_ptr(), cache.head_dim ** -0.5 if scale is None else scale,
-                     bool(causal), window, outr, None if lse is None else lse.data_ptr())
-    check(load().mxk_cache_attention(cache.struct, args, _stream(stream)))
+    if q.dim() != 3 or page_table.dim() != 2:
+        raise _bad("q has 3 dimensions, page_table 2")
+    tokens, heads, _ = q.shape
+    dtype, i32 = q.dtype, _torch.int32
+    if out.dtype != dtype:
+        raise _bad("out must have q's type")
+    qr = _rows(q, "q", cache, tokens, heads)
+    outr = _rows(out, "out", cache, tokens, heads)
+    seqs, pages = page_table.shape
+    stride, step = page_table.stride()
+    if page_table.dtype != i32 or page_table.get_device() != cache.index or step != 1 < pages:
+        raise _bad(f"page_table: int32 rows on {cache.device} are needed")
+    if pages * cache.page_size < max_kv:
+        raise _bad("page_table has fewer pages than max_kv tokens need")
+    args = Attention(_DTYPES.get(dtype, -1), heads, tokens, seqs, max_q, max_kv, qr,
+                     _vector(cu_q, "cu_q", cache, i32, seqs + 1), page_table.data_ptr(), stride,
+                     _vector(kv_lens, "kv_lens", cache, i32, seqs),
+                     cache.head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, outr,
+                     None if lse is None else _vector(lse, "lse", cache, _torch.float32, tokens, heads))
+    check(load().mxk_cache_attention(cache.handle, ctypes.byref(args), _launch_stream(cache, stream)))
 
 
 def profile_enable(on=True):

@@ -7,6 +7,10 @@ import pytest
 BUF = 0x7f0000000000  # a plausible, aligned address; nothing here reads it
 
 
+def ref(x):
+    return ctypes.byref(x)
+
+
 def make_cache(mxk, **kw):
     f = dict(bits=8, kv_heads=2, head_dim=128, page_size=64, pages=10, k_values=BUF, k_scales=BUF, v_values=BUF,
              v_scales=BUF)
@@ -33,9 +37,9 @@ def test_bad_cache_is_refused(mxk, bad):
     lib = mxk.load()
     c = make_cache(mxk, **bad)
     rows = mxk.Rows(BUF, 256, 128)
-    for st in (lib.mxk_cache_write(c, mxk.BF16, 1, rows, rows, BUF, None),
-               lib.mxk_cache_read(c, mxk.BF16, 1, BUF, rows, rows, None),
-               lib.mxk_cache_attention(c, make_args(mxk), None)):
+    for st in (lib.mxk_cache_write(ref(c), mxk.BF16, 1, ref(rows), ref(rows), BUF, None),
+               lib.mxk_cache_read(ref(c), mxk.BF16, 1, BUF, ref(rows), ref(rows), None),
+               lib.mxk_cache_attention(ref(c), ref(make_args(mxk)), None)):
         assert st == mxk.ERR_INVALID
         assert lib.mxk_last_error()
 
@@ -43,20 +47,18 @@ def test_bad_cache_is_refused(mxk, bad):
 def test_bad_moves_are_refused(mxk):
     lib = mxk.load()
     c = make_cache(mxk)
-    rows, none, odd = mxk.Rows(BUF, 256, 128), mxk.Rows(None, 256, 128), mxk.Rows(BUF + 1, 256, 128)
-    null = ctypes.POINTER(mxk.Rows)()
+    rows, none, odd = (ref(mxk.Rows(at, 256, 128)) for at in (BUF, None, BUF + 1))
     for args in ((3, 1, rows, rows, BUF), (-1, 1, rows, rows, BUF), (mxk.F16, -1, rows, rows, BUF),
                  (mxk.F16, 1, none, rows, BUF), (mxk.F16, 1, rows, none, BUF), (mxk.F16, 1, rows, rows, None),
-                 (mxk.F16, 1, odd, rows, BUF), (mxk.F32, 1, rows, mxk.Rows(BUF + 2, 256, 128), BUF),
-                 (mxk.F16, 1, rows, rows, BUF + 4), (mxk.F16, 1, null, rows, BUF)):
+                 (mxk.F16, 1, odd, rows, BUF), (mxk.F32, 1, rows, ref(mxk.Rows(BUF + 2, 256, 128)), BUF),
+                 (mxk.F16, 1, rows, rows, BUF + 4), (mxk.F16, 1, None, rows, BUF)):
         dtype, tokens, k, v, slots = args
-        assert lib.mxk_cache_write(c, dtype, tokens, k, v, slots, None) == mxk.ERR_INVALID
-        assert lib.mxk_cache_read(c, dtype, tokens, slots, k, v, None) == mxk.ERR_INVALID
-    null_cache = ctypes.POINTER(mxk.Cache)()
-    assert lib.mxk_cache_write(null_cache, mxk.F16, 1, rows, rows, BUF, None) == mxk.ERR_INVALID
+        assert lib.mxk_cache_write(ref(c), dtype, tokens, k, v, slots, None) == mxk.ERR_INVALID
+        assert lib.mxk_cache_read(ref(c), dtype, tokens, slots, k, v, None) == mxk.ERR_INVALID
+    assert lib.mxk_cache_write(None, mxk.F16, 1, rows, rows, BUF, None) == mxk.ERR_INVALID
     # nothing to do: no pointer is looked at
-    assert lib.mxk_cache_write(c, mxk.F16, 0, null, null, None, None) == mxk.OK
-    assert lib.mxk_cache_read(c, mxk.F16, 0, None, null, null, None) == mxk.OK
+    assert lib.mxk_cache_write(ref(c), mxk.F16, 0, None, None, None, None) == mxk.OK
+    assert lib.mxk_cache_read(ref(c), mxk.F16, 0, None, None, None, None) == mxk.OK
 
 
 BAD_ATTENTION = [dict(dtype=0), dict(dtype=7), dict(heads=0), dict(heads=3), dict(heads=-2), dict(tokens=-1),
@@ -68,20 +70,20 @@ BAD_ATTENTION = [dict(dtype=0), dict(dtype=7), dict(heads=0), dict(heads=3), dic
 
 @pytest.mark.parametrize("bad", BAD_ATTENTION, ids=str)
 def test_bad_attention_is_refused(mxk, bad):
-    assert mxk.load().mxk_cache_attention(make_cache(mxk), make_args(mxk, **bad), None) == mxk.ERR_INVALID
+    assert mxk.load().mxk_cache_attention(ref(make_cache(mxk)), ref(make_args(mxk, **bad)), None) == mxk.ERR_INVALID
 
 
 def test_bad_attention_rows_are_refused(mxk):
     lib, c = mxk.load(), make_cache(mxk)
     for rows in (mxk.Rows(None, 512, 128), mxk.Rows(BUF + 1, 512, 128)):
-        assert lib.mxk_cache_attention(c, make_args(mxk, q=rows), None) == mxk.ERR_INVALID
-        assert lib.mxk_cache_attention(c, make_args(mxk, out=rows), None) == mxk.ERR_INVALID
-    assert lib.mxk_cache_attention(c, ctypes.POINTER(mxk.Attention)(), None) == mxk.ERR_INVALID
+        assert lib.mxk_cache_attention(ref(c), ref(make_args(mxk, q=rows)), None) == mxk.ERR_INVALID
+        assert lib.mxk_cache_attention(ref(c), ref(make_args(mxk, out=rows)), None) == mxk.ERR_INVALID
+    assert lib.mxk_cache_attention(ref(c), None, None) == mxk.ERR_INVALID
 
 
 @pytest.mark.parametrize("dim", [32, 96, 160, 256])
 def test_other_head_dims_are_unsupported(mxk, dim):
-    st = mxk.load().mxk_cache_attention(make_cache(mxk, head_dim=dim), make_args(mxk), None)
+    st = mxk.load().mxk_cache_attention(ref(make_cache(mxk, head_dim=dim)), ref(make_args(mxk)), None)
     assert st == mxk.ERR_UNSUPPORTED
 
 
@@ -89,7 +91,7 @@ def test_other_head_dims_are_unsupported(mxk, dim):
 def test_no_queries_is_nothing_to_do(mxk, nothing):
     args = make_args(mxk, q=mxk.Rows(None, 0, 0), out=mxk.Rows(None, 0, 0), cu_q=None, page_table=None, kv_lens=None,
                      **nothing)
-    assert mxk.load().mxk_cache_attention(make_cache(mxk), args, None) == mxk.OK
+    assert mxk.load().mxk_cache_attention(ref(make_cache(mxk)), ref(args), None) == mxk.OK
 
 
 def test_binding_refuses_host_and_misshapen_tensors(mxk):
