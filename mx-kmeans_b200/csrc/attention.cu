@@ -18,12 +18,14 @@
 //    long as q and k agree, so a lane reads a contiguous quarter of a key row, and
 //    a contiguous eighth of four value rows, and converts in registers.  The row
 //    pitches in shared memory keep those reads free of bank conflicts.
-//  * The MX scale of a key block becomes an f16 factor relative to the row's
-//    largest scale (exact unless two blocks of one row differ by more than 2^30),
-//    the row's own factor goes onto the finished score.  Value blocks are scaled
+//  * The MX scale of a key block becomes an f16 factor relative to the granule's
+//    largest scale (exact unless two blocks differ by more than 2^30), which goes
+//    onto the finished scores.  Value blocks are scaled
 //    relative to the power of two of the largest value scale met so far, which
 //    only moves up, like the running maximum.
+#include <algorithm>
 #include <limits>
+#include <type_traits>
 
 #include "attention.cuh"
 
@@ -79,8 +81,18 @@ struct Stage {
     static_assert(bytes % 16 == 0, "stages start on 16-byte boundaries");
 };
 
+// 16 bytes to shared memory, the first `bytes` of them from src, the rest zero.  The
+// offsets are immediates of the instruction.
+template <int TO, int FROM>
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(TO),
+                 "n"(FROM)
+                 : "memory");
+}
+template <int TO, int FROM>
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(dst), "l"(src), "n"(TO), "n"(FROM)
+                 : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -88,36 +100,36 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// N bytes of shared memory into words (the last one zero-extended).
-template <int N>
+// N bytes of shared memory at `at` + OFF into words (the last one zero-extended), in
+// accesses of W bytes, the widest that divides N and so the alignment of `at` + OFF.
+constexpr int widest(int n) { return n % 16 == 0 ? 16 : (n % 8 == 0 ? 8 : (n % 4 == 0 ? 4 : 2)); }
+template <int N, int OFF, int W = widest(N)>
 __device__ __forceinline__ void lds_bytes(uint32_t at, uint32_t* w) {
-    if constexpr (N % 16 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 16; ++i)
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
-                         : "r"(at + 16 * i));
-    } else if constexpr (N % 8 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 8; ++i)
-            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[2 * i]), "=r"(w[2 * i + 1]) : "r"(at + 8 * i));
-    } else if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(at + 4 * i));
+    static_assert(N % W == 0 && OFF % W == 0, "aligned accesses");
+    if constexpr (W == 16) {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(at), "n"(OFF));
+    } else if constexpr (W == 8) {
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2 + %3];" : "=r"(w[0]), "=r"(w[1]) : "r"(at), "n"(OFF));
+    } else if constexpr (W == 4) {
+        asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(w[0]) : "r"(at), "n"(OFF));
     } else {
         static_assert(N == 6, "rows end on even bytes");
         uint16_t a, b, c;
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(a) : "r"(at));
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(at + 2));
-        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(c) : "r"(at + 4));
+        asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=h"(a) : "r"(at), "n"(OFF));
+        asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=h"(b) : "r"(at), "n"(OFF + 2));
+        asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=h"(c) : "r"(at), "n"(OFF + 4));
         w[0] = a | ((uint32_t)b << 16);
         w[1] = c;
     }
+    if constexpr (W >= 4 && N > W) lds_bytes<N - W, OFF + W, W>(at, w + W / 4);
 }
 
-__device__ __forceinline__ uint32_t lds_u8(uint32_t at) {
-    uint32_t v;
-    asm volatile("{\n\t.reg .u16 t;\n\tld.shared.u8 t, [%1];\n\tcvt.u32.u16 %0, t;\n\t}" : "=r"(v) : "r"(at));
+template <int OFF>
+__device__ __forceinline__ int lds_u8(uint32_t at) {
+    int v;
+    asm volatile("ld.shared.u8 %0, [%1 + %2];" : "=r"(v) : "r"(at), "n"(OFF));
     return v;
 }
 
@@ -130,15 +142,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Largest of the scale bytes of a key row (at least 1, so that 2^(max - 127) is a
-// normal float; blocks are scaled relative to it whatever it is).
-template <int D>
-__device__ __forceinline__ int row_scale(uint32_t w) {
-    int m = max((int)(w & 255u), (int)((w >> 8) & 255u));
-    if constexpr (D == 128) m = max(m, max((int)((w >> 16) & 255u), (int)(w >> 24)));
-    return max(m, 1);
-}
-
 template <int D, int BITS>
 __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const AttentionParams p) {
     using S = Stage<D, BITS>;
@@ -148,12 +151,32 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
     constexpr int kShare = S::row / 4;   // bytes of a key row a lane reads
     constexpr int vShare = S::row / 8;   // bytes of a value row a lane reads
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int64_t scratch[kWarps + 2];
+    __shared__ int scratch[kWarps + 2];
     __shared__ float stat_max[kWarps][kRows], stat_sum[kWarps][kRows];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, c = lane & 3;
     const uint32_t ring = dev::smem_addr(smem) + warp * (S::stages * S::bytes);
+    // Where a lane's 16 bytes of a granule go: the i-th of them lie 512 bytes further in the
+    // cache, and a constant further here where rows lie without gaps or 32 pieces fill rows.
+    constexpr int kPieces = kGranule * S::chunks;  // of a side
+    constexpr int kCopies = (kPieces + 31) / 32;
+    constexpr int kStep = P::k == S::row ? 512 : 32 / S::chunks * P::k;
+    constexpr int vStep = P::v == S::row ? 512 : 32 / S::chunks * P::v;
+    static_assert(P::k == S::row || 32 % S::chunks == 0, "key rows without gaps, or whole rows in a copy");
+    constexpr bool vEven = P::v == S::row || 32 % S::chunks == 0;
+    auto v_place = [&](int i) -> uint32_t { const int x = lane + 32 * i; return x / S::chunks * P::v + x % S::chunks * 16; };
+    const uint32_t k_lane = ring + (P::k == S::row ? lane * 16 : lane / S::chunks * P::k + lane % S::chunks * 16);
+    uint32_t v_lane[vEven ? 1 : kCopies];
+#pragma unroll
+    for (int i = 0; i < (vEven ? 1 : kCopies); ++i)
+        v_lane[i] = ring + S::v_at + (P::v == S::row ? lane * 16 : v_place(i));
+    static_assert(P::k % widest(kShare) == 0 && P::v % widest(vShare) == 0 && S::v_at % 16 == 0 && S::bytes % 16 == 0,
+                  "reads are aligned to their width");
+    const uint32_t k_read = ring + g * P::k + c * kShare;
+    const uint32_t v_read = ring + S::v_at + 2 * c * P::v + g * vShare;
+    const uint32_t ks_read = ring + S::ks_at + g * S::scale_bytes + (D == 128 ? c : c >> 1);
+    const uint32_t vs_read = ring + S::vs_at + 2 * c * S::scale_bytes + (D == 128 ? g >> 1 : g >> 2);
 
     const dev::Share share = dev::take_share<kRows, kKeys, kThreads>(p, scratch);
     if (share.tiles == 0) {
@@ -161,21 +184,20 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
         return;
     }
     dev::Walk w = dev::walk_to<kRows, kKeys>(p, share.seq, share.offset);
-    int64_t left = share.tiles;
+    int left = share.tiles;
     bool open = false;
 
     while (left > 0) {
         const int tile0 = w.tile;
-        const int tiles = (int)(left < w.tiles - tile0 ? left : w.tiles - tile0);
-        const int rows = w.view.n * p.group - w.rt * kRows < kRows ? w.view.n * p.group - w.rt * kRows : kRows;
-        const int64_t len = w.view.len;
+        const int tiles = min(left, w.tiles - tile0);
+        const int rows = min(w.view.n * p.group - w.rt * kRows, kRows);
+        const int len = w.view.len;
 
         // This lane's rows (g and g + 8): tokens [lo, hi) take part.  Rows past the
         // unit's see everything; they are zero queries and never written.
-        int64_t lo[2], hi[2];
+        int lo[2], hi[2], all_lo = 0, all_hi = len, any_lo, any_hi;
         int64_t row_at[2];
         bool real[2];
-        int64_t all_lo = 0, all_hi = len, any_lo, any_hi;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = w.rt * kRows + g + 8 * i;
@@ -187,12 +209,71 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
                         (int64_t)(w.head * p.group + (r - j * p.group)) * p.q_head;
         }
         {
-            const int r0 = w.rt * kRows, r1 = r0 + rows - 1;
-            dev::seen_range(p, w.view, r0 / p.group, r1 / p.group, any_lo, any_hi);  // seen by some row
-            int64_t a, b;
-            dev::seen_range(p, w.view, r0 / p.group, r0 / p.group, a, all_hi);  // the first row ends first,
-            dev::seen_range(p, w.view, r1 / p.group, r1 / p.group, all_lo, b);  // the last begins last
+            const int r0 = w.rt * kRows, j0 = r0 / p.group, j1 = (r0 + rows - 1) / p.group;
+            int x;
+            dev::seen_range(p, w.view, j0, j1, any_lo, any_hi);  // seen by some row
+            dev::seen_range(p, w.view, j0, j0, x, all_hi);       // the first row ends first,
+            dev::seen_range(p, w.view, j1, j1, all_lo, x);       // the last begins last
         }
+
+        // The warp's granules: numbers gran0, gran0 + 4, ... of the sequence below `end`.
+        // A granule is contiguous in its page, so a lane copies 16 bytes every 512.
+        const int gran0 = (w.first + tile0) * kWarps + warp;
+        const int end = min((w.first + tile0 + tiles) * kWarps,
+                            any_hi <= any_lo ? 0 : (any_hi + kGranule - 1) / kGranule);
+        const int steps = end > gran0 ? (end - gran0 + kWarps - 1) / kWarps : 0;
+        const int* table = p.page_table + (int64_t)w.seq * p.table_stride;
+        const int per_page = p.page_size / kGranule;
+        const int jump = kWarps / per_page, rest = kWarps - jump * per_page;  // pages and granules of one step
+        int next_at = gran0 / per_page, next_in = gran0 - next_at * per_page;  // page and granule of the next copy
+        auto next_page = [&](int step) -> int {
+            return step < steps ? min(max(__ldg(table + next_at), 0), p.pages - 1) : 0;
+        };
+        // The lane's first bytes of page 0 of the head, and where the scales go.
+        constexpr int sc = kGranule * S::scale_bytes / 16;  // 16-byte pieces of a side's scales
+        const int64_t head_row = (int64_t)w.head * p.page_size;
+        const uint8_t* k_src = p.k_values + head_row * S::row + lane * 16;
+        const uint8_t* v_src = p.v_values + head_row * S::row + lane * 16;
+        const uint8_t* s_src = (lane < sc ? p.k_scales : p.v_scales - sc * 16) + head_row * S::scale_bytes + lane * 16;
+        const uint32_t page_rows = (uint32_t)p.kv_heads * p.page_size;
+        int copy_stage = 0;  // offset of the stage to copy to
+        auto copy_side = [&](auto index, const uint8_t* k, const uint8_t* v, int valid) {
+            constexpr int i = decltype(index)::value;
+            if (kPieces % 32 == 0 || lane + 32 * i < kPieces) {
+                const uint32_t to_k = k_lane + copy_stage, to_v = v_lane[vEven ? 0 : i] + copy_stage;
+                constexpr int v_off = vEven ? i * vStep : 0;
+                if (valid >= kGranule) {
+                    copy16<i * kStep, 512 * i>(to_k, k);
+                    copy16<v_off, 512 * i>(to_v, v);
+                } else {  // rows past the sequence's end are zeros
+                    const int bytes = (lane + 32 * i) / S::chunks < valid ? 16 : 0;
+                    copy16<i * kStep, 512 * i>(to_k, k, bytes);
+                    copy16<v_off, 512 * i>(to_v, v, bytes);
+                }
+            }
+        };
+        auto issue = [&](int step, int page) {
+            if (step < steps) {
+                const uint32_t row = (uint32_t)page * page_rows + (uint32_t)next_in * kGranule;
+                const uint8_t* k = k_src + (uint64_t)row * S::row;
+                const uint8_t* v = v_src + (uint64_t)row * S::row;
+                const int valid = len - (gran0 + step * kWarps) * kGranule;
+                copy_side(std::integral_constant<int, 0>{}, k, v, valid);
+                if constexpr (kCopies > 1) copy_side(std::integral_constant<int, 1>{}, k, v, valid);
+                if constexpr (kCopies > 2) copy_side(std::integral_constant<int, 2>{}, k, v, valid);
+                if constexpr (kCopies > 3) copy_side(std::integral_constant<int, 3>{}, k, v, valid);
+                if (lane < 2 * sc)
+                    copy16<S::ks_at, 0>(ring + copy_stage + lane * 16, s_src + (uint64_t)row * S::scale_bytes);
+                next_at += jump, next_in += rest;
+                if (next_in >= per_page) next_in -= per_page, ++next_at;
+                copy_stage = copy_stage == (S::stages - 1) * S::bytes ? 0 : copy_stage + S::bytes;
+            }
+            copy_commit();
+        };
+        static_assert(kCopies <= 4, "");
+#pragma unroll
+        for (int s = 0; s < S::stages - 1; ++s) issue(s, next_page(s));
+        int page = next_page(S::stages - 1);
 
         // q as the A operand: features c * D/4 + 4 i .. + 3 of rows g, g + 8 at step i.
         uint32_t qa[kSteps][4];
@@ -253,77 +334,36 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
         float sum[2] = {0.0f, 0.0f};               // this lane's share of the rows' sums
         int vref = 0;                              // values are held relative to 2^(vref - 127); 0: none yet
 
-        // The warp's granules: numbers first, first + 4, ... of the sequence below `end`.
-        const int64_t gran0 = (w.first + tile0) * kWarps + warp;
-        int64_t end = (w.first + tile0 + tiles) * kWarps;
-        const int64_t seen_end = any_hi <= any_lo ? 0 : (any_hi + kGranule - 1) / kGranule;
-        end = end < seen_end ? end : seen_end;
-        const int steps = end > gran0 ? (int)((end - gran0 + kWarps - 1) / kWarps) : 0;
-        const int* table = p.page_table + (int64_t)w.seq * p.table_stride;
-        const unsigned per_page = (unsigned)p.page_size / kGranule;
-
-        auto page_of = [&](int step) -> int {
-            if (step >= steps) return 0;
-            const unsigned gr = (unsigned)(gran0 + (int64_t)step * kWarps);
-            const int page = __ldg(table + gr / per_page);
-            return page < 0 ? 0 : (page >= p.pages ? p.pages - 1 : page);
-        };
-        auto issue = [&](int step, int page) {
-            if (step < steps) {
-                const int64_t gr = gran0 + (int64_t)step * kWarps;
-                const int in_page = (int)((unsigned)gr % per_page) * kGranule;
-                const int64_t row = ((int64_t)page * p.kv_heads + w.head) * p.page_size + in_page;
-                const int valid = (int)(len - gr * kGranule < kGranule ? len - gr * kGranule : kGranule);
-                const uint32_t at = ring + (step % S::stages) * S::bytes;
-#pragma unroll
-                for (int i = 0; i < S::chunks; ++i) {
-                    const int idx = lane + 32 * i;
-                    const bool is_v = idx >= kGranule * S::chunks;
-                    const int in = is_v ? idx - kGranule * S::chunks : idx;
-                    const int r = in / S::chunks, ch = in - r * S::chunks;
-                    const uint8_t* src = (is_v ? p.v_values : p.k_values) + (row + r) * S::row + ch * 16;
-                    copy16(at + (is_v ? S::v_at + r * P::v : r * P::k) + ch * 16, src, r < valid ? 16 : 0);
-                }
-                constexpr int sc = kGranule * S::scale_bytes / 16;
-                if (lane < 2 * sc) {
-                    const int side = lane / sc, ch = lane - side * sc;
-                    copy16(at + (side ? S::vs_at : S::ks_at) + ch * 16,
-                           (side ? p.v_scales : p.k_scales) + row * S::scale_bytes + ch * 16, 16);
-                }
-            }
-            copy_commit();
-        };
-
-#pragma unroll
-        for (int s = 0; s < S::stages - 1; ++s) issue(s, page_of(s));
-        int next_page = page_of(S::stages - 1);
-
+        int stage = 0;  // offset of the stage at hand
         for (int step = 0; step < steps; ++step) {
             copy_wait<S::stages - 2>();
             __syncwarp();
-            issue(step + S::stages - 1, next_page);
-            next_page = page_of(step + S::stages);
-            const uint32_t at = ring + (step % S::stages) * S::bytes;
-            const int64_t t0 = (gran0 + (int64_t)step * kWarps) * kGranule;
+            issue(step + S::stages - 1, page);
+            page = next_page(step + S::stages);
+            const int now = stage;
+            stage = stage == (S::stages - 1) * S::bytes ? 0 : stage + S::bytes;
+            const int t0 = (gran0 + step * kWarps) * kGranule;
+
+            // The keys' reference: the granule's largest scale.
+            const bool last = t0 + kGranule > len;
+            int ks[2] = {lds_u8<0>(ks_read + now), lds_u8<8 * S::scale_bytes>(ks_read + now)};
+            if (last) {  // the keys past the sequence's end are zero
+                if (t0 + g >= len) ks[0] = 0;
+                if (t0 + g + 8 >= len) ks[1] = 0;
+            }
+            const int kref = max((int)__reduce_max_sync(kFull, (unsigned)max(ks[0], ks[1])), 1);
+            const float kfactor = __uint_as_float((uint32_t)kref << 23);
+            const float fa = row_factor[0] * kfactor, fb = row_factor[1] * kfactor;
 
             // scores: 16 rows x 2 tiles of 8 tokens
             float s[2][4];
+            uint32_t key_words[2][(kShare + 3) / 4];
+            lds_bytes<kShare, 0>(k_read + now, key_words[0]);
+            lds_bytes<kShare, 8 * P::k>(k_read + now, key_words[1]);
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
-                const int t = g + 8 * nt;
-                uint32_t kw[(kShare + 3) / 4];
-                lds_bytes<kShare>(at + t * P::k + c * kShare, kw);
-                uint32_t sw;
-                if constexpr (D == 128) {
-                    lds_bytes<4>(at + S::ks_at + t * 4, &sw);
-                } else {
-                    uint16_t h;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(at + S::ks_at + t * 2));
-                    sw = h;
-                }
-                const int top = row_scale<D>(sw);
-                const int own = (int)((sw >> (8 * (D == 128 ? c : c >> 1))) & 255u);
-                const uint32_t f = pow2_f16x2(own - top + kKeyLift, own - top + kKeyLift);
+                const uint32_t* kw = key_words[nt];
+                const uint32_t f = pow2_f16x2(ks[nt] - kref + kKeyLift, ks[nt] - kref + kKeyLift);
                 s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
                 if constexpr (BITS == 4) {
 #pragma unroll
@@ -342,11 +382,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
                                  hmul2(dev::codes_to_f16x2<kCode>(four >> 16), f));
                     }
                 }
-                // the rows' and the tokens' own factors
-                const float tok = __uint_as_float((uint32_t)top << 23);
-                const float ta = __shfl_sync(kFull, tok, 8 * c), tb = __shfl_sync(kFull, tok, 8 * c + 4);
-                s[nt][0] = s[nt][0] * row_factor[0] * ta, s[nt][1] = s[nt][1] * row_factor[0] * tb;
-                s[nt][2] = s[nt][2] * row_factor[1] * ta, s[nt][3] = s[nt][3] * row_factor[1] * tb;
+                s[nt][0] *= fa, s[nt][1] *= fa, s[nt][2] *= fb, s[nt][3] *= fb;
             }
             const bool partly = t0 < all_lo || t0 + kGranule > all_hi;
             if (partly) {
@@ -354,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
                 for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int64_t t = t0 + 8 * nt + 2 * c + (e & 1);
+                        const int t = t0 + 8 * nt + 2 * c + (e & 1);
                         if (t < lo[e >> 1] || t >= hi[e >> 1]) s[nt][e] = neg_inf;
                     }
             }
@@ -392,13 +428,16 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
             // values: this lane's tokens 2c, 2c + 1, 2c + 8, 2c + 9
             uint32_t vw[4][(vShare + 3) / 4];
             int vs[4];
-            constexpr int blocks = D / 32;
+            lds_bytes<vShare, 0>(v_read + now, vw[0]);
+            lds_bytes<vShare, P::v>(v_read + now, vw[1]);
+            lds_bytes<vShare, 8 * P::v>(v_read + now, vw[2]);
+            lds_bytes<vShare, 9 * P::v>(v_read + now, vw[3]);
+            vs[0] = lds_u8<0>(vs_read + now), vs[1] = lds_u8<S::scale_bytes>(vs_read + now);
+            vs[2] = lds_u8<8 * S::scale_bytes>(vs_read + now), vs[3] = lds_u8<9 * S::scale_bytes>(vs_read + now);
+            if (last) {  // as are the values
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = 2 * c + (i & 1) + 8 * (i >> 1);
-                lds_bytes<vShare>(at + S::v_at + t * P::v + g * vShare, vw[i]);
-                vs[i] = (int)lds_u8(at + S::vs_at + t * blocks + (D == 128 ? g >> 1 : g >> 2));
-                if (t0 + kGranule > len && t0 + t >= len) vs[i] = 0;  // the values there are zero
+                for (int i = 0; i < 4; ++i)
+                    if (t0 + 2 * c + (i & 1) + 8 * (i >> 1) >= len) vs[i] = 0;
             }
             const int top = (int)__reduce_max_sync(kFull, (unsigned)max(max(vs[0], vs[1]), max(vs[2], vs[3])));
             if (vref == 0 || top > vref + kValueMax) {
@@ -474,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
                         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
                             for (int e = 0; e < 2; ++e)
-                                if ((lds_u8(at + S::v_at + t * P::v + (2 * c + e) * vShare + n) & 0x7fu) == 0x7fu)
+                                if ((lds_u8<0>(ring + now + S::v_at + t * P::v + (2 * c + e) * vShare + n) & 0x7f) == 0x7f)
                                     o[n][2 * i + e] = __int_as_float(0x7fc00000);
                     }
             }
@@ -595,8 +634,8 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     MXK_REQUIRE(a->dtype == MXK_F16 || a->dtype == MXK_BF16, "cache_attention: dtype must be MXK_F16 or MXK_BF16");
     MXK_REQUIRE(a->heads >= 1 && a->heads <= 65535 && a->heads % cache->kv_heads == 0,
                 "cache_attention: heads must be a positive multiple of the cache's kv_heads");
-    MXK_REQUIRE(a->tokens >= 0 && a->tokens <= std::numeric_limits<int>::max() && a->seqs >= 0,
-                "cache_attention: tokens and seqs must be in [0, 2^31)");
+    MXK_REQUIRE(a->tokens >= 0 && a->tokens <= std::numeric_limits<int>::max() / 2 && a->seqs >= 0,
+                "cache_attention: tokens must be in [0, 2^30), seqs in [0, 2^31)");
     MXK_REQUIRE(a->max_q >= 0 && a->max_kv >= 0, "cache_attention: max_q and max_kv must not be negative");
     MXK_REQUIRE((int64_t)a->max_q * a->heads <= std::numeric_limits<int>::max() / 2 &&
                     a->max_kv <= std::numeric_limits<int>::max() / 2,
@@ -639,11 +678,12 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     p.cu_q = a->cu_q;
     p.page_table = a->page_table;
     p.table_stride = a->page_table_stride;
-    p.max_kv = a->max_kv;
+    p.max_kv = (int)a->max_kv;
+    p.max_q = a->max_q;
     p.kv_lens = a->kv_lens;
     p.scale_log2 = a->scale * 1.44269504088896f;
     p.causal = a->causal != 0;
-    p.window = a->window;
+    p.window = (int)std::min<int64_t>(a->window, 1 << 30);
     p.min_rows = 1;
     p.max_rows = std::numeric_limits<int>::max();
 
@@ -661,6 +701,7 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     }
     const int few_q = rows > kMostFewRows ? (kMostFewRows + p.group - 1) / p.group : a->max_q;
     const int64_t most = attention_tile_bound(p, few_q, kRows, kKeys);
+    MXK_REQUIRE(most <= std::numeric_limits<int>::max(), "cache_attention: too much work for one call");
     return cache->head_dim == 128 ? launch_rows_bits<128>(cache->bits, p, most, rows, st)
                                   : launch_rows_bits<64>(cache->bits, p, most, rows, st);
 }

@@ -30,16 +30,15 @@ struct AttentionParams {
     float* lse;
     int64_t q_token, q_head, out_token, out_head;  // strides in elements
     int64_t tokens;
-    int dtype, heads, group, seqs;
+    int dtype, heads, group, seqs, max_q;
     int q_vec, out_vec;  // rows can be moved 8 bytes at a time
     const int* cu_q;
     const int* page_table;
     int64_t table_stride;
-    int64_t max_kv;
+    int max_kv;
     const int* kv_lens;
     float scale_log2;  // scale * log2(e)
-    int causal;
-    int64_t window;
+    int causal, window;
     int min_rows, max_rows;  // this launch takes the sequences with min_rows <= n * group <= max_rows
     // partial sums
     float* part;  // [2 * CTAs][tile rows][head_dim]
@@ -58,7 +57,7 @@ struct AttentionParams {
 // row tile's tokens fill.
 inline int64_t attention_tile_bound(const AttentionParams& p, int max_q, int rows, int keys) {
     const int64_t row_tiles = ((int64_t)max_q * p.group + rows - 1) / rows;
-    int64_t span = p.max_kv;
+    int64_t span = p.max_kv;  // below 2^30, as the window
     if (p.window > 0 && p.window + rows < span) span = p.window + rows;
     return (int64_t)p.seqs * p.kv_heads * row_tiles * (span / keys + 2);
 }
@@ -111,149 +110,149 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 
 // One sequence as the host's bounds let it be seen.
 struct SeqView {
-    int row0;     // first query row
-    int n;        // query tokens
-    int64_t len;  // cached tokens
+    int row0;  // first query row
+    int n;     // query tokens
+    int len;   // cached tokens
 };
 
 __device__ __forceinline__ SeqView seq_view(const AttentionParams& p, int seq) {
     SeqView v;
-    const int64_t a = __ldg(p.cu_q + seq), b = __ldg(p.cu_q + seq + 1);
-    const int64_t lo = a < 0 ? 0 : (a > p.tokens ? p.tokens : a);
-    const int64_t hi = b < lo ? lo : (b > p.tokens ? p.tokens : b);
-    v.row0 = (int)lo;
-    v.n = (int)(hi - lo);
-    const int64_t len = __ldg(p.kv_lens + seq);
-    v.len = len < 0 ? 0 : (len > p.max_kv ? p.max_kv : len);
+    const int a = __ldg(p.cu_q + seq), b = __ldg(p.cu_q + seq + 1), len = __ldg(p.kv_lens + seq);
+    v.row0 = min(max(a, 0), (int)p.tokens);
+    v.n = min(min(max(b, v.row0), (int)p.tokens) - v.row0, p.max_q);
+    v.len = min(max(len, 0), p.max_kv);
     return v;
 }
 
 // Tokens [lo, hi) that the rows of query tokens j0..j1 see, all of them together
 // (empty: hi <= lo).
-__device__ __forceinline__ void seen_range(const AttentionParams& p, const SeqView& s, int j0, int j1, int64_t& lo,
-                                           int64_t& hi) {
-    const int64_t first = s.len - s.n + j0, last = s.len - s.n + j1;
-    hi = p.causal && last + 1 < s.len ? last + 1 : s.len;
-    lo = p.window > 0 && first - p.window + 1 > 0 ? first - p.window + 1 : 0;
+__device__ __forceinline__ void seen_range(const AttentionParams& p, const SeqView& s, int j0, int j1, int& lo, int& hi) {
+    const int first = s.len - s.n + j0, last = s.len - s.n + j1;
+    hi = p.causal ? min(last + 1, s.len) : s.len;
+    lo = p.window > 0 ? max(first - p.window + 1, 0) : 0;
 }
 
 // Key tiles of a row tile (at least one: rows that see nothing are written too).
 template <int ROWS, int KEYS>
-__device__ __forceinline__ int tile_count(const AttentionParams& p, const SeqView& s, int rt, int64_t* first = nullptr) {
-    const int rows = s.n * p.group;
-    const int j0 = rt * ROWS / p.group;
-    const int last = (rt + 1) * ROWS < rows ? (rt + 1) * ROWS - 1 : rows - 1;
-    int64_t lo, hi;
-    seen_range(p, s, j0, last / p.group, lo, hi);
-    const int64_t t0 = lo / KEYS;
+__device__ __forceinline__ int tile_count(const AttentionParams& p, const SeqView& s, int rt, int* first = nullptr) {
+    int lo, hi;
+    if (!p.causal) {
+        lo = 0, hi = s.len;
+    } else {
+        const int last = min((rt + 1) * ROWS, s.n * p.group) - 1;
+        seen_range(p, s, p.window > 0 ? rt * ROWS / p.group : 0, last / p.group, lo, hi);
+    }
+    const int t0 = lo / KEYS;
     if (first) *first = t0;
-    if (hi <= lo) return 1;
-    return (int)((hi + KEYS - 1) / KEYS - t0);
+    return hi <= lo ? 1 : (hi + KEYS - 1) / KEYS - t0;
 }
 
 template <int ROWS, int KEYS>
-__device__ __forceinline__ int64_t seq_tiles(const AttentionParams& p, const SeqView& s) {
-    const int64_t rows = (int64_t)s.n * p.group;
+__device__ __forceinline__ int seq_tiles(const AttentionParams& p, const SeqView& s) {
+    const int rows = s.n * p.group;
     if (rows < p.min_rows || rows > p.max_rows || rows == 0) return 0;
-    int64_t total = 0;
-    const int tiles = (int)((rows + ROWS - 1) / ROWS);
-    if (!p.causal && p.window == 0) return (int64_t)tiles * p.kv_heads * tile_count<ROWS, KEYS>(p, s, 0);
+    int total = 0;
+    const int tiles = (rows + ROWS - 1) / ROWS;
+    if (!p.causal) return tiles * p.kv_heads * tile_count<ROWS, KEYS>(p, s, 0);
     for (int rt = 0; rt < tiles; ++rt) total += tile_count<ROWS, KEYS>(p, s, rt);
     return total * p.kv_heads;
 }
 
-// Where a CTA's share begins, and how many tiles it has.
+// Where a CTA's share begins, and how many tiles it has: `each`, and one more for the
+// first `extra` CTAs.
 struct Share {
-    int64_t tiles;   // of this CTA
-    int seq;         // first sequence of the share
-    int64_t offset;  // of the share's first tile in that sequence
-    int64_t begin;   // the share's first tile among all,
-    int64_t total;   // of so many,
-    int64_t ctas;    // for so many CTAs
+    int tiles;   // of this CTA
+    int seq;     // first sequence of the share
+    int offset;  // of the share's first tile in that sequence
+    int begin;   // the share's first tile among all
+    int each, extra;
 
     // CTAs after this one that work on a unit of n tiles whose first is `at` of the share.
-    __device__ __forceinline__ int followers(int64_t at, int64_t n) const {
-        const int64_t last = begin + at + n - 1;  // tile x belongs to CTA ceil((x + 1) ctas / total) - 1
-        return (int)(((last + 1) * ctas + total - 1) / total - 1 - blockIdx.x);
+    __device__ __forceinline__ int followers(int at, int n) const {
+        const int last = begin + at + n - 1, longer = extra * (each + 1);
+        return (last < longer ? last / (each + 1) : extra + (last - longer) / each) - (int)blockIdx.x;
     }
 };
 
-// All threads of the CTA; scratch: THREADS / 32 + 4 words of shared memory.
+// All threads of the CTA; scratch: THREADS / 32 + 2 words of shared memory.
 // CTAs past the number of tiles get none.
 template <int ROWS, int KEYS, int THREADS>
-__device__ __forceinline__ Share take_share(const AttentionParams& p, int64_t* scratch) {
+__device__ __forceinline__ Share take_share(const AttentionParams& p, int* scratch) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kWarps = THREADS / 32;
-    int64_t* found = scratch + kWarps;  // sequence, offset
-    int64_t sum = 0;
+    int* found = scratch + kWarps;  // sequence, offset
+    int sum = 0;
     for (int i = tid; i < p.seqs; i += THREADS) sum += seq_tiles<ROWS, KEYS>(p, seq_view(p, i));
-    const int64_t mine = sum;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const int mine = sum;
+    sum = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum);
     if (lane == 0) scratch[warp] = sum;
     __syncthreads();
-    int64_t total = 0;
+    int total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) total += scratch[w];
-    const int64_t ctas = total < gridDim.x ? total : gridDim.x;
-    Share s{0, 0, 0, 0, total, ctas};
-    if ((int64_t)blockIdx.x >= ctas) return s;
-    const int64_t begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
-    s.tiles = end - begin;
-    s.begin = begin;
-    int64_t before = 0;  // tiles of the sequences before this round's
+    const int ctas = min(total, (int)gridDim.x);
+    Share s{0, 0, 0, 0, 1, 0};
+    if ((int)blockIdx.x >= ctas) return s;
+    s.each = total / ctas;
+    s.extra = total - s.each * ctas;
+    s.begin = (int)blockIdx.x * s.each + min((int)blockIdx.x, s.extra);
+    s.tiles = s.each + ((int)blockIdx.x < s.extra ? 1 : 0);
+    int before = 0;  // tiles of the sequences before this round's
     for (int base = 0; base < p.seqs; base += THREADS) {
         const int i = base + tid;
-        int64_t t = p.seqs <= THREADS ? mine : (i < p.seqs ? seq_tiles<ROWS, KEYS>(p, seq_view(p, i)) : 0);
-        int64_t incl = t;
+        const int t = p.seqs <= THREADS ? mine : (i < p.seqs ? seq_tiles<ROWS, KEYS>(p, seq_view(p, i)) : 0);
+        int incl = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
-        __syncthreads();
-        if (lane == 31) scratch[warp] = incl;
-        __syncthreads();
-        int64_t start = before, round = 0;
+        if (base > 0 || p.seqs > THREADS) {  // else the warps' sums are there already
+            __syncthreads();
+            if (lane == 31) scratch[warp] = incl;
+            __syncthreads();
+        }
+        int start = before, round = 0;
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) start += scratch[w];
-            round += scratch[w];
+            const int v = scratch[w];
+            if (w < warp) start += v;
+            round += v;
         }
         start += incl - t;
-        if (begin >= start && begin < start + t) found[0] = i, found[1] = begin - start;
+        if (s.begin >= start && s.begin < start + t) found[0] = i, found[1] = s.begin - start;
         before += round;
-        if (begin < before) break;
+        if (s.begin < before) break;
     }
     __syncthreads();
-    s.seq = (int)found[0];
+    s.seq = found[0];
     s.offset = found[1];
-    __syncthreads();
     return s;
 }
 
 // A position in the walk over the units.
 struct Walk {
     int seq, rt, head;
-    int tile, tiles;   // next key tile of the unit, and how many it has
-    int64_t first;     // number of the unit's first key tile in the sequence
+    int tile, tiles;  // next key tile of the unit, and how many it has
+    int first;        // number of the unit's first key tile in the sequence
     SeqView view;
 };
 
 template <int ROWS, int KEYS>
-__device__ __forceinline__ Walk walk_to(const AttentionParams& p, int seq, int64_t offset) {
+__device__ __forceinline__ Walk walk_to(const AttentionParams& p, int seq, int offset) {
     Walk w;
     w.seq = seq;
     w.view = seq_view(p, seq);
     w.rt = 0;
     while (true) {
         w.tiles = tile_count<ROWS, KEYS>(p, w.view, w.rt, &w.first);
-        const int64_t all = (int64_t)w.tiles * p.kv_heads;
+        const int all = w.tiles * p.kv_heads;
         if (offset < all) break;
         offset -= all;
         ++w.rt;
     }
-    w.head = (int)(offset / w.tiles);
-    w.tile = (int)(offset - (int64_t)w.head * w.tiles);
+    w.head = offset / w.tiles;
+    w.tile = offset - w.head * w.tiles;
     return w;
 }
 
@@ -264,14 +263,14 @@ __device__ __forceinline__ void walk_on(const AttentionParams& p, Walk& w) {
     if (++w.head < p.kv_heads) return;
     w.head = 0;
     ++w.rt;
-    if ((int64_t)w.rt * ROWS >= (int64_t)w.view.n * p.group) {
+    if (w.rt * ROWS >= w.view.n * p.group) {
         w.rt = 0;
-        int64_t rows;
+        int rows;
         do {
             ++w.seq;
             if (w.seq >= p.seqs) return;
             w.view = seq_view(p, w.seq);
-            rows = (int64_t)w.view.n * p.group;
+            rows = w.view.n * p.group;
         } while (rows == 0 || rows < p.min_rows || rows > p.max_rows);
     }
     w.tiles = tile_count<ROWS, KEYS>(p, w.view, w.rt, &w.first);

@@ -26,6 +26,7 @@
 // above its largest scale; the output rows are kept relative to the largest
 // reference so far, and a tile with a smaller one has its weights scaled down by the
 // difference, so a row is rescaled only when the reference goes up or its maximum does.
+#include <limits>
 #include <type_traits>
 
 #include "attention.cuh"
@@ -114,13 +115,13 @@ struct Block {
 // A pass over the CTA's share: every role makes the same one.
 struct Cursor {
     dev::Walk w;
-    int64_t left;
+    int left;
     int tile0, tiles;  // key tiles of the current unit that are this CTA's
     int unit;          // units begun so far
 
     __device__ __forceinline__ void take() {
         tile0 = w.tile;
-        tiles = (int)(left < w.tiles - tile0 ? left : w.tiles - tile0);
+        tiles = min(left, w.tiles - tile0);
     }
     __device__ __forceinline__ bool next(const AttentionParams& p) {
         left -= tiles;
@@ -143,14 +144,13 @@ struct Whole {
 };
 __device__ __forceinline__ Whole whole_tiles(const AttentionParams& p, const Cursor& c) {
     const int r0 = c.w.rt * kRows, j0 = r0 / p.group, j1 = (r0 + c.rows(p) - 1) / p.group;
-    int64_t lo, hi, x;
+    int lo, hi, x;
     dev::seen_range(p, c.w.view, j0, j0, x, hi);   // the first row ends first,
     dev::seen_range(p, c.w.view, j1, j1, lo, x);   // the last begins last
-    const int64_t first = c.w.first + c.tile0;
-    const int64_t a = (lo + kKeys - 1) / kKeys - first, b = (hi < 0 ? 0 : hi) / kKeys - first;
+    const int first = c.w.first + c.tile0;
     Whole wt;
-    wt.from = a < 0 ? 0 : (a < c.tiles ? (int)a : c.tiles);
-    wt.to = b < 0 ? 0 : (b < c.tiles ? (int)b : c.tiles);
+    wt.from = min(max((lo + kKeys - 1) / kKeys - first, 0), c.tiles);
+    wt.to = min(max(max(hi, 0) / kKeys - first, 0), c.tiles);
     return wt;
 }
 
@@ -215,7 +215,7 @@ struct Converter {
     }
 
     // Lane i < 8 has the cached row of the tile's token 16 i; `valid` tokens exist.
-    __device__ __forceinline__ uint32_t place(const AttentionParams& p, int seq, int head, int64_t t0, int valid) const {
+    __device__ __forceinline__ uint32_t place(const AttentionParams& p, int seq, int head, int t0, int valid) const {
         uint32_t row = 0;
         if (lane < 8 && 16 * lane < valid) {
             const unsigned per_page = (unsigned)p.page_size / 16u;
@@ -314,15 +314,14 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
     const int tile = blockIdx.x % p.max_tiles, sh = blockIdx.x / p.max_tiles;
     const int seq = sh / p.kv_heads, head = sh - seq * p.kv_heads;
     const dev::SeqView view = dev::seq_view(p, seq);
-    const int64_t rows = (int64_t)view.n * p.group;
+    const int rows = view.n * p.group;
     if (rows == 0 || rows < p.min_rows || rows > p.max_rows) return;
-    int64_t lo, hi;
+    int lo, hi;
     dev::seen_range(p, view, 0, view.n - 1, lo, hi);
-    const int64_t t0 = (int64_t)tile * kKeys;
+    const int t0 = tile * kKeys;
     // rows that see nothing still have key tile 0, of zeros where no token exists
     if (tile != 0 && (t0 >= hi || t0 + kKeys <= lo)) return;
-    const int64_t rest = view.len - t0;
-    const int valid = rest < 0 ? 0 : (rest < kKeys ? (int)rest : kKeys);
+    const int valid = min(max(view.len - t0, 0), kKeys);
     const C cv(threadIdx.x >> 5);
     const uint32_t place = cv.place(p, seq, head, t0, valid);
     uint32_t ks[4], vs[4];
@@ -354,8 +353,8 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
         int valid;  // tokens that exist; -1: no such tile
     };
     auto here = [&]() -> Place {
-        const int64_t t0 = (ahead.w.first + ahead.tile0 + at) * kKeys, rest = ahead.w.view.len - t0;
-        const int valid = rest < 0 ? 0 : (rest < kKeys ? (int)rest : kKeys);
+        const int t0 = (ahead.w.first + ahead.tile0 + at) * kKeys;
+        const int valid = min(max(ahead.w.view.len - t0, 0), kKeys);
         return Place{cv.place(p, ahead.w.seq, ahead.w.head, t0, valid), valid};
     };
     auto advance = [&]() -> Place {
@@ -628,9 +627,9 @@ __device__ __noinline__ float masked_weights(uint32_t s_col, int from, int to, f
 // a row sees, as bits.
 template <int D>
 __device__ __noinline__ uint4 nan_features(const uint8_t* values, const int* table, int page_size, int pages,
-                                           int kv_heads, int head, int64_t k0, int64_t k1) {
+                                           int kv_heads, int head, int k0, int k1) {
     uint32_t bad[4] = {0, 0, 0, 0};
-    for (int64_t k = k0; k < k1; ++k) {
+    for (int k = k0; k < k1; ++k) {
         int page = __ldg(table + k / page_size);
         page = page < 0 ? 0 : (page >= pages ? pages - 1 : page);
         const uint32_t* v = reinterpret_cast<const uint32_t*>(
@@ -712,7 +711,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
     uint32_t s_phase = 0, o_phase[2] = {0, 0};
     int meta_at = 0;
     bool open = false;
-    const int64_t share = c.left;
+    const int share = c.left;
     do {
         const int rows = c.rows(p);
         if (w * kTileRows < rows) {
@@ -721,9 +720,9 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             const int row = c.w.rt * kRows + w * kTileRows + r;
             const int j = row / p.group, head = c.w.head * p.group + (row - j * p.group);
             const Whole whole = whole_tiles(p, c);
-            int64_t lo = 0, hi = c.w.view.len;
+            int lo = 0, hi = c.w.view.len;
             if (real) dev::seen_range(p, c.w.view, j, j, lo, hi);
-            const int64_t first_key = (c.w.first + c.tile0) * kKeys;
+            const int first_key = (c.w.first + c.tile0) * kKeys;
             const float row_factor =
                 put_query<D>(p, (int64_t)(c.w.view.row0 + j) * p.q_token + (int64_t)head * p.q_head, real,
                              b.smem + L::q + w * L::tile + r * 128, r);
@@ -762,9 +761,9 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                     float top;
                     dev::tmem_wait_ld();
                     if (rare) {
-                        const int64_t t0 = first_key + (int64_t)t * kHalf;
-                        from = lo > t0 ? (lo - t0 < kHalf ? (int)(lo - t0) : kHalf) : 0;
-                        to = hi < t0 ? 0 : (hi - t0 < kHalf ? (int)(hi - t0) : kHalf);
+                        const int t0 = first_key + t * kHalf;
+                        from = min(max(lo - t0, 0), kHalf);
+                        to = min(max(hi - t0, 0), kHalf);
                         top = masked_top(s_at, from, to);
                     } else {
                         float m[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
@@ -842,10 +841,10 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                 uint32_t bad[4] = {0, 0, 0, 0};
                 if constexpr (!READY) nans = *reinterpret_cast<volatile int*>(&sh->nan_unit[c.unit & 3]) == c.unit;
                 if (nans && real) {
-                    const int64_t end = first_key + (int64_t)c.tiles * kKeys;
+                    const int end = first_key + c.tiles * kKeys;
                     const uint4 f = nan_features<D>(p.v_values, p.page_table + (int64_t)c.w.seq * p.table_stride,
                                                     p.page_size, p.pages, p.kv_heads, c.w.head,
-                                                    lo > first_key ? lo : first_key, hi < end ? hi : end);
+                                                    max(lo, first_key), min(hi, end));
                     bad[0] = f.x, bad[1] = f.y, bad[2] = f.z, bad[3] = f.w;
                 }
                 const float vfactor = __uint_as_float((uint32_t)vrun << 23);
@@ -901,7 +900,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
 
 // Barriers, TMEM and the cursor; false: the CTA has no share.
 template <int D, class Cfg, int FULL_COUNT>
-__device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_raw, Shared* sh, int64_t* scratch,
+__device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_raw, Shared* sh, int* scratch,
                                       unsigned* err, Block& b, Cursor& c) {
     const int tid = threadIdx.x;
     const dev::Share share = dev::take_share<kRows, kKeys, Cfg::threads>(p, scratch);
@@ -962,7 +961,7 @@ template <int D, int BITS>
 __global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(const AttentionParams p, unsigned* err) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared shared;
-    __shared__ int64_t scratch[Packed::threads / 32 + 2];
+    __shared__ int scratch[Packed::threads / 32 + 2];
     Block b;
     Cursor c;
     if (!begin<D, Packed, 32 * Packed::convert_warps>(p, smem_raw, &shared, scratch, err, b, c)) return;
@@ -984,7 +983,7 @@ template <int D>
 __global__ void __launch_bounds__(Ready::threads, 1) attention_ready_kernel(const AttentionParams p, unsigned* err) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared shared;
-    __shared__ int64_t scratch[Ready::threads / 32 + 2];
+    __shared__ int scratch[Ready::threads / 32 + 2];
     Block b;
     Cursor c;
     if (!begin<D, Ready, 1>(p, smem_raw, &shared, scratch, err, b, c)) return;
@@ -1076,6 +1075,7 @@ int launch_ready(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
 template <int D, int BITS>
 int launch(const AttentionParams& p, bool ready, int max_q, cudaStream_t stream) {
     const int64_t most = attention_tile_bound(p, max_q, kRows, kKeys);
+    MXK_REQUIRE(most <= std::numeric_limits<int>::max(), "cache_attention: too much work for one call");
     return ready ? launch_ready<D, BITS>(p, most, stream) : launch_packed<D, BITS>(p, most, stream);
 }
 
@@ -1091,7 +1091,7 @@ int launch_bits(int bits, const AttentionParams& p, bool ready, int max_q, cudaS
 int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, cudaStream_t stream) {
     // Several row tiles of a key head share its keys: converting those once pays for
     // writing and reading them as f16.
-    p.max_tiles = (int)((p.max_kv + kKeys - 1) / kKeys);
+    p.max_tiles = (p.max_kv + kKeys - 1) / kKeys;
     const int64_t bytes = (int64_t)p.seqs * p.kv_heads * p.max_tiles * 2 * kKeys * head_dim * 2;
     const bool many = (int64_t)max_q * p.group > kReadyRows && p.max_tiles > 0 && bytes <= kReadyBytes;
     const int few_q = (int)((kReadyRows + p.group - 1) / p.group);

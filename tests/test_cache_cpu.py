@@ -62,7 +62,7 @@ def test_bad_moves_are_refused(mxk):
 
 
 BAD_ATTENTION = [dict(dtype=0), dict(dtype=7), dict(heads=0), dict(heads=3), dict(heads=-2), dict(tokens=-1),
-                 dict(tokens=1 << 31), dict(seqs=-1), dict(max_q=-1), dict(max_kv=-1), dict(max_q=1 << 30),
+                 dict(tokens=1 << 30), dict(seqs=-1), dict(max_q=-1), dict(max_kv=-1), dict(max_q=1 << 30),
                  dict(max_kv=1 << 31), dict(window=-1), dict(window=5, causal=0), dict(scale=float("nan")),
                  dict(scale=float("inf")), dict(cu_q=None), dict(page_table=None), dict(kv_lens=None),
                  dict(cu_q=BUF + 2), dict(lse=BUF + 2), dict(page_table_stride=1)]
