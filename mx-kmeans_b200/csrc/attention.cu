@@ -49,6 +49,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kGranule = 16;  // tokens of one step of a warp
 constexpr int kKeys = kGranule * kWarps;
+constexpr int kCtasPerSm = 4;
 // Rows per key head up to which this kernel is taken, one pass over the keys for
 // every 16 of them.
 constexpr int kMostFewRows = 32;
@@ -74,7 +75,7 @@ struct Stage {
     static constexpr int ks_at = v_at + kGranule * Pitch<D, BITS>::v;
     static constexpr int vs_at = ks_at + kGranule * scale_bytes;
     static constexpr int bytes = vs_at + kGranule * scale_bytes;
-    static constexpr int stages = 3;
+    static constexpr int stages = 2;
     static constexpr int ring = kWarps * stages * bytes;
     static constexpr int join = kWarps * kRows * D * 4;  // the warps' outputs, after the ring is done
     static constexpr int smem = ring > join ? ring : join;
@@ -126,6 +127,10 @@ __device__ __forceinline__ void lds_bytes(uint32_t at, uint32_t* w) {
     if constexpr (W >= 4 && N > W) lds_bytes<N - W, OFF + W, W>(at, w + W / 4);
 }
 
+__device__ __forceinline__ void lds_at(uint32_t at, uint32_t (&w)[4]) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+}
+
 template <int OFF>
 __device__ __forceinline__ int lds_u8(uint32_t at) {
     int v;
@@ -143,7 +148,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 template <int D, int BITS>
-__global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const AttentionParams p) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(const AttentionParams p) {
     using S = Stage<D, BITS>;
     using P = Pitch<D, BITS>;
     constexpr int kSteps = D / 16;       // k-steps of q . k
@@ -153,6 +158,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int scratch[kWarps + 2];
     __shared__ float stat_max[kWarps][kRows], stat_sum[kWarps][kRows];
+    __shared__ __align__(16) uint4 query[kSteps][32];  // the A operand of every k-step, lane by lane
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, c = lane & 3;
@@ -276,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
         int page = next_page(S::stages - 1);
 
         // q as the A operand: features c * D/4 + 4 i .. + 3 of rows g, g + 8 at step i.
-        uint32_t qa[kSteps][4];
+        uint32_t qa[kSteps / kWarps][4];  // those of this warp's k-steps
         float row_factor[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -317,13 +323,19 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
             row_factor[i] = p.scale_log2 * __uint_as_float((uint32_t)(127 - down - kKeyLift / 2) << 23) *
                             __uint_as_float((uint32_t)(127 - rest - kKeyLift / 2) << 23);
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                const __half2 u = __floats2half2_rn(x[4 * k] * f0 * f1, x[4 * k + 1] * f0 * f1);
-                const __half2 v = __floats2half2_rn(x[4 * k + 2] * f0 * f1, x[4 * k + 3] * f0 * f1);
-                qa[k][i] = *reinterpret_cast<const uint32_t*>(&u);
-                qa[k][2 + i] = *reinterpret_cast<const uint32_t*>(&v);
-            }
+            for (int k = 0; k < kSteps; ++k)
+                if (k / (kSteps / kWarps) == warp) {
+                    const __half2 u = __floats2half2_rn(x[4 * k] * f0 * f1, x[4 * k + 1] * f0 * f1);
+                    const __half2 v = __floats2half2_rn(x[4 * k + 2] * f0 * f1, x[4 * k + 3] * f0 * f1);
+                    qa[k % (kSteps / kWarps)][i] = *reinterpret_cast<const uint32_t*>(&u);
+                    qa[k % (kSteps / kWarps)][2 + i] = *reinterpret_cast<const uint32_t*>(&v);
+                }
         }
+#pragma unroll
+        for (int k = 0; k < kSteps / kWarps; ++k)
+            query[warp * (kSteps / kWarps) + k][lane] = make_uint4(qa[k][0], qa[k][1], qa[k][2], qa[k][3]);
+        __syncthreads();
+        const uint32_t q_read = dev::smem_addr(&query[0][lane]);
 
         float o[kTiles][4];
 #pragma unroll
@@ -360,30 +372,34 @@ __global__ void __launch_bounds__(kThreads, 3) attention_rows_kernel(const Atten
             uint32_t key_words[2][(kShare + 3) / 4];
             lds_bytes<kShare, 0>(k_read + now, key_words[0]);
             lds_bytes<kShare, 8 * P::k>(k_read + now, key_words[1]);
+            const uint32_t kf[2] = {pow2_f16x2(ks[0] - kref + kKeyLift, ks[0] - kref + kKeyLift),
+                                    pow2_f16x2(ks[1] - kref + kKeyLift, ks[1] - kref + kKeyLift)};
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                const uint32_t* kw = key_words[nt];
-                const uint32_t f = pow2_f16x2(ks[nt] - kref + kKeyLift, ks[nt] - kref + kKeyLift);
-                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
-                if constexpr (BITS == 4) {
+            for (int nt = 0; nt < 2; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < kSteps; k += 2) {
-                        uint32_t h[4];
-                        dev::e2m1x8_to_f16(kw[k / 2], h);
-                        mma16816(s[nt], qa[k], hmul2(h[0], f), hmul2(h[1], f));
-                        mma16816(s[nt], qa[k + 1], hmul2(h[2], f), hmul2(h[3], f));
-                    }
-                } else {
+            for (int k = 0; k < kSteps; k += 2) {
+                uint32_t qa[2][4];
+                lds_at(q_read + 512 * k, qa[0]);
+                lds_at(q_read + 512 * (k + 1), qa[1]);
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        const uint32_t four = BITS == 8 ? kw[k] : four6(kw, k);
+                for (int nt = 0; nt < 2; ++nt) {
+                    uint32_t h[4];
+                    if constexpr (BITS == 4) {
+                        dev::e2m1x8_to_f16(key_words[nt][k / 2], h);
+                    } else {
                         constexpr int kCode = BITS == 4 ? 8 : BITS;
-                        mma16816(s[nt], qa[k], hmul2(dev::codes_to_f16x2<kCode>(four), f),
-                                 hmul2(dev::codes_to_f16x2<kCode>(four >> 16), f));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t four = BITS == 8 ? key_words[nt][k + i] : four6(key_words[nt], k + i);
+                            h[2 * i] = dev::codes_to_f16x2<kCode>(four), h[2 * i + 1] = dev::codes_to_f16x2<kCode>(four >> 16);
+                        }
                     }
+                    mma16816(s[nt], qa[0], hmul2(h[0], kf[nt]), hmul2(h[1], kf[nt]));
+                    mma16816(s[nt], qa[1], hmul2(h[2], kf[nt]), hmul2(h[3], kf[nt]));
                 }
-                s[nt][0] *= fa, s[nt][1] *= fa, s[nt][2] *= fb, s[nt][3] *= fb;
             }
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) s[nt][0] *= fa, s[nt][1] *= fa, s[nt][2] *= fb, s[nt][3] *= fb;
             const bool partly = t0 < all_lo || t0 + kGranule > all_hi;
             if (partly) {
 #pragma unroll
@@ -606,7 +622,7 @@ int launch_rows(AttentionParams p, int64_t most_tiles, int64_t most_rows, cudaSt
         ready_device = dev;
     }
     static const int sms = sm_count();
-    const int64_t ctas = most_tiles < 3 * sms ? most_tiles : 3 * sms;
+    const int64_t ctas = std::min<int64_t>(most_tiles, kCtasPerSm * sms);
     Workspace ws(stream);
     MXK_CHECK(ws.take(p, ctas, kRows, D));
     {

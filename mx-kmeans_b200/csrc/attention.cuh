@@ -304,26 +304,66 @@ __device__ __forceinline__ float row_lse(float m2, float sum) {
 
 }  // namespace dev
 
-// Block (x, y): the unit that CTA x began and did not finish, rows y, y + gridDim.y, ...
-// Its parts are the beginning (slot 2x + 1) and what the following CTAs did first (slots
-// 2j).  The four warps take every fourth part (with D = 64 every half-warp every eighth),
-// so a unit in hundreds of parts has several rows of loads under way, and add up in a
-// fixed order.
+// A row of a joined unit: v and the row's sum are over all parts, relative to `top`.
+template <int ROWS, int D>
+__device__ __forceinline__ void store_joined(const AttentionParams& p, const int4& unit, const dev::SeqView& view, int r,
+                                             int chunk, float4 v, float top, float total) {
+    const int row = unit.y * ROWS + r, j = row / p.group;
+    const int head = unit.z * p.group + (row - j * p.group);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    dev::store4(p, view.row0 + j, head, chunk * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
+}
+
+// Block (x, y): the unit that CTA x began and did not finish, some of its rows.  Its parts
+// are the beginning (slot 2x + 1) and what the following CTAs did first (slots 2j); they
+// add up in a fixed order.  Few parts: every D / 4 threads take a row and go through its
+// parts.  Many: the block takes a row, every D / 4 of its threads some of the parts, so a
+// unit in hundreds of parts has several loads under way.
 template <int ROWS, int D>
 __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionParams p) {
     constexpr int kLanes = D / 4;            // threads of a row
-    constexpr int kSub = 128 / kLanes;       // parts at a time
+    constexpr int kSub = 128 / kLanes;       // rows, or parts, at a time
+    constexpr int kFew = 8;
     __shared__ float4 sums[kSub][kLanes];
     __shared__ float stats[4], sub_totals[kSub];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 unit = p.part_open[blockIdx.x];
     if (!unit.w) return;
     const dev::SeqView view = dev::seq_view(p, unit.x);
-    const int rows = view.n * p.group - unit.y * ROWS < ROWS ? view.n * p.group - unit.y * ROWS : ROWS;
+    const int rows = min(view.n * p.group - unit.y * ROWS, ROWS);
     const int tid = threadIdx.x, chunk = tid % kLanes, sub = tid / kLanes, parts = unit.w + 1;
     auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(blockIdx.x + i) + (i == 0 ? 1 : 0); };
+    if (parts <= kFew) {
+        for (int r = blockIdx.y * kSub + sub; r < rows; r += gridDim.y * kSub) {
+            float2 st[kFew];
+            float4 x[kFew];
+#pragma unroll
+            for (int i = 0; i < kFew; ++i)
+                if (i < parts) {
+                    st[i] = p.part_stat[slot(i) * ROWS + r];
+                    x[i] = reinterpret_cast<const float4*>(p.part + (slot(i) * ROWS + r) * D)[chunk];
+                }
+            float top = st[0].x;
+#pragma unroll
+            for (int i = 1; i < kFew; ++i)
+                if (i < parts) top = fmaxf(top, st[i].x);
+            float total = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < kFew; ++i)
+                if (i < parts) {
+                    const float f = st[i].x == top ? 1.0f : dev::ex2(st[i].x - top);
+                    total += st[i].y * f;
+                    v.x += x[i].x * f, v.y += x[i].y * f, v.z += x[i].z * f, v.w += x[i].w * f;
+                }
+            store_joined<ROWS, D>(p, unit, view, r, chunk, v, top, total);
+        }
+        return;
+    }
     for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-        // the common maximum and the sum
+        // the common maximum
         float top = __int_as_float(0xff800000);
         for (int i = tid; i < parts; i += 128) top = fmaxf(top, p.part_stat[slot(i) * ROWS + r].x);
 #pragma unroll
@@ -342,7 +382,6 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionPara
             v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
         }
         sums[sub][chunk] = v;
-        // every thread of a sub has the same total
         if (chunk == 0) sub_totals[sub] = total;
         __syncthreads();
         if (tid < kLanes) {
@@ -354,12 +393,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionPara
                 v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
                 total += sub_totals[i];
             }
-            const int row = unit.y * ROWS + r, j = row / p.group;
-            const int head = unit.z * p.group + (row - j * p.group);
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            dev::store4(p, view.row0 + j, head, chunk * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-            if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
+            store_joined<ROWS, D>(p, unit, view, r, chunk, v, top, total);
         }
         __syncthreads();  // before the shared sums are written again
     }
