@@ -277,8 +277,7 @@ __device__ __forceinline__ void walk_on(const AttentionParams& p, Walk& w) {
 }
 
 // Four consecutive features of an output row.
-__device__ __forceinline__ void store4(const AttentionParams& p, int64_t token, int head, int feature, float4 v) {
-    const int64_t at = token * p.out_token + (int64_t)head * p.out_head + feature;
+__device__ __forceinline__ void store4_at(const AttentionParams& p, int64_t at, float4 v) {
     uint16_t h[4];
     if (p.dtype == MXK_F16) {
         h[0] = __half_as_ushort(__float2half_rn(v.x)), h[1] = __half_as_ushort(__float2half_rn(v.y));
@@ -294,6 +293,10 @@ __device__ __forceinline__ void store4(const AttentionParams& p, int64_t token, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = h[i];
     }
+}
+
+__device__ __forceinline__ void store4(const AttentionParams& p, int64_t token, int head, int feature, float4 v) {
+    store4_at(p, token * p.out_token + (int64_t)head * p.out_head + feature, v);
 }
 
 // log(sum exp) of a row from its running maximum (log2 units) and sum.

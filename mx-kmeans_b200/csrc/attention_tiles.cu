@@ -644,56 +644,119 @@ __device__ __noinline__ uint4 nan_features(const uint8_t* values, const int* tab
     return make_uint4(bad[0], bad[1], bad[2], bad[3]);
 }
 
-// This row's query into shared memory, scaled by a power of two to a largest magnitude in
-// [2^12, 2^13); a negative scale of the scores goes into its sign.  Returns the factor
-// that makes scores of its products with lifted keys, less the keys' reference.
+// The warp's 32 query rows into shared memory, each scaled by a power of two to a largest
+// magnitude in [2^12, 2^13); a negative scale of the scores goes into their sign.  Lane i
+// names row i (`at`, elements from p.q; `real`: it exists, else zeros) and gets the factor
+// that makes scores of its products with lifted keys, less the keys' reference.  D / 4
+// lanes load a row together: a thread that loads its own row touches 32 of them in every
+// access and takes ten times as long.
 template <int D>
-__device__ __forceinline__ float put_query(const AttentionParams& p, int64_t at, bool real, uint8_t* dst, int r) {
-    const uint16_t* q = static_cast<const uint16_t*>(p.q) + at;
-    uint32_t x[D / 2];
+__device__ __forceinline__ float put_queries(const AttentionParams& p, int64_t at, bool real, uint8_t* rows, int r0) {
+    constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes, kBatch = 8;
+    const int lane = threadIdx.x & 31, piece = lane % kLanes, sub = lane / kLanes;
+    const unsigned mask = kAtOnce == 1 ? kFull : 0xffffu << (16 * sub);
+    const unsigned reals = __ballot_sync(kFull, real);
+    const bool f16 = p.dtype == MXK_F16;
+    unsigned own = 0;  // the largest magnitude of this lane's row, as bits
+    auto fetch = [&](int base, uint2 (&x)[kBatch]) {
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-        x[2 * i] = x[2 * i + 1] = 0;
-        if (real) {
-            if (p.q_vec) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(q) + i);
-                x[2 * i] = v.x, x[2 * i + 1] = v.y;
+        for (int i = 0; i < kBatch; ++i) {
+            const int r = base + i * kAtOnce + sub;
+            const int64_t row = __shfl_sync(kFull, at, r);
+            x[i] = make_uint2(0, 0);
+            if (reals >> r & 1u) {
+                const uint16_t* q = static_cast<const uint16_t*>(p.q) + row + 4 * piece;
+                if (p.q_vec)
+                    x[i] = __ldg(reinterpret_cast<const uint2*>(q));
+                else
+                    x[i] = make_uint2(q[0] | ((uint32_t)q[1] << 16), q[2] | ((uint32_t)q[3] << 16));
+            }
+        }
+    };
+    auto factors = [&](unsigned amax, float& f0, float& f1) -> float {
+        const int e = amax ? max((int)(amax >> 23) - 127, -126) : 0;
+        const int down = (kQueryExp - e) / 2, rest = kQueryExp - e - down;
+        f0 = __uint_as_float((uint32_t)(down + 127) << 23);
+        f1 = copysignf(__uint_as_float((uint32_t)(rest + 127) << 23), p.scale_log2);
+        return fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 - down - kKeyLift / 2) << 23) *
+               __uint_as_float((uint32_t)(127 - rest - kKeyLift / 2) << 23);
+    };
+    // Rows past the last real one are left as they are: a row's scores are its own.
+    const int rows_here = 32 - __clz(reals);
+    uint2 next[kBatch];
+    fetch(0, next);
+#pragma unroll 1
+    for (int base = 0; base < rows_here; base += kBatch * kAtOnce) {
+        float4 x[kBatch];
+        unsigned amax[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            float2 u, v;
+            if (f16) {
+                u = __half22float2(*reinterpret_cast<const __half2*>(&next[i].x));
+                v = __half22float2(*reinterpret_cast<const __half2*>(&next[i].y));
             } else {
-                x[2 * i] = q[4 * i] | ((uint32_t)q[4 * i + 1] << 16);
-                x[2 * i + 1] = q[4 * i + 2] | ((uint32_t)q[4 * i + 3] << 16);
+                u = make_float2(__uint_as_float(next[i].x << 16), __uint_as_float(next[i].x & 0xffff0000u));
+                v = make_float2(__uint_as_float(next[i].y << 16), __uint_as_float(next[i].y & 0xffff0000u));
+            }
+            x[i] = make_float4(u.x, u.y, v.x, v.y);
+        }
+        if (base + kBatch * kAtOnce < rows_here) fetch(base + kBatch * kAtOnce, next);
+        // non-negative floats order as their bits (a NaN's row is NaN whatever its scale)
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            amax[i] = __reduce_max_sync(mask, __float_as_uint(fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)),
+                                                                    fmaxf(fabsf(x[i].z), fabsf(x[i].w)))));
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            float f0, f1;
+            factors(amax[i], f0, f1);
+            const __half2 a = __floats2half2_rn(x[i].x * f0 * f1, x[i].y * f0 * f1);
+            const __half2 b = __floats2half2_rn(x[i].z * f0 * f1, x[i].w * f0 * f1);
+            const int chunk = piece / 2, row = r0 + base + i * kAtOnce + sub;
+            *reinterpret_cast<uint2*>(rows + (chunk / 8) * Smem<D>::half + row * 128 +
+                                      (((chunk % 8) ^ (row & 7)) << 4) + (piece & 1) * 8) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const unsigned m = kAtOnce == 1 ? amax[i] : __shfl_sync(kFull, amax[i], 16 * k);
+                if (lane == base + i * kAtOnce + k) own = m;
             }
         }
     }
-    const bool f16 = p.dtype == MXK_F16;
-    auto pair = [&](uint32_t v) -> float2 {
-        if (f16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-    };
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 2; ++i) {
-        const float2 v = pair(x[i]);
-        amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+    float f0, f1;
+    return factors(own, f0, f1);
+}
+
+// A warp's 32 output rows from shared memory to where they belong, D / 8 lanes a row:
+// columns [col, col + D / 2), four a lane, staged by their owners with the 16-byte chunks
+// permuted by row.
+template <int D>
+__device__ __forceinline__ void put_rows(const AttentionParams& p, const float4* stage, unsigned reals, int64_t out_at,
+                                         float* part, int col) {
+    constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+    const int lane = threadIdx.x & 31, piece = lane % kLanes, sub = lane / kLanes;
+    const int rows_here = 32 - __clz(reals);
+    if (part) {
+#pragma unroll 4
+        for (int r = sub; r < rows_here; r += kAtOnce)
+            *reinterpret_cast<float4*>(part + r * D + col + 4 * piece) = stage[r * kLanes + (piece ^ (r & 7))];
+        return;
     }
-    int e = amax > 0.0f ? (int)(__float_as_uint(amax) >> 23) - 127 : 0;
-    e = max(e, -126);
-    const int down = (kQueryExp - e) / 2, rest = kQueryExp - e - down;
-    const float f0 = __uint_as_float((uint32_t)(down + 127) << 23);
-    const float f1 = copysignf(__uint_as_float((uint32_t)(rest + 127) << 23), p.scale_log2);
+#pragma unroll 1
+    for (int base = 0; base < rows_here; base += 4 * kAtOnce) {
+        int64_t at[4];
+        float4 v[4];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-        uint32_t h[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 v = pair(x[4 * i + k]);
-            const __half2 u = __floats2half2_rn(v.x * f0 * f1, v.y * f0 * f1);
-            h[k] = *reinterpret_cast<const uint32_t*>(&u);
+        for (int i = 0; i < 4; ++i) {
+            const int r = base + i * kAtOnce + sub;
+            at[i] = __shfl_sync(kFull, out_at, r);
+            v[i] = stage[r * kLanes + (piece ^ (r & 7))];
         }
-        *reinterpret_cast<uint4*>(dst + (i / 8) * Smem<D>::half + (((i % 8) ^ (r & 7)) << 4)) =
-            make_uint4(h[0], h[1], h[2], h[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (reals >> (base + i * kAtOnce + sub) & 1u) dev::store4_at(p, at[i] + col + 4 * piece, v[i]);
     }
-    return fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 - down - kKeyLift / 2) << 23) *
-           __uint_as_float((uint32_t)(127 - rest - kKeyLift / 2) << 23);
 }
 
 // READY: tiles were converted beforehand, their references lie in global memory.
@@ -723,9 +786,9 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             int lo = 0, hi = c.w.view.len;
             if (real) dev::seen_range(p, c.w.view, j, j, lo, hi);
             const int first_key = (c.w.first + c.tile0) * kKeys;
-            const float row_factor =
-                put_query<D>(p, (int64_t)(c.w.view.row0 + j) * p.q_token + (int64_t)head * p.q_head, real,
-                             b.smem + L::q + w * L::tile + r * 128, r);
+            const float row_factor = !warp_real ? 0.0f :
+                put_queries<D>(p, (int64_t)(c.w.view.row0 + j) * p.q_token + (int64_t)head * p.q_head, real,
+                               b.smem + L::q + w * L::tile, r & ~31);
             dev::fence_proxy_async();
             dev::mbar_arrive(&sh->q_ready[w]);
 
@@ -851,28 +914,36 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                 const float inv = all ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
                 const int64_t slot = 2 * (int64_t)blockIdx.x + (c.tile0 == 0 ? 1 : 0);
                 const int tile_row = w * kTileRows + r;
+                const unsigned reals = __ballot_sync(kFull, real);
+                const int64_t out_at = (int64_t)(c.w.view.row0 + j) * p.out_token + (int64_t)head * p.out_head;
+                float* part = all ? nullptr : p.part + (slot * kRows + (tile_row & ~31)) * D;
+                // The rows leave through the queries' shared memory, which no product reads any
+                // more: a warp's quarter of the row tile holds 32 rows of D / 2 floats.
+                float4* stage = reinterpret_cast<float4*>(b.smem + L::q + w * L::tile + (warp & 3) * (L::tile / 4));
 #pragma unroll
                 for (int h = 0; h < D / 32; ++h) {
                     uint32_t o[32];
                     dev::tmem_ld_32x32b_x32(o_col + 32 * h, o);
                     dev::tmem_wait_ld();
-                    if (real) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float v = __uint_as_float(o[i]) * inv * vfactor;
-                            if (sum == 0.0f) v = 0.0f;
-                            if (bad[h] >> i & 1u) v = __int_as_float(0x7fc00000);
-                            o[i] = __float_as_uint(v);
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 v = make_float4(__uint_as_float(o[i]) * inv * vfactor, __uint_as_float(o[i + 1]) * inv * vfactor,
+                                               __uint_as_float(o[i + 2]) * inv * vfactor, __uint_as_float(o[i + 3]) * inv * vfactor);
+                        if (sum == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (nans) {
+                            const float nan = __int_as_float(0x7fc00000);
+                            if (bad[h] >> i & 1u) v.x = nan;
+                            if (bad[h] >> (i + 1) & 1u) v.y = nan;
+                            if (bad[h] >> (i + 2) & 1u) v.z = nan;
+                            if (bad[h] >> (i + 3) & 1u) v.w = nan;
                         }
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 v = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
-                                                         __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-                            if (all)
-                                dev::store4(p, c.w.view.row0 + j, head, 32 * h + i, v);
-                            else
-                                *reinterpret_cast<float4*>(p.part + (slot * kRows + tile_row) * D + 32 * h + i) = v;
-                        }
+                        const int chunk = (h % (D / 64)) * 8 + i / 4;
+                        stage[(r & 31) * (D / 8) + (chunk ^ (r & 7))] = v;
+                    }
+                    if ((h + 1) % (D / 64) == 0) {
+                        __syncwarp();
+                        put_rows<D>(p, stage, reals, out_at, part, (h / (D / 64)) * (D / 2));
+                        __syncwarp();
                     }
                 }
                 if (real) {
