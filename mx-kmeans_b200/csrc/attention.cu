@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     const uint32_t ks_read = ring + S::ks_at + g * S::scale_bytes + (D == 128 ? c : c >> 1);
     const uint32_t vs_read = ring + S::vs_at + 2 * c * S::scale_bytes + (D == 128 ? g >> 1 : g >> 2);
 
+    dev::let_next_start();
     const dev::Share share = dev::take_share<kRows, kKeys, kThreads>(p, scratch);
     if (share.tiles == 0) {
         if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);

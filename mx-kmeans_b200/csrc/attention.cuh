@@ -75,6 +75,12 @@ namespace dev {
 constexpr float kExpShift = 11.0f;
 constexpr float kMaxSlack = 4.0f;
 
+// The kernels of a call follow one another with programmatic launches: a kernel lets the
+// next one be set up as soon as all its own CTAs have started, and the next one waits, before
+// it touches anything written here, until this one has finished.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -331,7 +337,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionPara
     constexpr int kFew = 8;
     __shared__ float4 sums[kSub][kLanes];
     __shared__ float stats[4], sub_totals[kSub];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    dev::wait_for_previous();
     const int4 unit = p.part_open[blockIdx.x];
     if (!unit.w) return;
     const dev::SeqView view = dev::seq_view(p, unit.x);

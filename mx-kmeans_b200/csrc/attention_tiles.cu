@@ -311,6 +311,7 @@ static_assert(kRefStep == 4, "value_ref rounds to multiples of four");
 template <int D, int BITS>
 __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionParams p) {
     using C = Converter<D, BITS>;
+    dev::let_next_start();
     const int tile = blockIdx.x % p.max_tiles, sh = blockIdx.x / p.max_tiles;
     const int seq = sh / p.kv_heads, head = sh - seq * p.kv_heads;
     const dev::SeqView view = dev::seq_view(p, seq);
@@ -974,6 +975,7 @@ template <int D, class Cfg, int FULL_COUNT>
 __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_raw, Shared* sh, int* scratch,
                                       unsigned* err, Block& b, Cursor& c) {
     const int tid = threadIdx.x;
+    dev::let_next_start();
     const dev::Share share = dev::take_share<kRows, kKeys, Cfg::threads>(p, scratch);
     if (share.tiles == 0) {
         if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -1058,7 +1060,7 @@ __global__ void __launch_bounds__(Ready::threads, 1) attention_ready_kernel(cons
     Block b;
     Cursor c;
     if (!begin<D, Ready, 1>(p, smem_raw, &shared, scratch, err, b, c)) return;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the converted tiles
+    dev::wait_for_previous();  // the converted tiles
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
     if (warp < kSoftmaxWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Ready::softmax_regs));
