@@ -8,8 +8,8 @@
 // bytes over HBM bandwidth bound it: 2 * (D * bits / 8 + D / 32) per token and key
 // head.  attention_rows_kernel keeps that stream busy:
 //
-//  * A CTA of four warps; every warp streams its own 16-token granules through its
-//    own ring of shared-memory stages (16-byte asynchronous copies, no barrier
+//  * A CTA of four warps; every warp streams its own pairs of 16-token granules through
+//    its own ring of shared-memory stages (16-byte asynchronous copies, no barrier
 //    between warps) and keeps its own running maximum, sum and output rows in
 //    registers.  The warps join once per unit.
 //  * Products are m16n8k16 f16 with the 16 query rows as M.  Tensor throughput is
@@ -47,24 +47,27 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kRows = 16;     // query rows of a unit
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kGranule = 16;  // tokens of one step of a warp
-constexpr int kKeys = kGranule * kWarps;
-constexpr int kCtasPerSm = 4;
+constexpr int kGranule = 16;     // tokens of one product, contiguous in their page
+constexpr int kGranules = 2;     // of one step of a warp
+constexpr int kPair = kGranule * kGranules;
+constexpr int kKeys = kPair * kWarps;
+constexpr int kCtasPerSm = 3;
 // Rows per key head up to which this kernel is taken, one pass over the keys for
 // every 16 of them.
 constexpr int kMostFewRows = 32;
 
-// Shared-memory row pitches (bytes) of the key and value granules; each makes the
-// lanes of one load instruction touch all banks once.  Keys are read row by row,
-// a quarter per lane; values four rows per lane, an eighth each.
+// Shared-memory row pitches (bytes) of the key and value granules.  Keys are read row by
+// row, a quarter per lane; values four rows per lane, an eighth each.  The pitches make the
+// lanes of one load touch all banks once; 128-byte rows, for which a gap would cost the
+// third CTA of an SM, have their 16-byte chunks permuted by row instead.
 template <int D, int BITS>
 struct Pitch;
-template <> struct Pitch<128, 8> { static constexpr int k = 144, v = 144; };
-template <> struct Pitch<128, 6> { static constexpr int k = 96, v = 112; };
-template <> struct Pitch<128, 4> { static constexpr int k = 64, v = 80; };
-template <> struct Pitch<64, 8> { static constexpr int k = 64, v = 80; };
-template <> struct Pitch<64, 6> { static constexpr int k = 48, v = 48; };
-template <> struct Pitch<64, 4> { static constexpr int k = 32, v = 48; };
+template <> struct Pitch<128, 8> { static constexpr int k = 128, v = 128; static constexpr bool swizzled = true; };
+template <> struct Pitch<128, 6> { static constexpr int k = 96, v = 112; static constexpr bool swizzled = false; };
+template <> struct Pitch<128, 4> { static constexpr int k = 64, v = 80; static constexpr bool swizzled = false; };
+template <> struct Pitch<64, 8> { static constexpr int k = 64, v = 80; static constexpr bool swizzled = false; };
+template <> struct Pitch<64, 6> { static constexpr int k = 48, v = 48; static constexpr bool swizzled = false; };
+template <> struct Pitch<64, 4> { static constexpr int k = 32, v = 48; static constexpr bool swizzled = false; };
 
 template <int D, int BITS>
 struct Stage {
@@ -74,12 +77,13 @@ struct Stage {
     static constexpr int v_at = kGranule * Pitch<D, BITS>::k;
     static constexpr int ks_at = v_at + kGranule * Pitch<D, BITS>::v;
     static constexpr int vs_at = ks_at + kGranule * scale_bytes;
-    static constexpr int bytes = vs_at + kGranule * scale_bytes;
+    static constexpr int granule = vs_at + kGranule * scale_bytes;
+    static constexpr int bytes = kGranules * granule;
     static constexpr int stages = 2;
     static constexpr int ring = kWarps * stages * bytes;
     static constexpr int join = kWarps * kRows * D * 4;  // the warps' outputs, after the ring is done
     static constexpr int smem = ring > join ? ring : join;
-    static_assert(bytes % 16 == 0, "stages start on 16-byte boundaries");
+    static_assert(granule % 16 == 0, "granules start on 16-byte boundaries");
 };
 
 // 16 bytes to shared memory, the first `bytes` of them from src, the rest zero.  The
@@ -171,16 +175,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     constexpr int vStep = P::v == S::row ? 512 : 32 / S::chunks * P::v;
     static_assert(P::k == S::row || 32 % S::chunks == 0, "key rows without gaps, or whole rows in a copy");
     constexpr bool vEven = P::v == S::row || 32 % S::chunks == 0;
-    auto v_place = [&](int i) -> uint32_t { const int x = lane + 32 * i; return x / S::chunks * P::v + x % S::chunks * 16; };
-    const uint32_t k_lane = ring + (P::k == S::row ? lane * 16 : lane / S::chunks * P::k + lane % S::chunks * 16);
-    uint32_t v_lane[vEven ? 1 : kCopies];
+    constexpr int kPlaces = P::swizzled ? 2 : 1;               // rows of copy i: lane / 8 + 4 i
+    constexpr int vPlaces = P::swizzled ? 2 : (vEven ? 1 : kCopies);
+    uint32_t k_lane[kPlaces], v_lane[vPlaces];
+    if constexpr (P::swizzled) {
 #pragma unroll
-    for (int i = 0; i < (vEven ? 1 : kCopies); ++i)
-        v_lane[i] = ring + S::v_at + (P::v == S::row ? lane * 16 : v_place(i));
-    static_assert(P::k % widest(kShare) == 0 && P::v % widest(vShare) == 0 && S::v_at % 16 == 0 && S::bytes % 16 == 0,
+        for (int i = 0; i < 2; ++i) {
+            k_lane[i] = ring + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) + 4 * i)) << 4);
+            v_lane[i] = k_lane[i] + S::v_at;
+        }
+    } else {
+        k_lane[0] = ring + (P::k == S::row ? lane * 16 : lane / S::chunks * P::k + lane % S::chunks * 16);
+#pragma unroll
+        for (int i = 0; i < vPlaces; ++i) {
+            const int x = lane + 32 * i;
+            v_lane[i] = ring + S::v_at + (P::v == S::row ? lane * 16 : x / S::chunks * P::v + x % S::chunks * 16);
+        }
+    }
+    static_assert(P::k % widest(kShare) == 0 && P::v % widest(vShare) == 0 && S::v_at % 16 == 0 && S::granule % 16 == 0,
                   "reads are aligned to their width");
-    const uint32_t k_read = ring + g * P::k + c * kShare;
-    const uint32_t v_read = ring + S::v_at + 2 * c * P::v + g * vShare;
+    // Where this lane reads: 16-byte halves of its key share; its even and odd tokens' values.
+    uint32_t k_read[2], v_read[2];
+    k_read[0] = ring + g * P::k + (P::swizzled ? (2 * c ^ g) << 4 : c * kShare);
+    k_read[1] = ring + g * P::k + ((2 * c + 1) ^ g) * 16;  // swizzled rows only
+    v_read[0] = ring + S::v_at + 2 * c * P::v + (P::swizzled ? (g ^ 2 * c) << 4 : g * vShare);
+    v_read[1] = ring + S::v_at + (2 * c + 1) * P::v + (P::swizzled ? (g ^ (2 * c + 1)) << 4 : g * vShare);
     const uint32_t ks_read = ring + S::ks_at + g * S::scale_bytes + (D == 128 ? c : c >> 1);
     const uint32_t vs_read = ring + S::vs_at + 2 * c * S::scale_bytes + (D == 128 ? g >> 1 : g >> 2);
 
@@ -223,18 +242,32 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             dev::seen_range(p, w.view, j1, j1, all_lo, x);       // the last begins last
         }
 
-        // The warp's granules: numbers gran0, gran0 + 4, ... of the sequence below `end`.
+        // The warp's pairs of granules: numbers pair0, pair0 + 4, ... of the sequence below `end`.
         // A granule is contiguous in its page, so a lane copies 16 bytes every 512.
-        const int gran0 = (w.first + tile0) * kWarps + warp;
-        const int end = min((w.first + tile0 + tiles) * kWarps,
-                            any_hi <= any_lo ? 0 : (any_hi + kGranule - 1) / kGranule);
-        const int steps = end > gran0 ? (end - gran0 + kWarps - 1) / kWarps : 0;
+        const int pair0 = (w.first + tile0) * kWarps + warp;
+        const int end = min((w.first + tile0 + tiles) * kWarps, any_hi <= any_lo ? 0 : (any_hi + kPair - 1) / kPair);
+        const int steps = end > pair0 ? (end - pair0 + kWarps - 1) / kWarps : 0;
         const int* table = p.page_table + (int64_t)w.seq * p.table_stride;
         const int per_page = p.page_size / kGranule;
-        const int jump = kWarps / per_page, rest = kWarps - jump * per_page;  // pages and granules of one step
-        int next_at = gran0 / per_page, next_in = gran0 - next_at * per_page;  // page and granule of the next copy
-        auto next_page = [&](int step) -> int {
-            return step < steps ? min(max(__ldg(table + next_at), 0), p.pages - 1) : 0;
+        // pages and granules from a step's first granule to the next step's
+        const int jump = kWarps * kGranules / per_page, rest = kWarps * kGranules - jump * per_page;
+        int next_at = pair0 * kGranules / per_page, next_in = pair0 * kGranules - next_at * per_page;
+        struct Pages {
+            int page[2];
+            int in[2];  // the granules' places in them
+        };
+        auto next_pages = [&](int step) -> Pages {
+            Pages n{{0, 0}, {next_in, next_in + 1}};
+            if (step < steps) {
+                const bool over = n.in[1] == per_page;
+                if (over) n.in[1] = 0;
+                n.page[0] = n.page[1] = min(max(__ldg(table + next_at), 0), p.pages - 1);
+                if (over && (pair0 + step * kWarps) * kPair + kGranule < len)
+                    n.page[1] = min(max(__ldg(table + next_at + 1), 0), p.pages - 1);
+                next_at += jump, next_in += rest;
+                if (next_in >= per_page) next_in -= per_page, ++next_at;
+            }
+            return n;
         };
         // The lane's first bytes of page 0 of the head, and where the scales go.
         constexpr int sc = kGranule * S::scale_bytes / 16;  // 16-byte pieces of a side's scales
@@ -244,43 +277,47 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         const uint8_t* s_src = (lane < sc ? p.k_scales : p.v_scales - sc * 16) + head_row * S::scale_bytes + lane * 16;
         const uint32_t page_rows = (uint32_t)p.kv_heads * p.page_size;
         int copy_stage = 0;  // offset of the stage to copy to
-        auto copy_side = [&](auto index, const uint8_t* k, const uint8_t* v, int valid) {
-            constexpr int i = decltype(index)::value;
-            if (kPieces % 32 == 0 || lane + 32 * i < kPieces) {
-                const uint32_t to_k = k_lane + copy_stage, to_v = v_lane[vEven ? 0 : i] + copy_stage;
-                constexpr int v_off = vEven ? i * vStep : 0;
+        auto copy_piece = [&](auto index, auto granule, const uint8_t* k, const uint8_t* v, int valid) {
+            constexpr int i = decltype(index)::value, at = decltype(granule)::value * S::granule;
+            if (i < kCopies && (kPieces % 32 == 0 || lane + 32 * i < kPieces)) {
+                const uint32_t to_k = k_lane[P::swizzled ? i & 1 : 0] + copy_stage;
+                const uint32_t to_v = v_lane[P::swizzled ? i & 1 : (vEven ? 0 : i)] + copy_stage;
+                constexpr int v_off = at + (vEven ? i * vStep : 0);
                 if (valid >= kGranule) {
-                    copy16<i * kStep, 512 * i>(to_k, k);
+                    copy16<at + i * kStep, 512 * i>(to_k, k);
                     copy16<v_off, 512 * i>(to_v, v);
                 } else {  // rows past the sequence's end are zeros
                     const int bytes = (lane + 32 * i) / S::chunks < valid ? 16 : 0;
-                    copy16<i * kStep, 512 * i>(to_k, k, bytes);
+                    copy16<at + i * kStep, 512 * i>(to_k, k, bytes);
                     copy16<v_off, 512 * i>(to_v, v, bytes);
                 }
             }
         };
-        auto issue = [&](int step, int page) {
+        auto copy_granule = [&](auto granule, int page, int in, int valid) {
+            constexpr int gi = decltype(granule)::value;
+            const uint32_t row = (uint32_t)page * page_rows + (uint32_t)in * kGranule;
+            const uint8_t* k = k_src + (uint64_t)row * S::row;
+            const uint8_t* v = v_src + (uint64_t)row * S::row;
+            static_assert(kCopies <= 4, "");
+            copy_piece(std::integral_constant<int, 0>{}, granule, k, v, valid);
+            copy_piece(std::integral_constant<int, 1>{}, granule, k, v, valid);
+            copy_piece(std::integral_constant<int, 2>{}, granule, k, v, valid);
+            copy_piece(std::integral_constant<int, 3>{}, granule, k, v, valid);
+            if (lane < 2 * sc)
+                copy16<S::ks_at + gi * S::granule, 0>(ring + copy_stage + lane * 16, s_src + (uint64_t)row * S::scale_bytes);
+        };
+        auto issue = [&](int step, const Pages& n) {
             if (step < steps) {
-                const uint32_t row = (uint32_t)page * page_rows + (uint32_t)next_in * kGranule;
-                const uint8_t* k = k_src + (uint64_t)row * S::row;
-                const uint8_t* v = v_src + (uint64_t)row * S::row;
-                const int valid = len - (gran0 + step * kWarps) * kGranule;
-                copy_side(std::integral_constant<int, 0>{}, k, v, valid);
-                if constexpr (kCopies > 1) copy_side(std::integral_constant<int, 1>{}, k, v, valid);
-                if constexpr (kCopies > 2) copy_side(std::integral_constant<int, 2>{}, k, v, valid);
-                if constexpr (kCopies > 3) copy_side(std::integral_constant<int, 3>{}, k, v, valid);
-                if (lane < 2 * sc)
-                    copy16<S::ks_at, 0>(ring + copy_stage + lane * 16, s_src + (uint64_t)row * S::scale_bytes);
-                next_at += jump, next_in += rest;
-                if (next_in >= per_page) next_in -= per_page, ++next_at;
+                const int valid = len - (pair0 + step * kWarps) * kPair;
+                copy_granule(std::integral_constant<int, 0>{}, n.page[0], n.in[0], valid);
+                copy_granule(std::integral_constant<int, 1>{}, n.page[1], n.in[1], valid - kGranule);
                 copy_stage = copy_stage == (S::stages - 1) * S::bytes ? 0 : copy_stage + S::bytes;
             }
             copy_commit();
         };
-        static_assert(kCopies <= 4, "");
 #pragma unroll
-        for (int s = 0; s < S::stages - 1; ++s) issue(s, next_page(s));
-        int page = next_page(S::stages - 1);
+        for (int s = 0; s < S::stages - 1; ++s) issue(s, next_pages(s));
+        Pages pages = next_pages(S::stages - 1);
 
         // q as the A operand: features c * D/4 + 4 i .. + 3 of rows g, g + 8 at step i.
         uint32_t qa[kSteps / kWarps][4];  // those of this warp's k-steps
@@ -351,60 +388,97 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         for (int step = 0; step < steps; ++step) {
             copy_wait<S::stages - 2>();
             __syncwarp();
-            issue(step + S::stages - 1, page);
-            page = next_page(step + S::stages);
+            issue(step + S::stages - 1, pages);
+            pages = next_pages(step + S::stages);
             const int now = stage;
             stage = stage == (S::stages - 1) * S::bytes ? 0 : stage + S::bytes;
-            const int t0 = (gran0 + step * kWarps) * kGranule;
+            const int t0 = (pair0 + step * kWarps) * kPair;
+            const bool last = t0 + kPair > len;
 
-            // The keys' reference: the granule's largest scale.
-            const bool last = t0 + kGranule > len;
-            int ks[2] = {lds_u8<0>(ks_read + now), lds_u8<8 * S::scale_bytes>(ks_read + now)};
-            if (last) {  // the keys past the sequence's end are zero
-                if (t0 + g >= len) ks[0] = 0;
-                if (t0 + g + 8 >= len) ks[1] = 0;
+            // The references of the keys, the step's largest scale, and of the values, which
+            // moves up with the data.  (What lies past the sequence's end is zero.)
+            int ks[4], vs[8];
+            ks[0] = lds_u8<0>(ks_read + now), ks[1] = lds_u8<8 * S::scale_bytes>(ks_read + now);
+            ks[2] = lds_u8<S::granule>(ks_read + now), ks[3] = lds_u8<S::granule + 8 * S::scale_bytes>(ks_read + now);
+            vs[0] = lds_u8<0>(vs_read + now), vs[1] = lds_u8<S::scale_bytes>(vs_read + now);
+            vs[2] = lds_u8<8 * S::scale_bytes>(vs_read + now), vs[3] = lds_u8<9 * S::scale_bytes>(vs_read + now);
+            vs[4] = lds_u8<S::granule>(vs_read + now), vs[5] = lds_u8<S::granule + S::scale_bytes>(vs_read + now);
+            vs[6] = lds_u8<S::granule + 8 * S::scale_bytes>(vs_read + now);
+            vs[7] = lds_u8<S::granule + 9 * S::scale_bytes>(vs_read + now);
+            if (last) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t0 + g + 8 * i >= len) ks[i] = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (t0 + 2 * c + (i & 1) + 8 * (i >> 1) >= len) vs[i] = 0;
             }
-            const int kref = max((int)__reduce_max_sync(kFull, (unsigned)max(ks[0], ks[1])), 1);
-            const float kfactor = __uint_as_float((uint32_t)kref << 23);
-            const float fa = row_factor[0] * kfactor, fb = row_factor[1] * kfactor;
-
-            // scores: 16 rows x 2 tiles of 8 tokens
-            float s[2][4];
-            uint32_t key_words[2][(kShare + 3) / 4];
-            lds_bytes<kShare, 0>(k_read + now, key_words[0]);
-            lds_bytes<kShare, 8 * P::k>(k_read + now, key_words[1]);
-            const uint32_t kf[2] = {pow2_f16x2(ks[0] - kref + kKeyLift, ks[0] - kref + kKeyLift),
-                                    pow2_f16x2(ks[1] - kref + kKeyLift, ks[1] - kref + kKeyLift)};
+            const int kref = max((int)__reduce_max_sync(kFull, (unsigned)max(max(ks[0], ks[1]), max(ks[2], ks[3]))), 1);
+            const int vtop = (int)__reduce_max_sync(kFull, (unsigned)max(max(max(vs[0], vs[1]), max(vs[2], vs[3])),
+                                                                         max(max(vs[4], vs[5]), max(vs[6], vs[7]))));
+            if (vref == 0 || vtop > vref + kValueMax) {
+                const int ref = max(vtop - kValueLift, 1);
+                if (vref != 0) {
+                    const float f = __uint_as_float((uint32_t)max(vref - ref + 127, 0) << 23);
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+                    for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-            for (int k = 0; k < kSteps; k += 2) {
-                uint32_t qa[2][4];
-                lds_at(q_read + 512 * k, qa[0]);
-                lds_at(q_read + 512 * (k + 1), qa[1]);
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    uint32_t h[4];
-                    if constexpr (BITS == 4) {
-                        dev::e2m1x8_to_f16(key_words[nt][k / 2], h);
-                    } else {
-                        constexpr int kCode = BITS == 4 ? 8 : BITS;
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t four = BITS == 8 ? key_words[nt][k + i] : four6(key_words[nt], k + i);
-                            h[2 * i] = dev::codes_to_f16x2<kCode>(four), h[2 * i + 1] = dev::codes_to_f16x2<kCode>(four >> 16);
-                        }
-                    }
-                    mma16816(s[nt], qa[0], hmul2(h[0], kf[nt]), hmul2(h[1], kf[nt]));
-                    mma16816(s[nt], qa[1], hmul2(h[2], kf[nt]), hmul2(h[3], kf[nt]));
+                        for (int e = 0; e < 4; ++e) o[n][e] *= f;
                 }
+                vref = ref;
             }
+
+            // scores: 16 rows x 4 tiles of 8 tokens
+            float s[4][4];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) s[nt][0] *= fa, s[nt][1] *= fa, s[nt][2] *= fb, s[nt][3] *= fb;
-            const bool partly = t0 < all_lo || t0 + kGranule > all_hi;
-            if (partly) {
+            for (int h = 0; h < 2; ++h) {
+                uint32_t key_words[2][(kShare + 3) / 4];
+                const uint32_t at = now + h * S::granule;
+                if constexpr (P::swizzled) {
+                    lds_bytes<16, 0>(k_read[0] + at, key_words[0]), lds_bytes<16, 0>(k_read[1] + at, key_words[0] + 4);
+                    lds_bytes<16, 8 * P::k>(k_read[0] + at, key_words[1]);
+                    lds_bytes<16, 8 * P::k>(k_read[1] + at, key_words[1] + 4);
+                } else {
+                    lds_bytes<kShare, 0>(k_read[0] + at, key_words[0]);
+                    lds_bytes<kShare, 8 * P::k>(k_read[0] + at, key_words[1]);
+                }
+                const int e0 = ks[2 * h] - kref + kKeyLift, e1 = ks[2 * h + 1] - kref + kKeyLift;
+                const uint32_t kf[2] = {pow2_f16x2(e0, e0), pow2_f16x2(e1, e1)};
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt)
+                    s[2 * h + nt][0] = s[2 * h + nt][1] = s[2 * h + nt][2] = s[2 * h + nt][3] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kSteps; k += 2) {
+                    uint32_t qa[2][4];
+                    lds_at(q_read + 512 * k, qa[0]);
+                    lds_at(q_read + 512 * (k + 1), qa[1]);
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        uint32_t x[4];
+                        if constexpr (BITS == 4) {
+                            dev::e2m1x8_to_f16(key_words[nt][k / 2], x);
+                        } else {
+                            constexpr int kCode = BITS == 4 ? 8 : BITS;
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t four = BITS == 8 ? key_words[nt][k + i] : four6(key_words[nt], k + i);
+                                x[2 * i] = dev::codes_to_f16x2<kCode>(four);
+                                x[2 * i + 1] = dev::codes_to_f16x2<kCode>(four >> 16);
+                            }
+                        }
+                        mma16816(s[2 * h + nt], qa[0], hmul2(x[0], kf[nt]), hmul2(x[1], kf[nt]));
+                        mma16816(s[2 * h + nt], qa[1], hmul2(x[2], kf[nt]), hmul2(x[3], kf[nt]));
+                    }
+                }
+            }
+            const float kfactor = __uint_as_float((uint32_t)kref << 23);
+            const float fa = row_factor[0] * kfactor, fb = row_factor[1] * kfactor;
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt) s[nt][0] *= fa, s[nt][1] *= fa, s[nt][2] *= fb, s[nt][3] *= fb;
+            const bool partly = t0 < all_lo || t0 + kPair > all_hi;
+            if (partly) {
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int t = t0 + 8 * nt + 2 * c + (e & 1);
@@ -414,10 +488,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
 
             // Raise the maximum of the rows where some score exceeds it by more than the
             // slack (row by row: a row's result does not depend on its neighbours).
-            const float m0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-            const float m1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-            if (__any_sync(kFull, m0 > run_max[0] + kMaxSlack || m1 > run_max[1] + kMaxSlack)) {
-                float m[2] = {m0, m1};
+            float m[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                m[i] = fmaxf(fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1])),
+                             fmaxf(fmaxf(s[2][2 * i], s[2][2 * i + 1]), fmaxf(s[3][2 * i], s[3][2 * i + 1])));
+            if (__any_sync(kFull, m[0] > run_max[0] + kMaxSlack || m[1] > run_max[1] + kMaxSlack)) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     m[i] = fmaxf(m[i], __shfl_xor_sync(kFull, m[i], 1));
@@ -431,108 +507,98 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                     for (int n = 0; n < kTiles; ++n) o[n][2 * i] *= f, o[n][2 * i + 1] *= f;
                 }
             }
-            uint32_t pa[4];
+            uint32_t pa[2][4];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
+            for (int nt = 0; nt < 4; ++nt) {
                 const float p0 = ex2(s[nt][0] - base[0]), p1 = ex2(s[nt][1] - base[0]);
                 const float p2 = ex2(s[nt][2] - base[1]), p3 = ex2(s[nt][3] - base[1]);
                 sum[0] += p0 + p1, sum[1] += p2 + p3;
                 const __half2 a = __floats2half2_rn(p0, p1), b = __floats2half2_rn(p2, p3);
-                pa[2 * nt] = *reinterpret_cast<const uint32_t*>(&a);
-                pa[2 * nt + 1] = *reinterpret_cast<const uint32_t*>(&b);
+                pa[nt >> 1][2 * (nt & 1)] = *reinterpret_cast<const uint32_t*>(&a);
+                pa[nt >> 1][2 * (nt & 1) + 1] = *reinterpret_cast<const uint32_t*>(&b);
             }
 
-            // values: this lane's tokens 2c, 2c + 1, 2c + 8, 2c + 9
-            uint32_t vw[4][(vShare + 3) / 4];
-            int vs[4];
-            lds_bytes<vShare, 0>(v_read + now, vw[0]);
-            lds_bytes<vShare, P::v>(v_read + now, vw[1]);
-            lds_bytes<vShare, 8 * P::v>(v_read + now, vw[2]);
-            lds_bytes<vShare, 9 * P::v>(v_read + now, vw[3]);
-            vs[0] = lds_u8<0>(vs_read + now), vs[1] = lds_u8<S::scale_bytes>(vs_read + now);
-            vs[2] = lds_u8<8 * S::scale_bytes>(vs_read + now), vs[3] = lds_u8<9 * S::scale_bytes>(vs_read + now);
-            if (last) {  // as are the values
+            // values: of each granule this lane's tokens 2c, 2c + 1, 2c + 8, 2c + 9
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (t0 + 2 * c + (i & 1) + 8 * (i >> 1) >= len) vs[i] = 0;
-            }
-            const int top = (int)__reduce_max_sync(kFull, (unsigned)max(max(vs[0], vs[1]), max(vs[2], vs[3])));
-            if (vref == 0 || top > vref + kValueMax) {
-                const int ref = max(top - kValueLift, 1);
-                if (vref != 0) {
-                    const float f = __uint_as_float((uint32_t)max(vref - ref + 127, 0) << 23);
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t at = now + h * S::granule;
+                uint32_t vw[4][(vShare + 3) / 4];
+                lds_bytes<vShare, 0>(v_read[0] + at, vw[0]);
+                lds_bytes<vShare, 0>(v_read[1] + at, vw[1]);
+                lds_bytes<vShare, 8 * P::v>(v_read[0] + at, vw[2]);
+                lds_bytes<vShare, 8 * P::v>(v_read[1] + at, vw[3]);
+                const uint32_t f0 = pow2_f16x2(vs[4 * h] - vref, vs[4 * h + 1] - vref);
+                const uint32_t f1 = pow2_f16x2(vs[4 * h + 2] - vref, vs[4 * h + 3] - vref);
+                bool nans = false;
+                if constexpr (BITS == 8) {
+                    // A stored NaN belongs to the rows that see its token: where some row
+                    // does not, it is taken out here and put into the others' sums below.
+                    if (partly) {
 #pragma unroll
-                    for (int n = 0; n < kTiles; ++n)
+                        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[n][e] *= f;
+                            for (int j = 0; j < vShare / 4; ++j) {
+                                const uint32_t bad = __vcmpeq4(vw[i][j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                                nans |= bad != 0;
+                                vw[i][j] &= ~bad;
+                            }
+                        nans = __any_sync(kFull, nans);
+                    }
                 }
-                vref = ref;
-            }
-            const uint32_t f0 = pow2_f16x2(vs[0] - vref, vs[1] - vref), f1 = pow2_f16x2(vs[2] - vref, vs[3] - vref);
-            bool nans = false;
-            if constexpr (BITS == 8) {
-                // A stored NaN belongs to the rows that see its token: where some row
-                // does not, it is taken out here and put into the others' sums below.
-                if (partly) {
+                if constexpr (BITS == 4) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int j = 0; j < vShare / 4; ++j) {
+                        // bytes of (token, token + 1) nibbles: even features, then odd ones
+                        uint32_t even[2][4], odd[2][4];
 #pragma unroll
-                        for (int j = 0; j < vShare / 4; ++j) {
-                            const uint32_t bad = __vcmpeq4(vw[i][j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                            nans |= bad != 0;
-                            vw[i][j] &= ~bad;
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t a = vw[2 * i][j], b = vw[2 * i + 1][j];
+                            dev::e2m1x8_to_f16((a & 0x0f0f0f0fu) | ((b << 4) & 0xf0f0f0f0u), even[i]);
+                            dev::e2m1x8_to_f16(((a >> 4) & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u), odd[i]);
                         }
-                    nans = __any_sync(kFull, nans);
-                }
-            }
-            if constexpr (BITS == 4) {
 #pragma unroll
-                for (int j = 0; j < vShare / 4; ++j) {
-                    // bytes of (token, token + 1) nibbles: even features, then odd ones
-                    uint32_t even[2][4], odd[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t a = vw[2 * h][j], b = vw[2 * h + 1][j];
-                        dev::e2m1x8_to_f16((a & 0x0f0f0f0fu) | ((b << 4) & 0xf0f0f0f0u), even[h]);
-                        dev::e2m1x8_to_f16(((a >> 4) & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u), odd[h]);
+                        for (int i = 0; i < 4; ++i) {
+                            mma16816(o[8 * j + 2 * i], pa[h], hmul2(even[0][i], f0), hmul2(even[1][i], f1));
+                            mma16816(o[8 * j + 2 * i + 1], pa[h], hmul2(odd[0][i], f0), hmul2(odd[1][i], f1));
+                        }
                     }
+                } else {
+                    constexpr int kCode = BITS == 4 ? 8 : BITS;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        mma16816(o[8 * j + 2 * i], pa, hmul2(even[0][i], f0), hmul2(even[1][i], f1));
-                        mma16816(o[8 * j + 2 * i + 1], pa, hmul2(odd[0][i], f0), hmul2(odd[1][i], f1));
+                    for (int j = 0; j < D / 32; ++j) {
+                        uint32_t four[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) four[i] = BITS == 8 ? vw[i][j] : four6(vw[i], j);
+                        // (token, token + 1) bytes of features 0, 1 and of 2, 3
+                        const uint32_t a01 = __byte_perm(four[0], four[1], 0x5140);
+                        const uint32_t a23 = __byte_perm(four[0], four[1], 0x7362);
+                        const uint32_t b01 = __byte_perm(four[2], four[3], 0x5140);
+                        const uint32_t b23 = __byte_perm(four[2], four[3], 0x7362);
+                        mma16816(o[4 * j], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a01), f0),
+                                 hmul2(dev::codes_to_f16x2<kCode>(b01), f1));
+                        mma16816(o[4 * j + 1], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a01 >> 16), f0),
+                                 hmul2(dev::codes_to_f16x2<kCode>(b01 >> 16), f1));
+                        mma16816(o[4 * j + 2], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a23), f0),
+                                 hmul2(dev::codes_to_f16x2<kCode>(b23), f1));
+                        mma16816(o[4 * j + 3], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a23 >> 16), f0),
+                                 hmul2(dev::codes_to_f16x2<kCode>(b23 >> 16), f1));
                     }
                 }
-            } else {
-                constexpr int kCode = BITS == 4 ? 8 : BITS;
+                if (nans) {
+                    for (int t = 0; t < kGranule; ++t)
+                        for (int i = 0; i < 2; ++i) {
+                            if (t0 + h * kGranule + t < lo[i] || t0 + h * kGranule + t >= hi[i]) continue;
 #pragma unroll
-                for (int j = 0; j < D / 32; ++j) {
-                    uint32_t four[4];
+                            for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) four[i] = BITS == 8 ? vw[i][j] : four6(vw[i], j);
-                    // (token, token + 1) bytes of features 0, 1 and of 2, 3
-                    const uint32_t a01 = __byte_perm(four[0], four[1], 0x5140), a23 = __byte_perm(four[0], four[1], 0x7362);
-                    const uint32_t b01 = __byte_perm(four[2], four[3], 0x5140), b23 = __byte_perm(four[2], four[3], 0x7362);
-                    mma16816(o[4 * j], pa, hmul2(dev::codes_to_f16x2<kCode>(a01), f0),
-                             hmul2(dev::codes_to_f16x2<kCode>(b01), f1));
-                    mma16816(o[4 * j + 1], pa, hmul2(dev::codes_to_f16x2<kCode>(a01 >> 16), f0),
-                             hmul2(dev::codes_to_f16x2<kCode>(b01 >> 16), f1));
-                    mma16816(o[4 * j + 2], pa, hmul2(dev::codes_to_f16x2<kCode>(a23), f0),
-                             hmul2(dev::codes_to_f16x2<kCode>(b23), f1));
-                    mma16816(o[4 * j + 3], pa, hmul2(dev::codes_to_f16x2<kCode>(a23 >> 16), f0),
-                             hmul2(dev::codes_to_f16x2<kCode>(b23 >> 16), f1));
+                                for (int e = 0; e < 2; ++e) {
+                                    const int byte = (2 * c + e) * vShare + n;
+                                    const int in_row = P::swizzled ? (((byte >> 4) ^ (t & 7)) << 4) + (byte & 15) : byte;
+                                    if ((lds_u8<0>(ring + at + S::v_at + t * P::v + in_row) & 0x7f) == 0x7f)
+                                        o[n][2 * i + e] = __int_as_float(0x7fc00000);
+                                }
+                        }
                 }
-            }
-            if (nans) {
-                for (int t = 0; t < kGranule; ++t)
-                    for (int i = 0; i < 2; ++i) {
-                        if (t0 + t < lo[i] || t0 + t >= hi[i]) continue;
-#pragma unroll
-                        for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                if ((lds_u8<0>(ring + now + S::v_at + t * P::v + (2 * c + e) * vShare + n) & 0x7f) == 0x7f)
-                                    o[n][2 * i + e] = __int_as_float(0x7fc00000);
-                    }
             }
         }
 
