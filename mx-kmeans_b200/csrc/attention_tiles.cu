@@ -42,42 +42,45 @@ using dev::kQueryExp;
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kTileRows = 128;           // M of one product
-constexpr int kRows = 2 * kTileRows;     // rows of a unit
 constexpr int kKeys = 128;               // tokens of a key tile
 constexpr int kHalf = kKeys / 2;         // tokens of one step of the softmax
 constexpr int kStages = 2;               // of keys and of values
 constexpr int kMeta = 4;                 // key tiles whose references are kept (converter warps)
 constexpr int kRefStep = 4;              // value references are multiples of this many octaves
 constexpr int kMostDown = 64;            // octaves that a float32 weight may be scaled down by
-constexpr int kSoftmaxWarps = 8;
-
 // Rows per key head above which its keys are converted beforehand, and the most
 // memory that may take.
-constexpr int kReadyRows = kRows;
+constexpr int kReadyRows = 256;
 constexpr int64_t kReadyBytes = 4ll << 30;
 
-// The two kernels' warps and registers.  Warpgroups give up or take registers of
-// those the block was launched with.
+// The two kernels' row tiles, warps and registers.  Warpgroups give up or take registers
+// of those the block was launched with.  Next to converter warps there are registers for
+// one row tile only (two, at 96 registers a thread, spilled: 16 query tokens over 16,384
+// took 55 us instead of PACKED_US).
 struct Packed {
+    static constexpr int row_tiles = 1, rows = row_tiles * kTileRows;
+    static constexpr int softmax_warps = 4 * row_tiles;
     static constexpr int convert_warps = 8;
-    static constexpr int product_warp = kSoftmaxWarps + convert_warps;
-    static constexpr int threads = 640;
-    static constexpr int launch_regs = 96, softmax_regs = 120, convert_regs = 80, product_regs = 72;
-    static_assert(256 * softmax_regs + 256 * convert_regs + 128 * product_regs <= threads * launch_regs, "");
+    static constexpr int product_warp = softmax_warps + convert_warps;
+    static constexpr int threads = 512;
+    static constexpr int launch_regs = 128, softmax_regs = 168, convert_regs = 128, product_regs = 88;
+    static_assert(128 * softmax_regs + 256 * convert_regs + 128 * product_regs <= threads * launch_regs, "");
 };
 struct Ready {
-    static constexpr int product_warp = kSoftmaxWarps, load_warp = kSoftmaxWarps + 1;
+    static constexpr int row_tiles = 2, rows = row_tiles * kTileRows;
+    static constexpr int softmax_warps = 4 * row_tiles;
+    static constexpr int product_warp = softmax_warps, load_warp = softmax_warps + 1;
     static constexpr int threads = 384;
     static constexpr int launch_regs = 168, softmax_regs = 200, product_regs = 104;
     static_assert(256 * softmax_regs + 128 * product_regs <= threads * launch_regs, "");
 };
 
-template <int D>
+template <int D, int TILES = 2>
 struct Smem {
     static constexpr int half = kKeys * 128;        // 128 rows x 64 features
     static constexpr int tile = (D / 64) * half;    // 128 rows x D features
-    static constexpr int q = 0;                     // two row tiles
-    static constexpr int k = 2 * tile;
+    static constexpr int q = 0;                     // the row tiles' queries
+    static constexpr int k = TILES * tile;
     static constexpr int v = k + kStages * tile;
     static constexpr int total = v + kStages * tile + 1024;  // 1024: alignment
 };
@@ -113,6 +116,7 @@ struct Block {
 };
 
 // A pass over the CTA's share: every role makes the same one.
+template <int ROWS>
 struct Cursor {
     dev::Walk w;
     int left;
@@ -126,14 +130,13 @@ struct Cursor {
     __device__ __forceinline__ bool next(const AttentionParams& p) {
         left -= tiles;
         if (left <= 0) return false;
-        dev::walk_on<kRows, kKeys>(p, w);
+        dev::walk_on<ROWS, kKeys>(p, w);
         ++unit;
         take();
         return true;
     }
     __device__ __forceinline__ int rows(const AttentionParams& p) const {
-        const int r = w.view.n * p.group - w.rt * kRows;
-        return r < kRows ? r : kRows;
+        return min(w.view.n * p.group - w.rt * ROWS, ROWS);
     }
     __device__ __forceinline__ bool whole() const { return tile0 == 0 && tiles == w.tiles; }
 };
@@ -142,8 +145,9 @@ struct Cursor {
 struct Whole {
     int from, to;
 };
-__device__ __forceinline__ Whole whole_tiles(const AttentionParams& p, const Cursor& c) {
-    const int r0 = c.w.rt * kRows, j0 = r0 / p.group, j1 = (r0 + c.rows(p) - 1) / p.group;
+template <int ROWS>
+__device__ __forceinline__ Whole whole_tiles(const AttentionParams& p, const Cursor<ROWS>& c) {
+    const int r0 = c.w.rt * ROWS, j0 = r0 / p.group, j1 = (r0 + c.rows(p) - 1) / p.group;
     int lo, hi, x;
     dev::seen_range(p, c.w.view, j0, j0, x, hi);   // the first row ends first,
     dev::seen_range(p, c.w.view, j1, j1, lo, x);   // the last begins last
@@ -341,12 +345,13 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
 // Converter warps: every key tile of the CTA's share, rows loaded one tile ahead of
 // their conversion and page numbers two.
 template <int D, int BITS>
-__device__ __forceinline__ bool convert_role(const AttentionParams& p, const Block& b, Cursor c, int warp) {
+__device__ __forceinline__ bool convert_role(const AttentionParams& p, const Block& b, Cursor<Packed::rows> c, int warp) {
     using C = Converter<D, BITS>;
+    using L = Smem<D, Packed::row_tiles>;
     const C cv(warp);
     typename C::Words kx, vx;
     uint32_t ks[4], vs[4];
-    Cursor ahead = c;
+    Cursor<Packed::rows> ahead = c;
     int at = 0;  // key tile of `ahead`'s unit
     bool more = true;
     struct Place {
@@ -379,7 +384,7 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
             for (int i = 0; i < 4; ++i) vs_now[i] = vs[i];
 
             if (!b.wait(&b.sh->k_empty[stage], phase)) return false;
-            cv.store(kx, ks, kref - kKeyLift, b.smem + Smem<D>::k + stage * Smem<D>::tile);
+            cv.store(kx, ks, kref - kKeyLift, b.smem + L::k + stage * L::tile);
             if (warp == 0 && cv.lane == 0) b.sh->meta[meta_at % kMeta] = make_int2(kref, vref);
             dev::fence_proxy_async();
             dev::mbar_arrive(&b.sh->k_full[stage]);
@@ -396,7 +401,7 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
             if (t < whole.from || t >= whole.to)
                 if (C::take_out_nans(vx)) *reinterpret_cast<volatile int*>(&b.sh->nan_unit[c.unit & 3]) = c.unit;
             if (!b.wait(&b.sh->v_empty[stage], phase)) return false;
-            cv.store(vx, vs_now, vref, b.smem + Smem<D>::v + stage * Smem<D>::tile);
+            cv.store(vx, vs_now, vref, b.smem + L::v + stage * L::tile);
             dev::fence_proxy_async();
             dev::mbar_arrive(&b.sh->v_full[stage]);
             if (pl.valid >= 0) cv.load(pl.row, pl.valid, p.v_values, vx);
@@ -409,14 +414,15 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
 }
 
 // Index of a key tile among the converted ones.
-__device__ __forceinline__ int64_t ready_at(const AttentionParams& p, const Cursor& c) {
+__device__ __forceinline__ int64_t ready_at(const AttentionParams& p, const Cursor<Ready::rows>& c) {
     return ((int64_t)c.w.seq * p.kv_heads + c.w.head) * p.max_tiles + c.w.first + c.tile0;
 }
 
 // One warp copying ready-made tiles (its elected lane).
 template <int D>
-__device__ __forceinline__ void load_role(const AttentionParams& p, const Block& b, Cursor c) {
-    constexpr int bytes = Smem<D>::tile;
+__device__ __forceinline__ void load_role(const AttentionParams& p, const Block& b, Cursor<Ready::rows> c) {
+    using L = Smem<D, Ready::row_tiles>;
+    constexpr int bytes = L::tile;
     int stage = 0, issued = 0;
     uint32_t phase = 1;
     bool ok = true, values = true;  // values: the last tile's were issued as well
@@ -427,13 +433,13 @@ __device__ __forceinline__ void load_role(const AttentionParams& p, const Block&
             if (!ok) break;
             if (dev::elect_one()) {
                 dev::mbar_arrive_expect_tx(&b.sh->k_full[stage], bytes);
-                dev::bulk_load(b.smem + Smem<D>::k + stage * bytes, p.ready_k + (at + t) * bytes, bytes, &b.sh->k_full[stage]);
+                dev::bulk_load(b.smem + L::k + stage * bytes, p.ready_k + (at + t) * bytes, bytes, &b.sh->k_full[stage]);
             }
             __syncwarp();
             values = ok = b.wait_lean(&b.sh->v_empty[stage], phase);
             if (ok && dev::elect_one()) {
                 dev::mbar_arrive_expect_tx(&b.sh->v_full[stage], bytes);
-                dev::bulk_load(b.smem + Smem<D>::v + stage * bytes, p.ready_v + (at + t) * bytes, bytes, &b.sh->v_full[stage]);
+                dev::bulk_load(b.smem + L::v + stage * bytes, p.ready_v + (at + t) * bytes, bytes, &b.sh->v_full[stage]);
             }
             __syncwarp();
             ++issued;
@@ -452,9 +458,10 @@ __device__ __forceinline__ void load_role(const AttentionParams& p, const Block&
 
 // --------------------------------------------------------------------------- products
 
-template <int D>
-__device__ __forceinline__ void product_role(const AttentionParams& p, const Block& b, Cursor c) {
-    using L = Smem<D>;
+template <int D, class Cfg>
+__device__ __forceinline__ void product_role(const AttentionParams& p, const Block& b, Cursor<Cfg::rows> c) {
+    using L = Smem<D, Cfg::row_tiles>;
+    constexpr int kTiles = Cfg::row_tiles;
     constexpr uint32_t idesc_s = dev::f16_idesc(kTileRows, kHalf, false);
     constexpr uint32_t idesc_o = dev::f16_idesc(kTileRows, D, true);
     // The whole warp walks, one elected lane issues: descriptors and addresses stay
@@ -487,18 +494,18 @@ __device__ __forceinline__ void product_role(const AttentionParams& p, const Blo
         if (++k_stage == kStages) k_stage = 0, k_phase ^= 1;
     };
     do {
-        const int nw = __shfl_sync(kFull, c.rows(p) > kTileRows ? 2 : 1, 0);
+        const int nw = kTiles == 1 ? 1 : __shfl_sync(kFull, c.rows(p) > kTileRows ? 2 : 1, 0);
         const int tiles = __shfl_sync(kFull, c.tiles, 0);
         ok = b.wait_lean(&sh->k_full[k_stage], k_phase);
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+        for (int w = 0; w < kTiles; ++w)
             if (w < nw && ok) ok = b.wait_lean(&sh->q_ready[w], q_phase[w]), q_phase[w] ^= 1;
         if (!ok) break;
         dev::tc_fence_after();
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
+            for (int w = 0; w < kTiles; ++w)
                 if (w < nw) scores(w, half);
         release_keys();
         for (int t = 0; t < tiles && ok; ++t) {
@@ -508,7 +515,7 @@ __device__ __forceinline__ void product_role(const AttentionParams& p, const Blo
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
+                for (int w = 0; w < kTiles; ++w) {
                     if (w >= nw || !ok) continue;
                     ok = b.wait_lean(&sh->p_ready[w][half], p_phase[w]);
                     if (!ok) continue;
@@ -518,7 +525,7 @@ __device__ __forceinline__ void product_role(const AttentionParams& p, const Blo
                     if (dev::elect_one()) {
 #pragma unroll
                         for (int i = 0; i < kHalf / 16; ++i)
-                            dev::tc_mma_f16_ta(b.tmem + 2 * kKeys + w * D, b.tmem + w * kKeys + half * kHalf + 8 * i,
+                            dev::tc_mma_f16_ta(b.tmem + kTiles * kKeys + w * D, b.tmem + w * kKeys + half * kHalf + 8 * i,
                                                vd + i * (2048 >> 4), idesc_o, i > 0 || half > 0 || t > 0);
                         dev::tc_commit(&sh->o_done[w][half]);
                         if (half == 1 && w == nw - 1) dev::tc_commit(&sh->v_empty[v_stage]);
@@ -761,14 +768,15 @@ __device__ __forceinline__ void put_rows(const AttentionParams& p, const float4*
 }
 
 // READY: tiles were converted beforehand, their references lie in global memory.
-template <int D, bool READY>
-__device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Block& b, Cursor c, int warp) {
-    using L = Smem<D>;
+template <int D, class Cfg, bool READY>
+__device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Block& b, Cursor<Cfg::rows> c, int warp) {
+    using L = Smem<D, Cfg::row_tiles>;
+    constexpr int kRows = Cfg::rows;
     Shared* sh = b.sh;
     const int w = warp >> 2;                                    // row tile
     const int r = threadIdx.x & (kTileRows - 1);                // row in the tile
     const uint32_t lane_base = b.tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-    const uint32_t s_col = lane_base + w * kKeys, o_col = lane_base + 2 * kKeys + w * D;
+    const uint32_t s_col = lane_base + w * kKeys, o_col = lane_base + Cfg::row_tiles * kKeys + w * D;
     const float neg_inf = __int_as_float(0xff800000);
     // Phases of s_full and o_done; a wait is never more than one completion behind, since
     // the scores of a half follow the products of the half before the last.
@@ -796,8 +804,9 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             float run_max = neg_inf, base = -kExpShift, sum = 0.0f;
             int vrun = 0;  // the output is held relative to 2^(vrun - 127)
             bool nans = false;
-            const int2* meta = READY ? p.ready_meta + ready_at(p, c) : nullptr;
-            int2 ref = READY ? __ldg(meta) : make_int2(0, 0);
+            const int2* meta = nullptr;
+            int2 ref = make_int2(0, 0);
+            if constexpr (READY) meta = p.ready_meta + ready_at(p, c), ref = __ldg(meta);
             // Scores of the half at hand; the next half's are fetched as the registers get free.
             uint32_t s[2][32];
             if (!b.wait(&sh->s_full[w][0], s_phase)) return false;
@@ -971,9 +980,12 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
 // ---------------------------------------------------------------------------- kernels
 
 // Barriers, TMEM and the cursor; false: the CTA has no share.
+constexpr int tmem_columns(int d, int row_tiles) { return row_tiles * (kKeys + d) <= 256 ? 256 : 512; }
+
 template <int D, class Cfg, int FULL_COUNT>
 __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_raw, Shared* sh, int* scratch,
-                                      unsigned* err, Block& b, Cursor& c) {
+                                      unsigned* err, Block& b, Cursor<Cfg::rows>& c) {
+    constexpr int kRows = Cfg::rows;
     const int tid = threadIdx.x;
     dev::let_next_start();
     const dev::Share share = dev::take_share<kRows, kKeys, Cfg::threads>(p, scratch);
@@ -1004,7 +1016,7 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
         dev::fence_barrier_init();
     }
     if (tid < 4) sh->nan_unit[tid] = -1;
-    if (tid < 32) dev::tmem_alloc(&sh->tmem, 512);
+    if (tid < 32) dev::tmem_alloc(&sh->tmem, tmem_columns(D, Cfg::row_tiles));
     dev::tc_fence_before();
     __syncthreads();
     dev::tc_fence_after();
@@ -1020,11 +1032,12 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
     return true;
 }
 
+template <int D, class Cfg>
 __device__ __forceinline__ void finish(const AttentionParams& p, const Block& b) {
     dev::tc_fence_before();
     __syncthreads();
     dev::tc_fence_after();
-    if (threadIdx.x < 32) dev::tmem_dealloc(b.tmem, 512);
+    if (threadIdx.x < 32) dev::tmem_dealloc(b.tmem, tmem_columns(D, Cfg::row_tiles));
     // After a wait gave up nothing of this CTA is joined.
     if (threadIdx.x == 0 && *b.abort_flag())
         p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -1036,20 +1049,19 @@ __global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(con
     __shared__ __align__(8) Shared shared;
     __shared__ int scratch[Packed::threads / 32 + 2];
     Block b;
-    Cursor c;
+    Cursor<Packed::rows> c;
     if (!begin<D, Packed, 32 * Packed::convert_warps>(p, smem_raw, &shared, scratch, err, b, c)) return;
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
-    if (warp < kSoftmaxWarps) {
+    if (warp < Packed::softmax_warps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Packed::softmax_regs));
-        softmax_role<D, false>(p, b, c, warp);
+        softmax_role<D, Packed, false>(p, b, c, warp);
     } else if (warp < Packed::product_warp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Packed::convert_regs));
-        convert_role<D, BITS>(p, b, c, warp - kSoftmaxWarps);
+        convert_role<D, BITS>(p, b, c, warp - Packed::softmax_warps);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Packed::product_regs));
-        if (warp == Packed::product_warp) product_role<D>(p, b, c);
+        if (warp == Packed::product_warp) product_role<D, Packed>(p, b, c);
     }
-    finish(p, b);
+    finish<D, Packed>(p, b);
 }
 
 template <int D>
@@ -1058,21 +1070,21 @@ __global__ void __launch_bounds__(Ready::threads, 1) attention_ready_kernel(cons
     __shared__ __align__(8) Shared shared;
     __shared__ int scratch[Ready::threads / 32 + 2];
     Block b;
-    Cursor c;
+    Cursor<Ready::rows> c;
     if (!begin<D, Ready, 1>(p, smem_raw, &shared, scratch, err, b, c)) return;
     dev::wait_for_previous();  // the converted tiles
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
-    if (warp < kSoftmaxWarps) {
+    if (warp < Ready::softmax_warps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Ready::softmax_regs));
-        softmax_role<D, true>(p, b, c, warp);
+        softmax_role<D, Ready, true>(p, b, c, warp);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Ready::product_regs));
         if (warp == Ready::product_warp)
-            product_role<D>(p, b, c);
+            product_role<D, Ready>(p, b, c);
         else if (warp == Ready::load_warp)
             load_role<D>(p, b, c);
     }
-    finish(p, b);
+    finish<D, Ready>(p, b);
 }
 
 // Once per device: shared memory, and that the build has the registers the split assumes.
@@ -1091,35 +1103,45 @@ int prepare_kernel(K kernel, int smem, int regs, int& ready_device) {
     return MXK_OK;
 }
 
-template <int D, int BITS>
-int launch_packed(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
-    static thread_local int ready_device = -1;
-    MXK_CHECK(prepare_kernel(attention_tiles_kernel<D, BITS>, Smem<D>::total, Packed::launch_regs, ready_device));
-    unsigned* err = device_error_word();
-    if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
+// One CTA an SM, or one a key tile if there cannot be as many.
+template <class Cfg>
+int grid_size(const AttentionParams& p, int max_q, int64_t* ctas) {
+    const int64_t most = attention_tile_bound(p, max_q, Cfg::rows, kKeys);
+    MXK_REQUIRE(most <= std::numeric_limits<int>::max(), "cache_attention: too much work for one call");
     static const int sms = sm_count();
-    const int64_t ctas = most_tiles < sms ? most_tiles : sms;
-    Workspace ws(stream);
-    MXK_CHECK(ws.take(p, ctas, kRows, D));
-    {
-        LaunchScope scope("attention_tiles", stream);
-        attention_tiles_kernel<D, BITS><<<(unsigned)ctas, Packed::threads, Smem<D>::total, stream>>>(p, err);
-        MXK_CUDA(cudaGetLastError());
-    }
-    return join_parts<kRows, D>(p, (int)ctas, 64, stream);
+    *ctas = most < sms ? most : sms;
+    return MXK_OK;
 }
 
 template <int D, int BITS>
-int launch_ready(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
+int launch_packed(AttentionParams p, int max_q, cudaStream_t stream) {
     static thread_local int ready_device = -1;
-    MXK_CHECK(prepare_kernel(attention_ready_kernel<D>, Smem<D>::total, Ready::launch_regs, ready_device));
+    MXK_CHECK(prepare_kernel(attention_tiles_kernel<D, BITS>, Smem<D, Packed::row_tiles>::total, Packed::launch_regs, ready_device));
     unsigned* err = device_error_word();
     if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
-    static const int sms = sm_count();
-    const int64_t ctas = most_tiles < sms ? most_tiles : sms;
+    int64_t ctas;
+    MXK_CHECK(grid_size<Packed>(p, max_q, &ctas));
+    Workspace ws(stream);
+    MXK_CHECK(ws.take(p, ctas, Packed::rows, D));
+    {
+        LaunchScope scope("attention_tiles", stream);
+        attention_tiles_kernel<D, BITS><<<(unsigned)ctas, Packed::threads, Smem<D, Packed::row_tiles>::total, stream>>>(p, err);
+        MXK_CUDA(cudaGetLastError());
+    }
+    return join_parts<Packed::rows, D>(p, (int)ctas, 64, stream);
+}
+
+template <int D, int BITS>
+int launch_ready(AttentionParams p, int max_q, cudaStream_t stream) {
+    static thread_local int ready_device = -1;
+    MXK_CHECK(prepare_kernel(attention_ready_kernel<D>, Smem<D, Ready::row_tiles>::total, Ready::launch_regs, ready_device));
+    unsigned* err = device_error_word();
+    if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
+    int64_t ctas;
+    MXK_CHECK(grid_size<Ready>(p, max_q, &ctas));
     const int64_t tiles = (int64_t)p.seqs * p.kv_heads * p.max_tiles;
     Workspace ws(stream);
-    MXK_CHECK(ws.take(p, ctas, kRows, D, tiles * (2 * Smem<D>::tile + (int64_t)sizeof(int2))));
+    MXK_CHECK(ws.take(p, ctas, Ready::rows, D, tiles * (2 * Smem<D>::tile + (int64_t)sizeof(int2))));
     p.ready_k = static_cast<uint8_t*>(ws.extra);
     p.ready_v = p.ready_k + tiles * Smem<D>::tile;
     p.ready_meta = reinterpret_cast<int2*>(p.ready_v + tiles * Smem<D>::tile);
@@ -1132,7 +1154,7 @@ int launch_ready(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)ctas);
         cfg.blockDim = dim3(Ready::threads);
-        cfg.dynamicSmemBytes = Smem<D>::total;
+        cfg.dynamicSmemBytes = Smem<D, Ready::row_tiles>::total;
         cfg.stream = stream;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1142,14 +1164,12 @@ int launch_ready(AttentionParams p, int64_t most_tiles, cudaStream_t stream) {
         LaunchScope scope("attention_ready", stream);
         MXK_CUDA(cudaLaunchKernelEx(&cfg, attention_ready_kernel<D>, p, err));
     }
-    return join_parts<kRows, D>(p, (int)ctas, 64, stream);
+    return join_parts<Ready::rows, D>(p, (int)ctas, 64, stream);
 }
 
 template <int D, int BITS>
 int launch(const AttentionParams& p, bool ready, int max_q, cudaStream_t stream) {
-    const int64_t most = attention_tile_bound(p, max_q, kRows, kKeys);
-    MXK_REQUIRE(most <= std::numeric_limits<int>::max(), "cache_attention: too much work for one call");
-    return ready ? launch_ready<D, BITS>(p, most, stream) : launch_packed<D, BITS>(p, most, stream);
+    return ready ? launch_ready<D, BITS>(p, max_q, stream) : launch_packed<D, BITS>(p, max_q, stream);
 }
 
 template <int D>
