@@ -93,6 +93,7 @@ struct Shared {
     uint64_t o_done[2][2];     // the half's product with the values has finished
     uint64_t drain;
     int2 meta[kMeta];          // converter warps: the key tile's references
+    float row_factor[2][kTileRows];
     int nan_unit[4];           // converter warps: unit in which a NaN was taken out of a partly seen tile
     int abort_word;
     uint32_t tmem;
@@ -109,6 +110,11 @@ struct Block {
     // Bounded wait of a whole warp; false: it gave up, leave for the end of the kernel.
     __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) const {
         return __all_sync(kFull, dev::mbar_wait(bar, parity, abort_flag(), err));
+    }
+    // One arrival for the whole warp, after all its lanes' writes.
+    __device__ __forceinline__ void arrive(uint64_t* bar) const {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) dev::mbar_arrive(bar);
     }
     __device__ __forceinline__ bool wait_lean(uint64_t* bar, uint32_t parity) const {
         return __all_sync(kFull, dev::mbar_wait_lean(bar, parity, abort_flag(), err));
@@ -218,18 +224,25 @@ struct Converter {
         high = warp_rows * warp >= 32;
     }
 
-    // Lane i < 8 has the cached row of the tile's token 16 i; `valid` tokens exist.
-    __device__ __forceinline__ uint32_t place(const AttentionParams& p, int seq, int head, int t0, int valid) const {
-        uint32_t row = 0;
+    // The page number and the place in it of the tile's token 16 i, in lane i < 8; `valid`
+    // tokens exist.  row_of makes the cached row of it, when the page number has arrived.
+    struct Place {
+        int page, in;
+    };
+    __device__ __forceinline__ Place place(const AttentionParams& p, int seq, int t0, int valid) const {
+        Place pl{0, 0};
         if (lane < 8 && 16 * lane < valid) {
             const unsigned per_page = (unsigned)p.page_size / 16u;
             const unsigned gr = (unsigned)(t0 / 16) + lane;
             const unsigned at = gr / per_page;
-            int page = __ldg(p.page_table + (int64_t)seq * p.table_stride + at);
-            page = page < 0 ? 0 : (page >= p.pages ? p.pages - 1 : page);
-            row = ((uint32_t)page * p.kv_heads + head) * p.page_size + (gr - at * per_page) * 16u;
+            pl.page = __ldg(p.page_table + (int64_t)seq * p.table_stride + at);
+            pl.in = (int)(gr - at * per_page) * 16;
         }
-        return row;
+        return pl;
+    }
+    static __device__ __forceinline__ uint32_t row_of(const AttentionParams& p, const Place& pl, int head) {
+        const int page = min(max(pl.page, 0), p.pages - 1);
+        return ((uint32_t)page * p.kv_heads + head) * p.page_size + pl.in;
     }
     __device__ __forceinline__ void load(uint32_t place, int valid, const uint8_t* values, Words& x) const {
 #pragma unroll
@@ -328,7 +341,7 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
     if (tile != 0 && (t0 >= hi || t0 + kKeys <= lo)) return;
     const int valid = min(max(view.len - t0, 0), kKeys);
     const C cv(threadIdx.x >> 5);
-    const uint32_t place = cv.place(p, seq, head, t0, valid);
+    const uint32_t place = C::row_of(p, cv.place(p, seq, t0, valid), head);
     uint32_t ks[4], vs[4];
     typename C::Words kx, vx;
     cv.load_scales(place, valid, p.k_scales, ks);
@@ -354,25 +367,28 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
     Cursor<Packed::rows> ahead = c;
     int at = 0;  // key tile of `ahead`'s unit
     bool more = true;
-    struct Place {
-        uint32_t row;
+    struct Next {
+        typename C::Place place;
+        int head;
         int valid;  // tokens that exist; -1: no such tile
     };
-    auto here = [&]() -> Place {
+    auto here = [&]() -> Next {
         const int t0 = (ahead.w.first + ahead.tile0 + at) * kKeys;
         const int valid = min(max(ahead.w.view.len - t0, 0), kKeys);
-        return Place{cv.place(p, ahead.w.seq, ahead.w.head, t0, valid), valid};
+        return Next{cv.place(p, ahead.w.seq, t0, valid), ahead.w.head, valid};
     };
-    auto advance = [&]() -> Place {
+    auto advance = [&]() -> Next {
         if (more && ++at == ahead.tiles) at = 0, more = ahead.next(p);
-        return more ? here() : Place{0, -1};
+        return more ? here() : Next{{0, 0}, 0, -1};
     };
-    Place pl = here();
-    cv.load_scales(pl.row, pl.valid, p.k_scales, ks);
-    cv.load_scales(pl.row, pl.valid, p.v_scales, vs);
-    cv.load(pl.row, pl.valid, p.k_values, kx);
-    cv.load(pl.row, pl.valid, p.v_values, vx);
-    Place then = advance();
+    Next then = here();
+    uint32_t row = C::row_of(p, then.place, then.head);
+    int valid = then.valid;
+    cv.load_scales(row, valid, p.k_scales, ks);
+    cv.load_scales(row, valid, p.v_scales, vs);
+    cv.load(row, valid, p.k_values, kx);
+    cv.load(row, valid, p.v_values, vx);
+    then = advance();
     int stage = 0, meta_at = 0;
     uint32_t phase = 1;  // the first pass over the stages finds them empty
     do {
@@ -387,14 +403,15 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
             cv.store(kx, ks, kref - kKeyLift, b.smem + L::k + stage * L::tile);
             if (warp == 0 && cv.lane == 0) b.sh->meta[meta_at % kMeta] = make_int2(kref, vref);
             dev::fence_proxy_async();
-            dev::mbar_arrive(&b.sh->k_full[stage]);
+            b.arrive(&b.sh->k_full[stage]);
 
             // the next key tile is on its way while this one's values are converted
-            pl = then;
-            if (pl.valid >= 0) {
-                cv.load_scales(pl.row, pl.valid, p.k_scales, ks);
-                cv.load_scales(pl.row, pl.valid, p.v_scales, vs);
-                cv.load(pl.row, pl.valid, p.k_values, kx);
+            valid = then.valid;
+            if (valid >= 0) {
+                row = C::row_of(p, then.place, then.head);
+                cv.load_scales(row, valid, p.k_scales, ks);
+                cv.load_scales(row, valid, p.v_scales, vs);
+                cv.load(row, valid, p.k_values, kx);
                 then = advance();
             }
             // a NaN belongs to the rows that see it: they get it at the end
@@ -403,8 +420,8 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
             if (!b.wait(&b.sh->v_empty[stage], phase)) return false;
             cv.store(vx, vs_now, vref, b.smem + L::v + stage * L::tile);
             dev::fence_proxy_async();
-            dev::mbar_arrive(&b.sh->v_full[stage]);
-            if (pl.valid >= 0) cv.load(pl.row, pl.valid, p.v_values, vx);
+            b.arrive(&b.sh->v_full[stage]);
+            if (valid >= 0) cv.load(row, valid, p.v_values, vx);
 
             ++meta_at;
             if (++stage == kStages) stage = 0, phase ^= 1;
@@ -652,12 +669,13 @@ __device__ __noinline__ uint4 nan_features(const uint8_t* values, const int* tab
     return make_uint4(bad[0], bad[1], bad[2], bad[3]);
 }
 
-// The warp's 32 query rows into shared memory, each scaled by a power of two to a largest
-// magnitude in [2^12, 2^13); a negative scale of the scores goes into their sign.  Lane i
-// names row i (`at`, elements from p.q; `real`: it exists, else zeros) and gets the factor
-// that makes scores of its products with lifted keys, less the keys' reference.  D / 4
-// lanes load a row together: a thread that loads its own row touches 32 of them in every
-// access and takes ten times as long.
+// Queries of a row tile into shared memory, each row scaled by a power of two to a largest
+// magnitude in [2^12, 2^13); a negative scale of the scores goes into their sign.  Of the
+// tile's four warps, warp r0 has rows r0, r0 + 4, ..., so a tile with few rows is loaded by
+// all of them.  Lane i names row r0 + 4 i (`at`, elements from p.q; `real`: it exists) and
+// returns the factor that makes scores of its products with lifted keys, less the keys'
+// reference.  D / 4 lanes load a row together: a thread that loads its own row touches 32
+// of them in every access.
 template <int D>
 __device__ __forceinline__ float put_queries(const AttentionParams& p, int64_t at, bool real, uint8_t* rows, int r0) {
     constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes, kBatch = 8;
@@ -691,6 +709,7 @@ __device__ __forceinline__ float put_queries(const AttentionParams& p, int64_t a
     };
     // Rows past the last real one are left as they are: a row's scores are its own.
     const int rows_here = 32 - __clz(reals);
+    if (rows_here == 0) return 0.0f;
     uint2 next[kBatch];
     fetch(0, next);
 #pragma unroll 1
@@ -721,7 +740,7 @@ __device__ __forceinline__ float put_queries(const AttentionParams& p, int64_t a
             factors(amax[i], f0, f1);
             const __half2 a = __floats2half2_rn(x[i].x * f0 * f1, x[i].y * f0 * f1);
             const __half2 b = __floats2half2_rn(x[i].z * f0 * f1, x[i].w * f0 * f1);
-            const int chunk = piece / 2, row = r0 + base + i * kAtOnce + sub;
+            const int chunk = piece / 2, row = r0 + 4 * (base + i * kAtOnce + sub);
             *reinterpret_cast<uint2*>(rows + (chunk / 8) * Smem<D>::half + row * 128 +
                                       (((chunk % 8) ^ (row & 7)) << 4) + (piece & 1) * 8) =
                 make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
@@ -795,11 +814,18 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             int lo = 0, hi = c.w.view.len;
             if (real) dev::seen_range(p, c.w.view, j, j, lo, hi);
             const int first_key = (c.w.first + c.tile0) * kKeys;
-            const float row_factor = !warp_real ? 0.0f :
-                put_queries<D>(p, (int64_t)(c.w.view.row0 + j) * p.q_token + (int64_t)head * p.q_head, real,
-                               b.smem + L::q + w * L::tile, r & ~31);
+            {
+                const int r_load = (warp & 3) + 4 * (r & 31);  // the row this lane names
+                const bool here = w * kTileRows + r_load < rows;
+                const int row_load = c.w.rt * kRows + w * kTileRows + r_load, j_load = row_load / p.group;
+                const int head_load = c.w.head * p.group + (row_load - j_load * p.group);
+                const float f = put_queries<D>(
+                    p, (int64_t)(c.w.view.row0 + j_load) * p.q_token + (int64_t)head_load * p.q_head, here,
+                    b.smem + L::q + w * L::tile, warp & 3);
+                sh->row_factor[w][r_load] = f;  // the row's own thread reads it after the first scores
+            }
             dev::fence_proxy_async();
-            dev::mbar_arrive(&sh->q_ready[w]);
+            b.arrive(&sh->q_ready[w]);
 
             float run_max = neg_inf, base = -kExpShift, sum = 0.0f;
             int vrun = 0;  // the output is held relative to 2^(vrun - 127)
@@ -816,6 +842,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                 dev::tmem_ld_32x32b_x32(s_col + 32, s[1]);
             }
             const int halves = 2 * c.tiles;
+            const float row_factor = *const_cast<volatile float*>(&sh->row_factor[w][r]);
             for (int t = 0; t < halves; ++t) {
                 const uint32_t s_at = s_col + (t & 1) * kHalf, s_next = s_col + (~t & 1) * kHalf;
                 const uint32_t next_phase = s_phase ^ (t & 1);
@@ -889,7 +916,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                     }
                 }
                 dev::tc_fence_before();
-                dev::mbar_arrive(&sh->p_ready[w][t & 1]);
+                b.arrive(&sh->p_ready[w][t & 1]);
                 if (t & 1)
                     o_phase[1] ^= 1;
                 else
@@ -997,11 +1024,11 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
         sh->abort_word = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            dev::mbar_init(&sh->q_ready[i], kTileRows);
+            dev::mbar_init(&sh->q_ready[i], kTileRows / 32);
             dev::mbar_init(&sh->s_full[i][0], 1);
             dev::mbar_init(&sh->s_full[i][1], 1);
-            dev::mbar_init(&sh->p_ready[i][0], kTileRows);
-            dev::mbar_init(&sh->p_ready[i][1], kTileRows);
+            dev::mbar_init(&sh->p_ready[i][0], kTileRows / 32);
+            dev::mbar_init(&sh->p_ready[i][1], kTileRows / 32);
             dev::mbar_init(&sh->o_done[i][0], 1);
             dev::mbar_init(&sh->o_done[i][1], 1);
         }
@@ -1050,7 +1077,7 @@ __global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(con
     __shared__ int scratch[Packed::threads / 32 + 2];
     Block b;
     Cursor<Packed::rows> c;
-    if (!begin<D, Packed, 32 * Packed::convert_warps>(p, smem_raw, &shared, scratch, err, b, c)) return;
+    if (!begin<D, Packed, Packed::convert_warps>(p, smem_raw, &shared, scratch, err, b, c)) return;
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
     if (warp < Packed::softmax_warps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Packed::softmax_regs));
