@@ -207,6 +207,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     const dev::Share share = dev::take_share<kRows, kKeys, kThreads>(p, scratch);
     if (share.tiles == 0) {
         if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
+        dev::wait_for_previous();
         return;
     }
     dev::Walk w = dev::walk_to<kRows, kKeys>(p, share.seq, share.offset);
@@ -675,10 +676,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         if (left > 0) dev::walk_on<kRows, kKeys>(p, w);
     }
     if (tid == 0 && !open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
+    dev::wait_for_previous();
 }
 
 template <int D, int BITS>
-int launch_rows(AttentionParams p, int64_t most_tiles, int64_t most_rows, cudaStream_t stream) {
+int launch_rows(AttentionParams p, int64_t most_tiles, int64_t most_rows, AttentionCall& call) {
     using S = Stage<D, BITS>;
     static thread_local int ready_device = -1;
     int dev = 0;
@@ -690,21 +692,17 @@ int launch_rows(AttentionParams p, int64_t most_tiles, int64_t most_rows, cudaSt
     }
     static const int sms = sm_count();
     const int64_t ctas = std::min<int64_t>(most_tiles, kCtasPerSm * sms);
-    Workspace ws(stream);
-    MXK_CHECK(ws.take(p, ctas, kRows, D));
-    {
-        LaunchScope scope("attention_rows", stream);
-        attention_rows_kernel<D, BITS><<<(unsigned)ctas, kThreads, S::smem, stream>>>(p);
-        MXK_CUDA(cudaGetLastError());
-    }
-    return join_parts<kRows, D>(p, (int)ctas, (int)(most_rows < kRows ? most_rows : kRows), stream);
+    MXK_CHECK(call.take(p, ctas, kRows, D));
+    MXK_CHECK(call.launch("attention_rows", attention_rows_kernel<D, BITS>, (unsigned)ctas, kThreads, S::smem, p));
+    call.join_later<kRows, D>(p, (int)ctas, (int)std::min<int64_t>(most_rows, kRows));
+    return MXK_OK;
 }
 
 template <int D>
-int launch_rows_bits(int bits, const AttentionParams& p, int64_t most_tiles, int64_t most_rows, cudaStream_t stream) {
-    if (bits == 8) return launch_rows<D, 8>(p, most_tiles, most_rows, stream);
-    if (bits == 6) return launch_rows<D, 6>(p, most_tiles, most_rows, stream);
-    return launch_rows<D, 4>(p, most_tiles, most_rows, stream);
+int launch_rows_bits(int bits, const AttentionParams& p, int64_t most_tiles, int64_t most_rows, AttentionCall& call) {
+    if (bits == 8) return launch_rows<D, 8>(p, most_tiles, most_rows, call);
+    if (bits == 6) return launch_rows<D, 6>(p, most_tiles, most_rows, call);
+    return launch_rows<D, 4>(p, most_tiles, most_rows, call);
 }
 
 }  // namespace
@@ -773,18 +771,21 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     // Sequences with few rows per key head go to the rows kernel, the others to the
     // tiles kernel; a single sequence has one kernel chosen by its bound, several are
     // sorted by the kernels themselves.
-    const cudaStream_t st = as_stream(stream);
+    AttentionCall call(as_stream(stream));
     const int64_t rows = (int64_t)a->max_q * p.group;
-    if (rows > kMostFewRows) {
-        AttentionParams many = p;
-        if (a->seqs > 1) many.min_rows = kMostFewRows + 1;
-        MXK_CHECK(launch_attention_tiles(cache->bits, cache->head_dim, many, a->max_q, st));
-        if (a->seqs == 1) return MXK_OK;
+    const bool many = rows > kMostFewRows;
+    if (many) {
+        AttentionParams q = p;
+        if (a->seqs > 1) q.min_rows = kMostFewRows + 1;
+        MXK_CHECK(launch_attention_tiles(cache->bits, cache->head_dim, q, a->max_q, call));
         p.max_rows = kMostFewRows;
     }
-    const int few_q = rows > kMostFewRows ? (kMostFewRows + p.group - 1) / p.group : a->max_q;
-    const int64_t most = attention_tile_bound(p, few_q, kRows, kKeys);
-    MXK_REQUIRE(most <= std::numeric_limits<int>::max(), "cache_attention: too much work for one call");
-    return cache->head_dim == 128 ? launch_rows_bits<128>(cache->bits, p, most, rows, st)
-                                  : launch_rows_bits<64>(cache->bits, p, most, rows, st);
+    if (!many || a->seqs > 1) {
+        const int64_t few = std::min<int64_t>(rows, kMostFewRows);
+        const int64_t most = attention_tile_bound(p, (int)((few + p.group - 1) / p.group), kRows, kKeys);
+        MXK_REQUIRE(most <= std::numeric_limits<int>::max(), "cache_attention: too much work for one call");
+        MXK_CHECK(cache->head_dim == 128 ? launch_rows_bits<128>(cache->bits, p, most, few, call)
+                                         : launch_rows_bits<64>(cache->bits, p, most, few, call));
+    }
+    return call.join_all();
 }

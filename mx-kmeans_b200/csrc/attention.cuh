@@ -62,9 +62,6 @@ inline int64_t attention_tile_bound(const AttentionParams& p, int max_q, int row
     return (int64_t)p.seqs * p.kv_heads * row_tiles * (span / keys + 2);
 }
 
-// attention_tiles.cu: many query rows per key head.
-int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, cudaStream_t stream);
-
 namespace dev {
 
 // exp(s - max) is held as 2^(s2 - m2 + kExpShift) with s2, m2 in log2 units: up
@@ -76,8 +73,8 @@ constexpr float kExpShift = 11.0f;
 constexpr float kMaxSlack = 4.0f;
 
 // The kernels of a call follow one another with programmatic launches: a kernel lets the
-// next one be set up as soon as all its own CTAs have started, and the next one waits, before
-// it touches anything written here, until this one has finished.
+// next one start as soon as all its own CTAs have, and the next one waits until this one
+// has finished before it reads anything written here, or else before it ends.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -408,46 +405,82 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionPara
     }
 }
 
-// Memory of a launch's partial sums.
-struct Workspace {
-    void* ptr = nullptr;
-    void* extra = nullptr;
-    cudaStream_t stream;
-    explicit Workspace(cudaStream_t s) : stream(s) {}
-    ~Workspace() {
-        if (ptr) cudaFreeAsync(ptr, stream);
+// The launches of one call and the memory of their partial sums, which goes back to the
+// pool, in stream order, at its end.  Kernels for sequences of different sizes write
+// different outputs, so each is launched as soon as the one before has started everywhere;
+// every one ends only when its predecessor has, so the joins, launched last, find all done.
+class AttentionCall {
+public:
+    explicit AttentionCall(cudaStream_t s) : stream_(s) {}
+    ~AttentionCall() {
+        for (int i = 0; i < blocks_; ++i) cudaFreeAsync(block_[i], stream_);
     }
-    Workspace(const Workspace&) = delete;
-    Workspace& operator=(const Workspace&) = delete;
-    // extra: bytes at `extra`, 256-byte aligned.
-    int take(AttentionParams& p, int64_t ctas, int rows, int d, int64_t extra_bytes = 0) {
+    AttentionCall(const AttentionCall&) = delete;
+    AttentionCall& operator=(const AttentionCall&) = delete;
+
+    // Partial sums of `ctas` CTAs with tiles of `rows` rows, and extra_bytes more at *extra
+    // (256-byte aligned).
+    int take(AttentionParams& p, int64_t ctas, int rows, int d, int64_t extra_bytes = 0, void** extra = nullptr) {
         const size_t part = (size_t)(2 * ctas * rows) * d * 4, stat = (size_t)(2 * ctas * rows) * 8;
         const size_t own = (part + stat + (size_t)ctas * 16 + 255) / 256 * 256;
         cudaMemPool_t pool = workspace_pool();
         if (!pool) return fail(MXK_ERR_CUDA, "cache_attention: cannot create the workspace pool");
-        MXK_CUDA(cudaMallocFromPoolAsync(&ptr, own + (size_t)extra_bytes, pool, stream));
-        extra = static_cast<char*>(ptr) + own;
+        void* ptr = nullptr;
+        MXK_CUDA(cudaMallocFromPoolAsync(&ptr, own + (size_t)extra_bytes, pool, stream_));
+        block_[blocks_++] = ptr;
+        if (extra) *extra = static_cast<char*>(ptr) + own;
         p.part = static_cast<float*>(ptr);
         p.part_stat = reinterpret_cast<float2*>(static_cast<char*>(ptr) + part);
         p.part_open = reinterpret_cast<int4*>(static_cast<char*>(ptr) + part + stat);
         return MXK_OK;
     }
+
+    template <class K, class... Args>
+    int launch(const char* name, K kernel, unsigned ctas, unsigned threads, size_t smem, const Args&... args) {
+        return launch(name, kernel, dim3(ctas), threads, smem, args...);
+    }
+    template <class K, class... Args>
+    int launch(const char* name, K kernel, dim3 grid, unsigned threads, size_t smem, const Args&... args) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream_;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = first_ ? 0 : 1;  // the call's first kernel waits for all that the stream held before
+        first_ = false;
+        LaunchScope scope(name, stream_);
+        MXK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+        return MXK_OK;
+    }
+
+    template <int ROWS, int D>
+    void join_later(const AttentionParams& p, int ctas, int grid_y) {
+        join_[joins_++] = Join{p, dim3((unsigned)ctas, (unsigned)grid_y), attention_join_kernel<ROWS, D>};
+    }
+    int join_all() {
+        for (int i = 0; i < joins_; ++i)
+            MXK_CHECK(launch("attention_join", join_[i].kernel, join_[i].grid, 128, 0, join_[i].p));
+        return MXK_OK;
+    }
+
+private:
+    struct Join {
+        AttentionParams p;
+        dim3 grid;
+        void (*kernel)(const AttentionParams);
+    };
+    cudaStream_t stream_;
+    bool first_ = true;
+    void* block_[3] = {};
+    Join join_[3];
+    int blocks_ = 0, joins_ = 0;
 };
 
-template <int ROWS, int D>
-inline int join_parts(const AttentionParams& p, int ctas, int grid_y, cudaStream_t stream) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas, (unsigned)grid_y);
-    cfg.blockDim = dim3(128);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    LaunchScope scope("attention_join", stream);
-    MXK_CUDA(cudaLaunchKernelEx(&cfg, attention_join_kernel<ROWS, D>, p));
-    return MXK_OK;
-}
+// attention_tiles.cu: many query rows per key head.
+int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, AttentionCall& call);
 
 }  // namespace mxk

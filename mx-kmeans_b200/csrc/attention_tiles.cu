@@ -579,14 +579,43 @@ __device__ __forceinline__ void fold_top(const uint32_t (&s)[32], float (&m)[4])
         m[(i / 2) & 3] = max3f(m[(i / 2) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
 }
 
-// Weights 2^(score * f - base) of 32 scores, added to sum, as f16 pairs.
+// 2^x of a pair on the FMA pipe, for x below 128: with n the integer nearest to x and
+// r = x - n, 2^x = 2^n 2^r, and on [-1/2, 1/2] a polynomial of degree five is within 7.5e-8
+// of 2^r (least squares on the relative error, reweighted towards its largest values).
+// Below -127 the result is zero; a NaN stays one.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+    const float2 magic = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: sums end in the integer
+    const float2 y = __fadd2_rn(x, magic);
+    const float2 n = __fadd2_rn(y, make_float2(-12582912.0f, -12582912.0f));
+    const float2 r = __fadd2_rn(x, make_float2(-n.x, -n.y));
+    auto c = [](float v) { return make_float2(v, v); };
+    float2 v = __ffma2_rn(c(1.3276469420750838e-3f), r, c(9.67554164625246e-3f));
+    v = __ffma2_rn(v, r, c(5.550713284339852e-2f));
+    v = __ffma2_rn(v, r, c(2.4022119718243962e-1f));
+    v = __ffma2_rn(v, r, c(6.931469670563168e-1f));
+    v = __ffma2_rn(v, r, c(1.000000071655749f));
+    const float2 p = make_float2(__uint_as_float(__float_as_uint(y.x) * 0x800000u + 0x3f800000u),
+                                 __uint_as_float(__float_as_uint(y.y) * 0x800000u + 0x3f800000u));
+    return __fmul2_rn(v, p);
+}
+
+// Weights 2^(score * f - base) of 32 scores, added to sum, as f16 pairs.  The exponential
+// unit, 16 a cycle and SM, takes as long for them as the tensor core for both products; one
+// pair in kFmaEvery is computed on the FMA pipe instead (chunk of 4096 over 16,384 tokens:
+// 945 us without, 900 with one in 8, 928 one in 4, 962 one in 2).
+constexpr int kFmaEvery = 8;
 __device__ __forceinline__ void fold_weights(const uint32_t (&s)[32], float f, float base, float2 (&sum)[2],
                                              uint32_t (&pw)[16]) {
     const float2 f2 = make_float2(f, f), b2 = make_float2(-base, -base);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
         float2 t = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, b2);
-        t.x = ex2(t.x), t.y = ex2(t.y);
+        if ((i / 2) % kFmaEvery == kFmaEvery - 1)
+            t = ex2_fma(t);
+        else
+            t.x = ex2(t.x), t.y = ex2(t.y);
         sum[(i / 2) & 1] = __fadd2_rn(sum[(i / 2) & 1], t);
         const __half2 u = __float22half2_rn(t);
         pw[i / 2] = *reinterpret_cast<const uint32_t*>(&u);
@@ -1018,6 +1047,7 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
     const dev::Share share = dev::take_share<kRows, kKeys, Cfg::threads>(p, scratch);
     if (share.tiles == 0) {
         if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
+        dev::wait_for_previous();
         return false;
     }
     if (tid == 0) {
@@ -1065,6 +1095,7 @@ __device__ __forceinline__ void finish(const AttentionParams& p, const Block& b)
     __syncthreads();
     dev::tc_fence_after();
     if (threadIdx.x < 32) dev::tmem_dealloc(b.tmem, tmem_columns(D, Cfg::row_tiles));
+    dev::wait_for_previous();
     // After a wait gave up nothing of this CTA is joined.
     if (threadIdx.x == 0 && *b.abort_flag())
         p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -1141,74 +1172,56 @@ int grid_size(const AttentionParams& p, int max_q, int64_t* ctas) {
 }
 
 template <int D, int BITS>
-int launch_packed(AttentionParams p, int max_q, cudaStream_t stream) {
+int launch_packed(AttentionParams p, int max_q, AttentionCall& call) {
+    constexpr int smem = Smem<D, Packed::row_tiles>::total;
     static thread_local int ready_device = -1;
-    MXK_CHECK(prepare_kernel(attention_tiles_kernel<D, BITS>, Smem<D, Packed::row_tiles>::total, Packed::launch_regs, ready_device));
+    MXK_CHECK(prepare_kernel(attention_tiles_kernel<D, BITS>, smem, Packed::launch_regs, ready_device));
     unsigned* err = device_error_word();
     if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
     int64_t ctas;
     MXK_CHECK(grid_size<Packed>(p, max_q, &ctas));
-    Workspace ws(stream);
-    MXK_CHECK(ws.take(p, ctas, Packed::rows, D));
-    {
-        LaunchScope scope("attention_tiles", stream);
-        attention_tiles_kernel<D, BITS><<<(unsigned)ctas, Packed::threads, Smem<D, Packed::row_tiles>::total, stream>>>(p, err);
-        MXK_CUDA(cudaGetLastError());
-    }
-    return join_parts<Packed::rows, D>(p, (int)ctas, 64, stream);
+    MXK_CHECK(call.take(p, ctas, Packed::rows, D));
+    MXK_CHECK(call.launch("attention_tiles", attention_tiles_kernel<D, BITS>, (unsigned)ctas, Packed::threads, smem, p, err));
+    call.join_later<Packed::rows, D>(p, (int)ctas, 64);
+    return MXK_OK;
 }
 
 template <int D, int BITS>
-int launch_ready(AttentionParams p, int max_q, cudaStream_t stream) {
+int launch_ready(AttentionParams p, int max_q, AttentionCall& call) {
+    constexpr int smem = Smem<D, Ready::row_tiles>::total;
     static thread_local int ready_device = -1;
-    MXK_CHECK(prepare_kernel(attention_ready_kernel<D>, Smem<D, Ready::row_tiles>::total, Ready::launch_regs, ready_device));
+    MXK_CHECK(prepare_kernel(attention_ready_kernel<D>, smem, Ready::launch_regs, ready_device));
     unsigned* err = device_error_word();
     if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
     int64_t ctas;
     MXK_CHECK(grid_size<Ready>(p, max_q, &ctas));
     const int64_t tiles = (int64_t)p.seqs * p.kv_heads * p.max_tiles;
-    Workspace ws(stream);
-    MXK_CHECK(ws.take(p, ctas, Ready::rows, D, tiles * (2 * Smem<D>::tile + (int64_t)sizeof(int2))));
-    p.ready_k = static_cast<uint8_t*>(ws.extra);
+    void* extra = nullptr;
+    MXK_CHECK(call.take(p, ctas, Ready::rows, D, tiles * (2 * Smem<D>::tile + (int64_t)sizeof(int2)), &extra));
+    p.ready_k = static_cast<uint8_t*>(extra);
     p.ready_v = p.ready_k + tiles * Smem<D>::tile;
     p.ready_meta = reinterpret_cast<int2*>(p.ready_v + tiles * Smem<D>::tile);
-    {
-        LaunchScope scope("attention_unpack", stream);
-        attention_unpack_kernel<D, BITS><<<(unsigned)tiles, 256, 0, stream>>>(p);
-        MXK_CUDA(cudaGetLastError());
-    }
-    {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)ctas);
-        cfg.blockDim = dim3(Ready::threads);
-        cfg.dynamicSmemBytes = Smem<D, Ready::row_tiles>::total;
-        cfg.stream = stream;
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        LaunchScope scope("attention_ready", stream);
-        MXK_CUDA(cudaLaunchKernelEx(&cfg, attention_ready_kernel<D>, p, err));
-    }
-    return join_parts<Ready::rows, D>(p, (int)ctas, 64, stream);
+    MXK_CHECK(call.launch("attention_unpack", attention_unpack_kernel<D, BITS>, (unsigned)tiles, 256, 0, p));
+    MXK_CHECK(call.launch("attention_ready", attention_ready_kernel<D>, (unsigned)ctas, Ready::threads, smem, p, err));
+    call.join_later<Ready::rows, D>(p, (int)ctas, 64);
+    return MXK_OK;
 }
 
 template <int D, int BITS>
-int launch(const AttentionParams& p, bool ready, int max_q, cudaStream_t stream) {
-    return ready ? launch_ready<D, BITS>(p, max_q, stream) : launch_packed<D, BITS>(p, max_q, stream);
+int launch(const AttentionParams& p, bool ready, int max_q, AttentionCall& call) {
+    return ready ? launch_ready<D, BITS>(p, max_q, call) : launch_packed<D, BITS>(p, max_q, call);
 }
 
 template <int D>
-int launch_bits(int bits, const AttentionParams& p, bool ready, int max_q, cudaStream_t stream) {
-    if (bits == 8) return launch<D, 8>(p, ready, max_q, stream);
-    if (bits == 6) return launch<D, 6>(p, ready, max_q, stream);
-    return launch<D, 4>(p, ready, max_q, stream);
+int launch_bits(int bits, const AttentionParams& p, bool ready, int max_q, AttentionCall& call) {
+    if (bits == 8) return launch<D, 8>(p, ready, max_q, call);
+    if (bits == 6) return launch<D, 6>(p, ready, max_q, call);
+    return launch<D, 4>(p, ready, max_q, call);
 }
 
 }  // namespace
 
-int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, cudaStream_t stream) {
+int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, AttentionCall& call) {
     // Several row tiles of a key head share its keys: converting those once pays for
     // writing and reading them as f16.
     p.max_tiles = (p.max_kv + kKeys - 1) / kKeys;
@@ -1218,14 +1231,14 @@ int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q,
     if (many) {
         AttentionParams q = p;
         if (p.seqs > 1 && q.min_rows <= kReadyRows) q.min_rows = kReadyRows + 1;
-        MXK_CHECK(head_dim == 128 ? launch_bits<128>(bits, q, true, max_q, stream)
-                                  : launch_bits<64>(bits, q, true, max_q, stream));
+        MXK_CHECK(head_dim == 128 ? launch_bits<128>(bits, q, true, max_q, call)
+                                  : launch_bits<64>(bits, q, true, max_q, call));
         if (p.seqs == 1) return MXK_OK;
         p.max_rows = kReadyRows;
         max_q = few_q;
     }
-    return head_dim == 128 ? launch_bits<128>(bits, p, false, max_q, stream)
-                           : launch_bits<64>(bits, p, false, max_q, stream);
+    return head_dim == 128 ? launch_bits<128>(bits, p, false, max_q, call)
+                           : launch_bits<64>(bits, p, false, max_q, call);
 }
 
 }  // namespace mxk
