@@ -91,6 +91,7 @@ struct Shared {
     uint64_t s_full[2][2];     // [row tile][half of the key tile] scores are in TMEM
     uint64_t p_ready[2][2];    // the half's weights are in TMEM, the output may be added to
     uint64_t o_done[2][2];     // the half's product with the values has finished
+    uint64_t rows_out[2];      // the tile's output rows have left the queries' shared memory
     uint64_t drain;
     int2 meta[kMeta];          // converter warps: the key tile's references
     float row_factor[2][kTileRows];
@@ -830,6 +831,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
     // the scores of a half follow the products of the half before the last.
     uint32_t s_phase = 0, o_phase[2] = {0, 0};
     int meta_at = 0;
+    uint32_t units_out = 0, out_phase = 0;  // units this row tile has put out, phase of the last
     bool open = false;
     const int share = c.left;
     do {
@@ -843,6 +845,8 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             int lo = 0, hi = c.w.view.len;
             if (real) dev::seen_range(p, c.w.view, j, j, lo, hi);
             const int first_key = (c.w.first + c.tile0) * kKeys;
+            // A warp's queries go where other warps' output rows of the unit before were.
+            if (units_out > 0 && !b.wait(&sh->rows_out[w], out_phase)) return false;
             {
                 const int r_load = (warp & 3) + 4 * (r & 31);  // the row this lane names
                 const bool here = w * kTileRows + r_load < rows;
@@ -1020,6 +1024,8 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                 }
             }
             dev::tc_fence_before();
+            b.arrive(&sh->rows_out[w]);
+            out_phase = units_out++ & 1u;
         }
         meta_at += c.tiles;
         if (!c.whole() && c.tile0 == 0) {
@@ -1055,6 +1061,7 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             dev::mbar_init(&sh->q_ready[i], kTileRows / 32);
+            dev::mbar_init(&sh->rows_out[i], kTileRows / 32);
             dev::mbar_init(&sh->s_full[i][0], 1);
             dev::mbar_init(&sh->s_full[i][1], 1);
             dev::mbar_init(&sh->p_ready[i][0], kTileRows / 32);

@@ -166,6 +166,23 @@ def test_long_axis_is_split_and_joined(torch_cuda, mxk, q_len, kv_len, kv_heads,
     assert torch.equal(out, again) and torch.equal(lse, lse2), "the same call twice differs"
 
 
+@pytest.mark.parametrize("q_len,kv_len,seqs,heads,kv_heads", [(1, 400, 150, 16, 8), (9, 260, 60, 28, 4),
+                                                              (40, 300, 60, 12, 4), (138, 150, 40, 12, 6),
+                                                              (100, 700, 30, 32, 8)])
+@pytest.mark.parametrize("bits,dim", [(8, 128), (4, 64)])
+def test_several_units_per_block(torch_cuda, mxk, q_len, kv_len, seqs, heads, kv_heads, bits, dim):
+    """More (sequence, head, row tile) units than the GPU has blocks: every block works
+    through several, whole and in part, with row tiles full and nearly empty."""
+    torch, g = torch_cuda, np.random.default_rng(16)
+    kv = [kv_len - int(x) for x in g.integers(0, kv_len // 2, seqs)]
+    q_lens = [min(l, q_len - int(x)) for l, x in zip(kv, g.integers(0, q_len // 3 + 1, seqs))]
+    b = build(torch, mxk, g, q_lens, kv, heads, kv_heads, dim, 16, bits, "bfloat16")
+    out, lse = attend(torch, mxk, b)
+    check(torch, b, out, lse)
+    again, lse2 = attend(torch, mxk, b)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
 def test_many_sequences(torch_cuda, mxk):
     """More sequences than a CTA has threads, many of them empty."""
     torch, g = torch_cuda, np.random.default_rng(4)
