@@ -335,6 +335,7 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  *     out = sum_t exp(s_t) v_t / sum_t exp(s_t),    lse = log(sum_t exp(s_t));
  * a row with no such token gets zeros and -inf.  Tokens outside [0, L) are never
  * read; a NaN among the keys or values reaches the rows that see its token only.
+ * (Scale bytes are taken to be 0 .. 254; cache_write never stores 255.)
  *
  * cu_q (seqs + 1), page_table, kv_lens: int32 on the device.  max_q and max_kv
  * are bounds on n and L known to the host: they choose the launch, and a longer
@@ -352,7 +353,12 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  * timing: partial sums join in a fixed order.
  *
  * Asynchronous on `stream`; partial sums live in the library's stream-ordered
- * pool on the current device (mxk_release_workspace). */
+ * pool on the current device (mxk_release_workspace): at most 40 MB, and, when
+ * sequences have more than 256 query rows per key head (n * heads / kv_heads), their
+ * keys and values converted to f16 once, seqs * kv_heads * max_kv * head_dim * 4 bytes
+ * (not done where that exceeds 4 GB).  May be captured into a graph.  A device-side
+ * wait that gives up leaves the call's output undefined; the next synchronous call of
+ * the library on the device reports MXK_ERR_TIMEOUT. */
 typedef struct {
     int dtype;
     int heads;

@@ -411,3 +411,15 @@ def test_binding_refusals(torch_cuda, mxk):
         with pytest.raises(mxk.MxkInvalidArgument):
             mxk.cache_write(b["cache"], *args)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_serving_example(torch_cuda, mxk, bits):
+    """The example's loop; what remains is the output's rounding and that of the weights."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(mxk.__file__), "examples", "serve_cache.py")
+    spec = importlib.util.spec_from_file_location("serve_cache", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.main(bits=bits, steps=9) < 2.0 ** -8 + 2.0 ** -10
