@@ -353,7 +353,7 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  * timing: partial sums join in a fixed order.
  *
  * Asynchronous on `stream`; partial sums live in the library's stream-ordered
- * pool on the current device (mxk_release_workspace): at most 40 MB, and, when
+ * pool on the current device (mxk_release_workspace): at most 70 MB, and, when
  * sequences have more than 256 query rows per key head (n * heads / kv_heads), their
  * keys and values converted to f16 once, seqs * kv_heads * max_kv * head_dim * 4 bytes
  * (not done where that exceeds 4 GB).  May be captured into a graph.  A device-side

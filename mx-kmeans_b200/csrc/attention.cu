@@ -51,6 +51,10 @@ constexpr int kGranule = 16;     // tokens of one product, contiguous in their p
 constexpr int kGranules = 2;     // of one step of a warp
 constexpr int kPair = kGranule * kGranules;
 constexpr int kKeys = kPair * kWarps;
+// Key tiles that starting and ending a unit is taken to be worth.  In us for 0, 1, 2, 4 and
+// 6: 64 sequences of 1 to 8192 tokens 150, 142, 140, 144, 146; 24 sequences with 2 to 5
+// query tokens and windows 35, 29, 27, 29, 29.
+constexpr int kUnitCost = 2;
 constexpr int kCtasPerSm = 3;
 // Rows per key head up to which this kernel is taken, one pass over the keys for
 // every 16 of them.
@@ -160,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     constexpr int kShare = S::row / 4;   // bytes of a key row a lane reads
     constexpr int vShare = S::row / 8;   // bytes of a value row a lane reads
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int scratch[kWarps + 2];
+    __shared__ int scratch[2 * kWarps + 2];
     __shared__ float stat_max[kWarps][kRows], stat_sum[kWarps][kRows];
     __shared__ __align__(16) uint4 query[kSteps][32];  // the A operand of every k-step, lane by lane
 
@@ -204,14 +208,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     const uint32_t vs_read = ring + S::vs_at + 2 * c * S::scale_bytes + (D == 128 ? g >> 1 : g >> 2);
 
     dev::let_next_start();
-    const dev::Share share = dev::take_share<kRows, kKeys, kThreads>(p, scratch);
+    const dev::Share share = dev::take_share<kRows, kKeys, kUnitCost, kThreads>(p, scratch);
     if (share.tiles == 0) {
         if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
         dev::wait_for_previous();
         return;
     }
-    dev::Walk w = dev::walk_to<kRows, kKeys>(p, share.seq, share.offset);
-    int left = share.tiles;
+    dev::Walk w = dev::walk_to<kRows, kKeys>(p, share);
+    int left = share.tiles - w.skip;
     bool open = false;
 
     while (left > 0) {
@@ -671,8 +675,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                     make_int4(w.seq, w.rt, w.head, share.followers(share.tiles - left, w.tiles));
         }
         __syncthreads();  // before the rings are filled again
-        left -= tiles;
-        w.tile += tiles;
+        left -= tiles + share.cost;
         if (left > 0) dev::walk_on<kRows, kKeys>(p, w);
     }
     if (tid == 0 && !open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -783,7 +786,7 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     if (!many || a->seqs > 1) {
         const int64_t few = std::min<int64_t>(rows, kMostFewRows);
         const int64_t most = attention_tile_bound(p, (int)((few + p.group - 1) / p.group), kRows, kKeys);
-        MXK_REQUIRE(most <= std::numeric_limits<int>::max(), "cache_attention: too much work for one call");
+        MXK_REQUIRE(most <= std::numeric_limits<int>::max() / (1 + kUnitCost), "cache_attention: too much work for one call");
         MXK_CHECK(cache->head_dim == 128 ? launch_rows_bits<128>(cache->bits, p, most, few, call)
                                          : launch_rows_bits<64>(cache->bits, p, most, few, call));
     }

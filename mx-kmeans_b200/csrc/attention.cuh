@@ -4,9 +4,11 @@
 // Work is divided without the host knowing the lengths.  A unit is one (sequence,
 // row tile, key head): the rows r = j * group + g (query token j, query head g of
 // the key head's group) of one tile, over the tokens that any of them sees, in
-// key tiles.  All units' key tiles, numbered one after the other, are split
-// evenly over the CTAs, so every CTA gets the same number whatever the lengths
-// are; a CTA walks its tiles unit by unit.  A unit that one CTA has to itself is
+// key tiles.  Starting and ending a unit takes a CTA as long as COST key tiles (a
+// constant of each kernel), so where there are more key tiles than CTAs a unit counts
+// as that many more, which come first and hold nothing.  All units' tiles, numbered
+// one after the other, are split evenly over the CTAs, so every CTA has about the same
+// to do whatever the lengths are; a CTA walks its tiles unit by unit.  A unit that one CTA has to itself is
 // written out by it; the parts of a unit that spans several go to the workspace
 // (at most two per CTA: the end of a unit that an earlier CTA began, and the
 // beginning of one that a later CTA goes on with) and attention_join_kernel adds
@@ -150,25 +152,27 @@ __device__ __forceinline__ int tile_count(const AttentionParams& p, const SeqVie
     return hi <= lo ? 1 : (hi + KEYS - 1) / KEYS - t0;
 }
 
+// Key tiles and units of a sequence.
 template <int ROWS, int KEYS>
-__device__ __forceinline__ int seq_tiles(const AttentionParams& p, const SeqView& s) {
+__device__ __forceinline__ int2 seq_tiles(const AttentionParams& p, const SeqView& s) {
     const int rows = s.n * p.group;
-    if (rows < p.min_rows || rows > p.max_rows || rows == 0) return 0;
+    if (rows < p.min_rows || rows > p.max_rows || rows == 0) return make_int2(0, 0);
+    const int tiles = (rows + ROWS - 1) / ROWS, units = tiles * p.kv_heads;
+    if (!p.causal) return make_int2(units * tile_count<ROWS, KEYS>(p, s, 0), units);
     int total = 0;
-    const int tiles = (rows + ROWS - 1) / ROWS;
-    if (!p.causal) return tiles * p.kv_heads * tile_count<ROWS, KEYS>(p, s, 0);
     for (int rt = 0; rt < tiles; ++rt) total += tile_count<ROWS, KEYS>(p, s, rt);
-    return total * p.kv_heads;
+    return make_int2(total * p.kv_heads, units);
 }
 
-// Where a CTA's share begins, and how many tiles it has: `each`, and one more for the
-// first `extra` CTAs.
+// Where a CTA's share begins, and how many tiles it counts as: `each`, and one more for
+// the first `extra` CTAs.
 struct Share {
     int tiles;   // of this CTA
     int seq;     // first sequence of the share
     int offset;  // of the share's first tile in that sequence
     int begin;   // the share's first tile among all
     int each, extra;
+    int cost;    // tiles that a unit counts as beside its own
 
     // CTAs after this one that work on a unit of n tiles whose first is `at` of the share.
     __device__ __forceinline__ int followers(int at, int n) const {
@@ -177,24 +181,29 @@ struct Share {
     }
 };
 
-// All threads of the CTA; scratch: THREADS / 32 + 2 words of shared memory.
+// All threads of the CTA; scratch: THREADS / 16 + 2 words of shared memory.
 // CTAs past the number of tiles get none.
-template <int ROWS, int KEYS, int THREADS>
+template <int ROWS, int KEYS, int COST, int THREADS>
 __device__ __forceinline__ Share take_share(const AttentionParams& p, int* scratch) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kWarps = THREADS / 32;
-    int* found = scratch + kWarps;  // sequence, offset
-    int sum = 0;
-    for (int i = tid; i < p.seqs; i += THREADS) sum += seq_tiles<ROWS, KEYS>(p, seq_view(p, i));
-    const int mine = sum;
-    sum = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum);
-    if (lane == 0) scratch[warp] = sum;
+    int* found = scratch + 2 * kWarps;  // sequence, offset
+    int2 mine = make_int2(0, 0);
+    for (int i = tid; i < p.seqs; i += THREADS) {
+        const int2 t = seq_tiles<ROWS, KEYS>(p, seq_view(p, i));
+        mine.x += t.x, mine.y += t.y;
+    }
+    const int tiles = (int)__reduce_add_sync(0xffffffffu, (unsigned)mine.x);
+    const int units = (int)__reduce_add_sync(0xffffffffu, (unsigned)mine.y);
+    if (lane == 0) scratch[2 * warp] = tiles, scratch[2 * warp + 1] = units;
     __syncthreads();
-    int total = 0;
+    int total = 0, all_units = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) total += scratch[w];
+    for (int w = 0; w < kWarps; ++w) total += scratch[2 * w], all_units += scratch[2 * w + 1];
+    const int cost = total > (int)gridDim.x ? COST : 0;
+    total += cost * all_units;
     const int ctas = min(total, (int)gridDim.x);
-    Share s{0, 0, 0, 0, 1, 0};
+    Share s{0, 0, 0, 0, 1, 0, cost};
     if ((int)blockIdx.x >= ctas) return s;
     s.each = total / ctas;
     s.extra = total - s.each * ctas;
@@ -203,22 +212,24 @@ __device__ __forceinline__ Share take_share(const AttentionParams& p, int* scrat
     int before = 0;  // tiles of the sequences before this round's
     for (int base = 0; base < p.seqs; base += THREADS) {
         const int i = base + tid;
-        const int t = p.seqs <= THREADS ? mine : (i < p.seqs ? seq_tiles<ROWS, KEYS>(p, seq_view(p, i)) : 0);
+        const int2 its = p.seqs <= THREADS ? mine
+                                           : (i < p.seqs ? seq_tiles<ROWS, KEYS>(p, seq_view(p, i)) : make_int2(0, 0));
+        const int t = its.x + cost * its.y;
         int incl = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
-        if (base > 0 || p.seqs > THREADS) {  // else the warps' sums are there already
+        if (p.seqs > THREADS) {  // else the warps' sums are there already
             __syncthreads();
-            if (lane == 31) scratch[warp] = incl;
+            if (lane == 31) scratch[2 * warp] = incl, scratch[2 * warp + 1] = 0;
             __syncthreads();
         }
         int start = before, round = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const int v = scratch[w];
+            const int v = scratch[2 * w] + cost * scratch[2 * w + 1];
             if (w < warp) start += v;
             round += v;
         }
@@ -237,29 +248,33 @@ __device__ __forceinline__ Share take_share(const AttentionParams& p, int* scrat
 struct Walk {
     int seq, rt, head;
     int tile, tiles;  // next key tile of the unit, and how many it has
+    int skip;         // empty ones to pass before it
     int first;        // number of the unit's first key tile in the sequence
     SeqView view;
 };
 
 template <int ROWS, int KEYS>
-__device__ __forceinline__ Walk walk_to(const AttentionParams& p, int seq, int offset) {
+__device__ __forceinline__ Walk walk_to(const AttentionParams& p, const Share& s) {
     Walk w;
-    w.seq = seq;
-    w.view = seq_view(p, seq);
+    w.seq = s.seq;
+    w.view = seq_view(p, s.seq);
+    int offset = s.offset;
     w.rt = 0;
     while (true) {
         w.tiles = tile_count<ROWS, KEYS>(p, w.view, w.rt, &w.first);
-        const int all = w.tiles * p.kv_heads;
+        const int all = (w.tiles + s.cost) * p.kv_heads;
         if (offset < all) break;
         offset -= all;
         ++w.rt;
     }
-    w.head = offset / w.tiles;
-    w.tile = offset - w.head * w.tiles;
+    w.head = offset / (w.tiles + s.cost);
+    offset -= w.head * (w.tiles + s.cost);
+    w.tile = max(offset - s.cost, 0);
+    w.skip = max(s.cost - offset, 0);
     return w;
 }
 
-// To the next unit; the caller knows that there is one.
+// To the next unit's first tile; the caller has passed its empty ones and knows that there is one.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ void walk_on(const AttentionParams& p, Walk& w) {
     w.tile = 0;

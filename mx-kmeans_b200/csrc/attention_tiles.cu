@@ -55,13 +55,19 @@ constexpr int64_t kReadyBytes = 4ll << 30;
 
 // The two kernels' row tiles, warps and registers.  Warpgroups give up or take registers
 // of those the block was launched with.  Next to converter warps there are registers for
-// one row tile only (two, at 96 registers a thread, spilled: 16 query tokens over 16,384
-// took 55 us instead of PACKED_US).
+// one row tile only (two, at 96 registers a thread, spilled: the kernel took 55 us instead
+// of 46 for 16 query tokens over 16,384, 32 heads of 128 on 8 key heads).
+// unit_cost: key tiles that starting and ending a unit is taken to be worth (queries in,
+// output out, and the pipeline between: 10 us against 1 to 2 a tile).  In us for 0, 3, 10
+// and 15 in Packed and 0, 3, 8 and 12 in Ready, over the same 16,384 tokens: 16 query
+// tokens 62, 54, 47, 47; 64: 86, 78, 70, 72; 512: 185, 181, 176, 178; nine sequences of 1
+// to 701 query tokens and 333 to 5003 cached ones 182, 153, 141, 143.
 struct Packed {
     static constexpr int row_tiles = 1, rows = row_tiles * kTileRows;
     static constexpr int softmax_warps = 4 * row_tiles;
     static constexpr int convert_warps = 8;
     static constexpr int product_warp = softmax_warps + convert_warps;
+    static constexpr int unit_cost = 10;
     static constexpr int threads = 512;
     static constexpr int launch_regs = 128, softmax_regs = 168, convert_regs = 128, product_regs = 88;
     static_assert(128 * softmax_regs + 256 * convert_regs + 128 * product_regs <= threads * launch_regs, "");
@@ -70,6 +76,7 @@ struct Ready {
     static constexpr int row_tiles = 2, rows = row_tiles * kTileRows;
     static constexpr int softmax_warps = 4 * row_tiles;
     static constexpr int product_warp = softmax_warps, load_warp = softmax_warps + 1;
+    static constexpr int unit_cost = 8;
     static constexpr int threads = 384;
     static constexpr int launch_regs = 168, softmax_regs = 200, product_regs = 104;
     static_assert(256 * softmax_regs + 128 * product_regs <= threads * launch_regs, "");
@@ -123,27 +130,28 @@ struct Block {
 };
 
 // A pass over the CTA's share: every role makes the same one.
-template <int ROWS>
+template <class Cfg>
 struct Cursor {
     dev::Walk w;
-    int left;
+    int left;          // tiles of the share from the current unit's on
     int tile0, tiles;  // key tiles of the current unit that are this CTA's
     int unit;          // units begun so far
+    int cost;          // tiles that the next unit counts as before its own
 
     __device__ __forceinline__ void take() {
         tile0 = w.tile;
         tiles = min(left, w.tiles - tile0);
     }
     __device__ __forceinline__ bool next(const AttentionParams& p) {
-        left -= tiles;
+        left -= tiles + cost;
         if (left <= 0) return false;
-        dev::walk_on<ROWS, kKeys>(p, w);
+        dev::walk_on<Cfg::rows, kKeys>(p, w);
         ++unit;
         take();
         return true;
     }
     __device__ __forceinline__ int rows(const AttentionParams& p) const {
-        return min(w.view.n * p.group - w.rt * ROWS, ROWS);
+        return min(w.view.n * p.group - w.rt * Cfg::rows, Cfg::rows);
     }
     __device__ __forceinline__ bool whole() const { return tile0 == 0 && tiles == w.tiles; }
 };
@@ -152,9 +160,9 @@ struct Cursor {
 struct Whole {
     int from, to;
 };
-template <int ROWS>
-__device__ __forceinline__ Whole whole_tiles(const AttentionParams& p, const Cursor<ROWS>& c) {
-    const int r0 = c.w.rt * ROWS, j0 = r0 / p.group, j1 = (r0 + c.rows(p) - 1) / p.group;
+template <class Cfg>
+__device__ __forceinline__ Whole whole_tiles(const AttentionParams& p, const Cursor<Cfg>& c) {
+    const int r0 = c.w.rt * Cfg::rows, j0 = r0 / p.group, j1 = (r0 + c.rows(p) - 1) / p.group;
     int lo, hi, x;
     dev::seen_range(p, c.w.view, j0, j0, x, hi);   // the first row ends first,
     dev::seen_range(p, c.w.view, j1, j1, lo, x);   // the last begins last
@@ -323,12 +331,13 @@ struct Converter {
 static_assert(kRefStep == 4, "value_ref rounds to multiples of four");
 
 // Converts the key tiles that some row sees once for all row tiles of a key head.
-// Block x: key tile x % max_tiles of (sequence, head) x / max_tiles; the f16 tiles lie
-// in the workspace as shared memory will hold them.  HBM bounds it: D * bits / 8 + D / 32
-// bytes of a row read, 2 D written.
+// Block (x, side): key tile x % max_tiles of (sequence, head) x / max_tiles, its keys or
+// its values; the f16 tiles lie in the workspace as shared memory will hold them, so each
+// is built there and leaves as one bulk copy.
 template <int D, int BITS>
 __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionParams p) {
     using C = Converter<D, BITS>;
+    __shared__ __align__(128) uint8_t image[Smem<D>::tile];
     dev::let_next_start();
     const int tile = blockIdx.x % p.max_tiles, sh = blockIdx.x / p.max_tiles;
     const int seq = sh / p.kv_heads, head = sh - seq * p.kv_heads;
@@ -341,31 +350,35 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
     // rows that see nothing still have key tile 0, of zeros where no token exists
     if (tile != 0 && (t0 >= hi || t0 + kKeys <= lo)) return;
     const int valid = min(max(view.len - t0, 0), kKeys);
+    const bool keys = blockIdx.y == 0;
     const C cv(threadIdx.x >> 5);
     const uint32_t place = C::row_of(p, cv.place(p, seq, t0, valid), head);
-    uint32_t ks[4], vs[4];
-    typename C::Words kx, vx;
-    cv.load_scales(place, valid, p.k_scales, ks);
-    cv.load_scales(place, valid, p.v_scales, vs);
-    cv.load(place, valid, p.k_values, kx);
-    cv.load(place, valid, p.v_values, vx);
-    const int kref = C::key_ref(ks), vref = C::value_ref(vs);
-    const int nans = __syncthreads_or(C::take_out_nans(vx));
-    cv.store(kx, ks, kref - kKeyLift, p.ready_k + (int64_t)blockIdx.x * Smem<D>::tile);
-    cv.store(vx, vs, vref, p.ready_v + (int64_t)blockIdx.x * Smem<D>::tile);
-    if (threadIdx.x == 0) p.ready_meta[blockIdx.x] = make_int2(kref, vref | (nans ? 1 << 16 : 0));
+    uint32_t s[4];
+    typename C::Words x;
+    cv.load_scales(place, valid, keys ? p.k_scales : p.v_scales, s);
+    cv.load(place, valid, keys ? p.k_values : p.v_values, x);
+    const int ref = keys ? C::key_ref(s) : C::value_ref(s);
+    const int nans = keys ? 0 : C::take_out_nans(x);
+    cv.store(x, s, keys ? ref - kKeyLift : ref, image);
+    dev::fence_proxy_async();
+    const int any_nans = __syncthreads_or(nans);
+    if (threadIdx.x == 0) {
+        int* meta = reinterpret_cast<int*>(p.ready_meta + blockIdx.x) + (keys ? 0 : 1);
+        *meta = ref | (any_nans ? 1 << 16 : 0);
+        dev::bulk_store_wait((keys ? p.ready_k : p.ready_v) + (int64_t)blockIdx.x * Smem<D>::tile, image, Smem<D>::tile);
+    }
 }
 
 // Converter warps: every key tile of the CTA's share, rows loaded one tile ahead of
 // their conversion and page numbers two.
 template <int D, int BITS>
-__device__ __forceinline__ bool convert_role(const AttentionParams& p, const Block& b, Cursor<Packed::rows> c, int warp) {
+__device__ __forceinline__ bool convert_role(const AttentionParams& p, const Block& b, Cursor<Packed> c, int warp) {
     using C = Converter<D, BITS>;
     using L = Smem<D, Packed::row_tiles>;
     const C cv(warp);
     typename C::Words kx, vx;
     uint32_t ks[4], vs[4];
-    Cursor<Packed::rows> ahead = c;
+    Cursor<Packed> ahead = c;
     int at = 0;  // key tile of `ahead`'s unit
     bool more = true;
     struct Next {
@@ -432,18 +445,19 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
 }
 
 // Index of a key tile among the converted ones.
-__device__ __forceinline__ int64_t ready_at(const AttentionParams& p, const Cursor<Ready::rows>& c) {
+__device__ __forceinline__ int64_t ready_at(const AttentionParams& p, const Cursor<Ready>& c) {
     return ((int64_t)c.w.seq * p.kv_heads + c.w.head) * p.max_tiles + c.w.first + c.tile0;
 }
 
 // One warp copying ready-made tiles (its elected lane).
 template <int D>
-__device__ __forceinline__ void load_role(const AttentionParams& p, const Block& b, Cursor<Ready::rows> c) {
+__device__ __forceinline__ void load_role(const AttentionParams& p, const Block& b, Cursor<Ready> c) {
     using L = Smem<D, Ready::row_tiles>;
     constexpr int bytes = L::tile;
     int stage = 0, issued = 0;
     uint32_t phase = 1;
     bool ok = true, values = true;  // values: the last tile's were issued as well
+    dev::wait_for_previous();       // the converted tiles
     do {
         const int64_t at = ready_at(p, c);
         for (int t = 0; t < c.tiles && ok; ++t) {
@@ -477,7 +491,7 @@ __device__ __forceinline__ void load_role(const AttentionParams& p, const Block&
 // --------------------------------------------------------------------------- products
 
 template <int D, class Cfg>
-__device__ __forceinline__ void product_role(const AttentionParams& p, const Block& b, Cursor<Cfg::rows> c) {
+__device__ __forceinline__ void product_role(const AttentionParams& p, const Block& b, Cursor<Cfg> c) {
     using L = Smem<D, Cfg::row_tiles>;
     constexpr int kTiles = Cfg::row_tiles;
     constexpr uint32_t idesc_s = dev::f16_idesc(kTileRows, kHalf, false);
@@ -818,7 +832,7 @@ __device__ __forceinline__ void put_rows(const AttentionParams& p, const float4*
 
 // READY: tiles were converted beforehand, their references lie in global memory.
 template <int D, class Cfg, bool READY>
-__device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Block& b, Cursor<Cfg::rows> c, int warp) {
+__device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Block& b, Cursor<Cfg> c, int warp) {
     using L = Smem<D, Cfg::row_tiles>;
     constexpr int kRows = Cfg::rows;
     Shared* sh = b.sh;
@@ -833,7 +847,6 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
     int meta_at = 0;
     uint32_t units_out = 0, out_phase = 0;  // units this row tile has put out, phase of the last
     bool open = false;
-    const int share = c.left;
     do {
         const int rows = c.rows(p);
         if (w * kTileRows < rows) {
@@ -865,7 +878,10 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             bool nans = false;
             const int2* meta = nullptr;
             int2 ref = make_int2(0, 0);
-            if constexpr (READY) meta = p.ready_meta + ready_at(p, c), ref = __ldg(meta);
+            if constexpr (READY) {
+                dev::wait_for_previous();  // the converted tiles' references
+                meta = p.ready_meta + ready_at(p, c), ref = *meta;
+            }
             // Scores of the half at hand; the next half's are fetched as the registers get free.
             uint32_t s[2][32];
             if (!b.wait(&sh->s_full[w][0], s_phase)) return false;
@@ -886,7 +902,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                     const int vref = ref.y & 0xffff;
                     if (READY && (t & 1)) {
                         nans |= ref.y >> 16;
-                        if (t + 1 < halves) ref = __ldg(meta + t / 2 + 1);
+                        if (t + 1 < halves) ref = meta[t / 2 + 1];
                     }
                     if (t == 0) vrun = vref;
                     const bool rare = t < 2 * whole.from || t >= 2 * whole.to || vrun - vref > kMostDown;
@@ -1032,7 +1048,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             open = true;
             if (threadIdx.x == 0)
                 p.part_open[blockIdx.x] =
-                    make_int4(c.w.seq, c.w.rt, c.w.head, b.share.followers(share - c.left, c.w.tiles));
+                    make_int4(c.w.seq, c.w.rt, c.w.head, b.share.followers(b.share.tiles - c.left, c.w.tiles));
         }
     } while (c.next(p));
     if (threadIdx.x == 0 && !open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -1046,12 +1062,17 @@ constexpr int tmem_columns(int d, int row_tiles) { return row_tiles * (kKeys + d
 
 template <int D, class Cfg, int FULL_COUNT>
 __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_raw, Shared* sh, int* scratch,
-                                      unsigned* err, Block& b, Cursor<Cfg::rows>& c) {
+                                      unsigned* err, Block& b, Cursor<Cfg>& c) {
     constexpr int kRows = Cfg::rows;
     const int tid = threadIdx.x;
     dev::let_next_start();
-    const dev::Share share = dev::take_share<kRows, kKeys, Cfg::threads>(p, scratch);
-    if (share.tiles == 0) {
+    const dev::Share share = dev::take_share<kRows, kKeys, Cfg::unit_cost, Cfg::threads>(p, scratch);
+    c.left = 0;
+    if (share.tiles > 0) {
+        c.w = dev::walk_to<kRows, kKeys>(p, share);
+        c.left = share.tiles - c.w.skip;
+    }
+    if (c.left <= 0) {
         if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
         dev::wait_for_previous();
         return false;
@@ -1089,9 +1110,8 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
     b.tmem = __shfl_sync(kFull, sh->tmem, 0);
     b.err = err;
     b.share = share;
-    c.w = dev::walk_to<kRows, kKeys>(p, share.seq, share.offset);
-    c.left = share.tiles;
     c.unit = 0;
+    c.cost = share.cost;
     c.take();
     return true;
 }
@@ -1112,9 +1132,9 @@ template <int D, int BITS>
 __global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(const AttentionParams p, unsigned* err) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared shared;
-    __shared__ int scratch[Packed::threads / 32 + 2];
+    __shared__ int scratch[Packed::threads / 16 + 2];
     Block b;
-    Cursor<Packed::rows> c;
+    Cursor<Packed> c;
     if (!begin<D, Packed, Packed::convert_warps>(p, smem_raw, &shared, scratch, err, b, c)) return;
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
     if (warp < Packed::softmax_warps) {
@@ -1133,11 +1153,10 @@ template <int D>
 __global__ void __launch_bounds__(Ready::threads, 1) attention_ready_kernel(const AttentionParams p, unsigned* err) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared shared;
-    __shared__ int scratch[Ready::threads / 32 + 2];
+    __shared__ int scratch[Ready::threads / 16 + 2];
     Block b;
-    Cursor<Ready::rows> c;
+    Cursor<Ready> c;
     if (!begin<D, Ready, 1>(p, smem_raw, &shared, scratch, err, b, c)) return;
-    dev::wait_for_previous();  // the converted tiles
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
     if (warp < Ready::softmax_warps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Ready::softmax_regs));
@@ -1172,7 +1191,7 @@ int prepare_kernel(K kernel, int smem, int regs, int& ready_device) {
 template <class Cfg>
 int grid_size(const AttentionParams& p, int max_q, int64_t* ctas) {
     const int64_t most = attention_tile_bound(p, max_q, Cfg::rows, kKeys);
-    MXK_REQUIRE(most <= std::numeric_limits<int>::max(), "cache_attention: too much work for one call");
+    MXK_REQUIRE(most <= std::numeric_limits<int>::max() / (1 + Cfg::unit_cost), "cache_attention: too much work for one call");
     static const int sms = sm_count();
     *ctas = most < sms ? most : sms;
     return MXK_OK;
@@ -1208,7 +1227,7 @@ int launch_ready(AttentionParams p, int max_q, AttentionCall& call) {
     p.ready_k = static_cast<uint8_t*>(extra);
     p.ready_v = p.ready_k + tiles * Smem<D>::tile;
     p.ready_meta = reinterpret_cast<int2*>(p.ready_v + tiles * Smem<D>::tile);
-    MXK_CHECK(call.launch("attention_unpack", attention_unpack_kernel<D, BITS>, (unsigned)tiles, 256, 0, p));
+    MXK_CHECK(call.launch("attention_unpack", attention_unpack_kernel<D, BITS>, dim3((unsigned)tiles, 2), 256, 0, p));
     MXK_CHECK(call.launch("attention_ready", attention_ready_kernel<D>, (unsigned)ctas, Ready::threads, smem, p, err));
     call.join_later<Ready::rows, D>(p, (int)ctas, 64);
     return MXK_OK;

@@ -207,6 +207,16 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                  : "memory");
 }
 
+// 1-D bulk copy shared -> global (16-byte aligned, size % 16 == 0) of the calling thread,
+// which waits until it is written.
+__device__ __forceinline__ void bulk_store_wait(void* dst, const void* src, uint32_t bytes) {
+    asm volatile(
+        "cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\t"
+        "cp.async.bulk.commit_group;\n\t"
+        "cp.async.bulk.wait_group 0;" ::"l"(dst), "r"(smem_addr(src)), "r"(bytes)
+        : "memory");
+}
+
 __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
