@@ -718,16 +718,15 @@ __device__ __noinline__ uint4 nan_features(const uint8_t* values, const int* tab
 // tile's four warps, warp r0 has rows r0, r0 + 4, ..., so a tile with few rows is loaded by
 // all of them.  Lane i names row r0 + 4 i (`at`, elements from p.q; `real`: it exists) and
 // returns the factor that makes scores of its products with lifted keys, less the keys'
-// reference.  D / 4 lanes load a row together: a thread that loads its own row touches 32
-// of them in every access.
+// reference.  D / 4 lanes load a row together (a thread that loads its own row touches 32
+// of them in every access), kBatch such loads at a time; what is needed once a row is done
+// by the lane that names it.
 template <int D>
 __device__ __forceinline__ float put_queries(const AttentionParams& p, int64_t at, bool real, uint8_t* rows, int r0) {
     constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes, kBatch = 8;
     const int lane = threadIdx.x & 31, piece = lane % kLanes, sub = lane / kLanes;
-    const unsigned mask = kAtOnce == 1 ? kFull : 0xffffu << (16 * sub);
     const unsigned reals = __ballot_sync(kFull, real);
     const bool f16 = p.dtype == MXK_F16;
-    unsigned own = 0;  // the largest magnitude of this lane's row, as bits
     auto fetch = [&](int base, uint2 (&x)[kBatch]) {
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
@@ -743,60 +742,59 @@ __device__ __forceinline__ float put_queries(const AttentionParams& p, int64_t a
             }
         }
     };
-    auto factors = [&](unsigned amax, float& f0, float& f1) -> float {
+    // row r0 + 4 r: its swizzle depends on r's lowest bit
+    const int chunk = piece / 2;
+    uint8_t* const to = rows + (chunk / 8) * Smem<D>::half + r0 * 128 + (piece & 1) * 8;
+    const int even = ((chunk % 8) ^ r0) << 4, odd = ((chunk % 8) ^ (r0 + 4)) << 4;
+    // Rows past the last real one are left as they are: a row's scores are its own.
+    const int rows_here = 32 - __clz(reals);
+    unsigned own = 0;  // the largest magnitude of this lane's row, as 16 bits
+    float f0 = 0.0f, f1 = 0.0f, factor = 0.0f;
+    uint2 next[kBatch];
+    if (rows_here) fetch(0, next);
+#pragma unroll 1
+    for (int base = 0; base < rows_here; base += kBatch * kAtOnce) {
+        uint2 x[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) x[i] = next[i];
+        if (base + kBatch * kAtOnce < rows_here) fetch(base + kBatch * kAtOnce, next);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            // 16-bit floats order as their bits (a NaN's row is NaN whatever its scale)
+            const unsigned m2 = __vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu);
+            const unsigned m = max(m2 & 0xffffu, m2 >> 16);
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const unsigned top = __reduce_max_sync(kFull, sub == k ? m : 0u);
+                if (lane == base + i * kAtOnce + k) own = top;
+            }
+        }
+        const unsigned amax = f16 ? __float_as_uint(__half2float(__ushort_as_half((unsigned short)own))) : own << 16;
         const int e = amax ? max((int)(amax >> 23) - 127, -126) : 0;
         const int down = (kQueryExp - e) / 2, rest = kQueryExp - e - down;
         f0 = __uint_as_float((uint32_t)(down + 127) << 23);
         f1 = copysignf(__uint_as_float((uint32_t)(rest + 127) << 23), p.scale_log2);
-        return fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 - down - kKeyLift / 2) << 23) *
-               __uint_as_float((uint32_t)(127 - rest - kKeyLift / 2) << 23);
-    };
-    // Rows past the last real one are left as they are: a row's scores are its own.
-    const int rows_here = 32 - __clz(reals);
-    if (rows_here == 0) return 0.0f;
-    uint2 next[kBatch];
-    fetch(0, next);
-#pragma unroll 1
-    for (int base = 0; base < rows_here; base += kBatch * kAtOnce) {
-        float4 x[kBatch];
-        unsigned amax[kBatch];
+        factor = fabsf(p.scale_log2) * __uint_as_float((uint32_t)(127 - down - kKeyLift / 2) << 23) *
+                 __uint_as_float((uint32_t)(127 - rest - kKeyLift / 2) << 23);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
+            const int r = base + i * kAtOnce + sub;
+            const float g0 = __shfl_sync(kFull, f0, r), g1 = __shfl_sync(kFull, f1, r);
             float2 u, v;
             if (f16) {
-                u = __half22float2(*reinterpret_cast<const __half2*>(&next[i].x));
-                v = __half22float2(*reinterpret_cast<const __half2*>(&next[i].y));
+                u = __half22float2(*reinterpret_cast<const __half2*>(&x[i].x));
+                v = __half22float2(*reinterpret_cast<const __half2*>(&x[i].y));
             } else {
-                u = make_float2(__uint_as_float(next[i].x << 16), __uint_as_float(next[i].x & 0xffff0000u));
-                v = make_float2(__uint_as_float(next[i].y << 16), __uint_as_float(next[i].y & 0xffff0000u));
+                u = make_float2(__uint_as_float(x[i].x << 16), __uint_as_float(x[i].x & 0xffff0000u));
+                v = make_float2(__uint_as_float(x[i].y << 16), __uint_as_float(x[i].y & 0xffff0000u));
             }
-            x[i] = make_float4(u.x, u.y, v.x, v.y);
-        }
-        if (base + kBatch * kAtOnce < rows_here) fetch(base + kBatch * kAtOnce, next);
-        // non-negative floats order as their bits (a NaN's row is NaN whatever its scale)
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            amax[i] = __reduce_max_sync(mask, __float_as_uint(fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)),
-                                                                    fmaxf(fabsf(x[i].z), fabsf(x[i].w)))));
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            float f0, f1;
-            factors(amax[i], f0, f1);
-            const __half2 a = __floats2half2_rn(x[i].x * f0 * f1, x[i].y * f0 * f1);
-            const __half2 b = __floats2half2_rn(x[i].z * f0 * f1, x[i].w * f0 * f1);
-            const int chunk = piece / 2, row = r0 + 4 * (base + i * kAtOnce + sub);
-            *reinterpret_cast<uint2*>(rows + (chunk / 8) * Smem<D>::half + row * 128 +
-                                      (((chunk % 8) ^ (row & 7)) << 4) + (piece & 1) * 8) =
-                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-#pragma unroll
-            for (int k = 0; k < kAtOnce; ++k) {
-                const unsigned m = kAtOnce == 1 ? amax[i] : __shfl_sync(kFull, amax[i], 16 * k);
-                if (lane == base + i * kAtOnce + k) own = m;
-            }
+            const __half2 a = __floats2half2_rn(u.x * g0 * g1, u.y * g0 * g1);
+            const __half2 c = __floats2half2_rn(v.x * g0 * g1, v.y * g0 * g1);
+            *reinterpret_cast<uint2*>(to + 512 * r + ((i * kAtOnce + sub) & 1 ? odd : even)) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
         }
     }
-    float f0, f1;
-    return factors(own, f0, f1);
+    return factor;
 }
 
 // A warp's 32 output rows from shared memory to where they belong, D / 8 lanes a row:
