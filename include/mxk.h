@@ -354,9 +354,9 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  *
  * Asynchronous on `stream`; partial sums live in the library's stream-ordered
  * pool on the current device (mxk_release_workspace): at most 70 MB, and, when
- * sequences have more than 256 query rows per key head (n * heads / kv_heads), their
- * keys and values converted to f16 once, seqs * kv_heads * max_kv * head_dim * 4 bytes
- * (not done where that exceeds 4 GB).  May be captured into a graph.  A device-side
+ * sequences have more than 512 query rows per key head (n * heads / kv_heads; 256 among
+ * several sequences), their keys and values converted to f16 once, seqs * kv_heads *
+ * max_kv * head_dim * 4 bytes (not done where that exceeds 4 GB).  May be captured into a graph.  A device-side
  * wait that gives up leaves the call's output undefined; the next synchronous call of
  * the library on the device reports MXK_ERR_TIMEOUT. */
 typedef struct {

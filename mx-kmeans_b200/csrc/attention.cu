@@ -23,6 +23,15 @@
 //    onto the finished scores.  Value blocks are scaled
 //    relative to the power of two of the largest value scale met so far, which
 //    only moves up, like the running maximum.
+//
+// Measured: 64 sequences of 1 to 8192 tokens (32 heads of 128 on 8, 8 bits, 555 MB) in
+// 129 to 138 us, 4.2 TB/s over all and 5.45 TB/s while every CTA streams; two of 131,072
+// (4 bits, 285 MB) in 96 to 101.  The rest is 6 us until the first rows are there, SMs that
+// differ by a fifth in the rate they get, and the join (4 us).  Finer shares did not help,
+// neither a grid of twice as many (140 and 109 us) nor short ones taken by CTAs as they got
+// done (159 and 122): every start costs more than it evens out.  In the loop a granule is
+// 478 instructions a warp (conversion to f16, products, softmax), at 3 CTAs 40 % of the ALU
+// pipe and 28 % of the tensor pipe, and none of them is the bound by itself.
 #include <algorithm>
 #include <limits>
 #include <type_traits>
@@ -55,9 +64,13 @@ constexpr int kKeys = kPair * kWarps;
 // 6: 64 sequences of 1 to 8192 tokens 150, 142, 140, 144, 146; 24 sequences with 2 to 5
 // query tokens and windows 35, 29, 27, 29, 29.
 constexpr int kUnitCost = 2;
+// CTAs that an SM holds (168 registers a thread, 75 KB of rings).  With two: 64 sequences of
+// 1 to 8192 tokens 146 us instead of 142.
 constexpr int kCtasPerSm = 3;
-// Rows per key head up to which this kernel is taken, one pass over the keys for
-// every 16 of them.
+// Rows per key head up to which this kernel is taken, one pass over the keys for every 16
+// of them.  In us, this and the tiles kernel, over 16,384 tokens (32 heads of 128 on 8): 32
+// rows 39, 45; 48 rows 47, 47; 64 rows 56, 47; 24 sequences with 2 to 5 query tokens of 8
+// heads a key head and windows 27, 54.
 constexpr int kMostFewRows = 32;
 
 // Shared-memory row pitches (bytes) of the key and value granules.  Keys are read row by
@@ -697,7 +710,7 @@ int launch_rows(AttentionParams p, int64_t most_tiles, int64_t most_rows, Attent
     const int64_t ctas = std::min<int64_t>(most_tiles, kCtasPerSm * sms);
     MXK_CHECK(call.take(p, ctas, kRows, D));
     MXK_CHECK(call.launch("attention_rows", attention_rows_kernel<D, BITS>, (unsigned)ctas, kThreads, S::smem, p));
-    call.join_later<kRows, D>(p, (int)ctas, (int)std::min<int64_t>(most_rows, kRows));
+    call.join_later(p, ctas, kRows, std::min<int64_t>(most_rows, kRows));
     return MXK_OK;
 }
 
@@ -790,5 +803,5 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
         MXK_CHECK(cache->head_dim == 128 ? launch_rows_bits<128>(cache->bits, p, most, few, call)
                                          : launch_rows_bits<64>(cache->bits, p, most, few, call));
     }
-    return call.join_all();
+    return call.join_all(cache->head_dim);
 }

@@ -325,11 +325,25 @@ __device__ __forceinline__ float row_lse(float m2, float sum) {
 
 }  // namespace dev
 
+// The partial sums of one kernel's CTAs: as in AttentionParams.
+struct Parts {
+    const float* part;
+    const float2* stat;
+    const int4* open;
+    int ctas, rows;  // rows: of its row tiles
+    int split;       // CTAs that join a unit
+};
+constexpr int kMostParts = 3;  // kernels of a call
+struct JoinParams {
+    AttentionParams p;
+    Parts parts[kMostParts];
+    int count;
+};
+
 // A row of a joined unit: v and the row's sum are over all parts, relative to `top`.
-template <int ROWS, int D>
-__device__ __forceinline__ void store_joined(const AttentionParams& p, const int4& unit, const dev::SeqView& view, int r,
-                                             int chunk, float4 v, float top, float total) {
-    const int row = unit.y * ROWS + r, j = row / p.group;
+__device__ __forceinline__ void store_joined(const AttentionParams& p, const int4& unit, const dev::SeqView& view,
+                                             int row, int chunk, float4 v, float top, float total) {
+    const int j = row / p.group;
     const int head = unit.z * p.group + (row - j * p.group);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -337,34 +351,42 @@ __device__ __forceinline__ void store_joined(const AttentionParams& p, const int
     if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
 }
 
-// Block (x, y): the unit that CTA x began and did not finish, some of its rows.  Its parts
-// are the beginning (slot 2x + 1) and what the following CTAs did first (slots 2j); they
-// add up in a fixed order.  Few parts: every D / 4 threads take a row and go through its
-// parts.  Many: the block takes a row, every D / 4 of its threads some of the parts, so a
-// unit in hundreds of parts has several loads under way.
-template <int ROWS, int D>
-__global__ void __launch_bounds__(128) attention_join_kernel(const AttentionParams p) {
+// Block (x, y) of a set of parts: the unit that CTA x began and did not finish, some of its
+// rows.  Its parts are the beginning (slot 2x + 1) and what the following CTAs did first
+// (slots 2j); they add up in a fixed order.  Few parts: every D / 4 threads take a row and
+// go through its parts.  Many: the block takes a row, every D / 4 of its threads some of the
+// parts, so a unit in hundreds of parts has several loads under way.  One launch joins the
+// parts of all of a call's kernels: a launch for each took 5 us more a kernel.
+template <int D>
+__global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams jp) {
+    const AttentionParams& p = jp.p;
     constexpr int kLanes = D / 4;            // threads of a row
     constexpr int kSub = 128 / kLanes;       // rows, or parts, at a time
     constexpr int kFew = 8;
     __shared__ float4 sums[kSub][kLanes];
     __shared__ float stats[4], sub_totals[kSub];
+    int local = blockIdx.x;
+    Parts set = jp.parts[0];
+#pragma unroll
+    for (int i = 1; i < kMostParts; ++i)
+        if (i < jp.count && local >= set.ctas * set.split) local -= set.ctas * set.split, set = jp.parts[i];
+    const int x = local / set.split, y = local - x * set.split;
     dev::wait_for_previous();
-    const int4 unit = p.part_open[blockIdx.x];
+    const int4 unit = set.open[x];
     if (!unit.w) return;
     const dev::SeqView view = dev::seq_view(p, unit.x);
-    const int rows = min(view.n * p.group - unit.y * ROWS, ROWS);
+    const int rows = min(view.n * p.group - unit.y * set.rows, set.rows);
     const int tid = threadIdx.x, chunk = tid % kLanes, sub = tid / kLanes, parts = unit.w + 1;
-    auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(blockIdx.x + i) + (i == 0 ? 1 : 0); };
+    auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(x + i) + (i == 0 ? 1 : 0); };
     if (parts <= kFew) {
-        for (int r = blockIdx.y * kSub + sub; r < rows; r += gridDim.y * kSub) {
+        for (int r = y * kSub + sub; r < rows; r += set.split * kSub) {
             float2 st[kFew];
-            float4 x[kFew];
+            float4 v_part[kFew];
 #pragma unroll
             for (int i = 0; i < kFew; ++i)
                 if (i < parts) {
-                    st[i] = p.part_stat[slot(i) * ROWS + r];
-                    x[i] = reinterpret_cast<const float4*>(p.part + (slot(i) * ROWS + r) * D)[chunk];
+                    st[i] = set.stat[slot(i) * set.rows + r];
+                    v_part[i] = reinterpret_cast<const float4*>(set.part + (slot(i) * set.rows + r) * D)[chunk];
                 }
             float top = st[0].x;
 #pragma unroll
@@ -377,16 +399,16 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionPara
                 if (i < parts) {
                     const float f = st[i].x == top ? 1.0f : dev::ex2(st[i].x - top);
                     total += st[i].y * f;
-                    v.x += x[i].x * f, v.y += x[i].y * f, v.z += x[i].z * f, v.w += x[i].w * f;
+                    v.x += v_part[i].x * f, v.y += v_part[i].y * f, v.z += v_part[i].z * f, v.w += v_part[i].w * f;
                 }
-            store_joined<ROWS, D>(p, unit, view, r, chunk, v, top, total);
+            store_joined(p, unit, view, unit.y * set.rows + r, chunk, v, top, total);
         }
         return;
     }
-    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    for (int r = y; r < rows; r += set.split) {
         // the common maximum
         float top = __int_as_float(0xff800000);
-        for (int i = tid; i < parts; i += 128) top = fmaxf(top, p.part_stat[slot(i) * ROWS + r].x);
+        for (int i = tid; i < parts; i += 128) top = fmaxf(top, set.stat[slot(i) * set.rows + r].x);
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if ((tid & 31) == 0) stats[tid >> 5] = top;
@@ -396,11 +418,11 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionPara
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
         for (int i = sub; i < parts; i += kSub) {
-            const float2 st = p.part_stat[slot(i) * ROWS + r];
-            const float4 x = reinterpret_cast<const float4*>(p.part + (slot(i) * ROWS + r) * D)[chunk];
+            const float2 st = set.stat[slot(i) * set.rows + r];
+            const float4 o = reinterpret_cast<const float4*>(set.part + (slot(i) * set.rows + r) * D)[chunk];
             const float f = st.x == top ? 1.0f : dev::ex2(st.x - top);
             total += st.y * f;
-            v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+            v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
         }
         sums[sub][chunk] = v;
         if (chunk == 0) sub_totals[sub] = total;
@@ -410,11 +432,11 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionPara
             v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int i = 0; i < kSub; ++i) {
-                const float4 x = sums[i][chunk];
-                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                const float4 o = sums[i][chunk];
+                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
                 total += sub_totals[i];
             }
-            store_joined<ROWS, D>(p, unit, view, r, chunk, v, top, total);
+            store_joined(p, unit, view, unit.y * set.rows + r, chunk, v, top, total);
         }
         __syncthreads();  // before the shared sums are written again
     }
@@ -423,7 +445,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionPara
 // The launches of one call and the memory of their partial sums, which goes back to the
 // pool, in stream order, at its end.  Kernels for sequences of different sizes write
 // different outputs, so each is launched as soon as the one before has started everywhere;
-// every one ends only when its predecessor has, so the joins, launched last, find all done.
+// every one ends only when its predecessor has, so the join, launched last, finds all done.
 class AttentionCall {
 public:
     explicit AttentionCall(cudaStream_t s) : stream_(s) {}
@@ -472,27 +494,25 @@ public:
         return MXK_OK;
     }
 
-    template <int ROWS, int D>
-    void join_later(const AttentionParams& p, int ctas, int grid_y) {
-        join_[joins_++] = Join{p, dim3((unsigned)ctas, (unsigned)grid_y), attention_join_kernel<ROWS, D>};
+    // Joins the parts of a kernel's CTAs, `split` blocks to a unit, when all are launched.
+    void join_later(const AttentionParams& p, int64_t ctas, int rows, int64_t split) {
+        join_.p = p;
+        join_.parts[join_.count++] = Parts{p.part, p.part_stat, p.part_open, (int)ctas, rows, (int)split};
     }
-    int join_all() {
-        for (int i = 0; i < joins_; ++i)
-            MXK_CHECK(launch("attention_join", join_[i].kernel, join_[i].grid, 128, 0, join_[i].p));
-        return MXK_OK;
+    int join_all(int d) {
+        if (!join_.count) return MXK_OK;
+        int64_t blocks = 0;
+        for (int i = 0; i < join_.count; ++i) blocks += (int64_t)join_.parts[i].ctas * join_.parts[i].split;
+        return launch("attention_join", d == 128 ? attention_join_kernel<128> : attention_join_kernel<64>,
+                      (unsigned)blocks, 128, 0, join_);
     }
 
 private:
-    struct Join {
-        AttentionParams p;
-        dim3 grid;
-        void (*kernel)(const AttentionParams);
-    };
     cudaStream_t stream_;
     bool first_ = true;
-    void* block_[3] = {};
-    Join join_[3];
-    int blocks_ = 0, joins_ = 0;
+    void* block_[kMostParts] = {};
+    JoinParams join_{};
+    int blocks_ = 0;
 };
 
 // attention_tiles.cu: many query rows per key head.

@@ -3,18 +3,30 @@
 //
 // With many rows the two products bound it (4 * rows * keys * D operations), with
 // the exponentials close behind: one per row and key, 16 a cycle and SM, against
-// 4 * D / 8192 cycles of tensor time.  A CTA works on 256 rows as two tiles of
-// 128, each with its scores and its output in TMEM, so the tensor core multiplies
-// for one tile while the other one is in its softmax.
+// 4 * D / 8192 cycles of tensor time.  A row tile is 128 rows, with its scores and its
+// output in TMEM; a key tile goes through in two halves of 64 tokens, so the tensor
+// core multiplies for one while the other is in the softmax.
 //
-//   softmax     two warpgroups, one per row tile; a thread owns one row: its query,
-//               running maximum and sum, its weights and its output row
+//   softmax     a warpgroup per row tile; a thread owns one row: its running maximum
+//               and sum, its weights and its output row
 //   products    one warp, whose elected lane issues S = Q K^T from shared memory and
 //               O += P V with P from TMEM
 //   keys and    two stages each of f16 tiles in shared memory (SWIZZLE_128B), filled
-//   values      either by four converter warps from the packed pages, or, when many
-//               row tiles share a key head, by bulk copies of tiles that
-//               attention_unpack_kernel has converted once for all of them
+//   values      by eight converter warps from the packed pages (attention_tiles_kernel,
+//               one row tile), or, when a key head has more rows than two row tiles, by
+//               bulk copies of tiles that attention_unpack_kernel has converted once for
+//               all of them (attention_ready_kernel, two row tiles)
+//
+// Measured at 32 heads of 128 on 8 key heads, 8 bits, 16,384 tokens cached:
+//   4096 query tokens   880 us, 1090 Tflop/s, 66 % of a library product's rate.  The
+//                       ready kernel takes 2.15 us for 256 rows x 128 keys where the
+//                       products alone need 0.57 x 2 and the exponentials 0.9 (1800 MHz):
+//                       two softmax warps a scheduler leave the waits between the steps
+//                       of a row (scores, maximum, weights, store) half uncovered.
+//   512 query tokens    179 us: 17 converting, 145 multiplying, 10 joining
+//   16 query tokens     46 us: the packed kernel converts a key tile for one row tile in
+//                       the time that tile's softmax takes
+// More query rows per thread, or two row tiles beside converters, ran out of registers.
 //
 // P (f16) overwrites the S it came from, so TMEM holds S0 S1 O0 O1, 512 columns at
 // D = 128.  Values are the right operand as they lie in the cache (one row per
@@ -48,9 +60,13 @@ constexpr int kStages = 2;               // of keys and of values
 constexpr int kMeta = 4;                 // key tiles whose references are kept (converter warps)
 constexpr int kRefStep = 4;              // value references are multiples of this many octaves
 constexpr int kMostDown = 64;            // octaves that a float32 weight may be scaled down by
-// Rows per key head above which its keys are converted beforehand, and the most
-// memory that may take.
-constexpr int kReadyRows = 256;
+// Rows per key head above which its keys are converted beforehand.  In us, packed and
+// ready kernel, over 16,384 tokens (32 heads of 128 on 8): 256 rows 72, 94; 384 rows 84,
+// 109; 512 rows 99, 111; 1024 rows (eight passes of the packed one) 121 ready.  Among
+// several sequences a lower bound, as the two kernels run one after the other and the
+// second has little to do: nine sequences with 4 to 2804 rows 147 us with 512, 132 with 256.
+constexpr int kReadyRows = 512, kReadyRowsMany = 256;
+// The most memory that converting may take: larger batches take the packed kernel.
 constexpr int64_t kReadyBytes = 4ll << 30;
 
 // The two kernels' row tiles, warps and registers.  Warpgroups give up or take registers
@@ -62,12 +78,15 @@ constexpr int64_t kReadyBytes = 4ll << 30;
 // and 15 in Packed and 0, 3, 8 and 12 in Ready, over the same 16,384 tokens: 16 query
 // tokens 62, 54, 47, 47; 64: 86, 78, 70, 72; 512: 185, 181, 176, 178; nine sequences of 1
 // to 701 query tokens and 333 to 5003 cached ones 182, 153, 141, 143.
+// join_split: blocks that join a unit.  In us for 8, 16, 32 and 64: 64 query tokens (units
+// in 18 parts) 89, 74, 68, 70; 512 (2 to 3 parts) 183, 179, 181, 181; the nine sequences
+// 128, 128, 132, 137.
 struct Packed {
     static constexpr int row_tiles = 1, rows = row_tiles * kTileRows;
     static constexpr int softmax_warps = 4 * row_tiles;
     static constexpr int convert_warps = 8;
     static constexpr int product_warp = softmax_warps + convert_warps;
-    static constexpr int unit_cost = 10;
+    static constexpr int unit_cost = 10, join_split = 32;
     static constexpr int threads = 512;
     static constexpr int launch_regs = 128, softmax_regs = 168, convert_regs = 128, product_regs = 88;
     static_assert(128 * softmax_regs + 256 * convert_regs + 128 * product_regs <= threads * launch_regs, "");
@@ -76,7 +95,7 @@ struct Ready {
     static constexpr int row_tiles = 2, rows = row_tiles * kTileRows;
     static constexpr int softmax_warps = 4 * row_tiles;
     static constexpr int product_warp = softmax_warps, load_warp = softmax_warps + 1;
-    static constexpr int unit_cost = 8;
+    static constexpr int unit_cost = 8, join_split = 16;
     static constexpr int threads = 384;
     static constexpr int launch_regs = 168, softmax_regs = 200, product_regs = 104;
     static_assert(256 * softmax_regs + 128 * product_regs <= threads * launch_regs, "");
@@ -1206,7 +1225,7 @@ int launch_packed(AttentionParams p, int max_q, AttentionCall& call) {
     MXK_CHECK(grid_size<Packed>(p, max_q, &ctas));
     MXK_CHECK(call.take(p, ctas, Packed::rows, D));
     MXK_CHECK(call.launch("attention_tiles", attention_tiles_kernel<D, BITS>, (unsigned)ctas, Packed::threads, smem, p, err));
-    call.join_later<Packed::rows, D>(p, (int)ctas, 64);
+    call.join_later(p, ctas, Packed::rows, Packed::join_split);
     return MXK_OK;
 }
 
@@ -1227,7 +1246,7 @@ int launch_ready(AttentionParams p, int max_q, AttentionCall& call) {
     p.ready_meta = reinterpret_cast<int2*>(p.ready_v + tiles * Smem<D>::tile);
     MXK_CHECK(call.launch("attention_unpack", attention_unpack_kernel<D, BITS>, dim3((unsigned)tiles, 2), 256, 0, p));
     MXK_CHECK(call.launch("attention_ready", attention_ready_kernel<D>, (unsigned)ctas, Ready::threads, smem, p, err));
-    call.join_later<Ready::rows, D>(p, (int)ctas, 64);
+    call.join_later(p, ctas, Ready::rows, Ready::join_split);
     return MXK_OK;
 }
 
@@ -1250,15 +1269,16 @@ int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q,
     // writing and reading them as f16.
     p.max_tiles = (p.max_kv + kKeys - 1) / kKeys;
     const int64_t bytes = (int64_t)p.seqs * p.kv_heads * p.max_tiles * 2 * kKeys * head_dim * 2;
-    const bool many = (int64_t)max_q * p.group > kReadyRows && p.max_tiles > 0 && bytes <= kReadyBytes;
-    const int few_q = (int)((kReadyRows + p.group - 1) / p.group);
+    const int ready_rows = p.seqs == 1 ? kReadyRows : kReadyRowsMany;
+    const bool many = (int64_t)max_q * p.group > ready_rows && p.max_tiles > 0 && bytes <= kReadyBytes;
+    const int few_q = (int)((ready_rows + p.group - 1) / p.group);
     if (many) {
         AttentionParams q = p;
-        if (p.seqs > 1 && q.min_rows <= kReadyRows) q.min_rows = kReadyRows + 1;
+        if (p.seqs > 1 && q.min_rows <= ready_rows) q.min_rows = ready_rows + 1;
         MXK_CHECK(head_dim == 128 ? launch_bits<128>(bits, q, true, max_q, call)
                                   : launch_bits<64>(bits, q, true, max_q, call));
         if (p.seqs == 1) return MXK_OK;
-        p.max_rows = kReadyRows;
+        p.max_rows = ready_rows;
         max_q = few_q;
     }
     return head_dim == 128 ? launch_bits<128>(bits, p, false, max_q, call)
