@@ -6,7 +6,8 @@
 // the key head's group) of one tile, over the tokens that any of them sees, in
 // key tiles.  Starting and ending a unit takes a CTA as long as COST key tiles (a
 // constant of each kernel), so where there are more key tiles than CTAs a unit counts
-// as that many more, which come first and hold nothing.  All units' tiles, numbered
+// as that many more (not more than a CTA's part of the tiles), which come first and
+// hold nothing.  All units' tiles, numbered
 // one after the other, are split evenly over the CTAs, so every CTA has about the same
 // to do whatever the lengths are; a CTA walks its tiles unit by unit.  A unit that one CTA has to itself is
 // written out by it; the parts of a unit that spans several go to the workspace
@@ -200,7 +201,9 @@ __device__ __forceinline__ Share take_share(const AttentionParams& p, int* scrat
     int total = 0, all_units = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) total += scratch[2 * w], all_units += scratch[2 * w + 1];
-    const int cost = total > (int)gridDim.x ? COST : 0;
+    // (A CTA that takes up a unit in its middle pays as well, so with little to do for each
+    // a high price would only leave CTAs without work.)
+    const int cost = total > (int)gridDim.x ? min(COST, total / (int)gridDim.x) : 0;
     total += cost * all_units;
     const int ctas = min(total, (int)gridDim.x);
     Share s{0, 0, 0, 0, 1, 0, cost};

@@ -183,6 +183,22 @@ def test_several_units_per_block(torch_cuda, mxk, q_len, kv_len, seqs, heads, kv
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("q_len,kv_len,seqs,heads,kv_heads", [(1, 600, 45, 8, 4), (2, 300, 400, 4, 2),
+                                                              (1, 90, 700, 4, 2), (16, 600, 10, 16, 4),
+                                                              (30, 1800, 10, 16, 4), (90, 700, 12, 16, 4)])
+@pytest.mark.parametrize("bits,dim,window", [(8, 128, 0), (4, 64, 0), (6, 64, 70)])
+def test_few_tiles_per_block(torch_cuda, mxk, q_len, kv_len, seqs, heads, kv_heads, bits, dim, window):
+    """One to a few key tiles for every block: where a block's share ends between a unit's
+    start and its first tile, blocks with nothing to do, more sequences than threads."""
+    torch, g = torch_cuda, np.random.default_rng(17)
+    kv = [kv_len - int(x) for x in g.integers(0, 41, seqs)]
+    b = build(torch, mxk, g, [q_len] * seqs, kv, heads, kv_heads, dim, 16, bits, "float16")
+    out, lse = attend(torch, mxk, b, window=window)
+    check(torch, b, out, lse, window=window)
+    again, lse2 = attend(torch, mxk, b, window=window)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
 def test_many_sequences(torch_cuda, mxk):
     """More sequences than a CTA has threads, many of them empty."""
     torch, g = torch_cuda, np.random.default_rng(4)
