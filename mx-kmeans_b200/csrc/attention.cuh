@@ -212,7 +212,7 @@ __device__ __forceinline__ Share take_share(const AttentionParams& p, int* scrat
     s.extra = total - s.each * ctas;
     s.begin = (int)blockIdx.x * s.each + min((int)blockIdx.x, s.extra);
     s.tiles = s.each + ((int)blockIdx.x < s.extra ? 1 : 0);
-    int before = 0;  // tiles of the sequences before this round's
+    int before = 0;  // tiles of the sequences before these
     for (int base = 0; base < p.seqs; base += THREADS) {
         const int i = base + tid;
         const int2 its = p.seqs <= THREADS ? mine
