@@ -8,9 +8,9 @@
 // the read the reverse, and neither does more than a few operations per element,
 // so HBM bounds both.
 //
-// Measured: 16,384 tokens of 8 heads of 128 in bf16 written as 8 bits (203 MB with the
-// cache's share) in 43 us, 4.7 TB/s; 65,536 tokens read back from 4 bits (340 MB) in 68 us,
-// 5.0 TB/s.  A token or a few take a launch's time, 3 us on the device.
+// Measured: 16,384 tokens of 8 heads of 128 in bf16 written as 8 bits and read back (203 MB)
+// in 39 us, 5.2 TB/s; 65,536 tokens read back from 4 bits (340 MB) in 62 us, 5.5 TB/s.  A
+// token or a few take a launch's time, 3 us on the device.
 #include <limits>
 
 #include "cache.cuh"
@@ -36,9 +36,10 @@ int check_cache(const mxk_cache* c, const char* who) {
 
 namespace {
 
-// Tokens that a thread handles at once.  65,536 tokens of 8 heads of 128: written in 84, 94
-// and 125 us with 1, 2 and 4 (registers cost the occupancy that hides the loads), read
-// alike with 2 and 4, which have more loads under way than 1.
+// Tokens that a thread handles at once.  65,536 tokens of 8 heads of 128, in us: written as
+// 8 bits from bf16 and read back 144 with 1 and 2, 159 with 2 and 3, 161 with 2 and 4 (a
+// second row's registers cost the write the occupancy that hides its loads); read back
+// from 4 bits 70, 63.5 and 65.5 with 1, 2 and 4.
 constexpr int kWritePasses = 1, kReadPasses = 2;
 
 struct Side {
@@ -105,7 +106,7 @@ struct Mover {
 
 // 32 bytes in one access (sm_100): a thread's 16 two-byte elements then are whole
 // sectors.  As two 16-byte accesses every sector is moved in two halves (65,536 tokens
-// read back: 8 bits to float32 156 us instead of 117, 4 bits to bf16 80 instead of 71).
+// read back: 8 bits to float32 156 us instead of 117).
 __device__ __forceinline__ void load32(const void* p, uint4& a, uint4& b) {
     asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
