@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     __shared__ int scratch[2 * kWarps + 2];
     __shared__ float stat_max[kWarps][kRows], stat_sum[kWarps][kRows];
     __shared__ __align__(16) uint4 query[kSteps][32];  // the A operand of every k-step, lane by lane
+    __shared__ int2 row_range[kRows];                  // tokens [x, y) take part in the row
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, c = lane & 3;
@@ -237,9 +238,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         const int rows = min(w.view.n * p.group - w.rt * kRows, kRows);
         const int len = w.view.len;
 
-        // This lane's rows (g and g + 8): tokens [lo, hi) take part.  Rows past the
-        // unit's see everything; they are zero queries and never written.
-        int lo[2], hi[2], all_lo = 0, all_hi = len, any_lo, any_hi;
+        // This lane's rows are g and g + 8.  Rows past the unit's see everything; they are
+        // zero queries and never written.
+        int all_lo = 0, all_hi = len, any_lo, any_hi;
         int64_t row_at[2];
         bool real[2];
 #pragma unroll
@@ -247,8 +248,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             const int r = w.rt * kRows + g + 8 * i;
             real[i] = g + 8 * i < rows;
             const int j = r / p.group;
-            lo[i] = 0, hi[i] = len;
-            if (real[i]) dev::seen_range(p, w.view, j, j, lo[i], hi[i]);
+            int lo = 0, hi = len;
+            if (real[i]) dev::seen_range(p, w.view, j, j, lo, hi);
+            if (warp == 0 && c == 0) row_range[g + 8 * i] = make_int2(lo, hi);
             row_at[i] = (int64_t)(w.view.row0 + j) * p.q_token +
                         (int64_t)(w.head * p.group + (r - j * p.group)) * p.q_head;
         }
@@ -411,10 +413,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             const int now = stage;
             stage = stage == (S::stages - 1) * S::bytes ? 0 : stage + S::bytes;
             const int t0 = (pair0 + step * kWarps) * kPair;
-            const bool last = t0 + kPair > len;
+            const bool beyond = t0 < any_lo || t0 + kPair > any_hi;  // holds tokens that no row sees
 
             // The references of the keys, the step's largest scale, and of the values, which
-            // moves up with the data.  (What lies past the sequence's end is zero.)
+            // moves up with the data.  Tokens that no row sees, before a window or past the end,
+            // count for nothing: their pages may have been given away and hold any bytes.
             int ks[4], vs[8];
             ks[0] = lds_u8<0>(ks_read + now), ks[1] = lds_u8<8 * S::scale_bytes>(ks_read + now);
             ks[2] = lds_u8<S::granule>(ks_read + now), ks[3] = lds_u8<S::granule + 8 * S::scale_bytes>(ks_read + now);
@@ -423,13 +426,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             vs[4] = lds_u8<S::granule>(vs_read + now), vs[5] = lds_u8<S::granule + S::scale_bytes>(vs_read + now);
             vs[6] = lds_u8<S::granule + 8 * S::scale_bytes>(vs_read + now);
             vs[7] = lds_u8<S::granule + 9 * S::scale_bytes>(vs_read + now);
-            if (last) {
+            if (beyond) {
+                const unsigned seen = (unsigned)(any_hi - any_lo);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (t0 + g + 8 * i >= len) ks[i] = 0;
+                    if ((unsigned)(t0 + g + 8 * i - any_lo) >= seen) ks[i] = 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (t0 + 2 * c + (i & 1) + 8 * (i >> 1) >= len) vs[i] = 0;
+                    if ((unsigned)(t0 + 2 * c + (i & 1) + 8 * (i >> 1) - any_lo) >= seen) vs[i] = 0;
             }
             const int kref = max((int)__reduce_max_sync(kFull, (unsigned)max(max(ks[0], ks[1]), max(ks[2], ks[3]))), 1);
             const int vtop = (int)__reduce_max_sync(kFull, (unsigned)max(max(max(vs[0], vs[1]), max(vs[2], vs[3])),
@@ -495,12 +499,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             for (int nt = 0; nt < 4; ++nt) s[nt][0] *= fa, s[nt][1] *= fa, s[nt][2] *= fb, s[nt][3] *= fb;
             const bool partly = t0 < all_lo || t0 + kPair > all_hi;
             if (partly) {
+                const int2 range[2] = {row_range[g], row_range[g + 8]};
 #pragma unroll
                 for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int t = t0 + 8 * nt + 2 * c + (e & 1);
-                        if (t < lo[e >> 1] || t >= hi[e >> 1]) s[nt][e] = neg_inf;
+                        if (t < range[e >> 1].x || t >= range[e >> 1].y) s[nt][e] = neg_inf;
                     }
             }
 
@@ -605,7 +610,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                 if (nans) {
                     for (int t = 0; t < kGranule; ++t)
                         for (int i = 0; i < 2; ++i) {
-                            if (t0 + h * kGranule + t < lo[i] || t0 + h * kGranule + t >= hi[i]) continue;
+                            const int2 range = row_range[g + 8 * i];
+                            if (t0 + h * kGranule + t < range.x || t0 + h * kGranule + t >= range.y) continue;
 #pragma unroll
                             for (int n = 0; n < kTiles; ++n)
 #pragma unroll

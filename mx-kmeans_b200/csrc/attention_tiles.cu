@@ -252,14 +252,22 @@ struct Converter {
         high = warp_rows * warp >= 32;
     }
 
-    // The page number and the place in it of the tile's token 16 i, in lane i < 8; `valid`
-    // tokens exist.  row_of makes the cached row of it, when the page number has arrived.
+    // Tokens [from, to) of a tile, those that some row sees: the others may lie in pages that
+    // were given away and hold any bytes, so they are not read and count for no reference.
+    struct Span {
+        int from, to;
+    };
+    static __device__ __forceinline__ Span span(int lo, int hi, int t0) {
+        return Span{min(max(lo - t0, 0), kKeys), min(max(hi - t0, 0), kKeys)};
+    }
+    // The page number and the place in it of the tile's token 16 i, in lane i < 8.
+    // row_of makes the cached row of it, when the page number has arrived.
     struct Place {
         int page, in;
     };
-    __device__ __forceinline__ Place place(const AttentionParams& p, int seq, int t0, int valid) const {
+    __device__ __forceinline__ Place place(const AttentionParams& p, int seq, int t0, Span sp) const {
         Place pl{0, 0};
-        if (lane < 8 && 16 * lane < valid) {
+        if (lane < 8 && 16 * lane < sp.to && 16 * lane + 16 > sp.from) {
             const unsigned per_page = (unsigned)p.page_size / 16u;
             const unsigned gr = (unsigned)(t0 / 16) + lane;
             const unsigned at = gr / per_page;
@@ -272,25 +280,25 @@ struct Converter {
         const int page = min(max(pl.page, 0), p.pages - 1);
         return ((uint32_t)page * p.kv_heads + head) * p.page_size + pl.in;
     }
-    __device__ __forceinline__ void load(uint32_t place, int valid, const uint8_t* values, Words& x) const {
+    __device__ __forceinline__ void load(uint32_t place, Span sp, const uint8_t* values, Words& x) const {
 #pragma unroll
         for (int i = 0; i < passes; ++i) {
             const int r = r0 + step * i;
             const uint32_t row = __shfl_sync(kFull, place, r >> 4) + (r & 15);
 #pragma unroll
             for (int k = 0; k < piece_words; ++k) x[i][k] = 0;
-            if (r < valid)
+            if (r >= sp.from && r < sp.to)
                 ldg_bytes<4 * piece_words>(values + (uint64_t)row * row_bytes + u * (4 * piece_words), x[i]);
         }
     }
     // Scale bytes of rows lane + 32 i.
-    __device__ __forceinline__ void load_scales(uint32_t place, int valid, const uint8_t* scales, uint32_t (&s)[4]) const {
+    __device__ __forceinline__ void load_scales(uint32_t place, Span sp, const uint8_t* scales, uint32_t (&s)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = lane + 32 * i;
             const uint32_t row = __shfl_sync(kFull, place, r >> 4) + (r & 15);
             s[i] = 0;
-            if (r < valid) {
+            if (r >= sp.from && r < sp.to) {
                 if constexpr (D == 128)
                     s[i] = __ldg(reinterpret_cast<const uint32_t*>(scales) + row);
                 else
@@ -368,14 +376,14 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
     const int t0 = tile * kKeys;
     // rows that see nothing still have key tile 0, of zeros where no token exists
     if (tile != 0 && (t0 >= hi || t0 + kKeys <= lo)) return;
-    const int valid = min(max(view.len - t0, 0), kKeys);
+    const typename C::Span sp = C::span(lo, hi, t0);
     const bool keys = blockIdx.y == 0;
     const C cv(threadIdx.x >> 5);
-    const uint32_t place = C::row_of(p, cv.place(p, seq, t0, valid), head);
+    const uint32_t place = C::row_of(p, cv.place(p, seq, t0, sp), head);
     uint32_t s[4];
     typename C::Words x;
-    cv.load_scales(place, valid, keys ? p.k_scales : p.v_scales, s);
-    cv.load(place, valid, keys ? p.k_values : p.v_values, x);
+    cv.load_scales(place, sp, keys ? p.k_scales : p.v_scales, s);
+    cv.load(place, sp, keys ? p.k_values : p.v_values, x);
     const int ref = keys ? C::key_ref(s) : C::value_ref(s);
     const int nans = keys ? 0 : C::take_out_nans(x);
     cv.store(x, s, keys ? ref - kKeyLift : ref, image);
@@ -403,24 +411,29 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
     struct Next {
         typename C::Place place;
         int head;
-        int valid;  // tokens that exist; -1: no such tile
+        typename C::Span span;  // to < 0: no such tile
     };
+    int lo = 0, hi = 0;  // tokens that some row of `ahead`'s unit sees
     auto here = [&]() -> Next {
         const int t0 = (ahead.w.first + ahead.tile0 + at) * kKeys;
-        const int valid = min(max(ahead.w.view.len - t0, 0), kKeys);
-        return Next{cv.place(p, ahead.w.seq, t0, valid), ahead.w.head, valid};
+        if (at == 0) {
+            const int r0 = ahead.w.rt * Packed::rows;
+            dev::seen_range(p, ahead.w.view, r0 / p.group, (r0 + ahead.rows(p) - 1) / p.group, lo, hi);
+        }
+        const typename C::Span sp = C::span(lo, hi, t0);
+        return Next{cv.place(p, ahead.w.seq, t0, sp), ahead.w.head, sp};
     };
     auto advance = [&]() -> Next {
         if (more && ++at == ahead.tiles) at = 0, more = ahead.next(p);
-        return more ? here() : Next{{0, 0}, 0, -1};
+        return more ? here() : Next{{0, 0}, 0, {0, -1}};
     };
     Next then = here();
     uint32_t row = C::row_of(p, then.place, then.head);
-    int valid = then.valid;
-    cv.load_scales(row, valid, p.k_scales, ks);
-    cv.load_scales(row, valid, p.v_scales, vs);
-    cv.load(row, valid, p.k_values, kx);
-    cv.load(row, valid, p.v_values, vx);
+    typename C::Span sp = then.span;
+    cv.load_scales(row, sp, p.k_scales, ks);
+    cv.load_scales(row, sp, p.v_scales, vs);
+    cv.load(row, sp, p.k_values, kx);
+    cv.load(row, sp, p.v_values, vx);
     then = advance();
     int stage = 0, meta_at = 0;
     uint32_t phase = 1;  // the first pass over the stages finds them empty
@@ -439,12 +452,12 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
             b.arrive(&b.sh->k_full[stage]);
 
             // the next key tile is on its way while this one's values are converted
-            valid = then.valid;
-            if (valid >= 0) {
+            sp = then.span;
+            if (sp.to >= 0) {
                 row = C::row_of(p, then.place, then.head);
-                cv.load_scales(row, valid, p.k_scales, ks);
-                cv.load_scales(row, valid, p.v_scales, vs);
-                cv.load(row, valid, p.k_values, kx);
+                cv.load_scales(row, sp, p.k_scales, ks);
+                cv.load_scales(row, sp, p.v_scales, vs);
+                cv.load(row, sp, p.k_values, kx);
                 then = advance();
             }
             // a NaN belongs to the rows that see it: they get it at the end
@@ -454,7 +467,7 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
             cv.store(vx, vs_now, vref, b.smem + L::v + stage * L::tile);
             dev::fence_proxy_async();
             b.arrive(&b.sh->v_full[stage]);
-            if (valid >= 0) cv.load(row, valid, p.v_values, vx);
+            if (sp.to >= 0) cv.load(row, sp, p.v_values, vx);
 
             ++meta_at;
             if (++stage == kStages) stage = 0, phase ^= 1;
