@@ -18,9 +18,11 @@
 //    long as q and k agree, so a lane reads a contiguous quarter of a key row, and
 //    a contiguous eighth of four value rows, and converts in registers.  The row
 //    pitches in shared memory keep those reads free of bank conflicts.
-//  * The MX scale of a key block becomes an f16 factor relative to the granule's
-//    largest scale (exact unless two blocks differ by more than 2^30), which goes
-//    onto the finished scores.  Value blocks are scaled
+//  * The MX scale of a key block becomes an f16 factor relative to the step's
+//    largest scale, which goes onto the finished scores.  Where that would not be
+//    exact (blocks that differ by more than 2^21 with 8 bits), each token's scores
+//    are relative to that token's largest scale instead, so one token's magnitude
+//    does not touch another's score.  Value blocks are scaled
 //    relative to the power of two of the largest value scale met so far, which
 //    only moves up, like the running maximum.
 //
@@ -44,6 +46,7 @@ namespace {
 using dev::ex2;
 using dev::four6;
 using dev::hmul2;
+using dev::kExactDown;
 using dev::kKeyLift;
 using dev::kQueryExp;
 using dev::kValueLift;
@@ -436,6 +439,30 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                     if ((unsigned)(t0 + 2 * c + (i & 1) + 8 * (i >> 1) - any_lo) >= seen) vs[i] = 0;
             }
             const int kref = max((int)__reduce_max_sync(kFull, (unsigned)max(max(ks[0], ks[1]), max(ks[2], ks[3]))), 1);
+            // (Tokens without a reference, at 0, count as the largest.)
+            const unsigned klow = __reduce_min_sync(kFull, min(min((unsigned)ks[0] - 1u, (unsigned)ks[1] - 1u),
+                                                               min((unsigned)ks[2] - 1u, (unsigned)ks[3] - 1u)));
+            uint32_t own_refs = 0;  // rare: the references of this lane's four tokens
+            if (kref - 1 > (int)klow + kKeyLift + kExactDown<BITS>) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t at = now + (i >> 1) * S::granule + (i & 1) * (8 * P::k);
+                    uint32_t words[(kShare + 3) / 4], any = 0;
+                    if constexpr (P::swizzled)
+                        lds_bytes<16, 0>(k_read[0] + at, words), lds_bytes<16, 0>(k_read[1] + at, words + 4);
+                    else
+                        lds_bytes<kShare, 0>(k_read[0] + at, words);
+#pragma unroll
+                    for (int k = 0; k < (kShare + 3) / 4; ++k) any |= words[k] & dev::magnitude_bits<BITS>(k);
+                    if (D == 64) any |= __shfl_xor_sync(kFull, any, 1);  // half a block a lane
+                    int ref = any ? ks[i] : 0;  // a block of zeros has no magnitude
+                    ks[i] = ref;
+                    ref = max(ref, __shfl_xor_sync(kFull, ref, 1));
+                    ref = max(max(ref, __shfl_xor_sync(kFull, ref, 2)), 1);
+                    own_refs |= (uint32_t)ref << (8 * i);
+                    ks[i] += kref - ref;
+                }
+            }
             const int vtop = (int)__reduce_max_sync(kFull, (unsigned)max(max(max(vs[0], vs[1]), max(vs[2], vs[3])),
                                                                          max(max(vs[4], vs[5]), max(vs[6], vs[7]))));
             if (vref == 0 || vtop > vref + kValueMax) {
@@ -493,10 +520,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                     }
                 }
             }
-            const float kfactor = __uint_as_float((uint32_t)kref << 23);
-            const float fa = row_factor[0] * kfactor, fb = row_factor[1] * kfactor;
+            if (own_refs == 0) {
+                const float kfactor = __uint_as_float((uint32_t)kref << 23);
+                const float fa = row_factor[0] * kfactor, fb = row_factor[1] * kfactor;
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) s[nt][0] *= fa, s[nt][1] *= fa, s[nt][2] *= fb, s[nt][3] *= fb;
+                for (int nt = 0; nt < 4; ++nt) s[nt][0] *= fa, s[nt][1] *= fa, s[nt][2] *= fb, s[nt][3] *= fb;
+            } else {
+                // columns 2c and 2c + 1 of the four tiles: the tokens of lanes 8c and 8c + 4
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t refs = __shfl_sync(kFull, own_refs, 8 * c + 4 * e);
+#pragma unroll
+                    for (int nt = 0; nt < 4; ++nt) {
+                        const float f = __uint_as_float(((refs >> (8 * nt)) & 255u) << 23);
+                        s[nt][e] *= row_factor[0] * f, s[nt][2 + e] *= row_factor[1] * f;
+                    }
+                }
+            }
             const bool partly = t0 < all_lo || t0 + kPair > all_hi;
             if (partly) {
                 const int2 range[2] = {row_range[g], row_range[g + 8]};

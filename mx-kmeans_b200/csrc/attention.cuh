@@ -51,7 +51,8 @@ struct AttentionParams {
     // keys and values converted beforehand (tiles kernel), [seqs][kv_heads][max_tiles]
     uint8_t* ready_k;
     uint8_t* ready_v;
-    int2* ready_meta;   // reference scales of the keys and values; bit 16 of y: NaNs taken out
+    int2* ready_meta;   // reference scales of the keys (or kWide) and values; bit 16 of y: NaNs taken out
+    uint8_t* ready_key_refs;  // [tile][token] reference scales of the keys of kWide tiles
     int max_tiles;
 };
 
@@ -92,7 +93,20 @@ __device__ __forceinline__ float ex2(float x) {
 // before their reference moves.
 constexpr int kKeyLift = 6;
 constexpr int kValueLift = 4, kValueMax = 6;
+// Octaves by which a block's scale may lie below what its f16 factors are relative to, so
+// that every element stays a multiple of f16's smallest, 2^-24 (elements are multiples of
+// 2^-9, 2^-3 and 2^-1).
+template <int BITS>
+constexpr int kExactDown = BITS == 8 ? 15 : (BITS == 6 ? 21 : 23);
 constexpr int kQueryExp = 12;  // query rows are scaled to a largest magnitude in [2^12, 2^13)
+
+// The magnitude bits of word i of packed elements that begin with word 0.
+template <int BITS>
+__device__ __forceinline__ uint32_t magnitude_bits(int i) {
+    if (BITS == 8) return 0x7f7f7f7fu;
+    if (BITS == 4) return 0x77777777u;
+    return i % 3 == 0 ? 0xdf7df7dfu : (i % 3 == 1 ? 0xf7df7df7u : 0x7df7df7du);
+}
 
 // The j-th group of four 6-bit codes of a packed row, one per byte.
 __device__ __forceinline__ uint32_t four6(const uint32_t* w, int j) {

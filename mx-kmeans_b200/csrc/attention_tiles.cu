@@ -33,7 +33,10 @@
 // token), read by the tensor core as an N-major operand, so nothing is transposed.
 //
 // Scales: the keys of a 128-token tile are held relative to the tile's largest
-// scale, which goes into the factor of the scores (per tile and row).  Values are
+// scale, which goes into the factor of the scores (per tile and row).  Where that would
+// not be exact (scales that differ by more than 2^21 with 8 bits) the tile is "wide":
+// each of its tokens has its own reference, and the softmax takes a slower path, so one
+// token's magnitude does not touch another's score.  Values are
 // held relative to a reference of their tile, a multiple of kRefStep octaves at or
 // above its largest scale; the output rows are kept relative to the largest
 // reference so far, and a tile with a smaller one has its weights scaled down by the
@@ -47,6 +50,7 @@ namespace mxk {
 namespace {
 
 using dev::ex2;
+using dev::kExactDown;
 using dev::kExpShift;
 using dev::kKeyLift;
 using dev::kMaxSlack;
@@ -58,6 +62,8 @@ constexpr int kKeys = 128;               // tokens of a key tile
 constexpr int kHalf = kKeys / 2;         // tokens of one step of the softmax
 constexpr int kStages = 2;               // of keys and of values
 constexpr int kMeta = 4;                 // key tiles whose references are kept (converter warps)
+constexpr int kWide = 1 << 17;           // in place of a tile's key reference: every token has its own
+constexpr int kWideRef = 200;            // what scales relative to a token's own reference are added to
 constexpr int kRefStep = 4;              // value references are multiples of this many octaves
 constexpr int kMostDown = 64;            // octaves that a float32 weight may be scaled down by
 // Rows per key head above which its keys are converted beforehand.  In us, packed and
@@ -120,6 +126,7 @@ struct Shared {
     uint64_t rows_out[2];      // the tile's output rows have left the queries' shared memory
     uint64_t drain;
     int2 meta[kMeta];          // converter warps: the key tile's references
+    uint8_t key_refs[kMeta][kKeys];  // those of its tokens, in wide tiles
     float row_factor[2][kTileRows];
     int nan_unit[4];           // converter warps: unit in which a NaN was taken out of a partly seen tile
     int abort_word;
@@ -229,6 +236,28 @@ __device__ __forceinline__ void convert16(const uint32_t* w, uint32_t f, uint32_
     }
 }
 
+// The scales s of a tile's rows lane + 32 i (place, [from, to): as in Converter), without
+// those of blocks whose elements are all zero: they have no magnitude.
+template <int D, int BITS>
+__device__ __noinline__ uint4 magnitude_scales(const uint8_t* values, uint32_t place, int from, int to, uint4 s) {
+    constexpr int kBlock = BITS;  // words of 32 elements
+    uint32_t out[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = (threadIdx.x & 31) + 32 * i;
+        const uint32_t row = __shfl_sync(kFull, place, r >> 4) + (r & 15);
+        if (r < from || r >= to) continue;
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(values + (uint64_t)row * (D * BITS / 8));
+        for (int b = 0; b < D / 32; ++b) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int k = 0; k < kBlock; ++k) any |= __ldg(w + b * kBlock + k) & dev::magnitude_bits<BITS>(k);
+            if (!any) out[i] &= ~(255u << (8 * b));
+        }
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
 // Eight warps turning a tile of 128 packed rows into f16: a thread converts 16-element
 // piece `u` of every kStep-th row.  Eight neighbouring lanes cover the 16-byte chunks of
 // two rows, so the swizzled stores meet no shared-memory bank twice.
@@ -306,16 +335,51 @@ struct Converter {
             }
         }
     }
+    static __device__ __forceinline__ unsigned top_byte(uint32_t w) {
+        const uint32_t m = max(w & 0xffffu, w >> 16);  // of the high bytes, or
+        return max(max(m >> 8, w & 255u), (w >> 16) & 255u);
+    }
     static __device__ __forceinline__ int top_scale(const uint32_t (&s)[4]) {
-        unsigned m = 0;
+        return (int)__reduce_max_sync(kFull, top_byte(__vmaxu4(__vmaxu4(s[0], s[1]), __vmaxu4(s[2], s[3]))));
+    }
+    // The smallest scale but 0 (a row that takes no part, or 2^-127); 256 if there is none.
+    static __device__ __forceinline__ int low_scale(const uint32_t (&s)[4]) {
+        uint32_t up = 0;  // bytewise 255 - (s - 1)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int b = 0; b < D / 32; ++b) m = max(m, (s[i] >> (8 * b)) & 255u);
-        return (int)__reduce_max_sync(kFull, m);
+        for (int i = 0; i < 4; ++i) up = __vmaxu4(up, ~__vsub4(s[i], 0x01010101u));
+        return 256 - (int)__reduce_max_sync(kFull, top_byte(up));
     }
     // The tile's references: keys are lifted to 2^kKeyLift below theirs.
     static __device__ __forceinline__ int key_ref(const uint32_t (&s)[4]) { return max(top_scale(s), 1); }
+    static __device__ __forceinline__ bool wide_keys(const uint32_t (&s)[4], int ref) {
+        return ref - low_scale(s) > kKeyLift + kExactDown<BITS>;
+    }
+    // Rare: the references of a tile of keys whose scales differ too much for one.  Zero
+    // blocks are left out, and if that is not enough each row gets its own at refs[row] (one
+    // warp has to write them), and the scales become relative to it.  Returns the tile's
+    // reference or kWide.
+    static __device__ __forceinline__ int spread_keys(const uint8_t* values, uint32_t place, Span sp,
+                                                      uint32_t (&s)[4], uint8_t* refs, bool write) {
+        const uint4 m = magnitude_scales<D, BITS>(values, place, sp.from, sp.to, make_uint4(s[0], s[1], s[2], s[3]));
+        s[0] = m.x, s[1] = m.y, s[2] = m.z, s[3] = m.w;
+        const int ref = key_ref(s);
+        if (!wide_keys(s, ref)) return ref;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int own = max((int)top_byte(s[i]), 1);
+            if (write) refs[(threadIdx.x & 31) + 32 * i] = (uint8_t)own;
+            uint32_t t = 0;
+#pragma unroll
+            for (int b = 0; b < D / 32; ++b) {
+                const int e = (int)((s[i] >> (8 * b)) & 255u);
+                t |= (uint32_t)(e ? max(e - own + kWideRef, 0) : 0) << (8 * b);
+            }
+            s[i] = t;
+        }
+        return kWide;
+    }
+    // What the scales of a tile are stored relative to.
+    static __device__ __forceinline__ int key_base(int ref) { return (ref == kWide ? kWideRef : ref) - kKeyLift; }
     static __device__ __forceinline__ int value_ref(const uint32_t (&s)[4]) {
         // top - ref in (kKeyLift - kRefStep, kKeyLift]
         return max(((top_scale(s) - kKeyLift + kRefStep - 1) >> 2) << 2, 1);
@@ -384,9 +448,11 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
     typename C::Words x;
     cv.load_scales(place, sp, keys ? p.k_scales : p.v_scales, s);
     cv.load(place, sp, keys ? p.k_values : p.v_values, x);
-    const int ref = keys ? C::key_ref(s) : C::value_ref(s);
+    int ref = keys ? C::key_ref(s) : C::value_ref(s);
+    if (keys && C::wide_keys(s, ref))
+        ref = C::spread_keys(p.k_values, place, sp, s, p.ready_key_refs + (int64_t)blockIdx.x * kKeys, threadIdx.x < 32);
     const int nans = keys ? 0 : C::take_out_nans(x);
-    cv.store(x, s, keys ? ref - kKeyLift : ref, image);
+    cv.store(x, s, keys ? C::key_base(ref) : ref, image);
     dev::fence_proxy_async();
     const int any_nans = __syncthreads_or(nans);
     if (threadIdx.x == 0) {
@@ -440,13 +506,16 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
     do {
         const Whole whole = whole_tiles(p, c);
         for (int t = 0; t < c.tiles; ++t) {
-            const int kref = C::key_ref(ks), vref = C::value_ref(vs);
+            int kref = C::key_ref(ks);
+            const int vref = C::value_ref(vs);
+            const bool wide = C::wide_keys(ks, kref);
             uint32_t vs_now[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) vs_now[i] = vs[i];
 
             if (!b.wait(&b.sh->k_empty[stage], phase)) return false;
-            cv.store(kx, ks, kref - kKeyLift, b.smem + L::k + stage * L::tile);
+            if (wide) kref = C::spread_keys(p.k_values, row, sp, ks, b.sh->key_refs[meta_at % kMeta], warp == 0);
+            cv.store(kx, ks, C::key_base(kref), b.smem + L::k + stage * L::tile);
             if (warp == 0 && cv.lane == 0) b.sh->meta[meta_at % kMeta] = make_int2(kref, vref);
             dev::fence_proxy_async();
             b.arrive(&b.sh->k_full[stage]);
@@ -477,7 +546,8 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
 }
 
 // Index of a key tile among the converted ones.
-__device__ __forceinline__ int64_t ready_at(const AttentionParams& p, const Cursor<Ready>& c) {
+template <class Cfg>
+__device__ __forceinline__ int64_t ready_at(const AttentionParams& p, const Cursor<Cfg>& c) {
     return ((int64_t)c.w.seq * p.kv_heads + c.w.head) * p.max_tiles + c.w.first + c.tile0;
 }
 
@@ -701,7 +771,23 @@ __device__ __noinline__ float masked_top(uint32_t s_col, int from, int to) {
     return m;
 }
 
-// Its weights, the f16 ones times `down`; returns their sum.
+// The same for a wide tile, with each token's reference: in the scores' true units.
+__device__ __noinline__ float wide_top(uint32_t s_col, int from, int to, float row_factor, const uint8_t* refs) {
+    float m = __int_as_float(0xff800000);
+#pragma unroll 1
+    for (int h = 0; h < kHalf / 32; ++h) {
+        uint32_t s[32];
+        dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
+        dev::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (32 * h + i >= from && 32 * h + i < to)
+                m = fmaxf(m, __uint_as_float(s[i]) * (row_factor * __uint_as_float((uint32_t)refs[32 * h + i] << 23)));
+    }
+    return m;
+}
+
+// Weights of the row's columns, the f16 ones times `down`; returns their sum.
 __device__ __noinline__ float masked_weights(uint32_t s_col, int from, int to, float f, float base, float down) {
     float sum = 0.0f;
 #pragma unroll 1
@@ -860,6 +946,34 @@ __device__ __forceinline__ void put_rows(const AttentionParams& p, const float4*
     }
 }
 
+// The same for a wide tile.
+__device__ __noinline__ float wide_weights(uint32_t s_col, int from, int to, float row_factor, const uint8_t* refs,
+                                           float base, float down) {
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int h = 0; h < kHalf / 32; ++h) {
+        uint32_t s[32], pw[16];
+        dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
+        dev::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            float w[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int t = 32 * h + i + k;
+                const float x = __uint_as_float(s[i + k]) * (row_factor * __uint_as_float((uint32_t)refs[t] << 23));
+                w[k] = t >= from && t < to ? ex2(x - base) : 0.0f;
+            }
+            sum += w[0] + w[1];
+            const __half2 u = __floats2half2_rn(w[0] * down, w[1] * down);
+            pw[i / 2] = *reinterpret_cast<const uint32_t*>(&u);
+        }
+        dev::tmem_st_32x32b_x16(s_col + 16 * h, pw);
+    }
+    dev::tmem_wait_st();
+    return sum;
+}
+
 // READY: tiles were converted beforehand, their references lie in global memory.
 template <int D, class Cfg, bool READY>
 __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Block& b, Cursor<Cfg> c, int warp) {
@@ -929,13 +1043,18 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                 if (!READY && !(t & 1)) ref = *const_cast<const int2*>(&sh->meta[(meta_at + t / 2) % kMeta]);
                 if (warp_real) {
                     const float f = row_factor * __uint_as_float((uint32_t)ref.x << 23);
+                    const bool wide = ref.x == kWide;
+                    const uint8_t* key_refs = nullptr;  // of this half, in wide tiles
+                    if (wide)
+                        key_refs = (READY ? p.ready_key_refs + (ready_at(p, c) + t / 2) * kKeys
+                                          : sh->key_refs[(meta_at + t / 2) % kMeta]) + (t & 1) * kHalf;
                     const int vref = ref.y & 0xffff;
                     if (READY && (t & 1)) {
                         nans |= ref.y >> 16;
                         if (t + 1 < halves) ref = meta[t / 2 + 1];
                     }
                     if (t == 0) vrun = vref;
-                    const bool rare = t < 2 * whole.from || t >= 2 * whole.to || vrun - vref > kMostDown;
+                    const bool rare = t < 2 * whole.from || t >= 2 * whole.to || vrun - vref > kMostDown || wide;
                     int from = 0, to = kHalf;
                     float top;
                     dev::tmem_wait_ld();
@@ -943,14 +1062,14 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                         const int t0 = first_key + t * kHalf;
                         from = min(max(lo - t0, 0), kHalf);
                         to = min(max(hi - t0, 0), kHalf);
-                        top = masked_top(s_at, from, to);
+                        top = wide ? wide_top(s_at, from, to, row_factor, key_refs) : masked_top(s_at, from, to);
                     } else {
                         float m[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
                         fold_top(s[0], m);
                         fold_top(s[1], m);
                         top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                     }
-                    if (top != neg_inf) top *= f;
+                    if (top != neg_inf && !wide) top *= f;
 
                     // Raise the row's maximum, or the reference of the output, if need be.
                     const bool raise = top > run_max + kMaxSlack;
@@ -973,8 +1092,9 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                     const int down = min(vrun - vref, kMostDown);
                     const float shifted = base + (float)down, up = __uint_as_float((uint32_t)(127 + down) << 23);
                     if (rare) {
-                        sum += up * masked_weights(s_at, from, to, f, shifted,
-                                                   __uint_as_float((uint32_t)max(vref - vrun + down + 127, 0) << 23));
+                        const float rest = __uint_as_float((uint32_t)max(vref - vrun + down + 127, 0) << 23);
+                        sum += up * (wide ? wide_weights(s_at, from, to, row_factor, key_refs, shifted, rest)
+                                          : masked_weights(s_at, from, to, f, shifted, rest));
                     } else {
                         float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                         uint32_t pw[16];
@@ -1253,10 +1373,11 @@ int launch_ready(AttentionParams p, int max_q, AttentionCall& call) {
     MXK_CHECK(grid_size<Ready>(p, max_q, &ctas));
     const int64_t tiles = (int64_t)p.seqs * p.kv_heads * p.max_tiles;
     void* extra = nullptr;
-    MXK_CHECK(call.take(p, ctas, Ready::rows, D, tiles * (2 * Smem<D>::tile + (int64_t)sizeof(int2)), &extra));
+    MXK_CHECK(call.take(p, ctas, Ready::rows, D, tiles * (2 * Smem<D>::tile + (int64_t)sizeof(int2) + kKeys), &extra));
     p.ready_k = static_cast<uint8_t*>(extra);
     p.ready_v = p.ready_k + tiles * Smem<D>::tile;
     p.ready_meta = reinterpret_cast<int2*>(p.ready_v + tiles * Smem<D>::tile);
+    p.ready_key_refs = reinterpret_cast<uint8_t*>(p.ready_meta + tiles);
     MXK_CHECK(call.launch("attention_unpack", attention_unpack_kernel<D, BITS>, dim3((unsigned)tiles, 2), 256, 0, p));
     MXK_CHECK(call.launch("attention_ready", attention_ready_kernel<D>, (unsigned)ctas, Ready::threads, smem, p, err));
     call.join_later(p, ctas, Ready::rows, Ready::join_split);

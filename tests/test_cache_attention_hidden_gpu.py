@@ -1,10 +1,67 @@
 """Attention over the paged MX cache: what a row does not see does not change it,
-whatever magnitudes and bytes lie there."""
+whatever magnitudes and bytes lie there; what it sees counts with its own magnitude.
+
+Tolerance, per output element, against the definition in float64 over what the row
+sees: the output's rounding (half a unit), exp(s) rounded to f16 (2^-11 of
+sum w |v|), an error of the score of token t of at most ds_t = 2^-19 * scale *
+sum_d |q_d k_td| (float32 sums, elements of q and k below 2^-24 of their row's
+largest), which changes its weight by a factor within exp(+-ds_t) and the sum of
+the weights accordingly, values below 2^-26 of the largest that the row sees, and the
+subnormal step of the output type.
+"""
+import math
+
 import numpy as np
 import pytest
-from test_cache_attention_gpu import attend, build, check
+from test_cache_attention_gpu import attend, build, cached_rows, check
 
 pytestmark = pytest.mark.gpu
+
+
+def check_rows(torch, b, out, lse, rows=None, causal=True, window=0, scale=None):
+    """Rows `rows` (query tokens of the one sequence; None: all) against the definition."""
+    c = b["cache"]
+    n, l, heads = b["q_lens"][0], b["kv_lens"][0], b["q"].shape[1]
+    scale = c.head_dim ** -0.5 if scale is None else scale
+    u, tiny = (2.0 ** -8, 0.0) if out.dtype == torch.bfloat16 else (2.0 ** -11, 2.0 ** -25)
+    k, v = cached_rows(torch, b, 0)
+    rows = torch.arange(n, device="cuda") if rows is None else rows
+    p, t = l - n + rows, torch.arange(l, device="cuda")
+    see = t[None] <= p[:, None] if causal else torch.ones(len(rows), l, dtype=torch.bool, device="cuda")
+    if window:
+        see &= t[None] > p[:, None] - window
+    for h in range(heads):
+        q = b["q"][rows, h].double()
+        kh, vh = k[:, h * c.kv_heads // heads], v[:, h * c.kv_heads // heads]
+        # nothing that is not seen enters the sums, infinite or not
+        s = torch.where(see, scale * (q @ torch.where(see.any(0)[:, None], kh, 0.0).T), -math.inf)
+        z = torch.logsumexp(s, -1)
+        w = torch.where(see, torch.exp(s - z[:, None]), 0.0)
+        ds = torch.where(w > 0, 2.0 ** -19 * abs(scale) * (q.abs() @ kh.abs().T), 0.0)
+        off = w * torch.expm1(ds)
+        vs = torch.where(see.any(0)[:, None], vh, 0.0)
+        want, size = w @ vs, w @ vs.abs()
+        most = torch.stack([vs[see[i]].abs().max() for i in range(len(rows))])[:, None]
+        tol = u * want.abs() + (2.0 ** -11 + 2.0 ** -20) * size * (1 + u) + \
+            2 * (off @ vs.abs() + off.sum(-1, keepdim=True) * size) + 2.0 ** -26 * most + tiny
+        assert bool(torch.isfinite(tol).all())
+        got = out[rows, h].double()
+        bad = ~((got - want).abs() <= tol)
+        assert not bad.any(), f"head {h}: {int(bad.sum())} values off, rows {bad.any(-1).nonzero()[:8, 0].tolist()}"
+        dz = 2 * off.sum(-1) + 2.0 ** -20 * (1 + z.abs())
+        assert bool(((lse[rows, h].double() - z).abs() <= dz).all()), f"head {h}: lse"
+
+
+def filled(torch, mxk, g, n, l, dim, bits, change, dtype="bfloat16", page=32, heads=4):
+    """One sequence of n new tokens in l, its keys and values changed by change(k, v)."""
+    k, v = (g.standard_normal((l, 2, dim)).astype(np.float32) for _ in range(2))
+    k[:, :, :3] *= 6
+    change(k, v)
+    return build(torch, mxk, g, [n], [l], heads, 2, dim, page, bits, dtype, cached=[(k, v)])
+
+
+SIZES = [(6, 200), (6, 333), (40, 300), (40, 450), (300, 700)]  # every kernel, cuts inside and at tiles
+FORMS = [(8, 128), (8, 64), (6, 128), (4, 64)]
 
 
 def poison(b, i, tokens, byte=0xff):
@@ -44,3 +101,66 @@ def test_what_lies_before_the_windows_of_several_sequences(torch_cuda, mxk):
         poison(b, i, np.arange(max(0, l - n + 1 - window)))
     got = attend(torch, mxk, b, window=window)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("n,l", SIZES)
+@pytest.mark.parametrize("size", [2.0 ** 30, 2.0 ** 60, math.inf])
+def test_a_later_key_of_any_size(torch_cuda, mxk, bits, dim, n, l, size):
+    """The key of a token in the middle of the chunk is huge or has overflowed: the rows
+    before it get their own scores."""
+    torch, g = torch_cuda, np.random.default_rng(23)
+    at = l - n + n // 2
+
+    def change(k, v):
+        k[at, :, 7] = size
+    b = filled(torch, mxk, g, n, l, dim, bits, change)
+    out, lse = attend(torch, mxk, b)
+    check_rows(torch, b, out, lse, torch.arange(n // 2, device="cuda"))
+
+
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("n,l", SIZES)
+def test_an_earlier_key_outside_the_window(torch_cuda, mxk, bits, dim, n, l):
+    """A huge key that only the first rows' windows hold."""
+    torch, g = torch_cuda, np.random.default_rng(24)
+    window = 90
+
+    def change(k, v):
+        k[l - n - window + n // 2, :, 7] = 2.0 ** 40
+    b = filled(torch, mxk, g, n, l, dim, bits, change)
+    out, lse = attend(torch, mxk, b, window=window)
+    check_rows(torch, b, out, lse, torch.arange(n // 2 + 1, n, device="cuda"), window=window)
+
+
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("n,l", SIZES)
+def test_scores_far_below_the_others(torch_cuda, mxk, bits, dim, n, l):
+    """Keys that point away from every query with a magnitude of 2^40: they weigh nothing,
+    and the others keep their scores."""
+    torch, g = torch_cuda, np.random.default_rng(25)
+
+    def change(k, v):
+        k[:, :, 5] = 0.25  # all queries are positive there
+        k[[3, l // 2, l - n // 2 - 1]] = 0
+        k[[3, l // 2, l - n // 2 - 1], :, 5] = -2.0 ** 40
+    b = filled(torch, mxk, g, n, l, dim, bits, change)
+    b["q"][..., 5] = 1.0
+    out, lse = attend(torch, mxk, b)
+    check_rows(torch, b, out, lse)
+
+
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("n,l", SIZES)
+def test_blocks_of_zeros_beside_small_keys(torch_cuda, mxk, bits, dim, n, l):
+    """Keys of about 2^-40 under a scale of 2^38, with blocks of zeros (whose scale byte
+    stands for 1) and whole rows of them."""
+    torch, g = torch_cuda, np.random.default_rng(26)
+
+    def change(k, v):
+        k *= 2.0 ** -40
+        k[:, :, 32:64] = 0
+        k[::7] = 0
+    b = filled(torch, mxk, g, n, l, dim, bits, change)
+    out, lse = attend(torch, mxk, b, scale=2.0 ** 38)
+    check_rows(torch, b, out, lse, scale=2.0 ** 38)
