@@ -334,7 +334,8 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  * products scale * q . k over the tokens that take part,
  *     out = sum_t exp(s_t) v_t / sum_t exp(s_t),    lse = log(sum_t exp(s_t));
  * a row with no such token gets zeros and -inf.  Tokens outside [0, L) are never
- * read; a NaN among the keys or values reaches the rows that see its token only.
+ * read.  What a row does not see does not change it: neither NaNs, whatever magnitude,
+ * nor, in tokens that no row of the sequence sees (before every window), any bytes.
  * (Scale bytes are taken to be 0 .. 254; cache_write never stores 255.)
  *
  * cu_q (seqs + 1), page_table, kv_lens: int32 on the device.  max_q and max_kv
@@ -346,9 +347,9 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  * head_dim must be 64 or 128 (others: MXK_ERR_UNSUPPORTED).
  *
  * Products are taken in f16 with float32 sums: every MX element times its scale
- * is exact in f16 relative to a power of two that moves with the data (values
- * below 2^-24 of the largest magnitude met in the same head may lose bits), q's
- * rows are scaled into f16 by a power of two, and exp(s - max) is rounded to f16
+ * is exact in f16 relative to a power of two that moves with the data, but for keys
+ * below 2^-21 of their token's largest block, and values below 2^-24 of the largest
+ * that the row sees, which may lose bits; q's rows are scaled into f16 by a power of two, and exp(s - max) is rounded to f16
  * for the product with v.  Statistics are float32.  The result does not depend on
  * timing: partial sums join in a fixed order.
  *

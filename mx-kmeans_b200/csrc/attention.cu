@@ -22,9 +22,12 @@
 //    largest scale, which goes onto the finished scores.  Where that would not be
 //    exact (blocks that differ by more than 2^21 with 8 bits), each token's scores
 //    are relative to that token's largest scale instead, so one token's magnitude
-//    does not touch another's score.  Value blocks are scaled
-//    relative to the power of two of the largest value scale met so far, which
-//    only moves up, like the running maximum.
+//    does not touch another's score.  Value blocks are scaled relative to a power of
+//    two that follows the largest scale of the steps; an output row is kept relative to
+//    the largest such power that the row itself met, and its weights are lowered by the
+//    difference.  Steps of which the rows see different tokens, with scales too far
+//    apart, are multiplied in bands of 8 octaves, each for the rows that see one of its
+//    tokens.
 //
 // Measured: 64 sequences of 1 to 8192 tokens (32 heads of 128 on 8, 8 bits, 555 MB) in
 // 129 to 138 us, 4.2 TB/s over all and 5.45 TB/s while every CTA streams; two of 131,072
@@ -49,11 +52,13 @@ using dev::hmul2;
 using dev::kExactDown;
 using dev::kKeyLift;
 using dev::kQueryExp;
+using dev::kScaleOfZeros;
 using dev::kValueLift;
 using dev::kValueMax;
 using dev::pow2_f16x2;
 using dev::kExpShift;
 using dev::kMaxSlack;
+using dev::kMostLift;
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kRows = 16;     // query rows of a unit
@@ -169,6 +174,19 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The magnitude bits of word k of a lane's N bytes of a packed row.
+template <int BITS, int N>
+__device__ __forceinline__ uint32_t share_bits(int k) {
+    if constexpr (BITS != 6) {
+        return dev::magnitude_bits<BITS>(k);
+    } else if constexpr (N % 12 == 0) {
+        return dev::magnitude_bits<6>(k);
+    } else {  // six bytes, from the first code of a group of four
+        static_assert(N == 6, "");
+        return k == 0 ? 0xdf7df7dfu : 0x7df7u;
+    }
 }
 
 template <int D, int BITS>
@@ -406,6 +424,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         float base[2] = {-kExpShift, -kExpShift};  // what is subtracted from a score: run_max - kExpShift
         float sum[2] = {0.0f, 0.0f};               // this lane's share of the rows' sums
         int vref = 0;                              // values are held relative to 2^(vref - 127); 0: none yet
+        int row_ref[2] = {0, 0};                   // the output rows relative to 2^(row_ref - 127)
+        int settled = -1;                          // the vref that all rows have taken note of; -1: not all
+        bool lowered = false;                      // some row's reference is above vref
 
         int stage = 0;  // offset of the stage at hand
         for (int step = 0; step < steps; ++step) {
@@ -416,10 +437,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             const int now = stage;
             stage = stage == (S::stages - 1) * S::bytes ? 0 : stage + S::bytes;
             const int t0 = (pair0 + step * kWarps) * kPair;
-            const bool beyond = t0 < any_lo || t0 + kPair > any_hi;  // holds tokens that no row sees
+            const bool partly = t0 < all_lo || t0 + kPair > all_hi;  // some row does not see all of it
 
             // The references of the keys, the step's largest scale, and of the values, which
-            // moves up with the data.  Tokens that no row sees, before a window or past the end,
+            // moves with the data.  Tokens that no row sees, before a window or past the end,
             // count for nothing: their pages may have been given away and hold any bytes.
             int ks[4], vs[8];
             ks[0] = lds_u8<0>(ks_read + now), ks[1] = lds_u8<8 * S::scale_bytes>(ks_read + now);
@@ -429,107 +450,168 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             vs[4] = lds_u8<S::granule>(vs_read + now), vs[5] = lds_u8<S::granule + S::scale_bytes>(vs_read + now);
             vs[6] = lds_u8<S::granule + 8 * S::scale_bytes>(vs_read + now);
             vs[7] = lds_u8<S::granule + 9 * S::scale_bytes>(vs_read + now);
-            if (beyond) {
+            int k_least = min(min(ks[0], ks[1]), min(ks[2], ks[3]));
+            int v_least = min(min(min(vs[0], vs[1]), min(vs[2], vs[3])), min(min(vs[4], vs[5]), min(vs[6], vs[7])));
+            bool leading = false, trailing = false;  // some rows see only its end, or only its beginning
+            if (partly) {
                 const unsigned seen = (unsigned)(any_hi - any_lo);
+                k_least = v_least = 255;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if ((unsigned)(t0 + g + 8 * i - any_lo) >= seen) ks[i] = 0;
+                    if ((unsigned)(t0 + g + 8 * i - any_lo) >= seen)
+                        ks[i] = 0;
+                    else
+                        k_least = min(k_least, ks[i]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if ((unsigned)(t0 + 2 * c + (i & 1) + 8 * (i >> 1) - any_lo) >= seen) vs[i] = 0;
-            }
-            const int kref = max((int)__reduce_max_sync(kFull, (unsigned)max(max(ks[0], ks[1]), max(ks[2], ks[3]))), 1);
-            // (Tokens without a reference, at 0, count as the largest.)
-            const unsigned klow = __reduce_min_sync(kFull, min(min((unsigned)ks[0] - 1u, (unsigned)ks[1] - 1u),
-                                                               min((unsigned)ks[2] - 1u, (unsigned)ks[3] - 1u)));
-            uint32_t own_refs = 0;  // rare: the references of this lane's four tokens
-            if (kref - 1 > (int)klow + kKeyLift + kExactDown<BITS>) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t at = now + (i >> 1) * S::granule + (i & 1) * (8 * P::k);
-                    uint32_t words[(kShare + 3) / 4], any = 0;
-                    if constexpr (P::swizzled)
-                        lds_bytes<16, 0>(k_read[0] + at, words), lds_bytes<16, 0>(k_read[1] + at, words + 4);
+                    if ((unsigned)(t0 + 2 * c + (i & 1) + 8 * (i >> 1) - any_lo) >= seen)
+                        vs[i] = 0;
                     else
-                        lds_bytes<kShare, 0>(k_read[0] + at, words);
-#pragma unroll
-                    for (int k = 0; k < (kShare + 3) / 4; ++k) any |= words[k] & dev::magnitude_bits<BITS>(k);
-                    if (D == 64) any |= __shfl_xor_sync(kFull, any, 1);  // half a block a lane
-                    int ref = any ? ks[i] : 0;  // a block of zeros has no magnitude
-                    ks[i] = ref;
-                    ref = max(ref, __shfl_xor_sync(kFull, ref, 1));
-                    ref = max(max(ref, __shfl_xor_sync(kFull, ref, 2)), 1);
-                    own_refs |= (uint32_t)ref << (8 * i);
-                    ks[i] += kref - ref;
-                }
+                        v_least = min(v_least, vs[i]);
+                leading = t0 < all_lo && any_lo < all_lo, trailing = t0 + kPair > all_hi && all_hi < any_hi;
             }
-            const int vtop = (int)__reduce_max_sync(kFull, (unsigned)max(max(max(vs[0], vs[1]), max(vs[2], vs[3])),
-                                                                         max(max(vs[4], vs[5]), max(vs[6], vs[7]))));
-            if (vref == 0 || vtop > vref + kValueMax) {
-                const int ref = max(vtop - kValueLift, 1);
-                if (vref != 0) {
-                    const float f = __uint_as_float((uint32_t)max(vref - ref + 127, 0) << 23);
+            auto largest = [&]() -> int {
+                return (int)__reduce_max_sync(kFull, (unsigned)max(max(max(vs[0], vs[1]), max(vs[2], vs[3])),
+                                                                   max(max(vs[4], vs[5]), max(vs[6], vs[7]))));
+            };
+            const int kref = max((int)__reduce_max_sync(kFull, (unsigned)max(max(ks[0], ks[1]), max(ks[2], ks[3]))), 1);
+            const int vtop = largest();
+
+            // An output row's reference goes up when the row meets a larger one.
+            auto raise_row = [&](int i, int ref) {
+                const float f = __uint_as_float((uint32_t)max(row_ref[i] - ref + 127, 0) << 23);
 #pragma unroll
-                    for (int n = 0; n < kTiles; ++n)
+                for (int n = 0; n < kTiles; ++n) o[n][2 * i] *= f, o[n][2 * i + 1] *= f;
+                row_ref[i] = ref;
+            };
+            uint32_t key_refs = 0;  // rare: the references of this lane's four tokens, a byte each
+            bool bands = false;     // rare: the values are multiplied in bands
+            if (__any_sync(kFull, k_least < kref - kKeyLift - kExactDown<BITS> || v_least < vref - kExactDown<BITS>) ||
+                (unsigned)(vtop - vref) > (unsigned)kValueMax || vref != settled || leading) {
+                // Blocks of zeros have no magnitude: scales without them, where they matter.
+                if (__any_sync(kFull, k_least < kref - kKeyLift - kExactDown<BITS>)) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[n][e] *= f;
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t at = now + (i >> 1) * S::granule + (i & 1) * (8 * P::k);
+                        uint32_t words[(kShare + 3) / 4], any = 0;
+                        if constexpr (P::swizzled)
+                            lds_bytes<16, 0>(k_read[0] + at, words), lds_bytes<16, 0>(k_read[1] + at, words + 4);
+                        else
+                            lds_bytes<kShare, 0>(k_read[0] + at, words);
+#pragma unroll
+                        for (int k = 0; k < (kShare + 3) / 4; ++k) any |= words[k] & share_bits<BITS, kShare>(k);
+                        if (D == 64) any |= __shfl_xor_sync(kFull, any, 1);  // half a block a lane
+                        int ref = any ? ks[i] : 0;
+                        ks[i] = ref;
+                        ref = max(ref, __shfl_xor_sync(kFull, ref, 1));
+                        ref = max(max(ref, __shfl_xor_sync(kFull, ref, 2)), 1);
+                        key_refs |= (uint32_t)ref << (8 * i);
+                        ks[i] += kref - ref;
+                    }
                 }
-                vref = ref;
+                // the smallest but 0; 256 if there is none
+                auto lowest = [&]() -> int {
+                    unsigned m = 255u;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) m = min(m, (unsigned)vs[i] - 1u);
+                    return (int)__reduce_min_sync(kFull, m) + 1;
+                };
+                const int most = leading ? kMostLift : kValueLift + kExactDown<BITS>;
+                int top = vtop, low = lowest();
+                if (top - low > most || (top == kScaleOfZeros && low == kScaleOfZeros)) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t at = v_read[i & 1] + now + (i >> 2) * S::granule + ((i >> 1) & 1) * (8 * P::v);
+                        uint32_t words[(vShare + 3) / 4], any = 0;
+                        lds_bytes<vShare, 0>(at, words);
+#pragma unroll
+                        for (int k = 0; k < (vShare + 3) / 4; ++k) any |= words[k] & share_bits<BITS, vShare>(k);
+                        any |= __shfl_xor_sync(kFull, any, 4);  // half a block a lane, or a quarter
+                        if (D == 64) any |= __shfl_xor_sync(kFull, any, 8);
+                        if (!any) vs[i] = 0;
+                    }
+                    top = largest(), low = lowest();
+                }
+                bands = (leading || trailing) && top - low > most;
+                // (A reference is at most the step's largest scale, so what earlier steps held,
+                // and some rows did not see, does not stay.)
+                if (!bands && top > 0 &&
+                    (vref == 0 || top > vref + kValueMax || top < vref || low < vref - kExactDown<BITS>))
+                    vref = max(top - kValueLift, 1);
+                if (bands) {
+                    settled = -1;
+                } else if (vref > 0 && vref != settled) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        bool sees = true;
+                        if (leading || trailing) {
+                            const int2 range = row_range[g + 8 * i];
+                            sees = range.x < t0 + kPair && range.y > t0;
+                        }
+                        if (sees && row_ref[i] < vref) raise_row(i, vref);
+                    }
+                    lowered = __any_sync(kFull, max(row_ref[0], row_ref[1]) > vref);
+                    settled = leading || trailing ? -1 : vref;
+                }
             }
 
             // scores: 16 rows x 4 tiles of 8 tokens
             float s[4][4];
+            auto multiply_keys = [&]() {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t key_words[2][(kShare + 3) / 4];
-                const uint32_t at = now + h * S::granule;
-                if constexpr (P::swizzled) {
-                    lds_bytes<16, 0>(k_read[0] + at, key_words[0]), lds_bytes<16, 0>(k_read[1] + at, key_words[0] + 4);
-                    lds_bytes<16, 8 * P::k>(k_read[0] + at, key_words[1]);
-                    lds_bytes<16, 8 * P::k>(k_read[1] + at, key_words[1] + 4);
-                } else {
-                    lds_bytes<kShare, 0>(k_read[0] + at, key_words[0]);
-                    lds_bytes<kShare, 8 * P::k>(k_read[0] + at, key_words[1]);
-                }
-                const int e0 = ks[2 * h] - kref + kKeyLift, e1 = ks[2 * h + 1] - kref + kKeyLift;
-                const uint32_t kf[2] = {pow2_f16x2(e0, e0), pow2_f16x2(e1, e1)};
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t key_words[2][(kShare + 3) / 4];
+                    const uint32_t at = now + h * S::granule;
+                    if constexpr (P::swizzled) {
+                        lds_bytes<16, 0>(k_read[0] + at, key_words[0]), lds_bytes<16, 0>(k_read[1] + at, key_words[0] + 4);
+                        lds_bytes<16, 8 * P::k>(k_read[0] + at, key_words[1]);
+                        lds_bytes<16, 8 * P::k>(k_read[1] + at, key_words[1] + 4);
+                    } else {
+                        lds_bytes<kShare, 0>(k_read[0] + at, key_words[0]);
+                        lds_bytes<kShare, 8 * P::k>(k_read[0] + at, key_words[1]);
+                    }
+                    const int e0 = ks[2 * h] - kref + kKeyLift, e1 = ks[2 * h + 1] - kref + kKeyLift;
+                    const uint32_t kf[2] = {pow2_f16x2(e0, e0), pow2_f16x2(e1, e1)};
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
-                    s[2 * h + nt][0] = s[2 * h + nt][1] = s[2 * h + nt][2] = s[2 * h + nt][3] = 0.0f;
+                    for (int nt = 0; nt < 2; ++nt)
+                        s[2 * h + nt][0] = s[2 * h + nt][1] = s[2 * h + nt][2] = s[2 * h + nt][3] = 0.0f;
 #pragma unroll
-                for (int k = 0; k < kSteps; k += 2) {
-                    uint32_t qa[2][4];
-                    lds_at(q_read + 512 * k, qa[0]);
-                    lds_at(q_read + 512 * (k + 1), qa[1]);
+                    for (int k = 0; k < kSteps; k += 2) {
+                        uint32_t qa[2][4];
+                        lds_at(q_read + 512 * k, qa[0]);
+                        lds_at(q_read + 512 * (k + 1), qa[1]);
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        uint32_t x[4];
-                        if constexpr (BITS == 4) {
-                            dev::e2m1x8_to_f16(key_words[nt][k / 2], x);
-                        } else {
-                            constexpr int kCode = BITS == 4 ? 8 : BITS;
+                        for (int nt = 0; nt < 2; ++nt) {
+                            uint32_t x[4];
+                            if constexpr (BITS == 4) {
+                                dev::e2m1x8_to_f16(key_words[nt][k / 2], x);
+                            } else {
+                                constexpr int kCode = BITS == 4 ? 8 : BITS;
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const uint32_t four = BITS == 8 ? key_words[nt][k + i] : four6(key_words[nt], k + i);
-                                x[2 * i] = dev::codes_to_f16x2<kCode>(four);
-                                x[2 * i + 1] = dev::codes_to_f16x2<kCode>(four >> 16);
+                                for (int i = 0; i < 2; ++i) {
+                                    const uint32_t four = BITS == 8 ? key_words[nt][k + i] : four6(key_words[nt], k + i);
+                                    x[2 * i] = dev::codes_to_f16x2<kCode>(four);
+                                    x[2 * i + 1] = dev::codes_to_f16x2<kCode>(four >> 16);
+                                }
                             }
+                            mma16816(s[2 * h + nt], qa[0], hmul2(x[0], kf[nt]), hmul2(x[1], kf[nt]));
+                            mma16816(s[2 * h + nt], qa[1], hmul2(x[2], kf[nt]), hmul2(x[3], kf[nt]));
                         }
-                        mma16816(s[2 * h + nt], qa[0], hmul2(x[0], kf[nt]), hmul2(x[1], kf[nt]));
-                        mma16816(s[2 * h + nt], qa[1], hmul2(x[2], kf[nt]), hmul2(x[3], kf[nt]));
                     }
                 }
-            }
-            if (own_refs == 0) {
+            };
+            if (key_refs == 0) {
+                multiply_keys();
                 const float kfactor = __uint_as_float((uint32_t)kref << 23);
                 const float fa = row_factor[0] * kfactor, fb = row_factor[1] * kfactor;
 #pragma unroll
                 for (int nt = 0; nt < 4; ++nt) s[nt][0] *= fa, s[nt][1] *= fa, s[nt][2] *= fb, s[nt][3] *= fb;
             } else {
+                multiply_keys();
                 // columns 2c and 2c + 1 of the four tiles: the tokens of lanes 8c and 8c + 4
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const uint32_t refs = __shfl_sync(kFull, own_refs, 8 * c + 4 * e);
+                    const uint32_t refs = __shfl_sync(kFull, key_refs, 8 * c + 4 * e);
 #pragma unroll
                     for (int nt = 0; nt < 4; ++nt) {
                         const float f = __uint_as_float(((refs >> (8 * nt)) & 255u) << 23);
@@ -537,7 +619,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                     }
                 }
             }
-            const bool partly = t0 < all_lo || t0 + kPair > all_hi;
             if (partly) {
                 const int2 range[2] = {row_range[g], row_range[g + 8]};
 #pragma unroll
@@ -571,97 +652,151 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                 }
             }
             uint32_t pa[2][4];
+            auto make_weights = [&]() {
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                const float p0 = ex2(s[nt][0] - base[0]), p1 = ex2(s[nt][1] - base[0]);
-                const float p2 = ex2(s[nt][2] - base[1]), p3 = ex2(s[nt][3] - base[1]);
-                sum[0] += p0 + p1, sum[1] += p2 + p3;
-                const __half2 a = __floats2half2_rn(p0, p1), b = __floats2half2_rn(p2, p3);
-                pa[nt >> 1][2 * (nt & 1)] = *reinterpret_cast<const uint32_t*>(&a);
-                pa[nt >> 1][2 * (nt & 1) + 1] = *reinterpret_cast<const uint32_t*>(&b);
-            }
+                for (int nt = 0; nt < 4; ++nt) {
+                    const float p0 = ex2(s[nt][0] - base[0]), p1 = ex2(s[nt][1] - base[0]);
+                    const float p2 = ex2(s[nt][2] - base[1]), p3 = ex2(s[nt][3] - base[1]);
+                    sum[0] += p0 + p1, sum[1] += p2 + p3;
+                    const __half2 a = __floats2half2_rn(p0, p1), b = __floats2half2_rn(p2, p3);
+                    pa[nt >> 1][2 * (nt & 1)] = *reinterpret_cast<const uint32_t*>(&a);
+                    pa[nt >> 1][2 * (nt & 1) + 1] = *reinterpret_cast<const uint32_t*>(&b);
+                }
 
-            // values: of each granule this lane's tokens 2c, 2c + 1, 2c + 8, 2c + 9
+            };
+            // values: of each granule this lane's tokens 2c, 2c + 1, 2c + 8, 2c + 9, their
+            // scales in vs relative to ref
+            auto add_values = [&](const int (&vs)[8], int ref) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t at = now + h * S::granule;
-                uint32_t vw[4][(vShare + 3) / 4];
-                lds_bytes<vShare, 0>(v_read[0] + at, vw[0]);
-                lds_bytes<vShare, 0>(v_read[1] + at, vw[1]);
-                lds_bytes<vShare, 8 * P::v>(v_read[0] + at, vw[2]);
-                lds_bytes<vShare, 8 * P::v>(v_read[1] + at, vw[3]);
-                const uint32_t f0 = pow2_f16x2(vs[4 * h] - vref, vs[4 * h + 1] - vref);
-                const uint32_t f1 = pow2_f16x2(vs[4 * h + 2] - vref, vs[4 * h + 3] - vref);
-                bool nans = false;
-                if constexpr (BITS == 8) {
-                    // A stored NaN belongs to the rows that see its token: where some row
-                    // does not, it is taken out here and put into the others' sums below.
-                    if (partly) {
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t at = now + h * S::granule;
+                    uint32_t vw[4][(vShare + 3) / 4];
+                    lds_bytes<vShare, 0>(v_read[0] + at, vw[0]);
+                    lds_bytes<vShare, 0>(v_read[1] + at, vw[1]);
+                    lds_bytes<vShare, 8 * P::v>(v_read[0] + at, vw[2]);
+                    lds_bytes<vShare, 8 * P::v>(v_read[1] + at, vw[3]);
+                    const uint32_t f0 = pow2_f16x2(vs[4 * h] - ref, vs[4 * h + 1] - ref);
+                    const uint32_t f1 = pow2_f16x2(vs[4 * h + 2] - ref, vs[4 * h + 3] - ref);
+                    bool nans = false;
+                    if constexpr (BITS == 8) {
+                        // A stored NaN belongs to the rows that see its token: where some row
+                        // does not, it is taken out here and put into the others' sums below.
+                        if (partly) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int j = 0; j < vShare / 4; ++j) {
-                                const uint32_t bad = __vcmpeq4(vw[i][j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                                nans |= bad != 0;
-                                vw[i][j] &= ~bad;
+                                for (int j = 0; j < vShare / 4; ++j) {
+                                    const uint32_t bad = __vcmpeq4(vw[i][j] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                                    nans |= bad != 0;
+                                    vw[i][j] &= ~bad;
+                                }
+                            nans = __any_sync(kFull, nans);
+                        }
+                    }
+                    if constexpr (BITS == 4) {
+#pragma unroll
+                        for (int j = 0; j < vShare / 4; ++j) {
+                            // bytes of (token, token + 1) nibbles: even features, then odd ones
+                            uint32_t even[2][4], odd[2][4];
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const uint32_t a = vw[2 * i][j], b = vw[2 * i + 1][j];
+                                dev::e2m1x8_to_f16((a & 0x0f0f0f0fu) | ((b << 4) & 0xf0f0f0f0u), even[i]);
+                                dev::e2m1x8_to_f16(((a >> 4) & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u), odd[i]);
                             }
-                        nans = __any_sync(kFull, nans);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                mma16816(o[8 * j + 2 * i], pa[h], hmul2(even[0][i], f0), hmul2(even[1][i], f1));
+                                mma16816(o[8 * j + 2 * i + 1], pa[h], hmul2(odd[0][i], f0), hmul2(odd[1][i], f1));
+                            }
+                        }
+                    } else {
+                        constexpr int kCode = BITS == 4 ? 8 : BITS;
+#pragma unroll
+                        for (int j = 0; j < D / 32; ++j) {
+                            uint32_t four[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) four[i] = BITS == 8 ? vw[i][j] : four6(vw[i], j);
+                            // (token, token + 1) bytes of features 0, 1 and of 2, 3
+                            const uint32_t a01 = __byte_perm(four[0], four[1], 0x5140);
+                            const uint32_t a23 = __byte_perm(four[0], four[1], 0x7362);
+                            const uint32_t b01 = __byte_perm(four[2], four[3], 0x5140);
+                            const uint32_t b23 = __byte_perm(four[2], four[3], 0x7362);
+                            mma16816(o[4 * j], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a01), f0),
+                                     hmul2(dev::codes_to_f16x2<kCode>(b01), f1));
+                            mma16816(o[4 * j + 1], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a01 >> 16), f0),
+                                     hmul2(dev::codes_to_f16x2<kCode>(b01 >> 16), f1));
+                            mma16816(o[4 * j + 2], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a23), f0),
+                                     hmul2(dev::codes_to_f16x2<kCode>(b23), f1));
+                            mma16816(o[4 * j + 3], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a23 >> 16), f0),
+                                     hmul2(dev::codes_to_f16x2<kCode>(b23 >> 16), f1));
+                        }
+                    }
+                    if (nans) {
+                        for (int t = 0; t < kGranule; ++t)
+                            for (int i = 0; i < 2; ++i) {
+                                const int2 range = row_range[g + 8 * i];
+                                if (t0 + h * kGranule + t < range.x || t0 + h * kGranule + t >= range.y) continue;
+#pragma unroll
+                                for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) {
+                                        const int byte = (2 * c + e) * vShare + n;
+                                        const int in_row = P::swizzled ? (((byte >> 4) ^ (t & 7)) << 4) + (byte & 15) : byte;
+                                        if ((lds_u8<0>(ring + at + S::v_at + t * P::v + in_row) & 0x7f) == 0x7f)
+                                            o[n][2 * i + e] = __int_as_float(0x7fc00000);
+                                    }
+                            }
                     }
                 }
-                if constexpr (BITS == 4) {
+            };
+            if (!bands && !lowered) {
+                make_weights();
+                add_values(vs, vref);
+            } else {
+                make_weights();
+                int down[2] = {0, 0};  // octaves that the rows' weights have been lowered by so far
+                auto lower_weights = [&](int ref) {
 #pragma unroll
-                    for (int j = 0; j < vShare / 4; ++j) {
-                        // bytes of (token, token + 1) nibbles: even features, then odd ones
-                        uint32_t even[2][4], odd[2][4];
+                    for (int i = 0; i < 2; ++i) {
+                        const int by = max(row_ref[i] - ref, 0) - down[i], part = min(by, 24);
+                        down[i] += by;
+                        const uint32_t f = pow2_f16x2(-part, -part), rest = pow2_f16x2(part - by, part - by);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint32_t a = vw[2 * i][j], b = vw[2 * i + 1][j];
-                            dev::e2m1x8_to_f16((a & 0x0f0f0f0fu) | ((b << 4) & 0xf0f0f0f0u), even[i]);
-                            dev::e2m1x8_to_f16(((a >> 4) & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u), odd[i]);
+                        for (int k = 0; k < 4; ++k) pa[k >> 1][2 * (k & 1) + i] = hmul2(hmul2(pa[k >> 1][2 * (k & 1) + i], f), rest);
+                    }
+                };
+                int now_vs[8], ref = vref;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) now_vs[i] = vs[i];
+                while (true) {
+                    if (bands) {
+                        // The next 8 octaves, from the largest scale left; vs becomes 0 as it is done.
+                        const int top = largest();
+                        if (top == 0) break;
+                        ref = max(top - kValueLift, 1);
+                        uint32_t tokens = 0;  // of the step that have a block in the band
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const bool in = vs[i] > max(top - kMostLift, 0);
+                            const unsigned lanes = __ballot_sync(kFull, in);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (lanes & (0x11111111u << k)) tokens |= 1u << (2 * k + (i & 1) + 8 * (i >> 1));
+                            now_vs[i] = in ? vs[i] : ref - 64;
+                            if (in) vs[i] = 0;
                         }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            mma16816(o[8 * j + 2 * i], pa[h], hmul2(even[0][i], f0), hmul2(even[1][i], f1));
-                            mma16816(o[8 * j + 2 * i + 1], pa[h], hmul2(odd[0][i], f0), hmul2(odd[1][i], f1));
-                        }
-                    }
-                } else {
-                    constexpr int kCode = BITS == 4 ? 8 : BITS;
-#pragma unroll
-                    for (int j = 0; j < D / 32; ++j) {
-                        uint32_t four[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) four[i] = BITS == 8 ? vw[i][j] : four6(vw[i], j);
-                        // (token, token + 1) bytes of features 0, 1 and of 2, 3
-                        const uint32_t a01 = __byte_perm(four[0], four[1], 0x5140);
-                        const uint32_t a23 = __byte_perm(four[0], four[1], 0x7362);
-                        const uint32_t b01 = __byte_perm(four[2], four[3], 0x5140);
-                        const uint32_t b23 = __byte_perm(four[2], four[3], 0x7362);
-                        mma16816(o[4 * j], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a01), f0),
-                                 hmul2(dev::codes_to_f16x2<kCode>(b01), f1));
-                        mma16816(o[4 * j + 1], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a01 >> 16), f0),
-                                 hmul2(dev::codes_to_f16x2<kCode>(b01 >> 16), f1));
-                        mma16816(o[4 * j + 2], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a23), f0),
-                                 hmul2(dev::codes_to_f16x2<kCode>(b23), f1));
-                        mma16816(o[4 * j + 3], pa[h], hmul2(dev::codes_to_f16x2<kCode>(a23 >> 16), f0),
-                                 hmul2(dev::codes_to_f16x2<kCode>(b23 >> 16), f1));
-                    }
-                }
-                if (nans) {
-                    for (int t = 0; t < kGranule; ++t)
                         for (int i = 0; i < 2; ++i) {
                             const int2 range = row_range[g + 8 * i];
-                            if (t0 + h * kGranule + t < range.x || t0 + h * kGranule + t >= range.y) continue;
-#pragma unroll
-                            for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const int byte = (2 * c + e) * vShare + n;
-                                    const int in_row = P::swizzled ? (((byte >> 4) ^ (t & 7)) << 4) + (byte & 15) : byte;
-                                    if ((lds_u8<0>(ring + at + S::v_at + t * P::v + in_row) & 0x7f) == 0x7f)
-                                        o[n][2 * i + e] = __int_as_float(0x7fc00000);
-                                }
+                            const int from = min(max(range.x - t0, 0), kPair), to = min(max(range.y - t0, 0), kPair);
+                            const uint32_t seen = to > from ? (0xffffffffu >> (32 - (to - from))) << from : 0u;
+                            if ((tokens & seen) && row_ref[i] < ref) raise_row(i, ref);
                         }
+                    }
+                    lower_weights(ref);
+                    add_values(now_vs, ref);
+                    if (!bands) break;
                 }
             }
         }
@@ -676,10 +811,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         }
         __syncthreads();  // the rings are done with as well
         float* joined = reinterpret_cast<float*>(smem);
-        const float vfactor = vref ? __uint_as_float((uint32_t)vref << 23) : 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = g + 8 * i;
+            const float vfactor = __uint_as_float((uint32_t)row_ref[i] << 23);
             float top = stat_max[0][r];
 #pragma unroll
             for (int k = 1; k < kWarps; ++k) top = fmaxf(top, stat_max[k][r]);
@@ -803,6 +938,7 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     p.v_values = static_cast<const uint8_t*>(cache->v_values);
     p.k_scales = cache->k_scales;
     p.v_scales = cache->v_scales;
+    p.bits = cache->bits;
     p.kv_heads = cache->kv_heads;
     p.page_size = cache->page_size;
     p.pages = (int)cache->pages;

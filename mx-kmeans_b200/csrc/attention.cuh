@@ -26,7 +26,7 @@ struct AttentionParams {
     const uint8_t* v_values;
     const uint8_t* k_scales;
     const uint8_t* v_scales;
-    int kv_heads, page_size, pages;
+    int bits, kv_heads, page_size, pages;
     // queries and outputs
     const void* q;
     void* out;
@@ -93,6 +93,10 @@ __device__ __forceinline__ float ex2(float x) {
 // before their reference moves.
 constexpr int kKeyLift = 6;
 constexpr int kValueLift = 4, kValueMax = 6;
+constexpr int kScaleOfZeros = 127;  // scale byte of a block of zeros, as written
+// Octaves that a token which a row does not see may lift the row's reference above what it
+// sees, when more tokens follow: its f16 weights then still reach down to 2^-24 of the largest.
+constexpr int kMostLift = 8;
 // Octaves by which a block's scale may lie below what its f16 factors are relative to, so
 // that every element stays a multiple of f16's smallest, 2^-24 (elements are multiples of
 // 2^-9, 2^-3 and 2^-1).

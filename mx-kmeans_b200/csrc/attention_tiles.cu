@@ -38,9 +38,13 @@
 // each of its tokens has its own reference, and the softmax takes a slower path, so one
 // token's magnitude does not touch another's score.  Values are
 // held relative to a reference of their tile, a multiple of kRefStep octaves at or
-// above its largest scale; the output rows are kept relative to the largest
-// reference so far, and a tile with a smaller one has its weights scaled down by the
-// difference, so a row is rescaled only when the reference goes up or its maximum does.
+// above its largest scale; an output row is kept relative to the largest reference of the
+// tiles that the row saw something of, and a tile with a smaller one has its weights
+// scaled down by the difference, so a row is rescaled only when the reference goes up or
+// its maximum does.  A tile of which the rows see different tokens and whose value scales
+// are too far apart for one reference is multiplied by hand (exact_values), in float32,
+// relative to what each row sees.  Blocks of zeros, whose scale byte stands for 1, are
+// left out where they would set a reference.
 #include <limits>
 #include <type_traits>
 
@@ -54,7 +58,11 @@ using dev::kExactDown;
 using dev::kExpShift;
 using dev::kKeyLift;
 using dev::kMaxSlack;
+using dev::kMostLift;
 using dev::kQueryExp;
+using dev::kScaleOfZeros;
+using dev::kValueLift;
+using dev::kValueMax;
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kTileRows = 128;           // M of one product
@@ -62,7 +70,8 @@ constexpr int kKeys = 128;               // tokens of a key tile
 constexpr int kHalf = kKeys / 2;         // tokens of one step of the softmax
 constexpr int kStages = 2;               // of keys and of values
 constexpr int kMeta = 4;                 // key tiles whose references are kept (converter warps)
-constexpr int kWide = 1 << 17;           // in place of a tile's key reference: every token has its own
+constexpr int kWide = 1 << 17;           // in place of a tile's key reference: every token has its own;
+                                         // beside its value reference: rows that see part of it work by hand
 constexpr int kWideRef = 200;            // what scales relative to a token's own reference are added to
 constexpr int kRefStep = 4;              // value references are multiples of this many octaves
 constexpr int kMostDown = 64;            // octaves that a float32 weight may be scaled down by
@@ -128,6 +137,7 @@ struct Shared {
     int2 meta[kMeta];          // converter warps: the key tile's references
     uint8_t key_refs[kMeta][kKeys];  // those of its tokens, in wide tiles
     float row_factor[2][kTileRows];
+    int kept[2];               // the output row tile holds values by hand before the unit's first product
     int nan_unit[4];           // converter warps: unit in which a NaN was taken out of a partly seen tile
     int abort_word;
     uint32_t tmem;
@@ -384,6 +394,26 @@ struct Converter {
         // top - ref in (kKeyLift - kRefStep, kKeyLift]
         return max(((top_scale(s) - kKeyLift + kRefStep - 1) >> 2) << 2, 1);
     }
+    // Whether the scales of a tile of values ask for spread_values: too far apart to be exact
+    // relative to one reference or, if some rows see the tile's end but not its beginning
+    // (leading) and go on to others, for those rows' references; or perhaps all zeros.
+    static __device__ __forceinline__ bool wide_values(const uint32_t (&s)[4], bool leading) {
+        const int top = top_scale(s), low = low_scale(s);
+        return too_far(top, low, leading) || (top == kScaleOfZeros && low == kScaleOfZeros);
+    }
+    // (top - value_ref is at least kKeyLift - kRefStep + 1.)
+    static __device__ __forceinline__ bool too_far(int top, int low, bool leading) {
+        return top - low > (leading ? kMostLift : kKeyLift - kRefStep + 1 + kExactDown<BITS>);
+    }
+    // Rare: leaves out zero blocks and returns the tile's reference, with kWide if that was not
+    // enough and the rows see different parts of the tile.
+    static __device__ __forceinline__ int spread_values(const uint8_t* values, uint32_t place, Span sp,
+                                                        uint32_t (&s)[4], bool leading, bool trailing) {
+        const uint4 m = magnitude_scales<D, BITS>(values, place, sp.from, sp.to, make_uint4(s[0], s[1], s[2], s[3]));
+        s[0] = m.x, s[1] = m.y, s[2] = m.z, s[3] = m.w;
+        const bool by_hand = (leading || trailing) && too_far(top_scale(s), low_scale(s), leading);
+        return value_ref(s) | (by_hand ? kWide : 0);
+    }
     // f16 relative to the scale byte `ref` into a SWIZZLE_128B tile image.
     __device__ __forceinline__ void store(const Words& x, const uint32_t (&s)[4], int ref, uint8_t* tile) const {
 #pragma unroll
@@ -451,8 +481,15 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
     int ref = keys ? C::key_ref(s) : C::value_ref(s);
     if (keys && C::wide_keys(s, ref))
         ref = C::spread_keys(p.k_values, place, sp, s, p.ready_key_refs + (int64_t)blockIdx.x * kKeys, threadIdx.x < 32);
+    if (!keys) {
+        int last_lo, first_hi, other;
+        dev::seen_range(p, view, view.n - 1, view.n - 1, last_lo, other);
+        dev::seen_range(p, view, 0, 0, other, first_hi);
+        const bool leading = max(t0, lo) < last_lo, trailing = min(t0 + kKeys, hi) > first_hi;
+        if (C::wide_values(s, leading)) ref = C::spread_values(p.v_values, place, sp, s, leading, trailing);
+    }
     const int nans = keys ? 0 : C::take_out_nans(x);
-    cv.store(x, s, keys ? C::key_base(ref) : ref, image);
+    cv.store(x, s, keys ? C::key_base(ref) : ref & 0xffff, image);
     dev::fence_proxy_async();
     const int any_nans = __syncthreads_or(nans);
     if (threadIdx.x == 0) {
@@ -506,9 +543,9 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
     do {
         const Whole whole = whole_tiles(p, c);
         for (int t = 0; t < c.tiles; ++t) {
-            int kref = C::key_ref(ks);
-            const int vref = C::value_ref(vs);
-            const bool wide = C::wide_keys(ks, kref);
+            int kref = C::key_ref(ks), vref = C::value_ref(vs);
+            const bool wide = C::wide_keys(ks, kref), leading = t < whole.from, trailing = t >= whole.to;
+            if (C::wide_values(vs, leading)) vref = C::spread_values(p.v_values, row, sp, vs, leading, trailing);
             uint32_t vs_now[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) vs_now[i] = vs[i];
@@ -533,7 +570,7 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
             if (t < whole.from || t >= whole.to)
                 if (C::take_out_nans(vx)) *reinterpret_cast<volatile int*>(&b.sh->nan_unit[c.unit & 3]) = c.unit;
             if (!b.wait(&b.sh->v_empty[stage], phase)) return false;
-            cv.store(vx, vs_now, vref, b.smem + L::v + stage * L::tile);
+            cv.store(vx, vs_now, vref & 0xffff, b.smem + L::v + stage * L::tile);
             dev::fence_proxy_async();
             b.arrive(&b.sh->v_full[stage]);
             if (sp.to >= 0) cv.load(row, sp, p.v_values, vx);
@@ -655,12 +692,14 @@ __device__ __forceinline__ void product_role(const AttentionParams& p, const Blo
                     if (!ok) continue;
                     if (half == 1) p_phase[w] ^= 1;
                     dev::tc_fence_after();
+                    // the first product of a unit begins the output, unless that holds something
+                    const bool more = t > 0 || half > 0 || *reinterpret_cast<volatile int*>(&sh->kept[w]);
                     const uint64_t vd = v_desc + (uint64_t)(v_stage * (L::tile >> 4) + half * (kHalf * 128 >> 4));
                     if (dev::elect_one()) {
 #pragma unroll
                         for (int i = 0; i < kHalf / 16; ++i)
                             dev::tc_mma_f16_ta(b.tmem + kTiles * kKeys + w * D, b.tmem + w * kKeys + half * kHalf + 8 * i,
-                                               vd + i * (2048 >> 4), idesc_o, i > 0 || half > 0 || t > 0);
+                                               vd + i * (2048 >> 4), idesc_o, i > 0 || more);
                         dev::tc_commit(&sh->o_done[w][half]);
                         if (half == 1 && w == nw - 1) dev::tc_commit(&sh->v_empty[v_stage]);
                     }
@@ -771,23 +810,7 @@ __device__ __noinline__ float masked_top(uint32_t s_col, int from, int to) {
     return m;
 }
 
-// The same for a wide tile, with each token's reference: in the scores' true units.
-__device__ __noinline__ float wide_top(uint32_t s_col, int from, int to, float row_factor, const uint8_t* refs) {
-    float m = __int_as_float(0xff800000);
-#pragma unroll 1
-    for (int h = 0; h < kHalf / 32; ++h) {
-        uint32_t s[32];
-        dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
-        dev::tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (32 * h + i >= from && 32 * h + i < to)
-                m = fmaxf(m, __uint_as_float(s[i]) * (row_factor * __uint_as_float((uint32_t)refs[32 * h + i] << 23)));
-    }
-    return m;
-}
-
-// Weights of the row's columns, the f16 ones times `down`; returns their sum.
+// Its weights, the f16 ones times `down`; returns their sum.
 __device__ __noinline__ float masked_weights(uint32_t s_col, int from, int to, float f, float base, float down) {
     float sum = 0.0f;
 #pragma unroll 1
@@ -808,6 +831,23 @@ __device__ __noinline__ float masked_weights(uint32_t s_col, int from, int to, f
     }
     dev::tmem_wait_st();
     return sum;
+}
+
+// The score of column i in log2 units: f, or f and the token's own reference, times s.
+__device__ __forceinline__ float own_score(const uint8_t* refs, int i, float s, float f) {
+    return s * (refs ? f * __uint_as_float((uint32_t)refs[i] << 23) : f);
+}
+
+// The same as masked_top for a tile whose keys have a reference each, in log2 units.
+__device__ __noinline__ float wide_top(uint32_t s_col, int from, int to, float f, const uint8_t* refs) {
+    float m = __int_as_float(0xff800000);
+#pragma unroll 1
+    for (int i = 0; i < kHalf; ++i) {
+        const float s = __uint_as_float(dev::tmem_ld_32x32b_x1(s_col + i));
+        dev::tmem_wait_ld();
+        if (i >= from && i < to) m = fmaxf(m, own_score(refs, i, s, f));
+    }
+    return m;
 }
 
 // Features of a value row that are NaN (8-bit elements) among the tokens [k0, k1) that
@@ -946,32 +986,164 @@ __device__ __forceinline__ void put_rows(const AttentionParams& p, const float4*
     }
 }
 
-// The same for a wide tile.
-__device__ __noinline__ float wide_weights(uint32_t s_col, int from, int to, float row_factor, const uint8_t* refs,
-                                           float base, float down) {
-    float sum = 0.0f;
-#pragma unroll 1
-    for (int h = 0; h < kHalf / 32; ++h) {
-        uint32_t s[32], pw[16];
-        dev::tmem_ld_32x32b_x32(s_col + 32 * h, s);
-        dev::tmem_wait_ld();
+// 32 packed elements as float32.
+template <int BITS>
+__device__ __forceinline__ void block_values(const uint32_t* w, float (&v)[32]) {
+    uint32_t h2[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (BITS == 4) {
+            uint32_t x[4];
+            dev::e2m1x8_to_f16(w[j], x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h2[4 * j + i] = x[i];
+        } else {
+            constexpr int kCode = BITS == 4 ? 8 : BITS;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t four = BITS == 8 ? w[2 * j + i] : dev::four6(w, 2 * j + i);
+                h2[4 * j + 2 * i] = dev::codes_to_f16x2<kCode>(four);
+                h2[4 * j + 2 * i + 1] = dev::codes_to_f16x2<kCode>(four >> 16);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h2[j]));
+        v[2 * j] = f.x, v[2 * j + 1] = f.y;
+    }
+}
+
+// The values of a sequence and key head.
+struct ValueRows {
+    const AttentionParams& p;
+    const int* table;
+    int head;
+    __device__ __forceinline__ int64_t row(int token) const {
+        const int at = token / p.page_size;
+        const int page = min(max(__ldg(table + at), 0), p.pages - 1);
+        return ((int64_t)page * p.kv_heads + head) * p.page_size + (token - at * p.page_size);
+    }
+    // Block b of `blocks` of a row; false: all zeros.
+    __device__ __forceinline__ bool block(int64_t row, int blocks, int b, float (&v)[32]) const {
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(p.v_values) + (row * blocks + b) * p.bits;
+        uint32_t w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = k < p.bits ? __ldg(at + k) : 0;
+        if (p.bits == 8)
+            block_values<8>(w, v);
+        else if (p.bits == 6)
+            block_values<6>(w, v);
+        else
+            block_values<4>(w, v);
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) any |= v[i] != 0.0f;
+        return any;
+    }
+};
+
+// 2^(to - from), of scale bytes, up to 2^127 and down to where it is 0.
+__device__ __forceinline__ float octaves(int to, int from) {
+    return __uint_as_float((uint32_t)min(max(to - from + 127, 0), 254) << 23);
+}
+
+// The weights of a half key tile's columns [from, to) where its keys have a reference each
+// (refs), or its values are worked through by hand (o_col).  Returns their sum and the
+// row's reference of the values.
+//
+// The weights are left for the product with the values in f16, relative to base and
+// lowered from vrun to vref.  By hand, because the tile's value scales are too far apart to be
+// held relative to one reference for rows that see different tokens, the weighted values are
+// added to the row's output in TMEM in float32 and the weights left for the product are zero.
+// The output is relative to 2^(vrun - 127) with a factor g yet to come, or holds nothing
+// yet (g = 0); vrun goes up where the row sees a token that asks for it.
+struct WideHalf {
+    uint32_t s_col, o_col;  // scores; output, or 0: weights only
+    int t0;                 // its first token
+    int seq, head;          // of the unit
+    const uint8_t* refs;    // or none: f then holds the tile's
+};
+struct WideSum {
+    float sum;
+    int vrun;
+};
+template <int D>
+__device__ __noinline__ WideSum wide_weights(const AttentionParams& p, WideHalf half, int from, int to, float f,
+                                             float base, int vref, int vrun_at, float g) {
+    constexpr int kBlocks = D / 32;
+    const uint32_t o_col = half.o_col;
+    float sum = 0.0f;
+    if (!o_col) {
+        // (a row that sees nothing of the tile may be below its reference)
+        const float lower = octaves(vref, max(vrun_at, vref));
+#pragma unroll 1
+        for (int i = 0; i < kHalf / 2; ++i) {
             float w[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int t = 32 * h + i + k;
-                const float x = __uint_as_float(s[i + k]) * (row_factor * __uint_as_float((uint32_t)refs[t] << 23));
-                w[k] = t >= from && t < to ? ex2(x - base) : 0.0f;
+                const int t = 2 * i + k;
+                const float s = __uint_as_float(dev::tmem_ld_32x32b_x1(half.s_col + t));
+                dev::tmem_wait_ld();
+                w[k] = t >= from && t < to ? ex2(own_score(half.refs, t, s, f) - base) : 0.0f;
             }
             sum += w[0] + w[1];
-            const __half2 u = __floats2half2_rn(w[0] * down, w[1] * down);
-            pw[i / 2] = *reinterpret_cast<const uint32_t*>(&u);
+            const __half2 u = __floats2half2_rn(w[0] * lower, w[1] * lower);
+            __syncwarp();
+            dev::tmem_st_32x32b_x1(half.s_col + i, *reinterpret_cast<const uint32_t*>(&u));
         }
-        dev::tmem_st_32x32b_x16(s_col + 16 * h, pw);
+        dev::tmem_wait_st();
+        return WideSum{sum, vrun_at};
     }
+    const ValueRows rows{p, p.page_table + (int64_t)half.seq * p.table_stride, half.head};
+    // (The warp goes through all 64 tokens together; those that no lane sees are not touched.)
+    int top = 0, vrun = vrun_at;
+#pragma unroll 1
+    for (int t = 0; t < kHalf; ++t) {
+        const bool sees = t >= from && t < to;
+        if (!__any_sync(kFull, sees)) continue;
+        const int64_t row = rows.row(half.t0 + t);
+#pragma unroll 1
+        for (int b = 0; b < kBlocks; ++b) {
+            float v[32];
+            if (rows.block(row, kBlocks, b, v) && sees) top = max(top, (int)__ldg(p.v_scales + row * kBlocks + b));
+        }
+    }
+    if (top > 0 && (vrun == 0 || top > vrun + kValueMax)) vrun = max(top - kValueLift, 1);
+    g *= octaves(vrun_at, vrun);
+#pragma unroll 1
+    for (int b = 0; b < kBlocks; ++b) {
+        uint32_t o[32];
+        dev::tmem_ld_32x32b_x32(o_col + 32 * b, o);
+        dev::tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = g == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[i]) * g);
+#pragma unroll 1
+        for (int t = 0; t < kHalf; ++t) {
+            const bool sees = t >= from && t < to;
+            if (!__any_sync(kFull, sees)) continue;
+            const float s = __uint_as_float(dev::tmem_ld_32x32b_x1(half.s_col + t));
+            dev::tmem_wait_ld();
+            const float weight = sees ? ex2(own_score(half.refs, t, s, f) - base) : 0.0f;
+            if (b == 0) sum += weight;
+            const int64_t row = rows.row(half.t0 + t);
+            float v[32];
+            rows.block(row, kBlocks, b, v);
+            const float factor = weight * octaves(__ldg(p.v_scales + row * kBlocks + b), vrun);
+            if (sees) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(factor, v[i], __uint_as_float(o[i])));
+            }
+        }
+        __syncwarp();
+        dev::tmem_st_32x32b_x32(o_col + 32 * b, o);
+    }
+    uint32_t none[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) none[i] = 0;
+    dev::tmem_st_32x32b_x32(half.s_col, none);
     dev::tmem_wait_st();
-    return sum;
+    return WideSum{sum, vrun};
 }
 
 // READY: tiles were converted beforehand, their references lie in global memory.
@@ -1018,7 +1190,8 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             b.arrive(&sh->q_ready[w]);
 
             float run_max = neg_inf, base = -kExpShift, sum = 0.0f;
-            int vrun = 0;  // the output is held relative to 2^(vrun - 127)
+            int vrun = 0;  // the output row is held relative to 2^(vrun - 127); 0: it saw nothing yet
+            int vleast = 0, vmost = 0;  // the warp's smallest and largest
             bool nans = false;
             const int2* meta = nullptr;
             int2 ref = make_int2(0, 0);
@@ -1030,78 +1203,99 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
             uint32_t s[2][32];
             if (!b.wait(&sh->s_full[w][0], s_phase)) return false;
             dev::tc_fence_after();
-            if (warp_real) {
+            const int halves = 2 * c.tiles;
+            // The half t's weights are in place; the next half's scores are waited for unless
+            // fetched has been done already.
+            auto pass_on = [&](int t, bool fetched) -> bool {
+                dev::tc_fence_before();
+                b.arrive(&sh->p_ready[w][t & 1]);
+                if (t & 1)
+                    o_phase[1] ^= 1;
+                else
+                    o_phase[0] ^= 1;
+                if (t + 1 < halves && !fetched) {
+                    if (!b.wait(&sh->s_full[w][~t & 1], s_phase ^ (t & 1))) return false;
+                    dev::tc_fence_after();
+                    if (warp_real) {
+                        dev::tmem_ld_32x32b_x32(s_col + (~t & 1) * kHalf, s[0]);
+                        dev::tmem_ld_32x32b_x32(s_col + (~t & 1) * kHalf + 32, s[1]);
+                    }
+                }
+                if (t & 1) s_phase ^= 1;
+                return true;
+            };
+            if (!warp_real) {
+                for (int t = 0; t < halves; ++t)
+                    if (!pass_on(t, false)) return false;
+            } else {
                 dev::tmem_ld_32x32b_x32(s_col, s[0]);
                 dev::tmem_ld_32x32b_x32(s_col + 32, s[1]);
-            }
-            const int halves = 2 * c.tiles;
-            const float row_factor = *const_cast<volatile float*>(&sh->row_factor[w][r]);
-            for (int t = 0; t < halves; ++t) {
-                const uint32_t s_at = s_col + (t & 1) * kHalf, s_next = s_col + (~t & 1) * kHalf;
-                const uint32_t next_phase = s_phase ^ (t & 1);
-                bool fetched = false;
-                if (!READY && !(t & 1)) ref = *const_cast<const int2*>(&sh->meta[(meta_at + t / 2) % kMeta]);
-                if (warp_real) {
-                    const float f = row_factor * __uint_as_float((uint32_t)ref.x << 23);
-                    const bool wide = ref.x == kWide;
-                    const uint8_t* key_refs = nullptr;  // of this half, in wide tiles
-                    if (wide)
-                        key_refs = (READY ? p.ready_key_refs + (ready_at(p, c) + t / 2) * kKeys
-                                          : sh->key_refs[(meta_at + t / 2) % kMeta]) + (t & 1) * kHalf;
-                    const int vref = ref.y & 0xffff;
-                    if (READY && (t & 1)) {
-                        nans |= ref.y >> 16;
-                        if (t + 1 < halves) ref = meta[t / 2 + 1];
-                    }
-                    if (t == 0) vrun = vref;
-                    const bool rare = t < 2 * whole.from || t >= 2 * whole.to || vrun - vref > kMostDown || wide;
-                    int from = 0, to = kHalf;
-                    float top;
-                    dev::tmem_wait_ld();
-                    if (rare) {
-                        const int t0 = first_key + t * kHalf;
-                        from = min(max(lo - t0, 0), kHalf);
-                        to = min(max(hi - t0, 0), kHalf);
-                        top = wide ? wide_top(s_at, from, to, row_factor, key_refs) : masked_top(s_at, from, to);
-                    } else {
+                const float row_factor = *const_cast<volatile float*>(&sh->row_factor[w][r]);
+                // The references of half t's tile, from where they lie to `ref`.
+                auto fetch_ref = [&](int t) {
+                    if (READY)
+                        ref = meta[t / 2];
+                    else
+                        ref = *const_cast<const int2*>(&sh->meta[(meta_at + t / 2) % kMeta]);
+                };
+                if (!READY) fetch_ref(0);
+                // Halves that are out of the ordinary leave the loop below.
+                auto partly = [&](int t) -> bool { return t < 2 * whole.from || t >= 2 * whole.to; };
+                auto rare = [&](int t) -> bool {
+                    return partly(t) || ref.x == kWide || vmost - (ref.y & 0xffff) > kMostDown;
+                };
+                // Waits for the products before half t, which have added to the output.
+                auto output_so_far = [&](int t) -> bool {
+                    if (!b.wait(&sh->o_done[w][(t - 1) & 1], (t & 1 ? o_phase[0] : o_phase[1]) ^ 1)) return false;
+                    dev::tc_fence_after();
+                    return true;
+                };
+                // Before this warp lets the unit's first product with the values start.
+                if ((threadIdx.x & 31) == 0)
+                    *reinterpret_cast<volatile int*>(&sh->kept[w]) = partly(0) && (ref.y & kWide) ? 1 : 0;
+                for (int t = 0; t < halves;) {
+                    while (t < halves && !rare(t)) {
+                        const uint32_t s_at = s_col + (t & 1) * kHalf, s_next = s_col + (~t & 1) * kHalf;
+                        const float f = row_factor * __uint_as_float((uint32_t)ref.x << 23);
+                        const int vref = ref.y & 0xffff;
+                        if (READY && (t & 1)) {
+                            nans |= ref.y >> 16 & 1;
+                            if (t + 1 < halves) fetch_ref(t + 1);
+                        }
                         float m[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
+                        dev::tmem_wait_ld();
                         fold_top(s[0], m);
                         fold_top(s[1], m);
-                        top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                    }
-                    if (top != neg_inf && !wide) top *= f;
+                        float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                        if (top != neg_inf) top *= f;
 
-                    // Raise the row's maximum, or the reference of the output, if need be.
-                    const bool raise = top > run_max + kMaxSlack;
-                    if (__any_sync(kFull, raise) || vref > vrun) {
-                        const float m = raise ? top : run_max;
-                        float g = m == run_max ? 1.0f : ex2(run_max - m);
-                        run_max = m;
-                        base = (m == neg_inf ? 0.0f : m) - kExpShift;
-                        sum *= g;
-                        if (vref > vrun) g *= __uint_as_float((uint32_t)max(vrun - vref + 127, 0) << 23);
-                        vrun = max(vrun, vref);
-                        if (t > 0) {  // the output so far, once the products before have finished
-                            if (!b.wait(&sh->o_done[w][(t - 1) & 1], (t & 1 ? o_phase[0] : o_phase[1]) ^ 1)) return false;
-                            dev::tc_fence_after();
-                            scale_output<D>(o_col, g);
+                        // Raise the row's maximum, or the reference of the output, if need be.
+                        const bool raise = top > run_max + kMaxSlack;
+                        if (__any_sync(kFull, raise) || vref > vleast) {
+                            const float x = raise ? top : run_max;
+                            float g = x == run_max ? 1.0f : ex2(run_max - x);
+                            run_max = x;
+                            base = (x == neg_inf ? 0.0f : x) - kExpShift;
+                            sum *= g;
+                            if (vref > vrun) g *= octaves(vrun, vref), vrun = vref;
+                            vleast = (int)__reduce_min_sync(kFull, (unsigned)vrun);
+                            vmost = max(vmost, vref);
+                            if (t > 0) {
+                                if (!output_so_far(t)) return false;
+                                scale_output<D>(o_col, g);
+                            }
                         }
-                    }
-                    // The weights, over the scores they come from, scaled by 2^(vref - vrun): up to
-                    // kMostDown octaves in their exponents, which float32 sums do not notice.
-                    const int down = min(vrun - vref, kMostDown);
-                    const float shifted = base + (float)down, up = __uint_as_float((uint32_t)(127 + down) << 23);
-                    if (rare) {
-                        const float rest = __uint_as_float((uint32_t)max(vref - vrun + down + 127, 0) << 23);
-                        sum += up * (wide ? wide_weights(s_at, from, to, row_factor, key_refs, shifted, rest)
-                                          : masked_weights(s_at, from, to, f, shifted, rest));
-                    } else {
+                        // The weights, over the scores they come from, scaled by 2^(vref - vrun):
+                        // up to kMostDown octaves in their exponents, which float32 sums do not notice.
+                        const int down = vrun - vref;
+                        const float shifted = base + (float)down, back = __uint_as_float((uint32_t)(127 + down) << 23);
                         float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                         uint32_t pw[16];
                         fold_weights(s[0], f, shifted, part, pw);
                         dev::tmem_st_32x32b_x16(s_at, pw);
+                        bool fetched = false;
                         if (t + 1 < halves) {
-                            fetched = __all_sync(kFull, dev::mbar_test(&sh->s_full[w][~t & 1], next_phase));
+                            fetched = __all_sync(kFull, dev::mbar_test(&sh->s_full[w][~t & 1], s_phase ^ (t & 1)));
                             if (fetched) {
                                 dev::tc_fence_after();
                                 dev::tmem_ld_32x32b_x32(s_next, s[0]);
@@ -1111,24 +1305,58 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                         dev::tmem_st_32x32b_x16(s_at + 16, pw);
                         if (fetched) dev::tmem_ld_32x32b_x32(s_next + 32, s[1]);
                         dev::tmem_wait_st();
-                        sum += up * ((part[0].x + part[0].y) + (part[1].x + part[1].y));
+                        sum += back * ((part[0].x + part[0].y) + (part[1].x + part[1].y));
+                        if (!pass_on(t, fetched)) return false;
+                        ++t;
+                        if (!READY && !(t & 1) && t < halves) fetch_ref(t);
                     }
-                }
-                dev::tc_fence_before();
-                b.arrive(&sh->p_ready[w][t & 1]);
-                if (t & 1)
-                    o_phase[1] ^= 1;
-                else
-                    o_phase[0] ^= 1;
-                if (t + 1 < halves && !fetched) {
-                    if (!b.wait(&sh->s_full[w][~t & 1], next_phase)) return false;
-                    dev::tc_fence_after();
-                    if (warp_real) {
-                        dev::tmem_ld_32x32b_x32(s_next, s[0]);
-                        dev::tmem_ld_32x32b_x32(s_next + 32, s[1]);
+                    if (t == halves) break;
+                    // A half that the rows see different parts of, whose keys have a reference
+                    // each, or whose values lie far below those before.
+                    dev::tmem_wait_ld();
+                    const int t0 = first_key + t * kHalf, vref = ref.y & 0xffff;
+                    const bool by_hand = partly(t) && (ref.y & kWide);
+                    const int from = min(max(lo - t0, 0), kHalf), to = min(max(hi - t0, 0), kHalf);
+                    WideHalf half{s_col + (t & 1) * kHalf, by_hand ? o_col : 0, t0, c.w.seq, c.w.head, nullptr};
+                    float f = row_factor, top;
+                    if (ref.x == kWide) {
+                        half.refs = (READY ? p.ready_key_refs + (meta + t / 2 - p.ready_meta) * kKeys
+                                           : sh->key_refs[(meta_at + t / 2) % kMeta]) + (t & 1) * kHalf;
+                        top = wide_top(half.s_col, from, to, f, half.refs);
+                    } else {
+                        f *= __uint_as_float((uint32_t)ref.x << 23);
+                        top = masked_top(half.s_col, from, to);
+                        if (top != neg_inf) top *= f;
                     }
+                    if (READY && (t & 1)) nans |= ref.y >> 16 & 1;
+                    const bool raise = top > run_max + kMaxSlack;
+                    const bool up = vref > vrun && to > from && !by_hand;  // only rows that see something of it
+                    float g = 1.0f;
+                    if (__any_sync(kFull, raise || up) || by_hand) {
+                        const float x = raise ? top : run_max;
+                        g = x == run_max ? 1.0f : ex2(run_max - x);
+                        run_max = x;
+                        base = (x == neg_inf ? 0.0f : x) - kExpShift;
+                        sum *= g;
+                        if (up) g *= octaves(vrun, vref), vrun = vref;
+                        if (t > 0) {
+                            if (!output_so_far(t)) return false;
+                            if (!by_hand) scale_output<D>(o_col, g);
+                        }
+                    }
+                    if (by_hand || half.refs) {
+                        const WideSum ws = wide_weights<D>(p, half, from, to, f, base, vref, vrun, t > 0 ? g : 0.0f);
+                        sum += ws.sum, vrun = ws.vrun;
+                    } else {
+                        // (a row that sees nothing of the tile may be below its reference)
+                        sum += masked_weights(half.s_col, from, to, f, base, octaves(vref, max(vrun, vref)));
+                    }
+                    vleast = (int)__reduce_min_sync(kFull, (unsigned)vrun);
+                    vmost = (int)__reduce_max_sync(kFull, (unsigned)vrun);
+                    if (!pass_on(t, false)) return false;
+                    ++t;
+                    if (!(t & 1) && t < halves) fetch_ref(t);
                 }
-                if (t & 1) s_phase ^= 1;
             }
 
             // The output row.
@@ -1279,7 +1507,8 @@ __device__ __forceinline__ void finish(const AttentionParams& p, const Block& b)
 }
 
 template <int D, int BITS>
-__global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(const AttentionParams p, unsigned* err) {
+__global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(const __grid_constant__ AttentionParams p,
+                                                                                unsigned* err) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared shared;
     __shared__ int scratch[Packed::threads / 16 + 2];
@@ -1300,7 +1529,8 @@ __global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(con
 }
 
 template <int D>
-__global__ void __launch_bounds__(Ready::threads, 1) attention_ready_kernel(const AttentionParams p, unsigned* err) {
+__global__ void __launch_bounds__(Ready::threads, 1) attention_ready_kernel(const __grid_constant__ AttentionParams p,
+                                                                               unsigned* err) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared shared;
     __shared__ int scratch[Ready::threads / 16 + 2];

@@ -18,20 +18,22 @@ from test_cache_attention_gpu import attend, build, cached_rows, check
 pytestmark = pytest.mark.gpu
 
 
-def check_rows(torch, b, out, lse, rows=None, causal=True, window=0, scale=None):
-    """Rows `rows` (query tokens of the one sequence; None: all) against the definition."""
+def check_rows(torch, b, out, lse, rows=None, causal=True, window=0, scale=None, seq=0):
+    """Query tokens `rows` of a sequence (None: all) against the definition."""
     c = b["cache"]
-    n, l, heads = b["q_lens"][0], b["kv_lens"][0], b["q"].shape[1]
+    n, l, heads = b["q_lens"][seq], b["kv_lens"][seq], b["q"].shape[1]
+    first = sum(b["q_lens"][:seq])
+    out, lse, queries = out[first:first + n], lse[first:first + n], b["q"][first:first + n]
     scale = c.head_dim ** -0.5 if scale is None else scale
     u, tiny = (2.0 ** -8, 0.0) if out.dtype == torch.bfloat16 else (2.0 ** -11, 2.0 ** -25)
-    k, v = cached_rows(torch, b, 0)
+    k, v = cached_rows(torch, b, seq)
     rows = torch.arange(n, device="cuda") if rows is None else rows
     p, t = l - n + rows, torch.arange(l, device="cuda")
     see = t[None] <= p[:, None] if causal else torch.ones(len(rows), l, dtype=torch.bool, device="cuda")
     if window:
         see &= t[None] > p[:, None] - window
     for h in range(heads):
-        q = b["q"][rows, h].double()
+        q = queries[rows, h].double()
         kh, vh = k[:, h * c.kv_heads // heads], v[:, h * c.kv_heads // heads]
         # nothing that is not seen enters the sums, infinite or not
         s = torch.where(see, scale * (q @ torch.where(see.any(0)[:, None], kh, 0.0).T), -math.inf)
@@ -164,3 +166,114 @@ def test_blocks_of_zeros_beside_small_keys(torch_cuda, mxk, bits, dim, n, l):
     b = filled(torch, mxk, g, n, l, dim, bits, change)
     out, lse = attend(torch, mxk, b, scale=2.0 ** 38)
     check_rows(torch, b, out, lse, scale=2.0 ** 38)
+
+
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("n,l", SIZES + [(6, 6), (100, 100), (300, 300)])
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 30, 2.0 ** 60, math.inf])
+def test_a_later_value_of_any_size(torch_cuda, mxk, bits, dim, n, l, size):
+    """The value of a token in the middle of the chunk is huge or has overflowed: the rows
+    before it get their own values, those after it its part of it."""
+    torch, g = torch_cuda, np.random.default_rng(27)
+    at = l - n + n // 2
+
+    def change(k, v):
+        v[at, :, 7] = size
+    b = filled(torch, mxk, g, n, l, dim, bits, change)
+    out, lse = attend(torch, mxk, b)
+    check_rows(torch, b, out, lse, torch.arange(n // 2 if size == math.inf else n, device="cuda"))
+
+
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("n,l", SIZES)
+@pytest.mark.parametrize("size", [2.0 ** 9, 2.0 ** 20, 2.0 ** 70])
+def test_earlier_values_outside_the_window(torch_cuda, mxk, bits, dim, n, l, size):
+    """Huge values of several sizes that only the first rows' windows hold, one by one and
+    a stretch of them."""
+    torch, g = torch_cuda, np.random.default_rng(28)
+    window = 140
+
+    def change(k, v):
+        start = l - n - window + 1
+        v[start:start + n // 2] *= size
+        v[start + n // 3] *= 2.0 ** 9
+    b = filled(torch, mxk, g, n, l, dim, bits, change)
+    out, lse = attend(torch, mxk, b, window=window)
+    check_rows(torch, b, out, lse, window=window)
+
+
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("n,l", SIZES)
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 180), (False, 0)])
+def test_blocks_of_zeros_beside_small_values(torch_cuda, mxk, bits, dim, n, l, causal, window):
+    """Values of about 2^-40 with blocks of zeros (whose scale byte stands for 1), whole
+    rows and a stretch of them."""
+    torch, g = torch_cuda, np.random.default_rng(29)
+
+    def change(k, v):
+        v *= 2.0 ** -40
+        v[:, :, 32:64] = 0
+        v[::7] = 0
+        v[l // 2 - 64:l // 2 + 100] = 0
+    b = filled(torch, mxk, g, n, l, dim, bits, change)
+    out, lse = attend(torch, mxk, b, causal=causal, window=window)
+    check_rows(torch, b, out, lse, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("n,l", SIZES + [(300, 300)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_magnitudes_all_over(torch_cuda, mxk, bits, dim, n, l, window):
+    """Keys and values whose scales go up and down by 2^60 from token to token."""
+    torch, g = torch_cuda, np.random.default_rng(30)
+
+    def change(k, v):
+        k *= np.ldexp(1.0, g.integers(-60, 1, (l, 2, 1))).astype(np.float32)
+        v *= np.ldexp(1.0, g.integers(-30, 31, (l, 2, 1))).astype(np.float32)
+    b = filled(torch, mxk, g, n, l, dim, bits, change)
+    out, lse = attend(torch, mxk, b, window=window)
+    check_rows(torch, b, out, lse, window=window)
+
+
+@pytest.mark.parametrize("n", [5, 60, 300])
+def test_nan_beside_huge_values(torch_cuda, mxk, n):
+    """A NaN among the elements of a token, in a tile that is worked through by hand: it
+    reaches the rows that see it, in its feature."""
+    torch, g = torch_cuda, np.random.default_rng(31)
+    l, at = 400, 400 - n + n // 2
+
+    def change(k, v):
+        v[at, :, 9] = 2.0 ** 50
+    b = filled(torch, mxk, g, n, l, 128, 8, change)
+    clean, lse = attend(torch, mxk, b)
+    slot = int(b["slots"][0][at])
+    b["cache"].v_values[slot // 32, 1, slot % 32, 37] = 0x7f
+    out, lse2 = attend(torch, mxk, b)
+    assert torch.equal(lse, lse2) and torch.equal(out[:, :2], clean[:, :2])
+    assert torch.equal(out[:n // 2], clean[:n // 2])
+    assert torch.isnan(out[n // 2:, 2:, 37]).all()
+    rest = torch.arange(128, device="cuda") != 37
+    assert torch.equal(out[:, 2:, rest], clean[:, 2:, rest])
+
+
+@pytest.mark.parametrize("bits,dim", FORMS)
+@pytest.mark.parametrize("sizes", [[(90, 90), (40, 333), (33, 33), (200, 460)] * 5, [(300, 300), (260, 700)] * 3],
+                         ids=["packed", "ready"])
+def test_units_one_after_the_other(torch_cuda, mxk, bits, dim, sizes):
+    """Blocks that work through several units, by hand and not, first tiles and later ones."""
+    torch, g = torch_cuda, np.random.default_rng(32)
+    cached = []
+    for i, (n, l) in enumerate(sizes):
+        k, v = (g.standard_normal((l, 2, dim)).astype(np.float32) for _ in range(2))
+        if i % 3 < 2:
+            v[l - n + n // 3, :, 3] = 2.0 ** 40
+            k[l - n + n // 4, :, 5] = 2.0 ** 30
+        cached.append((k, v))
+    q_lens, kv_lens = [n for n, _ in sizes], [l for _, l in sizes]
+    b = build(torch, mxk, g, q_lens, kv_lens, 8, 2, dim, 32, bits, "bfloat16", cached=cached)
+    out, lse = attend(torch, mxk, b)
+    for i, (n, l) in enumerate(sizes):
+        check_rows(torch, b, out, lse, torch.arange(n // 4, device="cuda") if i % 3 < 2 else None, seq=i)
+    again, lse2 = attend(torch, mxk, b)
+    same = (out == again) | (torch.isnan(out) & torch.isnan(again))
+    assert bool(same.all()), "the same call twice differs"
