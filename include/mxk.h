@@ -343,7 +343,9 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  * sequence's output is not defined (no memory outside the given buffers is
  * touched).  The page table holds max_kv / page_size pages (rounded up) per
  * sequence.  q and out: dtype MXK_F16 or MXK_BF16, `tokens` rows of `heads` heads
- * (out may not overlap q).  lse (optional): float32 [tokens][heads].
+ * (out may not overlap q).  lse (optional): float32 [tokens][heads].  With
+ * G = heads / kv_heads, (tokens * G / 128 + 2 * seqs) * kv_heads * (max_kv / 128 + 2)
+ * must be below 1.9e8, and the sequences' rows may not overlap.
  * head_dim must be 64 or 128 (others: MXK_ERR_UNSUPPORTED).
  *
  * Products are taken in f16 with float32 sums: every MX element times its scale

@@ -958,7 +958,7 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     p.page_table = a->page_table;
     p.table_stride = a->page_table_stride;
     p.max_kv = (int)a->max_kv;
-    p.max_q = a->max_q;
+    p.max_q = (int)std::min<int64_t>(a->max_q, a->tokens);
     p.kv_lens = a->kv_lens;
     p.scale_log2 = a->scale * 1.44269504088896f;
     p.causal = a->causal != 0;
@@ -970,12 +970,12 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     // tiles kernel; a single sequence has one kernel chosen by its bound, several are
     // sorted by the kernels themselves.
     AttentionCall call(as_stream(stream));
-    const int64_t rows = (int64_t)a->max_q * p.group;
+    const int64_t rows = (int64_t)p.max_q * p.group;
     const bool many = rows > kMostFewRows;
     if (many) {
         AttentionParams q = p;
         if (a->seqs > 1) q.min_rows = kMostFewRows + 1;
-        MXK_CHECK(launch_attention_tiles(cache->bits, cache->head_dim, q, a->max_q, call));
+        MXK_CHECK(launch_attention_tiles(cache->bits, cache->head_dim, q, p.max_q, call));
         p.max_rows = kMostFewRows;
     }
     if (!many || a->seqs > 1) {

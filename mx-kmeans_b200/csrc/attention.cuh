@@ -16,6 +16,8 @@
 // them in CTA order, so the result does not depend on timing.
 #pragma once
 
+#include <algorithm>
+
 #include "cache.cuh"
 
 namespace mxk {
@@ -57,13 +59,15 @@ struct AttentionParams {
 };
 
 // Key tiles there can be at most when no sequence has more than max_q query and
-// p.max_kv cached tokens: a window touches at most one tile more than it and the
-// row tile's tokens fill.
+// p.max_kv cached tokens, and all of them p.tokens query tokens: a window touches at
+// most one tile more than it and the row tile's tokens fill.  (One long sequence among
+// many short ones has few row tiles, so their number is not seqs times its own.)
 inline int64_t attention_tile_bound(const AttentionParams& p, int max_q, int rows, int keys) {
-    const int64_t row_tiles = ((int64_t)max_q * p.group + rows - 1) / rows;
+    const int64_t one = ((int64_t)max_q * p.group + rows - 1) / rows;
+    const int64_t row_tiles = std::min<int64_t>(p.seqs * one, p.tokens * p.group / rows + std::min<int64_t>(p.seqs, p.tokens));
     int64_t span = p.max_kv;  // below 2^30, as the window
     if (p.window > 0 && p.window + rows < span) span = p.window + rows;
-    return (int64_t)p.seqs * p.kv_heads * row_tiles * (span / keys + 2);
+    return p.kv_heads * row_tiles * (span / keys + 2);
 }
 
 namespace dev {
@@ -201,7 +205,9 @@ struct Share {
 };
 
 // All threads of the CTA; scratch: THREADS / 16 + 2 words of shared memory.
-// CTAs past the number of tiles get none.
+// CTAs past the number of tiles get none.  Sequences whose rows overlap can have more
+// tiles together than the host's bound, which counts every query token once; where that
+// is more than can be numbered, nobody gets any.
 template <int ROWS, int KEYS, int COST, int THREADS>
 __device__ __forceinline__ Share take_share(const AttentionParams& p, int* scratch) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -210,15 +216,20 @@ __device__ __forceinline__ Share take_share(const AttentionParams& p, int* scrat
     int2 mine = make_int2(0, 0);
     for (int i = tid; i < p.seqs; i += THREADS) {
         const int2 t = seq_tiles<ROWS, KEYS>(p, seq_view(p, i));
-        mine.x += t.x, mine.y += t.y;
+        mine.x = (int)min((unsigned)mine.x + (unsigned)t.x, 0x7fffffffu), mine.y += t.y;
     }
-    const int tiles = (int)__reduce_add_sync(0xffffffffu, (unsigned)mine.x);
+    // (the sum of 32 numbers below 2^31, in two halves, at most 2^31 - 1)
+    const unsigned low = __reduce_add_sync(0xffffffffu, (unsigned)mine.x & 0xffffu);
+    const unsigned high = __reduce_add_sync(0xffffffffu, (unsigned)mine.x >> 16) + (low >> 16);
+    const int tiles = high > 0x7fffu ? 0x7fffffff : (int)(high << 16 | (low & 0xffffu));
     const int units = (int)__reduce_add_sync(0xffffffffu, (unsigned)mine.y);
     if (lane == 0) scratch[2 * warp] = tiles, scratch[2 * warp + 1] = units;
     __syncthreads();
-    int total = 0, all_units = 0;
+    int64_t all = 0;
+    int all_units = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) total += scratch[2 * w], all_units += scratch[2 * w + 1];
+    for (int w = 0; w < kWarps; ++w) all += scratch[2 * w], all_units += scratch[2 * w + 1];
+    int total = all <= 0x7fffffff / (1 + COST) ? (int)all : 0;
     // (A CTA that takes up a unit in its middle pays as well, so with little to do for each
     // a high price would only leave CTAs without work.)
     const int cost = total > (int)gridDim.x ? min(COST, total / (int)gridDim.x) : 0;

@@ -1,0 +1,54 @@
+"""Attention over the paged MX cache: batches whose sequences differ much, bounds far
+above the lengths, and what such calls take in memory."""
+import numpy as np
+import pytest
+from test_cache_attention_gpu import attend, build, check
+
+pytestmark = pytest.mark.gpu
+
+
+def widened(torch, b, max_kv):
+    """The batch with a page table for max_kv tokens a sequence; what lies past a
+    sequence's pages is any number."""
+    table = torch.full((b["table"].shape[0], -(-max_kv // b["cache"].page_size)), -7, dtype=torch.int32, device="cuda")
+    table[:, :b["table"].shape[1]] = b["table"]
+    return dict(b, table=table)
+
+
+@pytest.mark.parametrize("max_kv", [2048, 1 << 20])
+def test_one_long_chunk_beside_many_decoding_sequences(torch_cuda, mxk, max_kv):
+    """Few row tiles in all, though 256 sequences of the longest chunk over the longest
+    cache would have more key tiles than can be numbered."""
+    torch, g = torch_cuda, np.random.default_rng(41)
+    q_lens = [1] * 256
+    q_lens[77] = 2000
+    kv_lens = [int(x) for x in g.integers(1, 200, 256)]
+    kv_lens[77] = 2040
+    b = widened(torch, build(torch, mxk, g, q_lens, kv_lens, 16, 2, 64, 128, 8, "bfloat16"), max_kv)
+    check(torch, b, *attend(torch, mxk, b, max_kv=max_kv))
+
+
+def test_unused_entries_at_the_end(torch_cuda, mxk):
+    """A batch padded with sequences whose row range is empty or runs backwards."""
+    torch, g = torch_cuda, np.random.default_rng(42)
+    b = build(torch, mxk, g, [1, 40, 300], [100, 90, 400], 4, 2, 64, 32, 8, "bfloat16")
+    want = attend(torch, mxk, b)
+    cu = torch.cat([b["cu"], torch.tensor([0, 0, 0], dtype=torch.int32, device="cuda")])
+    padded = dict(b, cu=cu, kv=torch.nn.functional.pad(b["kv"], (0, 3)),
+                  table=torch.nn.functional.pad(b["table"], (0, 0, 0, 3)))
+    got = attend(torch, mxk, padded)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_overlapping_rows_stay_inside(torch_cuda, mxk):
+    """Row ranges that overlap, so that there is far more work than the query tokens
+    make: nothing outside the output is written."""
+    torch, g = torch_cuda, np.random.default_rng(43)
+    n, seqs = 1, 4000
+    b = build(torch, mxk, g, [n], [64], 2, 2, 64, 16, 8, "bfloat16")
+    cu = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda")
+    cu[1::2] = n
+    over = dict(b, cu=cu, table=b["table"].expand(seqs, -1).contiguous(), kv=b["kv"].expand(seqs).contiguous())
+    out = torch.full((n + 2, 2, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    attend(torch, mxk, over, lse=False, out=out[1:1 + n])
+    assert (out[0] == 5.0).all() and (out[-1] == 5.0).all()
