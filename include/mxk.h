@@ -348,20 +348,21 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  * must be below 1.9e8, and the sequences' rows may not overlap.
  * head_dim must be 64 or 128 (others: MXK_ERR_UNSUPPORTED).
  *
- * Products are taken in f16 with float32 sums: every MX element times its scale
- * is exact in f16 relative to a power of two that moves with the data, but for keys
- * below 2^-21 of their token's largest block, and values below 2^-24 of the largest
- * that the row sees, which may lose bits; q's rows are scaled into f16 by a power of two, and exp(s - max) is rounded to f16
- * for the product with v.  Statistics are float32.  The result does not depend on
- * timing: partial sums join in a fixed order.
+ * Products are taken in f16 with float32 sums: every MX element times its scale is
+ * exact in f16 relative to a power of two that moves with the data, but for keys below
+ * 2^-21 of their token's largest block, and values below 2^-24 of the largest that the
+ * row sees, which may lose bits; q's rows are scaled into f16 by a power of two, and
+ * exp(s - max) is rounded to f16 for the product with v.  Statistics are float32.  The
+ * result does not depend on timing: partial sums join in a fixed order.
  *
- * Asynchronous on `stream`; partial sums live in the library's stream-ordered
- * pool on the current device (mxk_release_workspace): at most 70 MB, and, when
- * sequences have more than 512 query rows per key head (n * heads / kv_heads; 256 among
- * several sequences), their keys and values converted to f16 once, seqs * kv_heads *
- * max_kv * head_dim * 4 bytes (not done where that exceeds 4 GB).  May be captured into a graph.  A device-side
- * wait that gives up leaves the call's output undefined; the next synchronous call of
- * the library on the device reports MXK_ERR_TIMEOUT. */
+ * Asynchronous on `stream`; partial sums live in the library's stream-ordered pool on
+ * the current device (mxk_release_workspace): at most 70 MB, and, when sequences have
+ * more than R = 512 query rows per key head (n * G; R = 256 among several sequences),
+ * their keys and values converted to f16 once, m * kv_heads * max_kv * head_dim * 4
+ * bytes for the m = min(seqs, tokens * G / (R + 1)) that there can be (not done where
+ * that exceeds 4 GB).  May be captured into a graph.  A device-side wait that gives up
+ * leaves the call's output undefined; the next synchronous call of the library on the
+ * device reports MXK_ERR_TIMEOUT. */
 typedef struct {
     int dtype;
     int heads;

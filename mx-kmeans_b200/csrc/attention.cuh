@@ -50,12 +50,13 @@ struct AttentionParams {
     float2* part_stat;  // [2 * CTAs][tile rows]: running maximum (log2 units), sum
     int4* part_open;    // [CTAs]: {sequence, row tile, key head, n} of the unit that the CTA began and the n
                         // following ones went on with; n = 0: it left none unfinished
-    // keys and values converted beforehand (tiles kernel), [seqs][kv_heads][max_tiles]
+    // keys and values converted beforehand (tiles kernel), [ready_seqs][kv_heads][max_tiles], of
+    // this launch's sequences, one after the other
     uint8_t* ready_k;
     uint8_t* ready_v;
     int2* ready_meta;   // reference scales of the keys (or kWide) and values; bit 16 of y: NaNs taken out
     uint8_t* ready_key_refs;  // [tile][token] reference scales of the keys of kWide tiles
-    int max_tiles;
+    int max_tiles, ready_seqs;
 };
 
 // Key tiles there can be at most when no sequence has more than max_q query and
@@ -175,11 +176,17 @@ __device__ __forceinline__ int tile_count(const AttentionParams& p, const SeqVie
     return hi <= lo ? 1 : (hi + KEYS - 1) / KEYS - t0;
 }
 
+// Whether this launch takes a sequence.
+__device__ __forceinline__ bool taken(const AttentionParams& p, const SeqView& s) {
+    const int rows = s.n * p.group;
+    return rows != 0 && rows >= p.min_rows && rows <= p.max_rows;
+}
+
 // Key tiles and units of a sequence.
 template <int ROWS, int KEYS>
 __device__ __forceinline__ int2 seq_tiles(const AttentionParams& p, const SeqView& s) {
     const int rows = s.n * p.group;
-    if (rows < p.min_rows || rows > p.max_rows || rows == 0) return make_int2(0, 0);
+    if (!taken(p, s)) return make_int2(0, 0);
     const int tiles = (rows + ROWS - 1) / ROWS, units = tiles * p.kv_heads;
     if (!p.causal) return make_int2(units * tile_count<ROWS, KEYS>(p, s, 0), units);
     int total = 0;
@@ -282,6 +289,7 @@ struct Walk {
     int tile, tiles;  // next key tile of the unit, and how many it has
     int skip;         // empty ones to pass before it
     int first;        // number of the unit's first key tile in the sequence
+    int rank;         // of the sequence among those that the launch takes (the ready kernel sets it)
     SeqView view;
 };
 
@@ -289,6 +297,7 @@ template <int ROWS, int KEYS>
 __device__ __forceinline__ Walk walk_to(const AttentionParams& p, const Share& s) {
     Walk w;
     w.seq = s.seq;
+    w.rank = 0;
     w.view = seq_view(p, s.seq);
     int offset = s.offset;
     w.rt = 0;
@@ -315,13 +324,12 @@ __device__ __forceinline__ void walk_on(const AttentionParams& p, Walk& w) {
     ++w.rt;
     if (w.rt * ROWS >= w.view.n * p.group) {
         w.rt = 0;
-        int rows;
+        ++w.rank;
         do {
             ++w.seq;
             if (w.seq >= p.seqs) return;
             w.view = seq_view(p, w.seq);
-            rows = w.view.n * p.group;
-        } while (rows == 0 || rows < p.min_rows || rows > p.max_rows);
+        } while (!taken(p, w.view));
     }
     w.tiles = tile_count<ROWS, KEYS>(p, w.view, w.rt, &w.first);
 }

@@ -451,9 +451,37 @@ struct Converter {
 };
 static_assert(kRefStep == 4, "value_ref rounds to multiples of four");
 
+// The sequence that is the rank-th of those the launch takes, -1 if there is none.  A whole warp.
+__device__ __forceinline__ int seq_of_rank(const AttentionParams& p, int rank) {
+    for (int base = 0; base < p.seqs; base += 32) {
+        const int i = base + (threadIdx.x & 31);
+        const unsigned m = __ballot_sync(kFull, i < p.seqs && dev::taken(p, dev::seq_view(p, min(i, p.seqs - 1))));
+        if (rank < __popc(m)) return base + (int)__fns(m, 0, rank + 1);
+        rank -= __popc(m);
+    }
+    return -1;
+}
+
+// The other way round: the rank of a sequence, and how many there are.
+struct Ranks {
+    int rank, all;
+};
+__device__ __forceinline__ Ranks rank_of_seq(const AttentionParams& p, int seq) {
+    Ranks r{0, 0};
+#pragma unroll 4
+    for (int base = 0; base < p.seqs; base += 32) {
+        const int i = base + (threadIdx.x & 31);
+        const unsigned m = __ballot_sync(kFull, i < p.seqs && dev::taken(p, dev::seq_view(p, min(i, p.seqs - 1))));
+        const int before = min(max(seq - base, 0), 32);
+        r.all += __popc(m);
+        r.rank += __popc(before ? m & (0xffffffffu >> (32 - before)) : 0u);
+    }
+    return r;
+}
+
 // Converts the key tiles that some row sees once for all row tiles of a key head.
-// Block (x, side): key tile x % max_tiles of (sequence, head) x / max_tiles, its keys or
-// its values; the f16 tiles lie in the workspace as shared memory will hold them, so each
+// Block (x, side): key tile x % max_tiles of (rank of the sequence, head) x / max_tiles, its
+// keys or its values; the f16 tiles lie in the workspace as shared memory will hold them, so each
 // is built there and leaves as one bulk copy.
 template <int D, int BITS>
 __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionParams p) {
@@ -461,10 +489,11 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
     __shared__ __align__(128) uint8_t image[Smem<D>::tile];
     dev::let_next_start();
     const int tile = blockIdx.x % p.max_tiles, sh = blockIdx.x / p.max_tiles;
-    const int seq = sh / p.kv_heads, head = sh - seq * p.kv_heads;
+    const int rank = sh / p.kv_heads, head = sh - rank * p.kv_heads;
+    const int seq = p.seqs == 1 ? rank : seq_of_rank(p, rank);
+    if (seq < 0) return;
     const dev::SeqView view = dev::seq_view(p, seq);
-    const int rows = view.n * p.group;
-    if (rows == 0 || rows < p.min_rows || rows > p.max_rows) return;
+    if (!dev::taken(p, view)) return;
     int lo, hi;
     dev::seen_range(p, view, 0, view.n - 1, lo, hi);
     const int t0 = tile * kKeys;
@@ -585,7 +614,7 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
 // Index of a key tile among the converted ones.
 template <class Cfg>
 __device__ __forceinline__ int64_t ready_at(const AttentionParams& p, const Cursor<Cfg>& c) {
-    return ((int64_t)c.w.seq * p.kv_heads + c.w.head) * p.max_tiles + c.w.first + c.tile0;
+    return ((int64_t)c.w.rank * p.kv_heads + c.w.head) * p.max_tiles + c.w.first + c.tile0;
 }
 
 // One warp copying ready-made tiles (its elected lane).
@@ -1449,6 +1478,12 @@ __device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_ra
     if (share.tiles > 0) {
         c.w = dev::walk_to<kRows, kKeys>(p, share);
         c.left = share.tiles - c.w.skip;
+        if (std::is_same<Cfg, Ready>::value && p.seqs > 1) {
+            // More than the host made room for can only be sequences whose rows overlap.
+            const Ranks r = rank_of_seq(p, share.seq);
+            c.w.rank = r.rank;
+            if (r.all > p.ready_seqs) c.left = 0;
+        }
     }
     if (c.left <= 0) {
         if (tid == 0) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -1601,7 +1636,7 @@ int launch_ready(AttentionParams p, int max_q, AttentionCall& call) {
     if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
     int64_t ctas;
     MXK_CHECK(grid_size<Ready>(p, max_q, &ctas));
-    const int64_t tiles = (int64_t)p.seqs * p.kv_heads * p.max_tiles;
+    const int64_t tiles = (int64_t)p.ready_seqs * p.kv_heads * p.max_tiles;
     void* extra = nullptr;
     MXK_CHECK(call.take(p, ctas, Ready::rows, D, tiles * (2 * Smem<D>::tile + (int64_t)sizeof(int2) + kKeys), &extra));
     p.ready_k = static_cast<uint8_t*>(extra);
@@ -1630,11 +1665,12 @@ int launch_bits(int bits, const AttentionParams& p, bool ready, int max_q, Atten
 
 int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, AttentionCall& call) {
     // Several row tiles of a key head share its keys: converting those once pays for
-    // writing and reading them as f16.
+    // writing and reading them as f16.  So many sequences can have enough rows for that:
     p.max_tiles = (p.max_kv + kKeys - 1) / kKeys;
-    const int64_t bytes = (int64_t)p.seqs * p.kv_heads * p.max_tiles * 2 * kKeys * head_dim * 2;
     const int ready_rows = p.seqs == 1 ? kReadyRows : kReadyRowsMany;
-    const bool many = (int64_t)max_q * p.group > ready_rows && p.max_tiles > 0 && bytes <= kReadyBytes;
+    p.ready_seqs = p.seqs == 1 ? 1 : (int)std::min<int64_t>(p.seqs, p.tokens * p.group / (ready_rows + 1));
+    const int64_t bytes = (int64_t)p.ready_seqs * p.kv_heads * p.max_tiles * 2 * kKeys * head_dim * 2;
+    const bool many = (int64_t)max_q * p.group > ready_rows && p.ready_seqs > 0 && p.max_tiles > 0 && bytes <= kReadyBytes;
     const int few_q = (int)((ready_rows + p.group - 1) / p.group);
     if (many) {
         AttentionParams q = p;

@@ -52,3 +52,45 @@ def test_overlapping_rows_stay_inside(torch_cuda, mxk):
     out = torch.full((n + 2, 2, 64), 5.0, dtype=torch.bfloat16, device="cuda")
     attend(torch, mxk, over, lse=False, out=out[1:1 + n])
     assert (out[0] == 5.0).all() and (out[-1] == 5.0).all()
+
+
+def launched(torch, mxk, call):
+    """Names of the kernels that a call launches."""
+    mxk.profile_enable(True)
+    mxk.profile_read()
+    call()
+    names = {n for n, _ in mxk.profile_read().items()}
+    mxk.profile_enable(False)
+    return names
+
+
+@pytest.mark.parametrize("max_kv", [8192, 32768])
+def test_memory_goes_by_the_chunks_there_are(torch_cuda, mxk, max_kv):
+    """One prompt chunk beside 63 decoding sequences: room is made for the sequences that
+    can be converted, not for all of them, and the chunk has the kernel it has alone."""
+    torch, g = torch_cuda, np.random.default_rng(44)
+    q_lens, kv_lens = [1] * 64, [int(x) for x in g.integers(1, 300, 64)]
+    q_lens[20], kv_lens[20] = 300, 700
+    b = widened(torch, build(torch, mxk, g, q_lens, kv_lens, 32, 8, 128, 64, 8, "bfloat16"), max_kv)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    mxk.release_workspace()
+    free = torch.cuda.mem_get_info()[0]
+    names = launched(torch, mxk, lambda: attend(torch, mxk, b, max_kv=max_kv))
+    taken = free - torch.cuda.mem_get_info()[0]
+    assert "attention_ready" in names
+    # 363 query tokens of 4 rows: at most five sequences of more than 256 rows
+    assert taken <= 5 * 8 * max_kv * 128 * 4 * 1.05 + (128 << 20), f"{taken >> 20} MB"
+    mxk.release_workspace()
+    check(torch, b, *attend(torch, mxk, b, max_kv=max_kv))
+
+
+@pytest.mark.parametrize("bits,dim", [(8, 128), (4, 64)])
+def test_long_chunks_among_short_ones(torch_cuda, mxk, bits, dim):
+    """Converted tiles are numbered by the sequences that have them."""
+    torch, g = torch_cuda, np.random.default_rng(45)
+    q_lens = [1, 300, 0, 2, 150, 260, 5, 0, 500, 1] + [1] * 40 + [270]
+    kv_lens = [n + int(x) for n, x in zip(q_lens, g.integers(0, 500, len(q_lens)))]
+    b = build(torch, mxk, g, q_lens, kv_lens, 4, 2, dim, 32, bits, "bfloat16")
+    for kw in (dict(), dict(window=140), dict(causal=False)):
+        check(torch, b, *attend(torch, mxk, b, **kw), **kw)
