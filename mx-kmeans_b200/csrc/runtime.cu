@@ -142,16 +142,44 @@ LaunchScope::~LaunchScope() {
 PhaseRange::PhaseRange(const char* name) { nvtxRangePushA(name); }
 PhaseRange::~PhaseRange() { nvtxRangePop(); }
 
+namespace {
+// What a call sets up once and keeps may be asked for first by a call that is being captured
+// into a graph, or while another thread captures one: this thread's CUDA calls are taken out
+// of the captures' rules meanwhile.
+class OutsideCapture {
+public:
+    OutsideCapture() { ok_ = cudaThreadExchangeStreamCaptureMode(&mode_) == cudaSuccess; }
+    ~OutsideCapture() {
+        if (ok_) cudaThreadExchangeStreamCaptureMode(&mode_);
+    }
+    OutsideCapture(const OutsideCapture&) = delete;
+    OutsideCapture& operator=(const OutsideCapture&) = delete;
+
+private:
+    cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+    bool ok_;
+};
+
+// `bytes` of zeros on the current device; nullptr on failure.  They are cleared on a stream of
+// their own: the legacy stream may not be used while others that it waits for are captured.
+void* zeroed_device_memory(size_t bytes) {
+    const OutsideCapture outside;
+    void* p = nullptr;
+    cudaStream_t stream = nullptr;
+    const bool ok = cudaMalloc(&p, bytes) == cudaSuccess &&
+                    cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking) == cudaSuccess &&
+                    cudaMemsetAsync(p, 0, bytes, stream) == cudaSuccess && cudaStreamSynchronize(stream) == cudaSuccess;
+    if (stream) cudaStreamDestroy(stream);
+    if (!ok && p) cudaFree(p);
+    return ok ? p : nullptr;
+}
+}  // namespace
+
 unsigned* device_error_word() {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lock(g_mutex);
-    if (!g_error_words[dev]) {
-        void* p = nullptr;
-        if (cudaMalloc(&p, sizeof(unsigned)) != cudaSuccess) return nullptr;
-        if (cudaMemset(p, 0, sizeof(unsigned)) != cudaSuccess) return nullptr;
-        g_error_words[dev] = static_cast<unsigned*>(p);
-    }
+    if (!g_error_words[dev]) g_error_words[dev] = static_cast<unsigned*>(zeroed_device_memory(sizeof(unsigned)));
     return g_error_words[dev];
 }
 
@@ -213,6 +241,7 @@ cudaMemPool_t workspace_pool() {
         props.location.type = cudaMemLocationTypeDevice;
         props.location.id = dev;
         cudaMemPool_t pool = nullptr;
+        const OutsideCapture outside;
         if (cudaMemPoolCreate(&pool, &props) != cudaSuccess) return nullptr;
         uint64_t keep = ~0ull;  // keep freed blocks mapped for the next call
         if (cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep) != cudaSuccess) {
