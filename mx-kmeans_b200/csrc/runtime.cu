@@ -111,6 +111,7 @@ int fail(int status, const std::string& message) {
 
 int fail_cuda(const char* what, cudaError_t err) {
     g_last_error = std::string(what) + ": " + cudaGetErrorString(err);
+    cudaGetLastError();  // reported here: it is not the next launch's
     return MXK_ERR_CUDA;
 }
 
@@ -171,6 +172,7 @@ void* zeroed_device_memory(size_t bytes) {
                     cudaMemsetAsync(p, 0, bytes, stream) == cudaSuccess && cudaStreamSynchronize(stream) == cudaSuccess;
     if (stream) cudaStreamDestroy(stream);
     if (!ok && p) cudaFree(p);
+    if (!ok) cudaGetLastError();
     return ok ? p : nullptr;
 }
 }  // namespace
@@ -242,7 +244,10 @@ cudaMemPool_t workspace_pool() {
         props.location.id = dev;
         cudaMemPool_t pool = nullptr;
         const OutsideCapture outside;
-        if (cudaMemPoolCreate(&pool, &props) != cudaSuccess) return nullptr;
+        if (cudaMemPoolCreate(&pool, &props) != cudaSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
         uint64_t keep = ~0ull;  // keep freed blocks mapped for the next call
         if (cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep) != cudaSuccess) {
             cudaMemPoolDestroy(pool);

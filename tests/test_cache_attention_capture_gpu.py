@@ -99,3 +99,38 @@ def test_calls_on_two_streams(torch_cuda, mxk, threads):
     for i in range(2):
         for out in outs[i]:
             assert torch.equal(out, want[i])
+
+
+def test_a_failure_is_reported_once(torch_cuda, mxk):
+    """A call that the CUDA runtime refuses (here: waiting for the device while another
+    thread captures) fails itself, and not the calls that its thread makes afterwards."""
+    import threading
+    torch = torch_cuda
+    b = build(torch, mxk, np.random.default_rng(55), [3], [50], 4, 2, 64, 16, 8, "bfloat16")
+    k = torch.zeros(3, 2, 64, device="cuda")
+    slots = torch.full((3,), -1, device="cuda")
+    capturing, refused, ended = (threading.Event() for _ in range(3))
+    seen = []
+
+    def other():
+        capturing.wait(60)
+        try:
+            mxk.release_workspace()
+        except mxk.MxkError:
+            seen.append("refused")
+        refused.set()
+        ended.wait(60)
+        mxk.cache_write(b["cache"], k, k, slots)
+        seen.append("written")
+    thread = threading.Thread(target=other)
+    thread.start()
+    try:
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            capturing.set()
+            refused.wait(60)
+    except RuntimeError:
+        pass  # the other thread's call has invalidated the capture
+    ended.set()
+    thread.join()
+    torch.cuda.synchronize()
+    assert seen == ["refused", "written"]
