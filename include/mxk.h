@@ -346,7 +346,8 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  * (out may not overlap q).  lse (optional): float32 [tokens][heads].  With
  * G = heads / kv_heads, (tokens * G / 128 + 2 * seqs) * kv_heads * (max_kv / 128 + 2)
  * must be below 1.9e8, and the sequences' rows may not overlap.
- * head_dim must be 64 or 128 (others: MXK_ERR_UNSUPPORTED).
+ * head_dim must be 64 or 128, pages * kv_heads * page_size at most 2^32 (others:
+ * MXK_ERR_UNSUPPORTED).
  *
  * Products are taken in f16 with float32 sums: every MX element times its scale is
  * exact in f16 relative to a power of two that moves with the data, but for keys below

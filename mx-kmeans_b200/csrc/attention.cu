@@ -922,6 +922,9 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     MXK_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, "cache_attention: scale must be finite");
     if (cache->head_dim != 64 && cache->head_dim != 128)
         return fail(MXK_ERR_UNSUPPORTED, "cache_attention: head_dim must be 64 or 128");
+    // (The kernels number the cache's rows in 32 bits.)
+    if (cache->pages * cache->kv_heads > (1ll << 32) / cache->page_size)
+        return fail(MXK_ERR_UNSUPPORTED, "cache_attention: pages * kv_heads * page_size must be at most 2^32");
     if (a->tokens == 0 || a->seqs == 0 || a->max_q == 0) return MXK_OK;
     MXK_REQUIRE(a->q.data && a->out.data && a->cu_q && a->page_table && a->kv_lens,
                 "cache_attention: q, out, cu_q, page_table and kv_lens must be non-null");

@@ -8,7 +8,7 @@
 
 namespace mxk {
 
-// Checks the cache's fields (mxk.h) and that its buffers can be addressed.
+// Checks the cache's fields (mxk.h).
 int check_cache(const mxk_cache* c, const char* who);
 
 inline int64_t cache_slots(const mxk_cache& c) { return c.pages * c.page_size; }
