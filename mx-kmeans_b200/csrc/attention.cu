@@ -926,7 +926,7 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     if (cache->pages * cache->kv_heads > (1ll << 32) / cache->page_size)
         return fail(MXK_ERR_UNSUPPORTED, "cache_attention: pages * kv_heads * page_size must be at most 2^32");
     if (a->tokens == 0 || a->seqs == 0 || a->max_q == 0) return MXK_OK;
-    MXK_REQUIRE(a->q.data && a->out.data && a->cu_q && a->page_table && a->kv_lens,
+    MXK_REQUIRE(a->q.data && a->out.data && a->cu_q && (a->page_table || a->max_kv == 0) && a->kv_lens,
                 "cache_attention: q, out, cu_q, page_table and kv_lens must be non-null");
     MXK_REQUIRE((reinterpret_cast<uintptr_t>(a->q.data) | reinterpret_cast<uintptr_t>(a->out.data)) % 2 == 0 &&
                     (reinterpret_cast<uintptr_t>(a->cu_q) | reinterpret_cast<uintptr_t>(a->page_table) |

@@ -94,3 +94,18 @@ def test_long_chunks_among_short_ones(torch_cuda, mxk, bits, dim):
     b = build(torch, mxk, g, q_lens, kv_lens, 4, 2, dim, 32, bits, "bfloat16")
     for kw in (dict(), dict(window=140), dict(causal=False)):
         check(torch, b, *attend(torch, mxk, b, **kw), **kw)
+
+
+@pytest.mark.parametrize("q_lens", [[3], [2, 0, 70, 1], [300, 300]])
+def test_nothing_cached_and_no_pages(torch_cuda, mxk, q_lens):
+    """max_kv of zero needs no page table: zeros and -inf."""
+    torch = torch_cuda
+    cache = mxk.PagedCache.empty(2, 16, 2, 64, 8)
+    seqs, tokens = len(q_lens), sum(q_lens)
+    q = torch.randn(tokens, 4, 64, device="cuda").to(torch.bfloat16)
+    out, lse = torch.full_like(q, 3.0), torch.full((tokens, 4), 3.0, device="cuda")
+    cu = torch.tensor([0] + list(np.cumsum(q_lens)), dtype=torch.int32, device="cuda")
+    mxk.cache_attention(cache, q, cu, torch.empty(seqs, 0, dtype=torch.int32, device="cuda"),
+                        torch.zeros(seqs, dtype=torch.int32, device="cuda"), out, max_q=max(q_lens), max_kv=0, lse=lse)
+    torch.cuda.synchronize()
+    assert (out == 0).all() and (lse == -float("inf")).all()
