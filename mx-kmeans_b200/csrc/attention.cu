@@ -801,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             }
         }
 
-        // Join the warps: common maxima, outputs in true units, sums.
+        // Join the warps: maxima, sums of weights, and outputs as means in true units.
         copy_wait<0>();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -815,10 +815,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         for (int i = 0; i < 2; ++i) {
             const int r = g + 8 * i;
             const float vfactor = __uint_as_float((uint32_t)row_ref[i] << 23);
-            float top = stat_max[0][r];
-#pragma unroll
-            for (int k = 1; k < kWarps; ++k) top = fmaxf(top, stat_max[k][r]);
-            const float f = run_max[i] == top ? 1.0f : ex2(run_max[i] - top);
+            const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
             // features (2c + e) * D/8 + n, four at a time; the 16-byte chunks of a row are
             // permuted so that eight lanes write to eight different bank groups
             float4* dst = reinterpret_cast<float4*>(joined + (warp * kRows + r) * D);
@@ -827,8 +824,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
 #pragma unroll
                 for (int n = 0; n < kTiles; n += 4) {
                     const int chunk = (2 * c + e) * (D / 32) + n / 4;
-                    const float4 v = make_float4(o[n][2 * i + e] * f * vfactor, o[n + 1][2 * i + e] * f * vfactor,
-                                                 o[n + 2][2 * i + e] * f * vfactor, o[n + 3][2 * i + e] * f * vfactor);
+                    const float4 v = make_float4(o[n][2 * i + e] * inv * vfactor, o[n + 1][2 * i + e] * inv * vfactor,
+                                                 o[n + 2][2 * i + e] * inv * vfactor, o[n + 3][2 * i + e] * inv * vfactor);
                     dst[chunk ^ (c | ((g & 1) << 2))] = v;
                 }
         }
@@ -838,23 +835,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         for (int idx = tid; idx < rows * (D / 4); idx += kThreads) {
             const int r = idx / (D / 4), chunk = idx - r * (D / 4);
             const int at = chunk ^ ((chunk / (D / 16)) | ((r & 1) << 2));
-            float top = neg_inf, total = 0.0f;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float top = neg_inf, total = 0.0f, weight[kWarps];
 #pragma unroll
             for (int k = 0; k < kWarps; ++k) top = fmaxf(top, stat_max[k][r]);
 #pragma unroll
             for (int k = 0; k < kWarps; ++k) {
-                const float4 x = reinterpret_cast<const float4*>(joined + (k * kRows + r) * D)[at];
-                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-                total += stat_sum[k][r] * (stat_max[k][r] == top ? 1.0f : ex2(stat_max[k][r] - top));
+                weight[k] = stat_sum[k][r] * (stat_max[k][r] == top ? 1.0f : ex2(stat_max[k][r] - top));
+                total += weight[k];
             }
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                const float4 x = reinterpret_cast<const float4*>(joined + (k * kRows + r) * D)[at];
+                const float f = weight[k] * inv;
+                v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+            }
+            if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (whole) {
                 const int row = w.rt * kRows + r, j = row / p.group;
                 const int head = w.head * p.group + (row - j * p.group);
-                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-                if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                dev::store4(p, w.view.row0 + j, head, chunk * 4,
-                            make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                dev::store4(p, w.view.row0 + j, head, chunk * 4, v);
                 if (p.lse && chunk == 0)
                     p.lse[(int64_t)(w.view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
             } else {

@@ -13,7 +13,9 @@
 // written out by it; the parts of a unit that spans several go to the workspace
 // (at most two per CTA: the end of a unit that an earlier CTA began, and the
 // beginning of one that a later CTA goes on with) and attention_join_kernel adds
-// them in CTA order, so the result does not depend on timing.
+// them in CTA order, so the result does not depend on timing.  A part holds the weighted
+// mean of the values it saw, which is no larger than they are, and the maximum and sum of
+// its weights.
 #pragma once
 
 #include <algorithm>
@@ -46,7 +48,7 @@ struct AttentionParams {
     int causal, window;
     int min_rows, max_rows;  // this launch takes the sequences with min_rows <= n * group <= max_rows
     // partial sums
-    float* part;  // [2 * CTAs][tile rows][head_dim]
+    float* part;  // [2 * CTAs][tile rows][head_dim]: means
     float2* part_stat;  // [2 * CTAs][tile rows]: running maximum (log2 units), sum
     int4* part_open;    // [CTAs]: {sequence, row tile, key head, n} of the unit that the CTA began and the n
                         // following ones went on with; n = 0: it left none unfinished
@@ -380,14 +382,13 @@ struct JoinParams {
     int count;
 };
 
-// A row of a joined unit: v and the row's sum are over all parts, relative to `top`.
+// A row of a joined unit; total: the sum of its weights relative to `top`.
 __device__ __forceinline__ void store_joined(const AttentionParams& p, const int4& unit, const dev::SeqView& view,
                                              int row, int chunk, float4 v, float top, float total) {
     const int j = row / p.group;
     const int head = unit.z * p.group + (row - j * p.group);
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    dev::store4(p, view.row0 + j, head, chunk * 4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    dev::store4(p, view.row0 + j, head, chunk * 4, v);
     if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
 }
 
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams jp
     constexpr int kSub = 128 / kLanes;       // rows, or parts, at a time
     constexpr int kFew = 8;
     __shared__ float4 sums[kSub][kLanes];
-    __shared__ float stats[4], sub_totals[kSub];
+    __shared__ float stats[4], sub_totals[4];
     int local = blockIdx.x;
     Parts set = jp.parts[0];
 #pragma unroll
@@ -433,12 +434,18 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams jp
             for (int i = 1; i < kFew; ++i)
                 if (i < parts) top = fmaxf(top, st[i].x);
             float total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kFew; ++i)
+                if (i < parts) {
+                    st[i].y *= st[i].x == top ? 1.0f : dev::ex2(st[i].x - top);
+                    total += st[i].y;
+                }
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int i = 0; i < kFew; ++i)
                 if (i < parts) {
-                    const float f = st[i].x == top ? 1.0f : dev::ex2(st[i].x - top);
-                    total += st[i].y * f;
+                    const float f = st[i].y * inv;
                     v.x += v_part[i].x * f, v.y += v_part[i].y * f, v.z += v_part[i].z * f, v.w += v_part[i].w * f;
                 }
             store_joined(p, unit, view, unit.y * set.rows + r, chunk, v, top, total);
@@ -454,27 +461,34 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams jp
         if ((tid & 31) == 0) stats[tid >> 5] = top;
         __syncthreads();
         top = fmaxf(fmaxf(stats[0], stats[1]), fmaxf(stats[2], stats[3]));
+        // the sum of the weights
         float total = 0.0f;
+        for (int i = tid; i < parts; i += 128) {
+            const float2 st = set.stat[slot(i) * set.rows + r];
+            total += st.y * (st.x == top ? 1.0f : dev::ex2(st.x - top));
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if ((tid & 31) == 0) sub_totals[tid >> 5] = total;
+        __syncthreads();
+        total = (sub_totals[0] + sub_totals[1]) + (sub_totals[2] + sub_totals[3]);
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
         for (int i = sub; i < parts; i += kSub) {
             const float2 st = set.stat[slot(i) * set.rows + r];
             const float4 o = reinterpret_cast<const float4*>(set.part + (slot(i) * set.rows + r) * D)[chunk];
-            const float f = st.x == top ? 1.0f : dev::ex2(st.x - top);
-            total += st.y * f;
+            const float f = st.y * (st.x == top ? 1.0f : dev::ex2(st.x - top)) * inv;
             v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
         }
         sums[sub][chunk] = v;
-        if (chunk == 0) sub_totals[sub] = total;
         __syncthreads();
         if (tid < kLanes) {
-            total = 0.0f;
             v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int i = 0; i < kSub; ++i) {
                 const float4 o = sums[i][chunk];
                 v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
-                total += sub_totals[i];
             }
             store_joined(p, unit, view, unit.y * set.rows + r, chunk, v, top, total);
         }

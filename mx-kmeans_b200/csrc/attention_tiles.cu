@@ -1404,7 +1404,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                     bad[0] = f.x, bad[1] = f.y, bad[2] = f.z, bad[3] = f.w;
                 }
                 const float vfactor = __uint_as_float((uint32_t)vrun << 23);
-                const float inv = all ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 const int64_t slot = 2 * (int64_t)blockIdx.x + (c.tile0 == 0 ? 1 : 0);
                 const int tile_row = w * kTileRows + r;
                 const unsigned reals = __ballot_sync(kFull, real);
