@@ -109,3 +109,36 @@ def test_nothing_cached_and_no_pages(torch_cuda, mxk, q_lens):
                         torch.zeros(seqs, dtype=torch.int32, device="cuda"), out, max_q=max(q_lens), max_kv=0, lse=lse)
     torch.cuda.synchronize()
     assert (out == 0).all() and (lse == -float("inf")).all()
+
+
+@pytest.mark.parametrize("q_lens,kv_lens", [([300], [700]), ([400, 1, 90], [1000, 50, 300])])
+def test_a_cache_too_long_to_be_converted(torch_cuda, mxk, q_lens, kv_lens):
+    """Where the bounds ask for more than 4 GB of converted tiles, chunks of any length go
+    through the packed kernel."""
+    torch, g = torch_cuda, np.random.default_rng(46)
+    max_kv = (1 << 20) + 128
+    b = widened(torch, build(torch, mxk, g, q_lens, kv_lens, 32, 8, 128, 128, 8, "bfloat16"), max_kv)
+    torch.cuda.synchronize()
+    names = launched(torch, mxk, lambda: attend(torch, mxk, b, max_kv=max_kv))
+    assert "attention_tiles" in names and "attention_ready" not in names
+    check(torch, b, *attend(torch, mxk, b, max_kv=max_kv))
+
+
+@pytest.mark.parametrize("max_q", [64, 512])
+def test_a_graph_for_chunks_replayed_with_one_token(torch_cuda, mxk, max_q):
+    """One sequence, captured for chunks, whose kernels then see a single row."""
+    torch, g = torch_cuda, np.random.default_rng(47)
+    b = build(torch, mxk, g, [max_q], [1500], 8, 2, 128, 64, 8, "bfloat16")
+    out, lse = torch.empty_like(b["q"]), torch.empty(max_q, 8, device="cuda")
+    attend(torch, mxk, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mxk.cache_attention(b["cache"], b["q"], b["cu"], b["table"], b["kv"], out, max_q=max_q, max_kv=1500, lse=lse)
+    for n in (1, 3, 60):
+        b["cu"].copy_(torch.tensor([0, n], dtype=torch.int32))
+        b["q_lens"] = [n]
+        out.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(torch, b, out, lse)
+        assert (out[n:] == 9.0).all()
