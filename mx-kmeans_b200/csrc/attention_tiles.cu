@@ -18,15 +18,19 @@
 //               all of them (attention_ready_kernel, two row tiles)
 //
 // Measured at 32 heads of 128 on 8 key heads, 8 bits, 16,384 tokens cached:
-//   4096 query tokens   880 us, 1090 Tflop/s, 66 % of a library product's rate.  The
-//                       ready kernel takes 2.15 us for 256 rows x 128 keys where the
-//                       products alone need 0.57 x 2 and the exponentials 0.9 (1800 MHz):
-//                       two softmax warps a scheduler leave the waits between the steps
-//                       of a row (scores, maximum, weights, store) half uncovered.
-//   512 query tokens    179 us: 17 converting, 145 multiplying, 10 joining
-//   16 query tokens     46 us: the packed kernel converts a key tile for one row tile in
-//                       the time that tile's softmax takes
-// More query rows per thread, or two row tiles beside converters, ran out of registers.
+//   4096 query tokens   975 to 996 us one after the other, 966 to 986 Tflop/s, 59 % of a
+//                       library product's rate; 912 us on an idle card (the power cap).
+//                       The ready kernel takes 2.2 to 2.4 us for 256 rows x 128 keys where
+//                       the products need 0.57 x 2 and the exponentials 1.0 (1800 MHz, one
+//                       pair in eight on the FMA pipe): two softmax warps a scheduler leave
+//                       the waits between the steps of a row (scores, maximum, weights,
+//                       store) half uncovered.  Tensor pipe 52 % of the cycles, MUFU 46 %.
+//   512 query tokens    176 to 187 us; one by one 21 converting, 156 multiplying, 15 joining
+//   16 query tokens     58 us with a cold L2 (42 and the join): the packed kernel converts a
+//                       key tile for one row tile in the time that tile's softmax takes
+// More query rows per thread, or two row tiles beside converters, ran out of registers; as
+// it is, the softmax spills some 280 (ready) and 380 (packed) bytes a thread.  The times beside
+// the choices below are from when they were made.
 //
 // P (f16) overwrites the S it came from, so TMEM holds S0 S1 O0 O1, 512 columns at
 // D = 128.  Values are the right operand as they lie in the cache (one row per
@@ -77,11 +81,13 @@ constexpr int kRefStep = 4;              // value references are multiples of th
 constexpr int kMostDown = 64;            // octaves that a float32 weight may be scaled down by
 // Rows per key head above which its keys are converted beforehand.  In us, packed and
 // ready kernel, over 16,384 tokens (32 heads of 128 on 8): 256 rows 72, 94; 384 rows 84,
-// 109; 512 rows 99, 111; 1024 rows (eight passes of the packed one) 121 ready.  Among
-// several sequences a lower bound, as the two kernels run one after the other and the
-// second has little to do: nine sequences with 4 to 2804 rows 147 us with 512, 132 with 256.
+// 109; 512 rows 99, 111; 1024 rows (eight passes of the packed one) 121 ready.  (Where the
+// two cross above 512 was not measured.)  Among several sequences a lower bound, as the two
+// kernels run one after the other and the second has little to do: nine sequences with 4
+// to 2804 rows 147 us with 512, 132 with 256.
 constexpr int kReadyRows = 512, kReadyRowsMany = 256;
-// The most memory that converting may take: larger batches take the packed kernel.
+// The most memory that converting may take: above it the packed kernel goes over the keys
+// once for every 128 rows.
 constexpr int64_t kReadyBytes = 4ll << 30;
 
 // The two kernels' row tiles, warps and registers.  Warpgroups give up or take registers
@@ -257,11 +263,14 @@ __device__ __noinline__ uint4 magnitude_scales(const uint8_t* values, uint32_t p
         const int r = (threadIdx.x & 31) + 32 * i;
         const uint32_t row = __shfl_sync(kFull, place, r >> 4) + (r & 15);
         if (r < from || r >= to) continue;
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(values + (uint64_t)row * (D * BITS / 8));
-        for (int b = 0; b < D / 32; ++b) {
-            uint32_t any = 0;
+        const uint8_t* at = values + (uint64_t)row * (D * BITS / 8);
 #pragma unroll
-            for (int k = 0; k < kBlock; ++k) any |= __ldg(w + b * kBlock + k) & dev::magnitude_bits<BITS>(k);
+        for (int b = 0; b < D / 32; ++b) {
+            uint32_t w[kBlock], any = 0;
+#pragma unroll
+            for (int k = 0; k < kBlock; k += kBlock % 4 ? 2 : 4) ldg_bytes<kBlock % 4 ? 8 : 16>(at + 4 * (b * kBlock + k), w + k);
+#pragma unroll
+            for (int k = 0; k < kBlock; ++k) any |= w[k] & dev::magnitude_bits<BITS>(k);
             if (!any) out[i] &= ~(255u << (8 * b));
         }
     }
@@ -766,8 +775,9 @@ __device__ __forceinline__ void fold_top(const uint32_t (&s)[32], float (&m)[4])
 
 // 2^x of a pair on the FMA pipe, for x below 128: with n the integer nearest to x and
 // r = x - n, 2^x = 2^n 2^r, and on [-1/2, 1/2] a polynomial of degree five is within 7.5e-8
-// of 2^r (least squares on the relative error, reweighted towards its largest values).
-// Below -127 the result is zero; a NaN stays one.
+// of 2^r (least squares on the relative error, reweighted towards its largest values);
+// in float32, whose constant term is 1 + 2^-23, within 2.2e-7.  The weights it makes are
+// rounded to f16 afterwards.  Below -127 the result is zero; a NaN stays one.
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
     asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));  // -127
     asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
@@ -788,8 +798,8 @@ __device__ __forceinline__ float2 ex2_fma(float2 x) {
 
 // Weights 2^(score * f - base) of 32 scores, added to sum, as f16 pairs.  The exponential
 // unit, 16 a cycle and SM, takes as long for them as the tensor core for both products; one
-// pair in kFmaEvery is computed on the FMA pipe instead (chunk of 4096 over 16,384 tokens:
-// 945 us without, 900 with one in 8, 928 one in 4, 962 one in 2).
+// pair in kFmaEvery is computed on the FMA pipe instead (chunk of 4096 over 16,384 tokens of
+// heads of 128: 945 us without, 900 with one in 8, 928 one in 4, 962 one in 2).
 constexpr int kFmaEvery = 8;
 __device__ __forceinline__ void fold_weights(const uint32_t (&s)[32], float f, float base, float2 (&sum)[2],
                                              uint32_t (&pw)[16]) {
@@ -807,7 +817,8 @@ __device__ __forceinline__ void fold_weights(const uint32_t (&s)[32], float f, f
     }
 }
 
-// The rare steps, out of the way of the loop's registers.
+// The rare steps.  Rescaling the output happens inside the loop over the usual halves and is
+// kept out of its registers by a call; the others have a place of their own outside it.
 
 // An output row in TMEM times g.
 template <int D>
@@ -825,7 +836,7 @@ __device__ __noinline__ void scale_output(uint32_t o_col, float g) {
 }
 
 // The largest score of a half key tile of which the row sees columns [from, to).
-__device__ __noinline__ float masked_top(uint32_t s_col, int from, int to) {
+__device__ __forceinline__ float masked_top(uint32_t s_col, int from, int to) {
     float m = __int_as_float(0xff800000);
 #pragma unroll 1
     for (int h = 0; h < kHalf / 32; ++h) {
@@ -840,7 +851,7 @@ __device__ __noinline__ float masked_top(uint32_t s_col, int from, int to) {
 }
 
 // Its weights, the f16 ones times `down`; returns their sum.
-__device__ __noinline__ float masked_weights(uint32_t s_col, int from, int to, float f, float base, float down) {
+__device__ __forceinline__ float masked_weights(uint32_t s_col, int from, int to, float f, float base, float down) {
     float sum = 0.0f;
 #pragma unroll 1
     for (int h = 0; h < kHalf / 32; ++h) {
@@ -868,7 +879,7 @@ __device__ __forceinline__ float own_score(const uint8_t* refs, int i, float s, 
 }
 
 // The same as masked_top for a tile whose keys have a reference each, in log2 units.
-__device__ __noinline__ float wide_top(uint32_t s_col, int from, int to, float f, const uint8_t* refs) {
+__device__ __forceinline__ float wide_top(uint32_t s_col, int from, int to, float f, const uint8_t* refs) {
     float m = __int_as_float(0xff800000);
 #pragma unroll 1
     for (int i = 0; i < kHalf; ++i) {
@@ -1043,35 +1054,6 @@ __device__ __forceinline__ void block_values(const uint32_t* w, float (&v)[32]) 
     }
 }
 
-// The values of a sequence and key head.
-struct ValueRows {
-    const AttentionParams& p;
-    const int* table;
-    int head;
-    __device__ __forceinline__ int64_t row(int token) const {
-        const int at = token / p.page_size;
-        const int page = min(max(__ldg(table + at), 0), p.pages - 1);
-        return ((int64_t)page * p.kv_heads + head) * p.page_size + (token - at * p.page_size);
-    }
-    // Block b of `blocks` of a row; false: all zeros.
-    __device__ __forceinline__ bool block(int64_t row, int blocks, int b, float (&v)[32]) const {
-        const uint32_t* at = reinterpret_cast<const uint32_t*>(p.v_values) + (row * blocks + b) * p.bits;
-        uint32_t w[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = k < p.bits ? __ldg(at + k) : 0;
-        if (p.bits == 8)
-            block_values<8>(w, v);
-        else if (p.bits == 6)
-            block_values<6>(w, v);
-        else
-            block_values<4>(w, v);
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) any |= v[i] != 0.0f;
-        return any;
-    }
-};
-
 // 2^(to - from), of scale bytes, up to 2^127 and down to where it is 0.
 __device__ __forceinline__ float octaves(int to, int from) {
     return __uint_as_float((uint32_t)min(max(to - from + 127, 0), 254) << 23);
@@ -1086,7 +1068,9 @@ __device__ __forceinline__ float octaves(int to, int from) {
 // held relative to one reference for rows that see different tokens, the weighted values are
 // added to the row's output in TMEM in float32 and the weights left for the product are zero.
 // The output is relative to 2^(vrun - 127) with a factor g yet to come, or holds nothing
-// yet (g = 0); vrun goes up where the row sees a token that asks for it.
+// yet (g = 0); vrun goes up where the row sees a token that asks for it.  A tile takes 115 to
+// 140 us this way (chunks of 16 to 512 tokens, one overflowed value), most of it decoding
+// that every row repeats.
 struct WideHalf {
     uint32_t s_col, o_col;  // scores; output, or 0: weights only
     int t0;                 // its first token
@@ -1098,7 +1082,7 @@ struct WideSum {
     int vrun;
 };
 template <int D>
-__device__ __noinline__ WideSum wide_weights(const AttentionParams& p, WideHalf half, int from, int to, float f,
+__device__ __forceinline__ WideSum wide_weights(const AttentionParams& p, WideHalf half, int from, int to, float f,
                                              float base, int vref, int vrun_at, float g) {
     constexpr int kBlocks = D / 32;
     const uint32_t o_col = half.o_col;
@@ -1124,18 +1108,53 @@ __device__ __noinline__ WideSum wide_weights(const AttentionParams& p, WideHalf 
         dev::tmem_wait_st();
         return WideSum{sum, vrun_at};
     }
-    const ValueRows rows{p, p.page_table + (int64_t)half.seq * p.table_stride, half.head};
-    // (The warp goes through all 64 tokens together; those that no lane sees are not touched.)
+    // The warp goes through the tokens that some lane sees together; lane i fetches what is
+    // needed of tokens i and i + 32.
+    const int lane = threadIdx.x & 31;
+    const int first = (int)__reduce_min_sync(kFull, (unsigned)(from < to ? from : kHalf));
+    const int end = (int)__reduce_max_sync(kFull, (unsigned)(from < to ? to : 0));
+    int64_t row[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int t = lane + 32 * k, token = half.t0 + t, at = token / p.page_size;
+        row[k] = -1;
+        if (t >= first && t < end) {
+            const int page = min(max(__ldg(p.page_table + (int64_t)half.seq * p.table_stride + at), 0), p.pages - 1);
+            row[k] = ((int64_t)page * p.kv_heads + half.head) * p.page_size + (token - at * p.page_size);
+        }
+    }
+    // Block b of a lane's token: its words and scale byte, zeros without a token.
+    auto fetch = [&](int k, int b, uint32_t (&w)[8]) -> int {
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(p.v_values) + (row[k] * kBlocks + b) * p.bits;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const uint2 x = row[k] >= 0 && i < p.bits ? __ldg(reinterpret_cast<const uint2*>(at + i)) : make_uint2(0, 0);
+            w[i] = x.x, w[i + 1] = x.y;
+        }
+        return row[k] >= 0 ? __ldg(p.v_scales + row[k] * kBlocks + b) : 0;
+    };
+    auto magnitude = [&](const uint32_t (&w)[8]) -> bool {
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            any |= w[i] & (p.bits == 8 ? dev::magnitude_bits<8>(i)
+                                       : (p.bits == 6 ? dev::magnitude_bits<6>(i) : dev::magnitude_bits<4>(i)));
+        return any != 0;
+    };
     int top = 0, vrun = vrun_at;
-#pragma unroll 1
-    for (int t = 0; t < kHalf; ++t) {
-        const bool sees = t >= from && t < to;
-        if (!__any_sync(kFull, sees)) continue;
-        const int64_t row = rows.row(half.t0 + t);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        int own = 0;  // the largest scale of this lane's token, blocks of zeros left out
 #pragma unroll 1
         for (int b = 0; b < kBlocks; ++b) {
-            float v[32];
-            if (rows.block(row, kBlocks, b, v) && sees) top = max(top, (int)__ldg(p.v_scales + row * kBlocks + b));
+            uint32_t w[8];
+            const int scale = fetch(k, b, w);
+            if (magnitude(w)) own = max(own, scale);
+        }
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+            const int t = 32 * k + i, x = __shfl_sync(kFull, own, i);
+            if (t >= from && t < to) top = max(top, x);
         }
     }
     if (top > 0 && (vrun == 0 || top > vrun + kValueMax)) vrun = max(top - kValueLift, 1);
@@ -1148,20 +1167,32 @@ __device__ __noinline__ WideSum wide_weights(const AttentionParams& p, WideHalf 
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = g == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[i]) * g);
 #pragma unroll 1
-        for (int t = 0; t < kHalf; ++t) {
-            const bool sees = t >= from && t < to;
-            if (!__any_sync(kFull, sees)) continue;
-            const float s = __uint_as_float(dev::tmem_ld_32x32b_x1(half.s_col + t));
-            dev::tmem_wait_ld();
-            const float weight = sees ? ex2(own_score(half.refs, t, s, f) - base) : 0.0f;
-            if (b == 0) sum += weight;
-            const int64_t row = rows.row(half.t0 + t);
-            float v[32];
-            rows.block(row, kBlocks, b, v);
-            const float factor = weight * octaves(__ldg(p.v_scales + row * kBlocks + b), vrun);
-            if (sees) {
+        for (int k = 0; k < 2; ++k) {
+            uint32_t w[8];
+            const int scale = fetch(k, b, w);
+#pragma unroll 1
+            for (int i = max(first - 32 * k, 0); i < min(end - 32 * k, 32); ++i) {
+                const int t = 32 * k + i;
+                const float s = __uint_as_float(dev::tmem_ld_32x32b_x1(half.s_col + t));
+                uint32_t x[8];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(factor, v[i], __uint_as_float(o[i])));
+                for (int j = 0; j < 8; ++j) x[j] = __shfl_sync(kFull, w[j], i);
+                float v[32];
+                if (p.bits == 8)
+                    block_values<8>(x, v);
+                else if (p.bits == 6)
+                    block_values<6>(x, v);
+                else
+                    block_values<4>(x, v);
+                const float unit = octaves(__shfl_sync(kFull, scale, i), vrun);
+                dev::tmem_wait_ld();
+                const bool sees = t >= from && t < to;
+                const float weight = sees ? ex2(own_score(half.refs, t, s, f) - base) : 0.0f;
+                if (b == 0) sum += weight;
+                if (sees) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(fmaf(weight * unit, v[j], __uint_as_float(o[j])));
+                }
             }
         }
         __syncwarp();
