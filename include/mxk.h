@@ -333,15 +333,17 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  * causal is set, and when t > p - window if window > 0 (causal only).  With s the
  * products scale * q . k over the tokens that take part,
  *     out = sum_t exp(s_t) v_t / sum_t exp(s_t),    lse = log(sum_t exp(s_t));
- * a row with no such token gets zeros and -inf.  Tokens outside [0, L) are never
- * read.  What a row does not see does not change it: neither NaNs, whatever magnitude,
- * nor, in tokens that no row of the sequence sees (before every window), any bytes.
+ * a row with no such token gets zeros and -inf.  What a row does not see does not change
+ * it: neither NaNs nor values of any magnitude, nor, in tokens that no row of the
+ * sequence sees (outside [0, L), before every window), any bytes at all.
  * (Scale bytes are taken to be 0 .. 254; cache_write never stores 255.)
  *
  * cu_q (seqs + 1), page_table, kv_lens: int32 on the device.  max_q and max_kv
- * are bounds on n and L known to the host: they choose the launch, and a longer
- * sequence's output is not defined (no memory outside the given buffers is
- * touched).  The page table holds max_kv / page_size pages (rounded up) per
+ * are bounds on n and L known to the host: they choose the kernels and their
+ * workspace, and a longer sequence's output is not defined (no memory outside the given
+ * buffers is touched).  For one sequence the kernel follows max_q alone: a graph
+ * captured for chunks takes longer for single tokens (52 us instead of 31 over 16,384
+ * tokens of 8 heads of 128), so capture one for each.  The page table holds max_kv / page_size pages (rounded up) per
  * sequence.  q and out: dtype MXK_F16 or MXK_BF16, `tokens` rows of `heads` heads
  * (out may not overlap q).  lse (optional): float32 [tokens][heads].  With
  * G = heads / kv_heads, (tokens * G / 128 + 2 * seqs) * kv_heads * (max_kv / 128 + 2)

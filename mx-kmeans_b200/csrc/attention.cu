@@ -30,13 +30,15 @@
 //    tokens.
 //
 // Measured: 64 sequences of 1 to 8192 tokens (32 heads of 128 on 8, 8 bits, 555 MB) in
-// 129 to 138 us, 4.2 TB/s over all and 5.45 TB/s while every CTA streams; two of 131,072
-// (4 bits, 285 MB) in 96 to 101.  The rest is 6 us until the first rows are there, SMs that
-// differ by a fifth in the rate they get, and the join (4 us).  Finer shares did not help,
-// neither a grid of twice as many (140 and 109 us) nor short ones taken by CTAs as they got
-// done (159 and 122): every start costs more than it evens out.  In the loop a granule is
-// 478 instructions a warp (conversion to f16, products, softmax), at 3 CTAs 40 % of the ALU
-// pipe and 28 % of the tensor pipe, and none of them is the bound by itself.
+// 138 to 147 us, 3.8 to 4.0 TB/s; two of 131,072 (4 bits, 285 MB) in 101 to 102, 2.8 TB/s.
+// Counters of the two: DRAM 50 and 35 % of its peak, instructions issued in 50 and 56 % of the
+// cycles, ALU pipe 39 and 44 %, tensor pipe 25 and 34 %, so no unit is the bound: three
+// warps a scheduler wait for their own chains (scales, conversion to f16, products,
+// maximum, weights).  4 bits hold twice the elements a byte, and the instructions go by
+// elements.  Finer shares did not help, neither a grid of twice as many CTAs nor short
+// shares taken by CTAs as they got done: every start costs more than it evens out.  Looking
+// for scales that are too far apart costs 4 to 5 % (133 and 97 us on the card with 138 and
+// 101); the times beside the choices below are from before it.
 #include <algorithm>
 #include <limits>
 #include <type_traits>

@@ -9,7 +9,9 @@
 // so HBM bounds both.
 //
 // Measured: 16,384 tokens of 8 heads of 128 in bf16 written as 8 bits and read back (203 MB)
-// in 39 us, 5.2 TB/s; 65,536 tokens read back from 4 bits (340 MB) in 62 us, 5.5 TB/s.  A
+// in 39 us, 5.2 TB/s; 65,536 tokens read back from 4 bits (340 MB) in 62 us, 5.5 TB/s.  One by
+// one with a cold L2, 65,536 tokens: 4 bits from bf16 written 74 us (4.6 TB/s) and read 66,
+// 6 bits from float32 111 both ways (5.8 TB/s), where a copy of the rows runs at 5.5 to 6.1.  A
 // token or a few take a launch's time, 3 us on the device.
 #include <limits>
 
