@@ -323,6 +323,42 @@ int mxk_cache_write(const mxk_cache* cache, int dtype, int64_t tokens, const mxk
 int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int64_t* slots, const mxk_rows* k,
                    const mxk_rows* v, void* stream);
 
+/* mxk_cache_write of keys that are rotated by their positions on the way, and the
+ * rotation of the same tokens' queries: with r = rot_dim, c_i = cos_sin[position][i] and
+ * s_i = cos_sin[position][r / 2 + i],
+ *     y_i = x_i c_i - x_j s_i,   y_j = x_j c_i + x_i s_i,   i < r / 2,
+ * for the features (i, j) = (i, i + r / 2), or (2 i, 2 i + 1) if interleaved is set, of
+ * every head; features from r on and the values are not rotated.
+ *
+ * q_out (`heads` heads) receives the rotated queries, computed in float32 and rounded once
+ * to dtype; it may be q itself (the same data and strides) and may not overlap it in any
+ * other way.  heads = 0: keys and values alone.  Slot slots[i] receives what
+ * mxk_cache_write(bits, ...) would store for the exact rotation of token i's keys (decided
+ * in about 48 bits) and for its values.
+ *
+ * slots, positions: int64 on the device.  A slot outside [0, pages * page_size) marks a
+ * token that is not kept; its queries are rotated all the same.  A position outside
+ * [0, table_rows): the token is not kept and its queries come out as zeros.  Two tokens with
+ * the same slot: which one stays is not defined.  cos_sin: float32 [table_rows][rot_dim],
+ * 16-byte aligned; rot_dim a multiple of 16 in [16, head_dim].
+ * Asynchronous on `stream`; no workspace. */
+typedef struct {
+    int dtype;
+    int heads;
+    int64_t tokens;
+    mxk_rows q;
+    mxk_rows q_out;
+    mxk_rows k;
+    mxk_rows v;
+    const int64_t* slots;
+    const int64_t* positions;
+    const float* cos_sin;
+    int64_t table_rows;
+    int rot_dim;
+    int interleaved;
+} mxk_append;
+int mxk_cache_append(const mxk_cache* cache, const mxk_append* args, void* stream);
+
 /* Attention of the newest tokens of `seqs` sequences over their cached tokens.
  *
  * Sequence i has L = kv_lens[i] cached tokens (token t in slot

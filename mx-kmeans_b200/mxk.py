@@ -63,6 +63,15 @@ class Rows(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
+class Append(ctypes.Structure):
+    """mxk_append: the arguments of mxk_cache_append."""
+
+    _fields_ = [("dtype", ctypes.c_int), ("heads", ctypes.c_int), ("tokens", ctypes.c_int64), ("q", Rows),
+                ("q_out", Rows), ("k", Rows), ("v", Rows), ("slots", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("cos_sin", ctypes.c_void_p), ("table_rows", ctypes.c_int64), ("rot_dim", ctypes.c_int),
+                ("interleaved", ctypes.c_int)]
+
+
 class Attention(ctypes.Structure):
     """mxk_attention: the arguments of mxk_cache_attention."""
 
@@ -119,6 +128,7 @@ SIGNATURES = {
     "mxk_host_write_labels": ([ctypes.c_char_p, _P, _I64], _I),
     "mxk_cache_write": ([_P, _I, _I64, _P, _P, _P, _P], _I),
     "mxk_cache_read": ([_P, _I, _I64, _P, _P, _P, _P], _I),
+    "mxk_cache_append": ([_P, _P, _P], _I),
     "mxk_cache_attention": ([_P, _P, _P], _I),
     "mxk_profile_enable": ([_I], _I),
     "mxk_profile_read": ([ctypes.POINTER(KernelStat), _I, ctypes.POINTER(_I)], _I),
@@ -462,6 +472,39 @@ def cache_read(cache, slots, k, v, stream=None):
     head_dim] (zeros for a slot outside the cache)."""
     fn, dtype, tokens, kr, vr, at, st = _move(load().mxk_cache_read, cache, k, v, slots, stream)
     check(fn(cache.handle, dtype, tokens, at, ctypes.byref(kr), ctypes.byref(vr), st))
+
+
+_NO_ROWS = Rows(None, 0, 0)
+
+
+def cache_append(cache, q, k, v, positions, cos_sin, slots, q_out=None, interleaved=False, stream=None):
+    """Rotate q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] by their
+    positions (int64 [tokens]) and quantise the rotated k, and v, into the cache's slots
+    (int64 [tokens]; mxk.h, mxk_cache_append).  cos_sin: float32 [positions, rot_dim],
+    cosines then sines; pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) if interleaved.  The
+    rotated queries go to q_out, or into q itself without one; q may be None."""
+    dtype, tokens = k.dtype, k.shape[0]
+    code = _DTYPES.get(dtype)
+    if code is None or v.dtype != dtype:
+        raise _bad("k and v: the same one of float32, float16 and bfloat16 is needed")
+    heads, qr, outr = 0, _NO_ROWS, _NO_ROWS
+    if q is not None:
+        if q.dim() != 3 or q.dtype != dtype or (q_out is not None and q_out.dtype != dtype):
+            raise _bad("q and q_out: 3 dimensions and k's type are needed")
+        heads = q.shape[1]
+        qr = _rows(q, "q", cache, tokens, heads)
+        outr = qr if q_out is None else _rows(q_out, "q_out", cache, tokens, heads)
+    elif q_out is not None:
+        raise _bad("q_out without q")
+    if cos_sin.dim() != 2:
+        raise _bad("cos_sin has 2 dimensions")
+    rows, rot = cos_sin.shape
+    table = _vector(cos_sin, "cos_sin", cache, _torch.float32, rows, rot)
+    args = Append(code, heads, tokens, qr, outr, _rows(k, "k", cache, tokens, cache.kv_heads),
+                  _rows(v, "v", cache, tokens, cache.kv_heads), _vector(slots, "slots", cache, _torch.int64, tokens),
+                  _vector(positions, "positions", cache, _torch.int64, tokens), table, rows, rot,
+                  1 if interleaved else 0)
+    check(load().mxk_cache_append(cache.handle, ctypes.byref(args), _launch_stream(cache, stream)))
 
 
 def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale=None, causal=True, window=0,
