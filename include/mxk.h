@@ -422,6 +422,38 @@ typedef struct {
 } mxk_attention;
 int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* args, void* stream);
 
+/* ---- E4M3 rows with float32 scales, and their products (no counterpart in the reference) ---- */
+
+/* Quantises `rows` rows of k features (dtype MXK_F32, MXK_F16 or MXK_BF16, contiguous,
+ * row_stride elements apart) to E4M3 with a scale per block of block_rows (1 or 128) rows and
+ * 128 features: scale = max(max |x| / 448, 2^-126) rounded to float32, code = the E4M3 value
+ * nearest to the exact quotient x / scale (of two the even one).  values: [rows][k];
+ * scales: [rows / block_rows][k / 128], both rounded up.  NaNs set no scale and stay NaN;
+ * a block with an infinity has scale infinity, its finite elements code 0 and the
+ * infinities NaN.  k % 16 == 0; values 16-byte aligned.  Asynchronous on `stream`. */
+int mxk_quantize_fp8(int dtype, int64_t rows, int64_t k, const void* x, int64_t row_stride, int block_rows,
+                     uint8_t* values, float* scales, void* stream);
+
+/* out[i][j] = sum over the blocks b of 128 features of
+ *     a_scales[i][b] * b_scales[j / 128][b] * sum over k in b of a[i][k] * b[j][k],
+ * a [m][k] and b [n][k] in E4M3, as mxk_quantize_fp8 gives them with block_rows 1 and 128;
+ * out: m rows of n elements of dtype MXK_F32, MXK_F16 or MXK_BF16, out_stride >= n elements
+ * apart, rounded once.  k % 16 == 0 (the last block may be short), a and b 16-byte aligned.
+ * A block's products are summed by the tensor core in float32, the blocks in float32 in a
+ * fixed order; the two scales are multiplied first (in float32: below 2^-126 their product
+ * loses bits).  A row's result does not depend on other rows' values.  Asynchronous on
+ * `stream`; no workspace.  A device-side wait that gives up leaves the output undefined; the
+ * next synchronous call of the library on the device reports MXK_ERR_TIMEOUT. */
+int mxk_gemm_fp8(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, const float* a_scales,
+                 const uint8_t* b, const float* b_scales, void* out, int64_t out_stride, void* stream);
+
+/* A layer's product: rows x (m rows of k features of dtype, x_stride elements apart) quantised
+ * as mxk_quantize_fp8 with block_rows 1 does, times b as mxk_gemm_fp8 takes it, with the same
+ * result as the two; x and out have the same dtype and may not overlap.  The quantised rows
+ * live in the library's stream-ordered pool on the current device (mxk_release_workspace). */
+int mxk_linear_fp8(int dtype, int64_t m, int64_t n, int64_t k, const void* x, int64_t x_stride, const uint8_t* b,
+                   const float* b_scales, void* out, int64_t out_stride, void* stream);
+
 /* ---- kernel timing (CUDA events around each launch on its stream) ---------- */
 int mxk_profile_enable(int on);
 /* Copies up to max entries of {name, launches, total_ms} for the current device. */

@@ -83,12 +83,6 @@ namespace dev {
 constexpr float kExpShift = 11.0f;
 constexpr float kMaxSlack = 4.0f;
 
-// The kernels of a call follow one another with programmatic launches: a kernel lets the
-// next one start as soon as all its own CTAs have, and the next one waits until this one
-// has finished before it reads anything written here, or else before it ends.
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -1,0 +1,385 @@
+// E4M3 products with a float32 scale per block of 128 (no counterpart in the reference,
+// whose products have MX scales, src/kernels/gemm.cu:348-363).
+//
+//     out[i][j] = sum_b sa[i][b] sb[j / 128][b] sum_{k in block b} a[i][k] b[j][k]
+//
+// The tensor core sums the 128 products of a block in float32 (tcgen05.mma kind::f8f6f4,
+// TMEM accumulators); threads take each block's sums from TMEM, one row a thread, and add
+// them to float32 registers with the factor sa sb, which is one number per thread and block.
+// Two TMEM buffers let the tensor core multiply the next block meanwhile.
+//
+// With few rows the weights' bytes over HBM bound it, so all SMs have to stream: a tile's
+// blocks are split over the CTAs of a cluster, which add their sums through distributed
+// shared memory in rank order, so results do not depend on timing.
+#include <algorithm>
+#include <limits>
+
+#include "cache.cuh"
+#include "gemm_fp8.cuh"
+
+namespace mxk {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kBlock = 128;  // features of a scale
+
+struct GemmFp8Params {
+    int m, n, blocks;        // blocks: of k
+    int tiles_m;
+    const float* a_scales;   // [m][blocks]
+    const float* b_scales;   // [n / 128][blocks]
+    char* out;
+    int64_t out_stride;      // elements
+    int dtype, out_vec;      // out_vec: four elements can be stored at once
+    unsigned* err;
+};
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// The address of a CTA's shared memory in the window of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 cluster_ld4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr));
+    return v;
+}
+
+// Up to four elements of an output row.
+__device__ __forceinline__ void store_out(const GemmFp8Params& p, int row, int col, float4 v) {
+    const int64_t at = (int64_t)row * p.out_stride + col;
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    if (p.dtype == MXK_F32) {
+        float* o = reinterpret_cast<float*>(p.out) + at;
+        if (p.out_vec && col + 4 <= p.n)
+            *reinterpret_cast<float4*>(o) = v;
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + i < p.n) o[i] = x[i];
+        return;
+    }
+    uint16_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        h[i] = p.dtype == MXK_F16 ? __half_as_ushort(__float2half_rn(x[i])) : __bfloat16_as_ushort(__float2bfloat16_rn(x[i]));
+    uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + at;
+    if (p.out_vec && col + 4 <= p.n)
+        *reinterpret_cast<uint2*>(o) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (col + i < p.n) o[i] = h[i];
+}
+
+// ------------------------------------------------------------------ one tile a cluster
+
+namespace tile {
+
+constexpr int kM = 128, kN = 128;
+constexpr int kStages = 3, kBuffers = 2;
+constexpr int kSide = kM * kBlock;            // bytes of an operand's tile
+constexpr int kStage = 2 * kSide;
+constexpr int kSumWarps = 8, kLoadWarp = 8, kProductWarp = 9, kThreads = 320;
+constexpr int kCols = kN / 2;                 // columns of a warp: four lane quarters, two halves
+constexpr int kSmem = kStages * kStage + 1024;  // 1024: alignment
+static_assert(kN * kM * 4 <= kStages * kStage, "the sums go out through the operands' memory");
+
+struct Shared {
+    uint64_t full[kStages], done[kStages];  // loaded; multiplied, so the sums are in TMEM
+    uint64_t taken[kBuffers];               // a buffer's sums have been read
+    uint64_t drain;
+    int abort_word;
+    uint32_t tmem;
+};
+
+// A wait that goes on after an abort: for copies and products in flight.
+__device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
+    const long long start = clock64();
+    while (!dev::mbar_try_wait(bar, parity))
+        if (clock64() - start > dev::kWaitLimitCycles) break;
+}
+
+__global__ void __launch_bounds__(kThreads, 2)
+    gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                         const GemmFp8Params p, int split) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) Shared sh;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(kFull, tid >> 5, 0);
+    const int tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
+    const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
+    const int first = (int)((int64_t)rank * p.blocks / split), last = (int)((int64_t)(rank + 1) * p.blocks / split);
+    const int count = last - first;
+    volatile int* abort = &sh.abort_word;
+
+    if (tid == 0) {
+        sh.abort_word = 0;
+        for (int i = 0; i < kStages; ++i) dev::mbar_init(&sh.full[i], 1), dev::mbar_init(&sh.done[i], 1);
+        for (int i = 0; i < kBuffers; ++i) dev::mbar_init(&sh.taken[i], kSumWarps);
+        dev::mbar_init(&sh.drain, 1);
+        dev::fence_barrier_init();
+    }
+    if (warp == kProductWarp) dev::tmem_alloc(&sh.tmem, kBuffers * kN);
+    if (warp == kLoadWarp && lane == 0) dev::prefetch_tensor_map(&map_a), dev::prefetch_tensor_map(&map_b);
+    dev::tc_fence_before();
+    __syncthreads();
+    dev::tc_fence_after();
+    const uint32_t tmem = __shfl_sync(kFull, sh.tmem, 0);
+    dev::let_next_start();
+
+    float acc[kCols];
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) acc[i] = 0.0f;
+
+    if (warp == kLoadWarp) {
+        if (dev::elect_one()) {
+            // The weights are no output of the kernel before (which may be the quantiser).
+            const int early = min(count, kStages);
+            for (int i = 0; i < early; ++i) {
+                dev::mbar_arrive_expect_tx(&sh.full[i], kStage);
+                dev::tma_load_2d(smem + i * kStage + kSide, &map_b, (first + i) * kBlock, tn * kN, &sh.full[i]);
+            }
+            dev::wait_for_previous();
+            for (int i = 0; i < early; ++i)
+                dev::tma_load_2d(smem + i * kStage, &map_a, (first + i) * kBlock, tm * kM, &sh.full[i]);
+            int i = early, stage = 0;
+            uint32_t phase = 0;
+            for (; i < count; ++i) {
+                if (!dev::mbar_wait(&sh.done[stage], phase, abort, p.err)) break;
+                dev::mbar_arrive_expect_tx(&sh.full[stage], kStage);
+                dev::tma_load_2d(smem + stage * kStage + kSide, &map_b, (first + i) * kBlock, tn * kN, &sh.full[stage]);
+                dev::tma_load_2d(smem + stage * kStage, &map_a, (first + i) * kBlock, tm * kM, &sh.full[stage]);
+                if (++stage == kStages) stage = 0, phase ^= 1;
+            }
+            if (*abort)
+                for (int k = max(i - kStages, 0); k < i; ++k) settle(&sh.full[k % kStages], (uint32_t)(k / kStages) & 1u);
+        }
+        __syncwarp();
+    } else if (warp == kProductWarp) {
+        constexpr uint32_t idesc = dev::f16_idesc(kM, kN, false);
+        const uint64_t a_desc = dev::smem_desc(dev::smem_addr(smem), 16, 1024, dev::kLayoutSwizzle128);
+        int stage = 0, buffer = 0;
+        uint32_t phase = 0, taken_phase = 1;
+        bool ok = true;
+        for (int i = 0; i < count && ok; ++i) {
+            ok = __all_sync(kFull, dev::mbar_wait(&sh.taken[buffer], taken_phase, abort, p.err)) &&
+                 __all_sync(kFull, dev::mbar_wait(&sh.full[stage], phase, abort, p.err));
+            if (!ok) break;
+            dev::tc_fence_after();
+            if (dev::elect_one()) {
+                const uint64_t a = a_desc + (uint64_t)(stage * (kStage >> 4)), b = a + (kSide >> 4);
+#pragma unroll
+                for (int k = 0; k < kBlock / 32; ++k)
+                    dev::tc_mma_f8(tmem + buffer * kN, a + 2 * k, b + 2 * k, idesc, k > 0);
+                dev::tc_commit(&sh.done[stage]);
+            }
+            __syncwarp();
+            if (++stage == kStages) stage = 0, phase ^= 1;
+            if (++buffer == kBuffers) buffer = 0, taken_phase ^= 1;
+        }
+        if (!ok && dev::elect_one()) {  // products in flight must not outlive the CTA's memory
+            dev::tc_commit(&sh.drain);
+            settle(&sh.drain, 0);
+        }
+        __syncwarp();
+    } else {
+        const int row = tm * kM + (warp & 3) * 32 + lane;
+        const bool real = row < p.m;
+        const float* sa = p.a_scales + (int64_t)(real ? row : 0) * p.blocks + first;
+        const float* sb = p.b_scales + (int64_t)tn * p.blocks + first;
+        const uint32_t column = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * kCols;
+        dev::wait_for_previous();
+        float fa = 0.0f, fb = 0.0f;
+        if (count > 0) fa = real ? sa[0] : 0.0f, fb = __ldg(sb);
+        int stage = 0, buffer = 0;
+        uint32_t phase = 0;
+        for (int i = 0; i < count; ++i) {
+            const float f = fa * fb;
+            if (i + 1 < count) fa = real ? sa[i + 1] : 0.0f, fb = __ldg(sb + i + 1);
+            if (!__all_sync(kFull, dev::mbar_wait(&sh.done[stage], phase, abort, p.err))) break;
+            dev::tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < kCols; c += 16) {
+                uint32_t v[16];
+                dev::tmem_ld_32x32b_x16(column + buffer * kN + c, v);
+                dev::tmem_wait_ld();
+                if (c + 16 == kCols) {
+                    dev::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) dev::mbar_arrive(&sh.taken[buffer]);
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) acc[c + k] = fmaf(__uint_as_float(v[k]), f, acc[c + k]);
+            }
+            if (++stage == kStages) stage = 0, phase ^= 1;
+            if (++buffer == kBuffers) buffer = 0;
+        }
+        // All products have read their operands: the sums take that memory, a row's 16-byte
+        // chunks permuted so that eight rows' chunks lie in different banks.
+        const int r = (warp & 3) * 32 + lane;
+        if (real) {
+#pragma unroll
+            for (int c = 0; c < kCols / 4; ++c)
+                *reinterpret_cast<float4*>(smem + r * (kN * 4) + ((((warp >> 2) * (kCols / 4) + c) ^ (r & 7)) << 4)) =
+                    make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+        }
+    }
+    if (split > 1)
+        cluster_arrive(), cluster_wait();
+    else
+        __syncthreads();
+    // The cluster's sums, each CTA its part of the tile's rows and chunks.
+    const int rows = min(p.m - tm * kM, kM), total = rows * (kN / 4);
+    const uint32_t sums = dev::smem_addr(smem);
+    const int end = (int)((int64_t)(rank + 1) * total / split);
+    for (int i = (int)((int64_t)rank * total / split) + tid; i < end; i += kThreads) {
+        const int r = i >> 5, c = i & 31;
+        if (tn * kN + 4 * c >= p.n) continue;
+        const uint32_t at = sums + r * (kN * 4) + ((c ^ (r & 7)) << 4);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < split; ++k) {
+            const float4 x = cluster_ld4(in_cta(at, k));
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+        store_out(p, tm * kM + r, tn * kN + 4 * c, v);
+    }
+    dev::tc_fence_before();
+    if (split > 1)
+        cluster_arrive(), cluster_wait();  // nobody leaves while its sums are read
+    else
+        __syncthreads();
+    dev::tc_fence_after();
+    if (warp == kProductWarp) dev::tmem_dealloc(tmem, kBuffers * kN);
+}
+
+int launch(const GemmFp8& g, GemmFp8Params p, bool follows, cudaStream_t stream) {
+    CUtensorMap map_a, map_b;
+    MXK_CHECK(encode_tensor_map_2d(&map_a, g.a, (uint64_t)g.k, (uint64_t)g.m, (uint64_t)g.k, kBlock, kM,
+                                   CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
+    MXK_CHECK(encode_tensor_map_2d(&map_b, g.b, (uint64_t)g.k, (uint64_t)g.n, (uint64_t)g.k, kBlock, kN,
+                                   CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
+    static thread_local int ready_device = -1;
+    int dev = 0;
+    MXK_CUDA(cudaGetDevice(&dev));
+    if (ready_device != dev) {
+        MXK_CUDA(cudaFuncSetAttribute(gemm_fp8_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        ready_device = dev;
+    }
+    static const int sms = sm_count();
+    p.tiles_m = (p.m + kM - 1) / kM;
+    const int64_t tiles = (int64_t)p.tiles_m * ((p.n + kN - 1) / kN);
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= 2 * sms && p.blocks >= 4 * split) split *= 2;
+    MXK_REQUIRE(tiles * split <= std::numeric_limits<int>::max(), "gemm_fp8: too much work for one call");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(tiles * split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = follows ? 2 : 1;
+    LaunchScope scope("gemm_fp8", stream);
+    MXK_CUDA(cudaLaunchKernelEx(&cfg, gemm_fp8_tile_kernel, map_a, map_b, p, split));
+    return MXK_OK;
+}
+
+}  // namespace tile
+
+int check_product(const char* who, int dtype, int64_t m, int64_t n, int64_t k, const void* b, const float* b_scales,
+                  const void* out) {
+    const std::string w(who);
+    MXK_REQUIRE(dtype == MXK_F32 || dtype == MXK_F16 || dtype == MXK_BF16, w + ": unknown dtype");
+    MXK_REQUIRE(m >= 0 && n >= 0 && k >= 0 && k % 16 == 0, w + ": k must be a multiple of 16, sizes not negative");
+    MXK_REQUIRE(m < (1ll << 30) && n < (1ll << 30) && k < (1ll << 30), w + ": sizes must be below 2^30");
+    if (m == 0 || n == 0) return MXK_OK;
+    MXK_REQUIRE(out, w + ": out must be non-null");
+    MXK_REQUIRE(reinterpret_cast<uintptr_t>(out) % (dtype == MXK_F32 ? 4 : 2) == 0, w + ": out must be aligned to its elements");
+    if (k == 0) return MXK_OK;
+    MXK_REQUIRE(b && b_scales, w + ": an operand is null");
+    MXK_REQUIRE(reinterpret_cast<uintptr_t>(b) % 16 == 0 && reinterpret_cast<uintptr_t>(b_scales) % 4 == 0,
+                w + ": operands must be aligned to 16 bytes, scales to 4");
+    return MXK_OK;
+}
+
+int gemm_fp8(const GemmFp8& g, bool follows, cudaStream_t stream) {
+    const int size = g.dtype == MXK_F32 ? 4 : 2;
+    GemmFp8Params p{};
+    p.m = (int)g.m, p.n = (int)g.n;
+    p.blocks = (int)((g.k + kBlock - 1) / kBlock);
+    p.a_scales = g.a_scales, p.b_scales = g.b_scales;
+    p.out = static_cast<char*>(g.out);
+    p.out_stride = g.out_stride;
+    p.dtype = g.dtype;
+    p.out_vec = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % (4 * size) == 0;
+    p.err = device_error_word();
+    if (!p.err) return fail(MXK_ERR_CUDA, "gemm_fp8: cannot allocate the device error word");
+    return tile::launch(g, p, follows, stream);
+}
+
+// Products of no features.
+int zero_out(const GemmFp8& g, cudaStream_t stream) {
+    const size_t size = g.dtype == MXK_F32 ? 4 : 2;
+    MXK_CUDA(cudaMemset2DAsync(g.out, (size_t)g.out_stride * size, 0, (size_t)g.n * size, (size_t)g.m, stream));
+    return MXK_OK;
+}
+
+}  // namespace
+}  // namespace mxk
+
+extern "C" {
+
+int mxk_gemm_fp8(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, const float* a_scales, const uint8_t* b,
+                 const float* b_scales, void* out, int64_t out_stride, void* stream) {
+    using namespace mxk;
+    MXK_CHECK(check_product("gemm_fp8", dtype, m, n, k, b, b_scales, out));
+    MXK_REQUIRE(out_stride >= n, "gemm_fp8: out_stride must be at least n");
+    if (m == 0 || n == 0) return MXK_OK;
+    const GemmFp8 g{dtype, m, n, k, a, a_scales, b, b_scales, out, out_stride};
+    if (k == 0) return zero_out(g, as_stream(stream));
+    MXK_REQUIRE(a && a_scales, "gemm_fp8: an operand is null");
+    MXK_REQUIRE(reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(a_scales) % 4 == 0,
+                "gemm_fp8: operands must be aligned to 16 bytes, scales to 4");
+    return gemm_fp8(g, false, as_stream(stream));
+}
+
+int mxk_linear_fp8(int dtype, int64_t m, int64_t n, int64_t k, const void* x, int64_t x_stride, const uint8_t* b,
+                   const float* b_scales, void* out, int64_t out_stride, void* stream) {
+    using namespace mxk;
+    MXK_CHECK(check_product("linear_fp8", dtype, m, n, k, b, b_scales, out));
+    MXK_REQUIRE(out_stride >= n, "linear_fp8: out_stride must be at least n");
+    if (m == 0 || n == 0) return MXK_OK;
+    GemmFp8 g{dtype, m, n, k, nullptr, nullptr, b, b_scales, out, out_stride};
+    const cudaStream_t st = as_stream(stream);
+    if (k == 0) return zero_out(g, st);
+    MXK_REQUIRE(x && reinterpret_cast<uintptr_t>(x) % (dtype == MXK_F32 ? 4 : 2) == 0,
+                "linear_fp8: x must be non-null and aligned to its elements");
+    const int64_t blocks = (k + kBlock - 1) / kBlock;
+    const size_t values = ((size_t)m * k + 255) / 256 * 256;
+    cudaMemPool_t pool = workspace_pool();
+    if (!pool) return fail(MXK_ERR_CUDA, "linear_fp8: cannot create the workspace pool");
+    void* work = nullptr;
+    MXK_CUDA(cudaMallocFromPoolAsync(&work, values + (size_t)m * blocks * 4, pool, st));
+    uint8_t* a = static_cast<uint8_t*>(work);
+    float* scales = reinterpret_cast<float*>(a + values);
+    g.a = a, g.a_scales = scales;
+    int status = launch_quantize_fp8({dtype, 1, m, k, x, x_stride, a, scales}, st);
+    if (status == MXK_OK) status = gemm_fp8(g, true, st);
+    const cudaError_t freed = cudaFreeAsync(work, st);
+    MXK_CHECK(status);
+    MXK_CUDA(freed);
+    return MXK_OK;
+}
+
+}  // extern "C"

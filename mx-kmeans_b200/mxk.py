@@ -130,6 +130,9 @@ SIGNATURES = {
     "mxk_cache_read": ([_P, _I, _I64, _P, _P, _P, _P], _I),
     "mxk_cache_append": ([_P, _P, _P], _I),
     "mxk_cache_attention": ([_P, _P, _P], _I),
+    "mxk_quantize_fp8": ([_I, _I64, _I64, _P, _I64, _I, _P, _P, _P], _I),
+    "mxk_gemm_fp8": ([_I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P], _I),
+    "mxk_linear_fp8": ([_I, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _P], _I),
     "mxk_profile_enable": ([_I], _I),
     "mxk_profile_read": ([ctypes.POINTER(KernelStat), _I, ctypes.POINTER(_I)], _I),
 }
@@ -534,6 +537,86 @@ def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, sca
                      cache.head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, outr,
                      None if lse is None else _vector(lse, "lse", cache, _torch.float32, tokens, heads))
     check(load().mxk_cache_attention(cache.handle, ctypes.byref(args), _launch_stream(cache, stream)))
+
+
+# ----------------------------------------------------------------------------- E4M3 products
+
+def _matrix(t, name, dtype, index):
+    """(address, row stride) of a matrix on cuda:index whose rows are contiguous."""
+    if t.dim() != 2 or t.dtype != dtype or t.get_device() != index or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise _bad(f"{name}: {dtype} rows on cuda:{index} are needed, got {t.device} {t.dtype} {tuple(t.shape)} with "
+                   f"strides {t.stride()}")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]  # (one row may have any stride)
+
+
+def _whole(t, name, dtype, index, *shape):
+    """Address of a contiguous tensor of `shape` on cuda:index.  Its elements may be bytes or
+    torch.float8_e4m3fn where dtype is uint8."""
+    if (t.dtype != dtype and (dtype != _torch.uint8 or t.dtype != _torch.float8_e4m3fn)) or tuple(t.shape) != shape or \
+            t.get_device() != index or not t.is_contiguous():
+        raise _bad(f"{name}: a contiguous {dtype} tensor of shape {shape} on cuda:{index} is needed, got {t.device} "
+                   f"{t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _device_of(t, name):
+    """Index of t's device, which must be the current one."""
+    if _torch is None:
+        _setup()
+    index = t.get_device()
+    if index < 0 or _torch._C._cuda_getDevice() != index:
+        raise _bad(f"{name} must lie on the current GPU, is on {t.device}")
+    return index
+
+
+def _stream_on(index, stream):
+    return stream.cuda_stream if stream is not None else _torch._C._cuda_getCurrentRawStream(index)
+
+
+def quantize_fp8(x, values, scales, block_rows=1, stream=None):
+    """E4M3 values (uint8 or float8_e4m3fn [rows, k]) and float32 scales [rows / block_rows,
+    k / 128] (rounded up) of the rows of x (mxk.h, mxk_quantize_fp8); block_rows 1 or 128."""
+    index = _device_of(x, "x")
+    code = _DTYPES.get(x.dtype)
+    if code is None or block_rows not in (1, 128):
+        raise _bad("x: float32, float16 or bfloat16 is needed; block_rows is 1 or 128")
+    at, stride = _matrix(x, "x", x.dtype, index)
+    rows, k = x.shape
+    check(load().mxk_quantize_fp8(code, rows, k, at, stride, block_rows, _whole(values, "values", _torch.uint8, index, rows, k),
+                                  _whole(scales, "scales", _torch.float32, index, -(-rows // block_rows), -(-k // 128)),
+                                  _stream_on(index, stream)))
+
+
+def gemm_fp8(a, a_scales, b, b_scales, out, stream=None):
+    """out [m, n] (float32, float16 or bfloat16 rows) = a [m, k] times b [n, k] transposed, E4M3
+    with scales per row (a) or 128 rows (b) and 128 features (mxk.h, mxk_gemm_fp8)."""
+    index = _device_of(out, "out")
+    code = _DTYPES.get(out.dtype)
+    if code is None or out.dim() != 2 or a.dim() != 2:
+        raise _bad("out: a matrix of float32, float16 or bfloat16 is needed; a has 2 dimensions")
+    at, stride = _matrix(out, "out", out.dtype, index)
+    (m, n), k = out.shape, a.shape[1]
+    blocks = -(-k // 128)
+    check(load().mxk_gemm_fp8(code, m, n, k, _whole(a, "a", _torch.uint8, index, m, k),
+                              _whole(a_scales, "a_scales", _torch.float32, index, m, blocks),
+                              _whole(b, "b", _torch.uint8, index, n, k),
+                              _whole(b_scales, "b_scales", _torch.float32, index, -(-n // 128), blocks), at,
+                              stride, _stream_on(index, stream)))
+
+
+def linear_fp8(x, b, b_scales, out, stream=None):
+    """out [m, n] = x [m, k] times b [n, k] transposed: quantize_fp8 of x's rows and gemm_fp8 in
+    one call (mxk.h, mxk_linear_fp8); x and out have the same type."""
+    index = _device_of(out, "out")
+    code = _DTYPES.get(out.dtype)
+    if code is None or out.dim() != 2 or x.dim() != 2 or x.shape[0] != out.shape[0]:
+        raise _bad("x and out: matrices of as many rows, of one of float32, float16 and bfloat16, are needed")
+    xa, x_stride = _matrix(x, "x", out.dtype, index)
+    at, stride = _matrix(out, "out", out.dtype, index)
+    (m, n), k = out.shape, x.shape[1]
+    check(load().mxk_linear_fp8(code, m, n, k, xa, x_stride, _whole(b, "b", _torch.uint8, index, n, k),
+                                _whole(b_scales, "b_scales", _torch.float32, index, -(-n // 128), -(-k // 128)), at,
+                                stride, _stream_on(index, stream)))
 
 
 def profile_enable(on=True):
