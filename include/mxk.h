@@ -422,6 +422,28 @@ typedef struct {
 } mxk_attention;
 int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* args, void* stream);
 
+/* mxk_cache_attention of a batch in which groups of sequences begin with the same tokens, which
+ * are read once for the group.  Sequences cu_groups[g] .. cu_groups[g + 1] - 1 are group g
+ * (groups may not overlap; a sequence may belong to none); the first prefix_lens[g] tokens of
+ * all of them that have query tokens lie in the same slots (pages: their page table rows begin
+ * alike).  The result is that of mxk_cache_attention, but for rounding, whatever the lengths
+ * are: a group shares what comes before the first query token of any of its sequences, in
+ * multiples of 128 tokens (so up to 127 tokens of a prefix are read by each), and one sequence
+ * by itself shares nothing.
+ *
+ * cu_groups (groups + 1), prefix_lens: int32 on the device.  max_prefix: a bound on the prefixes
+ * known to the host; longer ones are shared up to it.  args->window must be 0, tokens * heads
+ * below 2^30.  Besides mxk_cache_attention's, whose limits count a group's prefix as a sequence
+ * of its rows, the call takes tokens * heads * (head_dim + 1) * 8 bytes of workspace. */
+typedef struct {
+    int groups;
+    const int* cu_groups;
+    const int* prefix_lens;
+    int64_t max_prefix;
+} mxk_prefixes;
+int mxk_cache_attention_shared(const mxk_cache* cache, const mxk_attention* args, const mxk_prefixes* prefixes,
+                               void* stream);
+
 /* ---- E4M3 rows with float32 scales, and their products (no counterpart in the reference) ---- */
 
 /* Quantises `rows` rows of k features (dtype MXK_F32, MXK_F16 or MXK_BF16, contiguous,

@@ -191,10 +191,10 @@ __device__ __forceinline__ uint32_t share_bits(int k) {
     }
 }
 
-template <int D, int BITS>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(const AttentionParams p) {
+template <int D, int BITS, class P>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(const P p) {
     using S = Stage<D, BITS>;
-    using P = Pitch<D, BITS>;
+    using Row = Pitch<D, BITS>;
     constexpr int kSteps = D / 16;       // k-steps of q . k
     constexpr int kTiles = D / 8;        // 8-feature tiles of the output
     constexpr int kShare = S::row / 4;   // bytes of a key row a lane reads
@@ -212,35 +212,35 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     // cache, and a constant further here where rows lie without gaps or 32 pieces fill rows.
     constexpr int kPieces = kGranule * S::chunks;  // of a side
     constexpr int kCopies = (kPieces + 31) / 32;
-    constexpr int kStep = P::k == S::row ? 512 : 32 / S::chunks * P::k;
-    constexpr int vStep = P::v == S::row ? 512 : 32 / S::chunks * P::v;
-    static_assert(P::k == S::row || 32 % S::chunks == 0, "key rows without gaps, or whole rows in a copy");
-    constexpr bool vEven = P::v == S::row || 32 % S::chunks == 0;
-    constexpr int kPlaces = P::swizzled ? 2 : 1;               // rows of copy i: lane / 8 + 4 i
-    constexpr int vPlaces = P::swizzled ? 2 : (vEven ? 1 : kCopies);
+    constexpr int kStep = Row::k == S::row ? 512 : 32 / S::chunks * Row::k;
+    constexpr int vStep = Row::v == S::row ? 512 : 32 / S::chunks * Row::v;
+    static_assert(Row::k == S::row || 32 % S::chunks == 0, "key rows without gaps, or whole rows in a copy");
+    constexpr bool vEven = Row::v == S::row || 32 % S::chunks == 0;
+    constexpr int kPlaces = Row::swizzled ? 2 : 1;               // rows of copy i: lane / 8 + 4 i
+    constexpr int vPlaces = Row::swizzled ? 2 : (vEven ? 1 : kCopies);
     uint32_t k_lane[kPlaces], v_lane[vPlaces];
-    if constexpr (P::swizzled) {
+    if constexpr (Row::swizzled) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             k_lane[i] = ring + (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) + 4 * i)) << 4);
             v_lane[i] = k_lane[i] + S::v_at;
         }
     } else {
-        k_lane[0] = ring + (P::k == S::row ? lane * 16 : lane / S::chunks * P::k + lane % S::chunks * 16);
+        k_lane[0] = ring + (Row::k == S::row ? lane * 16 : lane / S::chunks * Row::k + lane % S::chunks * 16);
 #pragma unroll
         for (int i = 0; i < vPlaces; ++i) {
             const int x = lane + 32 * i;
-            v_lane[i] = ring + S::v_at + (P::v == S::row ? lane * 16 : x / S::chunks * P::v + x % S::chunks * 16);
+            v_lane[i] = ring + S::v_at + (Row::v == S::row ? lane * 16 : x / S::chunks * Row::v + x % S::chunks * 16);
         }
     }
-    static_assert(P::k % widest(kShare) == 0 && P::v % widest(vShare) == 0 && S::v_at % 16 == 0 && S::granule % 16 == 0,
+    static_assert(Row::k % widest(kShare) == 0 && Row::v % widest(vShare) == 0 && S::v_at % 16 == 0 && S::granule % 16 == 0,
                   "reads are aligned to their width");
     // Where this lane reads: 16-byte halves of its key share; its even and odd tokens' values.
     uint32_t k_read[2], v_read[2];
-    k_read[0] = ring + g * P::k + (P::swizzled ? (2 * c ^ g) << 4 : c * kShare);
-    k_read[1] = ring + g * P::k + ((2 * c + 1) ^ g) * 16;  // swizzled rows only
-    v_read[0] = ring + S::v_at + 2 * c * P::v + (P::swizzled ? (g ^ 2 * c) << 4 : g * vShare);
-    v_read[1] = ring + S::v_at + (2 * c + 1) * P::v + (P::swizzled ? (g ^ (2 * c + 1)) << 4 : g * vShare);
+    k_read[0] = ring + g * Row::k + (Row::swizzled ? (2 * c ^ g) << 4 : c * kShare);
+    k_read[1] = ring + g * Row::k + ((2 * c + 1) ^ g) * 16;  // swizzled rows only
+    v_read[0] = ring + S::v_at + 2 * c * Row::v + (Row::swizzled ? (g ^ 2 * c) << 4 : g * vShare);
+    v_read[1] = ring + S::v_at + (2 * c + 1) * Row::v + (Row::swizzled ? (g ^ (2 * c + 1)) << 4 : g * vShare);
     const uint32_t ks_read = ring + S::ks_at + g * S::scale_bytes + (D == 128 ? c : c >> 1);
     const uint32_t vs_read = ring + S::vs_at + 2 * c * S::scale_bytes + (D == 128 ? g >> 1 : g >> 2);
 
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         dev::wait_for_previous();
         return;
     }
-    dev::Walk w = dev::walk_to<kRows, kKeys>(p, share);
+    dev::Walk<P> w = dev::walk_to<kRows, kKeys>(p, share);
     int left = share.tiles - w.skip;
     bool open = false;
 
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         const int pair0 = (w.first + tile0) * kWarps + warp;
         const int end = min((w.first + tile0 + tiles) * kWarps, any_hi <= any_lo ? 0 : (any_hi + kPair - 1) / kPair);
         const int steps = end > pair0 ? (end - pair0 + kWarps - 1) / kWarps : 0;
-        const int* table = p.page_table + (int64_t)w.seq * p.table_stride;
+        const int* table = dev::table_of(p, w.seq);
         const int per_page = p.page_size / kGranule;
         // pages and granules from a step's first granule to the next step's
         const int jump = kWarps * kGranules / per_page, rest = kWarps * kGranules - jump * per_page;
@@ -323,8 +323,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         auto copy_piece = [&](auto index, auto granule, const uint8_t* k, const uint8_t* v, int valid) {
             constexpr int i = decltype(index)::value, at = decltype(granule)::value * S::granule;
             if (i < kCopies && (kPieces % 32 == 0 || lane + 32 * i < kPieces)) {
-                const uint32_t to_k = k_lane[P::swizzled ? i & 1 : 0] + copy_stage;
-                const uint32_t to_v = v_lane[P::swizzled ? i & 1 : (vEven ? 0 : i)] + copy_stage;
+                const uint32_t to_k = k_lane[Row::swizzled ? i & 1 : 0] + copy_stage;
+                const uint32_t to_v = v_lane[Row::swizzled ? i & 1 : (vEven ? 0 : i)] + copy_stage;
                 constexpr int v_off = at + (vEven ? i * vStep : 0);
                 if (valid >= kGranule) {
                     copy16<at + i * kStep, 512 * i>(to_k, k);
@@ -494,9 +494,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                 if (__any_sync(kFull, k_least < kref - kKeyLift - kExactDown<BITS>)) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t at = now + (i >> 1) * S::granule + (i & 1) * (8 * P::k);
+                        const uint32_t at = now + (i >> 1) * S::granule + (i & 1) * (8 * Row::k);
                         uint32_t words[(kShare + 3) / 4], any = 0;
-                        if constexpr (P::swizzled)
+                        if constexpr (Row::swizzled)
                             lds_bytes<16, 0>(k_read[0] + at, words), lds_bytes<16, 0>(k_read[1] + at, words + 4);
                         else
                             lds_bytes<kShare, 0>(k_read[0] + at, words);
@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                 if (top - low > most || (top == kScaleOfZeros && low == kScaleOfZeros)) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const uint32_t at = v_read[i & 1] + now + (i >> 2) * S::granule + ((i >> 1) & 1) * (8 * P::v);
+                        const uint32_t at = v_read[i & 1] + now + (i >> 2) * S::granule + ((i >> 1) & 1) * (8 * Row::v);
                         uint32_t words[(vShare + 3) / 4], any = 0;
                         lds_bytes<vShare, 0>(at, words);
 #pragma unroll
@@ -564,13 +564,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                 for (int h = 0; h < 2; ++h) {
                     uint32_t key_words[2][(kShare + 3) / 4];
                     const uint32_t at = now + h * S::granule;
-                    if constexpr (P::swizzled) {
+                    if constexpr (Row::swizzled) {
                         lds_bytes<16, 0>(k_read[0] + at, key_words[0]), lds_bytes<16, 0>(k_read[1] + at, key_words[0] + 4);
-                        lds_bytes<16, 8 * P::k>(k_read[0] + at, key_words[1]);
-                        lds_bytes<16, 8 * P::k>(k_read[1] + at, key_words[1] + 4);
+                        lds_bytes<16, 8 * Row::k>(k_read[0] + at, key_words[1]);
+                        lds_bytes<16, 8 * Row::k>(k_read[1] + at, key_words[1] + 4);
                     } else {
                         lds_bytes<kShare, 0>(k_read[0] + at, key_words[0]);
-                        lds_bytes<kShare, 8 * P::k>(k_read[0] + at, key_words[1]);
+                        lds_bytes<kShare, 8 * Row::k>(k_read[0] + at, key_words[1]);
                     }
                     const int e0 = ks[2 * h] - kref + kKeyLift, e1 = ks[2 * h + 1] - kref + kKeyLift;
                     const uint32_t kf[2] = {pow2_f16x2(e0, e0), pow2_f16x2(e1, e1)};
@@ -675,8 +675,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                     uint32_t vw[4][(vShare + 3) / 4];
                     lds_bytes<vShare, 0>(v_read[0] + at, vw[0]);
                     lds_bytes<vShare, 0>(v_read[1] + at, vw[1]);
-                    lds_bytes<vShare, 8 * P::v>(v_read[0] + at, vw[2]);
-                    lds_bytes<vShare, 8 * P::v>(v_read[1] + at, vw[3]);
+                    lds_bytes<vShare, 8 * Row::v>(v_read[0] + at, vw[2]);
+                    lds_bytes<vShare, 8 * Row::v>(v_read[1] + at, vw[3]);
                     const uint32_t f0 = pow2_f16x2(vs[4 * h] - ref, vs[4 * h + 1] - ref);
                     const uint32_t f1 = pow2_f16x2(vs[4 * h + 2] - ref, vs[4 * h + 3] - ref);
                     bool nans = false;
@@ -744,8 +744,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
 #pragma unroll
                                     for (int e = 0; e < 2; ++e) {
                                         const int byte = (2 * c + e) * vShare + n;
-                                        const int in_row = P::swizzled ? (((byte >> 4) ^ (t & 7)) << 4) + (byte & 15) : byte;
-                                        if ((lds_u8<0>(ring + at + S::v_at + t * P::v + in_row) & 0x7f) == 0x7f)
+                                        const int in_row = Row::swizzled ? (((byte >> 4) ^ (t & 7)) << 4) + (byte & 15) : byte;
+                                        if ((lds_u8<0>(ring + at + S::v_at + t * Row::v + in_row) & 0x7f) == 0x7f)
                                             o[n][2 * i + e] = __int_as_float(0x7fc00000);
                                     }
                             }
@@ -857,9 +857,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             if (whole) {
                 const int row = w.rt * kRows + r, j = row / p.group;
                 const int head = w.head * p.group + (row - j * p.group);
-                dev::store4(p, w.view.row0 + j, head, chunk * 4, v);
-                if (p.lse && chunk == 0)
-                    p.lse[(int64_t)(w.view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
+                const int64_t to = dev::out_row(p, w.view) + j;
+                dev::store4(p, to, head, chunk * 4, v);
+                if (p.lse && chunk == 0) p.lse[to * p.heads + head] = dev::row_lse(top, total);
             } else {
                 reinterpret_cast<float4*>(p.part + (slot * kRows + r) * D)[chunk] = v;
                 if (chunk == 0) p.part_stat[slot * kRows + r] = make_float2(top, total);
@@ -879,67 +879,92 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     dev::wait_for_previous();
 }
 
-template <int D, int BITS>
-int launch_rows(AttentionParams p, int64_t most_tiles, int64_t most_rows, AttentionCall& call) {
+template <int D, int BITS, class P>
+int launch_rows(P p, int64_t most_tiles, int64_t most_rows, AttentionCall<P>& call) {
     using S = Stage<D, BITS>;
     static thread_local int ready_device = -1;
     int dev = 0;
     MXK_CUDA(cudaGetDevice(&dev));
     if (ready_device != dev) {
-        MXK_CUDA(cudaFuncSetAttribute(attention_rows_kernel<D, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        MXK_CUDA(cudaFuncSetAttribute(attention_rows_kernel<D, BITS, P>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       S::smem));
         ready_device = dev;
     }
     static const int sms = sm_count();
     const int64_t ctas = std::min<int64_t>(most_tiles, kCtasPerSm * sms);
     MXK_CHECK(call.take(p, ctas, kRows, D));
-    MXK_CHECK(call.launch("attention_rows", attention_rows_kernel<D, BITS>, (unsigned)ctas, kThreads, S::smem, p));
+    MXK_CHECK(call.launch("attention_rows", attention_rows_kernel<D, BITS, P>, (unsigned)ctas, kThreads, S::smem, p));
     call.join_later(p, ctas, kRows, std::min<int64_t>(most_rows, kRows));
     return MXK_OK;
 }
 
-template <int D>
-int launch_rows_bits(int bits, const AttentionParams& p, int64_t most_tiles, int64_t most_rows, AttentionCall& call) {
+template <int D, class P>
+int launch_rows_bits(int bits, const P& p, int64_t most_tiles, int64_t most_rows, AttentionCall<P>& call) {
     if (bits == 8) return launch_rows<D, 8>(p, most_tiles, most_rows, call);
     if (bits == 6) return launch_rows<D, 6>(p, most_tiles, most_rows, call);
     return launch_rows<D, 4>(p, most_tiles, most_rows, call);
 }
 
 }  // namespace
-}  // namespace mxk
 
-extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* a, void* stream) {
-    using namespace mxk;
-    MXK_CHECK(check_cache(cache, "cache_attention"));
-    MXK_REQUIRE(a, "cache_attention: args is null");
-    MXK_REQUIRE(a->dtype == MXK_F16 || a->dtype == MXK_BF16, "cache_attention: dtype must be MXK_F16 or MXK_BF16");
+template <class P>
+int launch_attention(const mxk_cache& cache, P p, int max_rows, AttentionCall<P>& call) {
+    // Sequences with few rows per key head go to the rows kernel, the others to the
+    // tiles kernel; a single sequence has one kernel chosen by its bound, several are
+    // sorted by the kernels themselves.
+    const int64_t rows = (int64_t)std::max(p.max_q, max_rows) * p.group;
+    const bool many = rows > kMostFewRows;
+    if (many) {
+        P q = p;
+        if (p.seqs > 1) q.min_rows = kMostFewRows + 1;
+        MXK_CHECK(launch_attention_tiles(cache.bits, cache.head_dim, q, p.max_q, max_rows, call));
+        p.max_rows = kMostFewRows;
+    }
+    if (!many || p.seqs > 1) {
+        const int64_t few = std::min<int64_t>(rows, kMostFewRows);
+        const int few_q = (int)((few + p.group - 1) / p.group);
+        const int64_t most = attention_tile_bound(p, few_q, few_q, kRows, kKeys);
+        MXK_REQUIRE(most <= std::numeric_limits<int>::max() / (1 + kUnitCost), "cache_attention: too much work for one call");
+        MXK_CHECK(cache.head_dim == 128 ? launch_rows_bits<128>(cache.bits, p, most, few, call)
+                                        : launch_rows_bits<64>(cache.bits, p, most, few, call));
+    }
+    return call.join_all(cache.head_dim);
+}
+template int launch_attention(const mxk_cache&, AttentionParams, int, AttentionCall<AttentionParams>&);
+template int launch_attention(const mxk_cache&, SharedParams, int, AttentionCall<SharedParams>&);
+
+int check_attention(const char* who, const mxk_cache* cache, const mxk_attention* a, AttentionParams& p) {
+    const std::string name(who);
+    p.tokens = 0;
+    MXK_CHECK(check_cache(cache, who));
+    MXK_REQUIRE(a, name + ": args is null");
+    MXK_REQUIRE(a->dtype == MXK_F16 || a->dtype == MXK_BF16, name + ": dtype must be MXK_F16 or MXK_BF16");
     MXK_REQUIRE(a->heads >= 1 && a->heads <= 65535 && a->heads % cache->kv_heads == 0,
-                "cache_attention: heads must be a positive multiple of the cache's kv_heads");
+                name + ": heads must be a positive multiple of the cache's kv_heads");
     MXK_REQUIRE(a->tokens >= 0 && a->tokens <= std::numeric_limits<int>::max() / 2 && a->seqs >= 0,
-                "cache_attention: tokens must be in [0, 2^30), seqs in [0, 2^31)");
-    MXK_REQUIRE(a->max_q >= 0 && a->max_kv >= 0, "cache_attention: max_q and max_kv must not be negative");
+                name + ": tokens must be in [0, 2^30), seqs in [0, 2^31)");
+    MXK_REQUIRE(a->max_q >= 0 && a->max_kv >= 0, name + ": max_q and max_kv must not be negative");
     MXK_REQUIRE((int64_t)a->max_q * a->heads <= std::numeric_limits<int>::max() / 2 &&
                     a->max_kv <= std::numeric_limits<int>::max() / 2,
-                "cache_attention: max_q * heads and max_kv must be below 2^30");
-    MXK_REQUIRE(a->window >= 0 && (a->window == 0 || a->causal), "cache_attention: a window needs causal");
-    MXK_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, "cache_attention: scale must be finite");
+                name + ": max_q * heads and max_kv must be below 2^30");
+    MXK_REQUIRE(a->window >= 0 && (a->window == 0 || a->causal), name + ": a window needs causal");
+    MXK_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, name + ": scale must be finite");
     if (cache->head_dim != 64 && cache->head_dim != 128)
-        return fail(MXK_ERR_UNSUPPORTED, "cache_attention: head_dim must be 64 or 128");
+        return fail(MXK_ERR_UNSUPPORTED, name + ": head_dim must be 64 or 128");
     // (The kernels number the cache's rows in 32 bits.)
     if (cache->pages * cache->kv_heads > (1ll << 32) / cache->page_size)
-        return fail(MXK_ERR_UNSUPPORTED, "cache_attention: pages * kv_heads * page_size must be at most 2^32");
+        return fail(MXK_ERR_UNSUPPORTED, name + ": pages * kv_heads * page_size must be at most 2^32");
     if (a->tokens == 0 || a->seqs == 0 || a->max_q == 0) return MXK_OK;
     MXK_REQUIRE(a->q.data && a->out.data && a->cu_q && (a->page_table || a->max_kv == 0) && a->kv_lens,
-                "cache_attention: q, out, cu_q, page_table and kv_lens must be non-null");
+                name + ": q, out, cu_q, page_table and kv_lens must be non-null");
     MXK_REQUIRE((reinterpret_cast<uintptr_t>(a->q.data) | reinterpret_cast<uintptr_t>(a->out.data)) % 2 == 0 &&
                     (reinterpret_cast<uintptr_t>(a->cu_q) | reinterpret_cast<uintptr_t>(a->page_table) |
                      reinterpret_cast<uintptr_t>(a->kv_lens) | reinterpret_cast<uintptr_t>(a->lse)) % 4 == 0,
-                "cache_attention: pointers must be aligned to their elements");
+                name + ": pointers must be aligned to their elements");
     const int64_t need = (a->max_kv + cache->page_size - 1) / cache->page_size;
     MXK_REQUIRE(a->seqs == 1 || a->page_table_stride >= need,
-                "cache_attention: page_table_stride is below the pages of max_kv tokens");
+                name + ": page_table_stride is below the pages of max_kv tokens");
 
-    AttentionParams p{};
     p.k_values = static_cast<const uint8_t*>(cache->k_values);
     p.v_values = static_cast<const uint8_t*>(cache->v_values);
     p.k_scales = cache->k_scales;
@@ -972,24 +997,16 @@ extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* 
     p.min_rows = 1;
     p.max_rows = std::numeric_limits<int>::max();
 
-    // Sequences with few rows per key head go to the rows kernel, the others to the
-    // tiles kernel; a single sequence has one kernel chosen by its bound, several are
-    // sorted by the kernels themselves.
-    AttentionCall call(as_stream(stream));
-    const int64_t rows = (int64_t)p.max_q * p.group;
-    const bool many = rows > kMostFewRows;
-    if (many) {
-        AttentionParams q = p;
-        if (a->seqs > 1) q.min_rows = kMostFewRows + 1;
-        MXK_CHECK(launch_attention_tiles(cache->bits, cache->head_dim, q, p.max_q, call));
-        p.max_rows = kMostFewRows;
-    }
-    if (!many || a->seqs > 1) {
-        const int64_t few = std::min<int64_t>(rows, kMostFewRows);
-        const int64_t most = attention_tile_bound(p, (int)((few + p.group - 1) / p.group), kRows, kKeys);
-        MXK_REQUIRE(most <= std::numeric_limits<int>::max() / (1 + kUnitCost), "cache_attention: too much work for one call");
-        MXK_CHECK(cache->head_dim == 128 ? launch_rows_bits<128>(cache->bits, p, most, few, call)
-                                         : launch_rows_bits<64>(cache->bits, p, most, few, call));
-    }
-    return call.join_all(cache->head_dim);
+    return MXK_OK;
+}
+
+}  // namespace mxk
+
+extern "C" int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* args, void* stream) {
+    using namespace mxk;
+    AttentionParams p{};
+    MXK_CHECK(check_attention("cache_attention", cache, args, p));
+    if (p.tokens == 0) return MXK_OK;
+    AttentionCall<AttentionParams> call(as_stream(stream));
+    return launch_attention(*cache, p, 0, call);
 }

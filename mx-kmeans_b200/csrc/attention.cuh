@@ -61,6 +61,17 @@ struct AttentionParams {
     int max_tiles, ready_seqs;
 };
 
+// A call whose sequences share prefixes.  Its units belong to parts of the sequences' tokens:
+// part g < groups is the prefix of group g, seen by all its sequences' rows, part groups + i
+// what sequence i has behind it.  `seqs` counts the parts.  Rows come out in float32 with
+// their lse, those of the prefixes before those of the rest, and are joined by
+// attention_merge_kernel (attention_shared.cu).
+struct SharedParams : AttentionParams {
+    const int4* parts;  // two to a part: {first row, rows, tokens end, position of the first row},
+                        // {first token, page table row, 0, 0}
+    int groups, max_prefix;
+};
+
 // Key tiles there can be at most when no sequence has more than max_q query and
 // p.max_kv cached tokens, and all of them p.tokens query tokens: a window touches at
 // most one tile more than it and the row tile's tokens fill.  (One long sequence among
@@ -71,6 +82,18 @@ inline int64_t attention_tile_bound(const AttentionParams& p, int max_q, int row
     int64_t span = p.max_kv;  // below 2^30, as the window
     if (p.window > 0 && p.window + rows < span) span = p.window + rows;
     return p.kv_heads * row_tiles * (span / keys + 2);
+}
+
+// The same of a call with prefixes: of the sequences and of the groups, whose rows are those
+// of up to max_rows query tokens.
+inline int64_t attention_tile_bound(const SharedParams& p, int max_q, int max_rows, int rows, int keys) {
+    AttentionParams own = p, prefix = p;
+    own.seqs = p.seqs - p.groups;
+    prefix.seqs = p.groups, prefix.max_kv = p.max_prefix;
+    return attention_tile_bound(own, max_q, rows, keys) + attention_tile_bound(prefix, max_rows, rows, keys);
+}
+inline int64_t attention_tile_bound(const AttentionParams& p, int max_q, int, int rows, int keys) {
+    return attention_tile_bound(p, max_q, rows, keys);
 }
 
 namespace dev {
@@ -140,6 +163,42 @@ struct SeqView {
     int len;   // cached tokens
 };
 
+__device__ __forceinline__ int first_position(const SeqView& s) { return s.len - s.n; }  // of its query tokens
+__device__ __forceinline__ int first_token(const SeqView&) { return 0; }
+
+// A part of a call with prefixes, rows and tokens as a sequence's.
+struct PartView {
+    int row0, n, len;
+    int position;  // of its first query token
+    int start;     // its tokens begin here; -1: it is a prefix
+};
+__device__ __forceinline__ int first_position(const PartView& s) { return s.position; }
+__device__ __forceinline__ int first_token(const PartView& s) { return max(s.start, 0); }
+
+template <class P>
+struct ViewOf { using type = SeqView; };
+template <>
+struct ViewOf<SharedParams> { using type = PartView; };
+
+// A sequence's page numbers.
+__device__ __forceinline__ const int* table_of(const AttentionParams& p, int seq) {
+    return p.page_table + (int64_t)seq * p.table_stride;
+}
+__device__ __forceinline__ const int* table_of(const SharedParams& p, int part) {
+    return p.page_table + (int64_t)__ldg(&p.parts[2 * part + 1].y) * p.table_stride;
+}
+
+// Where a sequence's rows go.
+__device__ __forceinline__ int64_t out_row(const AttentionParams&, const SeqView& s) { return s.row0; }
+__device__ __forceinline__ int64_t out_row(const SharedParams& p, const PartView& s) {
+    return s.row0 + (s.start < 0 ? 0 : p.tokens);
+}
+
+__device__ __forceinline__ PartView seq_view(const SharedParams& p, int part) {
+    const int4 a = __ldg(p.parts + 2 * part), b = __ldg(p.parts + 2 * part + 1);
+    return PartView{a.x, a.y, a.z, a.w, b.x};
+}
+
 __device__ __forceinline__ SeqView seq_view(const AttentionParams& p, int seq) {
     SeqView v;
     const int a = __ldg(p.cu_q + seq), b = __ldg(p.cu_q + seq + 1), len = __ldg(p.kv_lens + seq);
@@ -151,18 +210,19 @@ __device__ __forceinline__ SeqView seq_view(const AttentionParams& p, int seq) {
 
 // Tokens [lo, hi) that the rows of query tokens j0..j1 see, all of them together
 // (empty: hi <= lo).
-__device__ __forceinline__ void seen_range(const AttentionParams& p, const SeqView& s, int j0, int j1, int& lo, int& hi) {
-    const int first = s.len - s.n + j0, last = s.len - s.n + j1;
+template <class P, class V>
+__device__ __forceinline__ void seen_range(const P& p, const V& s, int j0, int j1, int& lo, int& hi) {
+    const int first = first_position(s) + j0, last = first_position(s) + j1;
     hi = p.causal ? min(last + 1, s.len) : s.len;
-    lo = p.window > 0 ? max(first - p.window + 1, 0) : 0;
+    lo = p.window > 0 ? max(first - p.window + 1, 0) : first_token(s);
 }
 
 // Key tiles of a row tile (at least one: rows that see nothing are written too).
-template <int ROWS, int KEYS>
-__device__ __forceinline__ int tile_count(const AttentionParams& p, const SeqView& s, int rt, int* first = nullptr) {
+template <int ROWS, int KEYS, class P, class V>
+__device__ __forceinline__ int tile_count(const P& p, const V& s, int rt, int* first = nullptr) {
     int lo, hi;
     if (!p.causal) {
-        lo = 0, hi = s.len;
+        lo = first_token(s), hi = s.len;
     } else {
         const int last = min((rt + 1) * ROWS, s.n * p.group) - 1;
         seen_range(p, s, p.window > 0 ? rt * ROWS / p.group : 0, last / p.group, lo, hi);
@@ -173,14 +233,15 @@ __device__ __forceinline__ int tile_count(const AttentionParams& p, const SeqVie
 }
 
 // Whether this launch takes a sequence.
-__device__ __forceinline__ bool taken(const AttentionParams& p, const SeqView& s) {
+template <class V>
+__device__ __forceinline__ bool taken(const AttentionParams& p, const V& s) {
     const int rows = s.n * p.group;
     return rows != 0 && rows >= p.min_rows && rows <= p.max_rows;
 }
 
 // Key tiles and units of a sequence.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ int2 seq_tiles(const AttentionParams& p, const SeqView& s) {
+template <int ROWS, int KEYS, class P, class V>
+__device__ __forceinline__ int2 seq_tiles(const P& p, const V& s) {
     const int rows = s.n * p.group;
     if (!taken(p, s)) return make_int2(0, 0);
     const int tiles = (rows + ROWS - 1) / ROWS, units = tiles * p.kv_heads;
@@ -211,8 +272,8 @@ struct Share {
 // CTAs past the number of tiles get none.  Sequences whose rows overlap can have more
 // tiles together than the host's bound, which counts every query token once; where that
 // is more than can be numbered, nobody gets any.
-template <int ROWS, int KEYS, int COST, int THREADS>
-__device__ __forceinline__ Share take_share(const AttentionParams& p, int* scratch) {
+template <int ROWS, int KEYS, int COST, int THREADS, class P>
+__device__ __forceinline__ Share take_share(const P& p, int* scratch) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kWarps = THREADS / 32;
     int* found = scratch + 2 * kWarps;  // sequence, offset
@@ -280,18 +341,19 @@ __device__ __forceinline__ Share take_share(const AttentionParams& p, int* scrat
 }
 
 // A position in the walk over the units.
+template <class P>
 struct Walk {
     int seq, rt, head;
     int tile, tiles;  // next key tile of the unit, and how many it has
     int skip;         // empty ones to pass before it
     int first;        // number of the unit's first key tile in the sequence
     int rank;         // of the sequence among those that the launch takes (the ready kernel sets it)
-    SeqView view;
+    typename ViewOf<P>::type view;
 };
 
-template <int ROWS, int KEYS>
-__device__ __forceinline__ Walk walk_to(const AttentionParams& p, const Share& s) {
-    Walk w;
+template <int ROWS, int KEYS, class P>
+__device__ __forceinline__ Walk<P> walk_to(const P& p, const Share& s) {
+    Walk<P> w;
     w.seq = s.seq;
     w.rank = 0;
     w.view = seq_view(p, s.seq);
@@ -312,8 +374,8 @@ __device__ __forceinline__ Walk walk_to(const AttentionParams& p, const Share& s
 }
 
 // To the next unit's first tile; the caller has passed its empty ones and knows that there is one.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ void walk_on(const AttentionParams& p, Walk& w) {
+template <int ROWS, int KEYS, class P>
+__device__ __forceinline__ void walk_on(const P& p, Walk<P>& w) {
     w.tile = 0;
     if (++w.head < p.kv_heads) return;
     w.head = 0;
@@ -349,7 +411,12 @@ __device__ __forceinline__ void store4_at(const AttentionParams& p, int64_t at, 
     }
 }
 
-__device__ __forceinline__ void store4(const AttentionParams& p, int64_t token, int head, int feature, float4 v) {
+__device__ __forceinline__ void store4_at(const SharedParams& p, int64_t at, float4 v) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
+}
+
+template <class P>
+__device__ __forceinline__ void store4(const P& p, int64_t token, int head, int feature, float4 v) {
     store4_at(p, token * p.out_token + (int64_t)head * p.out_head + feature, v);
 }
 
@@ -370,20 +437,22 @@ struct Parts {
     int split;       // CTAs that join a unit
 };
 constexpr int kMostParts = 3;  // kernels of a call
+template <class P>
 struct JoinParams {
-    AttentionParams p;
+    P p;
     Parts parts[kMostParts];
     int count;
 };
 
 // A row of a joined unit; total: the sum of its weights relative to `top`.
-__device__ __forceinline__ void store_joined(const AttentionParams& p, const int4& unit, const dev::SeqView& view,
-                                             int row, int chunk, float4 v, float top, float total) {
+template <class P, class V>
+__device__ __forceinline__ void store_joined(const P& p, const int4& unit, const V& view, int row, int chunk, float4 v, float top, float total) {
     const int j = row / p.group;
     const int head = unit.z * p.group + (row - j * p.group);
     if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    dev::store4(p, view.row0 + j, head, chunk * 4, v);
-    if (p.lse && chunk == 0) p.lse[(int64_t)(view.row0 + j) * p.heads + head] = dev::row_lse(top, total);
+    const int64_t to = dev::out_row(p, view) + j;
+    dev::store4(p, to, head, chunk * 4, v);
+    if (p.lse && chunk == 0) p.lse[to * p.heads + head] = dev::row_lse(top, total);
 }
 
 // Block (x, y) of a set of parts: the unit that CTA x began and did not finish, some of its
@@ -392,9 +461,9 @@ __device__ __forceinline__ void store_joined(const AttentionParams& p, const int
 // go through its parts.  Many: the block takes a row, every D / 4 of its threads some of the
 // parts, so a unit in hundreds of parts has several loads under way.  One launch joins the
 // parts of all of a call's kernels: a launch for each took 5 us more a kernel.
-template <int D>
-__global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams jp) {
-    const AttentionParams& p = jp.p;
+template <int D, class P>
+__global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams<P> jp) {
+    const P& p = jp.p;
     constexpr int kLanes = D / 4;            // threads of a row
     constexpr int kSub = 128 / kLanes;       // rows, or parts, at a time
     constexpr int kFew = 8;
@@ -409,7 +478,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams jp
     dev::wait_for_previous();
     const int4 unit = set.open[x];
     if (!unit.w) return;
-    const dev::SeqView view = dev::seq_view(p, unit.x);
+    const auto view = dev::seq_view(p, unit.x);
     const int rows = min(view.n * p.group - unit.y * set.rows, set.rows);
     const int tid = threadIdx.x, chunk = tid % kLanes, sub = tid / kLanes, parts = unit.w + 1;
     auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(x + i) + (i == 0 ? 1 : 0); };
@@ -494,6 +563,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams jp
 // pool, in stream order, at its end.  Kernels for sequences of different sizes write
 // different outputs, so each is launched as soon as the one before has started everywhere;
 // every one ends only when its predecessor has, so the join, launched last, finds all done.
+template <class P>
 class AttentionCall {
 public:
     explicit AttentionCall(cudaStream_t s) : stream_(s) {}
@@ -505,7 +575,7 @@ public:
 
     // Partial sums of `ctas` CTAs with tiles of `rows` rows, and extra_bytes more at *extra
     // (256-byte aligned).
-    int take(AttentionParams& p, int64_t ctas, int rows, int d, int64_t extra_bytes = 0, void** extra = nullptr) {
+    int take(P& p, int64_t ctas, int rows, int d, int64_t extra_bytes = 0, void** extra = nullptr) {
         const size_t part = (size_t)(2 * ctas * rows) * d * 4, stat = (size_t)(2 * ctas * rows) * 8;
         const size_t own = (part + stat + (size_t)ctas * 16 + 255) / 256 * 256;
         cudaMemPool_t pool = workspace_pool();
@@ -517,6 +587,15 @@ public:
         p.part = static_cast<float*>(ptr);
         p.part_stat = reinterpret_cast<float2*>(static_cast<char*>(ptr) + part);
         p.part_open = reinterpret_cast<int4*>(static_cast<char*>(ptr) + part + stat);
+        return MXK_OK;
+    }
+
+    // Room for something else of the call.
+    int room(size_t bytes, void** ptr) {
+        cudaMemPool_t pool = workspace_pool();
+        if (!pool) return fail(MXK_ERR_CUDA, "cache_attention: cannot create the workspace pool");
+        MXK_CUDA(cudaMallocFromPoolAsync(ptr, bytes, pool, stream_));
+        block_[blocks_++] = *ptr;
         return MXK_OK;
     }
 
@@ -543,7 +622,7 @@ public:
     }
 
     // Joins the parts of a kernel's CTAs, `split` blocks to a unit, when all are launched.
-    void join_later(const AttentionParams& p, int64_t ctas, int rows, int64_t split) {
+    void join_later(const P& p, int64_t ctas, int rows, int64_t split) {
         join_.p = p;
         join_.parts[join_.count++] = Parts{p.part, p.part_stat, p.part_open, (int)ctas, rows, (int)split};
     }
@@ -551,19 +630,28 @@ public:
         if (!join_.count) return MXK_OK;
         int64_t blocks = 0;
         for (int i = 0; i < join_.count; ++i) blocks += (int64_t)join_.parts[i].ctas * join_.parts[i].split;
-        return launch("attention_join", d == 128 ? attention_join_kernel<128> : attention_join_kernel<64>,
+        return launch("attention_join", d == 128 ? attention_join_kernel<128, P> : attention_join_kernel<64, P>,
                       (unsigned)blocks, 128, 0, join_);
     }
 
 private:
     cudaStream_t stream_;
     bool first_ = true;
-    void* block_[kMostParts] = {};
-    JoinParams join_{};
+    void* block_[kMostParts + 1] = {};
+    JoinParams<P> join_{};
     int blocks_ = 0;
 };
 
-// attention_tiles.cu: many query rows per key head.
-int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, AttentionCall& call);
+// attention_tiles.cu: many query rows per key head (max_rows: of query tokens that a part of a
+// call with prefixes can have).
+template <class P>
+int launch_attention_tiles(int bits, int head_dim, P p, int max_q, int max_rows, AttentionCall<P>& call);
+
+// attention.cu: few query rows, and all of a call's kernels; max_rows as above.
+template <class P>
+int launch_attention(const mxk_cache& cache, P p, int max_rows, AttentionCall<P>& call);
+
+// Checks of a call's arguments, and the kernels' parameters; p.tokens = 0: nothing to do.
+int check_attention(const char* who, const mxk_cache* cache, const mxk_attention* a, AttentionParams& p);
 
 }  // namespace mxk

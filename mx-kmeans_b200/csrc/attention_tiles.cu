@@ -172,9 +172,9 @@ struct Block {
 };
 
 // A pass over the CTA's share: every role makes the same one.
-template <class Cfg>
+template <class Cfg, class P>
 struct Cursor {
-    dev::Walk w;
+    dev::Walk<P> w;
     int left;          // tiles of the share from the current unit's on
     int tile0, tiles;  // key tiles of the current unit that are this CTA's
     int unit;          // units begun so far
@@ -184,7 +184,7 @@ struct Cursor {
         tile0 = w.tile;
         tiles = min(left, w.tiles - tile0);
     }
-    __device__ __forceinline__ bool next(const AttentionParams& p) {
+    __device__ __forceinline__ bool next(const P& p) {
         left -= tiles + cost;
         if (left <= 0) return false;
         dev::walk_on<Cfg::rows, kKeys>(p, w);
@@ -192,7 +192,7 @@ struct Cursor {
         take();
         return true;
     }
-    __device__ __forceinline__ int rows(const AttentionParams& p) const {
+    __device__ __forceinline__ int rows(const P& p) const {
         return min(w.view.n * p.group - w.rt * Cfg::rows, Cfg::rows);
     }
     __device__ __forceinline__ bool whole() const { return tile0 == 0 && tiles == w.tiles; }
@@ -202,8 +202,8 @@ struct Cursor {
 struct Whole {
     int from, to;
 };
-template <class Cfg>
-__device__ __forceinline__ Whole whole_tiles(const AttentionParams& p, const Cursor<Cfg>& c) {
+template <class Cfg, class P>
+__device__ __forceinline__ Whole whole_tiles(const P& p, const Cursor<Cfg, P>& c) {
     const int r0 = c.w.rt * Cfg::rows, j0 = r0 / p.group, j1 = (r0 + c.rows(p) - 1) / p.group;
     int lo, hi, x;
     dev::seen_range(p, c.w.view, j0, j0, x, hi);   // the first row ends first,
@@ -313,13 +313,14 @@ struct Converter {
     struct Place {
         int page, in;
     };
-    __device__ __forceinline__ Place place(const AttentionParams& p, int seq, int t0, Span sp) const {
+    template <class P>
+    __device__ __forceinline__ Place place(const P& p, int seq, int t0, Span sp) const {
         Place pl{0, 0};
         if (lane < 8 && 16 * lane < sp.to && 16 * lane + 16 > sp.from) {
             const unsigned per_page = (unsigned)p.page_size / 16u;
             const unsigned gr = (unsigned)(t0 / 16) + lane;
             const unsigned at = gr / per_page;
-            pl.page = __ldg(p.page_table + (int64_t)seq * p.table_stride + at);
+            pl.page = __ldg(dev::table_of(p, seq) + at);
             pl.in = (int)(gr - at * per_page) * 16;
         }
         return pl;
@@ -461,7 +462,8 @@ struct Converter {
 static_assert(kRefStep == 4, "value_ref rounds to multiples of four");
 
 // The sequence that is the rank-th of those the launch takes, -1 if there is none.  A whole warp.
-__device__ __forceinline__ int seq_of_rank(const AttentionParams& p, int rank) {
+template <class P>
+__device__ __forceinline__ int seq_of_rank(const P& p, int rank) {
     for (int base = 0; base < p.seqs; base += 32) {
         const int i = base + (threadIdx.x & 31);
         const unsigned m = __ballot_sync(kFull, i < p.seqs && dev::taken(p, dev::seq_view(p, min(i, p.seqs - 1))));
@@ -475,7 +477,8 @@ __device__ __forceinline__ int seq_of_rank(const AttentionParams& p, int rank) {
 struct Ranks {
     int rank, all;
 };
-__device__ __forceinline__ Ranks rank_of_seq(const AttentionParams& p, int seq) {
+template <class P>
+__device__ __forceinline__ Ranks rank_of_seq(const P& p, int seq) {
     Ranks r{0, 0};
 #pragma unroll 4
     for (int base = 0; base < p.seqs; base += 32) {
@@ -492,8 +495,8 @@ __device__ __forceinline__ Ranks rank_of_seq(const AttentionParams& p, int seq) 
 // Block (x, side): key tile x % max_tiles of (rank of the sequence, head) x / max_tiles, its
 // keys or its values; the f16 tiles lie in the workspace as shared memory will hold them, so each
 // is built there and leaves as one bulk copy.
-template <int D, int BITS>
-__global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionParams p) {
+template <int D, int BITS, class P>
+__global__ void __launch_bounds__(256) attention_unpack_kernel(const P p) {
     using C = Converter<D, BITS>;
     __shared__ __align__(128) uint8_t image[Smem<D>::tile];
     dev::let_next_start();
@@ -501,13 +504,13 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
     const int rank = sh / p.kv_heads, head = sh - rank * p.kv_heads;
     const int seq = p.seqs == 1 ? rank : seq_of_rank(p, rank);
     if (seq < 0) return;
-    const dev::SeqView view = dev::seq_view(p, seq);
+    const auto view = dev::seq_view(p, seq);
     if (!dev::taken(p, view)) return;
     int lo, hi;
     dev::seen_range(p, view, 0, view.n - 1, lo, hi);
     const int t0 = tile * kKeys;
-    // rows that see nothing still have key tile 0, of zeros where no token exists
-    if (tile != 0 && (t0 >= hi || t0 + kKeys <= lo)) return;
+    // rows that see nothing still have a first key tile, of zeros where no token exists
+    if (tile != dev::first_token(view) / kKeys && (t0 >= hi || t0 + kKeys <= lo)) return;
     const typename C::Span sp = C::span(lo, hi, t0);
     const bool keys = blockIdx.y == 0;
     const C cv(threadIdx.x >> 5);
@@ -539,14 +542,14 @@ __global__ void __launch_bounds__(256) attention_unpack_kernel(const AttentionPa
 
 // Converter warps: every key tile of the CTA's share, rows loaded one tile ahead of
 // their conversion and page numbers two.
-template <int D, int BITS>
-__device__ __forceinline__ bool convert_role(const AttentionParams& p, const Block& b, Cursor<Packed> c, int warp) {
+template <int D, int BITS, class P>
+__device__ __forceinline__ bool convert_role(const P& p, const Block& b, Cursor<Packed, P> c, int warp) {
     using C = Converter<D, BITS>;
     using L = Smem<D, Packed::row_tiles>;
     const C cv(warp);
     typename C::Words kx, vx;
     uint32_t ks[4], vs[4];
-    Cursor<Packed> ahead = c;
+    Cursor<Packed, P> ahead = c;
     int at = 0;  // key tile of `ahead`'s unit
     bool more = true;
     struct Next {
@@ -621,14 +624,14 @@ __device__ __forceinline__ bool convert_role(const AttentionParams& p, const Blo
 }
 
 // Index of a key tile among the converted ones.
-template <class Cfg>
-__device__ __forceinline__ int64_t ready_at(const AttentionParams& p, const Cursor<Cfg>& c) {
+template <class Cfg, class P>
+__device__ __forceinline__ int64_t ready_at(const P& p, const Cursor<Cfg, P>& c) {
     return ((int64_t)c.w.rank * p.kv_heads + c.w.head) * p.max_tiles + c.w.first + c.tile0;
 }
 
 // One warp copying ready-made tiles (its elected lane).
-template <int D>
-__device__ __forceinline__ void load_role(const AttentionParams& p, const Block& b, Cursor<Ready> c) {
+template <int D, class P>
+__device__ __forceinline__ void load_role(const P& p, const Block& b, Cursor<Ready, P> c) {
     using L = Smem<D, Ready::row_tiles>;
     constexpr int bytes = L::tile;
     int stage = 0, issued = 0;
@@ -667,8 +670,8 @@ __device__ __forceinline__ void load_role(const AttentionParams& p, const Block&
 
 // --------------------------------------------------------------------------- products
 
-template <int D, class Cfg>
-__device__ __forceinline__ void product_role(const AttentionParams& p, const Block& b, Cursor<Cfg> c) {
+template <int D, class Cfg, class P>
+__device__ __forceinline__ void product_role(const P& p, const Block& b, Cursor<Cfg, P> c) {
     using L = Smem<D, Cfg::row_tiles>;
     constexpr int kTiles = Cfg::row_tiles;
     constexpr uint32_t idesc_s = dev::f16_idesc(kTileRows, kHalf, false);
@@ -998,8 +1001,8 @@ __device__ __forceinline__ float put_queries(const AttentionParams& p, int64_t a
 // A warp's 32 output rows from shared memory to where they belong, D / 8 lanes a row:
 // columns [col, col + D / 2), four a lane, staged by their owners with the 16-byte chunks
 // permuted by row.
-template <int D>
-__device__ __forceinline__ void put_rows(const AttentionParams& p, const float4* stage, unsigned reals, int64_t out_at,
+template <int D, class P>
+__device__ __forceinline__ void put_rows(const P& p, const float4* stage, unsigned reals, int64_t out_at,
                                          float* part, int col) {
     constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
     const int lane = threadIdx.x & 31, piece = lane % kLanes, sub = lane / kLanes;
@@ -1081,8 +1084,8 @@ struct WideSum {
     float sum;
     int vrun;
 };
-template <int D>
-__device__ __forceinline__ WideSum wide_weights(const AttentionParams& p, WideHalf half, int from, int to, float f,
+template <int D, class P>
+__device__ __forceinline__ WideSum wide_weights(const P& p, WideHalf half, int from, int to, float f,
                                              float base, int vref, int vrun_at, float g) {
     constexpr int kBlocks = D / 32;
     const uint32_t o_col = half.o_col;
@@ -1119,7 +1122,7 @@ __device__ __forceinline__ WideSum wide_weights(const AttentionParams& p, WideHa
         const int t = lane + 32 * k, token = half.t0 + t, at = token / p.page_size;
         row[k] = -1;
         if (t >= first && t < end) {
-            const int page = min(max(__ldg(p.page_table + (int64_t)half.seq * p.table_stride + at), 0), p.pages - 1);
+            const int page = min(max(__ldg(dev::table_of(p, half.seq) + at), 0), p.pages - 1);
             row[k] = ((int64_t)page * p.kv_heads + half.head) * p.page_size + (token - at * p.page_size);
         }
     }
@@ -1207,8 +1210,8 @@ __device__ __forceinline__ WideSum wide_weights(const AttentionParams& p, WideHa
 }
 
 // READY: tiles were converted beforehand, their references lie in global memory.
-template <int D, class Cfg, bool READY>
-__device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Block& b, Cursor<Cfg> c, int warp) {
+template <int D, class Cfg, bool READY, class P>
+__device__ __forceinline__ bool softmax_role(const P& p, const Block& b, Cursor<Cfg, P> c, int warp) {
     using L = Smem<D, Cfg::row_tiles>;
     constexpr int kRows = Cfg::rows;
     Shared* sh = b.sh;
@@ -1429,9 +1432,8 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                 if constexpr (!READY) nans = *reinterpret_cast<volatile int*>(&sh->nan_unit[c.unit & 3]) == c.unit;
                 if (nans && real) {
                     const int end = first_key + c.tiles * kKeys;
-                    const uint4 f = nan_features<D>(p.v_values, p.page_table + (int64_t)c.w.seq * p.table_stride,
-                                                    p.page_size, p.pages, p.kv_heads, c.w.head,
-                                                    max(lo, first_key), min(hi, end));
+                    const uint4 f = nan_features<D>(p.v_values, dev::table_of(p, c.w.seq), p.page_size, p.pages, p.kv_heads,
+                                                    c.w.head, max(lo, first_key), min(hi, end));
                     bad[0] = f.x, bad[1] = f.y, bad[2] = f.z, bad[3] = f.w;
                 }
                 const float vfactor = __uint_as_float((uint32_t)vrun << 23);
@@ -1439,7 +1441,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                 const int64_t slot = 2 * (int64_t)blockIdx.x + (c.tile0 == 0 ? 1 : 0);
                 const int tile_row = w * kTileRows + r;
                 const unsigned reals = __ballot_sync(kFull, real);
-                const int64_t out_at = (int64_t)(c.w.view.row0 + j) * p.out_token + (int64_t)head * p.out_head;
+                const int64_t out_at = (dev::out_row(p, c.w.view) + j) * p.out_token + (int64_t)head * p.out_head;
                 float* part = all ? nullptr : p.part + (slot * kRows + (tile_row & ~31)) * D;
                 // The rows leave through the queries' shared memory, which no product reads any
                 // more: a warp's quarter of the row tile holds 32 rows of D / 2 floats.
@@ -1474,7 +1476,7 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
                     if (!all)
                         p.part_stat[slot * kRows + tile_row] = make_float2(run_max, sum);
                     else if (p.lse)
-                        p.lse[(int64_t)(c.w.view.row0 + j) * p.heads + head] = dev::row_lse(run_max, sum);
+                        p.lse[(dev::out_row(p, c.w.view) + j) * p.heads + head] = dev::row_lse(run_max, sum);
                 }
             }
             dev::tc_fence_before();
@@ -1498,9 +1500,9 @@ __device__ __forceinline__ bool softmax_role(const AttentionParams& p, const Blo
 // Barriers, TMEM and the cursor; false: the CTA has no share.
 constexpr int tmem_columns(int d, int row_tiles) { return row_tiles * (kKeys + d) <= 256 ? 256 : 512; }
 
-template <int D, class Cfg, int FULL_COUNT>
-__device__ __forceinline__ bool begin(const AttentionParams& p, uint8_t* smem_raw, Shared* sh, int* scratch,
-                                      unsigned* err, Block& b, Cursor<Cfg>& c) {
+template <int D, class Cfg, int FULL_COUNT, class P>
+__device__ __forceinline__ bool begin(const P& p, uint8_t* smem_raw, Shared* sh, int* scratch, unsigned* err, Block& b,
+                                      Cursor<Cfg, P>& c) {
     constexpr int kRows = Cfg::rows;
     const int tid = threadIdx.x;
     dev::let_next_start();
@@ -1572,14 +1574,13 @@ __device__ __forceinline__ void finish(const AttentionParams& p, const Block& b)
         p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
 }
 
-template <int D, int BITS>
-__global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(const __grid_constant__ AttentionParams p,
-                                                                                unsigned* err) {
+template <int D, int BITS, class P>
+__global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(const __grid_constant__ P p, unsigned* err) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared shared;
     __shared__ int scratch[Packed::threads / 16 + 2];
     Block b;
-    Cursor<Packed> c;
+    Cursor<Packed, P> c;
     if (!begin<D, Packed, Packed::convert_warps>(p, smem_raw, &shared, scratch, err, b, c)) return;
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
     if (warp < Packed::softmax_warps) {
@@ -1594,14 +1595,13 @@ __global__ void __launch_bounds__(Packed::threads, 1) attention_tiles_kernel(con
     finish<D, Packed>(p, b);
 }
 
-template <int D>
-__global__ void __launch_bounds__(Ready::threads, 1) attention_ready_kernel(const __grid_constant__ AttentionParams p,
-                                                                               unsigned* err) {
+template <int D, class P>
+__global__ void __launch_bounds__(Ready::threads, 1) attention_ready_kernel(const __grid_constant__ P p, unsigned* err) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared shared;
     __shared__ int scratch[Ready::threads / 16 + 2];
     Block b;
-    Cursor<Ready> c;
+    Cursor<Ready, P> c;
     if (!begin<D, Ready, 1>(p, smem_raw, &shared, scratch, err, b, c)) return;
     const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0);
     if (warp < Ready::softmax_warps) {
@@ -1634,39 +1634,39 @@ int prepare_kernel(K kernel, int smem, int regs, int& ready_device) {
 }
 
 // One CTA an SM, or one a key tile if there cannot be as many.
-template <class Cfg>
-int grid_size(const AttentionParams& p, int max_q, int64_t* ctas) {
-    const int64_t most = attention_tile_bound(p, max_q, Cfg::rows, kKeys);
+template <class Cfg, class P>
+int grid_size(const P& p, int max_q, int max_rows, int64_t* ctas) {
+    const int64_t most = attention_tile_bound(p, max_q, max_rows, Cfg::rows, kKeys);
     MXK_REQUIRE(most <= std::numeric_limits<int>::max() / (1 + Cfg::unit_cost), "cache_attention: too much work for one call");
     static const int sms = sm_count();
     *ctas = most < sms ? most : sms;
     return MXK_OK;
 }
 
-template <int D, int BITS>
-int launch_packed(AttentionParams p, int max_q, AttentionCall& call) {
+template <int D, int BITS, class P>
+int launch_packed(P p, int max_q, int max_rows, AttentionCall<P>& call) {
     constexpr int smem = Smem<D, Packed::row_tiles>::total;
     static thread_local int ready_device = -1;
-    MXK_CHECK(prepare_kernel(attention_tiles_kernel<D, BITS>, smem, Packed::launch_regs, ready_device));
+    MXK_CHECK(prepare_kernel(attention_tiles_kernel<D, BITS, P>, smem, Packed::launch_regs, ready_device));
     unsigned* err = device_error_word();
     if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
     int64_t ctas;
-    MXK_CHECK(grid_size<Packed>(p, max_q, &ctas));
+    MXK_CHECK((grid_size<Packed>(p, max_q, max_rows, &ctas)));
     MXK_CHECK(call.take(p, ctas, Packed::rows, D));
-    MXK_CHECK(call.launch("attention_tiles", attention_tiles_kernel<D, BITS>, (unsigned)ctas, Packed::threads, smem, p, err));
+    MXK_CHECK(call.launch("attention_tiles", attention_tiles_kernel<D, BITS, P>, (unsigned)ctas, Packed::threads, smem, p, err));
     call.join_later(p, ctas, Packed::rows, Packed::join_split);
     return MXK_OK;
 }
 
-template <int D, int BITS>
-int launch_ready(AttentionParams p, int max_q, AttentionCall& call) {
+template <int D, int BITS, class P>
+int launch_ready(P p, int max_q, int max_rows, AttentionCall<P>& call) {
     constexpr int smem = Smem<D, Ready::row_tiles>::total;
     static thread_local int ready_device = -1;
-    MXK_CHECK(prepare_kernel(attention_ready_kernel<D>, smem, Ready::launch_regs, ready_device));
+    MXK_CHECK(prepare_kernel(attention_ready_kernel<D, P>, smem, Ready::launch_regs, ready_device));
     unsigned* err = device_error_word();
     if (!err) return fail(MXK_ERR_CUDA, "cache_attention: cannot allocate the device error word");
     int64_t ctas;
-    MXK_CHECK(grid_size<Ready>(p, max_q, &ctas));
+    MXK_CHECK((grid_size<Ready>(p, max_q, max_rows, &ctas)));
     const int64_t tiles = (int64_t)p.ready_seqs * p.kv_heads * p.max_tiles;
     void* extra = nullptr;
     MXK_CHECK(call.take(p, ctas, Ready::rows, D, tiles * (2 * Smem<D>::tile + (int64_t)sizeof(int2) + kKeys), &extra));
@@ -1674,46 +1674,72 @@ int launch_ready(AttentionParams p, int max_q, AttentionCall& call) {
     p.ready_v = p.ready_k + tiles * Smem<D>::tile;
     p.ready_meta = reinterpret_cast<int2*>(p.ready_v + tiles * Smem<D>::tile);
     p.ready_key_refs = reinterpret_cast<uint8_t*>(p.ready_meta + tiles);
-    MXK_CHECK(call.launch("attention_unpack", attention_unpack_kernel<D, BITS>, dim3((unsigned)tiles, 2), 256, 0, p));
-    MXK_CHECK(call.launch("attention_ready", attention_ready_kernel<D>, (unsigned)ctas, Ready::threads, smem, p, err));
+    MXK_CHECK(call.launch("attention_unpack", attention_unpack_kernel<D, BITS, P>, dim3((unsigned)tiles, 2), 256, 0, p));
+    MXK_CHECK(call.launch("attention_ready", attention_ready_kernel<D, P>, (unsigned)ctas, Ready::threads, smem, p, err));
     call.join_later(p, ctas, Ready::rows, Ready::join_split);
     return MXK_OK;
 }
 
-template <int D, int BITS>
-int launch(const AttentionParams& p, bool ready, int max_q, AttentionCall& call) {
-    return ready ? launch_ready<D, BITS>(p, max_q, call) : launch_packed<D, BITS>(p, max_q, call);
+template <int D, int BITS, class P>
+int launch(const P& p, bool ready, int max_q, int max_rows, AttentionCall<P>& call) {
+    return ready ? launch_ready<D, BITS>(p, max_q, max_rows, call) : launch_packed<D, BITS>(p, max_q, max_rows, call);
 }
 
-template <int D>
-int launch_bits(int bits, const AttentionParams& p, bool ready, int max_q, AttentionCall& call) {
-    if (bits == 8) return launch<D, 8>(p, ready, max_q, call);
-    if (bits == 6) return launch<D, 6>(p, ready, max_q, call);
-    return launch<D, 4>(p, ready, max_q, call);
+template <int D, class P>
+int launch_bits(int bits, const P& p, bool ready, int max_q, int max_rows, AttentionCall<P>& call) {
+    if (bits == 8) return launch<D, 8>(p, ready, max_q, max_rows, call);
+    if (bits == 6) return launch<D, 6>(p, ready, max_q, max_rows, call);
+    return launch<D, 4>(p, ready, max_q, max_rows, call);
+}
+
+// Sequences (parts) that can have more than `rows` rows per key head, and their most tokens.
+struct Most {
+    int64_t seqs;
+    int tokens;
+};
+[[maybe_unused]] Most most_ready(const AttentionParams& p, int max_q, int, int rows) {
+    if ((int64_t)max_q * p.group <= rows) return {0, 0};
+    return {p.seqs == 1 ? 1 : std::min<int64_t>(p.seqs, p.tokens * p.group / (rows + 1)), p.max_kv};
+}
+[[maybe_unused]] Most most_ready(const SharedParams& p, int max_q, int max_rows, int rows) {
+    AttentionParams own = p, prefix = p;
+    own.seqs = p.seqs - p.groups;
+    prefix.seqs = p.groups, prefix.max_kv = p.max_prefix;
+    const Most a = own.seqs ? most_ready(own, max_q, 0, rows) : Most{0, 0};
+    const Most b = prefix.seqs ? most_ready(prefix, max_rows, 0, rows) : Most{0, 0};
+    return {a.seqs + b.seqs, std::max(a.tokens, b.tokens)};
 }
 
 }  // namespace
 
-int launch_attention_tiles(int bits, int head_dim, AttentionParams p, int max_q, AttentionCall& call) {
+template <class P>
+int launch_attention_tiles(int bits, int head_dim, P p, int max_q, int max_rows, AttentionCall<P>& call) {
     // Several row tiles of a key head share its keys: converting those once pays for
     // writing and reading them as f16.  So many sequences can have enough rows for that:
-    p.max_tiles = (p.max_kv + kKeys - 1) / kKeys;
     const int ready_rows = p.seqs == 1 ? kReadyRows : kReadyRowsMany;
-    p.ready_seqs = p.seqs == 1 ? 1 : (int)std::min<int64_t>(p.seqs, p.tokens * p.group / (ready_rows + 1));
-    const int64_t bytes = (int64_t)p.ready_seqs * p.kv_heads * p.max_tiles * 2 * kKeys * head_dim * 2;
-    const bool many = (int64_t)max_q * p.group > ready_rows && p.ready_seqs > 0 && p.max_tiles > 0 && bytes <= kReadyBytes;
+    const Most most = most_ready(p, max_q, max_rows, ready_rows);
+    p.max_tiles = (most.tokens + kKeys - 1) / kKeys;
+    p.ready_seqs = (int)most.seqs;
+    const int64_t bytes = most.seqs * p.kv_heads * p.max_tiles * 2 * kKeys * head_dim * 2;
+    const bool many = most.seqs > 0 && p.max_tiles > 0 && bytes <= kReadyBytes;
     const int few_q = (int)((ready_rows + p.group - 1) / p.group);
     if (many) {
-        AttentionParams q = p;
+        P q = p;
         if (p.seqs > 1 && q.min_rows <= ready_rows) q.min_rows = ready_rows + 1;
-        MXK_CHECK(head_dim == 128 ? launch_bits<128>(bits, q, true, max_q, call)
-                                  : launch_bits<64>(bits, q, true, max_q, call));
+        MXK_CHECK(head_dim == 128 ? launch_bits<128>(bits, q, true, max_q, max_rows, call)
+                                  : launch_bits<64>(bits, q, true, max_q, max_rows, call));
         if (p.seqs == 1) return MXK_OK;
         p.max_rows = ready_rows;
-        max_q = few_q;
+        max_q = max_rows = few_q;
     }
-    return head_dim == 128 ? launch_bits<128>(bits, p, false, max_q, call)
-                           : launch_bits<64>(bits, p, false, max_q, call);
+    return head_dim == 128 ? launch_bits<128>(bits, p, false, max_q, max_rows, call)
+                           : launch_bits<64>(bits, p, false, max_q, max_rows, call);
 }
+
+// Compiled for each kind of calls (attention_tiles_shared.cu).
+#ifndef MXK_ATTENTION_PARAMS
+#define MXK_ATTENTION_PARAMS AttentionParams
+#endif
+template int launch_attention_tiles(int, int, MXK_ATTENTION_PARAMS, int, int, AttentionCall<MXK_ATTENTION_PARAMS>&);
 
 }  // namespace mxk

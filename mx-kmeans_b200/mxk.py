@@ -82,6 +82,13 @@ class Attention(ctypes.Structure):
                 ("window", ctypes.c_int64), ("out", Rows), ("lse", ctypes.c_void_p)]
 
 
+class Prefixes(ctypes.Structure):
+    """mxk_prefixes: the groups of sequences of mxk_cache_attention_shared."""
+
+    _fields_ = [("groups", ctypes.c_int), ("cu_groups", ctypes.c_void_p), ("prefix_lens", ctypes.c_void_p),
+                ("max_prefix", ctypes.c_int64)]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
@@ -130,6 +137,7 @@ SIGNATURES = {
     "mxk_cache_read": ([_P, _I, _I64, _P, _P, _P, _P], _I),
     "mxk_cache_append": ([_P, _P, _P], _I),
     "mxk_cache_attention": ([_P, _P, _P], _I),
+    "mxk_cache_attention_shared": ([_P, _P, _P, _P], _I),
     "mxk_quantize_fp8": ([_I, _I64, _I64, _P, _I64, _I, _P, _P, _P], _I),
     "mxk_gemm_fp8": ([_I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P], _I),
     "mxk_linear_fp8": ([_I, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _P], _I),
@@ -510,13 +518,8 @@ def cache_append(cache, q, k, v, positions, cos_sin, slots, q_out=None, interlea
     check(load().mxk_cache_append(cache.handle, ctypes.byref(args), _launch_stream(cache, stream)))
 
 
-def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale=None, causal=True, window=0,
-                    lse=None, stream=None):
-    """Attention of each sequence's newest tokens over its cached ones (mxk.h,
-    mxk_cache_attention): q, out [tokens, heads, head_dim] float16 or bfloat16;
-    cu_q [seqs + 1], page_table [seqs, pages], kv_lens [seqs] int32; max_q, max_kv:
-    bounds on a sequence's new and cached tokens; scale: 1 / sqrt(head_dim) unless
-    given; lse: float32 [tokens, heads] or None."""
+def _attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale, causal, window, lse):
+    """mxk_attention of a call's tensors."""
     if q.dim() != 3 or page_table.dim() != 2:
         raise _bad("q has 3 dimensions, page_table 2")
     tokens, heads, _ = q.shape
@@ -531,12 +534,35 @@ def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, sca
         raise _bad(f"page_table: int32 rows on {cache.device} are needed")
     if pages * cache.page_size < max_kv:
         raise _bad("page_table has fewer pages than max_kv tokens need")
-    args = Attention(_DTYPES.get(dtype, -1), heads, tokens, seqs, max_q, max_kv, qr,
+    return Attention(_DTYPES.get(dtype, -1), heads, tokens, seqs, max_q, max_kv, qr,
                      _vector(cu_q, "cu_q", cache, i32, seqs + 1), page_table.data_ptr(), stride,
                      _vector(kv_lens, "kv_lens", cache, i32, seqs),
                      cache.head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, outr,
                      None if lse is None else _vector(lse, "lse", cache, _torch.float32, tokens, heads))
+
+
+def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale=None, causal=True, window=0,
+                    lse=None, stream=None):
+    """Attention of each sequence's newest tokens over its cached ones (mxk.h,
+    mxk_cache_attention): q, out [tokens, heads, head_dim] float16 or bfloat16;
+    cu_q [seqs + 1], page_table [seqs, pages], kv_lens [seqs] int32; max_q, max_kv:
+    bounds on a sequence's new and cached tokens; scale: 1 / sqrt(head_dim) unless
+    given; lse: float32 [tokens, heads] or None."""
+    args = _attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale, causal, window, lse)
     check(load().mxk_cache_attention(cache.handle, ctypes.byref(args), _launch_stream(cache, stream)))
+
+
+def cache_attention_shared(cache, q, cu_q, page_table, kv_lens, cu_groups, prefix_lens, out, max_q, max_kv, max_prefix,
+                           scale=None, causal=True, lse=None, stream=None):
+    """cache_attention of a batch in which sequences cu_groups[g] .. cu_groups[g + 1] - 1 (int32
+    [groups + 1]) have their first prefix_lens[g] (int32 [groups], at most max_prefix) tokens in
+    the same slots, which are read once for them all (mxk.h, mxk_cache_attention_shared)."""
+    args = _attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale, causal, 0, lse)
+    groups = prefix_lens.shape[0] if prefix_lens.dim() else 0
+    prefixes = Prefixes(groups, _vector(cu_groups, "cu_groups", cache, _torch.int32, groups + 1),
+                        _vector(prefix_lens, "prefix_lens", cache, _torch.int32, groups), max_prefix)
+    check(load().mxk_cache_attention_shared(cache.handle, ctypes.byref(args), ctypes.byref(prefixes),
+                                            _launch_stream(cache, stream)))
 
 
 # ----------------------------------------------------------------------------- E4M3 products
