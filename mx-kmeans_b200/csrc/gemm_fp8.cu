@@ -14,7 +14,7 @@
 #include <algorithm>
 #include <limits>
 
-#include "cache.cuh"
+#include "cache_rows.cuh"
 #include "gemm_fp8.cuh"
 
 namespace mxk {
@@ -30,26 +30,11 @@ struct GemmFp8Params {
     const float* b_scales;   // [n / 128][blocks]
     char* out;
     int64_t out_stride;      // elements
-    int dtype, out_vec;      // out_vec: four elements can be stored at once
+    int dtype;
+    int out_vec, out_wide;   // four elements, or 32 bytes, can be stored at once
+    int a_wide, b_wide;      // rows of scales can be loaded four at a time
     unsigned* err;
 };
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
-// The address of a CTA's shared memory in the window of CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float4 cluster_ld4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr));
-    return v;
-}
 
 // Up to four elements of an output row.
 __device__ __forceinline__ void store_out(const GemmFp8Params& p, int row, int col, float4 v) {
@@ -78,6 +63,58 @@ __device__ __forceinline__ void store_out(const GemmFp8Params& p, int row, int c
             if (col + i < p.n) o[i] = h[i];
 }
 
+// Scales i .. i + 3 of `count`, zeros past them.  They are asked for four blocks ahead: every
+// lane has a row of scales of its own, and while tiles stream past they take their time.
+__device__ __forceinline__ void load_scales(const float* p, int i, int count, bool wide, float (&v)[4]) {
+    if (wide && i < count) {
+        const float4 x = *reinterpret_cast<const float4*>(p + i);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = i + k < count ? p[i + k] : 0.0f;
+    }
+}
+
+// N elements of an output row that begin at a multiple of N, as pairs.
+template <int N>
+__device__ __forceinline__ void store_row(const GemmFp8Params& p, int row, int col, const float2 (&x)[N / 2]) {
+    if (p.out_wide && col + N <= p.n) {
+        char* at = p.out + ((int64_t)row * p.out_stride + col) * (p.dtype == MXK_F32 ? 4 : 2);
+        if (p.dtype == MXK_F32) {
+#pragma unroll
+            for (int i = 0; i < N / 2; i += 4)
+                dev::store32(at + 8 * i, *reinterpret_cast<const uint4*>(&x[i]), *reinterpret_cast<const uint4*>(&x[i + 2]));
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < N / 2; i += 8) {
+            uint32_t h[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (p.dtype == MXK_F16) {
+                    const __half2 v = __float22half2_rn(x[i + k]);
+                    h[k] = *reinterpret_cast<const uint32_t*>(&v);
+                } else {
+                    const __nv_bfloat162 v = __float22bfloat162_rn(x[i + k]);
+                    h[k] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+            }
+            dev::store32(at + 4 * i, make_uint4(h[0], h[1], h[2], h[3]), make_uint4(h[4], h[5], h[6], h[7]));
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; i += 2)
+        if (col + 2 * i < p.n) store_out(p, row, col + 2 * i, make_float4(x[i].x, x[i].y, x[i + 1].x, x[i + 1].y));
+}
+
+// A wait that goes on after an abort: for copies and products in flight.
+__device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
+    const long long start = clock64();
+    while (!dev::mbar_try_wait(bar, parity))
+        if (clock64() - start > dev::kWaitLimitCycles) break;
+}
+
 // ------------------------------------------------------------------ one tile a cluster
 
 namespace tile {
@@ -98,13 +135,6 @@ struct Shared {
     int abort_word;
     uint32_t tmem;
 };
-
-// A wait that goes on after an abort: for copies and products in flight.
-__device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity) {
-    const long long start = clock64();
-    while (!dev::mbar_try_wait(bar, parity))
-        if (clock64() - start > dev::kWaitLimitCycles) break;
-}
 
 __global__ void __launch_bounds__(kThreads, 2)
     gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -196,30 +226,38 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float* sb = p.b_scales + (int64_t)tn * p.blocks + first;
         const uint32_t column = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * kCols;
         dev::wait_for_previous();
-        float fa = 0.0f, fb = 0.0f;
-        if (count > 0) fa = real ? sa[0] : 0.0f, fb = __ldg(sb);
+        float fa[4], fb[4];
+        load_scales(sa, 0, count, false, fa), load_scales(sb, 0, count, false, fb);
         int stage = 0, buffer = 0;
         uint32_t phase = 0;
-        for (int i = 0; i < count; ++i) {
-            const float f = fa * fb;
-            if (i + 1 < count) fa = real ? sa[i + 1] : 0.0f, fb = __ldg(sb + i + 1);
-            if (!__all_sync(kFull, dev::mbar_wait(&sh.done[stage], phase, abort, p.err))) break;
-            dev::tc_fence_after();
+        bool ok = true;
+        for (int i0 = 0; i0 < count && ok; i0 += 4) {
+            float f[4];
 #pragma unroll
-            for (int c = 0; c < kCols; c += 16) {
-                uint32_t v[16];
-                dev::tmem_ld_32x32b_x16(column + buffer * kN + c, v);
-                dev::tmem_wait_ld();
-                if (c + 16 == kCols) {
-                    dev::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) dev::mbar_arrive(&sh.taken[buffer]);
+            for (int k = 0; k < 4; ++k) f[k] = fa[k] * fb[k];
+            load_scales(sa, i0 + 4, count, false, fa), load_scales(sb, i0 + 4, count, false, fb);
+#pragma unroll
+            for (int at = 0; at < 4; ++at) {
+                if (i0 + at >= count) break;
+                ok = __all_sync(kFull, dev::mbar_wait(&sh.done[stage], phase, abort, p.err));
+                if (!ok) break;
+                dev::tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < kCols; c += 16) {
+                    uint32_t v[16];
+                    dev::tmem_ld_32x32b_x16(column + buffer * kN + c, v);
+                    dev::tmem_wait_ld();
+                    if (c + 16 == kCols) {
+                        dev::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) dev::mbar_arrive(&sh.taken[buffer]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) acc[c + k] = fmaf(__uint_as_float(v[k]), f[at], acc[c + k]);
                 }
-#pragma unroll
-                for (int k = 0; k < 16; ++k) acc[c + k] = fmaf(__uint_as_float(v[k]), f, acc[c + k]);
+                if (++stage == kStages) stage = 0, phase ^= 1;
+                if (++buffer == kBuffers) buffer = 0;
             }
-            if (++stage == kStages) stage = 0, phase ^= 1;
-            if (++buffer == kBuffers) buffer = 0;
         }
         // All products have read their operands: the sums take that memory, a row's 16-byte
         // chunks permuted so that eight rows' chunks lie in different banks.
@@ -232,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
     }
     if (split > 1)
-        cluster_arrive(), cluster_wait();
+        dev::cluster_arrive(), dev::cluster_wait();
     else
         __syncthreads();
     // The cluster's sums, each CTA its part of the tile's rows and chunks.
@@ -245,14 +283,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t at = sums + r * (kN * 4) + ((c ^ (r & 7)) << 4);
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int k = 0; k < split; ++k) {
-            const float4 x = cluster_ld4(in_cta(at, k));
+            const float4 x = dev::cluster_ld4(dev::in_cta(at, k));
             v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
         }
         store_out(p, tm * kM + r, tn * kN + 4 * c, v);
     }
     dev::tc_fence_before();
     if (split > 1)
-        cluster_arrive(), cluster_wait();  // nobody leaves while its sums are read
+        dev::cluster_arrive(), dev::cluster_wait();  // nobody leaves while its sums are read
     else
         __syncthreads();
     dev::tc_fence_after();
@@ -297,6 +335,235 @@ int launch(const GemmFp8& g, GemmFp8Params p, bool follows, cudaStream_t stream)
 
 }  // namespace tile
 
+// ------------------------------------------------------------------ large products
+
+namespace pair {
+
+// A pair of CTAs holds 256 rows and 256 columns: each loads its 128 rows of A and 128 of the 256
+// rows of B, which the pair's products read from both.  The pairs stay and go from tile to tile.
+constexpr int kM = 256, kN = 256;
+constexpr int kStages = 6, kBuffers = 2;
+constexpr int kSide = 128 * kBlock;  // bytes of an operand's tile in one CTA
+constexpr int kStage = 2 * kSide;
+constexpr int kSumWarps = 8, kLoadWarp = 8, kProductWarp = 9, kThreads = 384;
+constexpr int kLaunchRegs = 168, kSumRegs = 216, kOtherRegs = 72;
+static_assert(256 * kSumRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "");
+constexpr int kCols = kN / 2;        // columns of a warp: four lane quarters, two halves
+constexpr int kSmem = kStages * kStage + 1024;  // 1024: alignment
+constexpr int kRaster = 8;           // row tiles that are gone through side by side
+
+struct Shared {
+    uint64_t full[kStages];   // (even CTA) both CTAs' tiles are loaded
+    uint64_t done[kStages];   // multiplied, so the sums are in TMEM
+    uint64_t taken[kBuffers]; // (even CTA) a buffer's sums have been read by both CTAs
+    uint64_t drain;
+    int abort_word;
+    uint32_t tmem;
+};
+
+// Tiles are numbered so that those at hand at a time share operands: kRaster row tiles, column
+// tile by column tile.
+__device__ __forceinline__ void place_of(int tile, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int band = tile / (kRaster * tiles_n), first = band * kRaster, high = min(kRaster, tiles_m - first);
+    const int in = tile - first * tiles_n;
+    tn = in / high;
+    tm = first + in - tn * high;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                         const GemmFp8Params p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) Shared sh;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(kFull, tid >> 5, 0);
+    const int rank = blockIdx.x & 1, pairs = gridDim.x >> 1;
+    const int tiles_n = (p.n + kN - 1) / kN, tiles = p.tiles_m * tiles_n;
+    volatile int* abort = &sh.abort_word;
+
+    if (tid == 0) {
+        sh.abort_word = 0;
+        for (int i = 0; i < kStages; ++i) dev::mbar_init(&sh.full[i], 1), dev::mbar_init(&sh.done[i], 1);
+        for (int i = 0; i < kBuffers; ++i) dev::mbar_init(&sh.taken[i], 2 * kSumWarps);
+        dev::mbar_init(&sh.drain, 1);
+        dev::fence_barrier_init();
+    }
+    if (warp == kProductWarp) dev::tmem_alloc_pair(&sh.tmem, kBuffers * kN);
+    if (warp == kLoadWarp && lane == 0) dev::prefetch_tensor_map(&map_a), dev::prefetch_tensor_map(&map_b);
+    dev::tc_fence_before();
+    __syncthreads();
+    dev::cluster_arrive(), dev::cluster_wait();  // the other CTA's barriers are there
+    dev::tc_fence_after();
+    const uint32_t tmem = __shfl_sync(kFull, sh.tmem, 0);
+    dev::let_next_start();
+
+    if (warp < kSumWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
+        const int half = warp >> 2;
+        const uint32_t column = tmem + ((uint32_t)(warp & 3) << 21) + half * kCols;
+        const uint32_t taken = dev::in_cta(dev::smem_addr(&sh.taken[0]), 0);
+        dev::wait_for_previous();
+        int stage = 0, buffer = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
+            int tm, tn;
+            place_of(tile, p.tiles_m, tiles_n, tm, tn);
+            const int row = tm * kM + rank * 128 + (warp & 3) * 32 + lane, col = tn * kN + half * kCols;
+            const bool real = row < p.m;
+            const float* sa = p.a_scales + (int64_t)(real ? row : 0) * p.blocks;
+            const float* sb = p.b_scales + (int64_t)min(col / kBlock, (p.n - 1) / kBlock) * p.blocks;
+            float2 acc[kCols / 2];
+#pragma unroll
+            for (int i = 0; i < kCols / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
+            float fa[4], fb[4];
+            load_scales(sa, 0, p.blocks, p.a_wide, fa), load_scales(sb, 0, p.blocks, p.b_wide, fb);
+            for (int i0 = 0; i0 < p.blocks && ok; i0 += 4) {
+                float f[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) f[k] = fa[k] * fb[k];
+                load_scales(sa, i0 + 4, p.blocks, p.a_wide, fa), load_scales(sb, i0 + 4, p.blocks, p.b_wide, fb);
+#pragma unroll
+                for (int at = 0; at < 4; ++at) {
+                    if (i0 + at >= p.blocks) break;
+                    ok = __all_sync(kFull, dev::mbar_wait(&sh.done[stage], phase, abort, p.err));
+                    if (!ok) break;
+                    dev::tc_fence_after();
+                    uint32_t v[2][16];
+                    dev::tmem_ld_32x32b_x16(column + buffer * kN, v[0]);
+#pragma unroll
+                    for (int c = 0; c < kCols / 16; ++c) {
+                        dev::tmem_wait_ld();
+                        if (c + 1 < kCols / 16) {
+                            dev::tmem_ld_32x32b_x16(column + buffer * kN + 16 * (c + 1), v[(c + 1) & 1]);
+                        } else {
+                            dev::tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) dev::cluster_mbar_arrive(taken + 8 * buffer);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            acc[8 * c + k] = __ffma2_rn(
+                                make_float2(__uint_as_float(v[c & 1][2 * k]), __uint_as_float(v[c & 1][2 * k + 1])),
+                                make_float2(f[at], f[at]), acc[8 * c + k]);
+                    }
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                    if (++buffer == kBuffers) buffer = 0;
+                }
+            }
+            if (real && ok) store_row<kCols>(p, row, col, acc);
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kLoadWarp) {
+            if (dev::elect_one()) {
+                const uint32_t full = dev::in_cta(dev::smem_addr(&sh.full[0]), 0);
+                int stage = 0;
+                int64_t issued = 0;
+                uint32_t phase = 1;  // the first pass over the stages finds them free
+                bool ok = true;
+                dev::wait_for_previous();
+                for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
+                    int tm, tn;
+                    place_of(tile, p.tiles_m, tiles_n, tm, tn);
+                    for (int i = 0; i < p.blocks; ++i) {
+                        ok = dev::mbar_wait(&sh.done[stage], phase, abort, p.err);
+                        if (!ok) break;
+                        if (rank == 0) dev::mbar_arrive_expect_tx(&sh.full[stage], 2 * kStage);
+                        uint8_t* at = smem + stage * kStage;
+                        dev::tma_load_2d_pair(at, &map_a, i * kBlock, tm * kM + rank * 128, full + 8 * stage);
+                        dev::tma_load_2d_pair(at + kSide, &map_b, i * kBlock, tn * kN + rank * 128, full + 8 * stage);
+                        ++issued;
+                        if (++stage == kStages) stage = 0, phase ^= 1;
+                    }
+                }
+                if (!ok && rank == 0)  // copies in flight must not outlive the CTAs' memory
+                    for (int64_t k = issued > kStages ? issued - kStages : 0; k < issued; ++k)
+                        settle(&sh.full[k % kStages], (uint32_t)(k / kStages) & 1u);
+            }
+            __syncwarp();
+        } else if (warp == kProductWarp && rank == 0) {
+            constexpr uint32_t idesc = dev::f16_idesc(kM, kN, false);
+            const uint64_t a_desc = dev::smem_desc(dev::smem_addr(smem), 16, 1024, dev::kLayoutSwizzle128);
+            int stage = 0, buffer = 0;
+            uint32_t phase = 0, taken_phase = 1;
+            bool ok = true;
+            for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
+                for (int i = 0; i < p.blocks; ++i) {
+                    ok = __all_sync(kFull, dev::mbar_wait_lean(&sh.taken[buffer], taken_phase, abort, p.err)) &&
+                         __all_sync(kFull, dev::mbar_wait_lean(&sh.full[stage], phase, abort, p.err));
+                    if (!ok) break;
+                    dev::tc_fence_after();
+                    if (dev::elect_one()) {
+                        const uint64_t a = a_desc + (uint64_t)(stage * (kStage >> 4)), b = a + (kSide >> 4);
+#pragma unroll
+                        for (int k = 0; k < kBlock / 32; ++k)
+                            dev::tc_mma_f8_pair(tmem + buffer * kN, a + 2 * k, b + 2 * k, idesc, k > 0);
+                        dev::tc_commit_pair(&sh.done[stage]);
+                    }
+                    __syncwarp();
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                    if (++buffer == kBuffers) buffer = 0, taken_phase ^= 1;
+                }
+            }
+            if (!ok && dev::elect_one()) {
+                dev::tc_commit_pair(&sh.drain);
+                settle(&sh.drain, 0);
+            }
+            __syncwarp();
+        }
+    }
+    dev::tc_fence_before();
+    __syncthreads();
+    dev::cluster_arrive(), dev::cluster_wait();  // nobody leaves while the other CTA arrives or multiplies
+    dev::tc_fence_after();
+    if (warp == kProductWarp) dev::tmem_dealloc_pair(tmem, kBuffers * kN);
+}
+
+int launch(const GemmFp8& g, GemmFp8Params p, bool follows, cudaStream_t stream) {
+    CUtensorMap map_a, map_b;
+    MXK_CHECK(encode_tensor_map_2d(&map_a, g.a, (uint64_t)g.k, (uint64_t)g.m, (uint64_t)g.k, kBlock, 128,
+                                   CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
+    MXK_CHECK(encode_tensor_map_2d(&map_b, g.b, (uint64_t)g.k, (uint64_t)g.n, (uint64_t)g.k, kBlock, 128,
+                                   CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
+    static thread_local int ready_device = -1, most_pairs = 0;
+    int dev = 0;
+    MXK_CUDA(cudaGetDevice(&dev));
+    if (ready_device != dev) {
+        MXK_CUDA(cudaFuncSetAttribute(gemm_fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        cudaFuncAttributes attr{};
+        MXK_CUDA(cudaFuncGetAttributes(&attr, gemm_fp8_pair_kernel));
+        if (attr.numRegs != kLaunchRegs)
+            return fail(MXK_ERR_UNSUPPORTED, "gemm_fp8: kernel built with " + std::to_string(attr.numRegs) +
+                                                 " registers, the register split needs " + std::to_string(kLaunchRegs));
+        // Pairs lie in one GPC each, so there can be fewer than half the SMs.
+        cudaLaunchConfig_t all{};
+        all.gridDim = dim3((unsigned)sm_count() / 2 * 2), all.blockDim = dim3(kThreads), all.dynamicSmemBytes = kSmem;
+        MXK_CUDA(cudaOccupancyMaxActiveClusters(&most_pairs, gemm_fp8_pair_kernel, &all));
+        MXK_REQUIRE(most_pairs > 0, "gemm_fp8: the device holds no pair of CTAs");
+        ready_device = dev;
+    }
+    p.tiles_m = (p.m + kM - 1) / kM;
+    const int64_t tiles = (int64_t)p.tiles_m * ((p.n + kN - 1) / kN);
+    MXK_REQUIRE(tiles <= std::numeric_limits<int>::max() / 2, "gemm_fp8: too much work for one call");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, most_pairs)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = follows ? 1 : 0;
+    LaunchScope scope("gemm_fp8_pair", stream);
+    MXK_CUDA(cudaLaunchKernelEx(&cfg, gemm_fp8_pair_kernel, map_a, map_b, p));
+    return MXK_OK;
+}
+
+}  // namespace pair
+
 int check_product(const char* who, int dtype, int64_t m, int64_t n, int64_t k, const void* b, const float* b_scales,
                   const void* out) {
     const std::string w(who);
@@ -323,9 +590,12 @@ int gemm_fp8(const GemmFp8& g, bool follows, cudaStream_t stream) {
     p.out_stride = g.out_stride;
     p.dtype = g.dtype;
     p.out_vec = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % (4 * size) == 0;
+    p.out_wide = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % 32 == 0;
+    p.a_wide = p.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(g.a_scales) % 16 == 0;
+    p.b_wide = p.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(g.b_scales) % 16 == 0;
     p.err = device_error_word();
     if (!p.err) return fail(MXK_ERR_CUDA, "gemm_fp8: cannot allocate the device error word");
-    return tile::launch(g, p, follows, stream);
+    return g.m >= 256 && g.m * g.n >= 256 * 256 * 74 ? pair::launch(g, p, follows, stream) : tile::launch(g, p, follows, stream);
 }
 
 // Products of no features.
