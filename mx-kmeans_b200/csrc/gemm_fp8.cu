@@ -31,10 +31,20 @@ struct GemmFp8Params {
     char* out;
     int64_t out_stride;      // elements
     int dtype;
-    int out_vec, out_wide;   // four elements, or 32 bytes, can be stored at once
+    int out_vec, out_wide;   // four elements, or 16 bytes, can be stored at once
     int a_wide, b_wide;      // rows of scales can be loaded four at a time
     unsigned* err;
 };
+
+// Four 16-bit elements.
+__device__ __forceinline__ uint2 pack4(int dtype, float2 a, float2 b) {
+    if (dtype == MXK_F16) {
+        const __half2 u = __float22half2_rn(a), v = __float22half2_rn(b);
+        return make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+    }
+    const __nv_bfloat162 u = __float22bfloat162_rn(a), v = __float22bfloat162_rn(b);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+}
 
 // Up to four elements of an output row.
 __device__ __forceinline__ void store_out(const GemmFp8Params& p, int row, int col, float4 v) {
@@ -50,17 +60,14 @@ __device__ __forceinline__ void store_out(const GemmFp8Params& p, int row, int c
                 if (col + i < p.n) o[i] = x[i];
         return;
     }
-    uint16_t h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        h[i] = p.dtype == MXK_F16 ? __half_as_ushort(__float2half_rn(x[i])) : __bfloat16_as_ushort(__float2bfloat16_rn(x[i]));
+    const uint2 h = pack4(p.dtype, make_float2(v.x, v.y), make_float2(v.z, v.w));
     uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + at;
     if (p.out_vec && col + 4 <= p.n)
-        *reinterpret_cast<uint2*>(o) = make_uint2(h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16));
+        *reinterpret_cast<uint2*>(o) = h;
     else
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (col + i < p.n) o[i] = h[i];
+            if (col + i < p.n) o[i] = (uint16_t)((i < 2 ? h.x : h.y) >> (16 * (i & 1)));
 }
 
 // Scales i .. i + 3 of `count`, zeros past them.  They are asked for four blocks ahead: every
@@ -75,37 +82,57 @@ __device__ __forceinline__ void load_scales(const float* p, int i, int count, bo
     }
 }
 
-// N elements of an output row that begin at a multiple of N, as pairs.
+// 32 rows of N elements, a row a lane, to the output, by way of 4 KB of shared memory: 128 bytes
+// of each row at a time, which leave as whole lines.  (As 32 bytes a lane, a row each, the
+// 256 x 256 tile's rows took 4100 cycles.)  Rows from `rows` on are left out.
 template <int N>
-__device__ __forceinline__ void store_row(const GemmFp8Params& p, int row, int col, const float2 (&x)[N / 2]) {
-    if (p.out_wide && col + N <= p.n) {
-        char* at = p.out + ((int64_t)row * p.out_stride + col) * (p.dtype == MXK_F32 ? 4 : 2);
-        if (p.dtype == MXK_F32) {
+__device__ __forceinline__ void store_rows(const GemmFp8Params& p, uint8_t* stage, int row0, int rows, int col,
+                                           const float2 (&x)[N / 2]) {
+    const int lane = threadIdx.x & 31, size = p.dtype == MXK_F32 ? 4 : 2;
+    auto line = [&](int c) {  // the line that begins at element c
+        __syncwarp();
+        const int per = 16 / size, chunk = lane & 7, at = col + c + chunk * per;
 #pragma unroll
-            for (int i = 0; i < N / 2; i += 4)
-                dev::store32(at + 8 * i, *reinterpret_cast<const uint4*>(&x[i]), *reinterpret_cast<const uint4*>(&x[i + 2]));
-            return;
-        }
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((chunk ^ (r & 7)) << 4));
+            if (r >= rows || at >= p.n) continue;
+            char* to = p.out + ((int64_t)(row0 + r) * p.out_stride + at) * size;
+            if (p.out_wide && at + per <= p.n) {
+                *reinterpret_cast<uint4*>(to) = v;
+            } else {
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < N / 2; i += 8) {
-            uint32_t h[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (p.dtype == MXK_F16) {
-                    const __half2 v = __float22half2_rn(x[i + k]);
-                    h[k] = *reinterpret_cast<const uint32_t*>(&v);
-                } else {
-                    const __nv_bfloat162 v = __float22bfloat162_rn(x[i + k]);
-                    h[k] = *reinterpret_cast<const uint32_t*>(&v);
+                for (int k = 0; k < 8; ++k) {
+                    if (size == 2 && at + k < p.n) reinterpret_cast<uint16_t*>(to)[k] = (uint16_t)(w[k / 2] >> (16 * (k & 1)));
+                    if (size == 4 && k < 4 && at + k < p.n) reinterpret_cast<uint32_t*>(to)[k] = w[k & 3];
                 }
             }
-            dev::store32(at + 4 * i, make_uint4(h[0], h[1], h[2], h[3]), make_uint4(h[4], h[5], h[6], h[7]));
         }
-        return;
-    }
+        __syncwarp();
+    };
+    uint8_t* mine = stage + lane * 128;
+    if (size == 4) {
 #pragma unroll
-    for (int i = 0; i < N / 2; i += 2)
-        if (col + 2 * i < p.n) store_out(p, row, col + 2 * i, make_float4(x[i].x, x[i].y, x[i + 1].x, x[i + 1].y));
+        for (int c = 0; c < N; c += 32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(mine + ((i ^ (lane & 7)) << 4)) =
+                    make_float4(x[c / 2 + 2 * i].x, x[c / 2 + 2 * i].y, x[c / 2 + 2 * i + 1].x, x[c / 2 + 2 * i + 1].y);
+            line(c);
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; c += 64) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint2 u = pack4(p.dtype, x[c / 2 + 4 * i], x[c / 2 + 4 * i + 1]);
+                const uint2 v = pack4(p.dtype, x[c / 2 + 4 * i + 2], x[c / 2 + 4 * i + 3]);
+                *reinterpret_cast<uint4*>(mine + ((i ^ (lane & 7)) << 4)) = make_uint4(u.x, u.y, v.x, v.y);
+            }
+            line(c);
+        }
+    }
 }
 
 // A wait that goes on after an abort: for copies and products in flight.
@@ -342,20 +369,24 @@ namespace pair {
 // A pair of CTAs holds 256 rows and 256 columns: each loads its 128 rows of A and 128 of the 256
 // rows of B, which the pair's products read from both.  The pairs stay and go from tile to tile.
 constexpr int kM = 256, kN = 256;
-constexpr int kStages = 6, kBuffers = 2;
+constexpr int kStages = 5, kBuffers = 2;
 constexpr int kSide = 128 * kBlock;  // bytes of an operand's tile in one CTA
 constexpr int kStage = 2 * kSide;
 constexpr int kSumWarps = 8, kLoadWarp = 8, kProductWarp = 9, kThreads = 384;
 constexpr int kLaunchRegs = 168, kSumRegs = 216, kOtherRegs = 72;
 static_assert(256 * kSumRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "");
 constexpr int kCols = kN / 2;        // columns of a warp: four lane quarters, two halves
-constexpr int kSmem = kStages * kStage + 1024;  // 1024: alignment
+constexpr int kGroup = 4, kGroups = 4;  // blocks whose scales come together; groups at hand
+constexpr int kScales = kGroups * kGroup * 2 * 128 * 4;  // bytes
+constexpr int kSmem = kStages * kStage + kScales + kSumWarps * 4096 + 1024;  // 1024: alignment
+constexpr int kScaleWarps = 2;          // the last two
 constexpr int kRaster = 8;           // row tiles that are gone through side by side
 
 struct Shared {
     uint64_t full[kStages];   // (even CTA) both CTAs' tiles are loaded
     uint64_t done[kStages];   // multiplied, so the sums are in TMEM
     uint64_t taken[kBuffers]; // (even CTA) a buffer's sums have been read by both CTAs
+    uint64_t scales_full[kGroups], scales_free[kGroups];
     uint64_t drain;
     int abort_word;
     uint32_t tmem;
@@ -380,11 +411,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int rank = blockIdx.x & 1, pairs = gridDim.x >> 1;
     const int tiles_n = (p.n + kN - 1) / kN, tiles = p.tiles_m * tiles_n;
     volatile int* abort = &sh.abort_word;
+    // a[row] b[half of the columns] of the groups' blocks: [group][block][half][row]
+    float* scales = reinterpret_cast<float*>(smem + kStages * kStage);
+    uint8_t* out_stage = smem + kStages * kStage + kScales;
 
     if (tid == 0) {
         sh.abort_word = 0;
         for (int i = 0; i < kStages; ++i) dev::mbar_init(&sh.full[i], 1), dev::mbar_init(&sh.done[i], 1);
         for (int i = 0; i < kBuffers; ++i) dev::mbar_init(&sh.taken[i], 2 * kSumWarps);
+        for (int i = 0; i < kGroups; ++i) dev::mbar_init(&sh.scales_full[i], 1), dev::mbar_init(&sh.scales_free[i], kSumWarps);
         dev::mbar_init(&sh.drain, 1);
         dev::fence_barrier_init();
     }
@@ -402,57 +437,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int half = warp >> 2;
         const uint32_t column = tmem + ((uint32_t)(warp & 3) << 21) + half * kCols;
         const uint32_t taken = dev::in_cta(dev::smem_addr(&sh.taken[0]), 0);
+        const float* my_scales = scales + half * 128 + (warp & 3) * 32 + lane;
         dev::wait_for_previous();
-        int stage = 0, buffer = 0;
-        uint32_t phase = 0;
+        int stage = 0, buffer = 0, group = 0;
+        uint32_t phase = 0, group_phase = 0;
         bool ok = true;
         for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
             int tm, tn;
             place_of(tile, p.tiles_m, tiles_n, tm, tn);
-            const int row = tm * kM + rank * 128 + (warp & 3) * 32 + lane, col = tn * kN + half * kCols;
-            const bool real = row < p.m;
-            const float* sa = p.a_scales + (int64_t)(real ? row : 0) * p.blocks;
-            const float* sb = p.b_scales + (int64_t)min(col / kBlock, (p.n - 1) / kBlock) * p.blocks;
+            const int row0 = tm * kM + rank * 128 + (warp & 3) * 32, col = tn * kN + half * kCols;
             float2 acc[kCols / 2];
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
-            float fa[4], fb[4];
-            load_scales(sa, 0, p.blocks, p.a_wide, fa), load_scales(sb, 0, p.blocks, p.b_wide, fb);
-            for (int i0 = 0; i0 < p.blocks && ok; i0 += 4) {
-                float f[4];
+            for (int i = 0; i < p.blocks; ++i) {
+                if (i % kGroup == 0) ok = __all_sync(kFull, dev::mbar_wait(&sh.scales_full[group], group_phase, abort, p.err));
+                if (!ok) break;
+                const float f = my_scales[(group * kGroup + i % kGroup) * 256];
+                ok = __all_sync(kFull, dev::mbar_wait(&sh.done[stage], phase, abort, p.err));
+                if (!ok) break;
+                dev::tc_fence_after();
+                uint32_t v[2][16];
+                dev::tmem_ld_32x32b_x16(column + buffer * kN, v[0]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) f[k] = fa[k] * fb[k];
-                load_scales(sa, i0 + 4, p.blocks, p.a_wide, fa), load_scales(sb, i0 + 4, p.blocks, p.b_wide, fb);
-#pragma unroll
-                for (int at = 0; at < 4; ++at) {
-                    if (i0 + at >= p.blocks) break;
-                    ok = __all_sync(kFull, dev::mbar_wait(&sh.done[stage], phase, abort, p.err));
-                    if (!ok) break;
-                    dev::tc_fence_after();
-                    uint32_t v[2][16];
-                    dev::tmem_ld_32x32b_x16(column + buffer * kN, v[0]);
-#pragma unroll
-                    for (int c = 0; c < kCols / 16; ++c) {
-                        dev::tmem_wait_ld();
-                        if (c + 1 < kCols / 16) {
-                            dev::tmem_ld_32x32b_x16(column + buffer * kN + 16 * (c + 1), v[(c + 1) & 1]);
-                        } else {
-                            dev::tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) dev::cluster_mbar_arrive(taken + 8 * buffer);
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            acc[8 * c + k] = __ffma2_rn(
-                                make_float2(__uint_as_float(v[c & 1][2 * k]), __uint_as_float(v[c & 1][2 * k + 1])),
-                                make_float2(f[at], f[at]), acc[8 * c + k]);
+                for (int c = 0; c < kCols / 16; ++c) {
+                    dev::tmem_wait_ld();
+                    if (c + 1 < kCols / 16) {
+                        dev::tmem_ld_32x32b_x16(column + buffer * kN + 16 * (c + 1), v[(c + 1) & 1]);
+                    } else {
+                        dev::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) dev::cluster_mbar_arrive(taken + 8 * buffer);
                     }
-                    if (++stage == kStages) stage = 0, phase ^= 1;
-                    if (++buffer == kBuffers) buffer = 0;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        acc[8 * c + k] =
+                            __ffma2_rn(make_float2(__uint_as_float(v[c & 1][2 * k]), __uint_as_float(v[c & 1][2 * k + 1])),
+                                       make_float2(f, f), acc[8 * c + k]);
+                }
+                if (++stage == kStages) stage = 0, phase ^= 1;
+                if (++buffer == kBuffers) buffer = 0;
+                if (i % kGroup == kGroup - 1 || i + 1 == p.blocks) {
+                    __syncwarp();
+                    if (lane == 0) dev::mbar_arrive(&sh.scales_free[group]);
+                    if (++group == kGroups) group = 0, group_phase ^= 1;
                 }
             }
-            if (real && ok) store_row<kCols>(p, row, col, acc);
-            __syncwarp();
+            if (ok) store_rows<kCols>(p, out_stage + warp * 4096, row0, p.m - row0, col, acc);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -483,6 +513,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         settle(&sh.full[k % kStages], (uint32_t)(k / kStages) & 1u);
             }
             __syncwarp();
+        } else if (warp >= kThreads / 32 - kScaleWarps) {
+            // Each of these warps takes every other group, four rows a lane: under way while tiles
+            // stream past, such a load takes up to 2000 cycles.
+            dev::wait_for_previous();
+            int count = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
+                int tm, tn;
+                place_of(tile, p.tiles_m, tiles_n, tm, tn);
+                const int row = tm * kM + rank * 128 + lane, block_n = tn * (kN / kBlock), last_n = (p.n - 1) / kBlock;
+                const float* sb = p.b_scales + (int64_t)block_n * p.blocks;
+                const float* sb1 = p.b_scales + (int64_t)min(block_n + 1, last_n) * p.blocks;
+                for (int i = 0; i < p.blocks; i += kGroup, ++count) {
+                    if (count % kScaleWarps != kThreads / 32 - 1 - warp) continue;
+                    float a[4][kGroup], b0[kGroup], b1[kGroup];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        load_scales(p.a_scales + (int64_t)min(row + 32 * r, p.m - 1) * p.blocks, i, p.blocks, p.a_wide, a[r]);
+                    load_scales(sb, i, p.blocks, p.b_wide, b0), load_scales(sb1, i, p.blocks, p.b_wide, b1);
+                    const int group = count % kGroups;
+                    ok = __all_sync(kFull, dev::mbar_wait(&sh.scales_free[group], ~(count / kGroups) & 1u, abort, p.err));
+                    if (!ok) break;
+                    float* to = scales + group * kGroup * 256 + lane;
+#pragma unroll
+                    for (int k = 0; k < kGroup; ++k)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            to[k * 256 + 32 * r] = a[r][k] * b0[k], to[k * 256 + 128 + 32 * r] = a[r][k] * b1[k];
+                    __syncwarp();
+                    if (lane == 0) dev::mbar_arrive(&sh.scales_full[group]);
+                }
+            }
         } else if (warp == kProductWarp && rank == 0) {
             constexpr uint32_t idesc = dev::f16_idesc(kM, kN, false);
             const uint64_t a_desc = dev::smem_desc(dev::smem_addr(smem), 16, 1024, dev::kLayoutSwizzle128);
@@ -491,8 +553,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             bool ok = true;
             for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
                 for (int i = 0; i < p.blocks; ++i) {
-                    ok = __all_sync(kFull, dev::mbar_wait_lean(&sh.taken[buffer], taken_phase, abort, p.err)) &&
-                         __all_sync(kFull, dev::mbar_wait_lean(&sh.full[stage], phase, abort, p.err));
+                    ok = __all_sync(kFull, dev::mbar_wait_lean(&sh.full[stage], phase, abort, p.err)) &&
+                         __all_sync(kFull, dev::mbar_wait_lean(&sh.taken[buffer], taken_phase, abort, p.err));
                     if (!ok) break;
                     dev::tc_fence_after();
                     if (dev::elect_one()) {
@@ -590,7 +652,7 @@ int gemm_fp8(const GemmFp8& g, bool follows, cudaStream_t stream) {
     p.out_stride = g.out_stride;
     p.dtype = g.dtype;
     p.out_vec = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % (4 * size) == 0;
-    p.out_wide = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % 32 == 0;
+    p.out_wide = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % 16 == 0;
     p.a_wide = p.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(g.a_scales) % 16 == 0;
     p.b_wide = p.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(g.b_scales) % 16 == 0;
     p.err = device_error_word();

@@ -127,7 +127,7 @@ def product_limit(torch, a, b, blocks, dtype, want):
 
 
 SIZES = [(1, 1, 16), (1, 128, 128), (3, 130, 144), (64, 256, 1024), (128, 127, 2048), (129, 129, 400), (200, 64, 4096),
-         (777, 1003, 1040), (1, 4096, 4096), (17, 1000, 16384), (512, 2304, 640), (2500, 640, 256), (33, 8, 112)]
+         (777, 1003, 1040), (1, 4096, 4096), (17, 1000, 16384), (512, 2304, 640), (2500, 640, 256), (33, 8, 112), (2100, 2561, 400), (4097, 1300, 1040), (300, 16500, 128)]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
