@@ -82,56 +82,65 @@ __device__ __forceinline__ void load_scales(const float* p, int i, int count, bo
     }
 }
 
-// 32 rows of N elements, a row a lane, to the output, by way of 4 KB of shared memory: 128 bytes
-// of each row at a time, which leave as whole lines.  (As 32 bytes a lane, a row each, the
-// 256 x 256 tile's rows took 4100 cycles.)  Rows from `rows` on are left out.
-template <int N>
-__device__ __forceinline__ void store_rows(const GemmFp8Params& p, uint8_t* stage, int row0, int rows, int col,
-                                           const float2 (&x)[N / 2]) {
-    const int lane = threadIdx.x & 31, size = p.dtype == MXK_F32 ? 4 : 2;
-    auto line = [&](int c) {  // the line that begins at element c
-        __syncwarp();
-        const int per = 16 / size, chunk = lane & 7, at = col + c + chunk * per;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + (lane >> 3);
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((chunk ^ (r & 7)) << 4));
-            if (r >= rows || at >= p.n) continue;
-            char* to = p.out + ((int64_t)(row0 + r) * p.out_stride + at) * size;
-            if (p.out_wide && at + per <= p.n) {
-                *reinterpret_cast<uint4*>(to) = v;
-            } else {
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    if (size == 2 && at + k < p.n) reinterpret_cast<uint16_t*>(to)[k] = (uint16_t)(w[k / 2] >> (16 * (k & 1)));
-                    if (size == 4 && k < 4 && at + k < p.n) reinterpret_cast<uint32_t*>(to)[k] = w[k & 3];
-                }
-            }
-        }
+// 32 rows of 128 elements, a row a lane, to the output, by way of 8 KB of shared memory.  Where
+// the output is aligned they leave as asynchronous copies and the warp goes on; the next call
+// waits until they have been read.  (With stores the warps of all CTAs wait at about the same time:
+// 4500 cycles of 50,000.  So they do for a copy from each lane, which are issued one by one.)
+// 16-byte pieces of a row are permuted by row, so that eight lanes write to different banks.
+__device__ __forceinline__ void store_rows(const GemmFp8Params& p, const CUtensorMap* map, uint8_t* stage, int row0,
+                                           int col, const float2 (&x)[64]) {
+    constexpr int kPart = 32 * 128;  // bytes of 32 rows' 128 bytes each
+    const int lane = threadIdx.x & 31, size = p.dtype == MXK_F32 ? 4 : 2, part = 128 / size;
+    auto piece = [&](int row, int i) { return stage + i / 8 * kPart + row * 128 + (((i ^ row) & 7) << 4); };
+    auto wait_for_copies = [&]() {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
     };
-    uint8_t* mine = stage + lane * 128;
-    if (size == 4) {
-#pragma unroll
-        for (int c = 0; c < N; c += 32) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<float4*>(mine + ((i ^ (lane & 7)) << 4)) =
-                    make_float4(x[c / 2 + 2 * i].x, x[c / 2 + 2 * i].y, x[c / 2 + 2 * i + 1].x, x[c / 2 + 2 * i + 1].y);
-            line(c);
+    auto send = [&](int at) {  // two parts, which begin with element `at` of the row
+        if (p.out_wide) dev::fence_proxy_async();
+        __syncwarp();
+        if (row0 >= p.m) return;
+        if (p.out_wide) {
+            if (lane == 0) {
+                for (int i = 0; i < 2; ++i)
+                    if (at + i * part < p.n)
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map),
+                                     "r"(at + i * part), "r"(row0), "r"(dev::smem_addr(stage + i * kPart))
+                                     : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+            return;
         }
+        const int rows = min(p.m - row0, 32), count = min(p.n - at, 2 * part);
+        for (int r = 0; r < rows; ++r)
+            for (int c = lane; c < count; c += 32) {
+                const uint8_t* from = piece(r, c * size / 16) + c * size % 16;
+                char* to = p.out + ((int64_t)(row0 + r) * p.out_stride + at + c) * size;
+                if (size == 4)
+                    *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+                else
+                    *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+            }
+    };
+    wait_for_copies();
+    if (size == 4) {  // two halves
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            *reinterpret_cast<float4*>(piece(lane, i)) = make_float4(x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y);
+        send(col);
+        wait_for_copies();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            *reinterpret_cast<float4*>(piece(lane, i)) =
+                make_float4(x[32 + 2 * i].x, x[32 + 2 * i].y, x[33 + 2 * i].x, x[33 + 2 * i].y);
+        send(col + 64);
     } else {
 #pragma unroll
-        for (int c = 0; c < N; c += 64) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint2 u = pack4(p.dtype, x[c / 2 + 4 * i], x[c / 2 + 4 * i + 1]);
-                const uint2 v = pack4(p.dtype, x[c / 2 + 4 * i + 2], x[c / 2 + 4 * i + 3]);
-                *reinterpret_cast<uint4*>(mine + ((i ^ (lane & 7)) << 4)) = make_uint4(u.x, u.y, v.x, v.y);
-            }
-            line(c);
+        for (int i = 0; i < 16; ++i) {
+            const uint2 u = pack4(p.dtype, x[4 * i], x[4 * i + 1]), v = pack4(p.dtype, x[4 * i + 2], x[4 * i + 3]);
+            *reinterpret_cast<uint4*>(piece(lane, i)) = make_uint4(u.x, u.y, v.x, v.y);
         }
+        send(col);
     }
 }
 
@@ -369,7 +378,7 @@ namespace pair {
 // A pair of CTAs holds 256 rows and 256 columns: each loads its 128 rows of A and 128 of the 256
 // rows of B, which the pair's products read from both.  The pairs stay and go from tile to tile.
 constexpr int kM = 256, kN = 256;
-constexpr int kStages = 5, kBuffers = 2;
+constexpr int kStages = 4, kBuffers = 2;
 constexpr int kSide = 128 * kBlock;  // bytes of an operand's tile in one CTA
 constexpr int kStage = 2 * kSide;
 constexpr int kSumWarps = 8, kLoadWarp = 8, kProductWarp = 9, kThreads = 384;
@@ -378,7 +387,7 @@ static_assert(256 * kSumRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "");
 constexpr int kCols = kN / 2;        // columns of a warp: four lane quarters, two halves
 constexpr int kGroup = 4, kGroups = 4;  // blocks whose scales come together; groups at hand
 constexpr int kScales = kGroups * kGroup * 2 * 128 * 4;  // bytes
-constexpr int kSmem = kStages * kStage + kScales + kSumWarps * 4096 + 1024;  // 1024: alignment
+constexpr int kSmem = kStages * kStage + kScales + kSumWarps * 8192 + 1024;  // 1024: alignment
 constexpr int kScaleWarps = 2;          // the last two
 constexpr int kRaster = 8;           // row tiles that are gone through side by side
 
@@ -403,7 +412,7 @@ __device__ __forceinline__ void place_of(int tile, int tiles_m, int tiles_n, int
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                         const GemmFp8Params p) {
+                         const __grid_constant__ CUtensorMap map_out, const GemmFp8Params p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared sh;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -482,8 +491,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (++group == kGroups) group = 0, group_phase ^= 1;
                 }
             }
-            if (ok) store_rows<kCols>(p, out_stage + warp * 4096, row0, p.m - row0, col, acc);
+            if (ok) store_rows(p, &map_out, out_stage + warp * 8192, row0, col, acc);
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kLoadWarp) {
@@ -614,13 +624,20 @@ int launch(const GemmFp8& g, GemmFp8Params p, bool follows, cudaStream_t stream)
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kSmem;
     cfg.stream = stream;
+    CUtensorMap map_out{};
+    if (p.out_wide) {
+        const bool full = p.dtype == MXK_F32;
+        MXK_CHECK(encode_tensor_map_2d(&map_out, g.out, (uint64_t)g.n, (uint64_t)g.m, (uint64_t)g.out_stride * (full ? 4 : 2),
+                                       full ? 32 : 64, 32, full ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                                       CU_TENSOR_MAP_SWIZZLE_128B));
+    }
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = follows ? 1 : 0;
     LaunchScope scope("gemm_fp8_pair", stream);
-    MXK_CUDA(cudaLaunchKernelEx(&cfg, gemm_fp8_pair_kernel, map_a, map_b, p));
+    MXK_CUDA(cudaLaunchKernelEx(&cfg, gemm_fp8_pair_kernel, map_a, map_b, map_out, p));
     return MXK_OK;
 }
 
