@@ -63,14 +63,21 @@ struct AttentionParams {
 
 // A call whose sequences share prefixes.  Its units belong to parts of the sequences' tokens:
 // part g < groups is the prefix of group g, seen by all its sequences' rows, part groups + i
-// what sequence i has behind it.  `seqs` counts the parts.  Rows come out in float32 with
-// their lse, those of the prefixes before those of the rest, and are joined by
-// attention_merge_kernel (attention_shared.cu).
+// what sequence i has behind it.  `seqs` counts the parts.  The rows of units that one CTA has to
+// itself come out in float32 with their maxima and sums, those of the prefixes before those of
+// the rest; for all rows `where` tells attention_merge_kernel (attention_shared.cu), which joins
+// what there is of a row, where that lies.
 struct SharedParams : AttentionParams {
+    float2* row_stat;  // [2][tokens][heads]: as part_stat
+    int4* where;       // [2][tokens][heads]: {kernel of the call, or -1: the row is whole, -2: no such row;
+                       // CTA that began the unit; CTAs that went on with it; row in its tile, and kHasPrefix}
+    int kernel;        // of the call: 0, 1, ...
     const int4* parts;  // two to a part: {first row, rows, tokens end, position of the first row},
                         // {first token, page table row, 0, 0}
     int groups, max_prefix;
 };
+
+constexpr int kHasPrefix = 1 << 30;  // what the row sees of the prefix comes to it
 
 // Key tiles there can be at most when no sequence has more than max_q query and
 // p.max_kv cached tokens, and all of them p.tokens query tokens: a window touches at
@@ -392,6 +399,65 @@ __device__ __forceinline__ void walk_on(const P& p, Walk<P>& w) {
     w.tiles = tile_count<ROWS, KEYS>(p, w.view, w.rt, &w.first);
 }
 
+// Shares cut at the ends of units, for calls with many short ones: a unit that counts no more
+// than a share is all its CTA's in whose share more than half of it lies (of two halves, the
+// first), and nothing of it has to be joined.  `left` as the walk's: positions of the share after
+// the unit's cost.  WholeUnits::begin and ::next return whether the CTA has a (next) unit.
+template <int ROWS, int KEYS>
+struct WholeUnits {
+    template <class P>
+    static __device__ __forceinline__ bool fits(const Share& s, const Walk<P>& w) {
+        return w.tiles + s.cost <= s.each;
+    }
+    // At the beginning of a unit of which `left + cost` positions are in the share.
+    template <class P>
+    static __device__ __forceinline__ bool mine(const Share& s, const Walk<P>& w, int left) {
+        return fits(s, w) ? 2 * (left + s.cost) >= w.tiles + s.cost : left > 0;
+    }
+    template <class P>
+    static __device__ __forceinline__ bool next(const P& p, const Share& s, Walk<P>& w, int left) {
+        if (left + s.cost <= 0) return false;
+        walk_on<ROWS, KEYS>(p, w);
+        return mine(s, w, left);
+    }
+    template <class P>
+    static __device__ __forceinline__ bool begin(const P& p, const Share& s, Walk<P>& w, int& left) {
+        const int before = w.tile > 0 ? w.tile + s.cost : s.cost - w.skip;  // positions of the unit in earlier shares
+        if (before == 0 || !fits(s, w)) return left > 0;
+        if (2 * before < w.tiles + s.cost) {
+            w.tile = 0;
+            left = s.tiles + before - s.cost;
+            return true;
+        }
+        left = s.tiles - (w.tiles + s.cost - before) - s.cost;
+        return next(p, s, w, left);
+    }
+};
+
+// log(sum exp) of a row from its running maximum (log2 units) and sum.
+__device__ __forceinline__ float row_lse(float m2, float sum) {
+    return sum > 0.0f ? (m2 - kExpShift) * 0.693147180559945f + logf(sum)
+                      : (sum == 0.0f ? __int_as_float(0xff800000) : sum);
+}
+
+// What is known of the weights of a row that is whole, with its output.
+__device__ __forceinline__ void store_stat(const AttentionParams& p, const SeqView&, int64_t row, int head, float top,
+                                           float total) {
+    if (p.lse) p.lse[row * p.heads + head] = row_lse(top, total);
+}
+__device__ __forceinline__ void store_stat(const SharedParams& p, const PartView& view, int64_t row, int head, float top,
+                                           float total) {
+    p.row_stat[row * p.heads + head] = make_float2(top, total);
+    p.where[row * p.heads + head] = make_int4(-1, 0, 0, view.start > 0 ? kHasPrefix : 0);
+}
+// Where the parts of a row are that this CTA began and `followers` went on with.
+__device__ __forceinline__ void store_where(const AttentionParams&, const SeqView&, int64_t, int, int, int) {}
+__device__ __forceinline__ void store_where(const SharedParams& p, const PartView& view, int64_t row, int head,
+                                            int in_tile, int followers) {
+    p.where[row * p.heads + head] =
+        make_int4(p.kernel, (int)blockIdx.x, followers, in_tile | (view.start > 0 ? kHasPrefix : 0));
+}
+
 // Four consecutive features of an output row.
 __device__ __forceinline__ void store4_at(const AttentionParams& p, int64_t at, float4 v) {
     uint16_t h[4];
@@ -420,12 +486,6 @@ __device__ __forceinline__ void store4(const P& p, int64_t token, int head, int 
     store4_at(p, token * p.out_token + (int64_t)head * p.out_head + feature, v);
 }
 
-// log(sum exp) of a row from its running maximum (log2 units) and sum.
-__device__ __forceinline__ float row_lse(float m2, float sum) {
-    return sum > 0.0f ? (m2 - kExpShift) * 0.693147180559945f + logf(sum)
-                      : (sum == 0.0f ? __int_as_float(0xff800000) : sum);
-}
-
 }  // namespace dev
 
 // The partial sums of one kernel's CTAs: as in AttentionParams.
@@ -437,22 +497,20 @@ struct Parts {
     int split;       // CTAs that join a unit
 };
 constexpr int kMostParts = 3;  // kernels of a call
-template <class P>
 struct JoinParams {
-    P p;
+    AttentionParams p;
     Parts parts[kMostParts];
     int count;
 };
 
 // A row of a joined unit; total: the sum of its weights relative to `top`.
-template <class P, class V>
-__device__ __forceinline__ void store_joined(const P& p, const int4& unit, const V& view, int row, int chunk, float4 v, float top, float total) {
+__device__ __forceinline__ void store_joined(const AttentionParams& p, const int4& unit, const dev::SeqView& view, int row, int chunk, float4 v, float top, float total) {
     const int j = row / p.group;
     const int head = unit.z * p.group + (row - j * p.group);
     if (total == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const int64_t to = dev::out_row(p, view) + j;
     dev::store4(p, to, head, chunk * 4, v);
-    if (p.lse && chunk == 0) p.lse[to * p.heads + head] = dev::row_lse(top, total);
+    if (chunk == 0) dev::store_stat(p, view, to, head, top, total);
 }
 
 // Block (x, y) of a set of parts: the unit that CTA x began and did not finish, some of its
@@ -461,9 +519,9 @@ __device__ __forceinline__ void store_joined(const P& p, const int4& unit, const
 // go through its parts.  Many: the block takes a row, every D / 4 of its threads some of the
 // parts, so a unit in hundreds of parts has several loads under way.  One launch joins the
 // parts of all of a call's kernels: a launch for each took 5 us more a kernel.
-template <int D, class P>
-__global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams<P> jp) {
-    const P& p = jp.p;
+template <int D>
+__global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams jp) {
+    const AttentionParams& p = jp.p;
     constexpr int kLanes = D / 4;            // threads of a row
     constexpr int kSub = 128 / kLanes;       // rows, or parts, at a time
     constexpr int kFew = 8;
@@ -478,7 +536,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams<P>
     dev::wait_for_previous();
     const int4 unit = set.open[x];
     if (!unit.w) return;
-    const auto view = dev::seq_view(p, unit.x);
+    const dev::SeqView view = dev::seq_view(p, unit.x);
     const int rows = min(view.n * p.group - unit.y * set.rows, set.rows);
     const int tid = threadIdx.x, chunk = tid % kLanes, sub = tid / kLanes, parts = unit.w + 1;
     auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(x + i) + (i == 0 ? 1 : 0); };
@@ -584,6 +642,7 @@ public:
         MXK_CUDA(cudaMallocFromPoolAsync(&ptr, own + (size_t)extra_bytes, pool, stream_));
         block_[blocks_++] = ptr;
         if (extra) *extra = static_cast<char*>(ptr) + own;
+        number(p, join_.count);
         p.part = static_cast<float*>(ptr);
         p.part_stat = reinterpret_cast<float2*>(static_cast<char*>(ptr) + part);
         p.part_open = reinterpret_cast<int4*>(static_cast<char*>(ptr) + part + stat);
@@ -626,19 +685,22 @@ public:
         join_.p = p;
         join_.parts[join_.count++] = Parts{p.part, p.part_stat, p.part_open, (int)ctas, rows, (int)split};
     }
+    const Parts* parts() const { return join_.parts; }
     int join_all(int d) {
         if (!join_.count) return MXK_OK;
         int64_t blocks = 0;
         for (int i = 0; i < join_.count; ++i) blocks += (int64_t)join_.parts[i].ctas * join_.parts[i].split;
-        return launch("attention_join", d == 128 ? attention_join_kernel<128, P> : attention_join_kernel<64, P>,
+        return launch("attention_join", d == 128 ? attention_join_kernel<128> : attention_join_kernel<64>,
                       (unsigned)blocks, 128, 0, join_);
     }
 
 private:
+    static void number(AttentionParams&, int) {}
+    static void number(SharedParams& p, int kernel) { p.kernel = kernel; }
     cudaStream_t stream_;
     bool first_ = true;
     void* block_[kMostParts + 1] = {};
-    JoinParams<P> join_{};
+    JoinParams join_{};
     int blocks_ = 0;
 };
 
@@ -647,7 +709,7 @@ private:
 template <class P>
 int launch_attention_tiles(int bits, int head_dim, P p, int max_q, int max_rows, AttentionCall<P>& call);
 
-// attention.cu: few query rows, and all of a call's kernels; max_rows as above.
+// attention.cu: few query rows, and all of a call's kernels but the join; max_rows as above.
 template <class P>
 int launch_attention(const mxk_cache& cache, P p, int max_rows, AttentionCall<P>& call);
 

@@ -12,8 +12,10 @@
 // seen by a prefix's rows.
 //
 //   attention_parts_kernel   lengths to parts, on the device: graphs replay as they grow
-//   the attention kernels    rows in float32 with their log-sums, prefixes' and own
-//   attention_merge_kernel   the formula above, a row by D / 4 threads
+//   the attention kernels    rows in float32 with their maxima and sums, whole or in parts, prefixes'
+//                            and own, and where they are
+//   attention_merge_kernel   everything there is of a row, by the formula above
+#include <algorithm>
 #include <limits>
 
 #include "attention.cuh"
@@ -22,6 +24,7 @@ namespace mxk {
 namespace {
 
 constexpr int kTile = 128;  // tokens that prefixes are multiples of: a key tile
+constexpr int64_t kFewRows = 2048;
 
 struct PartsParams {
     const int* cu_q;
@@ -29,11 +32,20 @@ struct PartsParams {
     const int* cu_groups;
     const int* prefix_lens;
     int4* parts;
+    int4* where;  // the sequences' side
+    int64_t rows;
     int tokens, seqs, groups, max_q, max_kv, max_prefix;
 };
 
-// One block: the sequences' parts, a thread each, then the groups', a warp each.
+// Block 0: the sequences' parts, a thread each, then the groups', a warp each.  The others: no row
+// is anywhere yet (a row behind the last sequence stays so).
+constexpr int kClear = 4096;  // rows of a block
 __global__ void __launch_bounds__(1024) attention_parts_kernel(const PartsParams p) {
+    if (blockIdx.x > 0) {
+        const int64_t first = (int64_t)(blockIdx.x - 1) * kClear, end = min(first + kClear, p.rows);
+        for (int64_t i = first + threadIdx.x; i < end; i += blockDim.x) p.where[i] = make_int4(-2, 0, 0, 0);
+        return;
+    }
     AttentionParams a{};  // (for seq_view)
     a.cu_q = p.cu_q, a.kv_lens = p.kv_lens, a.tokens = p.tokens, a.max_q = p.max_q, a.max_kv = p.max_kv;
     for (int i = threadIdx.x; i < p.seqs; i += blockDim.x) {
@@ -67,51 +79,98 @@ __global__ void __launch_bounds__(1024) attention_parts_kernel(const PartsParams
 }
 
 struct MergeParams {
-    AttentionParams p;  // the caller's queries and outputs
-    const float* rows;  // [2][tokens][heads][D]
-    const float* lse;   // [2][tokens][heads]
-    const int4* parts;
-    int groups;
+    AttentionParams p;    // the caller's queries and outputs
+    const float* rows;    // [2][tokens][heads][D]
+    const float2* stat;   // [2][tokens][heads]
+    const int4* where;    // [2][tokens][heads]
+    Parts parts[kMostParts];
 };
 
+// What there is of a row: means, maxima and sums from one slot of the workspace to the next.
 template <int D>
-__global__ void __launch_bounds__(128) attention_merge_kernel(const MergeParams m) {
-    const AttentionParams& p = m.p;
-    constexpr int kLanes = D / 4;
-    const int64_t all = p.tokens * p.heads, row = (int64_t)blockIdx.x * (128 / kLanes) + threadIdx.x / kLanes;
-    if (row >= all) return;
-    const int chunk = threadIdx.x % kLanes, token = (int)(row / p.heads), head = (int)(row - (int64_t)token * p.heads);
-    // the token's sequence: the last that begins at it or before
-    int seq = -1, after = p.seqs;
-    while (after - seq > 1) {
-        const int mid = (seq + after) / 2;
-        (__ldg(p.cu_q + mid) <= token ? seq : after) = mid;
-    }
-    if (seq < 0) return;
-    const int first = max(__ldg(p.cu_q + seq), 0);
-    if (token >= __ldg(p.cu_q + seq + 1) || token - first >= p.max_q) return;
-    dev::wait_for_previous();
-    float4 v = reinterpret_cast<const float4*>(m.rows + (all + row) * D)[chunk];
-    float lse = m.lse[all + row];
-    if (m.parts[2 * (m.groups + seq) + 1].x > 0) {
-        const float4 u = reinterpret_cast<const float4*>(m.rows + row * D)[chunk];
-        const float other = m.lse[row], top = fmaxf(lse, other);
-        if (top > __int_as_float(0xff800000)) {
-            const float f = expf(lse - top), g = expf(other - top), sum = f + g, inv = 1.0f / sum;
-            // (a part that weighs nothing has no say, whatever it holds)
-            const float a = f * inv, b = g * inv;
-            v.x = (a == 0.0f ? 0.0f : a * v.x) + (b == 0.0f ? 0.0f : b * u.x);
-            v.y = (a == 0.0f ? 0.0f : a * v.y) + (b == 0.0f ? 0.0f : b * u.y);
-            v.z = (a == 0.0f ? 0.0f : a * v.z) + (b == 0.0f ? 0.0f : b * u.z);
-            v.w = (a == 0.0f ? 0.0f : a * v.w) + (b == 0.0f ? 0.0f : b * u.w);
-            lse = top + logf(sum);
-        } else if (other != other || lse != lse) {
-            lse = other + lse;
-            v = make_float4(lse, lse, lse, lse);
+struct Found {
+    const float* mean;
+    const float2* stat;
+    int count, rows;  // rows: of a slot; 0: the row is whole
+    __device__ __forceinline__ Found(const MergeParams& m, const int4& w, int64_t at) {
+        // (What a wait that gave up left unwritten is not followed out of the workspace.)
+        const Parts& set = m.parts[min(max(w.x, 0), kMostParts - 1)];
+        if (w.x < 0 || !set.part) {
+            mean = m.rows + at * D, stat = m.stat + at, count = w.x == -2 ? 0 : 1, rows = 0;
+        } else {
+            const int x = min(max(w.y, 0), set.ctas - 1), r = min(w.w & (kHasPrefix - 1), set.rows - 1);
+            mean = set.part + ((int64_t)2 * x * set.rows + r) * D, stat = set.stat + (int64_t)2 * x * set.rows + r;
+            count = min(max(w.z, 0), set.ctas - 1 - x) + 1, rows = set.rows;
         }
     }
+    // Its i-th part: the beginning in the second slot of its CTA, the others in the first of theirs.
+    __device__ __forceinline__ int64_t slot(int i) const { return rows ? (2 * (int64_t)i + (i == 0 ? 1 : 0)) * rows : 0; }
+};
+
+// A row of the output, by SPLIT warps, every D / 4 threads of which take some of its parts.  They
+// add up in a fixed order.
+template <int D, int SPLIT>
+__global__ void __launch_bounds__(128) attention_merge_kernel(const MergeParams m) {
+    const AttentionParams& p = m.p;
+    constexpr int kLanes = D / 4, kSub = 32 * SPLIT / kLanes, kAtOnce = 4 / SPLIT;  // parts, rows at a time
+    __shared__ float4 sums[kAtOnce][kSub][kLanes];
+    const int tid = threadIdx.x % (32 * SPLIT), lane = threadIdx.x & 31, chunk = tid % kLanes, sub = tid / kLanes;
+    const int64_t all = p.tokens * p.heads, row = (int64_t)blockIdx.x * kAtOnce + threadIdx.x / (32 * SPLIT);
+    dev::wait_for_previous();
+    if (row >= all) return;
+    const int4 at_own = m.where[all + row], at_prefix = m.where[row];
+    if (at_own.x == -2) return;
+    const Found<D> own(m, at_own, all + row);
+    Found<D> prefix(m, at_prefix, row);
+    if (!(at_own.w & kHasPrefix)) prefix.count = 0;
+    const int count = prefix.count + own.count;
+    auto stat_of = [&](int i) -> float2 {
+        return i < prefix.count ? prefix.stat[prefix.slot(i)] : own.stat[own.slot(i - prefix.count)];
+    };
+    // the common maximum and the sum of the weights (every warp, all parts)
+    const float neg_inf = __int_as_float(0xff800000);
+    const float2 mine = lane < count ? stat_of(lane) : make_float2(neg_inf, 0.0f);
+    float top = mine.x;
+    for (int i = lane + 32; i < count; i += 32) top = fmaxf(top, stat_of(i).x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    auto weight = [&](float2 st) { return st.y * (st.x == top ? 1.0f : dev::ex2(st.x - top)); };
+    const float first = weight(mine);
+    float total = first;
+    for (int i = lane + 32; i < count; i += 32) total += weight(stat_of(i));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int base = 0; base < count; base += kSub) {
+        const int i = base + sub;
+        float f = __shfl_sync(0xffffffffu, first, i & 31);
+        if (i >= count) f = 0.0f;
+        if (i >= 32 && i < count) f = weight(stat_of(i));
+        if (f == 0.0f) continue;  // a part that weighs nothing has no say, whatever it holds
+        const float* at = i < prefix.count ? prefix.mean + prefix.slot(i) * D : own.mean + own.slot(i - prefix.count) * D;
+        const float4 o = reinterpret_cast<const float4*>(at)[chunk];
+        f *= inv;
+        v.x += o.x * f, v.y += o.y * f, v.z += o.z * f, v.w += o.w * f;
+    }
+    if (kSub > 1) {
+        float4 (*all_sums)[kLanes] = sums[threadIdx.x / (32 * SPLIT)];
+        all_sums[sub][chunk] = v;
+        if (SPLIT == 1)
+            __syncwarp();
+        else
+            __syncthreads();
+        if (sub > 0) return;
+#pragma unroll
+        for (int i = 1; i < kSub; ++i) {
+            const float4 o = all_sums[i][chunk];
+            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+        }
+    }
+    const int token = (int)(row / p.heads), head = (int)(row - (int64_t)token * p.heads);
     dev::store4(p, token, head, chunk * 4, v);
-    if (p.lse && chunk == 0) p.lse[row] = lse;
+    if (p.lse && chunk == 0) p.lse[row] = dev::row_lse(top, total);
 }
 
 }  // namespace
@@ -137,33 +196,40 @@ extern "C" int mxk_cache_attention_shared(const mxk_cache* cache, const mxk_atte
     const int64_t max_prefix = std::min<int64_t>(prefixes->max_prefix, p.max_kv) / kTile * kTile;
     if (prefixes->groups == 0 || p.seqs < 2 || max_prefix == 0) {  // nothing to share
         AttentionCall<AttentionParams> call(as_stream(stream));
-        return launch_attention(*cache, p, 0, call);
+        MXK_CHECK(launch_attention(*cache, p, 0, call));
+        return call.join_all(cache->head_dim);
     }
 
     AttentionCall<SharedParams> call(as_stream(stream));
     const int64_t rows = p.tokens * p.heads, parts = (int64_t)prefixes->groups + p.seqs;
-    const size_t out_bytes = (size_t)rows * 2 * cache->head_dim * 4, lse_bytes = ((size_t)rows * 8 + 15) / 16 * 16;
+    const size_t out_bytes = (size_t)rows * 2 * cache->head_dim * 4;
     void* room = nullptr;
-    MXK_CHECK(call.room(out_bytes + lse_bytes + (size_t)parts * 32, &room));
+    MXK_CHECK(call.room(out_bytes + (size_t)rows * 48 + (size_t)parts * 32, &room));
     SharedParams s;
     static_cast<AttentionParams&>(s) = p;
     s.out = room;
-    s.lse = reinterpret_cast<float*>(static_cast<char*>(room) + out_bytes);
-    int4* list = reinterpret_cast<int4*>(static_cast<char*>(room) + out_bytes + lse_bytes);
+    int4* list = reinterpret_cast<int4*>(static_cast<char*>(room) + out_bytes);
     s.parts = list;
+    s.where = list + 2 * parts;
+    s.row_stat = reinterpret_cast<float2*>(s.where + 2 * rows);
     s.out_token = (int64_t)p.heads * cache->head_dim, s.out_head = cache->head_dim;
     s.groups = prefixes->groups, s.max_prefix = (int)max_prefix;
     s.seqs = (int)parts;
-    const PartsParams pp{p.cu_q, p.kv_lens, prefixes->cu_groups, prefixes->prefix_lens, list,
+    const PartsParams pp{p.cu_q, p.kv_lens, prefixes->cu_groups, prefixes->prefix_lens, list, s.where + rows, rows,
                          (int)p.tokens, p.seqs, s.groups, p.max_q, p.max_kv, s.max_prefix};
     {
         LaunchScope scope("attention_parts", as_stream(stream));
-        attention_parts_kernel<<<1, 1024, 0, as_stream(stream)>>>(pp);
+        attention_parts_kernel<<<(unsigned)(1 + (rows + kClear - 1) / kClear), 1024, 0, as_stream(stream)>>>(pp);
         MXK_CUDA(cudaGetLastError());
     }
     MXK_CHECK(launch_attention(*cache, s, (int)p.tokens, call));
-    const int at_once = 128 / (cache->head_dim / 4);
-    const MergeParams m{p, static_cast<const float*>(room), s.lse, list, s.groups};
-    return call.launch("attention_merge", cache->head_dim == 128 ? attention_merge_kernel<128> : attention_merge_kernel<64>,
+    MergeParams m{p, static_cast<const float*>(room), s.row_stat, s.where, {}};
+    std::copy(call.parts(), call.parts() + kMostParts, m.parts);
+    // With few rows all four warps of a block take parts of one, else one each.
+    const bool few = rows <= kFewRows;
+    const int at_once = few ? 1 : 4;
+    return call.launch("attention_merge",
+                       cache->head_dim == 128 ? (few ? attention_merge_kernel<128, 4> : attention_merge_kernel<128, 1>)
+                                              : (few ? attention_merge_kernel<64, 4> : attention_merge_kernel<64, 1>),
                        (unsigned)((rows + at_once - 1) / at_once), 128, 0, m);
 }

@@ -1473,10 +1473,14 @@ __device__ __forceinline__ bool softmax_role(const P& p, const Block& b, Cursor<
                     }
                 }
                 if (real) {
-                    if (!all)
+                    if (all) {
+                        dev::store_stat(p, c.w.view, dev::out_row(p, c.w.view) + j, head, run_max, sum);
+                    } else {
                         p.part_stat[slot * kRows + tile_row] = make_float2(run_max, sum);
-                    else if (p.lse)
-                        p.lse[(dev::out_row(p, c.w.view) + j) * p.heads + head] = dev::row_lse(run_max, sum);
+                        if (std::is_same<P, SharedParams>::value && c.tile0 == 0)
+                            dev::store_where(p, c.w.view, dev::out_row(p, c.w.view) + j, head, tile_row,
+                                             b.share.followers(b.share.tiles - c.left, c.w.tiles));
+                    }
                 }
             }
             dev::tc_fence_before();
