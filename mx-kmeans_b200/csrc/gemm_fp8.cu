@@ -14,7 +14,6 @@
 #include <algorithm>
 #include <limits>
 
-#include "cache_rows.cuh"
 #include "gemm_fp8.cuh"
 
 namespace mxk {
@@ -22,6 +21,14 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kBlock = 128;  // features of a scale
+
+// Rows that the kernel quantises itself.
+struct RowsToQuantize {
+    const void* x;
+    int64_t stride;  // elements
+    int dtype, wide; // wide: 16 features can be loaded 16 bytes at a time
+    int k;
+};
 
 struct GemmFp8Params {
     int m, n, blocks;        // blocks: of k
@@ -164,17 +171,53 @@ constexpr int kCols = kN / 2;                 // columns of a warp: four lane qu
 constexpr int kSmem = kStages * kStage + 1024;  // 1024: alignment
 static_assert(kN * kM * 4 <= kStages * kStage, "the sums go out through the operands' memory");
 
+// With few rows, and no more than kOwnBytes of them, a CTA quantises its part of them itself: they
+// lie before the operands' stages, which then hold B alone.
+constexpr int kOwnRows = 16, kOwnBytes = 32768, kOwnStages = 4;
+constexpr int kOwnSmem = kOwnBytes + kOwnStages * kSide + kOwnBytes / kBlock * 4 + 1024;
+static_assert(kN * kOwnRows * 4 <= kOwnStages * kSide, "");
+
 struct Shared {
-    uint64_t full[kStages], done[kStages];  // loaded; multiplied, so the sums are in TMEM
+    uint64_t full[kOwnStages], done[kOwnStages];  // loaded; multiplied, so the sums are in TMEM
     uint64_t taken[kBuffers];               // a buffer's sums have been read
+    uint64_t rows_ready;                    // the CTA's own rows are quantised
     uint64_t drain;
     int abort_word;
     uint32_t tmem;
 };
 
+// 16 features of a row of any type.
+__device__ __forceinline__ void load16(const RowsToQuantize& q, int64_t at, float (&v)[16]) {
+    if (q.dtype == MXK_F32) {
+        dev::Raw16<float, 16> wide;
+        dev::Raw16<float, 0> any;
+        const float* from = static_cast<const float*>(q.x) + at;
+        if (q.wide) wide.load(from), wide.to_float(v);
+        else any.load(from), any.to_float(v);
+    } else {
+        dev::Raw16<__half, 16> raw;
+        if (q.wide) {
+            raw.load(static_cast<const __half*>(q.x) + at);
+        } else {
+            dev::Raw16<__half, 0> any;
+            any.load(static_cast<const __half*>(q.x) + at);
+            raw.w[0] = any.w[0], raw.w[1] = any.w[1];
+        }
+        if (q.dtype == MXK_F16) {
+            raw.to_float(v);
+        } else {
+            dev::Raw16<__nv_bfloat16, 16> b;
+            b.w[0] = raw.w[0], b.w[1] = raw.w[1];
+            b.to_float(v);
+        }
+    }
+}
+
+template <bool OWN>
 __global__ void __launch_bounds__(kThreads, 2)
     gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                         const GemmFp8Params p, int split, int rows_loaded) {
+                         const GemmFp8Params p, const RowsToQuantize q, int split, int rows_loaded) {
+    constexpr int kDepth = OWN ? kOwnStages : kStages, kStep = OWN ? kSide : kStage;  // stages, and bytes of one
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) Shared sh;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -184,16 +227,24 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int first = (int)((int64_t)rank * p.blocks / split), last = (int)((int64_t)(rank + 1) * p.blocks / split);
     const int count = last - first;
     volatile int* abort = &sh.abort_word;
+    uint8_t* stages = OWN ? smem + kOwnBytes : smem;  // of operands, or B alone
+    const int row_bytes = rows_loaded * kBlock;       // of a block's own rows
+    float* own_scales = reinterpret_cast<float*>(smem + kOwnBytes + kOwnStages * kSide);  // [block][row]
+    const int sum_warps = OWN ? 2 : kSumWarps;        // own rows lie in the first quarter of the lanes
 
     if (tid == 0) {
         sh.abort_word = 0;
-        for (int i = 0; i < kStages; ++i) dev::mbar_init(&sh.full[i], 1), dev::mbar_init(&sh.done[i], 1);
-        for (int i = 0; i < kBuffers; ++i) dev::mbar_init(&sh.taken[i], kSumWarps);
+        for (int i = 0; i < kDepth; ++i) dev::mbar_init(&sh.full[i], 1), dev::mbar_init(&sh.done[i], 1);
+        for (int i = 0; i < kBuffers; ++i) dev::mbar_init(&sh.taken[i], sum_warps);
+        dev::mbar_init(&sh.rows_ready, kSumWarps);
         dev::mbar_init(&sh.drain, 1);
         dev::fence_barrier_init();
     }
     if (warp == kProductWarp) dev::tmem_alloc(&sh.tmem, kBuffers * kN);
-    if (warp == kLoadWarp && lane == 0) dev::prefetch_tensor_map(&map_a), dev::prefetch_tensor_map(&map_b);
+    if (warp == kLoadWarp && lane == 0) {
+        if (!OWN) dev::prefetch_tensor_map(&map_a);
+        dev::prefetch_tensor_map(&map_b);
+    }
     dev::tc_fence_before();
     __syncthreads();
     dev::tc_fence_after();
@@ -207,48 +258,51 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (warp == kLoadWarp) {
         if (dev::elect_one()) {
             // The weights are no output of the kernel before (which may be the quantiser).
-            const int early = min(count, kStages);
-            const uint32_t bytes = kSide + rows_loaded * kBlock;
-            for (int i = 0; i < early; ++i) {
-                dev::mbar_arrive_expect_tx(&sh.full[i], bytes);
-                dev::tma_load_2d(smem + i * kStage + kSide, &map_b, (first + i) * kBlock, tn * kN, &sh.full[i]);
-            }
+            const int early = min(count, kDepth);
+            const uint32_t bytes = kSide + (OWN ? 0 : row_bytes);
+            auto load_b = [&](int i, int stage) {
+                dev::mbar_arrive_expect_tx(&sh.full[stage], bytes);
+                dev::tma_load_2d(stages + stage * kStep + kStep - kSide, &map_b, (first + i) * kBlock, tn * kN, &sh.full[stage]);
+            };
+            auto load_a = [&](int i, int stage) {
+                if (!OWN) dev::tma_load_2d(stages + stage * kStep, &map_a, (first + i) * kBlock, tm * kM, &sh.full[stage]);
+            };
+            for (int i = 0; i < early; ++i) load_b(i, i);
             dev::wait_for_previous();
-            for (int i = 0; i < early; ++i)
-                dev::tma_load_2d(smem + i * kStage, &map_a, (first + i) * kBlock, tm * kM, &sh.full[i]);
+            for (int i = 0; i < early; ++i) load_a(i, i);
             int i = early, stage = 0;
             uint32_t phase = 0;
             for (; i < count; ++i) {
                 if (!dev::mbar_wait(&sh.done[stage], phase, abort, p.err)) break;
-                dev::mbar_arrive_expect_tx(&sh.full[stage], bytes);
-                dev::tma_load_2d(smem + stage * kStage + kSide, &map_b, (first + i) * kBlock, tn * kN, &sh.full[stage]);
-                dev::tma_load_2d(smem + stage * kStage, &map_a, (first + i) * kBlock, tm * kM, &sh.full[stage]);
-                if (++stage == kStages) stage = 0, phase ^= 1;
+                load_b(i, stage), load_a(i, stage);
+                if (++stage == kDepth) stage = 0, phase ^= 1;
             }
             if (*abort)
-                for (int k = max(i - kStages, 0); k < i; ++k) settle(&sh.full[k % kStages], (uint32_t)(k / kStages) & 1u);
+                for (int k = max(i - kDepth, 0); k < i; ++k) settle(&sh.full[k % kDepth], (uint32_t)(k / kDepth) & 1u);
         }
         __syncwarp();
     } else if (warp == kProductWarp) {
         constexpr uint32_t idesc = dev::f16_idesc(kM, kN, false);
         const uint64_t a_desc = dev::smem_desc(dev::smem_addr(smem), 16, 1024, dev::kLayoutSwizzle128);
+        const uint64_t b_desc = dev::smem_desc(dev::smem_addr(stages + kStep - kSide), 16, 1024, dev::kLayoutSwizzle128);
         int stage = 0, buffer = 0;
         uint32_t phase = 0, taken_phase = 1;
-        bool ok = true;
+        bool ok = !OWN || __all_sync(kFull, dev::mbar_wait(&sh.rows_ready, 0, abort, p.err));
         for (int i = 0; i < count && ok; ++i) {
             ok = __all_sync(kFull, dev::mbar_wait(&sh.taken[buffer], taken_phase, abort, p.err)) &&
                  __all_sync(kFull, dev::mbar_wait(&sh.full[stage], phase, abort, p.err));
             if (!ok) break;
             dev::tc_fence_after();
             if (dev::elect_one()) {
-                const uint64_t a = a_desc + (uint64_t)(stage * (kStage >> 4)), b = a + (kSide >> 4);
+                const uint64_t a = a_desc + (uint64_t)(OWN ? i * (row_bytes >> 4) : stage * (kStep >> 4));
+                const uint64_t b = b_desc + (uint64_t)(stage * (kStep >> 4));
 #pragma unroll
                 for (int k = 0; k < kBlock / 32; ++k)
                     dev::tc_mma_f8(tmem + buffer * kN, a + 2 * k, b + 2 * k, idesc, k > 0);
                 dev::tc_commit(&sh.done[stage]);
             }
             __syncwarp();
-            if (++stage == kStages) stage = 0, phase ^= 1;
+            if (++stage == kDepth) stage = 0, phase ^= 1;
             if (++buffer == kBuffers) buffer = 0, taken_phase ^= 1;
         }
         if (!ok && dev::elect_one()) {  // products in flight must not outlive the CTA's memory
@@ -259,20 +313,55 @@ __global__ void __launch_bounds__(kThreads, 2)
     } else {
         const int row = tm * kM + (warp & 3) * 32 + lane;
         const bool real = row < p.m;
-        const float* sa = p.a_scales + (int64_t)(real ? row : 0) * p.blocks + first;
+        const float* sa = OWN ? nullptr : p.a_scales + (int64_t)(real ? row : 0) * p.blocks + first;
         const float* sb = p.b_scales + (int64_t)tn * p.blocks + first;
         const uint32_t column = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * kCols;
         dev::wait_for_previous();
+        if constexpr (OWN) {
+            // Eight threads to a row of a block, 16 features each, which are one 16-byte piece of the
+            // swizzled tile.
+            const int items = count * rows_loaded;
+            for (int base = 0; base < items; base += kSumWarps * 4) {
+                const int item = base + (tid >> 3), sub = tid & 7;
+                const int block = item / rows_loaded, r = item - block * rows_loaded, f = (first + block) * kBlock + sub * 16;
+                float v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+                if (item < items && r < p.m && f < q.k) load16(q, r * q.stride + f, v);
+                float amax = dev::largest16(v);
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, o));
+                const float s = dev::fp8_scale(amax);
+                if (item < items) {
+                    *reinterpret_cast<uint4*>(smem + block * row_bytes + r * kBlock + ((sub ^ (r & 7)) << 4)) =
+                        q.dtype == MXK_F32 ? dev::fp8_codes16(v, s, amax) : dev::fp8_codes16_narrow(v, s, amax);
+                    if (sub == 0) own_scales[item] = s;
+                }
+            }
+            dev::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) dev::mbar_arrive(&sh.rows_ready);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kSumWarps) : "memory");  // all rows' scales are there
+        }
         float fa[4], fb[4];
-        load_scales(sa, 0, count, false, fa), load_scales(sb, 0, count, false, fb);
+        auto scales_of = [&](int i) {
+            if constexpr (OWN) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) fa[k] = real && i + k < count ? own_scales[(i + k) * rows_loaded + row] : 0.0f;
+            } else {
+                load_scales(sa, i, count, false, fa);
+            }
+            load_scales(sb, i, count, false, fb);
+        };
+        scales_of(0);
         int stage = 0, buffer = 0;
         uint32_t phase = 0;
-        bool ok = true;
+        bool ok = !OWN || (warp & 3) == 0;  // (no rows of its own: nothing to add up)
         for (int i0 = 0; i0 < count && ok; i0 += 4) {
             float f[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) f[k] = fa[k] * fb[k];
-            load_scales(sa, i0 + 4, count, false, fa), load_scales(sb, i0 + 4, count, false, fb);
+            scales_of(i0 + 4);
 #pragma unroll
             for (int at = 0; at < 4; ++at) {
                 if (i0 + at >= count) break;
@@ -292,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                     for (int k = 0; k < 16; ++k) acc[c + k] = fmaf(__uint_as_float(v[k]), f[at], acc[c + k]);
                 }
-                if (++stage == kStages) stage = 0, phase ^= 1;
+                if (++stage == kDepth) stage = 0, phase ^= 1;
                 if (++buffer == kBuffers) buffer = 0;
             }
         }
@@ -302,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (real) {
 #pragma unroll
             for (int c = 0; c < kCols / 4; ++c)
-                *reinterpret_cast<float4*>(smem + r * (kN * 4) + ((((warp >> 2) * (kCols / 4) + c) ^ (r & 7)) << 4)) =
+                *reinterpret_cast<float4*>(stages + r * (kN * 4) + ((((warp >> 2) * (kCols / 4) + c) ^ (r & 7)) << 4)) =
                     make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
         }
     }
@@ -312,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         __syncthreads();
     // The cluster's sums, each CTA its part of the tile's rows and chunks.
     const int rows = min(p.m - tm * kM, kM), total = rows * (kN / 4);
-    const uint32_t sums = dev::smem_addr(smem);
+    const uint32_t sums = dev::smem_addr(stages);
     const int end = (int)((int64_t)(rank + 1) * total / split);
     for (int i = (int)((int64_t)rank * total / split) + tid; i < end; i += kThreads) {
         const int r = i >> 5, c = i & 31;
@@ -334,37 +423,58 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (warp == kProductWarp) dev::tmem_dealloc(tmem, kBuffers * kN);
 }
 
-int launch(const GemmFp8& g, GemmFp8Params p, bool follows, cudaStream_t stream) {
-    CUtensorMap map_a, map_b;
+// Parts of k, as long as there are not many more CTAs than SMs and a part has two blocks.  In us
+// for 1, 2, 4 and 8: one row through 4096 x 4096 (32 tiles) 15.3, 10.6, 8.5, 8.8, through
+// 14,336 x 4096 (112) 17.4, 15.9, 19.2, 27.4; 64 rows through 6144 x 4096 (48) 17.5, 13.0, 12.0,
+// 18.0; 16 through 1024 x 4096 (8) 14.8, 10.1, 7.6, 6.6.
+int split_of(int64_t tiles, int blocks) {
+    static const int sms = sm_count();
+    int split = 1;
+    while (split < 8 && tiles * split * 10 <= 8 * sms && blocks >= 4 * split) split *= 2;
+    return split;
+}
+
+int64_t tiles_of(const GemmFp8& g) { return (g.m + kM - 1) / kM * ((g.n + kN - 1) / kN); }
+
+// Whether the CTAs quantise the rows themselves, which saves a launch and a workspace but holds the
+// products up by the rows' way through registers.  In us, from a loop of calls and (in a graph) on
+// the device alone, with and without: one row through 4096 x 4096 10.8 (10.5) and 16.7 (9.6),
+// through 14,336 x 4096 19.6 (19.6) and 17.3 (17.3).
+constexpr int64_t kOwnWeights = 32 << 20;
+bool own_rows(const GemmFp8& g, int blocks) {
+    const int split = split_of(tiles_of(g), blocks);
+    return g.m <= kOwnRows && g.n * g.k <= kOwnWeights &&
+           (g.m + 7) / 8 * 8 * kBlock * ((blocks + split - 1) / split) <= kOwnBytes;
+}
+
+template <bool OWN>
+int launch(const GemmFp8& g, GemmFp8Params p, const RowsToQuantize& q, bool follows, cudaStream_t stream) {
+    CUtensorMap map_a{}, map_b;
     // With few rows only those are loaded (in multiples of 8): the products of the others' memory,
     // whatever it holds, go to rows that nobody stores.  (Rows past the end as zeros: one row
     // through 14,336 x 4096 took 22 us instead of 13.)
     const int rows_loaded = (int)std::min<int64_t>((g.m + 7) / 8 * 8, kM);
-    MXK_CHECK(encode_tensor_map_2d(&map_a, g.a, (uint64_t)g.k, (uint64_t)g.m, (uint64_t)g.k, kBlock, rows_loaded,
-                                   CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
+    if (!OWN)
+        MXK_CHECK(encode_tensor_map_2d(&map_a, g.a, (uint64_t)g.k, (uint64_t)g.m, (uint64_t)g.k, kBlock, rows_loaded,
+                                       CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
     MXK_CHECK(encode_tensor_map_2d(&map_b, g.b, (uint64_t)g.k, (uint64_t)g.n, (uint64_t)g.k, kBlock, kN,
                                    CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
+    constexpr int smem = OWN ? kOwnSmem : kSmem;
     static thread_local int ready_device = -1;
     int dev = 0;
     MXK_CUDA(cudaGetDevice(&dev));
     if (ready_device != dev) {
-        MXK_CUDA(cudaFuncSetAttribute(gemm_fp8_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        MXK_CUDA(cudaFuncSetAttribute(gemm_fp8_tile_kernel<OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         ready_device = dev;
     }
-    static const int sms = sm_count();
     p.tiles_m = (p.m + kM - 1) / kM;
-    const int64_t tiles = (int64_t)p.tiles_m * ((p.n + kN - 1) / kN);
-    // Parts of k, as long as there are not many more CTAs than SMs and a part has two blocks.  In us
-    // for 1, 2, 4 and 8: one row through 4096 x 4096 (32 tiles) 15.3, 10.6, 8.5, 8.8, through
-    // 14,336 x 4096 (112) 17.4, 15.9, 19.2, 27.4; 64 rows through 6144 x 4096 (48) 17.5, 13.0, 12.0,
-    // 18.0; 16 through 1024 x 4096 (8) 14.8, 10.1, 7.6, 6.6.
-    int split = 1;
-    while (split < 8 && tiles * split * 10 <= 8 * sms && p.blocks >= 4 * split) split *= 2;
+    const int64_t tiles = tiles_of(g);
+    const int split = split_of(tiles, p.blocks);
     MXK_REQUIRE(tiles * split <= std::numeric_limits<int>::max(), "gemm_fp8: too much work for one call");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(tiles * split));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmem;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2]{};
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -373,8 +483,8 @@ int launch(const GemmFp8& g, GemmFp8Params p, bool follows, cudaStream_t stream)
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = follows ? 2 : 1;
-    LaunchScope scope("gemm_fp8", stream);
-    MXK_CUDA(cudaLaunchKernelEx(&cfg, gemm_fp8_tile_kernel, map_a, map_b, p, split, rows_loaded));
+    LaunchScope scope(OWN ? "linear_fp8" : "gemm_fp8", stream);
+    MXK_CUDA(cudaLaunchKernelEx(&cfg, gemm_fp8_tile_kernel<OWN>, map_a, map_b, p, q, split, rows_loaded));
     return MXK_OK;
 }
 
@@ -668,7 +778,8 @@ int check_product(const char* who, int dtype, int64_t m, int64_t n, int64_t k, c
     return MXK_OK;
 }
 
-int gemm_fp8(const GemmFp8& g, bool follows, cudaStream_t stream) {
+// q: rows to quantise on the way, which tile::own_rows allows, in place of g.a.
+int gemm_fp8(const GemmFp8& g, const RowsToQuantize* q, bool follows, cudaStream_t stream) {
     const int size = g.dtype == MXK_F32 ? 4 : 2;
     GemmFp8Params p{};
     p.m = (int)g.m, p.n = (int)g.n;
@@ -683,7 +794,9 @@ int gemm_fp8(const GemmFp8& g, bool follows, cudaStream_t stream) {
     p.b_wide = p.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(g.b_scales) % 16 == 0;
     p.err = device_error_word();
     if (!p.err) return fail(MXK_ERR_CUDA, "gemm_fp8: cannot allocate the device error word");
-    return g.m >= 256 && g.m * g.n >= 256 * 256 * 74 ? pair::launch(g, p, follows, stream) : tile::launch(g, p, follows, stream);
+    if (q) return tile::launch<true>(g, p, *q, false, stream);
+    if (g.m >= 256 && g.m * g.n >= 256 * 256 * 74) return pair::launch(g, p, follows, stream);
+    return tile::launch<false>(g, p, RowsToQuantize{}, follows, stream);
 }
 
 // Products of no features.
@@ -709,7 +822,7 @@ int mxk_gemm_fp8(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, c
     MXK_REQUIRE(a && a_scales, "gemm_fp8: an operand is null");
     MXK_REQUIRE(reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(a_scales) % 4 == 0,
                 "gemm_fp8: operands must be aligned to 16 bytes, scales to 4");
-    return gemm_fp8(g, false, as_stream(stream));
+    return gemm_fp8(g, nullptr, false, as_stream(stream));
 }
 
 int mxk_linear_fp8(int dtype, int64_t m, int64_t n, int64_t k, const void* x, int64_t x_stride, const uint8_t* b,
@@ -724,6 +837,12 @@ int mxk_linear_fp8(int dtype, int64_t m, int64_t n, int64_t k, const void* x, in
     MXK_REQUIRE(x && reinterpret_cast<uintptr_t>(x) % (dtype == MXK_F32 ? 4 : 2) == 0,
                 "linear_fp8: x must be non-null and aligned to its elements");
     const int64_t blocks = (k + kBlock - 1) / kBlock;
+    if (tile::own_rows(g, (int)blocks)) {
+        const int size = dtype == MXK_F32 ? 4 : 2;
+        const bool wide = (reinterpret_cast<uintptr_t>(x) | (uint64_t)(x_stride * size)) % 16 == 0;
+        const RowsToQuantize q{x, x_stride, dtype, wide, (int)k};
+        return gemm_fp8(g, &q, false, st);
+    }
     const size_t values = ((size_t)m * k + 255) / 256 * 256;
     cudaMemPool_t pool = workspace_pool();
     if (!pool) return fail(MXK_ERR_CUDA, "linear_fp8: cannot create the workspace pool");
@@ -733,7 +852,7 @@ int mxk_linear_fp8(int dtype, int64_t m, int64_t n, int64_t k, const void* x, in
     float* scales = reinterpret_cast<float*>(a + values);
     g.a = a, g.a_scales = scales;
     int status = launch_quantize_fp8({dtype, 1, m, k, x, x_stride, a, scales}, st);
-    if (status == MXK_OK) status = gemm_fp8(g, true, st);
+    if (status == MXK_OK) status = gemm_fp8(g, nullptr, true, st);
     const cudaError_t freed = cudaFreeAsync(work, st);
     MXK_CHECK(status);
     MXK_CUDA(freed);

@@ -4,69 +4,21 @@
 //     s = max(fl(max |x| / 448), 2^-126),   code = RNE_E4M3(x / s)
 //
 // over 1 row (activations) or 128 rows (weights) by 128 features.  The codes are those of
-// the exact quotients.  With 16-bit elements quotients in the middle between two codes are
-// common, and s is rounded, so one that lies a hair beside the middle must not be rounded
-// onto it first: x * (1 / s) is within four units of the last place of the quotient, and
-// where a middle is as near as that (or the code is subnormal, with other middles) the
-// quotient is divided out, its remainder taken by fma, and the quotient rounded to odd,
-// which keeps it on its side.
+// the exact quotients (gemm_fp8.cuh): with 16-bit elements quotients in the middle between two
+// codes are common, and s is rounded, so one that lies a hair beside the middle must not be
+// rounded onto it first.
 //
 // A thread converts 16 features; 2 or 4 bytes are read and one is written per element, so
 // HBM bounds both kernels.
 #include <algorithm>
 #include <limits>
 
-#include "cache_rows.cuh"
 #include "gemm_fp8.cuh"
 
 namespace mxk {
 namespace {
 
 using dev::Raw16;
-
-// x / s rounded to odd, for quotients that are not below 2^-126.
-__device__ __noinline__ float quotient_to_odd(float x, float s) {
-    if (s < 9.1e-13f) x *= 1.2089258e24f, s *= 1.2089258e24f;  // (2^-40, 2^80) the remainder stays representable
-    const float t = __fdiv_rn(x, s), rest = __fmaf_rn(-t, s, x);
-    uint32_t bits = __float_as_uint(t);
-    if (rest != 0.0f && !(bits & 1u)) bits += (rest > 0.0f) == (t > 0.0f) ? 1u : ~0u;
-    return __uint_as_float(bits);
-}
-
-// Whether t, four units of the last place from a quotient at most, may lie on the other side
-// of a middle: mantissas near a half of the code's last bit, and subnormal codes.
-__device__ __forceinline__ bool next_to_border(float t) {
-    const uint32_t bits = __float_as_uint(t);
-    const float a = fabsf(t);
-    return ((bits - 0x7fffcu) & 0xfffffu) <= 8u || (a < 0.015625f && a >= 0.00048828125f);  // 2^-6, 2^-11
-}
-
-__device__ __forceinline__ uint4 codes16(const float (&x)[16], float s) {
-    const float inv = __frcp_rn(s);
-    float t[16];
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t[i] = x[i] * inv, any |= next_to_border(t[i]);
-    if (any) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (next_to_border(t[i])) t[i] = quotient_to_odd(x[i], s);
-    }
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = dev::e4m3x2_encode(t[4 * i], t[4 * i + 1]) | (dev::e4m3x2_encode(t[4 * i + 2], t[4 * i + 3]) << 16);
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-__device__ __forceinline__ float block_scale(float amax) { return fmaxf(__fdiv_rn(amax, 448.0f), 1.17549435e-38f); }
-
-__device__ __forceinline__ float largest(const float (&x)[16]) {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[i]));  // a NaN sets no scale
-    return m;
-}
 
 // Eight threads to a block of 128 features of a row.
 template <class T, int VEC>
@@ -85,12 +37,12 @@ __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const T* x, int6
         raw.zero();
     float v[16];
     raw.to_float(v);
-    float amax = largest(v);
+    float amax = dev::largest16(v);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float s = block_scale(amax);
+    const float s = dev::fp8_scale(amax);
     if (!real) return;
-    *reinterpret_cast<uint4*>(values + row * k + f) = codes16(v, s);
+    *reinterpret_cast<uint4*>(values + row * k + f) = dev::fp8_codes16<T>(v, s, amax);
     if (sub == 0) scales[row * blocks + b] = s;
 }
 
@@ -115,7 +67,7 @@ __global__ void __launch_bounds__(256) quantize_fp8_tiles_kernel(const T* x, int
     for (int i = 0; i < 4; ++i) {
         float v[16];
         raw[i].to_float(v);
-        amax = fmaxf(amax, largest(v));
+        amax = fmaxf(amax, dev::largest16(v));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
@@ -123,12 +75,12 @@ __global__ void __launch_bounds__(256) quantize_fp8_tiles_kernel(const T* x, int
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = fmaxf(amax, tops[i]);
-    const float s = block_scale(amax);
+    const float s = dev::fp8_scale(amax);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float v[16];
         raw[i].to_float(v);
-        if (row0 + 32 * i < rows && f < k) *reinterpret_cast<uint4*>(values + (row0 + 32 * i) * k + f) = codes16(v, s);
+        if (row0 + 32 * i < rows && f < k) *reinterpret_cast<uint4*>(values + (row0 + 32 * i) * k + f) = dev::fp8_codes16<T>(v, s, amax);
     }
     if (tid == 0) scales[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = s;
 }

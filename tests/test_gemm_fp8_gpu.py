@@ -156,7 +156,8 @@ def test_products(torch_cuda, mxk, dtype, m, n, k):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-@pytest.mark.parametrize("m,n,k,shift", [(1, 256, 512, 0), (5, 300, 4096, 0), (64, 1536, 2064, 8), (130, 100, 272, 1),
+@pytest.mark.parametrize("m,n,k,shift", [(1, 256, 512, 0), (1, 4096, 4096, 0), (5, 300, 4096, 0), (16, 1000, 4096, 8), (9, 130, 2064, 1),
+                                         (16, 20000, 1040, 0), (1, 16, 16, 0), (8, 200, 16384, 0), (17, 128, 512, 0), (64, 1536, 2064, 8), (130, 100, 272, 1),
                                          (1000, 520, 1024, 0)])
 def test_layers_are_quantisation_and_product(torch_cuda, mxk, dtype, m, n, k, shift):
     torch = torch_cuda
