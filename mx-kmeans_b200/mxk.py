@@ -7,6 +7,7 @@ library has not been built -- there is no fallback implementation.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmxkmeans.so")
@@ -410,19 +411,38 @@ def _launch_stream(cache, stream):
 
 def _vector(t, name, cache, dtype, *shape):
     """Address of t, a contiguous tensor of `dtype` and `shape` on the cache's device."""
-    if t.dtype != dtype or tuple(t.shape) != shape or t.get_device() != cache.index or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or t.get_device() != cache.index or not t.is_contiguous():
         raise _bad(f"{name}: a contiguous {dtype} tensor of shape {shape} on {cache.device} is needed, got {t.device} "
                    f"{t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _rows(t, name, cache, tokens, heads):
-    """mxk_rows of t [tokens, heads, head_dim], whose features must be contiguous."""
+def _row_fields(t, name, cache, tokens, heads):
+    """Fields of the mxk_rows of t [tokens, heads, head_dim], whose features must be contiguous."""
     strides = t.stride()
-    if tuple(t.shape) != (tokens, heads, cache.head_dim) or t.get_device() != cache.index or strides[2] != 1:
+    if t.shape != (tokens, heads, cache.head_dim) or t.get_device() != cache.index or strides[2] != 1:
         raise _bad(f"{name}: a tensor of shape [{tokens}, {heads}, {cache.head_dim}] on {cache.device} is needed, its "
                    f"features contiguous, got {t.device} {tuple(t.shape)} with strides {strides}")
-    return Rows(t.data_ptr(), strides[0], strides[1])
+    return t.data_ptr(), strides[0], strides[1]
+
+
+def _rows(t, name, cache, tokens, heads):
+    return Rows(*_row_fields(t, name, cache, tokens, heads))
+
+
+# Structs with many fields are packed into bytes, which takes a third of the time of filling
+# the ctypes ones.
+_APPEND = struct.Struct("@iiq" + "Pqq" * 4 + "PPPqii")
+_ATTENTION = struct.Struct("@iiqiiqPqqPPqPfiqPqqP")
+_PREFIXES = struct.Struct("@iPPq")
+assert [x.size for x in (_APPEND, _ATTENTION, _PREFIXES)] == [ctypes.sizeof(x) for x in (Append, Attention, Prefixes)]
+
+
+def _packed(layout, *fields):
+    try:
+        return layout.pack(*fields)
+    except struct.error as e:
+        raise _bad(f"a number is out of range: {e}") from None
 
 
 class PagedCache:
@@ -485,7 +505,7 @@ def cache_read(cache, slots, k, v, stream=None):
     check(fn(cache.handle, dtype, tokens, at, ctypes.byref(kr), ctypes.byref(vr), st))
 
 
-_NO_ROWS = Rows(None, 0, 0)
+_NO_ROWS = 0, 0, 0
 
 
 def cache_append(cache, q, k, v, positions, cos_sin, slots, q_out=None, interleaved=False, stream=None):
@@ -503,19 +523,19 @@ def cache_append(cache, q, k, v, positions, cos_sin, slots, q_out=None, interlea
         if q.dim() != 3 or q.dtype != dtype or (q_out is not None and q_out.dtype != dtype):
             raise _bad("q and q_out: 3 dimensions and k's type are needed")
         heads = q.shape[1]
-        qr = _rows(q, "q", cache, tokens, heads)
-        outr = qr if q_out is None else _rows(q_out, "q_out", cache, tokens, heads)
+        qr = _row_fields(q, "q", cache, tokens, heads)
+        outr = qr if q_out is None else _row_fields(q_out, "q_out", cache, tokens, heads)
     elif q_out is not None:
         raise _bad("q_out without q")
     if cos_sin.dim() != 2:
         raise _bad("cos_sin has 2 dimensions")
     rows, rot = cos_sin.shape
-    table = _vector(cos_sin, "cos_sin", cache, _torch.float32, rows, rot)
-    args = Append(code, heads, tokens, qr, outr, _rows(k, "k", cache, tokens, cache.kv_heads),
-                  _rows(v, "v", cache, tokens, cache.kv_heads), _vector(slots, "slots", cache, _torch.int64, tokens),
-                  _vector(positions, "positions", cache, _torch.int64, tokens), table, rows, rot,
-                  1 if interleaved else 0)
-    check(load().mxk_cache_append(cache.handle, ctypes.byref(args), _launch_stream(cache, stream)))
+    i64 = _torch.int64
+    args = _packed(_APPEND, code, heads, tokens, *qr, *outr, *_row_fields(k, "k", cache, tokens, cache.kv_heads),
+                   *_row_fields(v, "v", cache, tokens, cache.kv_heads), _vector(slots, "slots", cache, i64, tokens),
+                   _vector(positions, "positions", cache, i64, tokens),
+                   _vector(cos_sin, "cos_sin", cache, _torch.float32, rows, rot), rows, rot, 1 if interleaved else 0)
+    check(load().mxk_cache_append(cache.handle, args, _launch_stream(cache, stream)))
 
 
 def _attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale, causal, window, lse):
@@ -526,19 +546,19 @@ def _attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale, c
     dtype, i32 = q.dtype, _torch.int32
     if out.dtype != dtype:
         raise _bad("out must have q's type")
-    qr = _rows(q, "q", cache, tokens, heads)
-    outr = _rows(out, "out", cache, tokens, heads)
+    qr = _row_fields(q, "q", cache, tokens, heads)
+    outr = _row_fields(out, "out", cache, tokens, heads)
     seqs, pages = page_table.shape
     stride, step = page_table.stride()
     if page_table.dtype != i32 or page_table.get_device() != cache.index or step != 1 < pages:
         raise _bad(f"page_table: int32 rows on {cache.device} are needed")
     if pages * cache.page_size < max_kv:
         raise _bad("page_table has fewer pages than max_kv tokens need")
-    return Attention(_DTYPES.get(dtype, -1), heads, tokens, seqs, max_q, max_kv, qr,
-                     _vector(cu_q, "cu_q", cache, i32, seqs + 1), page_table.data_ptr(), stride,
-                     _vector(kv_lens, "kv_lens", cache, i32, seqs),
-                     cache.head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, outr,
-                     None if lse is None else _vector(lse, "lse", cache, _torch.float32, tokens, heads))
+    return _packed(_ATTENTION, _DTYPES.get(dtype, -1), heads, tokens, seqs, max_q, max_kv, *qr,
+                   _vector(cu_q, "cu_q", cache, i32, seqs + 1), page_table.data_ptr(), stride,
+                   _vector(kv_lens, "kv_lens", cache, i32, seqs),
+                   cache.head_dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, *outr,
+                   0 if lse is None else _vector(lse, "lse", cache, _torch.float32, tokens, heads))
 
 
 def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale=None, causal=True, window=0,
@@ -549,7 +569,7 @@ def cache_attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, sca
     bounds on a sequence's new and cached tokens; scale: 1 / sqrt(head_dim) unless
     given; lse: float32 [tokens, heads] or None."""
     args = _attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale, causal, window, lse)
-    check(load().mxk_cache_attention(cache.handle, ctypes.byref(args), _launch_stream(cache, stream)))
+    check(load().mxk_cache_attention(cache.handle, args, _launch_stream(cache, stream)))
 
 
 def cache_attention_shared(cache, q, cu_q, page_table, kv_lens, cu_groups, prefix_lens, out, max_q, max_kv, max_prefix,
@@ -559,10 +579,9 @@ def cache_attention_shared(cache, q, cu_q, page_table, kv_lens, cu_groups, prefi
     the same slots, which are read once for them all (mxk.h, mxk_cache_attention_shared)."""
     args = _attention(cache, q, cu_q, page_table, kv_lens, out, max_q, max_kv, scale, causal, 0, lse)
     groups = prefix_lens.shape[0] if prefix_lens.dim() else 0
-    prefixes = Prefixes(groups, _vector(cu_groups, "cu_groups", cache, _torch.int32, groups + 1),
-                        _vector(prefix_lens, "prefix_lens", cache, _torch.int32, groups), max_prefix)
-    check(load().mxk_cache_attention_shared(cache.handle, ctypes.byref(args), ctypes.byref(prefixes),
-                                            _launch_stream(cache, stream)))
+    prefixes = _packed(_PREFIXES, groups, _vector(cu_groups, "cu_groups", cache, _torch.int32, groups + 1),
+                       _vector(prefix_lens, "prefix_lens", cache, _torch.int32, groups), max_prefix)
+    check(load().mxk_cache_attention_shared(cache.handle, args, prefixes, _launch_stream(cache, stream)))
 
 
 # ----------------------------------------------------------------------------- E4M3 products
@@ -578,8 +597,8 @@ def _matrix(t, name, dtype, index):
 def _whole(t, name, dtype, index, *shape):
     """Address of a contiguous tensor of `shape` on cuda:index.  Its elements may be bytes or
     torch.float8_e4m3fn where dtype is uint8."""
-    if (t.dtype != dtype and (dtype != _torch.uint8 or t.dtype != _torch.float8_e4m3fn)) or tuple(t.shape) != shape or \
-            t.get_device() != index or not t.is_contiguous():
+    if t.shape != shape or t.get_device() != index or not t.is_contiguous() or \
+            (t.dtype != dtype and (dtype != _torch.uint8 or t.dtype != _torch.float8_e4m3fn)):
         raise _bad(f"{name}: a contiguous {dtype} tensor of shape {shape} on cuda:{index} is needed, got {t.device} "
                    f"{t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
