@@ -64,27 +64,24 @@ using dev::kMostLift;
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kRows = 16;     // query rows of a unit
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
 constexpr int kGranule = 16;     // tokens of one product, contiguous in their page
 constexpr int kGranules = 2;     // of one step of a warp
 constexpr int kPair = kGranule * kGranules;
-// CTAs of four warps, which share a unit's tokens, or of one.
-//
-// unit_cost: key tiles that starting and ending a unit is taken to be worth.  In us for 0, 1, 2, 4
-// and 6 with four warps: 64 sequences of 1 to 8192 tokens 150, 142, 140, 144, 146; 24 sequences
-// with 2 to 5 query tokens and windows 35, 29, 27, 29, 29.
-// ctas: that an SM holds (168 registers a thread, 75 KB of rings).  With two of four warps: 64
-// sequences of 1 to 8192 tokens 146 us instead of 142.
-template <int WARPS>
-struct Shape {
-    static constexpr int threads = 32 * WARPS, keys = kPair * WARPS;
-    static constexpr int unit_cost = WARPS == 4 ? 2 : 4, ctas = WARPS == 4 ? 3 : 10;
-};
+constexpr int kKeys = kPair * kWarps;
+// Key tiles that starting and ending a unit is taken to be worth.  In us for 0, 1, 2, 4 and
+// 6: 64 sequences of 1 to 8192 tokens 150, 142, 140, 144, 146; 24 sequences with 2 to 5
+// query tokens and windows 35, 29, 27, 29, 29.
+constexpr int kUnitCost = 2;
+// CTAs that an SM holds (168 registers a thread, 75 KB of rings).  With two: 64 sequences of
+// 1 to 8192 tokens 146 us instead of 142.
+constexpr int kCtasPerSm = 3;
 // Rows per key head up to which this kernel is taken, one pass over the keys for every 16
 // of them.  In us, this and the tiles kernel, over 16,384 tokens (32 heads of 128 on 8): 32
 // rows 39, 45; 48 rows 47, 47; 64 rows 56, 47; 24 sequences with 2 to 5 query tokens of 8
 // heads a key head and windows 27, 54.
 constexpr int kMostFewRows = 32;
-constexpr int kManyUnits = 1 << 30;
 
 // Shared-memory row pitches (bytes) of the key and value granules.  Keys are read row by
 // row, a quarter per lane; values four rows per lane, an eighth each.  The pitches make the
@@ -99,7 +96,7 @@ template <> struct Pitch<64, 8> { static constexpr int k = 64, v = 80; static co
 template <> struct Pitch<64, 6> { static constexpr int k = 48, v = 48; static constexpr bool swizzled = false; };
 template <> struct Pitch<64, 4> { static constexpr int k = 32, v = 48; static constexpr bool swizzled = false; };
 
-template <int D, int BITS, int WARPS>
+template <int D, int BITS>
 struct Stage {
     static constexpr int row = D * BITS / 8;
     static constexpr int chunks = row / 16;       // 16-byte copies of a row
@@ -110,8 +107,8 @@ struct Stage {
     static constexpr int granule = vs_at + kGranule * scale_bytes;
     static constexpr int bytes = kGranules * granule;
     static constexpr int stages = 2;
-    static constexpr int ring = WARPS * stages * bytes;
-    static constexpr int join = WARPS * kRows * D * 4;  // the warps' outputs, after the ring is done
+    static constexpr int ring = kWarps * stages * bytes;
+    static constexpr int join = kWarps * kRows * D * 4;  // the warps' outputs, after the ring is done
     static constexpr int smem = ring > join ? ring : join;
     static_assert(granule % 16 == 0, "granules start on 16-byte boundaries");
 };
@@ -194,11 +191,9 @@ __device__ __forceinline__ uint32_t share_bits(int k) {
     }
 }
 
-template <int D, int BITS, int WARPS, class P>
-__global__ void __launch_bounds__(Shape<WARPS>::threads, Shape<WARPS>::ctas) attention_rows_kernel(const P p) {
-    using S = Stage<D, BITS, WARPS>;
-    constexpr int kWarps = WARPS, kThreads = Shape<WARPS>::threads, kKeys = Shape<WARPS>::keys;
-    constexpr int kUnitCost = Shape<WARPS>::unit_cost;
+template <int D, int BITS, class P>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(const P p) {
+    using S = Stage<D, BITS>;
     using Row = Pitch<D, BITS>;
     constexpr int kSteps = D / 16;       // k-steps of q . k
     constexpr int kTiles = D / 8;        // 8-feature tiles of the output
@@ -259,15 +254,10 @@ __global__ void __launch_bounds__(Shape<WARPS>::threads, Shape<WARPS>::ctas) att
     dev::Walk<P> w = dev::walk_to<kRows, kKeys>(p, share);
     int left = share.tiles - w.skip;
     bool open = false;
-    constexpr bool kWhole = std::is_same<P, SharedParams>::value;
-    using Units = dev::WholeUnits<kRows, kKeys>;
-    bool more = left > 0;
-    if constexpr (kWhole) more = Units::begin(p, share, w, left);
 
-    while (more) {
+    while (left > 0) {
         const int tile0 = w.tile;
-        int tiles = min(left, w.tiles - tile0);
-        if (kWhole && Units::fits(share, w)) tiles = w.tiles;
+        const int tiles = min(left, w.tiles - tile0);
         const int rows = min(w.view.n * p.group - w.rt * kRows, kRows);
         const int len = w.view.len;
 
@@ -874,7 +864,7 @@ __global__ void __launch_bounds__(Shape<WARPS>::threads, Shape<WARPS>::ctas) att
                 reinterpret_cast<float4*>(p.part + (slot * kRows + r) * D)[chunk] = v;
                 if (chunk == 0) {
                     p.part_stat[slot * kRows + r] = make_float2(top, total);
-                    if (kWhole && tile0 == 0) {
+                    if (std::is_same<P, SharedParams>::value && tile0 == 0) {
                         const int row = w.rt * kRows + r, j = row / p.group;
                         dev::store_where(p, w.view, dev::out_row(p, w.view) + j, w.head * p.group + (row - j * p.group), r,
                                          share.followers(share.tiles - left, w.tiles));
@@ -890,63 +880,42 @@ __global__ void __launch_bounds__(Shape<WARPS>::threads, Shape<WARPS>::ctas) att
         }
         __syncthreads();  // before the rings are filled again
         left -= tiles + share.cost;
-        if constexpr (kWhole) {
-            more = Units::next(p, share, w, left);
-        } else {
-            more = left > 0;
-            if (more) dev::walk_on<kRows, kKeys>(p, w);
-        }
+        if (left > 0) dev::walk_on<kRows, kKeys>(p, w);
     }
     if (tid == 0 && !open) p.part_open[blockIdx.x] = make_int4(0, 0, 0, 0);
     dev::wait_for_previous();
 }
 
-template <int D, int BITS, int WARPS, class P>
-int launch_rows(P p, int few_q, int64_t most_rows, AttentionCall<P>& call) {
-    using S = Stage<D, BITS, WARPS>;
-    using C = Shape<WARPS>;
+template <int D, int BITS, class P>
+int launch_rows(P p, int64_t most_tiles, int64_t most_rows, AttentionCall<P>& call) {
+    using S = Stage<D, BITS>;
     static thread_local int ready_device = -1;
     int dev = 0;
     MXK_CUDA(cudaGetDevice(&dev));
     if (ready_device != dev) {
-        MXK_CUDA(cudaFuncSetAttribute(attention_rows_kernel<D, BITS, WARPS, P>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        MXK_CUDA(cudaFuncSetAttribute(attention_rows_kernel<D, BITS, P>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       S::smem));
         ready_device = dev;
     }
     static const int sms = sm_count();
-    const int64_t most = attention_tile_bound(p, few_q, few_q, kRows, C::keys);
-    MXK_REQUIRE(most <= std::numeric_limits<int>::max() / (1 + C::unit_cost), "cache_attention: too much work for one call");
-    const int64_t ctas = std::min<int64_t>(most, C::ctas * sms);
+    const int64_t ctas = std::min<int64_t>(most_tiles, kCtasPerSm * sms);
     MXK_CHECK(call.take(p, ctas, kRows, D));
-    MXK_CHECK(call.launch("attention_rows", attention_rows_kernel<D, BITS, WARPS, P>, (unsigned)ctas, C::threads, S::smem, p));
+    MXK_CHECK(call.launch("attention_rows", attention_rows_kernel<D, BITS, P>, (unsigned)ctas, kThreads, S::smem, p));
     call.join_later(p, ctas, kRows, std::min<int64_t>(most_rows, kRows));
     return MXK_OK;
 }
 
-template <int D, int WARPS, class P>
-int launch_rows_bits(int bits, const P& p, int few_q, int64_t most_rows, AttentionCall<P>& call) {
-    if (bits == 8) return launch_rows<D, 8, WARPS>(p, few_q, most_rows, call);
-    if (bits == 6) return launch_rows<D, 6, WARPS>(p, few_q, most_rows, call);
-    return launch_rows<D, 4, WARPS>(p, few_q, most_rows, call);
+template <int D, class P>
+int launch_rows_bits(int bits, const P& p, int64_t most_tiles, int64_t most_rows, AttentionCall<P>& call) {
+    if (bits == 8) return launch_rows<D, 8>(p, most_tiles, most_rows, call);
+    if (bits == 6) return launch_rows<D, 6>(p, most_tiles, most_rows, call);
+    return launch_rows<D, 4>(p, most_tiles, most_rows, call);
 }
 
-template <int WARPS, class P>
-int launch_rows_dim(const mxk_cache& cache, const P& p, int few_q, int64_t most_rows, AttentionCall<P>& call) {
-    return cache.head_dim == 128 ? launch_rows_bits<128, WARPS>(cache.bits, p, few_q, most_rows, call)
-                                 : launch_rows_bits<64, WARPS>(cache.bits, p, few_q, most_rows, call);
-}
-
-// Sequences that share prefixes are many and have few tokens of their own: with enough of them for
-// the SMs a warp takes a unit alone.
-int launch_rows_shape(const mxk_cache& cache, const AttentionParams& p, int few_q, int64_t most_rows,
-                      AttentionCall<AttentionParams>& call) {
-    return launch_rows_dim<4>(cache, p, few_q, most_rows, call);
-}
-int launch_rows_shape(const mxk_cache& cache, const SharedParams& p, int few_q, int64_t most_rows,
-                      AttentionCall<SharedParams>& call) {
-    if ((int64_t)(p.seqs - p.groups) * p.kv_heads >= kManyUnits) return launch_rows_dim<1>(cache, p, few_q, most_rows, call);
-    return launch_rows_dim<4>(cache, p, few_q, most_rows, call);
-}
+// Sequences whose parts of one token a kernel of their own takes: all there is then is prefixes,
+// and those of few rows need not be told from others.
+bool only_prefixes(const AttentionParams&) { return false; }
+bool only_prefixes(const SharedParams& p) { return p.solo && p.max_q == 1; }
 
 }  // namespace
 
@@ -959,13 +928,17 @@ int launch_attention(const mxk_cache& cache, P p, int max_rows, AttentionCall<P>
     const bool many = rows > kMostFewRows;
     if (many) {
         P q = p;
-        if (p.seqs > 1) q.min_rows = kMostFewRows + 1;
+        if (p.seqs > 1 && !only_prefixes(p)) q.min_rows = kMostFewRows + 1;
         MXK_CHECK(launch_attention_tiles(cache.bits, cache.head_dim, q, p.max_q, max_rows, call));
         p.max_rows = kMostFewRows;
     }
-    if (!many || p.seqs > 1) {
+    if (!many || (p.seqs > 1 && !only_prefixes(p))) {
         const int64_t few = std::min<int64_t>(rows, kMostFewRows);
-        MXK_CHECK(launch_rows_shape(cache, p, (int)((few + p.group - 1) / p.group), few, call));
+        const int few_q = (int)((few + p.group - 1) / p.group);
+        const int64_t most = attention_tile_bound(p, few_q, few_q, kRows, kKeys);
+        MXK_REQUIRE(most <= std::numeric_limits<int>::max() / (1 + kUnitCost), "cache_attention: too much work for one call");
+        MXK_CHECK(cache.head_dim == 128 ? launch_rows_bits<128>(cache.bits, p, most, few, call)
+                                        : launch_rows_bits<64>(cache.bits, p, most, few, call));
     }
     return MXK_OK;
 }

@@ -75,7 +75,13 @@ struct SharedParams : AttentionParams {
     const int4* parts;  // two to a part: {first row, rows, tokens end, position of the first row},
                         // {first token, page table row, 0, 0}
     int groups, max_prefix;
+    // Parts of single tokens, where attention_solo_kernel takes them (else null): chunks, two int4 each:
+    // {sequence, query row, first token, tokens end}, {number of the chunk in its part, chunks of the part,
+    // first token of the part}; and how many there are.
+    const int4* solo;
+    const int* solo_count;
 };
+constexpr int kSoloRows = 8;  // query rows of such a part, at most
 
 constexpr int kHasPrefix = 1 << 30;  // what the row sees of the prefix comes to it
 
@@ -240,10 +246,14 @@ __device__ __forceinline__ int tile_count(const P& p, const V& s, int rt, int* f
 }
 
 // Whether this launch takes a sequence.
-template <class V>
-__device__ __forceinline__ bool taken(const AttentionParams& p, const V& s) {
+__device__ __forceinline__ bool taken(const AttentionParams& p, const SeqView& s) {
     const int rows = s.n * p.group;
     return rows != 0 && rows >= p.min_rows && rows <= p.max_rows;
+}
+
+__device__ __forceinline__ bool taken(const SharedParams& p, const PartView& s) {
+    const int rows = s.n * p.group;
+    return rows != 0 && rows >= p.min_rows && rows <= p.max_rows && !(p.solo && s.start >= 0 && s.n == 1);
 }
 
 // Key tiles and units of a sequence.
@@ -399,41 +409,6 @@ __device__ __forceinline__ void walk_on(const P& p, Walk<P>& w) {
     w.tiles = tile_count<ROWS, KEYS>(p, w.view, w.rt, &w.first);
 }
 
-// Shares cut at the ends of units, for calls with many short ones: a unit that counts no more
-// than a share is all its CTA's in whose share more than half of it lies (of two halves, the
-// first), and nothing of it has to be joined.  `left` as the walk's: positions of the share after
-// the unit's cost.  WholeUnits::begin and ::next return whether the CTA has a (next) unit.
-template <int ROWS, int KEYS>
-struct WholeUnits {
-    template <class P>
-    static __device__ __forceinline__ bool fits(const Share& s, const Walk<P>& w) {
-        return w.tiles + s.cost <= s.each;
-    }
-    // At the beginning of a unit of which `left + cost` positions are in the share.
-    template <class P>
-    static __device__ __forceinline__ bool mine(const Share& s, const Walk<P>& w, int left) {
-        return fits(s, w) ? 2 * (left + s.cost) >= w.tiles + s.cost : left > 0;
-    }
-    template <class P>
-    static __device__ __forceinline__ bool next(const P& p, const Share& s, Walk<P>& w, int left) {
-        if (left + s.cost <= 0) return false;
-        walk_on<ROWS, KEYS>(p, w);
-        return mine(s, w, left);
-    }
-    template <class P>
-    static __device__ __forceinline__ bool begin(const P& p, const Share& s, Walk<P>& w, int& left) {
-        const int before = w.tile > 0 ? w.tile + s.cost : s.cost - w.skip;  // positions of the unit in earlier shares
-        if (before == 0 || !fits(s, w)) return left > 0;
-        if (2 * before < w.tiles + s.cost) {
-            w.tile = 0;
-            left = s.tiles + before - s.cost;
-            return true;
-        }
-        left = s.tiles - (w.tiles + s.cost - before) - s.cost;
-        return next(p, s, w, left);
-    }
-};
-
 // log(sum exp) of a row from its running maximum (log2 units) and sum.
 __device__ __forceinline__ float row_lse(float m2, float sum) {
     return sum > 0.0f ? (m2 - kExpShift) * 0.693147180559945f + logf(sum)
@@ -492,11 +467,11 @@ __device__ __forceinline__ void store4(const P& p, int64_t token, int head, int 
 struct Parts {
     const float* part;
     const float2* stat;
-    const int4* open;
-    int ctas, rows;  // rows: of its row tiles
-    int split;       // CTAs that join a unit
+    const int4* open;  // null: a row's parts lie in slots one after the other
+    int ctas, rows;    // rows: of its row tiles; without `open`, ctas is the number of slots
+    int split;         // CTAs that join a unit
 };
-constexpr int kMostParts = 3;  // kernels of a call
+constexpr int kMostParts = 4;  // kernels of a call
 struct JoinParams {
     AttentionParams p;
     Parts parts[kMostParts];
@@ -649,6 +624,20 @@ public:
         return MXK_OK;
     }
 
+    // Partial sums that lie one after the other: `slots` of them with `rows` rows each.
+    int take_slots(P& p, int64_t slots, int rows, int d) {
+        void* ptr = nullptr;
+        const size_t part = (size_t)(slots * rows) * d * 4;
+        MXK_CHECK(room(part + (size_t)(slots * rows) * 8, &ptr));
+        number(p, join_.count);
+        p.part = static_cast<float*>(ptr);
+        p.part_stat = reinterpret_cast<float2*>(static_cast<char*>(ptr) + part);
+        return MXK_OK;
+    }
+    void slots_later(const P& p, int64_t slots, int rows) {
+        join_.parts[join_.count++] = Parts{p.part, p.part_stat, nullptr, (int)slots, rows, 0};
+    }
+
     // Room for something else of the call.
     int room(size_t bytes, void** ptr) {
         cudaMemPool_t pool = workspace_pool();
@@ -712,6 +701,9 @@ int launch_attention_tiles(int bits, int head_dim, P p, int max_q, int max_rows,
 // attention.cu: few query rows, and all of a call's kernels but the join; max_rows as above.
 template <class P>
 int launch_attention(const mxk_cache& cache, P p, int max_rows, AttentionCall<P>& call);
+
+// attention_solo.cu: parts of single tokens.
+int launch_attention_solo(int bits, int head_dim, SharedParams p, int64_t slots, AttentionCall<SharedParams>& call);
 
 // Checks of a call's arguments, and the kernels' parameters; p.tokens = 0: nothing to do.
 int check_attention(const char* who, const mxk_cache* cache, const mxk_attention* a, AttentionParams& p);

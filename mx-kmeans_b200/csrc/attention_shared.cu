@@ -12,7 +12,8 @@
 // seen by a prefix's rows.
 //
 //   attention_parts_kernel   lengths to parts, on the device: graphs replay as they grow
-//   the attention kernels    rows in float32 with their maxima and sums, whole or in parts, prefixes'
+//   attention_solo_kernel    what sequences with one query token have behind the prefix (attention_solo.cu)
+//   the attention kernels    everything else; rows in float32 with their maxima and sums, whole or in parts, prefixes'
 //                            and own, and where they are
 //   attention_merge_kernel   everything there is of a row, by the formula above
 #include <algorithm>
@@ -25,6 +26,7 @@ namespace {
 
 constexpr int kTile = 128;  // tokens that prefixes are multiples of: a key tile
 constexpr int64_t kFewRows = 2048;
+constexpr int kManyParts = 128;
 
 struct PartsParams {
     const int* cu_q;
@@ -35,6 +37,9 @@ struct PartsParams {
     int4* where;  // the sequences' side
     int64_t rows;
     int tokens, seqs, groups, max_q, max_kv, max_prefix;
+    int4* solo;  // as SharedParams
+    int* solo_count;
+    int solo_warps;  // key heads of that many chunks the work is to be cut into, or more
 };
 
 // Block 0: the sequences' parts, a thread each, then the groups', a warp each.  The others: no row
@@ -76,6 +81,53 @@ __global__ void __launch_bounds__(1024) attention_parts_kernel(const PartsParams
         }
         for (int i = first + lane; i < end && prefix; i += 32) p.parts[2 * (p.groups + i) + 1].x = prefix;
     }
+    if (!p.solo) return;
+    // The chunks of single tokens' parts: as long that there are as many as warps, in multiples of a
+    // key tile, and at least one a part.
+    __shared__ int64_t sums[32];
+    __shared__ int counts[32];
+    const int warp = threadIdx.x >> 5;
+    __syncthreads();
+    auto tokens_of = [&](int i, int4& view, int& start) -> int {  // behind the prefix; -1: no such part
+        if (i >= p.seqs) return -1;
+        view = p.parts[2 * (p.groups + i)], start = p.parts[2 * (p.groups + i) + 1].x;
+        return view.y == 1 ? max(view.z - start, 0) : -1;
+    };
+    int4 view;
+    int start;
+    int64_t mine = 0;
+    for (int i = threadIdx.x; i < p.seqs; i += blockDim.x) mine += max(tokens_of(i, view, start), 0);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+    int64_t all = 0;
+    for (int w = 0; w < 32; ++w) all += sums[w];
+    const int chunk = (int)((all / p.solo_warps + kTile) / kTile * kTile);
+    int before = 0;
+    for (int base = 0; base < p.seqs; base += blockDim.x) {
+        const int i = base + threadIdx.x, tokens = tokens_of(i, view, start);
+        const int chunks = tokens < 0 ? 0 : max((tokens + chunk - 1) / chunk, 1);
+        int incl = chunks;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        __syncthreads();
+        if (lane == 31) counts[warp] = incl;
+        __syncthreads();
+        int at = before + incl - chunks;
+        for (int w = 0; w < 32; ++w) {
+            if (w < warp) at += counts[w];
+            before += counts[w];
+        }
+        for (int k = 0; k < chunks; ++k) {
+            p.solo[2 * (at + k)] = make_int4(i, view.x, start + k * chunk, min(start + (k + 1) * chunk, view.z));
+            p.solo[2 * (at + k) + 1] = make_int4(k, chunks, start, 0);
+        }
+    }
+    if (threadIdx.x == 0) *p.solo_count = before;
 }
 
 struct MergeParams {
@@ -92,6 +144,7 @@ struct Found {
     const float* mean;
     const float2* stat;
     int count, rows;  // rows: of a slot; 0: the row is whole
+    bool pairs = false;  // a CTA has two slots
     __device__ __forceinline__ Found(const MergeParams& m, const int4& w, int64_t at) {
         // (What a wait that gave up left unwritten is not followed out of the workspace.)
         const Parts& set = m.parts[min(max(w.x, 0), kMostParts - 1)];
@@ -99,12 +152,14 @@ struct Found {
             mean = m.rows + at * D, stat = m.stat + at, count = w.x == -2 ? 0 : 1, rows = 0;
         } else {
             const int x = min(max(w.y, 0), set.ctas - 1), r = min(w.w & (kHasPrefix - 1), set.rows - 1);
-            mean = set.part + ((int64_t)2 * x * set.rows + r) * D, stat = set.stat + (int64_t)2 * x * set.rows + r;
-            count = min(max(w.z, 0), set.ctas - 1 - x) + 1, rows = set.rows;
+            const int64_t at = (int64_t)(set.open ? 2 * x : x) * set.rows + r;
+            mean = set.part + at * D, stat = set.stat + at;
+            count = min(max(w.z, 0), set.ctas - 1 - x) + 1, rows = set.rows, pairs = set.open != nullptr;
         }
     }
-    // Its i-th part: the beginning in the second slot of its CTA, the others in the first of theirs.
-    __device__ __forceinline__ int64_t slot(int i) const { return rows ? (2 * (int64_t)i + (i == 0 ? 1 : 0)) * rows : 0; }
+    // Its i-th part: the beginning in the second slot of its CTA, the others in the first of theirs, or
+    // one after the other.
+    __device__ __forceinline__ int64_t slot(int i) const { return (int64_t)(pairs ? 2 * i + (i == 0 ? 1 : 0) : i) * rows; }
 };
 
 // A row of the output, by SPLIT warps, every D / 4 threads of which take some of its parts.  They
@@ -204,25 +259,34 @@ extern "C" int mxk_cache_attention_shared(const mxk_cache* cache, const mxk_atte
     const int64_t rows = p.tokens * p.heads, parts = (int64_t)prefixes->groups + p.seqs;
     const size_t out_bytes = (size_t)rows * 2 * cache->head_dim * 4;
     void* room = nullptr;
-    MXK_CHECK(call.room(out_bytes + (size_t)rows * 48 + (size_t)parts * 32, &room));
+    // Parts of one token are cut into about as many chunks as there are warps for them, key heads counted.
+    const bool solo = cache->bits != 6 && p.group <= kSoloRows && (int64_t)p.seqs * p.kv_heads >= kManyParts;
+    static const int solo_warps = 12 * sm_count();
+    const int64_t per_head = std::max(solo_warps / p.kv_heads, 1), chunks = solo ? per_head + p.seqs + 1 : 0;
+    MXK_CHECK(call.room(out_bytes + (size_t)rows * 48 + (size_t)(parts + chunks) * 32 + 16, &room));
     SharedParams s;
     static_cast<AttentionParams&>(s) = p;
     s.out = room;
     int4* list = reinterpret_cast<int4*>(static_cast<char*>(room) + out_bytes);
     s.parts = list;
-    s.where = list + 2 * parts;
+    int4* solo_list = list + 2 * parts;
+    int* solo_count = reinterpret_cast<int*>(solo_list + 2 * chunks);
+    s.solo = solo ? solo_list : nullptr, s.solo_count = solo_count;
+    s.where = solo_list + 2 * chunks + 1;
     s.row_stat = reinterpret_cast<float2*>(s.where + 2 * rows);
     s.out_token = (int64_t)p.heads * cache->head_dim, s.out_head = cache->head_dim;
     s.groups = prefixes->groups, s.max_prefix = (int)max_prefix;
     s.seqs = (int)parts;
     const PartsParams pp{p.cu_q, p.kv_lens, prefixes->cu_groups, prefixes->prefix_lens, list, s.where + rows, rows,
-                         (int)p.tokens, p.seqs, s.groups, p.max_q, p.max_kv, s.max_prefix};
+                         (int)p.tokens, p.seqs, s.groups, p.max_q, p.max_kv, s.max_prefix,
+                         solo ? solo_list : nullptr, solo_count, (int)per_head};
     {
         LaunchScope scope("attention_parts", as_stream(stream));
         attention_parts_kernel<<<(unsigned)(1 + (rows + kClear - 1) / kClear), 1024, 0, as_stream(stream)>>>(pp);
         MXK_CUDA(cudaGetLastError());
     }
     MXK_CHECK(launch_attention(*cache, s, (int)p.tokens, call));
+    if (solo) MXK_CHECK(launch_attention_solo(cache->bits, cache->head_dim, s, chunks * p.kv_heads, call));
     MergeParams m{p, static_cast<const float*>(room), s.row_stat, s.where, {}};
     std::copy(call.parts(), call.parts() + kMostParts, m.parts);
     // With few rows all four warps of a block take parts of one, else one each.
