@@ -245,3 +245,101 @@ def test_bad_tensors_are_refused(torch_cuda, mxk):
                 dict(table=b["table"][:, :2]), dict(most=-1), dict(q=b["q"].float())):
         with pytest.raises(mxk.MxkInvalidArgument):
             attend(torch, mxk, {**b, **bad}, out=None)
+
+
+# ---- parts of one token, which a warp takes alone where there are many of them
+
+SOLO = [(bits, dim, dtype) for bits in (8, 4) for dim in (64, 128) for dtype in ("bfloat16", "float16")]
+
+
+@pytest.mark.parametrize("bits,dim,dtype", SOLO)
+@pytest.mark.parametrize("heads,kv_heads", [(8, 8), (12, 4), (10, 2), (16, 2)])
+def test_many_single_tokens(torch_cuda, mxk, bits, dim, dtype, heads, kv_heads):
+    """Own tokens around granules, tiles and pages; groups with and without a prefix, sequences
+    without queries or tokens, one with several queries, one much longer than the others."""
+    torch, g = torch_cuda, np.random.default_rng(13)
+    n = 128 // kv_heads + 4
+    owns = [1, 2, 15, 16, 17, 31, 33, 47, 48, 49, 95, 96, 127, 128, 129, 300]
+    groups = [(0, None, [(1, 700), (0, 5), (0, 0), (1, 0)]),
+              (144, 144, [(1, owns[i % 16]) for i in range(n)]),
+              (48, 48, [(1, 40), (2, 3), (1, 5)]),
+              (384, 384, [(1, 1), (3, 9), (0, 30), (1, 2500)])]
+    b = build(torch, mxk, g, groups, heads, kv_heads, dim, 48, bits, dtype)
+    check(torch, b, *attend(torch, mxk, b))
+    check(torch, b, *attend(torch, mxk, b, causal=False, scale=0.3), causal=False, scale=0.3)
+
+
+@pytest.mark.parametrize("bits,dim", [(8, 128), (4, 64)])
+def test_many_single_tokens_only(torch_cuda, mxk, bits, dim):
+    """No sequence has two: prefixes of all sizes go to one kernel.  Unaligned queries, no lse."""
+    torch, g = torch_cuda, np.random.default_rng(14)
+    groups = [(256, 256, [(1, 1 + 7 * i % 90) for i in range(n)]) for n in (2, 3, 60, 9)] + [(128, None, [(1, 5)] * 3)]
+    b = build(torch, mxk, g, groups, 8, 4, dim, 64, bits, "bfloat16")
+    want, lse = attend(torch, mxk, b)
+    check(torch, b, want, lse)
+    n = b["q"].shape[0]
+    wide = torch.zeros(n + 2, 8, dim + 1, dtype=torch.bfloat16, device="cuda")
+    wide[:n, :, 1:] = b["q"]
+    out = torch.full_like(wide, 77.0)
+    attend(torch, mxk, b, q=wide[..., 1:], out=out[..., 1:], lse=False)
+    assert torch.equal(out[:n, :, 1:], want) and (out[n:] == 77.0).all() and (out[..., 0] == 77.0).all()
+
+
+@pytest.mark.parametrize("bits,dim", [(8, 128), (8, 64), (4, 128)])
+def test_single_tokens_of_many_magnitudes(torch_cuda, mxk, bits, dim):
+    """Keys and values that differ by many powers of two from block to block and from token to
+    token, blocks of zeros beside tiny values, and single elements that dwarf their block."""
+    torch, g = torch_cuda, np.random.default_rng(15)
+    b = build(torch, mxk, g, [(128, 128, [(1, 33 + i) for i in range(70)])], 4, 2, dim, 16, bits, "float16", scale_k=0.2)
+    for i, kind in enumerate(("blocks", "tokens", "zeros", "tiny", "up", "down")):
+        slots = torch.from_numpy(b["slots"][i][128:]).cuda()
+        n = len(slots)
+        k = torch.randn(n, 2, dim, generator=torch.Generator().manual_seed(i)) * 0.2
+        v = torch.randn(n, 2, dim, generator=torch.Generator().manual_seed(i + 10))
+        if kind == "blocks":
+            f = torch.exp2(torch.randint(-9, 10, (n, 2, dim // 32, 1), generator=torch.Generator().manual_seed(3)).float())
+            v = (v.view(n, 2, -1, 32) * f).view(n, 2, dim)
+            k = (k.view(n, 2, -1, 32) / f.clamp(min=1)).view(n, 2, dim)
+        elif kind == "tokens":
+            v = v * torch.exp2(torch.randint(-10, 11, (n, 1, 1), generator=torch.Generator().manual_seed(4)).float())
+        elif kind == "zeros":
+            v[::3], k[1::3], v[:, :, :32] = 0, 0, 0
+        elif kind == "tiny":
+            v = v * 2.0 ** -30
+            v[::4] = 0
+        elif kind == "up":
+            v = v * torch.exp2(torch.arange(n).float() / 3 - 12)[:, None, None]
+        else:
+            v = v * torch.exp2(12 - torch.arange(n).float() / 3)[:, None, None]
+        if kind == "tiny":  # the prefix of its own group is part of what it sees: measured alone below
+            continue
+        mxk.cache_write(b["cache"], k.cuda(), v.cuda(), slots)
+    check(torch, b, *attend(torch, mxk, b))
+    # no prefix: what a row sees is tiny values and blocks of zeros
+    b = build(torch, mxk, g, [(0, None, [(1, 33 + i) for i in range(70)]), (128, 128, [(1, 1), (1, 2)])], 4, 2, dim, 16, bits,
+              "bfloat16", scale_v=2.0 ** -30)
+    for i in range(70):
+        slots = torch.from_numpy(b["slots"][i][::2]).cuda()
+        k = torch.randn(len(slots), 2, dim, device="cuda")
+        mxk.cache_write(b["cache"], k, torch.zeros_like(k), slots)
+    check(torch, b, *attend(torch, mxk, b))
+
+
+def test_single_tokens_and_numbers_that_are_none(torch_cuda, mxk):
+    """A NaN or an overflowed value stays with its sequence and, where it is a value, its feature."""
+    torch, g = torch_cuda, np.random.default_rng(16)
+    b = build(torch, mxk, g, [(128, 128, [(1, 20 + i) for i in range(80)])], 4, 2, 64, 32, 8, "bfloat16")
+    want, want_lse = attend(torch, mxk, b)
+    slot = lambda i, t: torch.tensor([b["slots"][i][128 + t]], device="cuda")  # noqa: E731
+    k, v = torch.randn(1, 2, 64, device="cuda"), torch.randn(1, 2, 64, device="cuda")
+    v[0, 1, 7] = float("nan")
+    mxk.cache_write(b["cache"], k, v, slot(3, 5))
+    k[0, 0, 9] = float("nan")
+    mxk.cache_write(b["cache"], k, v.nan_to_num(), slot(5, 24))
+    out, lse = attend(torch, mxk, b)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[3, 2:, 7] = True
+    hit[5, :2] = True
+    assert out[hit].isnan().all() and not out[~hit].isnan().any()
+    others = [i for i in range(80) if i not in (3, 5)]
+    assert torch.equal(out[others], want[others]) and torch.equal(lse[others], want_lse[others])

@@ -127,7 +127,8 @@ def product_limit(torch, a, b, blocks, dtype, want):
 
 
 SIZES = [(1, 1, 16), (1, 128, 128), (3, 130, 144), (64, 256, 1024), (128, 127, 2048), (129, 129, 400), (200, 64, 4096),
-         (777, 1003, 1040), (1, 4096, 4096), (17, 1000, 16384), (512, 2304, 640), (2500, 640, 256), (33, 8, 112), (2100, 2561, 400), (4097, 1300, 1040), (300, 16500, 128)]
+         (777, 1003, 1040), (1, 4096, 4096), (17, 1000, 16384), (512, 2304, 640), (2500, 640, 256), (33, 8, 112), (2100, 2561, 400), (4097, 1300, 1040), (300, 16500, 128),
+         (129, 7100, 144), (200, 7168, 1024), (400, 3600, 656), (128, 9000, 272)]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
@@ -229,6 +230,81 @@ def test_captured_layers_on_another_stream(torch_cuda, mxk):
             want = torch.empty_like(out)
             mxk.linear_fp8(x, b, s, want)
             assert torch.equal(out, want)
+
+
+FIRST = """
+import sys
+sys.path[:0] = ["mx-kmeans_b200"]
+import torch, mxk
+m, n, k = {sizes}
+x = torch.ones(m, k, device="cuda", dtype=torch.bfloat16)
+b, s = torch.full((n, k), 56, dtype=torch.uint8, device="cuda"), torch.full((-(-n // 128), k // 128), 0.5, device="cuda")
+out = torch.zeros(m, n, device="cuda", dtype=torch.bfloat16)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    mxk.linear_fp8(x, b, s, out)
+graph.replay()
+torch.cuda.synchronize()
+assert (out == 0.5 * k).all()
+"""
+
+
+@pytest.mark.parametrize("sizes", [(1, 128, 256), (40, 128, 256), (2560, 2048, 128)])
+def test_first_call_of_a_process_may_be_captured(torch_cuda, mxk, sizes):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST.format(sizes=sizes)], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_offsets_past_32_bits(torch_cuda, mxk):
+    """More than 2^32 elements of rows and of quantised rows; the last rows' products."""
+    torch = torch_cuda
+    m, n, k = (1 << 18) + 300, 48, 16384
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    x[-300:] = torch.randn(300, k, device="cuda")
+    b, b_scales = expected(torch, torch.randn(n, k, device="cuda") * k ** -0.5, 128)
+    b = b.to(torch.uint8)
+    out = torch.full((m, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    mxk.linear_fp8(x, b, b_scales, out)
+    # against 64 bits and not against a call of 300 rows: that splits the 16,384 features over
+    # eight CTAs, adds in another order, and may round to the other neighbour
+    a, w = (scaled(torch, v.to(torch.uint8), s, rows) for v, s, rows in ((*expected(torch, x[-300:], 1), 1), (b, b_scales, 128)))
+    want = a @ w.T
+    limit = product_limit(torch, a, w, k // 128, torch.bfloat16, want)
+    assert ((out[-300:].double() - want).abs() <= limit).all() and (out[:-300] == 0).all()
+    del x, out
+    # an output whose rows lie far apart
+    wide = torch.zeros(2100, (1 << 21) + 16, dtype=torch.bfloat16, device="cuda")
+    a, a_scales = expected(torch, torch.randn(2100, 256, device="cuda"), 1)
+    c, c_scales = expected(torch, torch.randn(2400, 256, device="cuda"), 128)
+    near = torch.empty(2100, 2400, dtype=torch.bfloat16, device="cuda")
+    a, c = a.to(torch.uint8), c.to(torch.uint8)
+    mxk.gemm_fp8(a, a_scales, c, c_scales, near)
+    mxk.gemm_fp8(a, a_scales, c, c_scales, wide[:, -2400:])
+    assert torch.equal(wide[:, -2400:], near) and (wide[:, -2500:-2400] == 0).all()
+
+
+def test_two_streams_at_once(torch_cuda, mxk):
+    """Layers on two streams, each with its own workspace."""
+    torch = torch_cuda
+    weights = [expected(torch, torch.randn(512, 1024, device="cuda"), 128) for _ in range(2)]
+    weights = [(b.to(torch.uint8), s) for b, s in weights]
+    xs = [torch.randn(200, 1024, device="cuda").half() for _ in range(2)]
+    want = [torch.empty(200, 512, dtype=torch.float16, device="cuda") for _ in range(2)]
+    for x, w, out in zip(xs, weights, want):
+        mxk.linear_fp8(x, *w, out)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[torch.empty_like(want[0]) for _ in range(20)] for _ in range(2)]
+    for i in range(20):
+        for j in range(2):
+            mxk.linear_fp8(xs[j], *weights[j], got[j][i], stream=streams[j])
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want[j]) for j in range(2) for out in got[j])
 
 
 def test_bad_tensors_are_refused(torch_cuda, mxk):
