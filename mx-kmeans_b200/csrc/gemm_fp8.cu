@@ -795,7 +795,13 @@ int gemm_fp8(const GemmFp8& g, const RowsToQuantize* q, bool follows, cudaStream
     p.err = device_error_word();
     if (!p.err) return fail(MXK_ERR_CUDA, "gemm_fp8: cannot allocate the device error word");
     if (q) return tile::launch<true>(g, p, *q, false, stream);
-    if (g.m >= 256 && g.m * g.n >= 256 * 256 * 74) return pair::launch(g, p, follows, stream);
+    // Pairs from 28 tiles on: fewer leave SMs idle that the split of K puts to work.  us, pairs | tiles:
+    //   512 x 4096 x 4096 (32) 18.8 | 20.9, 512 x 8192 x 8192 (64) 33.7 | 51.0, 2048 x 4096 x 4096 (128) 34.9 | 54.5,
+    //   512 x 4096 x 512 (32) 7.5 | 8.3, 256 x 7168 x 4096 (28) 18.7 | 19.2, 640 x 2048 x 4096 (24) 18.6 | 18.5,
+    //   256 x 6144 x 16,384 (24) 57.3 | 50.4, 256 x 4096 x 4096 (16) 18.2 | 14.3.
+    // Rows of one of the smaller tiles leave half a pair without work: 129 x 8192 x 4096 18.6 | 20.7.
+    if (g.m > tile::kM && (g.m + pair::kM - 1) / pair::kM * ((g.n + pair::kN - 1) / pair::kN) >= 28)
+        return pair::launch(g, p, follows, stream);
     return tile::launch<false>(g, p, RowsToQuantize{}, follows, stream);
 }
 
