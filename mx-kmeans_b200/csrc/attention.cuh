@@ -77,7 +77,8 @@ struct SharedParams : AttentionParams {
     int groups, max_prefix;
     // Parts of single tokens, where attention_solo_kernel takes them (else null): chunks, two int4 each:
     // {sequence, query row, first token, tokens end}, {number of the chunk in its part, chunks of the part,
-    // first token of the part}; and how many there are.
+    // first token of the part, number of its first chunk among those of parts that have several}; and how
+    // many there are.
     const int4* solo;
     const int* solo_count;
 };

@@ -39,7 +39,8 @@ struct PartsParams {
     int tokens, seqs, groups, max_q, max_kv, max_prefix;
     int4* solo;  // as SharedParams
     int* solo_count;
-    int solo_warps;  // key heads of that many chunks the work is to be cut into, or more
+    int solo_warps;  // a key head's work is cut into about as many chunks
+    int solo_most;   // entries of the list
 };
 
 // Block 0: the sequences' parts, a thread each, then the groups', a warp each.  The others: no row
@@ -83,9 +84,10 @@ __global__ void __launch_bounds__(1024) attention_parts_kernel(const PartsParams
     }
     if (!p.solo) return;
     // The chunks of single tokens' parts: as long that there are as many as warps, in multiples of a
-    // key tile, and at least one a part.
+    // key tile, and at least one a part.  As a part in several chunks is longer than one, and
+    // solo_warps chunks are longer than everything, such parts have at most 2 solo_warps chunks.
     __shared__ int64_t sums[32];
-    __shared__ int counts[32];
+    __shared__ uint64_t counts[32];
     const int warp = threadIdx.x >> 5;
     __syncthreads();
     auto tokens_of = [&](int i, int4& view, int& start) -> int {  // behind the prefix; -1: no such part
@@ -104,30 +106,34 @@ __global__ void __launch_bounds__(1024) attention_parts_kernel(const PartsParams
     int64_t all = 0;
     for (int w = 0; w < 32; ++w) all += sums[w];
     const int chunk = (int)((all / p.solo_warps + kTile) / kTile * kTile);
-    int before = 0;
+    uint64_t before = 0;  // chunks so far, and from bit 32 on those of parts that have several
     for (int base = 0; base < p.seqs; base += blockDim.x) {
         const int i = base + threadIdx.x, tokens = tokens_of(i, view, start);
-        const int chunks = tokens < 0 ? 0 : max((tokens + chunk - 1) / chunk, 1);
-        int incl = chunks;
+        const int chunks = tokens < 0 ? 0 : max(tokens / chunk + (tokens % chunk != 0), 1);
+        const uint64_t mine = (uint64_t)chunks | (uint64_t)(chunks > 1 ? chunks : 0) << 32;
+        uint64_t incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
         __syncthreads();
         if (lane == 31) counts[warp] = incl;
         __syncthreads();
-        int at = before + incl - chunks;
+        uint64_t at = before + incl - mine;
         for (int w = 0; w < 32; ++w) {
             if (w < warp) at += counts[w];
             before += counts[w];
         }
-        for (int k = 0; k < chunks; ++k) {
-            p.solo[2 * (at + k)] = make_int4(i, view.x, start + k * chunk, min(start + (k + 1) * chunk, view.z));
-            p.solo[2 * (at + k) + 1] = make_int4(k, chunks, start, 0);
+        // (More sequences of one token than tokens, from a cu_q that does not ascend: not followed.)
+        for (int k = 0; k < chunks && (int)at + k < p.solo_most; ++k) {
+            int4* to = p.solo + 2 * ((int)at + k);
+            const int from = start + k * chunk;
+            to[0] = make_int4(i, view.x, from, from + min(view.z - from, chunk));
+            to[1] = make_int4(k, chunks, start, (int)(at >> 32));
         }
     }
-    if (threadIdx.x == 0) *p.solo_count = before;
+    if (threadIdx.x == 0) *p.solo_count = min((int)before, p.solo_most);
 }
 
 struct MergeParams {
@@ -260,9 +266,11 @@ extern "C" int mxk_cache_attention_shared(const mxk_cache* cache, const mxk_atte
     const size_t out_bytes = (size_t)rows * 2 * cache->head_dim * 4;
     void* room = nullptr;
     // Parts of one token are cut into about as many chunks as there are warps for them, key heads counted.
-    const bool solo = cache->bits != 6 && p.group <= kSoloRows && (int64_t)p.seqs * p.kv_heads >= kManyParts;
     static const int solo_warps = 12 * sm_count();
-    const int64_t per_head = std::max(solo_warps / p.kv_heads, 1), chunks = solo ? per_head + p.seqs + 1 : 0;
+    const int64_t per_head = std::max(solo_warps / p.kv_heads, 1), most = std::min<int64_t>(p.seqs, p.tokens);
+    const bool solo = cache->bits != 6 && p.group <= kSoloRows && (int64_t)p.seqs * p.kv_heads >= kManyParts &&
+                      most * p.max_kv / per_head < std::numeric_limits<int>::max() - 2 * kTile;
+    const int64_t chunks = solo ? per_head + most + 1 : 0;
     MXK_CHECK(call.room(out_bytes + (size_t)rows * 48 + (size_t)(parts + chunks) * 32 + 16, &room));
     SharedParams s;
     static_cast<AttentionParams&>(s) = p;
@@ -279,14 +287,14 @@ extern "C" int mxk_cache_attention_shared(const mxk_cache* cache, const mxk_atte
     s.seqs = (int)parts;
     const PartsParams pp{p.cu_q, p.kv_lens, prefixes->cu_groups, prefixes->prefix_lens, list, s.where + rows, rows,
                          (int)p.tokens, p.seqs, s.groups, p.max_q, p.max_kv, s.max_prefix,
-                         solo ? solo_list : nullptr, solo_count, (int)per_head};
+                         solo ? solo_list : nullptr, solo_count, (int)per_head, (int)chunks};
     {
         LaunchScope scope("attention_parts", as_stream(stream));
         attention_parts_kernel<<<(unsigned)(1 + (rows + kClear - 1) / kClear), 1024, 0, as_stream(stream)>>>(pp);
         MXK_CUDA(cudaGetLastError());
     }
     MXK_CHECK(launch_attention(*cache, s, (int)p.tokens, call));
-    if (solo) MXK_CHECK(launch_attention_solo(cache->bits, cache->head_dim, s, chunks * p.kv_heads, call));
+    if (solo) MXK_CHECK(launch_attention_solo(cache->bits, cache->head_dim, s, 2 * per_head * p.kv_heads, call));
     MergeParams m{p, static_cast<const float*>(room), s.row_stat, s.where, {}};
     std::copy(call.parts(), call.parts() + kMostParts, m.parts);
     // With few rows all four warps of a block take parts of one, else one each.

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_solo_kernel(const Share
     int4 chunk = make_int4(0, 0, 0, 0), rest = chunk, next_chunk = chunk, next_rest = chunk;
     chunk_of(warp, chunk, rest);
     for (int item = warp; item < items; item += warps, chunk = next_chunk, rest = next_rest) {
-        const int chunk_at = item / p.kv_heads, head = item - chunk_at * p.kv_heads;
+        const int head = item % p.kv_heads;
         const int seq = chunk.x, query = chunk.y, begin = chunk.z, end = chunk.w;  // tokens [begin, end)
         const int number = rest.x, chunks = rest.y;                                // of the part
         const int granules = (end - begin + kGranule - 1) / kGranule;
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_solo_kernel(const Share
         // The rows: means, maxima and sums.
         const float vfactor = __uint_as_float((uint32_t)vref << 23);
         const int64_t out_row = p.tokens + query;  // (the sequences' side)
-        const int64_t slot = (int64_t)(chunk_at - number) * p.kv_heads + (int64_t)head * chunks;  // of the part's first chunk
+        const int64_t slot = (int64_t)rest.w * p.kv_heads + (int64_t)head * chunks;  // of the part's first chunk
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
 #pragma unroll

@@ -343,3 +343,13 @@ def test_single_tokens_and_numbers_that_are_none(torch_cuda, mxk):
     assert out[hit].isnan().all() and not out[~hit].isnan().any()
     others = [i for i in range(80) if i not in (3, 5)]
     assert torch.equal(out[others], want[others]) and torch.equal(lse[others], want_lse[others])
+
+
+def test_single_tokens_in_a_padded_batch(torch_cuda, mxk):
+    """Most sequences have no tokens; among the others some are long enough for several chunks."""
+    torch, g = torch_cuda, np.random.default_rng(17)
+    some = [(1, 3 + 211 * i % 1900) for i in range(24)]
+    rest = [(0, 0)] * 1500
+    b = build(torch, mxk, g, [(0, None, rest), (128, 128, some[:12] + rest), (256, 256, rest[:40] + some[12:])], 8, 2, 64, 16, 8,
+              "bfloat16")
+    check(torch, b, *attend(torch, mxk, b))
