@@ -46,7 +46,8 @@ struct PartsParams {
 // Block 0: the sequences' parts, a thread each, then the groups', a warp each.  The others: no row
 // is anywhere yet (a row behind the last sequence stays so).
 constexpr int kClear = 4096;  // rows of a block
-__global__ void __launch_bounds__(1024) attention_parts_kernel(const PartsParams p) {
+constexpr int kPartsThreads = 1024;
+__global__ void __launch_bounds__(kPartsThreads) attention_parts_kernel(const PartsParams p) {
     if (blockIdx.x > 0) {
         const int64_t first = (int64_t)(blockIdx.x - 1) * kClear, end = min(first + kClear, p.rows);
         for (int64_t i = first + threadIdx.x; i < end; i += blockDim.x) p.where[i] = make_int4(-2, 0, 0, 0);
@@ -54,8 +55,13 @@ __global__ void __launch_bounds__(1024) attention_parts_kernel(const PartsParams
     }
     AttentionParams a{};  // (for seq_view)
     a.cu_q = p.cu_q, a.kv_lens = p.kv_lens, a.tokens = p.tokens, a.max_q = p.max_q, a.max_kv = p.max_kv;
-    for (int i = threadIdx.x; i < p.seqs; i += blockDim.x) {
+    // (of the first sequences, which are mostly all, what comes below is not read back)
+    __shared__ int starts[kPartsThreads];
+    dev::SeqView first_view{};
+    starts[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < p.seqs; i += kPartsThreads) {
         const dev::SeqView s = dev::seq_view(a, i);
+        if (i < kPartsThreads) first_view = s;
         p.parts[2 * (p.groups + i)] = make_int4(s.row0, s.n, s.len, s.len - s.n);
         p.parts[2 * (p.groups + i) + 1] = make_int4(0, i, 0, 0);
     }
@@ -80,56 +86,65 @@ __global__ void __launch_bounds__(1024) attention_parts_kernel(const PartsParams
             p.parts[2 * g] = make_int4(prefix ? row0 : 0, prefix ? row_end - row0 : 0, prefix, prefix);
             p.parts[2 * g + 1] = make_int4(-1, prefix ? lead : 0, 0, 0);
         }
-        for (int i = first + lane; i < end && prefix; i += 32) p.parts[2 * (p.groups + i) + 1].x = prefix;
+        for (int i = first + lane; i < end && prefix; i += 32) {
+            p.parts[2 * (p.groups + i) + 1].x = prefix;
+            if (i < kPartsThreads) starts[i] = prefix;
+        }
     }
     if (!p.solo) return;
     // The chunks of single tokens' parts: as long that there are as many as warps, in multiples of a
     // key tile, and at least one a part.  As a part in several chunks is longer than one, and
     // solo_warps chunks are longer than everything, such parts have at most 2 solo_warps chunks.
-    __shared__ int64_t sums[32];
-    __shared__ uint64_t counts[32];
+    __shared__ uint64_t sums[32];
     const int warp = threadIdx.x >> 5;
     __syncthreads();
-    auto tokens_of = [&](int i, int4& view, int& start) -> int {  // behind the prefix; -1: no such part
+    auto tokens_of = [&](int i, int& row, int& start, int& end) -> int {  // behind the prefix; -1: no such part
         if (i >= p.seqs) return -1;
-        view = p.parts[2 * (p.groups + i)], start = p.parts[2 * (p.groups + i) + 1].x;
-        return view.y == 1 ? max(view.z - start, 0) : -1;
+        if (i < kPartsThreads) {
+            row = first_view.row0, start = starts[i], end = first_view.len;
+            return first_view.n == 1 ? max(end - start, 0) : -1;
+        }
+        const int4 view = p.parts[2 * (p.groups + i)];
+        row = view.x, start = p.parts[2 * (p.groups + i) + 1].x, end = view.z;
+        return view.y == 1 ? max(end - start, 0) : -1;
     };
-    int4 view;
-    int start;
-    int64_t mine = 0;
-    for (int i = threadIdx.x; i < p.seqs; i += blockDim.x) mine += max(tokens_of(i, view, start), 0);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) sums[warp] = mine;
-    __syncthreads();
-    int64_t all = 0;
-    for (int w = 0; w < 32; ++w) all += sums[w];
-    const int chunk = (int)((all / p.solo_warps + kTile) / kTile * kTile);
-    uint64_t before = 0;  // chunks so far, and from bit 32 on those of parts that have several
-    for (int base = 0; base < p.seqs; base += blockDim.x) {
-        const int i = base + threadIdx.x, tokens = tokens_of(i, view, start);
-        const int chunks = tokens < 0 ? 0 : max(tokens / chunk + (tokens % chunk != 0), 1);
-        const uint64_t mine = (uint64_t)chunks | (uint64_t)(chunks > 1 ? chunks : 0) << 32;
-        uint64_t incl = mine;
+    // Of the block's threads: the sum of x, and that of the threads up to this one.
+    auto scan = [&](uint64_t x, uint64_t& all) -> uint64_t {
+        uint64_t incl = x;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
         __syncthreads();
-        if (lane == 31) counts[warp] = incl;
+        if (lane == 31) sums[warp] = incl;
         __syncthreads();
-        uint64_t at = before + incl - mine;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) at += counts[w];
-            before += counts[w];
+        uint64_t warps = sums[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t v = __shfl_up_sync(0xffffffffu, warps, o);
+            if (lane >= o) warps += v;
         }
+        all = __shfl_sync(0xffffffffu, warps, 31);
+        return incl + (warp ? __shfl_sync(0xffffffffu, warps, warp - 1) : 0);
+    };
+    int row, start, end;
+    uint64_t mine = 0, all;
+    for (int i = threadIdx.x; i < p.seqs; i += kPartsThreads) mine += max(tokens_of(i, row, start, end), 0);
+    scan(mine, all);
+    const int chunk = (int)((all / p.solo_warps + kTile) / kTile * kTile);
+    uint64_t before = 0;  // chunks so far, and from bit 32 on those of parts that have several
+    for (int base = 0; base < p.seqs; base += kPartsThreads) {
+        const int i = base + threadIdx.x, tokens = tokens_of(i, row, start, end);
+        const int chunks = tokens < 0 ? 0 : max(tokens / chunk + (tokens % chunk != 0), 1);
+        const uint64_t own = (uint64_t)chunks | (uint64_t)(chunks > 1 ? chunks : 0) << 32;
+        const uint64_t at = before + scan(own, all) - own;
+        before += all;
         // (More sequences of one token than tokens, from a cu_q that does not ascend: not followed.)
         for (int k = 0; k < chunks && (int)at + k < p.solo_most; ++k) {
             int4* to = p.solo + 2 * ((int)at + k);
             const int from = start + k * chunk;
-            to[0] = make_int4(i, view.x, from, from + min(view.z - from, chunk));
+            to[0] = make_int4(i, row, from, from + min(end - from, chunk));
             to[1] = make_int4(k, chunks, start, (int)(at >> 32));
         }
     }
@@ -290,7 +305,7 @@ extern "C" int mxk_cache_attention_shared(const mxk_cache* cache, const mxk_atte
                          solo ? solo_list : nullptr, solo_count, (int)per_head, (int)chunks};
     {
         LaunchScope scope("attention_parts", as_stream(stream));
-        attention_parts_kernel<<<(unsigned)(1 + (rows + kClear - 1) / kClear), 1024, 0, as_stream(stream)>>>(pp);
+        attention_parts_kernel<<<(unsigned)(1 + (rows + kClear - 1) / kClear), kPartsThreads, 0, as_stream(stream)>>>(pp);
         MXK_CUDA(cudaGetLastError());
     }
     MXK_CHECK(launch_attention(*cache, s, (int)p.tokens, call));
