@@ -86,6 +86,12 @@ constexpr int kMostDown = 64;            // octaves that a float32 weight may be
 // kernels run one after the other and the second has little to do: nine sequences with 4
 // to 2804 rows 147 us with 512, 132 with 256.
 constexpr int kReadyRows = 512, kReadyRowsMany = 256;
+// The same of calls with prefixes.  In us for 256, 384 and 512, one token a sequence but for the
+// drafts, 32 heads of 128 on 8: 80 sequences behind 8192 tokens 78, 73, 73; 128: 89, 89, 98; 96
+// behind 32,768 tokens 160, 167, 167; 128: 168, 167, 206; 2 groups of 48 behind 8192 103, 95, 96; 8 of
+// 12: 150, 144, 144; 17 sequences of 2 to 5 tokens in 3 groups (24 heads of 64 on 4, 4 bits) 38, 35, 35;
+// 34: 61, 49, 49.  (Where too few rows are there, the two launches are made for nothing.)
+constexpr int kReadyRowsShared = 384;
 // The most memory that converting may take: above it the packed kernel goes over the keys
 // once for every 128 rows.
 constexpr int64_t kReadyBytes = 4ll << 30;
@@ -1720,7 +1726,7 @@ template <class P>
 int launch_attention_tiles(int bits, int head_dim, P p, int max_q, int max_rows, AttentionCall<P>& call) {
     // Several row tiles of a key head share its keys: converting those once pays for
     // writing and reading them as f16.  So many sequences can have enough rows for that:
-    const int ready_rows = p.seqs == 1 ? kReadyRows : kReadyRowsMany;
+    const int ready_rows = std::is_same<P, SharedParams>::value ? kReadyRowsShared : (p.seqs == 1 ? kReadyRows : kReadyRowsMany);
     const Most most = most_ready(p, max_q, max_rows, ready_rows);
     p.max_tiles = (most.tokens + kKeys - 1) / kKeys;
     p.ready_seqs = (int)most.seqs;

@@ -129,7 +129,7 @@ def test_rows_that_see_nothing(torch_cuda, mxk):
     assert (out == 0).all() and (lse == -float("inf")).all()
 
 
-@pytest.mark.parametrize("n", [3, 30, 90])
+@pytest.mark.parametrize("n", [3, 30, 90, 120])
 def test_long_prefix(torch_cuda, mxk, n):
     """A prefix that all CTAs share, joined from many parts; without lse."""
     torch, g = torch_cuda, np.random.default_rng(6)
