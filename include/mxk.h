@@ -435,7 +435,7 @@ int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* args, void*
  * known to the host; longer ones are shared up to it.  args->window must be 0, tokens * heads
  * below 2^30.  Besides mxk_cache_attention's, whose limits count a group's prefix as a sequence
  * of its rows, the call takes tokens * heads * (head_dim + 6) * 8 bytes of workspace and some
- * 20 MB at most. */
+ * 30 MB at most. */
 typedef struct {
     int groups;
     const int* cu_groups;

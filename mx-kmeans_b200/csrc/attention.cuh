@@ -80,7 +80,7 @@ struct SharedParams : AttentionParams {
     // first token of the part, number of its first chunk among those of parts that have several}; and how
     // many there are.
     const int4* solo;
-    const int* solo_count;
+    int* solo_count;  // and of those taken from a counter
 };
 constexpr int kSoloRows = 8;  // query rows of such a part, at most
 

@@ -27,6 +27,11 @@ namespace {
 constexpr int kTile = 128;  // tokens that prefixes are multiples of: a key tile
 constexpr int64_t kFewRows = 2048;
 constexpr int kManyParts = 128;
+// Chunks of single tokens' parts that a warp is to have.  In us for 1, 2, 3 and 4 (before, with one and
+// no counter): 256 sequences with 10 to 300 own tokens 232, 225, 224, 224 (229), 128 with 1 to 2000
+// 159, 134, 134, 134 (142), 40 with 1 to 8000 156, 122, 126, 126 (141), 512 with 1 to 1000 265, 258, 249, 246
+// (281), 64 with 1 to 512 60, 60, 60, 60 (61).  More take more memory.
+constexpr int kSoloShares = 2;
 
 struct PartsParams {
     const int* cu_q;
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(kPartsThreads) attention_parts_kernel(const Pa
             to[1] = make_int4(k, chunks, start, (int)(at >> 32));
         }
     }
-    if (threadIdx.x == 0) *p.solo_count = min((int)before, p.solo_most);
+    if (threadIdx.x == 0) p.solo_count[0] = min((int)before, p.solo_most), p.solo_count[1] = 0;
 }
 
 struct MergeParams {
@@ -282,7 +287,7 @@ extern "C" int mxk_cache_attention_shared(const mxk_cache* cache, const mxk_atte
     void* room = nullptr;
     // Parts of one token are cut into about as many chunks as there are warps for them, key heads counted.
     static const int solo_warps = 12 * sm_count();
-    const int64_t per_head = std::max(solo_warps / p.kv_heads, 1), most = std::min<int64_t>(p.seqs, p.tokens);
+    const int64_t per_head = std::max(kSoloShares * solo_warps / p.kv_heads, 1), most = std::min<int64_t>(p.seqs, p.tokens);
     const bool solo = cache->bits != 6 && p.group <= kSoloRows && (int64_t)p.seqs * p.kv_heads >= kManyParts &&
                       most * p.max_kv / per_head < std::numeric_limits<int>::max() - 2 * kTile;
     const int64_t chunks = solo ? per_head + most + 1 : 0;

@@ -18,7 +18,8 @@
 //
 // A warp has a ring of four granules of 16 tokens in shared memory, three of them on their way
 // (asynchronous copies of 16 bytes); 12 warps an SM.  Long parts are cut into chunks
-// (attention_parts_kernel), which the merge joins like any others.
+// (attention_parts_kernel), which the merge joins like any others; warps take them from a counter, as
+// some start late (where the kernel before ends late) and chunks differ.
 #include <limits>
 
 #include "attention.cuh"
@@ -120,14 +121,16 @@ __global__ void __launch_bounds__(kThreads, 3) attention_solo_kernel(const Share
     const float neg_inf = __int_as_float(0xff800000);
     dev::let_next_start();
     const int items = __ldg(p.solo_count) * p.kv_heads;
-    // (read ahead, by a bound on the list that the count is below)
     auto chunk_of = [&](int item, int4& chunk, int4& rest) {
         if (item >= items) return;
         chunk = __ldg(p.solo + 2 * (item / p.kv_heads)), rest = __ldg(p.solo + 2 * (item / p.kv_heads) + 1);
     };
+    // A warp's first item goes by its number, the others are taken from a counter, one ahead.
     int4 chunk = make_int4(0, 0, 0, 0), rest = chunk, next_chunk = chunk, next_rest = chunk;
+    int next_item = 0;
     chunk_of(warp, chunk, rest);
-    for (int item = warp; item < items; item += warps, chunk = next_chunk, rest = next_rest) {
+    for (int item = warp; item < items; item = next_item, chunk = next_chunk, rest = next_rest) {
+        if (lane == 0) next_item = warps + atomicAdd(p.solo_count + 1, 1);
         const int head = item % p.kv_heads;
         const int seq = chunk.x, query = chunk.y, begin = chunk.z, end = chunk.w;  // tokens [begin, end)
         const int number = rest.x, chunks = rest.y;                                // of the part
@@ -164,7 +167,8 @@ __global__ void __launch_bounds__(kThreads, 3) attention_solo_kernel(const Share
         };
 #pragma unroll
         for (int i = 0; i < L::stages - 1; ++i) issue();
-        chunk_of(item + warps, next_chunk, next_rest);
+        next_item = __shfl_sync(kFull, next_item, 0);
+        chunk_of(next_item, next_chunk, next_rest);
 
         // Q^T as the right operand: features 8 c + 4 s + (0, 1 | 2, 3) of block b at step 2 b + s.
         uint32_t q[kSteps][2];
