@@ -83,3 +83,15 @@ def test_steps_of_a_batch_with_a_common_prompt(torch_cuda, mxk, heads, kv_heads,
         assert relative(out, want) < 2.0 ** -8 + 2.0 ** -11
         y, want = project(out.view(seqs, -1), w_out)
         assert relative(y, want) < 2.0 ** -8
+
+
+@pytest.mark.parametrize("bits,prompt", [(8, 1000), (6, 96), (4, 130)])
+def test_example_of_conversations_behind_an_instruction(torch_cuda, mxk, bits, prompt):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(mxk.__file__), "examples", "serve_prefix.py")
+    spec = importlib.util.spec_from_file_location("serve_prefix", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    # half a step of bfloat16 in the output, and of float16 in the weights
+    assert example.main(bits=bits, prompt=prompt, steps=6, batch=20) < 2.0 ** -8 + 2.0 ** -11
