@@ -77,11 +77,6 @@ constexpr int kUnitCost = 2;
 // CTAs that an SM holds (168 registers a thread, 75 KB of rings).  With two: 64 sequences of
 // 1 to 8192 tokens 146 us instead of 142.
 constexpr int kCtasPerSm = 3;
-// Rows per key head up to which this kernel is taken, one pass over the keys for every 16
-// of them.  In us, this and the tiles kernel, over 16,384 tokens (32 heads of 128 on 8): 32
-// rows 39, 45; 48 rows 47, 47; 64 rows 56, 47; 24 sequences with 2 to 5 query tokens of 8
-// heads a key head and windows 27, 54.
-constexpr int kMostFewRows = 32;
 
 // Shared-memory row pitches (bytes) of the key and value granules.  Keys are read row by
 // row, a quarter per lane; values four rows per lane, an eighth each.  The pitches make the
@@ -913,9 +908,11 @@ int launch_rows_bits(int bits, const P& p, int64_t most_tiles, int64_t most_rows
 }
 
 // Sequences whose parts of one token a kernel of their own takes: all there is then is prefixes,
-// and those of few rows need not be told from others.
+// and those of few rows need not be told from others, unless most are such.
 bool only_prefixes(const AttentionParams&) { return false; }
-bool only_prefixes(const SharedParams& p) { return p.solo && p.max_q == 1; }
+bool only_prefixes(const SharedParams& p) {
+    return p.solo && p.max_q == 1 && p.tokens * p.group > (int64_t)p.groups * kMostFewRows;
+}
 
 }  // namespace
 

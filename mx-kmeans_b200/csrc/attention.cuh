@@ -473,6 +473,19 @@ struct Parts {
     int split;         // CTAs that join a unit
 };
 constexpr int kMostParts = 4;  // kernels of a call
+
+// Rows per key head up to which attention_rows_kernel is taken, one pass over the keys for every 16
+// of them.  In us, it and the tiles kernel, over 16,384 tokens (32 heads of 128 on 8): 32
+// rows 39, 45; 48 rows 47, 47; 64 rows 56, 47; 24 sequences with 2 to 5 query tokens of 8
+// heads a key head and windows 27, 54.
+constexpr int kMostFewRows = 32;
+// Rows per key head above which its keys are converted beforehand.  In us, packed and
+// ready kernel, over 16,384 tokens (32 heads of 128 on 8): 256 rows 72, 94; 384 rows 84,
+// 109; 512 rows 99, 111; 1024 rows (eight passes of the packed one) 121 ready.  (Where the
+// two cross above 512 was not measured.)  Among several sequences a lower bound, as the two
+// kernels run one after the other and the second has little to do: nine sequences with 4
+// to 2804 rows 147 us with 512, 132 with 256.
+constexpr int kReadyRows = 512, kReadyRowsMany = 256;
 struct JoinParams {
     AttentionParams p;
     Parts parts[kMostParts];

@@ -16,6 +16,12 @@
 //   the attention kernels    everything else; rows in float32 with their maxima and sums, whole or in parts, prefixes'
 //                            and own, and where they are
 //   attention_merge_kernel   everything there is of a row, by the formula above
+//
+// With many rows the products bound it; short calls are a chain of launches and dependent loads.
+// Measured at 32 heads of 128 on 8, 8 bits: 64 sequences with 1 to 512 own tokens behind 8192 60 us (each
+// by itself 244), of which the prefix 35, the own tokens 10 behind it and the merge 5; 256 with 10 to
+// 300 behind 32,768 225 us (each by itself 3335): 137 GFLOP in 150 us, tiles converted before in 40, own
+// tokens in 30.
 #include <algorithm>
 #include <limits>
 
@@ -25,13 +31,36 @@ namespace mxk {
 namespace {
 
 constexpr int kTile = 128;  // tokens that prefixes are multiples of: a key tile
+// Rows (query tokens times heads) up to which a block of the merge takes one row, its four warps
+// the parts of it, instead of a warp a row.  In us with one row and with four: 4 sequences of 32 heads
+// behind 1024 tokens 17.5, 19.7, 16 behind 8192 43, 49, 64 60.6, 61.6, 256 134, 133.
 constexpr int64_t kFewRows = 2048;
+// Sequences times key heads from which on single tokens' parts go to attention_solo_kernel: fewer are
+// done sooner by four warps each, and the prefix's few rows by attention_rows_kernel beside them.  In
+// us with it and without, on 8 key heads: 4 sequences 28.6, 17.5, 8 38.3, 27.8, 16 42.9, 43.0, 32 45, 51, 64 60,
+// 70, 256 132, 170.
 constexpr int kManyParts = 128;
 // Chunks of single tokens' parts that a warp is to have.  In us for 1, 2, 3 and 4 (before, with one and
 // no counter): 256 sequences with 10 to 300 own tokens 232, 225, 224, 224 (229), 128 with 1 to 2000
 // 159, 134, 134, 134 (142), 40 with 1 to 8000 156, 122, 126, 126 (141), 512 with 1 to 1000 265, 258, 249, 246
 // (281), 64 with 1 to 512 60, 60, 60, 60 (61).  More take more memory.
 constexpr int kSoloShares = 2;
+
+// What a call has to save, in reads of a token of 128 features by a key head, to share: the
+// kernel of the parts, that of single tokens and the merge, and a prefix that waits for one
+// kernel's CTAs, cost up to 20 us.  In us, each sequence by itself and shared, 32 heads of 128 on 8:
+//   one token, up to 32 rows together: 2 sequences behind 8192 tokens (64 K) 21, 28, 4 behind 4096 (96 K) 21.6,
+//     22.4, 8 behind 1024 (56 K) 18, 19, behind 2048 (112 K) 22, 20
+//   more rows: 16 behind 2048 (240 K) 29, 36, behind 4096 (480 K) 43, 38; 64 behind 512 (252 K) 38, 39, behind 1024
+//     (504 K) 52, 40
+//   more than 256 rows each, which are converted for each by itself: 4 with 100 tokens behind 2048 (48 K) 66, 65,
+//     behind 4096 (96 K) 92, 77; 8 behind 1024 (56 K) 73, 77, behind 2048 (112 K) 101, 93
+// (4 bits: a fifth less for each by itself, 6 bits: a quarter more.)
+constexpr int64_t kWorthLittle = 96 << 10, kWorth = 400 << 10;
+// Sequences that fill a row tile by themselves multiply as many tiles together as apart, unless there
+// are rows for several of the ready kernel's: 4 with 32 tokens (512 rows) behind 16,384 94, 110; 8 (1024)
+// 166, 138; 8 with 16 (64 rows each) 159, 109.
+constexpr int64_t kFullRows = 96, kEnoughRows = 1024;
 
 struct PartsParams {
     const int* cu_q;
@@ -50,7 +79,7 @@ struct PartsParams {
 
 // Block 0: the sequences' parts, a thread each, then the groups', a warp each.  The others: no row
 // is anywhere yet (a row behind the last sequence stays so).
-constexpr int kClear = 4096;  // rows of a block
+constexpr int kClear = 4096;  // rows of a block: four a thread
 constexpr int kPartsThreads = 1024;
 __global__ void __launch_bounds__(kPartsThreads) attention_parts_kernel(const PartsParams p) {
     if (blockIdx.x > 0) {
@@ -254,6 +283,15 @@ __global__ void __launch_bounds__(128) attention_merge_kernel(const MergeParams 
     if (p.lse && chunk == 0) p.lse[row] = dev::row_lse(top, total);
 }
 
+// Whether the call shares anything, by what the host knows.
+bool worth_sharing(const AttentionParams& p, int groups, int64_t max_prefix, int head_dim) {
+    if (groups == 0 || p.seqs <= groups || max_prefix == 0) return false;
+    const int64_t rows = p.tokens * p.group, each = rows / p.seqs;
+    if (each >= kFullRows && rows < kEnoughRows) return false;
+    const int64_t saved = (int64_t)(p.seqs - groups) * max_prefix * p.kv_heads;
+    return saved >= (rows <= kMostFewRows || each > kReadyRowsMany ? kWorthLittle : kWorth) * 128 / head_dim;
+}
+
 }  // namespace
 }  // namespace mxk
 
@@ -275,7 +313,7 @@ extern "C" int mxk_cache_attention_shared(const mxk_cache* cache, const mxk_atte
     MXK_REQUIRE((reinterpret_cast<uintptr_t>(prefixes->cu_groups) | reinterpret_cast<uintptr_t>(prefixes->prefix_lens)) % 4 == 0,
                 "cache_attention_shared: pointers must be aligned to their elements");
     const int64_t max_prefix = std::min<int64_t>(prefixes->max_prefix, p.max_kv) / kTile * kTile;
-    if (prefixes->groups == 0 || p.seqs < 2 || max_prefix == 0) {  // nothing to share
+    if (!worth_sharing(p, prefixes->groups, max_prefix, cache->head_dim)) {
         AttentionCall<AttentionParams> call(as_stream(stream));
         MXK_CHECK(launch_attention(*cache, p, 0, call));
         return call.join_all(cache->head_dim);

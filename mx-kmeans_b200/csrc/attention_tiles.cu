@@ -79,14 +79,7 @@ constexpr int kWide = 1 << 17;           // in place of a tile's key reference: 
 constexpr int kWideRef = 200;            // what scales relative to a token's own reference are added to
 constexpr int kRefStep = 4;              // value references are multiples of this many octaves
 constexpr int kMostDown = 64;            // octaves that a float32 weight may be scaled down by
-// Rows per key head above which its keys are converted beforehand.  In us, packed and
-// ready kernel, over 16,384 tokens (32 heads of 128 on 8): 256 rows 72, 94; 384 rows 84,
-// 109; 512 rows 99, 111; 1024 rows (eight passes of the packed one) 121 ready.  (Where the
-// two cross above 512 was not measured.)  Among several sequences a lower bound, as the two
-// kernels run one after the other and the second has little to do: nine sequences with 4
-// to 2804 rows 147 us with 512, 132 with 256.
-constexpr int kReadyRows = 512, kReadyRowsMany = 256;
-// The same of calls with prefixes.  In us for 256, 384 and 512, one token a sequence but for the
+// kReadyRowsMany of calls with prefixes.  In us for 256, 384 and 512, one token a sequence but for the
 // drafts, 32 heads of 128 on 8: 80 sequences behind 8192 tokens 78, 73, 73; 128: 89, 89, 98; 96
 // behind 32,768 tokens 160, 167, 167; 128: 168, 167, 206; 2 groups of 48 behind 8192 103, 95, 96; 8 of
 // 12: 150, 144, 144; 17 sequences of 2 to 5 tokens in 3 groups (24 heads of 64 on 4, 4 bits) 38, 35, 35;

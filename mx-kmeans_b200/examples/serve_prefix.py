@@ -28,7 +28,7 @@ def quantised(n, k, gen):
     return values, scales
 
 
-def main(bits=8, steps=16, batch=48, prompt=1000, heads=16, kv_heads=4, dim=128, hidden=2048, page=32, seed=0):
+def main(bits=8, steps=16, batch=48, prompt=4000, heads=16, kv_heads=4, dim=128, hidden=2048, page=32, seed=0):
     gen = torch.Generator(device="cuda").manual_seed(seed)
     dtype, longest = torch.bfloat16, prompt + steps
     w_in, w_out = quantised((heads + 2 * kv_heads) * dim, hidden, gen), quantised(hidden, heads * dim, gen)

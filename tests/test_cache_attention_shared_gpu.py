@@ -60,8 +60,24 @@ def build(torch, mxk, g, groups, heads, kv_heads, dim, page, bits, dtype, scale_
                 groups=torch.tensor(cu_groups, **i32), prefixes=torch.tensor(told, **i32), most=max(told + [0]))
 
 
-def attend(torch, mxk, b, lse=True, q=None, out=None, max_q=None, max_kv=None, max_prefix=None, **kw):
+def wide_bounds(torch, b):
+    """Bounds on prefixes and tokens from which on a call shares whatever there is, and a page
+    table for them (the added pages are never looked at)."""
+    cache, spare = b["cache"], len(b["q_lens"]) - len(b["prefixes"])
+    if spare <= 0:
+        return b["table"], max(max(b["kv_lens"]), 1), b["most"]
+    tokens = max(-(-(400 << 10) * 128 // (cache.head_dim * spare * cache.kv_heads)), b["most"], *b["kv_lens"])
+    tokens = -(-tokens // 128) * 128
+    more = -(-tokens // cache.page_size) - b["table"].shape[1]
+    return torch.nn.functional.pad(b["table"], (0, max(more, 0)), value=1 << 30), tokens, tokens
+
+
+def attend(torch, mxk, b, lse=True, q=None, out=None, max_q=None, max_kv=None, max_prefix=None, tight=False, **kw):
+    """tight, or with bounds that are given: it goes by the sizes whether the call shares."""
     q = b["q"] if q is None else q
+    if not tight and max_kv is None and max_prefix is None:
+        b = dict(b)
+        b["table"], max_kv, max_prefix = wide_bounds(torch, b)
     out = torch.full_like(q, 77.0) if out is None else out
     z = torch.full(q.shape[:2], 55.0, dtype=torch.float32, device="cuda") if lse else None
     mxk.cache_attention_shared(b["cache"], q, b["cu"], b["table"], b["kv"], b["groups"], b["prefixes"], out,
@@ -117,12 +133,31 @@ def test_what_is_told_of_a_prefix(torch_cuda, mxk, told):
     check(torch, b, *attend(torch, mxk, b))
     for most in (0, 100, 128, 300):
         check(torch, b, *attend(torch, mxk, b, max_prefix=most))
+    check(torch, b, *attend(torch, mxk, b, tight=True))
+
+
+@pytest.mark.parametrize("most", [127, 128, 300, 384, 1000])
+def test_prefix_longer_than_its_bound(torch_cuda, mxk, most):
+    """32 key heads of one row a sequence: a prefix of 128 tokens is worth it."""
+    torch, g = torch_cuda, np.random.default_rng(18)
+    b = build(torch, mxk, g, [(384, 384, [(1, 1 + i) for i in range(30)])], 32, 32, 64, 16, 8, "bfloat16")
+    check(torch, b, *attend(torch, mxk, b, max_prefix=most))
+
+
+@pytest.mark.parametrize("new", [1, 8, 25, 70, 300])
+def test_sizes_around_what_is_worth_sharing(torch_cuda, mxk, new):
+    """Bounds that are tight, where some calls share and others do not."""
+    torch, g = torch_cuda, np.random.default_rng(19)
+    for prefix in (512, 2048, 6144):
+        b = build(torch, mxk, g, [(prefix, prefix, [(new, new + 7 * i) for i in range(6)])], 8, 2, 128, 64, 8, "bfloat16")
+        check(torch, b, *attend(torch, mxk, b, tight=True))
+        check(torch, b, *attend(torch, mxk, b))
 
 
 def test_rows_that_see_nothing(torch_cuda, mxk):
     """More queries than tokens in one sequence of a group: the group shares nothing."""
     torch, g = torch_cuda, np.random.default_rng(5)
-    b = build(torch, mxk, g, [(256, 256, [(1, 9), (260, 2), (0, 0)]), (128, 128, [(2, 3), (1, 1)])], 4, 2, 64, 16, 6, "float16")
+    b = build(torch, mxk, g, [(256, 256, [(1, 9), (260, 2)] + [(0, 0)] * 4), (128, 128, [(2, 3), (1, 1)])], 4, 2, 64, 16, 6, "float16")
     check(torch, b, *attend(torch, mxk, b))
     b = build(torch, mxk, g, [(0, 128, [(1, 0), (2, 0)])], 4, 2, 64, 16, 6, "float16")
     out, lse = attend(torch, mxk, b)
@@ -206,7 +241,9 @@ def test_captured_and_replayed_as_sequences_grow(torch_cuda, mxk):
         [(128, 128, [(1, 300), (1, 1)]), (384, 384, [(1, 7), (1, 9), (1, 400)])],
         [(0, 0, [(1, 9), (1, 9), (1, 9), (1, 9)]), (640, 640, [(1, 700)])])]
     base = made[0]
-    width = max(m["table"].shape[1] for m in made)
+    tables, tokens = zip(*((t, n) for t, n, _ in (wide_bounds(torch, m) for m in made)))
+    made = [dict(m, table=t) for m, t in zip(made, tables)]
+    width = max(t.shape[1] for t in tables)
     pages = max(m["cache"].pages for m in made)
     cache = mxk.PagedCache.empty(pages, 32, 2, 64, 8)
     held = dict(base, cache=cache, table=torch.zeros(5, width, dtype=torch.int32, device="cuda"),
@@ -220,7 +257,7 @@ def test_captured_and_replayed_as_sequences_grow(torch_cuda, mxk):
         graphs.append(torch.cuda.CUDAGraph())
         with torch.cuda.graph(graphs[-1], stream=stream):
             mxk.cache_attention_shared(cache, held["q"], held["cu"], held["table"], held["kv"], held["groups"],
-                                       held["prefixes"], out, max_q=1, max_kv=width * 32, max_prefix=640)
+                                       held["prefixes"], out, max_q=1, max_kv=width * 32, max_prefix=max(tokens))
     for m in made + made[:1]:
         for name in ("k_values", "k_scales", "v_values", "v_scales"):
             getattr(cache, name).fill_(0xff)
@@ -244,7 +281,7 @@ def test_bad_tensors_are_refused(torch_cuda, mxk):
                 dict(prefixes=b["prefixes"].float()), dict(prefixes=b["prefixes"].cpu()), dict(kv=b["kv"][:1]),
                 dict(table=b["table"][:, :2]), dict(most=-1), dict(q=b["q"].float())):
         with pytest.raises(mxk.MxkInvalidArgument):
-            attend(torch, mxk, {**b, **bad}, out=None)
+            attend(torch, mxk, {**b, **bad}, out=None, tight=True)
 
 
 # ---- parts of one token, which a warp takes alone where there are many of them

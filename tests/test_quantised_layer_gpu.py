@@ -34,7 +34,8 @@ def test_steps_of_a_batch_with_a_common_prompt(torch_cuda, mxk, heads, kv_heads,
     for i in range(seqs):
         rows[i, :prompt // page] = torch.arange(prompt // page)
         rows[i, prompt // page:] = prompt // page + i * own + torch.arange(own)
-    rows = rows.cuda()
+    longest = 16384  # (with bounds like these the prompt is worth sharing; the pages behind are not looked at)
+    rows = torch.nn.functional.pad(rows, (0, longest // page - rows.shape[1])).cuda()
     i32 = dict(dtype=torch.int32, device="cuda")
 
     def project(x, w):
@@ -72,7 +73,7 @@ def test_steps_of_a_batch_with_a_common_prompt(torch_cuda, mxk, heads, kv_heads,
         assert relative(q, torch.from_numpy(want_q).cuda()) < 2.0 ** -8
         out = torch.empty(seqs, heads, dim, dtype=dtype, device="cuda")
         mxk.cache_attention_shared(cache, q, cu_q, rows, torch.full((seqs,), length, **i32), groups, prefixes, out, max_q=1,
-                                   max_kv=length, max_prefix=prompt)
+                                   max_kv=longest, max_prefix=longest)
         want = torch.empty(seqs, heads, dim, dtype=torch.float64, device="cuda")
         for i in range(seqs):
             keys[i].append(torch.from_numpy(k[i:i + 1]).cuda()), values[i].append(torch.from_numpy(v[i:i + 1]).cuda())
@@ -85,7 +86,7 @@ def test_steps_of_a_batch_with_a_common_prompt(torch_cuda, mxk, heads, kv_heads,
         assert relative(y, want) < 2.0 ** -8
 
 
-@pytest.mark.parametrize("bits,prompt", [(8, 1000), (6, 96), (4, 130)])
+@pytest.mark.parametrize("bits,prompt", [(8, 4000), (6, 2900), (4, 130)])
 def test_example_of_conversations_behind_an_instruction(torch_cuda, mxk, bits, prompt):
     import importlib.util
     import os
@@ -94,4 +95,4 @@ def test_example_of_conversations_behind_an_instruction(torch_cuda, mxk, bits, p
     example = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(example)
     # half a step of bfloat16 in the output, and of float16 in the weights
-    assert example.main(bits=bits, prompt=prompt, steps=6, batch=20) < 2.0 ** -8 + 2.0 ** -11
+    assert example.main(bits=bits, prompt=prompt, steps=6, batch=40) < 2.0 ** -8 + 2.0 ** -11
