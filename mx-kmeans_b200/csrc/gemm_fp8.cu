@@ -47,6 +47,7 @@ struct GemmFp8Params {
     int dtype;
     int out_vec, out_wide;   // four elements, or 16 bytes, can be stored at once
     int a_wide, b_wide;      // rows of scales can be loaded four at a time
+    int beside;              // the kernel before writes nothing that this one reads
     unsigned* err;
 };
 
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (!OWN) dev::tma_load_2d(stages + stage * kStep, &map_a, (first + i) * kBlock, tm * kM, &sh.full[stage]);
             };
             for (int i = 0; i < early; ++i) load_b(i, i);
-            dev::wait_for_previous();
+            if (!p.beside) dev::wait_for_previous();
             for (int i = 0; i < early; ++i) load_a(i, i);
             int i = early, stage = 0;
             uint32_t phase = 0;
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float* sa = OWN ? nullptr : p.a_scales + (int64_t)(real ? row : 0) * p.blocks + first;
         const float* sb = p.b_scales + (int64_t)tn * p.blocks + first;
         const uint32_t column = tmem + ((uint32_t)(warp & 3) << 21) + (warp >> 2) * kCols;
-        dev::wait_for_previous();
+        if (!p.beside) dev::wait_for_previous();
         if constexpr (OWN) {
             // Eight threads to a row of a block, 16 features each, which are one 16-byte piece of the
             // swizzled tile.
@@ -428,6 +429,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         __syncthreads();
     dev::tc_fence_after();
     if (warp == kProductWarp) dev::tmem_dealloc(tmem, kBuffers * kN);
+    if (p.beside) dev::wait_for_previous();  // what comes after this kernel comes after both
 }
 
 // Parts of k, as long as there are not many more CTAs than SMs and a part has two blocks.  In us
@@ -721,12 +723,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (warp == kProductWarp) dev::tmem_dealloc_pair(tmem, kBuffers * kN);
 }
 
-int launch(const GemmFp8& g, GemmFp8Params p, bool follows, cudaStream_t stream) {
-    CUtensorMap map_a, map_b;
-    MXK_CHECK(encode_tensor_map_2d(&map_a, g.a, (uint64_t)g.k, (uint64_t)g.m, (uint64_t)g.k, kBlock, 128,
-                                   CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
-    MXK_CHECK(encode_tensor_map_2d(&map_b, g.b, (uint64_t)g.k, (uint64_t)g.n, (uint64_t)g.k, kBlock, 128,
-                                   CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
+// Sets the kernel up on the current device; how many pairs it holds at a time.
+int prepare(int* pairs) {
     static thread_local int ready_device = -1, most_pairs = 0;
     int dev = 0;
     MXK_CUDA(cudaGetDevice(&dev));
@@ -744,6 +742,16 @@ int launch(const GemmFp8& g, GemmFp8Params p, bool follows, cudaStream_t stream)
         MXK_REQUIRE(most_pairs > 0, "gemm_fp8: the device holds no pair of CTAs");
         ready_device = dev;
     }
+    *pairs = most_pairs;
+    return MXK_OK;
+}
+
+int launch(const GemmFp8& g, GemmFp8Params p, int most_pairs, bool follows, cudaStream_t stream) {
+    CUtensorMap map_a, map_b;
+    MXK_CHECK(encode_tensor_map_2d(&map_a, g.a, (uint64_t)g.k, (uint64_t)g.m, (uint64_t)g.k, kBlock, 128,
+                                   CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
+    MXK_CHECK(encode_tensor_map_2d(&map_b, g.b, (uint64_t)g.k, (uint64_t)g.n, (uint64_t)g.k, kBlock, 128,
+                                   CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B));
     p.tiles_m = (p.m + kM - 1) / kM;
     const int64_t tiles = (int64_t)p.tiles_m * ((p.n + kN - 1) / kN);
     MXK_REQUIRE(tiles <= std::numeric_limits<int>::max() / 2, "gemm_fp8: too much work for one call");
@@ -787,8 +795,13 @@ int check_product(const char* who, int dtype, int64_t m, int64_t n, int64_t k, c
     return MXK_OK;
 }
 
-// q: rows to quantise on the way, which tile::own_rows allows, in place of g.a.
-int gemm_fp8(const GemmFp8& g, const RowsToQuantize* q, bool follows, cudaStream_t stream) {
+// At most pairs / kLastTiles tiles are such, of kLastK features at least.  us without and with: 512 x 9728 x
+// 4096 (76 tiles) 34.5, 28.5, 512 x 9984 x 8192 (78) 62, 48, 2560 x 2048 x 14,336 (80) 112, 85, 1280 x 4096 x 4096
+// (80) 38.0, 36.1, 1024 x 19,200 x 4096 (300) 91, 80, 2048 x 14,336 x 4096 (448) 110.4, 110.2 (power); with
+// fewer features 2048 x 2560 x 2048 (80) 21.5, 22.1, 1280 x 4096 x 1024 16, 21.
+constexpr int kLastTiles = 2, kLastK = 4096;
+
+GemmFp8Params params_of(const GemmFp8& g, unsigned* err) {
     const int size = g.dtype == MXK_F32 ? 4 : 2;
     GemmFp8Params p{};
     p.m = (int)g.m, p.n = (int)g.n;
@@ -801,17 +814,46 @@ int gemm_fp8(const GemmFp8& g, const RowsToQuantize* q, bool follows, cudaStream
     p.out_wide = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % 16 == 0;
     p.a_wide = p.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(g.a_scales) % 16 == 0;
     p.b_wide = p.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(g.b_scales) % 16 == 0;
-    p.err = device_error_word();
-    if (!p.err) return fail(MXK_ERR_CUDA, "gemm_fp8: cannot allocate the device error word");
-    if (q) return tile::launch<true>(g, p, *q, false, stream);
+    p.err = err;
+    return p;
+}
+
+// Large products: the pairs, but where the last few tiles would keep all waiting for a whole
+// tile's time, the columns that they lie in go to the other kernel, whose CTAs start as pairs end.
+int gemm_fp8_large(const GemmFp8& g, unsigned* err, bool follows, cudaStream_t stream) {
+    int pairs;
+    MXK_CHECK(pair::prepare(&pairs));
+    const int64_t tiles_m = (g.m + pair::kM - 1) / pair::kM, tiles = tiles_m * ((g.n + pair::kN - 1) / pair::kN);
+    const int64_t rest = tiles % pairs, columns = (rest + tiles_m - 1) / tiles_m;  // of tiles
+    GemmFp8 first = g, last = g;
+    const bool split = rest > 0 && tiles > pairs && columns * tiles_m * kLastTiles <= pairs && g.k >= kLastK;
+    if (split) {
+        first.n = g.n / pair::kN * pair::kN - (columns - (g.n % pair::kN != 0)) * pair::kN;
+        last.n = g.n - first.n;
+        last.b = g.b + first.n * g.k;
+        last.b_scales = g.b_scales + first.n / kBlock * ((g.k + kBlock - 1) / kBlock);
+        last.out = static_cast<char*>(g.out) + first.n * (g.dtype == MXK_F32 ? 4 : 2);
+    }
+    MXK_CHECK(pair::launch(first, params_of(first, err), pairs, follows, stream));
+    if (!split) return MXK_OK;
+    GemmFp8Params p = params_of(last, err);
+    p.beside = 1;
+    return tile::launch<false>(last, p, RowsToQuantize{}, true, stream);
+}
+
+// q: rows to quantise on the way, which tile::own_rows allows, in place of g.a.
+int gemm_fp8(const GemmFp8& g, const RowsToQuantize* q, bool follows, cudaStream_t stream) {
+    unsigned* err = device_error_word();
+    if (!err) return fail(MXK_ERR_CUDA, "gemm_fp8: cannot allocate the device error word");
+    if (q) return tile::launch<true>(g, params_of(g, err), *q, false, stream);
     // Pairs from 28 tiles on: fewer leave SMs idle that the split of K puts to work.  us, pairs | tiles:
     //   512 x 4096 x 4096 (32) 18.8 | 20.9, 512 x 8192 x 8192 (64) 33.7 | 51.0, 2048 x 4096 x 4096 (128) 34.9 | 54.5,
     //   512 x 4096 x 512 (32) 7.5 | 8.3, 256 x 7168 x 4096 (28) 18.7 | 19.2, 640 x 2048 x 4096 (24) 18.6 | 18.5,
     //   256 x 6144 x 16,384 (24) 57.3 | 50.4, 256 x 4096 x 4096 (16) 18.2 | 14.3.
     // Rows of one of the smaller tiles leave half a pair without work: 129 x 8192 x 4096 18.6 | 20.7.
     if (g.m > tile::kM && (g.m + pair::kM - 1) / pair::kM * ((g.n + pair::kN - 1) / pair::kN) >= 28)
-        return pair::launch(g, p, follows, stream);
-    return tile::launch<false>(g, p, RowsToQuantize{}, follows, stream);
+        return gemm_fp8_large(g, err, follows, stream);
+    return tile::launch<false>(g, params_of(g, err), RowsToQuantize{}, follows, stream);
 }
 
 // Products of no features.

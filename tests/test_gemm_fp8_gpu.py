@@ -128,7 +128,7 @@ def product_limit(torch, a, b, blocks, dtype, want):
 
 SIZES = [(1, 1, 16), (1, 128, 128), (3, 130, 144), (64, 256, 1024), (128, 127, 2048), (129, 129, 400), (200, 64, 4096),
          (777, 1003, 1040), (1, 4096, 4096), (17, 1000, 16384), (512, 2304, 640), (2500, 640, 256), (33, 8, 112), (2100, 2561, 400), (4097, 1300, 1040), (300, 16500, 128),
-         (129, 7100, 144), (200, 7168, 1024), (400, 3600, 656), (128, 9000, 272)]
+         (2560, 2048, 4096), (2500, 1990, 4112), (2300, 2049, 4096), (600, 6700, 4112), (129, 7100, 144), (200, 7168, 1024), (400, 3600, 656), (128, 9000, 272)]
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
@@ -159,7 +159,7 @@ def test_products(torch_cuda, mxk, dtype, m, n, k):
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("m,n,k,shift", [(1, 256, 512, 0), (1, 4096, 4096, 0), (5, 300, 4096, 0), (16, 1000, 4096, 8), (9, 130, 2064, 1),
                                          (16, 20000, 1040, 0), (1, 16, 16, 0), (8, 200, 16384, 0), (17, 128, 512, 0), (64, 1536, 2064, 8), (130, 100, 272, 1),
-                                         (1000, 520, 1024, 0)])
+                                         (1000, 520, 1024, 0), (2500, 2000, 4112, 8)])
 def test_layers_are_quantisation_and_product(torch_cuda, mxk, dtype, m, n, k, shift):
     torch = torch_cuda
     dtype = getattr(torch, dtype)
