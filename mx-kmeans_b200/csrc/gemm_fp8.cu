@@ -569,7 +569,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     dev::cluster_arrive(), dev::cluster_wait();  // the other CTA's barriers are there
     dev::tc_fence_after();
     const uint32_t tmem = __shfl_sync(kFull, sh.tmem, 0);
-    dev::let_next_start();
 
     if (warp < kSumWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
@@ -634,6 +633,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 uint32_t phase = 1;  // the first pass over the stages finds them free
                 bool ok = true;
                 dev::wait_for_previous();
+                dev::let_next_start();  // a kernel beside this one reads the same rows, which are there now
                 for (int tile = blockIdx.x >> 1; tile < tiles && ok; tile += pairs) {
                     int tm, tn;
                     place_of(tile, p.tiles_m, tiles_n, tm, tn);
