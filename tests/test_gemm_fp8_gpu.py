@@ -232,6 +232,40 @@ def test_captured_layers_on_another_stream(torch_cuda, mxk):
             assert torch.equal(out, want)
 
 
+def test_large_layers_one_after_the_other(torch_cuda, mxk):
+    """Two kernels share a product, beside each other and behind the quantiser: captured, and with
+    other rows in every call, whose results go on into the next."""
+    torch = torch_cuda
+    m, n, k = 2500, 2048, 4112
+    first, second = (expected(torch, torch.randn(*size, device="cuda") * size[1] ** -0.5, 128) for size in ((n, k), (k, n)))
+    first, second = ((b.to(torch.uint8), s) for b, s in (first, second))
+    xs = [torch.randn(m, k, device="cuda").to(torch.bfloat16) for _ in range(4)]
+    hidden, out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda"), torch.empty(m, k, dtype=torch.bfloat16, device="cuda")
+    want = []
+    for x in xs:
+        mxk.linear_fp8(x, *first, hidden)
+        torch.cuda.synchronize()
+        mxk.linear_fp8(hidden, *second, out)
+        torch.cuda.synchronize()
+        want.append(out.clone())
+    got = [torch.empty_like(out) for _ in xs]
+    for _ in range(5):
+        for x, y in zip(xs, got):
+            mxk.linear_fp8(x, *first, hidden)
+            mxk.linear_fp8(hidden, *second, y)
+    assert all(torch.equal(y, w) for y, w in zip(got, want))
+    x = torch.empty_like(xs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            mxk.linear_fp8(x, *first, hidden)
+            mxk.linear_fp8(hidden, *second, out)
+    for i in (0, 1, 2, 3) * 5:
+        x.copy_(xs[i])
+        graph.replay()
+        assert torch.equal(out, want[i])
+
+
 FIRST = """
 import sys
 sys.path[:0] = ["mx-kmeans_b200"]
