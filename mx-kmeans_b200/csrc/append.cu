@@ -301,15 +301,20 @@ __global__ void __launch_bounds__(256, 4) cache_append_kernel(const AppendParams
     }
 }
 
-// Heads that a thread goes through: `kSpan` where that leaves every SM several blocks, else one,
-// for the shortest time of a few tokens.
-constexpr int kSpan = 4;
+// Heads that a thread goes through, which load the table's row once, by how often the blocks for one
+// head each would fill the SMs.  In us for 1, 2, 3, 4 and 5, 32 + 8 + 8 heads of 128 in bf16: 8 tokens 3.8, 5.6,
+// 7.2, 9.0, 10.8; 1500 (fill 3.8) 12.4, 12.6, 13.9, 13.6, 16.2; 2048 (5.2) 15.6, 14.6, 15.9, 18.0, 18.9; 4096 (10.4)
+// 30.1, 26.3, 26.7, 27.2, 28.8; 8192 (20.8) 60.4, 50.4, 48.9, 48.9, 50.3; 16,384 116, 94, 89, 87, 88.
+int heads_of_thread(int64_t blocks) {
+    const int64_t fill = blocks / (4 * sm_count());
+    return fill >= 16 ? 4 : (fill >= 4 ? 2 : 1);
+}
 
 template <int BITS, class T, int VEC, bool PAIRS>
 int launch(AppendParams& m, cudaStream_t stream) {
     const int64_t blocks = (m.tokens + m.block_rows - 1) / m.block_rows;
     MXK_REQUIRE(blocks <= std::numeric_limits<int>::max(), "cache_append: too many tokens for one call");
-    m.span = blocks * (m.heads + 2 * m.kv_heads) >= (int64_t)kSpan * 4 * sm_count() ? kSpan : 1;
+    m.span = heads_of_thread(blocks * (m.heads + 2 * m.kv_heads));
     m.q_blocks = (m.heads + m.span - 1) / m.span, m.kv_blocks = (m.kv_heads + m.span - 1) / m.span;
     const int64_t grid = blocks * (m.q_blocks + 2 * m.kv_blocks);
     MXK_REQUIRE(grid <= std::numeric_limits<int>::max(), "cache_append: too many tokens for one call");
