@@ -247,3 +247,25 @@ def test_bad_tensors_are_refused(torch_cuda, mxk):
             mxk.cache_append(cache, **{**good, **bad})
     torch.cuda.synchronize()
     assert all((t == 0xa5).all() for t in (cache.k_values, cache.v_values))
+
+
+@pytest.mark.parametrize("bits,dtype", [(8, "bfloat16"), (6, "float32"), (4, "float16")])
+@pytest.mark.parametrize("n,hq,hk,d,page,rot", [(8200, 7, 3, 96, 16, 64), (6001, 11, 9, 128, 32, 128), (12003, 13, 7, 128, 16, 96)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_tokens_are_those_of_a_few_at_a_time(torch_cuda, mxk, bits, dtype, n, hq, hk, d, page, rot, interleaved):
+    """With many a thread goes through several heads of its token, the last ones through fewer."""
+    torch = torch_cuda
+    cache, q, k, v, slots, positions, cos_sin = make(torch, mxk, n, hq, hk, d, page, bits, dtype, rot, n, fused=True)
+    other = mxk.PagedCache.empty(cache.pages, page, hk, d, bits)
+    buffers = ("k_values", "k_scales", "v_values", "v_scales")
+    for name in buffers:
+        getattr(other, name).copy_(getattr(cache, name))
+    out, want = (torch.empty(n, hq, d, dtype=q.dtype, device="cuda") for _ in range(2))
+    mxk.cache_append(cache, q, k, v, positions, cos_sin, slots, q_out=out, interleaved=interleaved)
+    for i in range(0, n, 300):
+        part = slice(i, i + 300)
+        mxk.cache_append(other, q[part], k[part], v[part], positions[part], cos_sin, slots[part], q_out=want[part],
+                         interleaved=interleaved)
+    assert torch.equal(out, want)
+    for name in buffers:
+        assert torch.equal(getattr(cache, name), getattr(other, name))
