@@ -285,10 +285,11 @@ __global__ void __launch_bounds__(128) attention_merge_kernel(const MergeParams 
 
 // Whether the call shares anything, by what the host knows.
 bool worth_sharing(const AttentionParams& p, int groups, int64_t max_prefix, int head_dim) {
-    if (groups == 0 || p.seqs <= groups || max_prefix == 0) return false;
-    const int64_t rows = p.tokens * p.group, each = rows / p.seqs;
+    const int64_t seqs = std::min<int64_t>(p.seqs, p.tokens);  // that can have query tokens
+    if (groups == 0 || seqs <= groups || max_prefix == 0) return false;
+    const int64_t rows = p.tokens * p.group, each = rows / seqs;
     if (each >= kFullRows && rows < kEnoughRows) return false;
-    const int64_t saved = (int64_t)(p.seqs - groups) * max_prefix * p.kv_heads;
+    const int64_t saved = (seqs - groups) * max_prefix * p.kv_heads;
     return saved >= (rows <= kMostFewRows || each > kReadyRowsMany ? kWorthLittle : kWorth) * 128 / head_dim;
 }
 

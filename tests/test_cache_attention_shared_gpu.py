@@ -63,7 +63,7 @@ def build(torch, mxk, g, groups, heads, kv_heads, dim, page, bits, dtype, scale_
 def wide_bounds(torch, b):
     """Bounds on prefixes and tokens from which on a call shares whatever there is, and a page
     table for them (the added pages are never looked at)."""
-    cache, spare = b["cache"], len(b["q_lens"]) - len(b["prefixes"])
+    cache, spare = b["cache"], min(len(b["q_lens"]), sum(b["q_lens"])) - len(b["prefixes"])
     if spare <= 0:
         return b["table"], max(max(b["kv_lens"]), 1), b["most"]
     tokens = max(-(-(400 << 10) * 128 // (cache.head_dim * spare * cache.kv_heads)), b["most"], *b["kv_lens"])
