@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_solo_kernel(const Share
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
         float run_max[2] = {neg_inf, neg_inf}, base[2] = {-kExpShift, -kExpShift}, sum[2] = {0.0f, 0.0f};
-        int vref = 0;  // the lane's values are relative to 2^(vref - 127); 0: none yet
+        int vref = 0;  // the lane's values are relative to 2^(vref - 127), at first to the least scale there is
 
         auto step = [&](uint32_t here, int t0) {
             // keys of tokens g and g + 8: scales, a byte a block; values of tokens 2 c, 2 c + 1, 2 c + 8 and
@@ -336,13 +336,13 @@ __global__ void __launch_bounds__(kThreads, 3) attention_solo_kernel(const Share
                     }
                     top = over_tokens(max(max(vs[0], vs[1]), max(vs[2], vs[3])));
                 }
-                if (top > vref + kValueMax || (vref == 0 && top > 0)) {
-                    const int ref = max(top - kValueLift, 1);
-                    const float f = vref == 0 ? 0.0f : __uint_as_float((uint32_t)max(vref - ref + 127, 0) << 23);
+                if (top > vref + kValueMax) {
+                    const int ref = top - kValueLift;
+                    const float f = __uint_as_float((uint32_t)max(vref - ref + 127, 0) << 23);
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[t][i] = vref == 0 ? o[t][i] : o[t][i] * f;
+                        for (int i = 0; i < 4; ++i) o[t][i] *= f;
                     vref = ref;
                 }
             }
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_solo_kernel(const Share
         __syncwarp();
 
         // The rows: means, maxima and sums.
-        const float vfactor = __uint_as_float((uint32_t)vref << 23);
+        const float vfactor = dev::ue8m0_value(vref);
         const int64_t out_row = p.tokens + query;  // (the sequences' side)
         const int64_t slot = (int64_t)rest.w * p.kv_heads + (int64_t)head * chunks;  // of the part's first chunk
 #pragma unroll
