@@ -44,6 +44,7 @@
 #include <type_traits>
 
 #include "attention.cuh"
+#include "mx_codec.cuh"
 
 namespace mxk {
 namespace {
@@ -811,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = g + 8 * i;
-            const float vfactor = __uint_as_float((uint32_t)row_ref[i] << 23);
+            const float vfactor = dev::ue8m0_value(row_ref[i]);
             const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
             // features (2c + e) * D/8 + n, four at a time; the 16-byte chunks of a row are
             // permuted so that eight lanes write to eight different bank groups

@@ -11,8 +11,9 @@ from test_cache_attention_shared_gpu import attend, build
 
 pytestmark = pytest.mark.gpu
 
-# Standard deviations of values whose blocks get scale bytes of 0 to 6.
+# Standard deviations of values whose blocks get scale bytes of 1 to 6, or only the lowest, 0.
 SMALL = {8: 2.0 ** -116, 6: 2.0 ** -121, 4: 2.0 ** -121}
+LEAST = {8: 2.0 ** -122, 6: 2.0 ** -127, 4: 2.0 ** -127}
 
 
 def calls(torch, mxk, b):
@@ -71,8 +72,9 @@ def test_small_values_before_ordinary_ones(torch_cuda, mxk, bits, dim, shape, bl
 @pytest.mark.parametrize("bits", [8, 6, 4])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("shape", SHAPES)
-def test_small_values_alone(torch_cuda, mxk, bits, dim, shape):
+@pytest.mark.parametrize("size", ["small", "least"])
+def test_small_values_alone(torch_cuda, mxk, bits, dim, shape, size):
     torch, g = torch_cuda, np.random.default_rng(2)
-    b = build(torch, mxk, g, groups(shape), 4, 2, dim, 16, bits, "bfloat16", scale_v=SMALL[bits])
+    b = build(torch, mxk, g, groups(shape), 4, 2, dim, 16, bits, "bfloat16", scale_v=(SMALL if size == "small" else LEAST)[bits])
     for out in calls(torch, mxk, b):
         check_small(torch, b, out)
