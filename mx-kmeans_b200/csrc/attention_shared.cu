@@ -166,7 +166,9 @@ __global__ void __launch_bounds__(kPartsThreads) attention_parts_kernel(const Pa
     uint64_t mine = 0, all;
     for (int i = threadIdx.x; i < p.seqs; i += kPartsThreads) mine += max(tokens_of(i, row, start, end), 0);
     scan(mine, all);
-    const int chunk = (int)((all / p.solo_warps + kTile) / kTile * kTile);
+    // (From a cu_q that does not ascend there can be more than fits; nothing is longer than that.)
+    constexpr uint64_t kMost = 0x7fffffff / kTile * kTile - kTile;
+    const int chunk = (int)((min(all / p.solo_warps, kMost) + kTile) / kTile * kTile);
     uint64_t before = 0;  // chunks so far, and from bit 32 on those of parts that have several
     for (int base = 0; base < p.seqs; base += kPartsThreads) {
         const int i = base + threadIdx.x, tokens = tokens_of(i, row, start, end);
