@@ -429,8 +429,9 @@ int mxk_cache_attention(const mxk_cache* cache, const mxk_attention* args, void*
  * alike).  The result is that of mxk_cache_attention, but for rounding, whatever the lengths
  * are: a group shares what comes before the first query token of any of its sequences, in
  * multiples of 128 tokens (so up to 127 tokens of a prefix are read by each), and one sequence
- * by itself shares nothing.  Nor does a call whose bounds (seqs, groups, tokens, max_prefix) say
- * that sharing takes longer: it is a call of mxk_cache_attention then.
+ * by itself shares nothing.  Nor does a call whose bounds (seqs, groups, tokens, max_prefix) and
+ * heads say that sharing takes longer, by the costs that were measured: it is a call of
+ * mxk_cache_attention then.
  *
  * cu_groups (groups + 1), prefix_lens: int32 on the device.  max_prefix: a bound on the prefixes
  * known to the host; longer ones are shared up to it.  args->window must be 0, tokens * heads

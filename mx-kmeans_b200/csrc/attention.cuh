@@ -486,6 +486,12 @@ constexpr int kMostFewRows = 32;
 // kernels run one after the other and the second has little to do: nine sequences with 4
 // to 2804 rows 147 us with 512, 132 with 256.
 constexpr int kReadyRows = 512, kReadyRowsMany = 256;
+// kReadyRowsMany of calls with prefixes.  In us for 256, 384 and 512, one token a sequence but for the
+// drafts, 32 heads of 128 on 8: 80 sequences behind 8192 tokens 78, 73, 73; 128: 89, 89, 98; 96
+// behind 32,768 tokens 160, 167, 167; 128: 168, 167, 206; 2 groups of 48 behind 8192 103, 95, 96; 8 of
+// 12: 150, 144, 144; 17 sequences of 2 to 5 tokens in 3 groups (24 heads of 64 on 4, 4 bits) 38, 35, 35;
+// 34: 61, 49, 49.  (Where too few rows are there, the two launches are made for nothing.)
+constexpr int kReadyRowsShared = 384;
 struct JoinParams {
     AttentionParams p;
     Parts parts[kMostParts];

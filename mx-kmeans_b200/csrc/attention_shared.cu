@@ -46,17 +46,26 @@ constexpr int kManyParts = 128;
 // (281), 64 with 1 to 512 60, 60, 60, 60 (61).  More take more memory.
 constexpr int kSoloShares = 2;
 
-// What a call has to save, in reads of a token of 128 features by a key head, to share: the
-// kernel of the parts, that of single tokens and the merge, and a prefix that waits for one
-// kernel's CTAs, cost up to 20 us.  In us, each sequence by itself and shared, 32 heads of 128 on 8:
-//   one token, up to 32 rows together: 2 sequences behind 8192 tokens (64 K) 21, 28, 4 behind 4096 (96 K) 21.6,
-//     22.4, 8 behind 1024 (56 K) 18, 19, behind 2048 (112 K) 22, 20
-//   more rows: 16 behind 2048 (240 K) 29, 36, behind 4096 (480 K) 43, 38; 64 behind 512 (252 K) 38, 39, behind 1024
-//     (504 K) 52, 40
-//   more than 256 rows each, which are converted for each by itself: 4 with 100 tokens behind 2048 (48 K) 66, 65,
-//     behind 4096 (96 K) 92, 77; 8 behind 1024 (56 K) 73, 77, behind 2048 (112 K) 101, 93
-// (4 bits: a fifth less for each by itself, 6 bits: a quarter more.)
-constexpr int64_t kWorthLittle = 96 << 10, kWorth = 400 << 10;
+// What a call has to save to share, in passes over a token of 128 features by a key head that wait
+// for its bytes (some 45 ps each).  A prefix's rows take one kernel's CTAs for themselves, the parts, single
+// tokens and the merge have kernels of their own (5 to 30 us), and every row is written twice in float32
+// and read again by the merge.  In us, each sequence by itself and shared, 32 heads of 128 on 8, 8 bits:
+//   up to 32 rows a prefix: 2 sequences of one token behind 16,384 (128 K saved) 28.7, 33.1, behind 32,768 (256 K)
+//     43, 39; 4 behind 4096 (96 K) 21.7, 22.7; 8 behind 4096 (192 K) 28.9, 25.0
+//   more: 16 of one token behind 1024 (120 K) 22, 33, behind 4096 (480 K) 43, 37; 64 behind 512 (248 K) 41, 40,
+//     behind 1024 (496 K) 54, 40
+//   of which the rows' way takes 1638 K: 64 with 32 tokens behind 1024 (1000 K) 154, 193, behind 4096 (4000 K) 340,
+//     277; 16 with 128 behind 1024 (360 K) 126, 150, behind 4096 (1440 K) 258, 246
+//   6554 K: 64 with 128 behind 1024 (1512 K) 360, 517, behind 4096 (6048 K) 869, 884; 4 with 2048 behind 4096
+//     (288 K) 684, 897
+// Over 1437 sizes (1 to 16 key heads, 2 to 128 sequences of 1 to 2048 tokens in 1 to 4 groups, 4 to 8 bits, prefixes
+// of 256 to 32,768) 24 calls took over 5 % longer than the ordinary one, most of them of single tokens and one
+// or two key heads (up to 1.75 of it), whose prefixes come in a hundred parts; 415 were faster, at 0.57 of it.
+constexpr int64_t kWorthFew = 160 << 10, kWorth = 300 << 10, kWorthReady = 50 << 10;
+constexpr int kWayCost = 5;  // elements of rows whose way takes as long as such a pass
+// A pass of 128 rows of a sequence by the tiles kernel, of a prefix, whose tiles all CTAs share, and keys that are
+// converted beforehand.
+constexpr double kTilePass = 2.0, kPrefixPass = 1.0, kReadyPass = 3.0;
 // Sequences that fill a row tile by themselves multiply as many tiles together as apart, unless there
 // are rows for several of the ready kernel's: 4 with 32 tokens (512 rows) behind 16,384 94, 110; 8 (1024)
 // 166, 138; 8 with 16 (64 rows each) 159, 109.
@@ -289,10 +298,16 @@ __global__ void __launch_bounds__(128) attention_merge_kernel(const MergeParams 
 bool worth_sharing(const AttentionParams& p, int groups, int64_t max_prefix, int head_dim) {
     const int64_t seqs = std::min<int64_t>(p.seqs, p.tokens);  // that can have query tokens
     if (groups == 0 || seqs <= groups || max_prefix == 0) return false;
-    const int64_t rows = p.tokens * p.group, each = rows / seqs;
+    const int64_t rows = p.tokens * p.group, each = rows / seqs, together = rows / groups;
     if (each >= kFullRows && rows < kEnoughRows) return false;
-    const int64_t saved = (seqs - groups) * max_prefix * p.kv_heads;
-    return saved >= (rows <= kMostFewRows || each > kReadyRowsMany ? kWorthLittle : kWorth) * 128 / head_dim;
+    const double width = head_dim / 128.0;
+    auto passes = [&](int64_t rows, int most_tiles, double tile) -> double {
+        if (rows <= kMostFewRows) return (double)((rows + 15) / 16) * width;  // of attention_rows_kernel
+        return rows <= most_tiles ? (double)((rows + 127) / 128) * tile : kReadyPass * width;
+    };
+    const double saved = seqs * passes(each, kReadyRowsMany, kTilePass) - groups * passes(together, kReadyRowsShared, kPrefixPass);
+    const int64_t worth = together <= kMostFewRows ? kWorthFew : (each > kReadyRowsMany ? kWorthReady : kWorth);
+    return saved * max_prefix * p.kv_heads >= worth + (double)(p.tokens * p.heads * head_dim) / kWayCost;
 }
 
 }  // namespace

@@ -79,12 +79,6 @@ constexpr int kWide = 1 << 17;           // in place of a tile's key reference: 
 constexpr int kWideRef = 200;            // what scales relative to a token's own reference are added to
 constexpr int kRefStep = 4;              // value references are multiples of this many octaves
 constexpr int kMostDown = 64;            // octaves that a float32 weight may be scaled down by
-// kReadyRowsMany of calls with prefixes.  In us for 256, 384 and 512, one token a sequence but for the
-// drafts, 32 heads of 128 on 8: 80 sequences behind 8192 tokens 78, 73, 73; 128: 89, 89, 98; 96
-// behind 32,768 tokens 160, 167, 167; 128: 168, 167, 206; 2 groups of 48 behind 8192 103, 95, 96; 8 of
-// 12: 150, 144, 144; 17 sequences of 2 to 5 tokens in 3 groups (24 heads of 64 on 4, 4 bits) 38, 35, 35;
-// 34: 61, 49, 49.  (Where too few rows are there, the two launches are made for nothing.)
-constexpr int kReadyRowsShared = 384;
 // The most memory that converting may take: above it the packed kernel goes over the keys
 // once for every 128 rows.
 constexpr int64_t kReadyBytes = 4ll << 30;
