@@ -466,9 +466,11 @@ int mxk_quantize_fp8(int dtype, int64_t rows, int64_t k, const void* x, int64_t 
  * apart, rounded once.  k % 16 == 0 (the last block may be short), a and b 16-byte aligned.
  * A block's products are summed by the tensor core in float32, the blocks in float32 in a
  * fixed order; the two scales are multiplied first (in float32: below 2^-126 their product
- * loses bits).  A row's result does not depend on other rows' values.  Asynchronous on
- * `stream`; no workspace.  A device-side wait that gives up leaves the output undefined; the
- * next synchronous call of the library on the device reports MXK_ERR_TIMEOUT. */
+ * loses bits, from 2^128 on it is infinite, and so is an output with such a block, or it is
+ * NaN, as where the block's products sum to 0).  A row's result does not depend on other rows'
+ * values.  Asynchronous on `stream`; no workspace.  A device-side wait that gives up leaves the
+ * output undefined; the next synchronous call of the library on the device reports
+ * MXK_ERR_TIMEOUT. */
 int mxk_gemm_fp8(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, const float* a_scales,
                  const uint8_t* b, const float* b_scales, void* out, int64_t out_stride, void* stream);
 
