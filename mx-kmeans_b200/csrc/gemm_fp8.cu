@@ -446,13 +446,17 @@ int split_of(int64_t tiles, int blocks) {
 int64_t tiles_of(const GemmFp8& g) { return (g.m + kM - 1) / kM * ((g.n + kN - 1) / kN); }
 
 // Whether the CTAs quantise the rows themselves, which saves a launch and a workspace but holds the
-// products up by the rows' way through registers.  In us, from a loop of calls and (in a graph) on
-// the device alone, with and without: one row through 4096 x 4096 10.8 (10.5) and 16.7 (9.6),
-// through 14,336 x 4096 19.6 (19.6) and 17.3 (17.3).
-constexpr int64_t kOwnWeights = 32 << 20;
+// products up by the rows' way through registers.  In us on the device alone, in a graph (in a loop of
+// calls), with and without, the weights of several layers in turn:
+//   1 row: 2048 x 2048 7.2, 7.6 (10.0, 11.6), 4096 x 2048 7.7, 7.3 (10.3, 11.6), 4096 x 4096 10.1, 10.1 (12.4, 12.5),
+//     6144 x 4096 11.0, 11.9 (12.9, 14.3), 5120 x 5120 13.0, 12.3 (15.2, 14.5), 8192 x 4096 15.4, 14.3 (17.0, 16.5)
+//   8 rows: 4096 x 4096 10.5, 10.5 (12.4, 12.5), 6144 x 4096 11.9, 12.2 (14.4, 14.5), 8192 x 4096 16.1, 14.4 (18.5, 16.5)
+//   16 rows: 2048 x 2048 8.2, 8.2 (10.3, 11.9), 2048 x 4096 9.8, 9.2 (12.4, 11.8), 4096 x 4096 12.9, 10.7 (14.6, 12.6),
+//     8192 x 4096 19.8, 14.7 (21.8, 16.5)
+constexpr int64_t kOwnWeights = 24 << 20, kOwnWeightsMore = 4 << 20;  // up to 8 rows; more
 bool own_rows(const GemmFp8& g, int blocks) {
     const int split = split_of(tiles_of(g), blocks);
-    return g.m <= kOwnRows && g.n * g.k <= kOwnWeights &&
+    return g.m <= kOwnRows && g.n * g.k <= (g.m <= 8 ? kOwnWeights : kOwnWeightsMore) &&
            (g.m + 7) / 8 * 8 * kBlock * ((blocks + split - 1) / split) <= kOwnBytes;
 }
 
