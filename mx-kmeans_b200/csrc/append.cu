@@ -25,9 +25,10 @@
 // fewer bits, as the exact one does.
 //
 // Measured: 16,384 tokens of 32 + 8 + 8 heads of 128 in bf16, 8 bits (370 MB) in 88 us, 4.2
-// TB/s, interleaved 81, in float32 (706 MB) 120, 5.9 TB/s; 8 tokens 3.3.  Threads wait for three
-// loads one after the other (position, table, rows), so occupancy counts: with 2, 3 and 4 blocks
-// an SM 123, 98 and 88 us.  Testing by an interval whether a code is in doubt before taking the
+// TB/s, interleaved 82, in float32 (706 MB) 120, 5.9 TB/s; 6 bits 89, 83 and 120, 4 bits 87, 80 and 118; 8 tokens
+// 3.3.  Threads wait for three loads one after the other (position, table, rows), so occupancy counts: with
+// 2, 3 and 4 blocks an SM 123, 98 and 88 us.  At four a thread has 64 registers, of which 24 bytes spill in
+// this case (up to 108 where float32 rows are not aligned).  Testing by an interval whether a code is in doubt before taking the
 // sum exactly cost the registers of a block and gave nothing (90 us).
 #include <algorithm>
 #include <limits>

@@ -12,6 +12,11 @@
 //   P^T, from S^T as it lies in the registers, transposed within the warp (movmatrix), is the right operand
 //   O^T (D x 8 rows) += V^T (16 features x 16 tokens) P^T, a lane holding 16 (D = 64: 8) neighbouring features
 //
+// The weights are rounded to f16 for the product with the values, by at most 2^-11 of each (the instruction
+// takes 16-bit operands at this rate, and of those f16 the most exact, as weights are held between 2^15 and
+// what no longer counts); the sums that they are divided by take them in float32.  As in the other
+// kernels of a call, so that a row does not depend on which of them it meets.
+//
 // All rows see the same tokens, so scales and NaNs need none of the rows kernel's care about what some
 // rows do not see.  Value scales become f16 factors relative to a reference of the lane's block, which
 // goes up with the largest; blocks of zeros count for none where that would cost the others bits.

@@ -12,11 +12,13 @@
 // blocks are split over the CTAs of a cluster, which add their sums through distributed
 // shared memory in rank order, so results do not depend on timing.
 //
-// Large ones (pair::) are bound by the sums' way: every block's products leave TMEM once, 64 KB a CTA
-// for 512 cycles of products, and go through two multiply-adds an instruction; and by the power cap.
+// Large ones (pair::) are bound by the sums' way and by the power cap: every block's products leave TMEM once,
+// 128 KB a CTA (128 rows of 256 columns) for 512 cycles of products, and go through two multiply-adds an
+// instruction.  A wait for TMEM is for all loads that a warp has under way, so a load of 16 columns is covered by
+// the sums of the 16 before it and no more; with issue slots at 44 % and FMA at 35 % the tensor pipe is busy for 60 %.
 // Measured: 8192^3 460 to 500 us on an idle card (2.2 to 2.4 Pflop/s; a library product of E4M3 with one scale
 // a matrix, which leaves TMEM once at the end, 350), 550 under the cap; 2048 x 14,336 x 4096 105 us, 777 x 1003 x
-// 1040 9, one row through 4096 x 4096 9.6 to 10.2 (1.7 TB/s), 64 rows through 6144 x 4096 11 (2.3 TB/s): these
+// 1040 9, one row through 4096 x 4096 9.6 to 10.5 (1.7 TB/s), 64 rows through 6144 x 4096 11 (2.3 TB/s): these
 // are a launch, an empty pipeline, eight steps and the cluster's sums.
 #include <algorithm>
 #include <limits>

@@ -9,7 +9,10 @@
 // rounded onto it first.
 //
 // A thread converts 16 features; 2 or 4 bytes are read and one is written per element, so
-// HBM bounds both kernels.  Measured: 16,384 x 8192 in bfloat16 97 us (4.2 TB/s), in float32 115 (5.9).
+// HBM bounds both kernels.  Measured, 16,384 x 8192, by row and in blocks of 128 rows: bfloat16 98 and 87 us (4.1
+// and 4.7 TB/s), f16 93 and 83, float32 116 and 118 (5.8).  With 16-bit elements a thread by row asks
+// for 32 bytes and then waits for them, half of what it has under way in float32; in blocks of 128 rows for
+// 128.
 #include <algorithm>
 #include <limits>
 
