@@ -22,6 +22,14 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA GPU (B200, sm_100a)")
 
 
+def pytest_collection_modifyitems(items):
+    """Where the reference's host code was not built (oracle/_ref), the GPU tests that need it fail;
+    they come last then, so that a run that stops at its first failure has run all others."""
+    if not os.path.exists(os.path.join(ROOT, "oracle", "_ref", "libref_host.so")):
+        items.sort(key=lambda i: i.originalname == "test_cli_matches_reference_host_path"
+                   or i.path.name == "test_init_gpu.py" and "ref" in i.fixturenames)
+
+
 @pytest.fixture(scope="session")
 def orc():
     import oracle
