@@ -332,7 +332,7 @@ int mxk_cache_read(const mxk_cache* cache, int dtype, int64_t tokens, const int6
  *
  * q_out (`heads` heads) receives the rotated queries, computed in float32 and rounded once
  * to dtype; it may be q itself (the same data and strides) and may not overlap it in any
- * other way.  heads = 0: keys and values alone.  Slot slots[i] receives what
+ * other way, nor its rows each other.  heads = 0: keys and values alone.  Slot slots[i] receives what
  * mxk_cache_write(bits, ...) would store for the exact rotation of token i's keys (decided
  * in about 48 bits) and for its values.
  *

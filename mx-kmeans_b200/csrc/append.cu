@@ -31,6 +31,7 @@
 // this case (up to 108 where float32 rows are not aligned).  Testing by an interval whether a code is in doubt before taking the
 // sum exactly cost the registers of a block and gave nothing (90 us).
 #include <algorithm>
+#include <cstdlib>
 #include <limits>
 
 #include "cache_rows.cuh"
@@ -372,6 +373,10 @@ extern "C" int mxk_cache_append(const mxk_cache* cache, const mxk_append* a, voi
                     (reinterpret_cast<uintptr_t>(a->slots) | reinterpret_cast<uintptr_t>(a->positions)) % 8 == 0,
                 "cache_append: q, q_out, k, v, slots and positions must be aligned to their elements");
     MXK_REQUIRE(reinterpret_cast<uintptr_t>(a->cos_sin) % 16 == 0, "cache_append: cos_sin must be 16-byte aligned");
+    // (Broadcast queries can be read but not written.)
+    MXK_REQUIRE((a->heads <= 1 || std::abs(q_out.head_stride) >= cache->head_dim) &&
+                    (a->heads == 0 || a->tokens == 1 || std::abs(q_out.token_stride) >= cache->head_dim),
+                "cache_append: rows of q_out must not overlap");
     AppendParams m{};
     m.q = rows_of(q), m.q_out = rows_of(q_out), m.k = rows_of(a->k), m.v = rows_of(a->v);
     m.k_values = static_cast<uint8_t*>(cache->k_values), m.k_scales = cache->k_scales;
