@@ -48,6 +48,7 @@ struct GemmFp8Params {
     int64_t out_stride;      // elements
     int dtype;
     int out_vec, out_wide;   // four elements, or 16 bytes, can be stored at once
+    int copied;              // columns that fill whole 16-byte pieces
     int a_wide, b_wide;      // rows of scales can be loaded four at a time
     int beside;              // the kernel before writes nothing that this one reads
     unsigned* err;
@@ -103,6 +104,8 @@ __device__ __forceinline__ void load_scales(const float* p, int i, int count, bo
 // the output is aligned they leave as asynchronous copies and the warp goes on; the next call
 // waits until they have been read.  (With stores the warps of all CTAs wait at about the same time:
 // 4500 cycles of 50,000.  So they do for a copy from each lane, which are issued one by one.)
+// The copies write whole 16-byte pieces, whatever the output's width is, so a row's last elements that fill
+// none are stored by themselves.
 // 16-byte pieces of a row are permuted by row, so that eight lanes write to different banks.
 __device__ __forceinline__ void store_rows(const GemmFp8Params& p, const CUtensorMap* map, uint8_t* stage, int row0,
                                            int col, const float2 (&x)[64]) {
@@ -120,11 +123,21 @@ __device__ __forceinline__ void store_rows(const GemmFp8Params& p, const CUtenso
         if (p.out_wide) {
             if (lane == 0) {
                 for (int i = 0; i < 2; ++i)
-                    if (at + i * part < p.n)
+                    if (at + i * part < p.copied)
                         asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map),
                                      "r"(at + i * part), "r"(row0), "r"(dev::smem_addr(stage + i * kPart))
                                      : "memory");
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+            if (p.copied >= at && p.copied < at + 2 * part && row0 + lane < p.m) {
+                for (int c = p.copied; c < p.n; ++c) {
+                    const uint8_t* from = piece(lane, (c - at) * size / 16) + (c - at) * size % 16;
+                    char* to = p.out + ((int64_t)(row0 + lane) * p.out_stride + c) * size;
+                    if (size == 4)
+                        *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+                    else
+                        *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+                }
             }
             return;
         }
@@ -769,7 +782,7 @@ int launch(const GemmFp8& g, GemmFp8Params p, int most_pairs, bool follows, cuda
     CUtensorMap map_out{};
     if (p.out_wide) {
         const bool full = p.dtype == MXK_F32;
-        MXK_CHECK(encode_tensor_map_2d(&map_out, g.out, (uint64_t)g.n, (uint64_t)g.m, (uint64_t)g.out_stride * (full ? 4 : 2),
+        MXK_CHECK(encode_tensor_map_2d(&map_out, g.out, (uint64_t)p.copied, (uint64_t)g.m, (uint64_t)g.out_stride * (full ? 4 : 2),
                                        full ? 32 : 64, 32, full ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
                                        CU_TENSOR_MAP_SWIZZLE_128B));
     }
@@ -817,7 +830,8 @@ GemmFp8Params params_of(const GemmFp8& g, unsigned* err) {
     p.out_stride = g.out_stride;
     p.dtype = g.dtype;
     p.out_vec = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % (4 * size) == 0;
-    p.out_wide = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % 16 == 0;
+    p.copied = (int)(g.n * size / 16 * 16 / size);
+    p.out_wide = (reinterpret_cast<uintptr_t>(g.out) | (uint64_t)(g.out_stride * size)) % 16 == 0 && p.copied > 0;
     p.a_wide = p.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(g.a_scales) % 16 == 0;
     p.b_wide = p.blocks % 4 == 0 && reinterpret_cast<uintptr_t>(g.b_scales) % 16 == 0;
     p.err = err;
